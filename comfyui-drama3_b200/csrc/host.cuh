@@ -1,0 +1,95 @@
+// Host helpers of the C ABI shared by the library's translation units: status codes, device properties, launches with
+// programmatic dependent launch, the tensor-map encoder.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include <cudaTypedefs.h>
+
+#include "../../include/drama3_b200.h"
+
+namespace d3host {
+
+inline thread_local int g_last_cuda = 0;
+
+inline int cuda_status(cudaError_t e) {
+  if (e == cudaSuccess) return D3_OK;
+  g_last_cuda = (int)e;
+  return D3_ERR_CUDA;
+}
+
+inline int launch_status() { return cuda_status(cudaGetLastError()); }
+
+inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
+
+constexpr int kMaxDevices = 64;
+
+struct DeviceInfo {
+  int sms = 0;
+  int smem_optin = 0;
+  int cc = 0;
+};
+
+inline std::mutex g_mu;
+inline DeviceInfo g_dev[kMaxDevices];
+
+inline int device_info(DeviceInfo* out) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return D3_ERR_DEVICE;
+  std::lock_guard<std::mutex> lock(g_mu);
+  DeviceInfo& d = g_dev[dev];
+  if (d.sms == 0) {
+    int major = 0, minor = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaDeviceGetAttribute(&d.smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    d.cc = major * 10 + minor;
+  }
+  *out = d;
+  if (d.cc != 100) return D3_ERR_DEVICE;
+  return D3_OK;
+}
+
+// Raise a kernel's dynamic shared-memory ceiling (once per device and kernel).
+template <class K>
+int allow_smem(K kernel, int bytes) {
+  if (bytes <= 48 * 1024) return D3_OK;
+  return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+template <class K, class... Args>
+int launch(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (pdl) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda).
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+  });
+  return fn;
+}
+
+}  // namespace d3host
