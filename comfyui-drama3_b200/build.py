@@ -14,7 +14,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = [HERE / "csrc" / "drama3_b200.cu", HERE / "csrc" / "pack.cpp"]
+SOURCES = [HERE / "csrc" / "drama3_b200.cu", HERE / "csrc" / "lines.cu", HERE / "csrc" / "pack.cpp"]
 DEPENDS = sorted((HERE / "csrc").glob("*.c*")) + [ROOT / "include" / "drama3_b200.h"]
 OUTPUT = HERE / "drama3_b200" / "libdrama3_b200.so"
 OBJECTS = HERE / "_build"

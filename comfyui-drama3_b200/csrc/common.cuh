@@ -19,6 +19,10 @@ enum : unsigned {
   FAULT_BAD_SLOT = 4u,      // a slot index outside [0, count): the expert was skipped
   FAULT_TILES = 8u,         // the groups need more row tiles than the caller sized: the excess rows were skipped
   FAULT_EXCHANGE = 16u,     // an expert-parallel exchange area that does not fit the call: nothing was exchanged
+  FAULT_PAGES = 32u,        // a cache page that is missing or outside the cache: skipped on writing, zeros on reading
+  FAULT_TOKENS = 64u,       // the lines append more tokens than the pass holds: the rest was left out
+  FAULT_POSITION = 128u,    // a position or axis outside the rotary table: the pair was left unrotated
+  FAULT_PLAN = 256u,        // a plan made for another pass (lines, tokens or heads): nothing was computed
 };
 __device__ unsigned int g_fault;
 

@@ -25,6 +25,8 @@
 
 using namespace d3host;
 
+int d3_lines_take_fault(unsigned int* fault);  // lines.cu
+
 namespace {
 
 // A 2-D byte tensor [rows, row_bytes] read in boxes of box_bytes x 128 rows, with the shared-memory swizzle of that
@@ -94,7 +96,10 @@ int d3_take_fault(unsigned int* fault) {
   int st = cuda_status(cudaMemcpyFromSymbol(&v, d3::g_fault, sizeof(v)));
   if (st) return st;
   st = cuda_status(cudaMemcpyToSymbol(d3::g_fault, &zero, sizeof(zero)));
-  *fault = v;
+  if (st) return st;
+  unsigned int lines = 0;
+  st = d3_lines_take_fault(&lines);
+  *fault = v | lines;
   return st;
 }
 

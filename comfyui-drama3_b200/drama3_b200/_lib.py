@@ -20,6 +20,7 @@ WEIGHT_KEY = {"fp8": "weight", "fp8c": "weight", "int8": "_qdata", "w4": "_qdata
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _d = ctypes.c_double
+_f = ctypes.c_float
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); every name here is a symbol include/drama3_b200.h declares
@@ -61,6 +62,13 @@ SIGNATURES = {
     "d3_ipc_handle": (_i, [_p, _p, ctypes.POINTER(ctypes.c_size_t)]),
     "d3_ipc_open": (_i, [_p, _sz, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_void_p)]),
     "d3_ipc_close": (_i, [_p]),
+    "d3_lines_plan_ints": (_sz, [_i, _i, _i]),
+    "d3_lines_plan": (_i, [_p, _p, _i, _p, _i, _p, _i, _p, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "d3_qk_norm_rope": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i, _f, _f, _p, _i, _i, _p, _i, _p, _i,
+                             _p, _p, _p, _p, _p, _p, _i, _i, _p, _p]),
+    "d3_lines_attention_workspace": (_sz, [_i, _i, _i, _i]),
+    "d3_lines_attention": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p, _p, _p, _i, _f,
+                                _p, _p, _p, _sz, _p]),
 }
 
 

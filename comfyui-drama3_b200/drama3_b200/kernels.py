@@ -7,9 +7,14 @@ and every launch goes on the device's current stream, so calls can be captured i
   - `route` and `weighted_sum` also take several rows at once;
   - `await_cpu` (the CPU-expert handshake) is not provided: this path has no CPU side;
   - `moe_decode` is new: the whole resident decode (gate_up, SwiGLU, down, combine) for 1..16 rows in one pass;
-  - `grouped_mma` is new: the grouped kernels on the tensor cores for banks held whole on the GPU.
+  - `grouped_mma` is new: the grouped kernels on the tensor cores for banks held whole on the GPU;
+  - `lines_plan`, `qk_norm_rope` and `lines_attention` are new: the attention half of a decoder layer for lines decoded
+    together, over a paged key/value cache with a prefix that the lines share.
 """
+import ctypes
 import functools
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -451,3 +456,199 @@ def moe_decode(kind, x, ids, weights, banks, codebooks=(None, None), workspace=N
                                   _ptr(scale2), _ptr(down.get("s_channel")), _ptr(codebooks[0]), _ptr(codebooks[1]),
                                   _ptr(out), _ptr(workspace), workspace.numel(), _stream(x.device)), "moe_decode")
     return out
+
+
+# ---- the attention half of a decoder layer, for lines decoded together
+
+ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class LinesPlan(NamedTuple):
+    """What `lines_plan` returns: the block tables (the caller's, updated), the new tokens' slots [T] and positions [T]
+    (int64) and lines [T] (int32, -1 past the last token), the first token of each line cu [B + 1], the lines' lengths
+    [B] and the used part of the free list [1] after the pass (int32), and the attention's work list for `group` query
+    heads per KV head."""
+    table: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    line: torch.Tensor
+    cu: torch.Tensor
+    lengths: torch.Tensor
+    used: torch.Tensor
+    work: torch.Tensor
+    page: int
+    group: int
+
+
+def _ints(name, t, device, *shape):
+    """Refuses anything but a contiguous int32 tensor of this shape (None: any size) on `device`."""
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device or t.dim() != len(shape) or any(
+            want is not None and want != got for want, got in zip(shape, t.shape)):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on {device}, not "
+                         f"{t.dtype} {list(t.shape)} on {t.device}")
+    return t
+
+
+def _strides(t, n):
+    return (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def lines_plan(lengths, counts, table, free, used, page, tokens, prefix=None, group=1):
+    """The plan of a pass that appends counts [B] tokens to lines that hold lengths [B] tokens of their own (int32, on
+    the GPU; nothing is read back to the host): a LinesPlan for `tokens` token places (the rows of the pass's tensors;
+    places past the lines' last token belong to no line). Each line takes the pages of `page` tokens that it needs
+    beyond its own from free[used:] (int32, used [1]) into its row of table [B, W], in line order; table is updated in
+    place, lengths and used are not: the plan's are the state after the pass. prefix [1] (int32): tokens of the prefix
+    that the lines share, which come first in their positions. group: query heads per KV head of the attention that
+    will use the plan. A page that the free list or the table has no room for is -1, as its tokens' slots are, and is
+    recorded in the fault word."""
+    device = lengths.device
+    B = lengths.shape[0] if lengths.dim() == 1 else 0
+    _ints("lengths", lengths, device, B)
+    _ints("counts", counts, device, B)
+    _ints("table", table, device, B, None)
+    _ints("free", free, device, None)
+    _ints("used", used, device, 1)
+    if prefix is not None:
+        _ints("prefix", prefix, device, 1)
+    T, group = int(tokens), int(group)
+    size = lib().d3_lines_plan_ints(B, T, group)
+    if size == 0:
+        raise ValueError(f"no plan for {B} lines, {T} tokens, {group} query heads per KV head")
+    with _on(device):
+        slots, positions = torch.empty((2, T), dtype=torch.int64, device=device)
+        line = torch.empty(T, dtype=torch.int32, device=device)
+        state = torch.empty(2 * B + 2, dtype=torch.int32, device=device)
+        cu, new_lengths, new_used = state[:B + 1], state[B + 1:2 * B + 1], state[2 * B + 1:]
+        work = torch.empty(size, dtype=torch.int32, device=device)
+        check(lib().d3_lines_plan(_ptr(lengths), _ptr(counts), B, _ptr(table), table.shape[1], _ptr(free), free.shape[0],
+                                  _ptr(used), _ptr(prefix), int(page), T, group, _ptr(slots), _ptr(positions), _ptr(line),
+                                  _ptr(cu), _ptr(new_lengths), _ptr(new_used), _ptr(work), size, _stream(device)),
+              "lines_plan")
+    return LinesPlan(table, slots, positions, line, cu, new_lengths, new_used, work, int(page), group)
+
+
+def rotary_table(inv_freq, length, device=None):
+    """[length, n, 2] float32: cosine and sine of position x inv_freq [n], formed in 64 bits (a 32-bit product of a
+    position of many thousands has lost the angle's last digits), for `qk_norm_rope`."""
+    angle = torch.arange(length, dtype=torch.float64)[:, None] * torch.as_tensor(inv_freq).detach().double().cpu()[None]
+    return torch.stack((angle.cos(), angle.sin()), dim=-1).float().to(device or "cpu")
+
+
+def rotary_axes(sections, woven=False, device=None):
+    """[sum(sections)] uint8: the axis of each rotary frequency, for positions with several axes (time, height,
+    width, ...): the first sections[0] frequencies turn by axis 0, the next by axis 1 and so on; with `woven` the axes
+    take turns frequency by frequency while they have frequencies left."""
+    if woven:
+        left, axes = list(sections), []
+        while any(left):
+            for a, n in enumerate(left):
+                if n:
+                    axes.append(a)
+                    left[a] -= 1
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.uint8, device=device or "cpu")
+
+
+def qk_norm_rope(q, k, rotary, positions, q_weight=None, k_weight=None, eps=1e-6, unit_offset=False, axes=None,
+                 pairs=False, v=None, k_cache=None, v_cache=None, slots=None):
+    """(q_out [T, Hq, D], k_out [T, Hkv, D]): queries and keys (bfloat16, float16 or float32; any strides with the last
+    dimension contiguous, so views of a fused projection's output) through the RMS norm of each head with q_weight /
+    k_weight [D] (of the rows' type or float32; 1 + weight with unit_offset; None: no norm) and the rotation of their
+    first 2 n columns by rotary [length, n, 2] (`rotary_table`), halves (f, f + n) or, with `pairs`, neighbours (2f,
+    2f + 1). positions: [T] int64, or [A, T] with axes [n] uint8 (`rotary_axes`) naming the row that turns each
+    frequency. With k_cache and v_cache [pages, page, Hkv, D], v [T, Hkv, D] and slots [T] (int64, a LinesPlan's) the
+    keys and the values go to their slots of the caches instead (-1: nowhere) and k_out is None. One launch; 32-bit
+    arithmetic, rounded once."""
+    T, Hq, D = q.shape
+    if q.dtype not in ROW_TYPES or k.dtype != q.dtype:
+        raise TypeError(f"qk_norm_rope takes bfloat16, float16 or float32 rows of one type, not {q.dtype} and {k.dtype}")
+    Hkv = k.shape[1]
+    if tuple(k.shape) != (T, Hkv, D) or q.stride(2) != 1 or k.stride(2) != 1:
+        raise ValueError("q [T, Hq, D] and k [T, Hkv, D] must agree in T and D, their last dimension contiguous")
+    device = q.device
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if tuple(w.shape) != (D,) or not w.is_contiguous() or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype:
+            raise ValueError("q_weight and k_weight must be contiguous [D] tensors of the rows' type or float32, alike")
+    if rotary.dtype != torch.float32 or rotary.dim() != 3 or rotary.shape[2] != 2 or not rotary.is_contiguous():
+        raise ValueError("rotary must be a contiguous float32 [length, n, 2] tensor")
+    length, n = rotary.shape[:2]
+    if 2 * n > D:
+        raise ValueError(f"rotary turns {2 * n} columns of {D}")
+    if positions.dtype != torch.int64 or positions.shape[-1] != T or positions.dim() != (1 if axes is None else 2):
+        raise ValueError("positions must be int64 [T], or [A, T] with axes")
+    positions = positions.contiguous()
+    if axes is not None and (axes.dtype != torch.uint8 or tuple(axes.shape) != (n,) or not axes.is_contiguous()):
+        raise ValueError("axes must be a contiguous uint8 tensor with the axis of each of the n frequencies")
+    cached = k_cache is not None
+    if any((x is not None) != cached for x in (v, v_cache, slots)):
+        raise ValueError("v, k_cache, v_cache and slots go together")
+    if cached:
+        if tuple(v.shape) != (T, Hkv, D) or v.dtype != q.dtype or v.stride(2) != 1:
+            raise ValueError("v must be [T, Hkv, D] of the rows' type, its last dimension contiguous")
+        for c in (k_cache, v_cache):
+            if c.dim() != 4 or c.shape != k_cache.shape or tuple(c.shape[2:]) != (Hkv, D) or c.dtype != q.dtype or c.stride(3) != 1:
+                raise ValueError("the caches must be [pages, page, Hkv, D] of the rows' type, alike, the last dimension contiguous")
+        if slots.dtype != torch.int64 or tuple(slots.shape) != (T,) or not slots.is_contiguous():
+            raise ValueError("slots must be a contiguous int64 [T] tensor")
+    for t in (k, rotary, positions, axes, v, k_cache, v_cache, slots, *weights):
+        if t is not None and t.device != device:
+            raise ValueError(f"qk_norm_rope: every tensor must be on {device}")
+    with _on(device):
+        q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
+        k_out = None if cached else torch.empty((T, Hkv, D), dtype=q.dtype, device=device)
+        pages, page = k_cache.shape[:2] if cached else (0, 0)
+        check(lib().d3_qk_norm_rope(_ptr(q), _strides(q, 2), _ptr(k), _strides(k, 2), _ptr(v),
+                                    _strides(v, 2) if cached else None, ROW_TYPES[q.dtype], T, Hq, Hkv, D, _ptr(q_weight),
+                                    _ptr(k_weight), int(bool(weights) and weights[0].dtype == torch.float32),
+                                    float(bool(unit_offset)), float(eps), _ptr(rotary), 2 * n, length, _ptr(positions),
+                                    1 if axes is None else positions.shape[0], _ptr(axes), int(bool(pairs)), _ptr(q_out),
+                                    _ptr(k_out), _ptr(k_cache), _strides(k_cache, 3) if cached else None, _ptr(v_cache),
+                                    _strides(v_cache, 3) if cached else None, pages, page, _ptr(slots), _stream(device)),
+              "qk_norm_rope")
+    return q_out, k_out
+
+
+def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, lse=False):
+    """[T, Hq, D] (and, with `lse`, [T, Hq] float32: the log of each row's sum of exponentials): the attention of the
+    plan's tokens q [T, Hq, D] (bfloat16 or float16) over the paged caches [pages, page, Hkv, D] of the same type, whose
+    keys of this pass are written (`qk_norm_rope`). A token sees the keys of the shared prefix, in the pages of
+    prefix_table [PW] (int32; their number was given to `lines_plan`), and its line's own keys up to its own; query
+    head h reads KV head h / (Hq / Hkv), scale defaults to 1 / sqrt(D). D 64, 128 or 256; page 16, 32 or a multiple of
+    64. Where the lines bring few tokens, the prefix's keys are read once for all of them. Places of the plan without a
+    token get zeros (lse -inf); what the cache holds past a line's length is never used."""
+    T, Hq, D = q.shape
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("lines_attention takes bfloat16 or float16 queries and caches of one type")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+        raise ValueError("the caches must be [pages, page, Hkv, D], alike")
+    pages, page, Hkv = k_cache.shape[:3]
+    if q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("the last dimension of the queries and the caches must be contiguous")
+    if plan.page != page or plan.slots.shape[0] != T or plan.group * Hkv != Hq:
+        raise ValueError(f"the plan is for {plan.slots.shape[0]} tokens, pages of {plan.page} and {plan.group} query heads "
+                         f"per KV head, not for {T}, {page} and {Hq} / {Hkv}")
+    device = q.device
+    B = plan.cu.shape[0] - 1
+    if prefix_table is not None:
+        _ints("prefix_table", prefix_table, device, None)
+    for t in (k_cache, v_cache, plan.work):
+        if t.device != device:
+            raise ValueError(f"lines_attention: every tensor must be on {device}")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    with _on(device):
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
+        sums = torch.empty((T, Hq), dtype=torch.float32, device=device) if lse else None
+        size = lib().d3_lines_attention_workspace(T, Hq, Hkv, D)
+        if size == 0:
+            raise ValueError(f"no attention kernel for {Hq} / {Hkv} heads of {D}")
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        check(lib().d3_lines_attention(_ptr(q), _strides(q, 2), ROW_TYPES[q.dtype], T, Hq, Hkv, D, _ptr(k_cache),
+                                       _strides(k_cache, 3), _ptr(v_cache), _strides(v_cache, 3), pages, page,
+                                       _ptr(plan.table), plan.table.shape[1], _ptr(prefix_table),
+                                       0 if prefix_table is None else prefix_table.shape[0], _ptr(plan.line), _ptr(plan.cu),
+                                       _ptr(plan.work), B, scale, _ptr(out), _ptr(sums), _ptr(ws), size, _stream(device)),
+              "lines_attention")
+    return (out, sums) if lse else out

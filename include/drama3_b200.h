@@ -55,12 +55,19 @@ int d3_device_check(void);
 /* Reads and clears the current device's fault word (synchronous). Bits: D3_FAULT_WAIT (1) a wait timed out,
  * D3_FAULT_EXPERT (2) an expert id out of range, D3_FAULT_SLOT (4) a slot out of range, D3_FAULT_TILES (8) a
  * grouped GEMM given fewer row tiles than its groups need, D3_FAULT_EXCHANGE (16) an expert-parallel exchange area
- * whose geometry does not fit the call. No counterpart in the reference, whose kernels do not check indices. */
+ * whose geometry does not fit the call, D3_FAULT_PAGES (32) a cache page that is missing or outside the cache,
+ * D3_FAULT_TOKENS (64) lines that append more tokens than the pass holds, D3_FAULT_POSITION (128) a position or axis
+ * outside the rotary table, D3_FAULT_PLAN (256) an attention given the plan of another pass. No counterpart in the
+ * reference, whose kernels do not check indices. */
 #define D3_FAULT_WAIT 1u
 #define D3_FAULT_EXPERT 2u
 #define D3_FAULT_SLOT 4u
 #define D3_FAULT_TILES 8u
 #define D3_FAULT_EXCHANGE 16u
+#define D3_FAULT_PAGES 32u
+#define D3_FAULT_TOKENS 64u
+#define D3_FAULT_POSITION 128u
+#define D3_FAULT_PLAN 256u
 int d3_take_fault(unsigned int* fault);
 
 /* Decode routing, `rows` independent rows: ids [rows, k] (int64) and weights [rows, k] (fp32 holding bfloat16
@@ -257,6 +264,56 @@ int d3_moe_decode_static(int fmt, const void* x, int x_bf16, int M, int k, int E
                          const float* weights, const uint8_t* w13, const void* s13, const float* c13,
                          const uint8_t* w2, const void* s2, const float* c2, const float* codebook13,
                          const float* codebook2, uint16_t* out, void* stream);
+
+/* ---- The attention half of a decoder layer, for lines decoded together. No counterpart in the reference, whose
+ * attention layers are its host application's. A key/value cache is two tensors [pages, page, kv_heads, D] (any
+ * strides, given in elements for page, key and head; the last dimension contiguous); slot s of it is key s % page of
+ * page s / page. A line's own keys lie in the pages of its row of a block table [B, W]; the keys of the prefix that
+ * all lines share lie in the pages of one table of its own. Row type: 0 bfloat16, 1 float16, 2 float32. */
+
+/* The plan of a pass that appends counts[b] tokens to line b, which has kept[b]: in line order, each line takes the
+ * pages it needs beyond those it has from free_pages[*used..F) into its table row (in place: only entries that the pass
+ * opens); then for each of the T token places, in line order, slots (-1 past the last token, or without a page),
+ * positions (*prefix + the token's number in its line; 0 past the last) and line (-1 past the last); cu [B + 1] the
+ * first token of each line; lengths [B] and used_out [1] the state after the pass (kept and used are not changed, so
+ * a plan can be made again); work the attention's work list for `group` query heads per KV head,
+ * d3_lines_plan_ints() ints. Negative lengths and counts are 0; tokens past T are left out (D3_FAULT_TOKENS); a page
+ * past the free list or the table's width is -1 (D3_FAULT_PAGES). prefix may be null (0). B <= 8192, group <= 128,
+ * T * group <= 2^30. */
+size_t d3_lines_plan_ints(int B, int T, int group);
+int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, const int* free_pages, int F,
+                  const int* used, const int* prefix, int page, int T, int group, int64_t* slots, int64_t* positions,
+                  int* line, int* cu, int* lengths, int* used_out, int* work, size_t work_ints, void* stream);
+
+/* Queries q [T, Hq, D] and keys k [T, Hkv, D] (strides in elements for token and head), each head divided by its
+ * root mean square (eps added to the mean square) and multiplied by q_weight / k_weight [D] + w_add (of the rows' type,
+ * or fp32 with w_f32; null: no norm for that tensor), then its first rot columns turned: pair f, columns (f, f +
+ * rot/2), or (2f, 2f + 1) with `pairs`, by (cos, sin) = rotary[positions[axis[f]][t]][f], rotary [length, rot/2, 2]
+ * fp32, positions [axes, T], axis [rot/2] (null with one axis; axes <= 4). 32-bit arithmetic, rounded once. q_out
+ * [T, Hq, D]. With k_out [T, Hkv, D] the keys go there and v and the caches are not used; with k_out null the keys
+ * and the rows of v go to slots[t] of the caches (-1: nowhere; past pages * page: nowhere, D3_FAULT_SLOT). Positions
+ * outside the table leave their pair unturned (D3_FAULT_POSITION). D <= 1024, rot even and <= D. */
+int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, int type, int T, int Hq, int Hkv, int D, const void* q_weight,
+                    const void* k_weight, int w_f32, float w_add, float eps, const float* rotary, int rot, int length,
+                    const int64_t* positions, int axes, const uint8_t* axis, int pairs, void* q_out, void* k_out,
+                    void* k_cache, const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides, int pages,
+                    int page, const int64_t* slots, void* stream);
+
+/* out [T, Hq, D] = softmax(scale q K^T) V for the tokens of a plan (q [T, Hq, D], strides in elements): token t of
+ * line b sees the prefix's keys (prefix_table [PW]; their number is the plan's) and the line's own keys up to its own,
+ * which d3_qk_norm_rope (or the caller) has written. Query head h reads KV head h / (Hq / Hkv). Types 0 and 1 (queries
+ * and caches alike); sums and softmax in 32 bits. lse [T, Hq] (or null): the log of each row's sum of exponentials.
+ * Tokens past the plan's last get zeros (lse -inf). A key past a length is never used, whatever the cache holds there;
+ * a page outside the cache reads as zeros (D3_FAULT_PAGES). table, W, line, cu, work, B: the plan's; the workspace
+ * is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128 or 256; page 16, 32 or a multiple of
+ * 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and all pointers 16-byte aligned. */
+size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D);
+int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
+                       const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,
+                       int pages, int page, const int* table, int W, const int* prefix_table, int PW, const int* line,
+                       const int* cu, const int* work, int B, float scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,486 @@
+"""The attention half of a decoder layer on the GPU (lines_plan, qk_norm_rope, lines_attention) against its plain
+restatements in tests/lines_ref.py.
+
+Tolerances. qk_norm_rope: one rounding to the row's type (half a unit in the last place: at most 2^-8 of the value for
+bfloat16's 8 significant bits, 2^-11 for float16's 11) of a 32-bit result whose error is a few 2^-24 of the pair's size; for float32 rows 2^-20 of the pair's size covers the sum of
+squares and a dozen operations. lines_attention: an output is a sum of p_j V_j whose p_j are rounded to the values'
+type and which is rounded once more at the end, each by at most half a unit in the last place, so |error| <= 2 x that x sum p_j |V_j|; a tenth more stands for everything in 32 bits, and 2^-24 for float16's
+smallest steps. lse: the scores' 32-bit sums (2^-22 of sum |q k|, below 2^4 where the scores are ordinary) and the exponentials'
+2^-21 make 2e-5; where the scores are large, 2^-21 of the sum's own size is added for the rounding of both."""
+import math
+import random
+
+import pytest
+import torch
+
+import lines_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF_UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def fault():
+    from drama3_b200._lib import take_fault
+    return take_fault()
+
+
+def i32(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+# ---- lines_plan
+
+PLANS = [
+    # lengths, counts, page, spare token places, prefix
+    ([0], [1], 16, 0, None),
+    ([0], [0], 16, 2, 5),
+    ([15, 16, 17, 0], [1, 1, 1, 1], 16, 0, 100),
+    ([0, 5, 64, 3], [0, 70, 0, 200], 16, 3, 7),
+    ([1, 2, 3], [4, 0, 1], 1, 1, 0),
+    ([6, 7, 8], [1, 1, 30], 7, 0, 3),
+    ([-4, 2], [3, -2], 16, 1, 1),
+]
+
+
+def lines_case(lengths, counts, page, spare, seed=0, room=2, extra=5):
+    rng = random.Random(seed)
+    have = [(max(0, n) + page - 1) // page for n in lengths]
+    need = [(max(0, n) + max(0, c) + page - 1) // page for n, c in zip(lengths, counts)]
+    width = max(need) + room
+    order = list(range(sum(need) + extra))
+    rng.shuffle(order)
+    table, used = [], 0
+    for h in have:
+        table.append(order[used:used + h] + [-1] * (width - h))
+        used += h
+    return table, order, used, sum(max(0, c) for c in counts) + spare
+
+
+def run_plan(cuda, lengths, counts, table, free, used, page, tokens, prefix, group=1):
+    from drama3_b200 import kernels
+    t = i32(table, cuda)
+    args = (i32(lengths, cuda), i32(counts, cuda), t, i32(free, cuda), i32([used], cuda), page, tokens)
+    p = kernels.lines_plan(*args, prefix=None if prefix is None else i32([prefix], cuda), group=group)
+    return args, p
+
+
+def check_plan(p, want, table):
+    for name in ("slots", "positions", "line", "cu", "lengths", "used"):
+        got = getattr(p, name).tolist()
+        assert got == want[name], name
+    assert p.table.tolist() == table
+
+
+@pytest.mark.parametrize("lengths,counts,page,spare,prefix", PLANS)
+def test_plan(cuda, lengths, counts, page, spare, prefix):
+    table, free, used, tokens = lines_case(lengths, counts, page, spare)
+    args, p = run_plan(cuda, lengths, counts, table, free, used, page, tokens, prefix)
+    want = ref.plan(lengths, counts, table, free, used, page, tokens, prefix or 0)
+    check_plan(p, want, table)
+    assert fault() == 0
+    # planning the same pass again gives the same plan
+    from drama3_b200 import kernels
+    again = kernels.lines_plan(*args, prefix=None if prefix is None else i32([prefix], cuda))
+    check_plan(again, want, table)
+
+
+@pytest.mark.parametrize("lines,most", [(1, 5000), (33, 400), (600, 3), (2500, 9), (8192, 2)])
+def test_plan_many(cuda, lines, most):
+    rng = random.Random(lines)
+    lengths = [rng.randrange(0, 300) for _ in range(lines)]
+    counts = [rng.randrange(0, most + 1) for _ in range(lines)]
+    table, free, used, tokens = lines_case(lengths, counts, 16, 9, seed=lines)
+    _, p = run_plan(cuda, lengths, counts, table, free, used, 16, tokens, 1234)
+    check_plan(p, ref.plan(lengths, counts, table, free, used, 16, tokens, 1234), table)
+    assert fault() == 0
+
+
+def test_plan_without_room(cuda):
+    lengths, counts = [3, 16, 30, 2], [20, 1, 10, 50]
+    table, free, used, tokens = lines_case(lengths, counts, 16, 0)
+    for cut_free, cut_width, cut_tokens in ((4, 0, 0), (0, 3, 0), (0, 0, 30), (5, 2, 7), (0, 0, tokens)):
+        f = free[:len(free) - 5 - cut_free]
+        t = [row[:len(row) - cut_width] for row in table]
+        _, p = run_plan(cuda, lengths, counts, t, f, used, 16, tokens - cut_tokens, 0)
+        want = ref.plan(lengths, counts, t, f, used, 16, tokens - cut_tokens, 0)
+        check_plan(p, want, t)
+        assert fault() == (32 if want["pages"] else 0) | (64 if want["tokens"] else 0)
+
+
+def units_of(p, B):
+    work = p.work.tolist()
+    at = (16 + 2 * B + 3) & ~3
+    return work, [tuple(work[at + 4 * u:at + 4 * u + 4]) for u in range(work[1])]
+
+
+@pytest.mark.parametrize("group", [1, 7, 8, 128])
+@pytest.mark.parametrize("lengths,counts,prefix", [
+    ([100] * 16, [1] * 16, 300), ([0, 9, 64, 63], [1, 40, 0, 200], 130), ([0], [3000], 0), ([5], [1], 64),
+    ([0, 0], [128, 130], 1)])
+def test_work_list_covers_every_row_and_key(cuda, group, lengths, counts, prefix):
+    table, free, used, tokens = lines_case(lengths, counts, 16, 2)
+    _, p = run_plan(cuda, lengths, counts, table, free, used, 16, tokens, prefix, group=group)
+    work, units = units_of(p, len(lengths))
+    total = sum(counts)
+    assert work[4] == prefix and work[6] == total and work[7] == group
+    starts = 0
+    own, shared = {}, []
+    for line, row0, start, tiles in units:
+        assert start == starts and tiles >= 1
+        starts += tiles
+        if line < 0:
+            shared.append(row0)
+            assert tiles == -(-prefix // 64)
+        else:
+            own[line, row0] = tiles
+    assert starts == work[2]
+    lead = -(-prefix // 64) if work[0] else 0
+    want = {}
+    for b, (kept, n) in enumerate(zip(lengths, counts)):
+        for row0 in range(0, n * group, 128):
+            last = (min(row0 + 128, n * group) - 1) // group
+            want[b, row0] = lead + -(-(kept + last + 1) // 64)
+    assert own == want
+    assert shared == ([] if work[0] or not prefix else list(range(0, total * group, 128)))
+
+
+# ---- qk_norm_rope
+
+def rope_inputs(cuda, T, hq, hkv, D, rot, axes, dtype, seed, strided=0):
+    from drama3_b200 import kernels
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    wide = (hq + 2 * hkv) * D + strided
+    qkv = (torch.randn((T, wide), generator=g, device=cuda) * 3).to(dtype)[:, strided:]
+    q, k, v = (x.unflatten(1, (-1, D)) for x in qkv.split((hq * D, hkv * D, hkv * D), 1))
+    qw, kw = ((1 + 0.3 * torch.randn(D, generator=g, device=cuda)).to(dtype) for _ in range(2))
+    n = rot // 2
+    rotary = kernels.rotary_table(10000.0 ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)), 500, cuda)
+    shape = (T,) if axes == 1 else (axes, T)
+    pos = torch.randint(0, 500, shape, generator=g, device=cuda)
+    amap = None if axes == 1 else kernels.rotary_axes([n - n // 3 * (axes - 1)] + [n // 3] * (axes - 1), woven=n % 2 == 0, device=cuda)
+    return q, k, v, qw, kw, rotary, pos, amap
+
+
+def close_rows(got, want, x, dtype):
+    """One rounding of `want` plus 32-bit noise in proportion to the head's largest value."""
+    size = want.abs().amax(-1, keepdim=True)
+    tol = want.abs() * HALF_UNIT[dtype] + size * 2.0 ** -20 if dtype in HALF_UNIT else size * 2.0 ** -20
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -24
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,hq,hkv,D,rot,axes,pairs,strided", [
+    (1, 32, 4, 128, 128, 1, False, 0), (16, 16, 2, 256, 64, 3, False, 0), (37, 8, 8, 64, 64, 1, True, 0),
+    (5, 5, 5, 80, 40, 1, False, 0), (5, 5, 5, 80, 40, 1, True, 8), (300, 7, 1, 96, 96, 2, False, 16),
+    (3, 2, 1, 512, 512, 1, False, 0), (3, 2, 1, 512, 128, 3, True, 0), (4, 3, 3, 1024, 64, 1, False, 0),
+    (9, 3, 1, 66, 20, 1, False, 0), (9, 3, 1, 33, 32, 4, True, 0), (6, 4, 2, 128, 128, 1, False, 1),
+    (2, 1, 1, 8, 8, 1, False, 0), (2, 1, 1, 2, 2, 1, True, 0), (11, 4, 4, 128, 0, 1, False, 0),
+    (1100, 12, 3, 128, 96, 3, False, 0)])
+def test_norm_rope(cuda, dtype, T, hq, hkv, D, rot, axes, pairs, strided):
+    from drama3_b200 import kernels
+    q, k, v, qw, kw, rotary, pos, amap = rope_inputs(cuda, T, hq, hkv, D, rot, axes, dtype, 7 * D + T, strided)
+    got = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw, eps=1e-5, axes=amap, pairs=pairs)
+    for x, w, y in ((q, qw, got[0]), (k, kw, got[1])):
+        assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+        close_rows(y, ref.norm_rope(x, w, 0, 1e-5, rotary, pos, amap, pairs), x, dtype)
+    assert fault() == 0
+
+
+@pytest.mark.parametrize("D,strided", [(128, 0), (96, 3)])
+def test_norm_rope_weights(cuda, D, strided):
+    from drama3_b200 import kernels
+    q, k, v, qw, kw, rotary, pos, _ = rope_inputs(cuda, 19, 6, 2, D, D, 1, torch.bfloat16, 3, strided)
+    for a, b, off in ((None, None, 0), (qw, None, 0), (None, kw, 1), (qw - 1, kw - 1, 1), (qw.float(), kw.float(), 0)):
+        got = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=a, k_weight=b, unit_offset=bool(off))
+        for x, w, y in ((q, a, got[0]), (k, b, got[1])):
+            close_rows(y, ref.norm_rope(x, w, off, 1e-6, rotary, pos, None, False), x, torch.bfloat16)
+
+
+def test_norm_rope_rows_of_zeros_and_extremes(cuda):
+    from drama3_b200 import kernels
+    q, k, v, qw, kw, rotary, pos, _ = rope_inputs(cuda, 4, 4, 4, 128, 128, 1, torch.float32, 5)
+    q, k = q.clone(), k.clone()
+    q[0], q[1], q[2] = 0, q[1] * 1e15, q[2] * 1e-15
+    k[0, 0, 3] = math.nan
+    k[1, 1, 5] = math.inf
+    out, kk = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw, eps=1e-6)
+    close_rows(out, ref.norm_rope(q, qw, 0, 1e-6, rotary, pos, None, False), q, torch.float32)
+    assert (out[0] == 0).all()
+    # a head that holds a NaN or an infinity stays its own trouble
+    bad = torch.zeros((4, 4), dtype=torch.bool, device=cuda)
+    bad[0, 0] = bad[1, 1] = True
+    assert torch.equal(kk.isnan().any(-1), bad)
+
+
+@pytest.mark.parametrize("order", ["plain", "heads_first", "odd"])
+@pytest.mark.parametrize("D", [64, 128, 72])
+def test_norm_rope_into_cache(cuda, order, D):
+    from drama3_b200 import kernels
+    T, hq, hkv, page, pages = 41, 6, 3, 16, 9
+    q, k, v, qw, kw, rotary, pos, _ = rope_inputs(cuda, T, hq, hkv, D, D, 1, torch.bfloat16, 11)
+
+    def cache(fill):
+        if order == "heads_first":  # [pages, heads, page, D]
+            return torch.full((pages, hkv, page, D), fill, dtype=torch.bfloat16, device=cuda).transpose(1, 2)
+        pad = 1 if order == "odd" else 0
+        return torch.full((pages, page, hkv, D + pad), fill, dtype=torch.bfloat16, device=cuda)[..., :D]
+
+    kc, vc = cache(7.0), cache(9.0)
+    slots = torch.randperm(pages * page, device=cuda)[:T]
+    slots[3], slots[8], slots[20] = -1, pages * page, 1 << 40
+    out, none = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw, v=v, k_cache=kc, v_cache=vc, slots=slots)
+    assert none is None and fault() == 4
+    plain, k_plain = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw)
+    assert torch.equal(out, plain)
+    want_k, want_v = torch.full((pages * page, hkv, D), 7.0, dtype=torch.bfloat16, device=cuda), None
+    want_v = torch.full_like(want_k, 9.0)
+    ok = (slots >= 0) & (slots < pages * page)
+    want_k[slots[ok]], want_v[slots[ok]] = k_plain[ok], v[ok]
+    assert torch.equal(kc.reshape(-1, hkv, D), want_k) and torch.equal(vc.reshape(-1, hkv, D), want_v)
+
+
+def test_norm_rope_positions_outside_the_table(cuda):
+    from drama3_b200 import kernels
+    for strided in (0, 1):
+        q, k, v, qw, kw, rotary, pos, amap = rope_inputs(cuda, 6, 4, 2, 128, 64, 3, torch.bfloat16, 2, strided)
+        pos[0, 1], pos[1, 2], pos[2, 5] = -1, 500, 1 << 40
+        got = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw, axes=amap)
+        assert fault() == 128
+        close_rows(got[0], ref.norm_rope(q, qw, 0, 1e-6, rotary, pos, amap, False), q, torch.bfloat16)
+        bad = amap.clone()
+        bad[4] = 3
+        kernels.qk_norm_rope(q, k, rotary, pos.clamp(0, 499), q_weight=qw, k_weight=kw, axes=bad)
+        assert fault() == 128
+
+
+def test_norm_rope_empty(cuda):
+    from drama3_b200 import kernels
+    q, k, v, qw, kw, rotary, pos, _ = rope_inputs(cuda, 2, 4, 2, 128, 128, 1, torch.bfloat16, 2)
+    got = kernels.qk_norm_rope(q[:0], k[:0], rotary, pos[:0], q_weight=qw, k_weight=kw)
+    assert got[0].shape == (0, 4, 128) and got[1].shape == (0, 2, 128)
+
+
+def test_rotary_helpers(cuda):
+    from drama3_b200 import kernels
+    t = kernels.rotary_table(torch.tensor([1.0, 0.001]), 200001, cuda)
+    for p in (0, 1, 777, 200000):
+        for f, w in enumerate((1.0, float(torch.tensor(0.001)))):
+            assert abs(float(t[p, f, 0]) - math.cos(p * w)) < 1e-7 and abs(float(t[p, f, 1]) - math.sin(p * w)) < 1e-7
+    assert kernels.rotary_axes([3, 2, 1]).tolist() == [0, 0, 0, 1, 1, 2]
+    assert kernels.rotary_axes([3, 2, 1], woven=True).tolist() == [0, 1, 2, 0, 1, 0]
+
+
+# ---- lines_attention
+
+def attn_case(cuda, hq, hkv, D, dtype, page, kept, counts, prefix, spare=0, seed=0, order="plain", poison=True, loud=1.5):
+    from drama3_b200 import kernels
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    table, free, used, tokens = lines_case(kept, counts, page, spare, seed=seed)
+    shared = (prefix + page - 1) // page
+    pages = len(free) + shared
+    names = list(range(pages))
+    random.Random(seed + 1).shuffle(names)
+    prefix_table = i32(names[len(free):], cuda)
+    free = [names[x] for x in free]
+    table = [[names[x] if x >= 0 else -1 for x in row] for row in table]
+    _, plan = run_plan(cuda, kept, counts, table, free, used, page, tokens, prefix, group=hq // hkv)
+    shape = (pages, hkv, page, D) if order == "heads_first" else (pages, page, hkv, D)
+    kc, vc = (torch.randn(shape, generator=g, device=cuda).to(dtype) for _ in range(2))
+    if order == "heads_first":
+        kc, vc = kc.transpose(1, 2), vc.transpose(1, 2)
+    if poison:  # whatever lies past the lengths is never used
+        used_slots = torch.zeros(pages * page, dtype=torch.bool, device=cuda)
+        for tab, n in [(prefix_table, prefix)] + [(plan.table[b], k + c) for b, (k, c) in enumerate(zip(kept, counts))]:
+            for j in range((n + page - 1) // page):
+                first = int(tab[j]) * page
+                used_slots[first:first + min(page, n - j * page)] = True
+        kc.view(pages, -1) if order == "plain" else None
+        for c, bad in ((kc, math.nan), (vc, math.inf)):
+            c[~used_slots.view(pages, page)] = bad
+            c[(~used_slots).view(pages, page) & (torch.arange(page, device=cuda) % 2 == 0)] = math.nan
+    q = (loud * torch.randn((tokens, hq, D), generator=g, device=cuda)).to(dtype)
+    return q, kc, vc, plan, prefix_table
+
+
+def check_attn(cuda, case, kept, counts, prefix, scale=None, lse=True):
+    from drama3_b200 import kernels
+    q, kc, vc, plan, prefix_table = case
+    got, sums = kernels.lines_attention(q, kc, vc, plan, prefix_table=prefix_table, scale=scale, lse=True)
+    want, want_lse, bound = ref.attention(q, kc, vc, kept, counts, plan.table, prefix, prefix_table,
+                                          scale or 1 / math.sqrt(q.shape[2]))
+    assert fault() == 0
+    tol = 2.2 * HALF_UNIT[q.dtype] * bound + (2.0 ** -24 if q.dtype == torch.float16 else 0)
+    err = (got.double() - want).abs()
+    assert not got.isnan().any()
+    assert (err <= tol).all(), float((err / tol.clamp(min=1e-30)).max())
+    empty = torch.isinf(want_lse)
+    assert torch.equal(empty, torch.isinf(sums)) and (sums[empty] < 0).all()
+    assert ((sums.double() - want_lse)[~empty].abs() <= 2e-5 + 2.0 ** -21 * want_lse[~empty].abs()).all()
+    return got
+
+
+SHAPES = [(32, 4, 128), (16, 2, 256), (8, 8, 64), (7, 1, 64), (24, 3, 128), (4, 2, 256), (128, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,D", SHAPES)
+@pytest.mark.parametrize("page,prefix", [(16, 0), (16, 200), (32, 63), (64, 64), (128, 1000), (192, 1)])
+def test_attention_decode(cuda, dtype, hq, hkv, D, page, prefix):
+    kept, counts = [0, 1, 15, 63, 64, 200, 31, 500], [1] * 8
+    case = attn_case(cuda, hq, hkv, D, dtype, page, kept, counts, prefix, seed=prefix + D)
+    check_attn(cuda, case, kept, counts, prefix)
+
+
+@pytest.mark.parametrize("hq,hkv,D", SHAPES)
+@pytest.mark.parametrize("kept,counts,prefix,spare", [
+    ([0], [1], 0, 0), ([0], [300], 0, 0), ([100, 0, 7], [50, 129, 1], 77, 0), ([5, 6, 7, 8], [1, 0, 3, 0], 130, 6),
+    ([3] * 20, [2] * 20, 260, 1), ([0, 0], [33, 65], 4, 0), ([64, 1], [64, 16], 64, 0), ([9, 9], [0, 0], 10, 3)])
+def test_attention_ragged(cuda, hq, hkv, D, kept, counts, prefix, spare):
+    case = attn_case(cuda, hq, hkv, D, torch.bfloat16, 16, kept, counts, prefix, spare=spare, seed=len(kept))
+    check_attn(cuda, case, kept, counts, prefix)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_long(cuda, D):
+    # runs of many tiles, cut in the middle of units, the maximum growing as they go
+    for kept, counts, prefix in (([6000], [1], 0), ([3000] * 3, [1] * 3, 9000), ([0], [2000], 0), ([700, 0], [900, 600], 1500)):
+        case = attn_case(cuda, 16, 2, D, torch.bfloat16, 64, kept, counts, prefix, seed=D, loud=4.0)
+        check_attn(cuda, case, kept, counts, prefix)
+
+
+def test_attention_growing_maximum(cuda):
+    # every key's score is far above those before it, so each tile moves the maximum, and far below, so none does
+    for sign in (1, -1):
+        kept, counts, prefix = [400, 90], [1, 40], 300
+        q, kc, vc, plan, pt = attn_case(cuda, 8, 1, 128, torch.bfloat16, 16, kept, counts, prefix, poison=False)
+        q[:], kc[:] = 1.0, 0.0
+        for tab, n, base in ((pt, prefix, 0), (plan.table[0], 401, 300), (plan.table[1], 130, 300)):
+            for j in range(n):
+                kc[int(tab[j // 16]), j % 16] = sign * (base + j) / 16.0
+        check_attn(cuda, (q, kc, vc, plan, pt), kept, counts, prefix)
+
+
+@pytest.mark.parametrize("order", ["plain", "heads_first"])
+def test_attention_strides(cuda, order):
+    kept, counts, prefix = [40, 3], [5, 70], 100
+    q, kc, vc, plan, pt = attn_case(cuda, 16, 4, 128, torch.bfloat16, 32, kept, counts, prefix, order=order)
+    wide = torch.zeros((q.shape[0], 24, 128), dtype=q.dtype, device=cuda)
+    wide[:, 8:] = q
+    a = check_attn(cuda, (wide[:, 8:], kc, vc, plan, pt), kept, counts, prefix)
+    assert torch.equal(a, check_attn(cuda, (q, kc, vc, plan, pt), kept, counts, prefix))
+    check_attn(cuda, (q, kc, vc, plan, pt), kept, counts, prefix, scale=0.031)
+
+
+def test_attention_past_32_bits(cuda):
+    # a cache whose last pages lie beyond 2^31 elements and 2^32 bytes
+    from drama3_b200 import kernels
+    page, hkv, D, pages = 64, 8, 128, 34000
+    assert pages * page * hkv * D > 1 << 31
+    kc, vc = (torch.zeros((pages, page, hkv, D), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    free = i32(list(range(pages - 1, pages - 12, -1)), cuda)
+    table, used = i32([[-1] * 8] * 2, cuda), i32([0], cuda)
+    counts = [150, 90]
+    plan = kernels.lines_plan(i32([0, 0], cuda), i32(counts, cuda), table, free, used, page, 240, group=2)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q, k, v = (torch.randn((240, h, D), generator=g, device=cuda).to(torch.bfloat16) for h in (16, 8, 8))
+    rotary = kernels.rotary_table(torch.ones(64), 256, cuda)
+    q2, _ = kernels.qk_norm_rope(q, k, rotary, plan.positions, v=v, k_cache=kc, v_cache=vc, slots=plan.slots)
+    assert int(plan.slots.min()) * hkv * D > 1 << 31
+    small_k, small_v = kc[pages - 12:].clone(), vc[pages - 12:].clone()
+    want, _, bound = ref.attention(q2, small_k, small_v, [0, 0], counts, plan.table - (pages - 12), 0, i32([], cuda), 1 / math.sqrt(D))
+    got = kernels.lines_attention(q2, kc, vc, plan)
+    assert ((got.double() - want).abs() <= 2.2 * HALF_UNIT[torch.bfloat16] * bound).all() and fault() == 0
+    assert (bound > 0).any()
+
+
+def test_attention_bad_page_reads_zeros(cuda):
+    from drama3_b200 import kernels
+    kept, counts, prefix = [60, 20], [1, 1], 50
+    q, kc, vc, plan, pt = attn_case(cuda, 8, 2, 64, torch.bfloat16, 16, kept, counts, prefix, poison=False)
+    for bad in (-1, kc.shape[0], 1 << 30):
+        table = plan.table.clone()
+        table[0, 1] = bad
+        got = kernels.lines_attention(q, kc, vc, plan._replace(table=table), prefix_table=pt)
+        assert fault() == 32
+        # the same with that page there and full of zeros
+        kz, vz = (torch.cat((c, torch.zeros_like(c[:1]))) for c in (kc, vc))
+        table[0, 1] = kc.shape[0]
+        assert torch.equal(got, kernels.lines_attention(q, kz, vz, plan._replace(table=table), prefix_table=pt))
+    # a prefix that no table holds
+    kernels.lines_attention(q, kc, vc, plan)
+    assert fault() == 32
+
+
+def test_attention_plan_of_another_pass_is_refused(cuda):
+    from drama3_b200 import kernels
+    kept, counts = [60, 20], [1, 1]
+    q, kc, vc, plan, pt = attn_case(cuda, 8, 2, 64, torch.bfloat16, 16, kept, counts, 0)
+    other = attn_case(cuda, 8, 2, 64, torch.bfloat16, 16, [3], [2], 0)[3]
+    with pytest.raises(ValueError):
+        kernels.lines_attention(q, kc, vc, plan._replace(group=2), prefix_table=pt)
+    kernels.lines_attention(q, kc, vc, plan._replace(work=other.work), prefix_table=pt)
+    assert fault() == 256
+
+
+def test_attention_twice_is_the_same_and_lines_do_not_mix(cuda):
+    # no result depends on the order in which blocks run; a line's rows do not change with what else is decoded
+    # beyond the way its keys are cut
+    from drama3_b200 import kernels
+    kept, counts, prefix = [300, 20, 77], [1, 1, 1], 500
+    q, kc, vc, plan, pt = attn_case(cuda, 16, 2, 128, torch.bfloat16, 16, kept, counts, prefix)
+    a = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt)
+    for _ in range(5):
+        assert torch.equal(a, kernels.lines_attention(q, kc, vc, plan, prefix_table=pt))
+    q2 = q.clone()
+    q2[1] = math.nan
+    b = kernels.lines_attention(q2, kc, vc, plan, prefix_table=pt)
+    assert torch.equal(a[[0, 2]], b[[0, 2]]) and b[1].isnan().all()
+
+
+def test_step_on_a_side_stream_and_in_a_graph(cuda):
+    """Plan, cache write and attention captured once and replayed as the lines grow, against the same steps alone."""
+    from drama3_b200 import kernels
+    hq, hkv, D, page, B, prefix = 8, 2, 64, 16, 3, 70
+    g = torch.Generator(device=cuda).manual_seed(4)
+    pages = 40
+    kc, vc = (torch.randn((pages, page, hkv, D), generator=g, device=cuda).to(torch.bfloat16) for _ in range(2))
+    kc2, vc2 = kc.clone(), vc.clone()
+    pt = i32(list(range(35, 40)), cuda)
+    rotary = kernels.rotary_table(10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32), 400, cuda)
+    free = i32(list(range(34, -1, -1)), cuda)
+    counts, pre = i32([1, 1, 1], cuda), i32([prefix], cuda)
+
+    def state():
+        return [i32([0, 30, 15], cuda), i32([[-1] * 10, [0, 1] + [-1] * 8, [2] + [-1] * 9], cuda), i32([0], cuda)]
+
+    def step(st, kc, vc, qkv):
+        q, k, v = (x.unflatten(1, (-1, D)) for x in qkv.split((hq * D, hkv * D, hkv * D), 1))
+        plan = kernels.lines_plan(st[0], counts, st[1], free, st[2], page, B, prefix=pre, group=hq // hkv)
+        qr, _ = kernels.qk_norm_rope(q, k, rotary, plan.positions, v=v, k_cache=kc, v_cache=vc, slots=plan.slots)
+        out = kernels.lines_attention(qr, kc, vc, plan, prefix_table=pt)
+        st[0].copy_(plan.lengths)
+        st[2].copy_(plan.used)
+        return out
+
+    xs = [torch.randn((B, (hq + 2 * hkv) * D), generator=g, device=cuda).to(torch.bfloat16) for _ in range(20)]
+    st = state()
+    want = [step(st, kc, vc, x) for x in xs]
+    held, x = state(), xs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([t.clone() for t in held], kc2.clone(), vc2.clone(), x)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(held, kc2, vc2, x)
+        for i, xi in enumerate(xs):
+            x.copy_(xi)
+            graph.replay()
+            side.synchronize()
+            assert torch.equal(out, want[i]), i
+    assert torch.equal(kc, kc2) and torch.equal(held[0], st[0]) and fault() == 0
+    del graph
