@@ -34,6 +34,20 @@ bool cache_map(CUtensorMap* map, bool f16, const void* base, int D, int heads, i
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries [T, heads, D] as a 3-D map (column, head, token), read in boxes of 64 columns x the heads of a KV head x the
+// tokens of a unit.
+bool query_map(CUtensorMap* map, bool f16, const void* base, int D, int heads, int T, const int64_t* st, int group) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
+  cuuint32_t boxes[3] = {64, (cuuint32_t)group, (cuuint32_t)d3::la_tile_tokens(group)};
+  cuuint32_t elem[3] = {1, 1, 1};
+  return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
+            dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
 int attn_runs(const DeviceInfo& d) {
   return d.sms * d3::LaShape<D>::PER_SM;
@@ -49,12 +63,13 @@ bool attn_shape(int T, int Hq, int Hkv, int D) {
 }
 
 template <int D, bool F16>
-int attn_launch(const CUtensorMap& km, const CUtensorMap& vm, const d3::LaArgs& a, int combine_blocks, cudaStream_t s) {
+int attn_launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const d3::LaArgs& a, dim3 combine,
+                cudaStream_t s) {
   constexpr int smem = d3::LaShape<D>::SMEM;
   if (int st = allow_smem(d3::lines_attn_kernel<D, F16>, smem)) return st;
-  if (int st = launch(d3::lines_attn_kernel<D, F16>, dim3(a.runs), dim3(d3::LA_THREADS), smem, s, true, km, vm, a))
+  if (int st = launch(d3::lines_attn_kernel<D, F16>, dim3(a.runs), dim3(d3::LA_THREADS), smem, s, true, qm, km, vm, a))
     return st;
-  return launch(d3::lines_combine_kernel<D, F16>, dim3(combine_blocks), dim3(d3::LC_WARPS * 32), 0, s, true, a);
+  return launch(d3::lines_combine_kernel<D, F16>, dim3(combine.x), dim3(d3::LC_WARPS * 32), 0, s, true, a, (int)combine.y);
 }
 
 template <int TYPE, int LANES, int NV>
@@ -99,7 +114,7 @@ extern "C" {
 
 size_t d3_lines_plan_ints(int B, int T, int group) {
   if (B < 1 || B > d3::LP_MAX_LINES || T < 0 || group < 1 || group > d3::LA_ROWS) return 0;
-  return (size_t)d3::la_unit_offset(B) + 4 * (size_t)d3::la_max_units(B, T, group);
+  return d3::la_unit_offset(T) + d3::LA_UNIT_INTS * (size_t)d3::la_max_units(B, T, group);
 }
 
 int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, const int* free_pages, int F,
@@ -115,7 +130,7 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
   if (work_ints < d3_lines_plan_ints(B, T, group)) return D3_ERR_WORKSPACE;
   DeviceInfo d;
   if (int st = device_info(&d)) return st;
-  const int smem = 3 * (B + 1) * 4;
+  const int smem = 5 * (B + 1) * 4;
   if (int st = allow_smem(d3::lines_plan_kernel, smem)) return st;
   const d3::LinesPlanArgs a = {kept, counts, B, table, W, free_pages, F, used, prefix, page, T, group, slots, positions,
                                line, cu, lengths, used_out, work};
@@ -178,13 +193,13 @@ size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D) {
   DeviceInfo d;
   if (!attn_shape(T, Hq, Hkv, D) || device_info(&d)) return 0;
   const long long rows = d3::la_part_rows(attn_runs_of(d, D), T, Hq / Hkv, Hkv);
-  return (size_t)rows * (D + 2) * 4;
+  return (size_t)rows * (D + 2) * 4 + (size_t)attn_runs_of(d, D) * 16;
 }
 
 int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
                        const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,
-                       int pages, int page, const int* table, int W, const int* prefix_table, int PW, const int* line,
-                       const int* cu, const int* work, int B, float scale, void* out, float* lse, void* workspace,
+                       int pages, int page, const int* table, int W, const int* prefix_table, int PW, const int* work,
+                       int B, float scale, void* out, float* lse, void* workspace,
                        size_t workspace_bytes, void* stream) {
   if ((type != d3::QR_BF16 && type != d3::QR_F16) || !attn_shape(T, Hq, Hkv, D) || pages < 1 ||
       !(page == 16 || page == 32 || (page >= 64 && page % 64 == 0)) || (long long)pages * page > 0x7fffffffLL || W < 1 ||
@@ -192,11 +207,10 @@ int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T,
     return D3_ERR_ARG;
   if (T == 0) return D3_OK;
   if (!q || !q_strides || !k_cache || !kc_strides || !v_cache || !vc_strides || !table || (PW > 0 && !prefix_table) ||
-      !line || !cu || !work || !out || !workspace)
+      !work || !out || !workspace)
     return D3_ERR_ARG;
-  for (const int64_t* st : {kc_strides, vc_strides})
-    for (int i = 0; i < 3; ++i)
-      if (st[i] < 1) return D3_ERR_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (kc_strides[i] < 1 || vc_strides[i] < 1 || (i < 2 && q_strides[i] < 1)) return D3_ERR_ARG;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) || !aligned(workspace, 16) ||
       !aligned(work, 16) || !multiple(q_strides, 2, 8) || !multiple(kc_strides, 3, 8) || !multiple(vc_strides, 3, 8))
     return D3_ERR_ALIGN;
@@ -204,33 +218,35 @@ int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T,
   if (int st = device_info(&d)) return st;
   if (workspace_bytes < d3_lines_attention_workspace(T, Hq, Hkv, D)) return D3_ERR_WORKSPACE;
   const bool f16 = type == d3::QR_F16;
-  const int box = page < d3::LA_KEYS ? page : d3::LA_KEYS;
-  CUtensorMap km, vm;
-  if (!cache_map(&km, f16, k_cache, D, Hkv, page, pages, kc_strides, box) ||
+  // a box is as many keys of a page as a tile can hold
+  const int box = page % d3::LA_KEYS == 0 ? d3::LA_KEYS : page < 64 ? page : 64;
+  CUtensorMap qm, km, vm;
+  if (!query_map(&qm, f16, q, D, Hq, T, q_strides, Hq / Hkv) ||
+      !cache_map(&km, f16, k_cache, D, Hkv, page, pages, kc_strides, box) ||
       !cache_map(&vm, f16, v_cache, D, Hkv, page, pages, vc_strides, box))
     return D3_ERR_ARG;
   d3::LaArgs a = {};
-  a.q = q, a.q_token = q_strides[0], a.q_head = q_strides[1];
   a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
   a.pages = pages, a.page = page, a.page_box = box;
   a.table = table, a.W = W, a.prefix_table = prefix_table, a.PW = PW;
-  a.line = line, a.cu = cu, a.work = work, a.B = B;
+  a.work = work, a.B = B;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out, a.lse = lse;
   a.runs = attn_runs_of(d, D);
   const long long rows = d3::la_part_rows(a.runs, T, a.G, Hkv);
-  a.part_o = (float*)workspace;
-  a.part_ml = (float2*)(a.part_o + rows * D);
-  // a block per row where every row may have parts, and no fewer than keep the joining of cut units short
-  const long long every = (long long)T * Hq;
-  const int floor_blocks = 16 * d.sms;
-  const int blocks = (int)((long long)T * a.G <= d3::LA_APART_ROWS && every > floor_blocks
-                               ? (every < 64 * d.sms ? every : 64 * d.sms) : floor_blocks);
+  a.part_o = (float4*)workspace;
+  a.part_ml = (float2*)((float*)workspace + rows * D);
+  a.cuts = (int4*)(a.part_ml + rows);
+  // the joining kernel: a block per run and per 32 rows that may have parts; with few of the latter, a block per 32 of
+  // their columns
+  const long long groups = (long long)T * a.G <= d3::LA_APART_ROWS ? d3::la_apart_rows(T, a.G) / 32 * Hkv : 0;
+  const int column_blocks = groups > 0 && groups < 4 * d.sms ? D / 32 : 1;
+  const dim3 combine((unsigned)(groups * column_blocks > a.runs ? groups * column_blocks : a.runs), column_blocks);
   cudaStream_t s = (cudaStream_t)stream;
   switch (D) {
-    case 64: return f16 ? attn_launch<64, true>(km, vm, a, blocks, s) : attn_launch<64, false>(km, vm, a, blocks, s);
-    case 128: return f16 ? attn_launch<128, true>(km, vm, a, blocks, s) : attn_launch<128, false>(km, vm, a, blocks, s);
-    default: return f16 ? attn_launch<256, true>(km, vm, a, blocks, s) : attn_launch<256, false>(km, vm, a, blocks, s);
+    case 64: return f16 ? attn_launch<64, true>(qm, km, vm, a, combine, s) : attn_launch<64, false>(qm, km, vm, a, combine, s);
+    case 128: return f16 ? attn_launch<128, true>(qm, km, vm, a, combine, s) : attn_launch<128, false>(qm, km, vm, a, combine, s);
+    default: return f16 ? attn_launch<256, true>(qm, km, vm, a, combine, s) : attn_launch<256, false>(qm, km, vm, a, combine, s);
   }
 }
 

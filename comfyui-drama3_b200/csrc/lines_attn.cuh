@@ -5,22 +5,23 @@
 // with 32-bit accumulators on the tensor cores, and p is rounded to the values' type for the second product (its sum
 // is taken before the rounding).
 //
-// A unit (lines_plan.cuh) is a tile of up to 128 rows (a token x one query head of a KV head) and its key tiles of 64.
-// The key tiles of all units of all KV heads, laid end to end, are cut into equal runs, one per CTA: every CTA streams
-// the same number of keys whatever the lengths are. A run crosses units; a unit cut by a run's end leaves parts, which
-// lines_combine_kernel joins. With few lines the rows of all of them share the prefix's tiles, so a prefix key is
-// read from memory once for all lines.
+// A unit (lines_plan.cuh) is a tile of up to 128 rows (whole tokens x the query heads of a KV head) and its key tiles
+// of 128. The units of all KV heads, laid end to end by what they cost, are cut into equal runs, one per CTA: every CTA
+// has the same work whatever the lengths are. A run crosses units; a unit cut by a run's end leaves parts, which
+// lines_combine_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
+// key is read once for all lines.
 //
-// Per CTA (192 threads; two CTAs per SM for heads of 64 and 128, so that one's products run under the other's
-// exponentials; one for 256):
-//   warp 0     loads: lane l issues one TMA box (a page's keys x 64 columns, 128-byte swizzle) of the stage's K or V
-//              tile into a ring; a page outside the cache reads as zeros (the tensor map's fill)
-//   warp 1     issues the MMAs (one elected thread) and owns the tensor memory: S = Q K^T (128 x 64, two buffers),
-//              O += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so
-//              it is the MN-major operand). S of the next tile is issued before O of this one.
-//   warps 2-5  a thread owns a row: S from tensor memory, mask, maximum, exponentials, P back over S, the row's
-//              sum. O is rescaled only when the maximum has grown by more than 2^8 since the last time (p <= 256 in
-//              between, the same value after the division). They also stage Q and write the results.
+// Per CTA (320 threads; two CTAs per SM for heads of 64 and 128, so that one's products run under the other's
+// exponentials; one for 256, with two buffers for S instead):
+//   warp 0     loads by TMA (128-byte swizzle) into a ring of 16 KB stages, a stage being 64 columns of a tile's 128
+//              keys of K or V: a box per page, a lane each. A page outside the cache reads as zeros (the map's fill).
+//              A unit's queries likewise, into a buffer of their own.
+//   warp 1     issues the MMAs and owns the tensor memory: S = Q K^T (128 x 128), O += P V (128 x D, A = P from tensor
+//              memory, B = V as it lies in the cache: keys are its rows, so it is the MN-major operand)
+//   warps 2-9  two threads own a row, 64 of a tile's keys each: S from tensor memory, mask, maximum, exponentials, P
+//              back over S, the row's sum. O is rescaled only when the maximum has grown by more than 2^8 since the
+//              last time (p <= 256 in between, the same value after the division). They also write the results.
+// Loads and first products of a run's next unit go on while the row warps write this one's results.
 // Keys of a tile past the end of the prefix or of the line are masked in S, and their V rows are cleared in shared
 // memory before the product, since the cache may hold anything there (0 x NaN is NaN).
 // Every wait is bounded (2 s) and records FAULT_WAIT_TIMEOUT instead of hanging.
@@ -34,169 +35,208 @@
 
 namespace d3 {
 
-constexpr int LA_THREADS = 192;
-constexpr int LA_ROW_WARP = 2;        // first of the four row warps
-constexpr int LA_MIN_TILES = 2;       // shortest run of key tiles worth a CTA
+constexpr int LA_THREADS = 320;
+constexpr int LA_ROW_WARP = 2;        // first of the eight row warps
+constexpr int LA_ROW_WARPS = 8;
+constexpr int LA_STAGE = LA_KEYS * 128;  // 64 columns of a K or V tile
+constexpr int LA_MIN_RUN = 3;         // shortest run (in costs) worth a CTA
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
+
+// Shared memory besides the operands: barriers, the row threads' exchange, and the row warps' copies of plan and walk
+// (which they need only between pieces: kept in registers they were spilled inside the loop over tiles).
+// 1 KB in all: two CTAs of heads of 128 fill an SM's shared memory to the byte.
+constexpr int LA_EXCHANGE = 192, LA_PLAN_AT = LA_EXCHANGE + LA_ROWS * 4, LA_WALK_AT = LA_PLAN_AT + 64;
+constexpr int LA_WALK_BYTES = 32, LA_SMALL = LA_WALK_AT + LA_ROW_WARPS * LA_WALK_BYTES;
+static_assert(LA_SMALL <= 1024, "two CTAs per SM");
 
 template <int D>
 struct LaShape {
-  static constexpr int SLICES = D / 64;                 // 128-byte column slices of a row
+  static constexpr int SLICES = D / 64;  // stages of a tile
   static constexpr int Q_BYTES = LA_ROWS * D * 2;
-  static constexpr int STAGE = LA_KEYS * D * 2;         // a K or V tile
   static constexpr int PER_SM = D == 256 ? 1 : 2;
-  static constexpr int STAGES = D == 256 ? 4 : D == 128 ? 5 : 8;
-  static constexpr int TMEM_COLS = D == 256 ? 512 : 256;  // O: D columns, S: 2 x 64
-  static constexpr int SMEM = Q_BYTES + STAGES * STAGE + 1024;
+  static constexpr int STAGES = D == 256 ? 10 : D == 128 ? 5 : 6;
+  static constexpr int S_BUFS = D == 256 ? 2 : 1;
+  static constexpr int TMEM_COLS = D == 256 ? 512 : 256;  // O: D columns, then S_BUFS x 128
+  static constexpr int SMEM = Q_BYTES + STAGES * LA_STAGE + LA_SMALL;
 };
 
 struct LaArgs {
-  const void* q;
-  long long q_token, q_head;  // strides in elements
   int T, Hq, Hkv, G;
-  int pages, page, page_box;  // page_box: keys of a TMA box, min(page, 64)
+  int pages, page, page_box;  // page_box: keys of a TMA box
   const int* table;
   int W;
   const int* prefix_table;
   int PW;
-  const int* line;
-  const int* cu;
   const int* work;
   int B;
   float scale_log2;  // scale * log2(e)
   void* out;         // [T, Hq, D]
   float* lse;        // [T, Hq] or null
-  float* part_o;     // partial rows [.., D], not divided
+  float4* part_o;    // partial rows, not divided: four columns of 32 rows together, see la_part_at
   float2* part_ml;   // their (maximum * scale_log2, sum)
+  int4* cuts;        // per run: the unit whose first cut is this run's start (token0, rows, head, last run), or rows 0
   int runs;          // CTAs of the attention kernel
 };
 
 // Partial rows: LA_ROWS for the part that a run starts in the middle of a unit, LA_ROWS for the part that it leaves
-// unfinished, then (prefix and own units apart) the first part of every row's prefix unit and of its own unit.
+// unfinished, then (prefix and own units apart) the first part of every row's prefix unit and of its own unit, by the
+// row's number token * G + head.
 D3_DEV long long la_part_rest(int run) { return (long long)run * LA_ROWS; }
 D3_DEV long long la_part_open(const LaArgs& a, int run) { return (long long)(a.runs + run) * LA_ROWS; }
-D3_DEV long long la_part_apart(const LaArgs& a, bool own, int h, int row) {
-  return (long long)2 * a.runs * LA_ROWS + ((long long)(own ? a.Hkv : 0) + h) * a.T * a.G + row;
+__host__ __device__ inline long long la_apart_rows(int T, int G) { return ((long long)T * G + 31) & ~31ll; }
+D3_DEV long long la_part_apart(const LaArgs& a, bool own, int h) {
+  return (long long)2 * a.runs * LA_ROWS + ((long long)(own ? a.Hkv : 0) + h) * la_apart_rows(a.T, a.G);
 }
 __host__ __device__ inline long long la_part_rows(int runs, int T, int G, int Hkv) {
-  return (long long)2 * runs * LA_ROWS + ((long long)T * G <= LA_APART_ROWS ? 2ll * Hkv * T * G : 0);
+  return (long long)2 * runs * LA_ROWS + ((long long)T * G <= LA_APART_ROWS ? 2ll * Hkv * la_apart_rows(T, G) : 0);
+}
+// Where columns 4c .. 4c + 3 of partial row r are: the same columns of 32 neighbouring rows together, so that a warp
+// whose lanes are rows writes and reads them as 512 bytes in a row.
+template <int D>
+D3_DEV long long la_part_at(long long r, int c) {
+  return ((r >> 5) * (D / 4) + c) * 32 + (r & 31);
 }
 
-// Key tiles of a run.
-D3_DEV long long la_run_tiles(const LaArgs& a) {
-  const long long total = (long long)a.work[LW_TILES] * a.Hkv;
-  const long long even = (total + a.runs - 1) / a.runs;
-  return even > LA_MIN_TILES ? even : LA_MIN_TILES;
-}
-
-D3_DEV bool la_plan_fits(const LaArgs& a) {
-  return a.work[LW_GROUP] == a.G && a.work[LW_LINES] == a.B && a.work[LW_T] == a.T;
-}
-
-D3_DEV LaUnit la_unit(const LaUnit* units, int u) {
-  const int4 v = __ldg((const int4*)(units + u));
-  return LaUnit{v.x, v.y, v.z, v.w};
-}
-
-// The last unit with start <= tile, by the whole warp: 32 probes a round.
-D3_DEV int la_find_unit(const LaUnit* units, int count, int tile) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = count;  // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int at = lo + lane * step;
-    const bool below = lane * step < n && __ldg(&units[at].start) <= tile;
-    const int hit = __popc(__ballot_sync(0xffffffffu, below)) - 1;
-    n = min(step, n - hit * step);
-    lo += hit * step;
-  }
-  return lo;
-}
-
-// A CTA's run, piece by piece (a piece: consecutive key tiles of one unit). Every warp walks it by itself.
-struct LaWalk {
-  long long pos, end;
-  int h, rem, u, W1, units_n;
+// The header of the work list, and the length of a run.
+struct LaPlan {
+  bool together;
+  int units_n, cost, prefix, prefix_tiles, tokens;
+  bool fits;
+  int per, total;  // of all KV heads; a plan of 2^30 or more is refused
   const LaUnit* units;
-  LaUnit unit;
-  int j0, n;  // the piece: tiles [j0, j0 + n) of the unit
+  D3_DEV explicit LaPlan(const LaArgs& a) {
+    const int4 x = __ldg((const int4*)a.work), y = __ldg((const int4*)a.work + 1);
+    const int T = __ldg(a.work + LW_T);
+    together = x.x != 0;
+    units_n = x.y;
+    cost = x.z;
+    prefix = x.w;
+    prefix_tiles = y.x;
+    tokens = y.y;
+    const long long all = (long long)cost * a.Hkv;
+    fits = y.z == a.G && y.w == a.B && T == a.T && all < 0x40000000;
+    total = fits ? (int)all : 0;
+    per = max((int)((unsigned)(total + a.runs - 1) / (unsigned)a.runs), LA_MIN_RUN);
+    units = (const LaUnit*)(a.work + la_unit_offset(a.T));
+  }
+  D3_DEV LaUnit unit(int u) const {
+    const int4 x = __ldg((const int4*)(units + u)), y = __ldg((const int4*)(units + u) + 1);
+    return LaUnit{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  }
+  // The last unit that begins at or before `place`, by the whole warp: 32 probes a round.
+  D3_DEV int find(int place) const {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = units_n;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const bool below = lane * step < n && __ldg(&units[lo + lane * step].at) - LA_UNIT_COST <= place;
+      const int hit = __popc(__ballot_sync(0xffffffffu, below)) - 1;
+      n = min(step, n - hit * step);
+      lo += hit * step;
+    }
+    return lo;
+  }
+};
 
-  D3_DEV void start(const LaArgs& a, int run) {
-    const long long per = la_run_tiles(a), total = (long long)a.work[LW_TILES] * a.Hkv;
-    pos = per * run;
-    end = pos + per < total ? pos + per : total;
-    W1 = a.work[LW_TILES];
-    units_n = a.work[LW_UNITS];
-    units = (const LaUnit*)(a.work + la_unit_offset(a.B));
+// A CTA's run, piece by piece (a piece: consecutive key tiles of one unit, one at least). Every warp walks it by
+// itself; the next unit is on its way while this one is worked on.
+struct LaWalk {
+  int pos, end;  // where the run goes on and ends
+  int head0;     // where the KV head's units begin
+  int h, u;
+  int j0, n;     // the piece: tiles [j0, j0 + n) of unit u
+  int tiles;     // of the unit
+
+  D3_DEV LaWalk(const LaArgs& a, const LaPlan& p, int run) {
+    pos = p.per * run;
+    end = p.fits ? min(pos + p.per, p.total) : 0;
     if (pos < end) {
-      h = (int)(pos / W1);
-      rem = (int)(pos - (long long)h * W1);
-      u = la_find_unit(units, units_n, rem);
+      h = (unsigned)pos / (unsigned)p.cost;
+      head0 = h * p.cost;
+      u = p.find(pos - head0);
     }
   }
-  D3_DEV bool next() {
-    if (pos >= end) return false;
-    unit = la_unit(units, u);
-    j0 = rem - unit.start;
-    n = (int)min((long long)(unit.tiles - j0), end - pos);
-    return true;
+  D3_DEV bool next(const LaPlan& p, LaUnit& unit) {
+    while (pos < end) {
+      unit = p.unit(u);
+      tiles = unit.tiles;
+      const int first = head0 + unit.at;
+      j0 = max(0, pos - first);
+      n = min(end, first + unit.tiles) - first - j0;
+      pos = first + j0;
+      if (n > 0) {
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.units + (u + 1 < p.units_n ? u + 1 : 0)));
+        return true;
+      }
+      pos = end;  // it ends before the unit's first tile
+    }
+    return false;
   }
-  D3_DEV void step() {
+  D3_DEV void step(const LaPlan& p) {
     pos += n;
-    rem += n;
-    if (++u == units_n) {
+    if (j0 + n == tiles && ++u == p.units_n) {
       u = 0;
-      rem = 0;
       ++h;
+      head0 += p.cost;
     }
   }
 };
 
-// What a unit's rows and key tiles are.
-struct LaSpan {
-  int rows;       // rows of the unit
-  int lead;       // key tiles of the prefix at its front
-  int prefix;     // keys of the prefix
-  int own_end;    // own keys that its last row sees (0 for a prefix unit)
-  int kept, token0;
-  D3_DEV LaSpan(const LaArgs& a, const LaUnit& u) {
-    prefix = a.work[LW_PREFIX];
-    if (u.line < 0) {
-      rows = min(LA_ROWS, a.work[LW_TOKENS] * a.G - u.row0);
-      lead = u.tiles;
-      own_end = kept = token0 = 0;
-    } else {
-      token0 = a.cu[u.line];
-      const int all = (a.cu[u.line + 1] - token0) * a.G;
-      rows = min(LA_ROWS, all - u.row0);
-      lead = a.work[LW_TOGETHER] ? a.work[LW_PREFIX_TILES] : 0;
-      kept = a.work[LW_HEADER + u.line];
-      own_end = kept + (u.row0 + rows - 1) / a.G + 1;
-    }
-  }
-  // first key of tile j (of the prefix when own is false) and how many of its LA_KEYS there are
-  D3_DEV int tile(int j, bool& own, int& valid) const {
-    own = j >= lead;
-    const int key0 = (own ? j - lead : j) * LA_KEYS;
-    valid = min(LA_KEYS, (own ? own_end : prefix) - key0);
-    return key0;
-  }
-};
-
-// Shared-memory descriptor of V as the MMA's B: MN-major (columns contiguous), 128-byte swizzle; 8 keys x 64 columns
-// atoms of 1024 bytes, SBO between groups of 8 keys, LBO between 64-column slices.
-D3_DEV uint64_t la_v_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((LA_KEYS * 128) >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// First key of tile j of a unit (of the prefix when own is false) and how many of its LA_KEYS there are.
+D3_DEV int la_tile(const LaPlan& p, const LaUnit& u, int j, bool& own, int& valid) {
+  own = j >= u.lead;
+  const int key0 = (own ? j - u.lead : j) * LA_KEYS;
+  valid = min(LA_KEYS, (own ? u.own_end : p.prefix) - key0);
+  return key0;
 }
 
-// D += A B with A in tensor memory (16-bit values, two to a column).
-D3_DEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory descriptor of a V stage as the MMA's B: MN-major (columns contiguous), 128-byte swizzle, atoms of 8
+// keys x 64 columns 1024 bytes apart (SBO); N is one atom wide, so that LBO is not used.
+D3_DEV uint64_t la_v_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(LA_STAGE >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// The MMA warp runs its loop with all lanes, so that descriptors stay in uniform registers, and issues from the lane
+// that elect.sync names. (Issued from a branch on the lane number, each MMA paid about 100 cycles to move its
+// operands into uniform registers: twelve a tile, twice the time of the products themselves.)
+D3_DEV uint32_t la_elect() {
+  uint32_t e;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+// D (+)= A B, both from shared memory.
+D3_DEV void la_mma_ss(uint32_t elected, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                      uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+// D (+)= A B with A in tensor memory (16-bit values, two to a column).
+D3_DEV void la_mma_ts(uint32_t elected, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                      uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+D3_DEV void la_commit(uint32_t elected, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(elected)
       : "memory");
 }
 
@@ -205,7 +245,7 @@ D3_DEV void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32
 #define LA_V8(r, o) \
   "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
 
-// 32 or 64 columns of this warp's 32 lanes. The wait is part of the statement, so that nothing reads the registers
+// 32 columns of this warp's 32 lanes. The wait is part of the statement, so that nothing reads the registers
 // ahead of it.
 D3_DEV void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -216,16 +256,6 @@ D3_DEV void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
-D3_DEV void tmem_ld64(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
-      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : LA_R8(r, 0), LA_R8(r, 8), LA_R8(r, 16), LA_R8(r, 24), LA_R8(r, 32), LA_R8(r, 40), LA_R8(r, 48), LA_R8(r, 56)
-      : "r"(taddr)
-      : "memory");
-}
 D3_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -233,7 +263,22 @@ D3_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
       LA_V8(r, 8), LA_V8(r, 16), LA_V8(r, 24), "r"(taddr)
       : "memory");
 }
+D3_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::LA_V8(r, 0),
+      LA_V8(r, 8), "r"(taddr)
+      : "memory");
+}
 D3_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Box of the 3-D map of the queries (column, head, token).
+D3_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
 
 // Box of the 4-D cache map (column, key in page, head, page).
 D3_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
@@ -246,12 +291,88 @@ D3_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, in
 
 // mbar_wait by a whole warp, with the same answer for all of its lanes, together again afterwards (the tensor-memory
 // instructions and shuffles that follow are the warp's).
-D3_DEV bool la_warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+D3_DEV bool la_warp_wait(uint64_t* bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const unsigned long long start = globaltimer();
+#pragma unroll 1
+  do {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  } while (__any_sync(0xffffffffu, globaltimer() - start < WAIT_LIMIT_NS));
+  record_fault(FAULT_WAIT_TIMEOUT);
+  return false;
+}
 
 D3_DEV float la_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Whether any of the `threads` threads that meet at named barrier `id` says yes; the barrier's threads all get the answer.
+D3_DEV bool la_any(int id, int threads, bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)yes), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+D3_DEV float la_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two 32-bit floats in a register pair, and arithmetic on both at once.
+D3_DEV uint64_t la_two(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+D3_DEV void la_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+D3_DEV uint64_t la_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+D3_DEV uint64_t la_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+D3_DEV uint64_t la_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two numbers without the special-function unit, which takes 16 a cycle of an SM where a tile of 128 x 128 scores
+// wants them as fast as its products: x = n + f with n the nearest whole number (by adding 1.5 x 2^23 + 127, which leaves
+// n + 127 in the low bits), 2^f on [-1/2, 1/2] by the polynomial of degree 4 whose largest relative error, 2.6e-6, is
+// the least (Remez' criterion; fitted by iteratively reweighted least squares), times 2^n built from its exponent.
+// Below -126: 2^-126. A NaN stays one.
+D3_DEV void la_exp2_poly(uint64_t x, float& lo, float& hi) {
+  float x0, x1;
+  la_split(x, x0, x1);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
+  x = la_two(x0, x1);
+  const float magic = 12582912.0f + 127.0f;
+  const uint64_t t = la_add2(x, la_two(magic, magic));
+  const uint64_t f = la_fma2(la_add2(t, la_two(-magic, -magic)), la_two(-1.0f, -1.0f), x);
+  uint64_t p = la_fma2(f, la_two(0.009570068679749966f, 0.009570068679749966f), la_two(0.055917806923389435f, 0.055917806923389435f));
+  p = la_fma2(p, f, la_two(0.240247443318367f, 0.240247443318367f));
+  p = la_fma2(p, f, la_two(0.6931218504905701f, 0.6931218504905701f));
+  p = la_fma2(p, f, la_two(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  la_split(t, t0, t1);
+  p = la_mul2(p, la_two(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
+  la_split(p, lo, hi);
 }
 
 template <bool F16>
@@ -264,20 +385,29 @@ D3_DEV uint32_t la_pack(float lo, float hi) {
   return r;
 }
 
+struct LaLimited { static constexpr bool value = true; };
+struct LaWhole { static constexpr bool value = false; };
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
-    lines_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, LaArgs a) {
+    lines_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap, LaArgs a) {
   using S = LaShape<D>;
   extern __shared__ __align__(1024) uint8_t la_smem[];
   uint8_t* q_s = la_smem;
   uint8_t* ring = la_smem + S::Q_BYTES;
-  uint64_t* bars = (uint64_t*)(la_smem + S::Q_BYTES + S::STAGES * S::STAGE);
+  uint64_t* bars = (uint64_t*)(la_smem + S::Q_BYTES + S::STAGES * LA_STAGE);
+  uint8_t* small = (uint8_t*)bars;
+  LaPlan* plan_s = (LaPlan*)(small + LA_PLAN_AT);
+  LaWalk* walk_s = (LaWalk*)(small + LA_WALK_AT) + (threadIdx.x >> 5) - LA_ROW_WARP;
+  static_assert(sizeof(LaPlan) <= LA_WALK_AT - LA_PLAN_AT && sizeof(LaWalk) == LA_WALK_BYTES, "layout");
   uint64_t* kv_full = bars;                    // [STAGES]
   uint64_t* kv_empty = kv_full + S::STAGES;    // [STAGES]
   uint64_t* q_full = kv_empty + S::STAGES;
-  uint64_t* s_full = q_full + 1;               // [2]
-  uint64_t* p_full = s_full + 2;               // [2]
-  uint64_t* o_full = p_full + 2;               // [2], by tile parity: a waiter may be up to two products behind
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;              // [2]
+  uint64_t* p_full = s_full + 2;               // [2][2], by halves of the keys
+  uint64_t* o_full = p_full + 4;               // [2], by tile parity: a waiter may be up to two products behind
   uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = blockIdx.x;
   const bool aligned = (smem_u32(la_smem) & 1023u) == 0;  // the swizzle's atoms
@@ -286,10 +416,12 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, 1);
     }
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(p_full + 2 * i, LA_ROW_WARPS);
+      mbar_init(p_full + 2 * i + 1, LA_ROW_WARPS);
       mbar_init(o_full + i, 1);
     }
     fence_mbar_init();
@@ -303,228 +435,344 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   tc_fence_after();
   allow_dependents();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_o = tmem, tmem_s = tmem + D;  // S / P buffer b: columns D + 64 b
-  const bool fits = la_plan_fits(a) && aligned;
-  if (!fits && tid == 0) record_fault(FAULT_PLAN);
-  LaWalk w;
-  w.pos = w.end = 0;
-  if (fits && a.work[LW_TILES] > 0) w.start(a, run);
+  const uint32_t tmem_o = tmem, tmem_s = tmem + D;  // S buffer b: columns D + 128 b;
+  // P of its keys 32 j .. 32 j + 31 in the first 16 columns of theirs
+  LaPlan plan(a);
+  if (!plan.fits || !aligned) {
+    plan.fits = false;
+    if (tid == 0) record_fault(FAULT_PLAN);
+  }
+  LaWalk w(a, plan, run);
 
   if (warp == 0) {
-    // ---- loads: K0, K1, V0, K2, V1, ... of each piece
-    uint32_t seq = 0;
+    // ---- loads: a piece's Q, then K0, V0, K1, V1, ... (two S buffers: K0, K1, V0, K2, V1, ...)
+    uint32_t seq = 0, pieces = 0;
     bool ok = true;
     int win_first = 0, win_page = -1;  // a window of 32 page ids, one per lane
     const int* win_table = nullptr;
-    const int slice = lane % S::SLICES, box = lane / S::SLICES;
-    auto fetch = [&](const CUtensorMap* map, int h, int boxes, int page_id, int in_page) {
-      const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
-      ++seq;
-      ok = la_warp_wait(kv_empty + st, ph ^ 1);
-      if (!ok) return;
-      if (lane == 0) mbar_arrive_expect_tx(kv_full + st, boxes * a.page_box * S::SLICES * 128);
-      __syncwarp();
-      if (box < boxes)
-        tma_load_4d(smem_u32(ring) + st * S::STAGE + slice * (LA_KEYS * 128) + box * a.page_box * 128, map, slice * 64,
-                    in_page, h, page_id, kv_full + st);
+    const uint32_t q_bytes = (uint32_t)(la_tile_tokens(a.G) * a.G * 128);  // of a 64-column slice
+    struct Boxes {  // a tile's: lane l issues box l
+      int n, page_id, in_page;
     };
-    for (; ok && w.next(); w.step()) {
-      const LaSpan sp(a, w.unit);
-      int before_boxes = 0, before_page = 0, before_in = 0;
+    auto fetch = [&](const CUtensorMap* map, int h, const Boxes& t) {
+#pragma unroll
+      for (int sl = 0; sl < S::SLICES; ++sl) {
+        const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
+        ++seq;
+        if (!(ok = la_warp_wait(kv_empty + st, ph ^ 1))) return;
+        if (lane == 0) mbar_arrive_expect_tx(kv_full + st, t.n * a.page_box * 128);
+        __syncwarp();
+        if (lane < t.n)
+          tma_load_4d(smem_u32(ring) + st * LA_STAGE + lane * a.page_box * 128, map, sl * 64, t.in_page, h, t.page_id,
+                      kv_full + st);
+      }
+    };
+    for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
+      if (!(ok = la_warp_wait(q_empty, (pieces & 1) ^ 1))) break;
+      ++pieces;
+      if (lane == 0) mbar_arrive_expect_tx(q_full, q_bytes * S::SLICES);
+      __syncwarp();
+      if (lane < S::SLICES)
+        tma_load_3d(smem_u32(q_s) + lane * (LA_ROWS * 128), &qmap, lane * 64, w.h * a.G, unit.token0, q_full);
+      Boxes before = {};
       for (int i = 0; ok && i < w.n; ++i) {
         bool own;
         int valid;
-        const int key0 = sp.tile(w.j0 + i, own, valid);
-        const int boxes = (valid + a.page_box - 1) / a.page_box;
-        const int first = key0 / a.page, in_page = key0 - first * a.page;
-        const int* table = own ? a.table + (size_t)w.unit.line * a.W : a.prefix_table;
+        const int key0 = la_tile(plan, unit, w.j0 + i, own, valid);
+        Boxes t;
+        t.n = (valid + a.page_box - 1) / a.page_box;
+        const int key = key0 + lane * a.page_box, first = key0 / a.page, last = (key0 + valid - 1) / a.page;
+        const int* table = own ? a.table + (size_t)unit.line * a.W : a.prefix_table;
         const int width = own ? a.W : a.PW;
-        if (table != win_table || first < win_first || first + boxes > win_first + 32) {
+        if (table != win_table || first < win_first || last >= win_first + 32) {
           win_table = table;
           win_first = first;
           win_page = first + lane < width ? table[first + lane] : -1;
         }
-        int page_id = __shfl_sync(0xffffffffu, win_page, (first - win_first + box) & 31);
-        if (box < boxes && (page_id < 0 || page_id >= a.pages)) {
+        const int index = key / a.page;
+        t.in_page = key - index * a.page;
+        t.page_id = __shfl_sync(0xffffffffu, win_page, (index - win_first) & 31);
+        if (lane < t.n && (t.page_id < 0 || t.page_id >= a.pages)) {
           record_fault(FAULT_PAGES);
-          page_id = -1;  // outside the map: zeros
+          t.page_id = -1;  // outside the map: zeros
         }
-        fetch(&kmap, w.h, boxes, page_id, in_page);
-        if (ok && i > 0) fetch(&vmap, w.h, before_boxes, before_page, before_in);
-        before_boxes = boxes;
-        before_page = page_id;
-        before_in = in_page;
+        fetch(&kmap, w.h, t);
+        if (S::S_BUFS == 1) {
+          if (ok) fetch(&vmap, w.h, t);
+        } else {
+          if (ok && i > 0) fetch(&vmap, w.h, before);
+          before = t;
+        }
       }
-      if (ok) fetch(&vmap, w.h, before_boxes, before_page, before_in);
+      if (S::S_BUFS == 2 && ok) fetch(&vmap, w.h, before);
     }
     // nothing may land after the CTA is gone: a stage's last load has arrived once its phase is complete
+    if (pieces > 0) mbar_wait(q_full, (pieces - 1) & 1);
     for (uint32_t i = seq < (uint32_t)S::STAGES ? 0 : seq - S::STAGES; i < seq; ++i)
       mbar_wait(kv_full + i % S::STAGES, (i / S::STAGES) & 1);
   } else if (warp == 1) {
     // ---- MMAs
-    if (lane == 0) {
-      const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
-      const uint32_t idesc_s = (1u << 4) | type | ((LA_KEYS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
-      const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((LA_ROWS >> 4) << 24);
-      uint32_t seq = 0, tiles = 0, pieces = 0;
-      bool ok = true;
-      const uint32_t q_base = smem_u32(q_s), ring_base = smem_u32(ring);
-      auto scores = [&](uint32_t tile) {
+    const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
+    const uint32_t idesc_s = (1u << 4) | type | ((LA_KEYS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((64 >> 3) << 17) | ((LA_ROWS >> 4) << 24);
+    const uint32_t elected = la_elect();
+    uint32_t seq = 0, tiles = 0, pieces = 0;
+    bool ok = true;
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(ring)),
+                   v_desc = la_v_desc(smem_u32(ring));  // addresses are in 16-byte units: sums stay within 14 bits
+    auto scores = [&](uint32_t tile, bool last) {
+      const uint32_t d = tmem_s + 128 * (tile % S::S_BUFS);
+#pragma unroll
+      for (int sl = 0; sl < S::SLICES; ++sl) {
         const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
         ++seq;
-        if (!(ok = mbar_wait(kv_full + st, ph))) return;
+        if (!(ok = la_warp_wait(kv_full + st, ph))) return;
         tc_fence_after();
-        const uint32_t kb = ring_base + st * S::STAGE;
+        const uint64_t kb = k_desc + st * (LA_STAGE >> 4), qb = q_desc + sl * (LA_ROWS * 128 >> 4);
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-          umma_f16(tmem_s + 64 * (tile & 1), umma_desc_sw128(q_base + (c >> 2) * (LA_ROWS * 128) + (c & 3) * 32),
-                   umma_desc_sw128(kb + (c >> 2) * (LA_KEYS * 128) + (c & 3) * 32), idesc_s, c > 0);
-        umma_commit(kv_empty + st);
-        umma_commit(s_full + (tile & 1));
-      };
-      for (; ok && w.next(); w.step()) {
-        if (!(ok = mbar_wait(q_full, pieces & 1))) break;
-        ++pieces;
-        tc_fence_after();
-        scores(tiles);
-        for (int i = 0; ok && i < w.n; ++i, ++tiles) {
-          if (i + 1 < w.n) {
-            // S of tile + 1 goes where P of tile - 1 is, once that product has read it
-            if (i > 0 && !(ok = mbar_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
-            scores(tiles + 1);
-          }
-          if (!ok || !(ok = mbar_wait(p_full + (tiles & 1), (tiles >> 1) & 1))) break;
-          const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
-          ++seq;
-          if (!(ok = mbar_wait(kv_full + st, ph))) break;
+        for (int c = 0; c < 4; ++c) la_mma_ss(elected, d, qb + 2 * c, kb + 2 * c, idesc_s, sl > 0 || c > 0);
+        la_commit(elected, kv_empty + st);
+      }
+      if (last) la_commit(elected, q_empty);
+      la_commit(elected, s_full + tile % S::S_BUFS);
+    };
+    // S of a tile goes where P of an earlier one is (with one buffer, the last one's): the tensor core takes a CTA's
+    // products in the order in which they were issued, and O += P V of that tile was issued before
+    for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
+      if (!(ok = la_warp_wait(q_full, pieces & 1))) break;
+      ++pieces;
+      tc_fence_after();
+      scores(tiles, w.n == 1);
+      for (int i = 0; ok && i < w.n; ++i, ++tiles) {
+        if (S::S_BUFS == 2 && i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
+        const uint32_t buf = tiles % S::S_BUFS;
+        // V (and the next K) before P, for which the wait is long: the products then follow one another
+        const uint32_t v0 = seq;
+        seq += S::SLICES;
+#pragma unroll
+        for (int sl = 0; sl < S::SLICES; ++sl)
+          ok = ok && la_warp_wait(kv_full + (v0 + sl) % S::STAGES, ((v0 + sl) / S::STAGES) & 1);
+        if (S::S_BUFS == 1 && i + 1 < w.n)
+#pragma unroll
+          for (int sl = 0; sl < S::SLICES; ++sl)
+            ok = ok && la_warp_wait(kv_full + (seq + sl) % S::STAGES, ((seq + sl) / S::STAGES) & 1);
+        // the product by halves of the keys, as their weights come: keys 32 .. 63 and 96 .. 127, then the others
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          if (!ok || !(ok = la_warp_wait(p_full + 2 * buf + part, (tiles / S::S_BUFS) & 1))) break;
           tc_fence_after();
-          const uint32_t vb = ring_base + st * S::STAGE;
 #pragma unroll
-          for (int c = 0; c < LA_KEYS / 16; ++c)
-            umma_f16_ts(tmem_o, tmem_s + 64 * (tiles & 1) + 8 * c, la_v_desc(vb + c * 2048), idesc_o, i > 0 || c > 0);
-          umma_commit(kv_empty + st);
-          umma_commit(o_full + (tiles & 1));
+          for (int sl = 0; sl < S::SLICES; ++sl) {
+            const uint32_t st = (v0 + sl) % S::STAGES;
+            const uint64_t vb = v_desc + st * (LA_STAGE >> 4);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int c = (x & 1) + 4 * (x >> 1) + 2 * (1 - part);  // 16 keys
+              la_mma_ts(elected, tmem_o + 64 * sl, tmem_s + 128 * buf + 32 * (c >> 1) + 8 * (c & 1), vb + (c * 2048 >> 4),
+                        idesc_o, i > 0 || part > 0 || x > 0);
+            }
+            if (part == 1) la_commit(elected, kv_empty + st);
+          }
         }
+        if (!ok) break;
+        la_commit(elected, o_full + (tiles & 1));
+        if (S::S_BUFS == 1 && i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
       }
     }
-    __syncwarp();
   } else {
     // ---- rows
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, half = (warp - LA_ROW_WARP) >> 2;  // tensor-memory lanes; keys 64 half .. + 63
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-    const int row = 32 * quarter + lane;
+    const int row = 32 * quarter + lane, tok = row / a.G, g = row - tok * a.G;
+    if (lane == 0) {
+      if (warp == LA_ROW_WARP) *plan_s = plan;
+      *walk_s = w;
+    }
+    named_sync(9, 32 * LA_ROW_WARPS);
+    // between a row's two threads: their maxima (as bfloat16, rounded to nearest: any number near the maximum serves,
+    // if both take the same), or a sum
+    uint16_t* maxima = (uint16_t*)(small + LA_EXCHANGE) + 2 * row;
+    float* total = (float*)(small + LA_EXCHANGE) + row;
     uint32_t seq = 0, tiles = 0;
-    bool ok = true;
-    for (; ok && w.next(); w.step()) {
-      const LaSpan sp(a, w.unit);
-      const int R = w.unit.row0 + row;
-      const bool live = row < sp.rows, any = 32 * quarter < sp.rows;
-      const int tok = R / a.G;
-      const int t = w.unit.line < 0 ? tok : sp.token0 + tok, head = w.h * a.G + R - tok * a.G;
-      const int own_keys = sp.kept + tok + 1;  // own keys that this row sees
-      // stage Q: this warp's 32 rows, 16 bytes a lane; rows past the unit's are zeros
-      if (any) {
-        constexpr int CH = D / 8;  // 16-byte chunks of a row
-        const long long off = live ? (long long)t * a.q_token + (long long)head * a.q_head : -1;
-#pragma unroll 8
-        for (int i = 0; i < CH; ++i) {
-          const int x = i * 32 + lane, r = x / CH, c = x % CH;
-          const long long o = __shfl_sync(0xffffffffu, off, r);
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (o >= 0) v = *(const uint4*)((const uint16_t*)a.q + o + 8 * c);
-          *(uint4*)(q_s + (c >> 3) * (LA_ROWS * 128) + sw128_offset(32 * quarter + r, c & 7)) = v;
-        }
-        fence_async_smem();
+    bool ok = true, cut = false;
+    while (ok) {
+      int n, n_shared;  // tiles of the piece, and those of them that are the prefix's
+      // keys that there are, from the piece's first tile on: of the prefix, of the line, of these that this row sees
+      int shared_end, own_end, own_sees;
+      bool any;  // whether this warp has rows
+      {
+        LaWalk w = *walk_s;
+        __syncwarp();
+        LaUnit unit;
+        if (!w.next(*plan_s, unit)) break;
+        if (lane == 0) *walk_s = w;
+        __syncwarp();
+        n = w.n;
+        n_shared = unit.lead - w.j0;
+        shared_end = plan_s->prefix - w.j0 * LA_KEYS;
+        own_end = unit.own_end - (w.j0 - unit.lead) * LA_KEYS;
+        own_sees = unit.sees + tok - (w.j0 - unit.lead) * LA_KEYS;
+        any = 32 * quarter < unit.rows;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-      float m = -INFINITY, l = 0.0f;
-      for (int i = 0; i < w.n; ++i, ++tiles) {
-        const uint32_t buf = tiles & 1;
-        if (!(ok = la_warp_wait(s_full + buf, (tiles >> 1) & 1))) break;
+      float m = -INFINITY, l = 0.0f;  // of the row; of this thread's keys
+      for (int i = 0; i < n; ++i, ++tiles) {
+        const uint32_t buf = tiles % S::S_BUFS;
+        if (!(ok = la_warp_wait(s_full + buf, (tiles / S::S_BUFS) & 1))) break;
         tc_fence_after();
-        bool own;
-        int valid;
-        const int key0 = sp.tile(w.j0 + i, own, valid);
-        if (any) {
-          uint32_t s[64];
-          tmem_ld64(tmem_s + lanes + 64 * buf, s);
-          const int lim = own ? min(valid, own_keys - key0) : valid;
-          if (lim < LA_KEYS) {
-#pragma unroll
-            for (int x = 0; x < 64; ++x)
-              if (x >= lim) s[x] = 0xff800000u;  // -inf
+        const int valid = (i < n_shared ? shared_end : own_end) - i * LA_KEYS;  // keys of this tile, if not all
+        if (valid < LA_KEYS) {
+          // V's rows past the end, in the stages of this tile's V
+          const uint32_t vs = seq + S::SLICES * (S::S_BUFS == 1 ? 2 * i + 1 : i + 1 < n ? 2 * i + 2 : 2 * n - 1);
+          for (int sl = 0; ok && sl < S::SLICES; ++sl) {
+            const uint32_t st = (vs + sl) % S::STAGES;
+            if (!(ok = la_warp_wait(kv_full + st, ((vs + sl) / S::STAGES) & 1))) break;
+            for (int r = valid + 4 * (warp - LA_ROW_WARP) + (lane >> 3); r < LA_KEYS; r += 4 * LA_ROW_WARPS)
+              *(uint4*)(ring + st * LA_STAGE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          float mx = __uint_as_float(s[0]);
+          if (!ok) break;
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (any) {
+          const uint32_t s_at = tmem_s + lanes + 128 * buf + 64 * half;
+          // of this thread's 64 keys, those that there are and that its row sees
+          const int lim = (i < n_shared ? valid : own_sees - i * LA_KEYS) - 64 * half;
+          // Two forms of the same steps, with and without a limit inside the tile, chosen by the whole warp: with the
+          // comparisons in the one form every tile paid for them.
+          const bool cut_tile = __any_sync(0xffffffffu, lim < 64);
+          uint32_t s[32];
+          // 32 keys' scores (-inf past the limit)
+          auto load = [&](int c, auto limited) {
+            tmem_ld32(s_at + c, s);
+            if constexpr (decltype(limited)::value) {
 #pragma unroll
-          for (int x = 1; x < 64; ++x) mx = fmaxf(mx, __uint_as_float(s[x]));
-          mx *= a.scale_log2;
-          if (i == 0) {
-            m = mx;
-          } else if (__any_sync(0xffffffffu, mx > m + LA_RESCALE || (m == -INFINITY && mx > m))) {
-            const float top = fmaxf(m, mx);
-            const float f = m == -INFINITY ? 0.0f : la_exp2(m - top);
-            m = top;
+              for (int x = 0; x < 32; ++x)
+                if (c + x >= lim) s[x] = 0xff800000u;
+            }
+          };
+          auto top = [&]() {
+            float t[4];  // four chains
+#pragma unroll
+            for (int x = 0; x < 4; ++x) t[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 4]));
+#pragma unroll
+            for (int x = 8; x < 32; x += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                t[y] = la_max3(t[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
+            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          };
+          auto maximum = [&](auto limited) {
+            load(0, limited);
+            const float first = top();
+            load(32, limited);
+            return fmaxf(first, top()) * a.scale_log2;
+          };
+          const float mx = cut_tile ? maximum(LaLimited{}) : maximum(LaWhole{});
+          if (la_any(1 + quarter, 64, i == 0 || mx > m + LA_RESCALE || (m == -INFINITY && mx > m))) {
+            maxima[half] = __bfloat16_as_ushort(__float2bfloat16_rn(mx));
+            named_sync(1 + quarter, 64);
+            const uint32_t both = *(const uint32_t*)maxima;
+            const float t = fmaxf(m, fmaxf(bf16_to_f32(both & 0xffffu), bf16_to_f32(both >> 16)));
+            const float f = m == -INFINITY ? 0.0f : la_exp2(m - t);
+            m = t;
             l *= f;
-            if (!(ok = la_warp_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
-            tc_fence_after();
+            if (i > 0) {
+              if (!(ok = la_warp_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 2; c += 32) {  // each of the two warps half of the columns
+                uint32_t o[32];
+                const uint32_t at = tmem_o + lanes + half * (D / 2) + c;
+                tmem_ld32(at, o);
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(tmem_o + lanes + c, o);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st32(tmem_o + lanes + c, o);
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                tmem_st32(at, o);
+              }
+              tmem_wait_st();
             }
           }
           const float base = m == -INFINITY ? 0.0f : m;
-          uint32_t p[32];
-          float sum = 0.0f;
+          const uint64_t scale2 = la_two(a.scale_log2, a.scale_log2), base2 = la_two(-base, -base);
+          uint64_t sums[2] = {0, 0};
+          auto weigh = [&](int c, auto limited) {
+            uint32_t p[16];
 #pragma unroll
-          for (int x = 0; x < 64; x += 2) {
-            const float p0 = la_exp2(fmaf(__uint_as_float(s[x]), a.scale_log2, -base));
-            const float p1 = la_exp2(fmaf(__uint_as_float(s[x + 1]), a.scale_log2, -base));
-            sum += p0 + p1;
-            p[x / 2] = la_pack<F16>(p0, p1);
-          }
-          l += sum;
-          tmem_st32(tmem_s + lanes + 64 * buf, p);
-          tmem_wait_st();
+            for (int x = 0; x < 32; x += 2) {
+              const uint64_t y = la_fma2(la_two(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, base2);
+              float p0, p1;
+              if (!decltype(limited)::value && x / 2 % 4 == 1) {  // a pair in four
+                la_exp2_poly(y, p0, p1);
+              } else {
+                la_split(y, p0, p1);
+                p0 = la_exp2(p0);
+                p1 = la_exp2(p1);
+              }
+              sums[x / 2 & 1] = la_add2(sums[x / 2 & 1], la_two(p0, p1));
+              p[x / 2] = la_pack<F16>(p0, p1);
+            }
+            tmem_st16(s_at + c, p);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+          };
+          auto weights = [&](auto limited) {
+            weigh(32, limited);  // still in registers
+            if (lane == 0) mbar_arrive(p_full + 2 * buf);
+            load(0, limited);
+            weigh(0, limited);
+            if (lane == 0) mbar_arrive(p_full + 2 * buf + 1);
+          };
+          if (cut_tile)
+            weights(LaLimited{});
+          else
+            weights(LaWhole{});
+          float s0, s1;
+          la_split(la_add2(sums[0], sums[1]), s0, s1);
+          l += s0 + s1;
+        } else if (lane == 0) {
+          mbar_arrive(p_full + 2 * buf);
+          mbar_arrive(p_full + 2 * buf + 1);
         }
-        if (valid < LA_KEYS) {
-          // V's rows past the end: V of tile i is the (i + 1 < n ? 2 i + 2 : 2 n - 1)-th load of the piece
-          const uint32_t vs = seq + (i + 1 < w.n ? 2 * i + 2 : 2 * w.n - 1);
-          if (!(ok = la_warp_wait(kv_full + vs % S::STAGES, (vs / S::STAGES) & 1))) break;
-          uint8_t* v = ring + (vs % S::STAGES) * S::STAGE;
-          for (int x = tid - 32 * LA_ROW_WARP; x < (LA_KEYS - valid) * 8 * S::SLICES; x += 128) {
-            const int c = x & 7, r = (x >> 3) % (LA_KEYS - valid), sl = (x >> 3) / (LA_KEYS - valid);
-            *(uint4*)(v + sl * (LA_KEYS * 128) + (valid + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_async_smem();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + buf);
       }
-      seq += 2 * w.n;
       if (!ok) break;
+      seq += 2 * S::SLICES * n;
       if (!(ok = la_warp_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
       tc_fence_after();
+      if (any) {  // the row's sum: both threads', the same order in both
+        if (half == 1) *total = l;
+        named_sync(1 + quarter, 64);
+        if (half == 0) *total = l += *total;
+        named_sync(1 + quarter, 64);
+        l = *total;
+      }
       // results: a whole unit's rows are done; a part's go to the workspace
-      const bool first = w.j0 == 0, last = w.j0 + w.n == w.unit.tiles;
-      const bool apart = !a.work[LW_TOGETHER];
-      const bool whole = first && last && !apart;
-      long long part = 0;
+      const LaPlan plan = *plan_s;
+      LaWalk w = *walk_s;
+      const LaUnit unit = plan.unit(w.u);
+      const bool live = row < unit.rows;
+      const bool first = w.j0 == 0, last = w.j0 + w.n == unit.tiles;
+      const bool whole = first && last && plan.together;
+      long long part = row;
       if (!first)
-        part = la_part_rest(run) + row;
-      else if (apart)
-        part = la_part_apart(a, w.unit.line >= 0, w.h, w.unit.line < 0 ? R : sp.token0 * a.G + R);
+        part += la_part_rest(run);
+      else if (!plan.together)
+        part += la_part_apart(a, unit.line >= 0, w.h) + (long long)unit.token0 * a.G;
       else
-        part = la_part_open(a, run) + row;
+        part += la_part_open(a, run);
+      if (!first && plan.together) {
+        // a unit's first cut, at this run's start, has it joined
+        const int from = w.head0 + unit.at;
+        if (from / plan.per == run - 1) {
+          cut = true;
+          if (tid == 32 * LA_ROW_WARP)
+            a.cuts[run] = make_int4(unit.token0, unit.rows, w.h, (from + unit.tiles - 1) / plan.per);
+        }
+      }
       if (any) {
+        const int t = unit.token0 + tok, head = w.h * a.G + g;
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
+#pragma unroll 1
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
           uint32_t o[32];
           tmem_ld32(tmem_o + lanes + c, o);
           if (live && whole) {
@@ -538,12 +786,13 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
               dst[x] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           } else if (live) {
-            uint4* dst = (uint4*)(a.part_o + part * D + c);
+            uint4* dst = (uint4*)a.part_o + la_part_at<D>(part, c / 4);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            for (int x = 0; x < 8; ++x)
+              dst[32 * x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
         }
-        if (live) {
+        if (live && half == 0) {
           if (!whole)
             a.part_ml[part] = make_float2(m, l);
           else if (a.lse)
@@ -551,13 +800,18 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
         }
       }
       tc_fence_before();
+      w.step(plan);
+      __syncwarp();
+      if (lane == 0) *walk_s = w;
+      __syncwarp();
     }
+    if (tid == 32 * LA_ROW_WARP && !cut) a.cuts[run] = make_int4(0, 0, 0, 0);
     // tokens of no line: nothing to see
-    if (fits) {
-      const int tokens = a.work[LW_TOKENS];
-      const long long total = (long long)(a.T - tokens) * a.Hq;
-      for (long long x = (long long)run * 4 + warp - LA_ROW_WARP; x < total; x += (long long)a.runs * 4) {
-        const long long r = (long long)tokens * a.Hq + x;
+    if (plan.fits) {
+      const long long total = (long long)(a.T - plan.tokens) * a.Hq;
+      for (long long x = (long long)run * LA_ROW_WARPS + warp - LA_ROW_WARP; x < total;
+           x += (long long)a.runs * LA_ROW_WARPS) {
+        const long long r = (long long)plan.tokens * a.Hq + x;
         for (int c = lane; c < D / 8; c += 32)
           *(uint4*)((uint16_t*)a.out + r * D + 8 * c) = make_uint4(0, 0, 0, 0);
         if (a.lse && lane == 0) a.lse[r] = -INFINITY;
@@ -572,113 +826,104 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   }
 }
 
-// Joins the parts of a row: with M the largest of their maxima, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i. A
-// block of four warps per row, part i to warp i mod 4, then the four through shared memory.
-constexpr int LC_WARPS = 4;
+// Joins the parts of a row: with M the largest of their maxima, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, the
+// parts taken in order. A lane is a row (of 32 neighbouring ones of a KV head); a warp takes groups of four columns.
+// Bound by latency: LC_AHEAD parts are in flight at a time.
+constexpr int LC_WARPS = 8;
+constexpr int LC_AHEAD = 8;
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(LC_WARPS * 32) lines_combine_kernel(LaArgs a) {
-  constexpr int PER = D / 32;  // columns a lane holds: lane, lane + 32, ...
-  __shared__ float s_o[LC_WARPS][D];
-  __shared__ float2 s_ml[LC_WARPS];
+__global__ void __launch_bounds__(LC_WARPS * 32) lines_combine_kernel(LaArgs a, int column_blocks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   allow_dependents();
-  if (!la_plan_fits(a) || a.work[LW_TILES] <= 0) return;
-  const LaUnit* units = (const LaUnit*)(a.work + la_unit_offset(a.B));
-  const bool apart = !a.work[LW_TOGETHER];
-  const long long per = la_run_tiles(a);
-  const int W1 = a.work[LW_TILES], tokens = a.work[LW_TOKENS];
+  const LaPlan plan(a);
+  if (!plan.fits) return;
 
-  float m, l, o[PER];
-  auto add = [&](long long part) {
-    const float2 ml = a.part_ml[part];
-    float v[PER];
-#pragma unroll
-    for (int c = 0; c < PER; ++c) v[c] = a.part_o[part * D + 32 * c + lane];
-    if (ml.x == -INFINITY) return;
-    const float top = fmaxf(m, ml.x);
-    const float f = m == -INFINITY ? 0.0f : la_exp2(m - top), g = la_exp2(ml.x - top);
-    m = top;
-    l = l * f + ml.y * g;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) o[c] = o[c] * f + v[c] * g;
+  // the parts of a row: `first`, then those that the runs r0 + 1 .. r1 left at `rest` rows into theirs; and, prefix and
+  // own units apart, the same again for its own unit
+  struct Parts {
+    long long first;
+    int rest, r0, r1;
   };
-  // parts of unit u's row: the first one at `first_part`, the others by the runs that start inside the unit
-  int turn = 0;
-  auto add_unit = [&](const LaUnit& u, int h, long long first_part, int row) {
-    const long long s0 = (long long)h * W1 + u.start, s1 = s0 + u.tiles - 1;
-    const int r0 = (int)(s0 / per), r1 = (int)(s1 / per);
-    for (int r = r0; r <= r1; ++r, ++turn)
-      if (turn % LC_WARPS == warp) add(r == r0 ? first_part : la_part_rest(r) + row);
-  };
-  auto begin = [&]() {
-    m = -INFINITY;
-    l = 0.0f;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) o[c] = 0.0f;
-    turn = 0;
-  };
-  auto finish = [&](int t, int head) {
-    if (lane == 0) s_ml[warp] = make_float2(m, l);
-#pragma unroll
-    for (int c = 0; c < PER; ++c) s_o[warp][32 * c + lane] = o[c];
-    __syncthreads();
+  auto join = [&](int c, bool live, const Parts& p, const Parts& q, int t, int head) {
+    const int np = live ? p.r1 - p.r0 + 1 : 0, n = live ? np + q.r1 - q.r0 + 1 : 0;
+    const int longest = __reduce_max_sync(0xffffffffu, n);
     float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < longest; i0 += LC_AHEAD) {
+      float2 ml[LC_AHEAD];
+      float4 v[LC_AHEAD];
 #pragma unroll
-    for (int i = 0; i < LC_WARPS; ++i) M = fmaxf(M, s_ml[i].x);
-    float f[LC_WARPS];
-#pragma unroll
-    for (int i = 0; i < LC_WARPS; ++i) {
-      f[i] = s_ml[i].x == -INFINITY ? 0.0f : la_exp2(s_ml[i].x - M);
-      L += s_ml[i].y * f[i];
-    }
-    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-    const long long r = (long long)t * a.Hq + head;
-    for (int c = threadIdx.x; c < D / 2; c += LC_WARPS * 32) {
-      float x = 0.0f, y = 0.0f;
-#pragma unroll
-      for (int i = 0; i < LC_WARPS; ++i) {
-        x += s_o[i][2 * c] * f[i];
-        y += s_o[i][2 * c + 1] * f[i];
+      for (int j = 0; j < LC_AHEAD; ++j) {
+        const int i = i0 + j;
+        ml[j] = make_float2(-INFINITY, 0.0f);
+        if (i < n) {
+          const long long r = i < np ? (i == 0 ? p.first : la_part_rest(p.r0 + i) + p.rest)
+                                     : (i == np ? q.first : la_part_rest(q.r0 + i - np) + q.rest);
+          ml[j] = a.part_ml[r];
+          v[j] = a.part_o[la_part_at<D>(r, c)];
+        }
       }
-      ((uint32_t*)a.out)[(r * D) / 2 + c] = la_pack<F16>(x * inv, y * inv);
+      float top = M;
+#pragma unroll
+      for (int j = 0; j < LC_AHEAD; ++j) top = fmaxf(top, ml[j].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float f = la_exp2(M - base);  // 0 at first
+      L *= f;
+      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+      M = top;
+#pragma unroll
+      for (int j = 0; j < LC_AHEAD; ++j) {
+        if (ml[j].y == 0.0f) continue;  // nothing there (a NaN stays one)
+        const float g = la_exp2(ml[j].x - base);
+        L = fmaf(g, ml[j].y, L);
+        o.x = fmaf(g, v[j].x, o.x);
+        o.y = fmaf(g, v[j].y, o.y);
+        o.z = fmaf(g, v[j].z, o.z);
+        o.w = fmaf(g, v[j].w, o.w);
+      }
     }
-    if (a.lse && threadIdx.x == 0) a.lse[r] = (M + log2f(L)) * 0.69314718055994531f;
-    __syncthreads();
+    if (live) {
+      const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+      const long long r = (long long)t * a.Hq + head;
+      ((uint2*)a.out)[r * (D / 4) + c] =
+          make_uint2(la_pack<F16>(o.x * inv, o.y * inv), la_pack<F16>(o.z * inv, o.w * inv));
+      if (a.lse && c == 0) a.lse[r] = (M + log2f(L)) * 0.69314718055994531f;
+    }
   };
 
-  if (apart) {
-    const long long rows = (long long)tokens * a.Hq;
-    for (long long x = blockIdx.x; x < rows; x += gridDim.x) {
-      const int t = (int)(x / a.Hq), head = (int)(x - (long long)t * a.Hq), h = head / a.G, g = head - h * a.G;
-      const int packed = t * a.G + g;
-      begin();
-      add_unit(la_unit(units, packed / LA_ROWS), h, la_part_apart(a, false, h, packed), packed % LA_ROWS);
-      const int b = a.line[t];
-      const int R = (t - a.cu[b]) * a.G + g;
-      add_unit(la_unit(units, a.work[LW_HEADER + a.B + b] + R / LA_ROWS), h, la_part_apart(a, true, h, packed),
-               R % LA_ROWS);
-      finish(t, head);
+  if (plan.together) {
+    // the units that a run's end cuts: a block each, a warp 32 rows and half of the columns
+    for (int run = blockIdx.x; run < a.runs; run += gridDim.x) {
+      const int4 cut = a.cuts[run];
+      const int row = (warp & 3) * 32 + lane;
+      if (cut.y <= row - lane) continue;
+      const int tok = row / a.G;
+      for (int c = warp >> 2; c < D / 4; c += LC_WARPS / 4)
+        join(c, row < cut.y, Parts{la_part_open(a, run - 1) + row, row, run - 1, cut.w}, Parts{0, 0, 0, -1}, cut.x + tok,
+             cut.z * a.G + row - tok * a.G);
     }
     return;
   }
-  // together: only the units that a run's end cuts; the first such run start inside a unit takes it
-  const long long total = (long long)W1 * a.Hkv;
-  for (long long x = blockIdx.x; x < (long long)(a.runs - 1) * LA_ROWS; x += gridDim.x) {
-    const int run = 1 + (int)(x / LA_ROWS), row = (int)(x % LA_ROWS);
-    const long long pos = per * run;
-    if (pos >= total) continue;
-    const int h = (int)(pos / W1), rem = (int)(pos - (long long)h * W1);
-    const LaUnit u = la_unit(units, la_find_unit(units, a.work[LW_UNITS], rem));
-    const long long s0 = (long long)h * W1 + u.start;
-    if (s0 == pos || s0 / per != run - 1) continue;
-    const LaSpan sp(a, u);
-    if (row >= sp.rows) continue;
-    const int R = u.row0 + row, tok = R / a.G;
-    begin();
-    add_unit(u, h, la_part_open(a, run - 1) + row, row);
-    finish(sp.token0 + tok, h * a.G + R - tok * a.G);
+  const int groups = (int)(la_apart_rows(a.T, a.G) / 32), columns = D / 4 / column_blocks;
+  for (int x = blockIdx.x; x < groups * a.Hkv * column_blocks; x += gridDim.x) {
+    const int y = x / column_blocks, h = y / groups, packed = (y - h * groups) * 32 + lane;
+    const int t = packed / a.G;
+    const bool live = t < plan.tokens;
+    Parts p[2] = {};
+    if (live) {
+      const int units[2] = {t / la_tile_tokens(a.G), __ldg(a.work + LW_HEADER + t)};  // prefix unit, own unit
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const LaUnit u = plan.unit(units[i]);
+        const int from = h * plan.cost + u.at;
+        p[i] = Parts{la_part_apart(a, i == 1, h) + packed, packed - u.token0 * a.G, from / plan.per,
+                     (from + u.tiles - 1) / plan.per};
+      }
+    }
+    const int c0 = (x - y * column_blocks) * columns;
+    for (int c = c0 + warp; c < c0 + columns; c += LC_WARPS) join(c, live, p[0], p[1], t, h * a.G + packed - t * a.G);
   }
 }
 

@@ -21,29 +21,34 @@ namespace d3 {
 constexpr int LP_THREADS = 512;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOKENS = 2048;     // tokens placed by a block
-constexpr int LP_MAX_LINES = 8192;  // three scanned int arrays of it fill 96 KB of shared memory
+constexpr int LP_MAX_LINES = 8192;  // five int arrays of it fill 160 KB of shared memory
 constexpr int LP_MAX_KEPT = 1 << 30;  // lengths are clamped to it, so no index below overflows
 
-// The attention's work list. A unit is a tile of up to LA_ROWS rows (a row = a token and one of the `group` query
-// heads of a KV head, tokens first) and the key tiles of LA_KEYS that these rows attend to. The list is the same for
-// every KV head.
+// The attention's work list. A unit is a tile of rows, a row being a token and one of the `group` query heads of a KV
+// head: la_tile_tokens(group) whole tokens, LA_ROWS rows at most; and the key tiles of LA_KEYS that these rows attend
+// to. The list is the same for every KV head. Units lie end to end on a line of costs on which a key tile takes 1 and
+// what a unit costs besides (its queries, its results) LA_UNIT_COST; the attention cuts that line into equal runs.
 constexpr int LA_ROWS = 128;
-constexpr int LA_KEYS = 64;
+constexpr int LA_KEYS = 128;
+constexpr int LA_UNIT_COST = 1;
 // Most rows of a KV head (T * group) whose prefix and own units may be apart: each row then keeps two fp32 partial
 // rows per KV head in the attention's workspace (136 MB at 4 KV heads of 128).
 constexpr int LA_APART_ROWS = 32768;
-struct LaUnit {
-  int line;   // the line, or -1: rows of all lines together against the prefix
-  int row0;   // first row: within the line's rows (token - cu[line]) * group + head, or within the pass's
-  int start;  // key tiles of the units before this one
-  int tiles;  // its key tiles (>= 1)
+struct __align__(16) LaUnit {
+  int line;     // the line, or -1: rows of all lines together against the prefix
+  int token0;   // its first token, of the pass
+  int rows;     // tokens * group
+  int at;       // its first key tile's place; its cost begins LA_UNIT_COST before
+  int tiles;    // its key tiles (>= 1)
+  int sees;     // own keys that its first token sees (0: prefix unit)
+  int own_end;  // own keys that its last token sees
+  int lead;     // key tiles of the prefix at its front
 };
-// work (int32): a header, kept [B], the first unit of each line [B], then (16-byte aligned) the units
+// work (int32): a header, the own unit of each token [T], then (16-byte aligned) the units
 enum {
   LW_TOGETHER = 0,  // 1: a line's unit covers the prefix and then its own keys; 0: prefix units, then own units
   LW_UNITS,         // units
-  LW_TILES,         // key tiles of all units (one KV head)
-  LW_PREFIX_UNITS,  // units of the prefix (LW_TOGETHER == 0)
+  LW_COST,          // cost of all units (one KV head)
   LW_PREFIX,        // prefix length
   LW_PREFIX_TILES,  // its key tiles
   LW_TOKENS,        // tokens placed (<= T)
@@ -52,9 +57,12 @@ enum {
   LW_T,
   LW_HEADER = 16
 };
-__host__ __device__ inline int la_unit_offset(int B) { return (LW_HEADER + 2 * B + 3) & ~3; }
+constexpr int LA_UNIT_INTS = sizeof(LaUnit) / 4;
+__host__ __device__ inline int la_tile_tokens(int group) { return LA_ROWS / group; }
+__host__ __device__ inline size_t la_unit_offset(int T) { return ((size_t)LW_HEADER + T + 3) & ~(size_t)3; }
 __host__ __device__ inline long long la_max_units(int B, int T, int group) {
-  return 2 * (((long long)T * group + LA_ROWS - 1) / LA_ROWS) + B;
+  const int tokens = la_tile_tokens(group);
+  return 2 * (((long long)T + tokens - 1) / tokens) + B;
 }
 
 struct LinesPlanArgs {
@@ -121,18 +129,14 @@ D3_DEV void lp_scan_lines(int B, int* out, long long most, long long* warp_sums,
 
 D3_DEV int lp_clamped(const int* p, int b) { return min(max(0, p[b]), LP_MAX_KEPT); }
 
-// Key tiles that rows [row0, row0 + LA_ROWS) of a line see among its own keys: up to the last of their tokens.
-D3_DEV int lp_own_tiles(int kept, int rows, int row0, int group) {
-  const int last = (min(row0 + LA_ROWS, rows) - 1) / group;
-  return (kept + last + LA_KEYS) / LA_KEYS;  // ceil((kept + last + 1) / LA_KEYS)
-}
-
 __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a) {
   extern __shared__ int lp_smem[];
   __shared__ long long warp_sums[LP_WARPS];
   int* cu = lp_smem;               // [B + 1] first token of each line, clipped to T
-  int* first = cu + a.B + 1;       // [B + 1] pages taken by the lines before; block 0: then its first unit
-  int* tiles_of = first + a.B + 1;  // [B + 1] block 0: key tiles of the line, then of the lines before
+  int* first = cu + a.B + 1;       // [B + 1] pages taken by the lines before
+  int* unit0 = first + a.B + 1;    // [B + 1] own units of the lines before
+  int* kept_of = unit0 + a.B + 1;  // [B] tokens that the line has
+  int* cost_of = kept_of + a.B;    // [B + 1] block 0: cost of the line's units, then of the lines before
   const int tid = threadIdx.x, B = a.B;
   grid_dependency_wait();
   allow_dependents();
@@ -141,22 +145,36 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
   const int prefix = a.prefix ? max(0, *a.prefix) : 0;
   lp_scan_lines(B, first, 0x7fffffffLL, warp_sums, [&](int b) {
     const int kept = lp_clamped(a.kept, b), p = a.page;
+    kept_of[b] = kept;
     return (kept + cu[b + 1] - cu[b] + p - 1) / p - (kept + p - 1) / p;
   });
+  const int G = a.group, tile = la_tile_tokens(G), tokens = cu[B];
+  lp_scan_lines(B, unit0, 0x7fffffffLL, warp_sums, [&](int b) { return (cu[b + 1] - cu[b] + tile - 1) / tile; });
+  const int own_units = unit0[B];
+  const int prefix_tiles = (prefix + LA_KEYS - 1) / LA_KEYS;
+  const int prefix_units = prefix > 0 ? (tokens + tile - 1) / tile : 0;
+  // The prefix is read once for the rows of all lines together, or by each line's units on the way to its own keys.
+  // Apart, the rows of short lines share tiles: a decode step of 16 lines x 8 heads needs one tile instead of 16. But
+  // each row's parts are then merged through memory, so lines that fill most of their own tiles go together.
+  const bool together = prefix_units == 0 || (long long)a.T * G > LA_APART_ROWS ||
+                        (long long)own_units * 4 <= (long long)prefix_units * 5;
+  const int lead = together ? prefix_tiles : 0;  // key tiles ahead of each own unit's own ones
+  const int u0 = together ? 0 : prefix_units;    // the first own unit
   if (blockIdx.x > 0) {
     // ---- tokens
     const int t0 = (blockIdx.x - 1) * LP_TOKENS, t1 = min(a.T, t0 + LP_TOKENS);
     for (int t = t0 + tid; t < t1; t += LP_THREADS) {
       int64_t slot = -1, position = 0;
-      int b = -1;
-      if (t < cu[B]) {
+      int b = -1, unit = -1;
+      if (t < tokens) {
         int lo = 0, hi = B;  // the last line with cu <= t has a token there
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
           if (cu[mid] <= t) lo = mid; else hi = mid;
         }
         b = lo;
-        const int kept = lp_clamped(a.kept, b);
+        const int kept = kept_of[b];
+        unit = u0 + unit0[b] + (t - cu[b]) / tile;
         const int s = kept + t - cu[b], j = s / a.page, off = s - j * a.page;
         const int have = (kept + a.page - 1) / a.page;
         int page = -1;
@@ -176,74 +194,62 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
       a.slots[t] = slot;
       a.positions[t] = position;
       a.line[t] = b;
+      a.work[LW_HEADER + t] = unit;
     }
     return;
   }
   // ---- block 0: the state after the pass, and the attention's work list
-  const int tokens = cu[B], G = a.group;
   int over = 0;
   for (int b = tid; b < B; b += LP_THREADS) {
-    const int kept = lp_clamped(a.kept, b), n = cu[b + 1] - cu[b];
+    const int kept = kept_of[b], n = cu[b + 1] - cu[b];
     over |= n < a.counts[b];
     a.cu[b] = cu[b];
     a.lengths[b] = kept + n;
-    a.work[LW_HEADER + b] = kept;
   }
   if (over) record_fault(FAULT_TOKENS);
   if (tid == 0) {
     a.cu[B] = tokens;
     *a.used_out = (int)min((long long)a.F, (long long)used + first[B]);
   }
-  __syncthreads();  // every read of first[] is done: it becomes the lines' first units
   const int warp = tid >> 5, lane = tid & 31;
-  lp_scan_lines(B, first, 0x7fffffffLL, warp_sums,
-                [&](int b) { return ((cu[b + 1] - cu[b]) * G + LA_ROWS - 1) / LA_ROWS; });
-  const int own_units = first[B];
-  const int prefix_tiles = (prefix + LA_KEYS - 1) / LA_KEYS;
-  const int prefix_units = prefix > 0 ? (int)(((long long)tokens * G + LA_ROWS - 1) / LA_ROWS) : 0;
-  // The prefix is read once for the rows of all lines together, or by each line's units on the way to its own keys.
-  // Apart, the rows of short lines share tiles: a decode step of 16 lines x 8 heads needs one tile instead of 16. But
-  // each row's parts are then merged through memory, so lines that fill most of their own tiles go together.
-  const bool together = prefix_units == 0 || (long long)a.T * G > LA_APART_ROWS ||
-                        (long long)own_units * 4 <= (long long)prefix_units * 5;
-  const int lead = together ? prefix_tiles : 0;  // key tiles ahead of each own unit's own ones
-  // each own unit's key tiles, a warp per line; the units' running sum restarts at each line and is based below
-  LaUnit* units = (LaUnit*)(a.work + la_unit_offset(B));
-  const int u0 = together ? 0 : prefix_units;
+  // each own unit's cost, a warp per line; the running sum restarts at each line and is based below
+  LaUnit* units = (LaUnit*)(a.work + la_unit_offset(a.T));
   for (int b = warp; b < B; b += LP_WARPS) {
-    const int rows = (cu[b + 1] - cu[b]) * G, n = first[b + 1] - first[b];
-    const int kept = lp_clamped(a.kept, b);
+    const int count = cu[b + 1] - cu[b], n = unit0[b + 1] - unit0[b];
+    const int kept = kept_of[b];
     int base = 0;
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + lane;
-      const int tiles = i < n ? lead + lp_own_tiles(kept, rows, LA_ROWS * i, G) : 0;
-      int incl = tiles;
+      const int from = i * tile, to = min(from + tile, count);  // its tokens within the line
+      const int tiles = i < n ? lead + (kept + to + LA_KEYS - 1) / LA_KEYS : 0;
+      const int cost = i < n ? tiles + LA_UNIT_COST : 0;
+      int incl = cost;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
-      if (i < n) units[u0 + first[b] + i] = LaUnit{b, LA_ROWS * i, base + incl - tiles, tiles};
+      if (i < n)
+        units[u0 + unit0[b] + i] = LaUnit{b, cu[b] + from, (to - from) * G, base + incl - tiles, tiles, kept + from + 1,
+                                          kept + to, lead};
       base += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) {
-      a.work[LW_HEADER + B + b] = u0 + first[b];
-      tiles_of[b] = base;
-    }
+    if (lane == 0) cost_of[b] = base;
   }
   __syncthreads();
   // in place: a thread's value is read into the scan before its own place is written
-  lp_scan_lines(B, tiles_of, 0x7fffffffLL, warp_sums, [&](int b) { return tiles_of[b]; });
-  const int own_tiles = tiles_of[B], shared_tiles = together ? 0 : prefix_units * prefix_tiles;
-  for (int u = tid; u < u0; u += LP_THREADS) units[u] = LaUnit{-1, LA_ROWS * u, u * prefix_tiles, prefix_tiles};
+  lp_scan_lines(B, cost_of, 0x7fffffffLL, warp_sums, [&](int b) { return cost_of[b]; });
+  const int shared_cost = together ? 0 : prefix_units * (prefix_tiles + LA_UNIT_COST);
+  for (int u = tid; u < u0; u += LP_THREADS)
+    units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G, u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST,
+                      prefix_tiles, 0, 0, prefix_tiles};
   for (int b = warp; b < B; b += LP_WARPS)
-    for (int i = first[b] + lane; i < first[b + 1]; i += 32) units[u0 + i].start += shared_tiles + tiles_of[b];
+    for (int i = unit0[b] + lane; i < unit0[b + 1]; i += 32) units[u0 + i].at += shared_cost + cost_of[b];
   if (tid == 0) {
     int* w = a.work;
     w[LW_TOGETHER] = together;
     w[LW_UNITS] = u0 + own_units;
-    w[LW_TILES] = shared_tiles + own_tiles;
-    w[LW_PREFIX_UNITS] = u0;
+    w[LW_COST] = shared_cost + cost_of[B];
     w[LW_PREFIX] = prefix;
     w[LW_PREFIX_TILES] = prefix_tiles;
     w[LW_TOKENS] = tokens;

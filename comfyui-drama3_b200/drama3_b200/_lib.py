@@ -67,7 +67,7 @@ SIGNATURES = {
     "d3_qk_norm_rope": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i, _f, _f, _p, _i, _i, _p, _i, _p, _i,
                              _p, _p, _p, _p, _p, _p, _i, _i, _p, _p]),
     "d3_lines_attention_workspace": (_sz, [_i, _i, _i, _i]),
-    "d3_lines_attention": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p, _p, _p, _i, _f,
+    "d3_lines_attention": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p, _i, _f,
                                 _p, _p, _p, _sz, _p]),
 }
 

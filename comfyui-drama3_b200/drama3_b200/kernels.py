@@ -648,7 +648,6 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
         check(lib().d3_lines_attention(_ptr(q), _strides(q, 2), ROW_TYPES[q.dtype], T, Hq, Hkv, D, _ptr(k_cache),
                                        _strides(k_cache, 3), _ptr(v_cache), _strides(v_cache, 3), pages, page,
                                        _ptr(plan.table), plan.table.shape[1], _ptr(prefix_table),
-                                       0 if prefix_table is None else prefix_table.shape[0], _ptr(plan.line), _ptr(plan.cu),
-                                       _ptr(plan.work), B, scale, _ptr(out), _ptr(sums), _ptr(ws), size, _stream(device)),
+                                       0 if prefix_table is None else prefix_table.shape[0], _ptr(plan.work), B, scale, _ptr(out), _ptr(sums), _ptr(ws), size, _stream(device)),
               "lines_attention")
     return (out, sums) if lse else out

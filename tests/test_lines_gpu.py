@@ -108,10 +108,10 @@ def test_plan_without_room(cuda):
         assert fault() == (32 if want["pages"] else 0) | (64 if want["tokens"] else 0)
 
 
-def units_of(p, B):
+def units_of(p):
     work = p.work.tolist()
-    at = (16 + 2 * B + 3) & ~3
-    return work, [tuple(work[at + 4 * u:at + 4 * u + 4]) for u in range(work[1])]
+    at = (16 + p.slots.shape[0] + 3) & ~3
+    return work, [tuple(work[at + 8 * u:at + 8 * u + 8]) for u in range(work[1])]
 
 
 @pytest.mark.parametrize("group", [1, 7, 8, 128])
@@ -121,28 +121,29 @@ def units_of(p, B):
 def test_work_list_covers_every_row_and_key(cuda, group, lengths, counts, prefix):
     table, free, used, tokens = lines_case(lengths, counts, 16, 2)
     _, p = run_plan(cuda, lengths, counts, table, free, used, 16, tokens, prefix, group=group)
-    work, units = units_of(p, len(lengths))
-    total = sum(counts)
-    assert work[4] == prefix and work[6] == total and work[7] == group
-    starts = 0
-    own, shared = {}, []
-    for line, row0, start, tiles in units:
-        assert start == starts and tiles >= 1
-        starts += tiles
-        if line < 0:
-            shared.append(row0)
-            assert tiles == -(-prefix // 64)
-        else:
-            own[line, row0] = tiles
-    assert starts == work[2]
-    lead = -(-prefix // 64) if work[0] else 0
-    want = {}
+    work, units = units_of(p)
+    total, tile = sum(counts), 128 // group
+    together = work[0] == 1
+    assert work[3] == prefix and work[5] == total and work[6] == group
+    keys, unit_cost = 128, 1  # of a key tile; what a unit costs besides its tiles
+    place, own, shared = 0, [], []
+    for line, token0, rows, at, tiles, sees, own_end, lead in units:
+        assert at == place + unit_cost and tiles >= 1
+        place = at + tiles
+        (own if line >= 0 else shared).append((line, token0, rows, tiles, sees, own_end, lead))
+    assert place == work[2]
+    key_tiles = -(-prefix // keys)
+    lead, want, first = key_tiles if together else 0, [], 0
     for b, (kept, n) in enumerate(zip(lengths, counts)):
-        for row0 in range(0, n * group, 128):
-            last = (min(row0 + 128, n * group) - 1) // group
-            want[b, row0] = lead + -(-(kept + last + 1) // 64)
+        for i in range(0, n, tile):
+            end = min(i + tile, n)
+            assert work[16 + first + i:16 + first + end] == [len(shared) + len(want)] * (end - i)
+            want.append((b, first + i, (end - i) * group, lead + -(-(kept + end) // keys), kept + i + 1, kept + end, lead))
+        first += n
     assert own == want
-    assert shared == ([] if work[0] or not prefix else list(range(0, total * group, 128)))
+    assert shared == ([] if together else [(-1, i, min(tile, total - i) * group, key_tiles, 0, 0, key_tiles)
+                                           for i in range(0, total, tile)])
+    assert together or prefix
 
 
 # ---- qk_norm_rope
