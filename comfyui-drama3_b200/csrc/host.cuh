@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <mutex>
 
 #include <cudaTypedefs.h>
@@ -59,6 +60,18 @@ template <class K>
 int allow_smem(K kernel, int bytes) {
   if (bytes <= 48 * 1024) return D3_OK;
   return cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+// The same, asked for once per device: `done` has a bit for each device on which it was.
+template <class K>
+int allow_smem_once(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (int st = cuda_status(cudaGetDevice(&dev))) return st;
+  const uint64_t bit = 1ull << (dev & 63);  // kMaxDevices
+  if (done.load(std::memory_order_relaxed) & bit) return D3_OK;
+  if (int st = allow_smem(kernel, bytes)) return st;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return D3_OK;
 }
 
 template <class K, class... Args>

@@ -63,42 +63,47 @@ bool attn_shape(int T, int Hq, int Hkv, int D) {
 }
 
 template <int D, bool F16>
-int attn_launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const d3::LaArgs& a, dim3 combine,
+int attn_launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const d3::LaArgs& a, int join_blocks,
                 cudaStream_t s) {
   constexpr int smem = d3::LaShape<D>::SMEM;
-  if (int st = allow_smem(d3::lines_attn_kernel<D, F16>, smem)) return st;
+  static std::atomic<uint64_t> done{0};
+  if (int st = allow_smem_once(d3::lines_attn_kernel<D, F16>, smem, done)) return st;
   if (int st = launch(d3::lines_attn_kernel<D, F16>, dim3(a.runs), dim3(d3::LA_THREADS), smem, s, true, qm, km, vm, a))
     return st;
-  return launch(d3::lines_combine_kernel<D, F16>, dim3(combine.x), dim3(d3::LC_WARPS * 32), 0, s, true, a, (int)combine.y);
+  return launch(d3::lines_join_kernel<D, F16>, dim3(join_blocks), dim3(d3::LJ_WARPS * 32), 0, s, true, a);
 }
 
-template <int TYPE, int LANES, int NV>
+template <int TYPE, int LANES>
 int rope_launch(const d3::QrArgs& a, int pairs, int blocks, cudaStream_t s) {
-  return pairs ? launch(d3::qk_rope_kernel<TYPE, LANES, NV, true>, dim3(blocks), dim3(d3::QR_WARPS * 32), 0, s, true, a)
-               : launch(d3::qk_rope_kernel<TYPE, LANES, NV, false>, dim3(blocks), dim3(d3::QR_WARPS * 32), 0, s, true, a);
+  const dim3 threads(d3::QR_WARPS * 32);
+  const size_t smem = (size_t)a.tokens * (a.rot / 2) * sizeof(float2);  // at most 4 x 256 x 8 bytes
+  return pairs ? launch(d3::qk_rope_kernel<TYPE, LANES, true>, dim3(blocks), threads, smem, s, true, a)
+               : launch(d3::qk_rope_kernel<TYPE, LANES, false>, dim3(blocks), threads, smem, s, true, a);
 }
 
 template <int TYPE>
 int rope_type(d3::QrArgs a, int pairs, bool vectors, const DeviceInfo& d, cudaStream_t s) {
   constexpr int VEC = TYPE == d3::QR_F32 ? 4 : 8;
-  const int heads = a.Hq + a.Hkv * (a.k_out ? 1 : 2), n = a.D / VEC;
-  const int lanes = n <= 8 ? 8 : n <= 16 ? 16 : 32;
-  // whole vectors need rows, strides and pointers of whole vectors and no pair split inside one; up to 64 of them
-  if (!vectors || a.D % VEC || n > 64 || (pairs ? a.rot : a.rot / 2) % VEC) {
-    const long long warps = (long long)a.T * heads;
+  const int slots = a.D / (2 * VEC);  // of two vectors: a lane each
+  const int lanes = slots <= 4 ? 4 : slots <= 8 ? 8 : slots <= 16 ? 16 : 32;
+  // vectors in twos need rows, strides and pointers of whole vectors, and turned columns and others in whole slots
+  if (!vectors || a.D % (2 * VEC) || slots > 32 || a.rot % (2 * VEC)) {
+    const long long warps = (long long)a.T * (a.Hq + a.Hkv * (a.k_out ? 1 : 2));
     return launch(d3::qk_rope_any_kernel<TYPE>, dim3((unsigned)((warps + d3::QR_WARPS - 1) / d3::QR_WARPS)),
                   dim3(d3::QR_WARPS * 32), 0, s, true, a, pairs);
   }
-  // warps per token: enough warps to fill the GPU (32 per SM) with few tokens, one per token with many
-  const int at_once = 32 / lanes, most = (heads + at_once - 1) / at_once;
-  const int want = (32 * d.sms + a.T - 1) / a.T;
-  a.share = want < 1 ? 1 : want < most ? want : most;
-  const int blocks = (int)(((long long)a.T * a.share + d3::QR_WARPS - 1) / d3::QR_WARPS);
-  if (n > 32) return rope_launch<TYPE, 32, 2>(a, pairs, blocks, s);
+  // a warp per token where that fills the GPU (16 warps per SM), several with fewer tokens
+  const int at_once = 32 / lanes, want = (16 * d.sms + a.T - 1) / a.T;
+  const int most = (a.Hq + at_once - 1) / at_once + (a.Hkv + at_once - 1) / at_once * (a.k_out ? 1 : 2);
+  a.share = want < most ? want : most;
+  a.tokens = a.share < d3::QR_WARPS ? d3::QR_WARPS / a.share : 1;
+  const int per = (a.share + d3::QR_WARPS - 1) / d3::QR_WARPS;
+  const int blocks = per > 1 ? a.T * per : (a.T + a.tokens - 1) / a.tokens;
   switch (lanes) {
-    case 8: return rope_launch<TYPE, 8, 1>(a, pairs, blocks, s);
-    case 16: return rope_launch<TYPE, 16, 1>(a, pairs, blocks, s);
-    default: return rope_launch<TYPE, 32, 1>(a, pairs, blocks, s);
+    case 4: return rope_launch<TYPE, 4>(a, pairs, blocks, s);
+    case 8: return rope_launch<TYPE, 8>(a, pairs, blocks, s);
+    case 16: return rope_launch<TYPE, 16>(a, pairs, blocks, s);
+    default: return rope_launch<TYPE, 32>(a, pairs, blocks, s);
   }
 }
 
@@ -131,7 +136,9 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
   DeviceInfo d;
   if (int st = device_info(&d)) return st;
   const int smem = 5 * (B + 1) * 4;
-  if (int st = allow_smem(d3::lines_plan_kernel, smem)) return st;
+  static std::atomic<uint64_t> done{0};
+  if (smem > 48 * 1024)
+    if (int st = allow_smem_once(d3::lines_plan_kernel, 5 * (d3::LP_MAX_LINES + 1) * 4, done)) return st;
   const d3::LinesPlanArgs a = {kept, counts, B, table, W, free_pages, F, used, prefix, page, T, group, slots, positions,
                                line, cu, lengths, used_out, work};
   return launch(d3::lines_plan_kernel, dim3(1 + (T + d3::LP_TOKENS - 1) / d3::LP_TOKENS), dim3(d3::LP_THREADS), smem,
@@ -169,7 +176,8 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
   a.axis = axes > 1 ? axis : nullptr;
   a.q_out = q_out, a.k_out = k_out, a.share = 1;
   const int64_t vec = 16 / size;
-  bool vectors = aligned(q, 16) && aligned(k, 16) && aligned(q_out, 16) && multiple(q_strides, 2, vec) &&
+  bool vectors = aligned(q, 16) && aligned(k, 16) && aligned(q_out, 16) && aligned(q_weight, 16) &&
+                 aligned(k_weight, 16) && multiple(q_strides, 2, vec) &&
                  multiple(k_strides, 2, vec);
   if (cache) {
     a.v = {v, v_strides[0], v_strides[1]};
@@ -236,17 +244,17 @@ int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T,
   const long long rows = d3::la_part_rows(a.runs, T, a.G, Hkv);
   a.part_o = (float4*)workspace;
   a.part_ml = (float2*)((float*)workspace + rows * D);
-  a.cuts = (int4*)(a.part_ml + rows);
-  // the joining kernel: a block per run and per 32 rows that may have parts; with few of the latter, a block per 32 of
-  // their columns
-  const long long groups = (long long)T * a.G <= d3::LA_APART_ROWS ? d3::la_apart_rows(T, a.G) / 32 * Hkv : 0;
-  const int column_blocks = groups > 0 && groups < 4 * d.sms ? D / 32 : 1;
-  const dim3 combine((unsigned)(groups * column_blocks > a.runs ? groups * column_blocks : a.runs), column_blocks);
+  a.joints = (int4*)(a.part_ml + rows);
+  a.units_most = (int)d3::la_max_units(B, T, a.G);
+  // the joining kernel: a block per run, or enough for a warp per 32 rows x 4 columns that may have parts
+  const long long tasks = (long long)T * a.G <= d3::LA_APART_ROWS ? d3::la_apart_rows(T, a.G) / 32 * Hkv * (D / 4) : 0;
+  const long long want = (tasks + d3::LJ_WARPS - 1) / d3::LJ_WARPS, most = 16ll * d.sms;
+  const int blocks = (int)(want < a.runs ? a.runs : want < most ? want : most);
   cudaStream_t s = (cudaStream_t)stream;
   switch (D) {
-    case 64: return f16 ? attn_launch<64, true>(qm, km, vm, a, combine, s) : attn_launch<64, false>(qm, km, vm, a, combine, s);
-    case 128: return f16 ? attn_launch<128, true>(qm, km, vm, a, combine, s) : attn_launch<128, false>(qm, km, vm, a, combine, s);
-    default: return f16 ? attn_launch<256, true>(qm, km, vm, a, combine, s) : attn_launch<256, false>(qm, km, vm, a, combine, s);
+    case 64: return f16 ? attn_launch<64, true>(qm, km, vm, a, blocks, s) : attn_launch<64, false>(qm, km, vm, a, blocks, s);
+    case 128: return f16 ? attn_launch<128, true>(qm, km, vm, a, blocks, s) : attn_launch<128, false>(qm, km, vm, a, blocks, s);
+    default: return f16 ? attn_launch<256, true>(qm, km, vm, a, blocks, s) : attn_launch<256, false>(qm, km, vm, a, blocks, s);
   }
 }
 

@@ -8,7 +8,7 @@
 // A unit (lines_plan.cuh) is a tile of up to 128 rows (whole tokens x the query heads of a KV head) and its key tiles
 // of 128. The units of all KV heads, laid end to end by what they cost, are cut into equal runs, one per CTA: every CTA
 // has the same work whatever the lengths are. A run crosses units; a unit cut by a run's end leaves parts, which
-// lines_combine_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
+// lines_join_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
 // key is read once for all lines.
 //
 // Per CTA (320 threads; two CTAs per SM for heads of 64 and 128, so that one's products run under the other's
@@ -30,6 +30,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "f32x2.cuh"
 #include "lines_plan.cuh"
 #include "tcgen05.cuh"
 
@@ -39,15 +40,8 @@ constexpr int LA_THREADS = 320;
 constexpr int LA_ROW_WARP = 2;        // first of the eight row warps
 constexpr int LA_ROW_WARPS = 8;
 constexpr int LA_STAGE = LA_KEYS * 128;  // 64 columns of a K or V tile
-constexpr int LA_MIN_RUN = 3;         // shortest run (in costs) worth a CTA
+constexpr int LA_MIN_RUN = 2;         // shortest run (in costs) worth a CTA
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
-
-// Shared memory besides the operands: barriers, the row threads' exchange, and the row warps' copies of plan and walk
-// (which they need only between pieces: kept in registers they were spilled inside the loop over tiles).
-// 1 KB in all: two CTAs of heads of 128 fill an SM's shared memory to the byte.
-constexpr int LA_EXCHANGE = 192, LA_PLAN_AT = LA_EXCHANGE + LA_ROWS * 4, LA_WALK_AT = LA_PLAN_AT + 64;
-constexpr int LA_WALK_BYTES = 32, LA_SMALL = LA_WALK_AT + LA_ROW_WARPS * LA_WALK_BYTES;
-static_assert(LA_SMALL <= 1024, "two CTAs per SM");
 
 template <int D>
 struct LaShape {
@@ -57,7 +51,15 @@ struct LaShape {
   static constexpr int STAGES = D == 256 ? 10 : D == 128 ? 5 : 6;
   static constexpr int S_BUFS = D == 256 ? 2 : 1;
   static constexpr int TMEM_COLS = D == 256 ? 512 : 256;  // O: D columns, then S_BUFS x 128
-  static constexpr int SMEM = Q_BYTES + STAGES * LA_STAGE + LA_SMALL;
+  // Shared memory besides the operands: barriers and the tensor-memory address, the row threads' exchange, and the row
+  // warps' copies of plan and walk (which they need only between pieces: kept in registers they were spilled
+  // inside the loop over tiles). 1 KB in all for heads of 128, two of whose CTAs fill an SM's shared memory to the byte.
+  static constexpr int BARRIERS = 2 * STAGES + 10;
+  static constexpr int EXCHANGE_AT = (BARRIERS * 8 + 4 + 63) / 64 * 64, PLAN_AT = EXCHANGE_AT + LA_ROWS * 4;
+  static constexpr int WALK_AT = PLAN_AT + 64, WALK_BYTES = 32;
+  static constexpr int SMALL = WALK_AT + LA_ROW_WARPS * WALK_BYTES;
+  static constexpr int SMEM = Q_BYTES + STAGES * LA_STAGE + SMALL;
+  static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024 && SMEM <= 227 * 1024, "the CTAs of an SM fit it");
 };
 
 struct LaArgs {
@@ -74,8 +76,9 @@ struct LaArgs {
   float* lse;        // [T, Hq] or null
   float4* part_o;    // partial rows, not divided: four columns of 32 rows together, see la_part_at
   float2* part_ml;   // their (maximum * scale_log2, sum)
-  int4* cuts;        // per run: the unit whose first cut is this run's start (token0, rows, head, last run), or rows 0
-  int runs;          // CTAs of the attention kernel
+  int4* joints;      // [runs] the unit that is first cut at this run's start: token0, rows, head, last run; or rows 0
+  int units_most;    // units that the plan has room for
+  int runs;          // CTAs
 };
 
 // Partial rows: LA_ROWS for the part that a run starts in the middle of a unit, LA_ROWS for the part that it leaves
@@ -103,8 +106,12 @@ struct LaPlan {
   int units_n, cost, prefix, prefix_tiles, tokens;
   bool fits;
   int per, total;  // of all KV heads; a plan of 2^30 or more is refused
+  int runs;        // with something to do
   const LaUnit* units;
-  D3_DEV explicit LaPlan(const LaArgs& a) {
+  D3_DEV LaPlan(const LaArgs& a, int& probe) {
+    units = (const LaUnit*)(a.work + la_unit_offset(a.T));
+    // a first probe for find, on its way with the header: where the first 32 units begin
+    probe = __ldg(&units[min((int)threadIdx.x & 31, a.units_most - 1)].at) - LA_UNIT_COST;
     const int4 x = __ldg((const int4*)a.work), y = __ldg((const int4*)a.work + 1);
     const int T = __ldg(a.work + LW_T);
     together = x.x != 0;
@@ -117,15 +124,16 @@ struct LaPlan {
     fits = y.z == a.G && y.w == a.B && T == a.T && all < 0x40000000;
     total = fits ? (int)all : 0;
     per = max((int)((unsigned)(total + a.runs - 1) / (unsigned)a.runs), LA_MIN_RUN);
-    units = (const LaUnit*)(a.work + la_unit_offset(a.T));
+    runs = (unsigned)(total + per - 1) / (unsigned)per;
   }
   D3_DEV LaUnit unit(int u) const {
     const int4 x = __ldg((const int4*)(units + u)), y = __ldg((const int4*)(units + u) + 1);
     return LaUnit{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   }
   // The last unit that begins at or before `place`, by the whole warp: 32 probes a round.
-  D3_DEV int find(int place) const {
+  D3_DEV int find(int place, int probe) const {
     const int lane = threadIdx.x & 31;
+    if (units_n <= 32) return __popc(__ballot_sync(0xffffffffu, lane < units_n && probe <= place)) - 1;
     int lo = 0, n = units_n;  // the answer is in [lo, lo + n)
     while (n > 1) {
       const int step = (n + 31) / 32;
@@ -147,13 +155,13 @@ struct LaWalk {
   int j0, n;     // the piece: tiles [j0, j0 + n) of unit u
   int tiles;     // of the unit
 
-  D3_DEV LaWalk(const LaArgs& a, const LaPlan& p, int run) {
+  D3_DEV LaWalk(const LaPlan& p, int run, int probe) {
     pos = p.per * run;
     end = p.fits ? min(pos + p.per, p.total) : 0;
     if (pos < end) {
       h = (unsigned)pos / (unsigned)p.cost;
       head0 = h * p.cost;
-      u = p.find(pos - head0);
+      u = p.find(pos - head0, probe);
     }
   }
   D3_DEV bool next(const LaPlan& p, LaUnit& unit) {
@@ -328,29 +336,6 @@ D3_DEV float la_max3(float a, float b, float c) {
   return r;
 }
 
-// Two 32-bit floats in a register pair, and arithmetic on both at once.
-D3_DEV uint64_t la_two(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-D3_DEV void la_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-D3_DEV uint64_t la_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-D3_DEV uint64_t la_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-D3_DEV uint64_t la_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // 2^x of two numbers without the special-function unit, which takes 16 a cycle of an SM where a tile of 128 x 128 scores
 // wants them as fast as its products: x = n + f with n the nearest whole number (by adding 1.5 x 2^23 + 127, which leaves
 // n + 127 in the low bits), 2^f on [-1/2, 1/2] by the polynomial of degree 4 whose largest relative error, 2.6e-6, is
@@ -358,21 +343,21 @@ D3_DEV uint64_t la_mul2(uint64_t a, uint64_t b) {
 // Below -126: 2^-126. A NaN stays one.
 D3_DEV void la_exp2_poly(uint64_t x, float& lo, float& hi) {
   float x0, x1;
-  la_split(x, x0, x1);
+  f2_split(x, x0, x1);
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
-  x = la_two(x0, x1);
+  x = f2_make(x0, x1);
   const float magic = 12582912.0f + 127.0f;
-  const uint64_t t = la_add2(x, la_two(magic, magic));
-  const uint64_t f = la_fma2(la_add2(t, la_two(-magic, -magic)), la_two(-1.0f, -1.0f), x);
-  uint64_t p = la_fma2(f, la_two(0.009570068679749966f, 0.009570068679749966f), la_two(0.055917806923389435f, 0.055917806923389435f));
-  p = la_fma2(p, f, la_two(0.240247443318367f, 0.240247443318367f));
-  p = la_fma2(p, f, la_two(0.6931218504905701f, 0.6931218504905701f));
-  p = la_fma2(p, f, la_two(0.9999992847442627f, 0.9999992847442627f));
+  const uint64_t t = f2_add(x, f2_make(magic, magic));
+  const uint64_t f = f2_fma(f2_add(t, f2_make(-magic, -magic)), f2_make(-1.0f, -1.0f), x);
+  uint64_t p = f2_fma(f, f2_make(0.009570068679749966f, 0.009570068679749966f), f2_make(0.055917806923389435f, 0.055917806923389435f));
+  p = f2_fma(p, f, f2_make(0.240247443318367f, 0.240247443318367f));
+  p = f2_fma(p, f, f2_make(0.6931218504905701f, 0.6931218504905701f));
+  p = f2_fma(p, f, f2_make(0.9999992847442627f, 0.9999992847442627f));
   float t0, t1;
-  la_split(t, t0, t1);
-  p = la_mul2(p, la_two(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
-  la_split(p, lo, hi);
+  f2_split(t, t0, t1);
+  p = f2_mul(p, f2_make(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23)));
+  f2_split(p, lo, hi);
 }
 
 template <bool F16>
@@ -398,9 +383,9 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   uint8_t* ring = la_smem + S::Q_BYTES;
   uint64_t* bars = (uint64_t*)(la_smem + S::Q_BYTES + S::STAGES * LA_STAGE);
   uint8_t* small = (uint8_t*)bars;
-  LaPlan* plan_s = (LaPlan*)(small + LA_PLAN_AT);
-  LaWalk* walk_s = (LaWalk*)(small + LA_WALK_AT) + (threadIdx.x >> 5) - LA_ROW_WARP;
-  static_assert(sizeof(LaPlan) <= LA_WALK_AT - LA_PLAN_AT && sizeof(LaWalk) == LA_WALK_BYTES, "layout");
+  LaPlan* plan_s = (LaPlan*)(small + S::PLAN_AT);
+  LaWalk* walk_s = (LaWalk*)(small + S::WALK_AT) + (threadIdx.x >> 5) - LA_ROW_WARP;
+  static_assert(sizeof(LaPlan) <= 64 && sizeof(LaWalk) == S::WALK_BYTES, "layout");
   uint64_t* kv_full = bars;                    // [STAGES]
   uint64_t* kv_empty = kv_full + S::STAGES;    // [STAGES]
   uint64_t* q_full = kv_empty + S::STAGES;
@@ -437,12 +422,13 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem, tmem_s = tmem + D;  // S buffer b: columns D + 128 b;
   // P of its keys 32 j .. 32 j + 31 in the first 16 columns of theirs
-  LaPlan plan(a);
+  int probe;
+  LaPlan plan(a, probe);
   if (!plan.fits || !aligned) {
     plan.fits = false;
     if (tid == 0) record_fault(FAULT_PLAN);
   }
-  LaWalk w(a, plan, run);
+  LaWalk w(plan, run, probe);
 
   if (warp == 0) {
     // ---- loads: a piece's Q, then K0, V0, K1, V1, ... (two S buffers: K0, K1, V0, K2, V1, ...)
@@ -585,16 +571,19 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const int row = 32 * quarter + lane, tok = row / a.G, g = row - tok * a.G;
     if (lane == 0) {
-      if (warp == LA_ROW_WARP) *plan_s = plan;
+      if (warp == LA_ROW_WARP) {
+        *plan_s = plan;
+        a.joints[run] = make_int4(0, 0, 0, 0);
+      }
       *walk_s = w;
     }
     named_sync(9, 32 * LA_ROW_WARPS);
     // between a row's two threads: their maxima (as bfloat16, rounded to nearest: any number near the maximum serves,
     // if both take the same), or a sum
-    uint16_t* maxima = (uint16_t*)(small + LA_EXCHANGE) + 2 * row;
-    float* total = (float*)(small + LA_EXCHANGE) + row;
+    uint16_t* maxima = (uint16_t*)(small + S::EXCHANGE_AT) + 2 * row;
+    float* total = (float*)(small + S::EXCHANGE_AT) + row;
     uint32_t seq = 0, tiles = 0;
-    bool ok = true, cut = false;
+    bool ok = true;
     while (ok) {
       int n, n_shared;  // tiles of the piece, and those of them that are the prefix's
       // keys that there are, from the piece's first tile on: of the prefix, of the line, of these that this row sees
@@ -692,22 +681,22 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
             }
           }
           const float base = m == -INFINITY ? 0.0f : m;
-          const uint64_t scale2 = la_two(a.scale_log2, a.scale_log2), base2 = la_two(-base, -base);
+          const uint64_t scale2 = f2_make(a.scale_log2, a.scale_log2), base2 = f2_make(-base, -base);
           uint64_t sums[2] = {0, 0};
           auto weigh = [&](int c, auto limited) {
             uint32_t p[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              const uint64_t y = la_fma2(la_two(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, base2);
+              const uint64_t y = f2_fma(f2_make(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, base2);
               float p0, p1;
               if (!decltype(limited)::value && x / 2 % 4 == 1) {  // a pair in four
                 la_exp2_poly(y, p0, p1);
               } else {
-                la_split(y, p0, p1);
+                f2_split(y, p0, p1);
                 p0 = la_exp2(p0);
                 p1 = la_exp2(p1);
               }
-              sums[x / 2 & 1] = la_add2(sums[x / 2 & 1], la_two(p0, p1));
+              sums[x / 2 & 1] = f2_add(sums[x / 2 & 1], f2_make(p0, p1));
               p[x / 2] = la_pack<F16>(p0, p1);
             }
             tmem_st16(s_at + c, p);
@@ -727,7 +716,7 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
           else
             weights(LaWhole{});
           float s0, s1;
-          la_split(la_add2(sums[0], sums[1]), s0, s1);
+          f2_split(f2_add(sums[0], sums[1]), s0, s1);
           l += s0 + s1;
         } else if (lane == 0) {
           mbar_arrive(p_full + 2 * buf);
@@ -759,14 +748,11 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
         part += la_part_apart(a, unit.line >= 0, w.h) + (long long)unit.token0 * a.G;
       else
         part += la_part_open(a, run);
-      if (!first && plan.together) {
-        // a unit's first cut, at this run's start, has it joined
+      if (!first && plan.together && tid == 32 * LA_ROW_WARP) {
+        // a unit's first cut: it is joined under this run's number
         const int from = w.head0 + unit.at;
-        if (from / plan.per == run - 1) {
-          cut = true;
-          if (tid == 32 * LA_ROW_WARP)
-            a.cuts[run] = make_int4(unit.token0, unit.rows, w.h, (from + unit.tiles - 1) / plan.per);
-        }
+        if (from / plan.per == run - 1)
+          a.joints[run] = make_int4(unit.token0, unit.rows, w.h, (from + unit.tiles - 1) / plan.per);
       }
       if (any) {
         const int t = unit.token0 + tok, head = w.h * a.G + g;
@@ -805,7 +791,6 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
       if (lane == 0) *walk_s = w;
       __syncwarp();
     }
-    if (tid == 32 * LA_ROW_WARP && !cut) a.cuts[run] = make_int4(0, 0, 0, 0);
     // tokens of no line: nothing to see
     if (plan.fits) {
       const long long total = (long long)(a.T - plan.tokens) * a.Hq;
@@ -826,104 +811,129 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   }
 }
 
-// Joins the parts of a row: with M the largest of their maxima, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, the
-// parts taken in order. A lane is a row (of 32 neighbouring ones of a KV head); a warp takes groups of four columns.
-// Bound by latency: LC_AHEAD parts are in flight at a time.
-constexpr int LC_WARPS = 8;
-constexpr int LC_AHEAD = 8;
+// The joining: with M the largest of a row's parts' maxima, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, the parts
+// taken in order. A lane is a row (of 32 neighbouring ones of a KV head), a warp takes groups of four columns. Bound
+// by latency: N x AHEAD loads are in flight at a time. (A barrier of all CTAs inside the attention kernel took as long
+// as the step to a second kernel, and needs all of them on the GPU together, which two CTAs of ten warps an SM do not
+// promise.)
+// The parts of a row: `first`, then those that the runs r0 + 1 .. r1 left at `rest` rows into theirs.
+struct LaParts {
+  long long first;
+  int rest, r0, r1;
+};
+
+// Columns 4c .. 4c + 4N - 1 of a row whose parts are p's, then q's.
+template <int D, bool F16, int N, int AHEAD>
+D3_DEV void la_join_row(const LaArgs& a, int c, bool live, const LaParts& p, const LaParts& q, int t, int head) {
+  const int np = live ? p.r1 - p.r0 + 1 : 0, n = live ? np + q.r1 - q.r0 + 1 : 0;
+  const int longest = __reduce_max_sync(0xffffffffu, n);
+  float M = -INFINITY, L = 0.0f;
+  float4 o[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int i0 = 0; i0 < longest; i0 += AHEAD) {
+    float2 ml[AHEAD];
+    float4 v[AHEAD][N];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = i0 + j;
+      ml[j] = make_float2(-INFINITY, 0.0f);
+      if (i < n) {
+        const long long r = i < np ? (i == 0 ? p.first : la_part_rest(p.r0 + i) + p.rest)
+                                   : (i == np ? q.first : la_part_rest(q.r0 + i - np) + q.rest);
+        ml[j] = a.part_ml[r];
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[j][k] = a.part_o[la_part_at<D>(r, c + k)];
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) top = fmaxf(top, ml[j].x);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float f = la_exp2(M - base);  // 0 at first
+    L *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o[k].x *= f, o[k].y *= f, o[k].z *= f, o[k].w *= f;
+    M = top;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (ml[j].y == 0.0f) continue;  // nothing there (a NaN stays one)
+      const float g = la_exp2(ml[j].x - base);
+      L = fmaf(g, ml[j].y, L);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        o[k].x = fmaf(g, v[j][k].x, o[k].x);
+        o[k].y = fmaf(g, v[j][k].y, o[k].y);
+        o[k].z = fmaf(g, v[j][k].z, o[k].z);
+        o[k].w = fmaf(g, v[j][k].w, o[k].w);
+      }
+    }
+  }
+  if (live) {
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const long long r = (long long)t * a.Hq + head;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      ((uint2*)a.out)[r * (D / 4) + c + k] =
+          make_uint2(la_pack<F16>(o[k].x * inv, o[k].y * inv), la_pack<F16>(o[k].z * inv, o[k].w * inv));
+    if (a.lse && c == 0) a.lse[r] = (M + log2f(L)) * 0.69314718055994531f;
+  }
+}
+
+constexpr int LJ_WARPS = 8;
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(LC_WARPS * 32) lines_combine_kernel(LaArgs a, int column_blocks) {
+__global__ void __launch_bounds__(LJ_WARPS * 32) lines_join_kernel(LaArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = (int)(la_apart_rows(a.T, a.G) / 32), tasks = groups * a.Hkv * (D / 4);
+  // task x, prefix and own units apart: 32 rows of a KV head x 4 columns
+  auto row_of = [&](int x, int& h, int& packed) {
+    const int y = x / (D / 4);
+    h = y / groups;
+    packed = (y - h * groups) * 32 + lane;
+    return packed / a.G;
+  };
+  int x = blockIdx.x * LJ_WARPS + warp, h, packed;
   grid_dependency_wait();
   allow_dependents();
-  const LaPlan plan(a);
+  // the first task's own unit on its way with the header
+  int t = row_of(min(x, tasks - 1), h, packed), own_unit = t < a.T ? __ldg(a.work + LW_HEADER + t) : -1;
+  int probe;
+  const LaPlan plan(a, probe);
   if (!plan.fits) return;
-
-  // the parts of a row: `first`, then those that the runs r0 + 1 .. r1 left at `rest` rows into theirs; and, prefix and
-  // own units apart, the same again for its own unit
-  struct Parts {
-    long long first;
-    int rest, r0, r1;
-  };
-  auto join = [&](int c, bool live, const Parts& p, const Parts& q, int t, int head) {
-    const int np = live ? p.r1 - p.r0 + 1 : 0, n = live ? np + q.r1 - q.r0 + 1 : 0;
-    const int longest = __reduce_max_sync(0xffffffffu, n);
-    float M = -INFINITY, L = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < longest; i0 += LC_AHEAD) {
-      float2 ml[LC_AHEAD];
-      float4 v[LC_AHEAD];
-#pragma unroll
-      for (int j = 0; j < LC_AHEAD; ++j) {
-        const int i = i0 + j;
-        ml[j] = make_float2(-INFINITY, 0.0f);
-        if (i < n) {
-          const long long r = i < np ? (i == 0 ? p.first : la_part_rest(p.r0 + i) + p.rest)
-                                     : (i == np ? q.first : la_part_rest(q.r0 + i - np) + q.rest);
-          ml[j] = a.part_ml[r];
-          v[j] = a.part_o[la_part_at<D>(r, c)];
-        }
-      }
-      float top = M;
-#pragma unroll
-      for (int j = 0; j < LC_AHEAD; ++j) top = fmaxf(top, ml[j].x);
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float f = la_exp2(M - base);  // 0 at first
-      L *= f;
-      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-      M = top;
-#pragma unroll
-      for (int j = 0; j < LC_AHEAD; ++j) {
-        if (ml[j].y == 0.0f) continue;  // nothing there (a NaN stays one)
-        const float g = la_exp2(ml[j].x - base);
-        L = fmaf(g, ml[j].y, L);
-        o.x = fmaf(g, v[j].x, o.x);
-        o.y = fmaf(g, v[j].y, o.y);
-        o.z = fmaf(g, v[j].z, o.z);
-        o.w = fmaf(g, v[j].w, o.w);
-      }
-    }
-    if (live) {
-      const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-      const long long r = (long long)t * a.Hq + head;
-      ((uint2*)a.out)[r * (D / 4) + c] =
-          make_uint2(la_pack<F16>(o.x * inv, o.y * inv), la_pack<F16>(o.z * inv, o.w * inv));
-      if (a.lse && c == 0) a.lse[r] = (M + log2f(L)) * 0.69314718055994531f;
-    }
-  };
-
   if (plan.together) {
-    // the units that a run's end cuts: a block each, a warp 32 rows and half of the columns
-    for (int run = blockIdx.x; run < a.runs; run += gridDim.x) {
-      const int4 cut = a.cuts[run];
-      const int row = (warp & 3) * 32 + lane;
-      if (cut.y <= row - lane) continue;
-      const int tok = row / a.G;
-      for (int c = warp >> 2; c < D / 4; c += LC_WARPS / 4)
-        join(c, row < cut.y, Parts{la_part_open(a, run - 1) + row, row, run - 1, cut.w}, Parts{0, 0, 0, -1}, cut.x + tok,
-             cut.z * a.G + row - tok * a.G);
+    // the unit that is first cut at a run's start, 32 rows x 16 columns a warp at a time (two or three parts, as a rule),
+    // by as many blocks as there are
+    const int split = max(1, (int)gridDim.x / max(1, plan.runs));
+    for (int y = blockIdx.x; y < plan.runs * split; y += gridDim.x) {
+      const int run = y / split;
+      const int4 joint = a.joints[run];
+      const int count = (joint.y + 31) / 32 * (D / 16);
+      for (int z = (y - run * split) * LJ_WARPS + warp; z < count; z += split * LJ_WARPS) {
+        const int row = z / (D / 16) * 32 + lane, tok = row / a.G;
+        la_join_row<D, F16, 4, 4>(a, z % (D / 16) * 4, row < joint.y,
+                                  LaParts{la_part_open(a, run - 1) + row, row, run - 1, joint.w}, LaParts{0, 0, 0, -1},
+                                  joint.x + tok, joint.z * a.G + row - tok * a.G);
+      }
     }
     return;
   }
-  const int groups = (int)(la_apart_rows(a.T, a.G) / 32), columns = D / 4 / column_blocks;
-  for (int x = blockIdx.x; x < groups * a.Hkv * column_blocks; x += gridDim.x) {
-    const int y = x / column_blocks, h = y / groups, packed = (y - h * groups) * 32 + lane;
-    const int t = packed / a.G;
+  for (; x < tasks; x += gridDim.x * LJ_WARPS, t = row_of(min(x, tasks - 1), h, packed),
+                    own_unit = t < a.T ? __ldg(a.work + LW_HEADER + t) : -1) {
     const bool live = t < plan.tokens;
-    Parts p[2] = {};
+    LaParts p[2] = {};
     if (live) {
-      const int units[2] = {t / la_tile_tokens(a.G), __ldg(a.work + LW_HEADER + t)};  // prefix unit, own unit
+      const int units[2] = {t / la_tile_tokens(a.G), own_unit};  // its prefix unit, its own
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const LaUnit u = plan.unit(units[i]);
         const int from = h * plan.cost + u.at;
-        p[i] = Parts{la_part_apart(a, i == 1, h) + packed, packed - u.token0 * a.G, from / plan.per,
-                     (from + u.tiles - 1) / plan.per};
+        p[i] = LaParts{la_part_apart(a, i == 1, h) + packed, packed - u.token0 * a.G, from / plan.per,
+                       (from + u.tiles - 1) / plan.per};
       }
     }
-    const int c0 = (x - y * column_blocks) * columns;
-    for (int c = c0 + warp; c < c0 + columns; c += LC_WARPS) join(c, live, p[0], p[1], t, h * a.G + packed - t * a.G);
+    la_join_row<D, F16, 1, 8>(a, x % (D / 4), live, p[0], p[1], t, h * a.G + packed - t * a.G);
   }
 }
 

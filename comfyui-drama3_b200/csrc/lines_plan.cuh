@@ -212,39 +212,48 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
     *a.used_out = (int)min((long long)a.F, (long long)used + first[B]);
   }
   const int warp = tid >> 5, lane = tid & 31;
-  // each own unit's cost, a warp per line; the running sum restarts at each line and is based below
+  // The own units, a warp per line: first what each line costs, then, with the lines' costs summed up, the units
+  // themselves. (Written at once and moved to their places afterwards, each unit of a line waited for memory twice.)
   LaUnit* units = (LaUnit*)(a.work + la_unit_offset(a.T));
+  auto cost_at = [&](int b, int i, int n, int count, int& from, int& to) {  // of unit i of line b, its tokens
+    from = i * tile;
+    to = min(from + tile, count);
+    return i < n ? lead + (kept_of[b] + to + LA_KEYS - 1) / LA_KEYS + LA_UNIT_COST : 0;
+  };
   for (int b = warp; b < B; b += LP_WARPS) {
     const int count = cu[b + 1] - cu[b], n = unit0[b + 1] - unit0[b];
-    const int kept = kept_of[b];
-    int base = 0;
+    int sum = 0, from, to;
+    for (int i = lane; i < n; i += 32) sum += cost_at(b, i, n, count, from, to);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) cost_of[b] = sum;
+  }
+  __syncthreads();
+  // in place: a thread's value is read into the scan before its own place is written
+  lp_scan_lines(B, cost_of, 0x7fffffffLL, warp_sums, [&](int b) { return cost_of[b]; });
+  const int shared_cost = together ? 0 : prefix_units * (prefix_tiles + LA_UNIT_COST);
+  for (int b = warp; b < B; b += LP_WARPS) {
+    const int count = cu[b + 1] - cu[b], n = unit0[b + 1] - unit0[b];
+    int base = shared_cost + cost_of[b];
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + lane;
-      const int from = i * tile, to = min(from + tile, count);  // its tokens within the line
-      const int tiles = i < n ? lead + (kept + to + LA_KEYS - 1) / LA_KEYS : 0;
-      const int cost = i < n ? tiles + LA_UNIT_COST : 0;
+      int from, to;
+      const int cost = cost_at(b, i, n, count, from, to);
       int incl = cost;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
+      const int tiles = cost - LA_UNIT_COST;
       if (i < n)
-        units[u0 + unit0[b] + i] = LaUnit{b, cu[b] + from, (to - from) * G, base + incl - tiles, tiles, kept + from + 1,
-                                          kept + to, lead};
+        units[u0 + unit0[b] + i] = LaUnit{b, cu[b] + from, (to - from) * G, base + incl - tiles, tiles,
+                                          kept_of[b] + from + 1, kept_of[b] + to, lead};
       base += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) cost_of[b] = base;
   }
-  __syncthreads();
-  // in place: a thread's value is read into the scan before its own place is written
-  lp_scan_lines(B, cost_of, 0x7fffffffLL, warp_sums, [&](int b) { return cost_of[b]; });
-  const int shared_cost = together ? 0 : prefix_units * (prefix_tiles + LA_UNIT_COST);
   for (int u = tid; u < u0; u += LP_THREADS)
     units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G, u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST,
                       prefix_tiles, 0, 0, prefix_tiles};
-  for (int b = warp; b < B; b += LP_WARPS)
-    for (int i = unit0[b] + lane; i < unit0[b + 1]; i += 32) units[u0 + i].at += shared_cost + cost_of[b];
   if (tid == 0) {
     int* w = a.work;
     w[LW_TOGETHER] = together;

@@ -7,21 +7,25 @@
 // names the one that turns pair f.
 // q goes to a fresh tensor; k to one too, or, with the rows of v, to their slots of a paged cache.
 //
-// Bound by memory: each row is read once and written once. A warp owns a token (or, where the tokens are too few to
-// fill the GPU, a share of its heads) and walks its heads with the same cosines and sines in registers: a lane holds
-// 16 bytes of a head (8 columns of 16 bits), a head of 128 takes 16 lanes, so a warp takes two heads at a time, and
-// four such loads are in flight before the first is used.
+// Bound by memory: each row is read once and written once. A lane holds two 16-byte vectors of a head: the ones that turn
+// with one another (columns 8i .. and rot/2 + 8i ..), so that the rotation stays within the lane; a head of 128 takes 8
+// lanes and a warp four heads at a time, with QR_AHEAD such loads in flight. A warp owns a token, or, where the tokens are
+// too few to fill the GPU, a share of its heads. The token's cosines and sines are looked up into shared memory (axis,
+// position and table are three loads that wait for one another), then the warp takes its queries, keys and values in
+// turn, with the weights in registers. 16 warps an SM of 128 registers; 24 of 80 spilled and took a quarter longer.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace d3 {
 
 enum { QR_BF16 = 0, QR_F16 = 1, QR_F32 = 2 };
-constexpr int QR_WARPS = 8;
+constexpr int QR_WARPS = 4;
+constexpr int QR_AHEAD = 2;
 constexpr int QR_MAX_AXES = 4;
 constexpr int QR_MAX_D = 1024;
 
@@ -52,17 +56,36 @@ struct QrArgs {
   const int64_t* slots;  // [T]
   int page;
   long long slot_count;
-  int share;  // warps per token
+  int share;   // warps per token
+  int tokens;  // tokens per block (1 where a token's warps fill more than one)
 };
 
 template <int TYPE> struct QrType;
 template <> struct QrType<QR_BF16> {
   using T = uint16_t;
+  static D3_DEV void get2(uint32_t w, float& lo, float& hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
+  static D3_DEV uint32_t put2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
   static D3_DEV float get(uint16_t v) { return bf16_to_f32(v); }
   static D3_DEV uint16_t put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 };
 template <> struct QrType<QR_F16> {
   using T = uint16_t;
+  static D3_DEV void get2(uint32_t w, float& lo, float& hi) {
+    lo = h_lo(w);
+    hi = h_hi(w);
+  }
+  static D3_DEV uint32_t put2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
   static D3_DEV float get(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static D3_DEV uint16_t put(float v) { return __half_as_ushort(__float2half_rn(v)); }
 };
@@ -72,9 +95,54 @@ template <> struct QrType<QR_F32> {
   static D3_DEV float put(float v) { return v; }
 };
 
+// The values of a 16-byte vector, and back (rounded to nearest).
+template <int TYPE, int VEC>
+D3_DEV void qr_unpack(const uint32_t* w, float* x) {
+  if constexpr (TYPE == QR_F32) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = __uint_as_float(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) QrType<TYPE>::get2(w[e / 2], x[e], x[e + 1]);
+  }
+}
+template <int TYPE, int VEC>
+D3_DEV void qr_pack(const float* y, uint32_t* w) {
+  if constexpr (TYPE == QR_F32) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) w[e] = __float_as_uint(y[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) w[e / 2] = QrType<TYPE>::put2(y[e], y[e + 1]);
+  }
+}
+
 template <int TYPE> D3_DEV float qr_weight(const void* w, bool f32, float add, int d) {
   if (!w) return 1.0f;
   return (f32 ? ((const float*)w)[d] : QrType<TYPE>::get(((const typename QrType<TYPE>::T*)w)[d])) + add;
+}
+
+// A vector's weights: of 16 bytes' columns from d on (aligned, or fp32 and aligned).
+template <int TYPE, int VEC>
+D3_DEV void qr_weights(const void* w, bool f32, float add, int d, float* out) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = 1.0f;
+    return;
+  }
+  if (f32) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      const float4 x = __ldg((const float4*)((const float*)w + d + e));
+      out[e] = x.x, out[e + 1] = x.y, out[e + 2] = x.z, out[e + 3] = x.w;
+    }
+  } else {
+    const uint4 x = __ldg((const uint4*)((const typename QrType<TYPE>::T*)w + d));
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    qr_unpack<TYPE, VEC>(words, out);
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) out[e] += add;
 }
 
 // (cos, sin) of pair f of token t; (1, 0) with the fault word set where the table has none.
@@ -122,122 +190,184 @@ D3_DEV E* qr_target(const QrArgs& a, int t, int h, int64_t slot) {
   return h < a.Hkv ? qr_slot<E>(a, a.kc, slot, h) : qr_slot<E>(a, a.vc, slot, h - a.Hkv);
 }
 
-// ---- rows of whole 16-byte vectors, no pair's halves inside one vector (with `pairs`: no pair cut by one). LANES
-// lanes (a power of two) per head, NV vectors a lane; vector i of lane l is number l + i * LANES of the head.
-template <int TYPE, int LANES, int NV, bool PAIRS>
-__global__ void __launch_bounds__(QR_WARPS * 32) qk_rope_kernel(QrArgs a) {
+// ---- rows of whole 16-byte vectors in twos. A slot is two vectors of a head that one lane has: number i and i + rot / 2
+// columns further on of the turned columns (with `pairs`, two neighbours), two neighbours of the others. LANES (a power
+// of two) lanes per head, one per slot. Dynamic shared memory: float2 [tokens][rot / 2].
+template <int TYPE, int LANES, bool PAIRS>
+__global__ void __launch_bounds__(QR_WARPS * 32, 4) qk_rope_kernel(QrArgs a) {
   using TT = QrType<TYPE>;
   using E = typename TT::T;
   constexpr int VEC = 16 / (int)sizeof(E);
-  constexpr int HEADS = 32 / LANES;  // heads a warp takes at a time
-  constexpr int AHEAD = 4;
+  constexpr int HEADS = 32 / LANES;  // heads a warp takes at a time, all queries, keys or values
+  constexpr int AHEAD = QR_AHEAD;
   union Vec {
     uint4 q;
-    E e[VEC];
+    uint32_t w[4];
   };
-  const int lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES;
-  const int gw = blockIdx.x * QR_WARPS + (threadIdx.x >> 5);
-  const int t = gw / a.share, part = gw - t * a.share;
+  extern __shared__ __align__(16) float2 qr_turns[];
+  const int lane = threadIdx.x & 31, sub = lane / LANES, l = lane % LANES, warp = threadIdx.x >> 5;
+  const int per = (a.share + QR_WARPS - 1) / QR_WARPS;  // blocks of a token, where there are more than one
+  const int group = per > 1 ? 0 : warp / a.share;       // of the block's tokens
+  const int t = per > 1 ? blockIdx.x / per : blockIdx.x * a.tokens + group;
+  const int before = per > 1 ? (blockIdx.x - t * per) * QR_WARPS : 0;  // the token's warps in earlier blocks
+  const int part = before + warp - group * a.share;
+  const bool active = group < a.tokens && t < a.T && part < a.share;
+  const int half = a.rot / 2;
+  const bool there = l < a.D / (2 * VEC);
+  const bool turned = l * 2 * VEC < a.rot;
+  // the first columns of the lane's two vectors
+  const int d0 = turned && !PAIRS ? l * VEC : l * 2 * VEC, d1 = turned && !PAIRS ? d0 + half : d0 + VEC;
+  const int apart = (d1 - d0) * (int)sizeof(E);
+  const int q_items = (a.Hq + HEADS - 1) / HEADS, k_items = (a.Hkv + HEADS - 1) / HEADS;
+  float2* turns = qr_turns + group * half;
   grid_dependency_wait();
   allow_dependents();
-  if (t >= a.T) return;
-  const int vectors = a.D / VEC, half = a.rot / 2, shift = half / VEC;
-  const int heads = a.Hq + a.Hkv * (a.k_out ? 1 : 2);
-  const int64_t slot = a.k_out ? -1 : a.slots[t];
-  Vec raw[AHEAD][NV];
-  auto load = [&](int h, Vec (&r)[NV]) {
-    if (h >= heads) return;
-    const uint4* p = (const uint4*)qr_row(a, t, h, sizeof(E));
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (l + i * LANES < vectors) r[i].q = p[l + i * LANES];
+  // An item is HEADS heads of the token's queries (0), keys (1) or values (2); of the items in that order a warp takes
+  // part, part + share, ...
+  Vec raw[AHEAD][2] = {};  // a lane without a slot keeps zeros
+  const int first = part < q_items ? 0 : part < q_items + k_items ? 1 : 2;
+  int n0 = 0, count = 0, heads = 0;  // this warp's first item of the kind, the kind's items and heads
+  const char* from = nullptr;        // this lane's row of the next fetch
+  long long from_step = 0;
+  auto fetch = [&](int n, Vec (&r)[2]) {
+    if (n < count && n * HEADS + sub < heads && there) {
+      r[0].q = *(const uint4*)from;
+      r[1].q = *(const uint4*)(from + apart);
+    }
+    from += from_step;
   };
-  const int step = HEADS * a.share;
-  const int h_first = HEADS * part + sub;
+  auto begin = [&](int kind) {
+    const QrTensor& x = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int earlier = kind == 0 ? 0 : kind == 1 ? q_items : q_items + k_items;
+    n0 = part >= earlier ? part - earlier : (a.share - (earlier - part) % a.share) % a.share;
+    count = kind == 0 ? q_items : k_items;
+    heads = kind == 0 ? a.Hq : a.Hkv;
+    const long long step = HEADS * x.head * (long long)sizeof(E);
+    from = (const char*)x.p + (t * x.token + sub * x.head + d0) * (long long)sizeof(E) + n0 * step;
+    from_step = a.share * step;
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) load(h_first + j * step, raw[j]);
-  // this lane's cosines and sines: with halves, column d becomes y[d] * c + y[partner] * s (s of the first half
-  // negative); with pairs, entries 2e and 2e + 1 of a vector share cs[e]
-  float c[NV][VEC], s[NV][VEC], wq[NV][VEC], wk[NV][VEC];
-  bool turned[NV];
+    for (int j = 0; j < AHEAD; ++j) fetch(n0 + j * a.share, raw[j]);
+  };
+  if (active) {
+    begin(first);
+    const int warps = min(a.share - before, QR_WARPS);  // of the token, in this block
+    for (int f = (part - before) * 32 + lane; f < half; f += warps * 32) turns[f] = qr_turn(a, t, f);
+  }
+  if (a.share > 1)
+    __syncthreads();
+  else
+    __syncwarp();
+  if (!active) return;
+  // the turned columns' cosines and sines: with halves, column e of both vectors turns by the same ones
+  uint64_t c2[VEC / 2], s2[VEC / 2];
+  if (!PAIRS && turned) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int vi = l + i * LANES, d0 = vi * VEC;
-    turned[i] = d0 < a.rot;
-    const bool second = !PAIRS && d0 >= half;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      c[i][e] = 1.0f;
-      s[i][e] = 0.0f;
-      if (turned[i] && (!PAIRS || e % 2 == 0)) {
-        const float2 cs = qr_turn(a, t, PAIRS ? (d0 + e) / 2 : d0 + e - (second ? half : 0));
-        c[i][e] = cs.x;
-        s[i][e] = PAIRS || second ? cs.y : -cs.y;
-      }
-      wq[i][e] = vi < vectors ? qr_weight<TYPE>(a.qw, a.w_f32, a.w_add, d0 + e) : 0.0f;
-      wk[i][e] = vi < vectors ? qr_weight<TYPE>(a.kw, a.w_f32, a.w_add, d0 + e) : 0.0f;
+    for (int e = 0; e < VEC / 2; ++e) {
+      const float4 x = *(const float4*)(turns + d0 + 2 * e);  // d0 is even
+      c2[e] = f2_make(x.x, x.z);
+      s2[e] = f2_make(x.y, x.w);
     }
   }
   const float inv_d = 1.0f / (float)a.D;
-  for (int h0 = h_first; h0 - sub < heads; h0 += AHEAD * step) {
+#pragma unroll 1
+  for (int kind = first; kind < (a.k_out ? 2 : 3); ++kind) {
+    if (kind != first) begin(kind);
+    if (n0 >= count) continue;
+    char* to;
+    long long to_step;
+    if (kind > 0 && !a.k_out) {
+      const QrCache& cache = kind == 1 ? a.kc : a.vc;
+      to = (char*)qr_slot<E>(a, cache, a.slots[t], sub);
+      if (!to) continue;
+      to_step = HEADS * cache.head * (long long)sizeof(E);
+    } else {
+      to = (char*)(kind == 0 ? a.q_out : a.k_out) + ((size_t)t * heads + sub) * a.D * sizeof(E);
+      to_step = HEADS * (long long)a.D * (long long)sizeof(E);
+    }
+    to += d0 * (long long)sizeof(E) + n0 * to_step;
+    to_step *= a.share;
+    const void* w = kind == 0 ? a.qw : a.kw;
+    uint64_t W[2][VEC / 2];  // two columns each
+    if (kind < 2 && there) {
+      float x[VEC];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      const int h = h0 + j * step;
-      if (h - sub >= heads) break;  // the same for the whole warp
-      const bool live = h < heads, is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
-      float y[NV][VEC], sum = 0.0f;
+      for (int v = 0; v < 2; ++v) {
+        qr_weights<TYPE, VEC>(w, a.w_f32, a.w_add, v ? d1 : d0, x);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          y[i][e] = live && l + i * LANES < vectors ? TT::get(raw[j][i].e[e]) : 0.0f;
-          sum = fmaf(y[i][e], y[i][e], sum);
-        }
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = (is_q ? a.qw : a.kw) ? rsqrtf(fmaf(sum, inv_d, a.eps)) : 1.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) y[i][e] *= inv * (is_q ? wq[i][e] : wk[i][e]);
-      Vec out[NV];
-      if (PAIRS) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            out[i].e[e] = TT::put(fmaf(y[i][e], c[i][e], -y[i][e + 1] * s[i][e]));
-            out[i].e[e + 1] = TT::put(fmaf(y[i][e + 1], c[i][e], y[i][e] * s[i][e]));
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int vi = l + i * LANES;
-          const int pv = vi < shift ? vi + shift : vi - shift;  // partner vector (unused where not turned)
-          const int src = sub * LANES + (pv & (LANES - 1));
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float other = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NV; ++n) {
-              const float o = __shfl_sync(0xffffffffu, y[n][e], src);
-              if (NV == 1 || pv / LANES == n) other = o;
-            }
-            out[i].e[e] = TT::put(turned[i] ? fmaf(y[i][e], c[i][e], other * s[i][e]) : y[i][e]);
-          }
-        }
-      }
-      if (live) {
-        E* p = qr_target<E>(a, t, h, slot);
-        if (p) {
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-            if (l + i * LANES < vectors) ((uint4*)p)[l + i * LANES] = is_v ? raw[j][i].q : out[i].q;
-        }
+        for (int e = 0; e < VEC / 2; ++e) W[v][e] = f2_make(x[2 * e], x[2 * e + 1]);
       }
     }
+#pragma unroll 1
+    for (int n = n0; n < count; n += AHEAD * a.share) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) load(h0 + (AHEAD + j) * step, raw[j]);
+      for (int j = 0; j < AHEAD; ++j) {
+        const int nj = n + j * a.share;
+        if (nj >= count) break;  // the same for the whole warp
+        Vec out[2];
+        if (kind == 2) {
+          out[0].q = raw[j][0].q;
+          out[1].q = raw[j][1].q;
+          fetch(nj + AHEAD * a.share, raw[j]);
+        } else {
+          uint64_t x2[2][VEC / 2], sums = 0;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            float x[VEC];
+            qr_unpack<TYPE, VEC>(raw[j][v].w, x);
+#pragma unroll
+            for (int e = 0; e < VEC / 2; ++e) {
+              x2[v][e] = f2_make(x[2 * e], x[2 * e + 1]);
+              sums = f2_fma(x2[v][e], x2[v][e], sums);
+              x2[v][e] = f2_mul(x2[v][e], W[v][e]);
+            }
+          }
+          fetch(nj + AHEAD * a.share, raw[j]);
+          float inv = 1.0f;
+          if (w) {
+            float s0, s1;
+            f2_split(sums, s0, s1);
+            float sum = s0 + s1;
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            inv = rsqrtf(fmaf(sum, inv_d, a.eps));
+          }
+          const uint64_t inv2 = f2_make(inv, inv);
+          float y[2][VEC];
+          if (!turned) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int e = 0; e < VEC / 2; ++e) f2_split(f2_mul(x2[v][e], inv2), y[v][2 * e], y[v][2 * e + 1]);
+          } else if (!PAIRS) {
+#pragma unroll
+            for (int e = 0; e < VEC / 2; ++e) {
+              const uint64_t c = f2_mul(c2[e], inv2), s = f2_mul(s2[e], inv2), minus = f2_mul(s, f2_make(-1.0f, -1.0f));
+              f2_split(f2_fma(x2[1][e], minus, f2_mul(x2[0][e], c)), y[0][2 * e], y[0][2 * e + 1]);
+              f2_split(f2_fma(x2[0][e], s, f2_mul(x2[1][e], c)), y[1][2 * e], y[1][2 * e + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int e = 0; e < VEC / 2; ++e) {
+                const float2 cs = turns[(v ? d1 : d0) / 2 + e];
+                const float c = cs.x * inv, s = cs.y * inv;
+                float lo, hi;
+                f2_split(x2[v][e], lo, hi);
+                y[v][2 * e] = fmaf(hi, -s, lo * c);
+                y[v][2 * e + 1] = fmaf(lo, s, hi * c);
+              }
+          }
+          qr_pack<TYPE, VEC>(y[0], out[0].w);
+          qr_pack<TYPE, VEC>(y[1], out[1].w);
+        }
+        if (nj * HEADS + sub < heads && there) {
+          *(uint4*)to = out[0].q;
+          *(uint4*)(to + apart) = out[1].q;
+        }
+        to += to_step;
+      }
+    }
   }
 }
 
@@ -270,16 +400,16 @@ __global__ void __launch_bounds__(QR_WARPS * 32) qk_rope_any_kernel(QrArgs a, in
     }
     inv = rsqrtf(fmaf(warp_sum(sum), 1.0f / (float)a.D, a.eps));
   }
-  auto normed = [&](int d) { return TT::get(x[d]) * (inv * qr_weight<TYPE>(w, a.w_f32, a.w_add, d)); };
+  auto normed = [&](int d) { return TT::get(x[d]) * qr_weight<TYPE>(w, a.w_f32, a.w_add, d); };
   const int half = a.rot / 2;
-  for (int f = lane; f < half; f += 32) {
+  for (int f = lane; f < half; f += 32) {  // the same steps as in the other form
     const int da = pairs ? 2 * f : f, db = pairs ? 2 * f + 1 : f + half;
     const float2 cs = qr_turn(a, t, f);
-    const float ya = normed(da), yb = normed(db);
-    out[da] = TT::put(fmaf(ya, cs.x, -yb * cs.y));
-    out[db] = TT::put(fmaf(yb, cs.x, ya * cs.y));
+    const float xa = normed(da), xb = normed(db), c = cs.x * inv, s = cs.y * inv;
+    out[da] = TT::put(fmaf(xb, -s, xa * c));
+    out[db] = TT::put(fmaf(xa, s, xb * c));
   }
-  for (int d = a.rot + lane; d < a.D; d += 32) out[d] = TT::put(normed(d));
+  for (int d = a.rot + lane; d < a.D; d += 32) out[d] = TT::put(normed(d) * inv);
 }
 
 }  // namespace d3

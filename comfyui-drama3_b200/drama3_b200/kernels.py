@@ -480,17 +480,38 @@ class LinesPlan(NamedTuple):
     group: int
 
 
-def _ints(name, t, device, *shape):
-    """Refuses anything but a contiguous int32 tensor of this shape (None: any size) on `device`."""
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device or t.dim() != len(shape) or any(
-            want is not None and want != got for want, got in zip(shape, t.shape)):
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)} on {device}, not "
-                         f"{t.dtype} {list(t.shape)} on {t.device}")
-    return t
+def _ints(name, t, device, count):
+    """Refuses anything but a contiguous int32 tensor of `count` values on `device`."""
+    if t.dtype is not torch.int32 or t.numel() != count or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} values on {device}, not {t.dtype} "
+                         f"{list(t.shape)} on {t.device}")
 
 
-def _strides(t, n):
-    return (ctypes.c_int64 * n)(*t.stride()[:n])
+@functools.lru_cache(maxsize=1024)
+def _int64s(values):
+    """The strides as the C array that the library takes (kept by value: a step's tensors have the same ones)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _launch(device, what, fn, *args):
+    """fn(*args, stream) on the device's current stream; raises on a refusal. Made for calls of a few microseconds:
+    the device is switched only where it is another than the current one."""
+    _device_ok(device.index)
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if status:
+        check(status, what)
+
+
+def _gpu_of(t, what):
+    """The CUDA device of a tensor; raises where it is on none."""
+    device = t.device
+    if device.type != "cuda":
+        raise ValueError(f"{what} takes tensors on a GPU, not on {device}")
+    return device
 
 
 def lines_plan(lengths, counts, table, free, used, page, tokens, prefix=None, group=1):
@@ -502,30 +523,38 @@ def lines_plan(lengths, counts, table, free, used, page, tokens, prefix=None, gr
     that the lines share, which come first in their positions. group: query heads per KV head of the attention that
     will use the plan. A page that the free list or the table has no room for is -1, as its tokens' slots are, and is
     recorded in the fault word."""
-    device = lengths.device
-    B = lengths.shape[0] if lengths.dim() == 1 else 0
+    device = _gpu_of(lengths, "lines_plan")
+    if lengths.dim() != 1 or table.dim() != 2 or free.dim() != 1:
+        raise ValueError("lines_plan takes lengths and counts [B], a table [B, W], free [F] and used [1]")
+    B, T, group = lengths.shape[0], int(tokens), int(group)
+    W, F = table.shape[1], free.shape[0]
     _ints("lengths", lengths, device, B)
     _ints("counts", counts, device, B)
-    _ints("table", table, device, B, None)
-    _ints("free", free, device, None)
+    _ints("table", table, device, B * W)
+    _ints("free", free, device, F)
     _ints("used", used, device, 1)
     if prefix is not None:
         _ints("prefix", prefix, device, 1)
-    T, group = int(tokens), int(group)
+    size = _plan_ints(B, T, group)
+    # one allocation for everything, cut up: slots and positions (int64), then the work list (16-byte aligned) and the rest
+    ints = (size + T + 2 * B + 3) // 2
+    slots, positions, rest = torch.empty(2 * T + ints, dtype=torch.int64, device=device).split_with_sizes((T, T, ints))
+    work, line, cu, new_lengths, new_used, _ = rest.view(torch.int32).split_with_sizes(
+        (size, T, B + 1, B, 1, 2 * ints - size - T - 2 * B - 2))
+    _launch(device, "lines_plan", lib().d3_lines_plan, lengths.data_ptr(), counts.data_ptr(), B, table.data_ptr(), W,
+            free.data_ptr(), F, used.data_ptr(), _ptr(prefix), int(page), T, group, slots.data_ptr(),
+            positions.data_ptr(), line.data_ptr(), cu.data_ptr(), new_lengths.data_ptr(), new_used.data_ptr(),
+            work.data_ptr(), size)
+    return LinesPlan(table, slots, positions, line, cu, new_lengths, new_used, work, int(page), group)
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_ints(B, T, group):
+    """Ints of a plan's work list, an even number; raises where there is no plan for these sizes."""
     size = lib().d3_lines_plan_ints(B, T, group)
     if size == 0:
         raise ValueError(f"no plan for {B} lines, {T} tokens, {group} query heads per KV head")
-    with _on(device):
-        slots, positions = torch.empty((2, T), dtype=torch.int64, device=device)
-        line = torch.empty(T, dtype=torch.int32, device=device)
-        state = torch.empty(2 * B + 2, dtype=torch.int32, device=device)
-        cu, new_lengths, new_used = state[:B + 1], state[B + 1:2 * B + 1], state[2 * B + 1:]
-        work = torch.empty(size, dtype=torch.int32, device=device)
-        check(lib().d3_lines_plan(_ptr(lengths), _ptr(counts), B, _ptr(table), table.shape[1], _ptr(free), free.shape[0],
-                                  _ptr(used), _ptr(prefix), int(page), T, group, _ptr(slots), _ptr(positions), _ptr(line),
-                                  _ptr(cu), _ptr(new_lengths), _ptr(new_used), _ptr(work), size, _stream(device)),
-              "lines_plan")
-    return LinesPlan(table, slots, positions, line, cu, new_lengths, new_used, work, int(page), group)
+    return size + size % 2
 
 
 def rotary_table(inv_freq, length, device=None):
@@ -558,57 +587,80 @@ def qk_norm_rope(q, k, rotary, positions, q_weight=None, k_weight=None, eps=1e-6
     k_weight [D] (of the rows' type or float32; 1 + weight with unit_offset; None: no norm) and the rotation of their
     first 2 n columns by rotary [length, n, 2] (`rotary_table`), halves (f, f + n) or, with `pairs`, neighbours (2f,
     2f + 1). positions: [T] int64, or [A, T] with axes [n] uint8 (`rotary_axes`) naming the row that turns each
-    frequency. With k_cache and v_cache [pages, page, Hkv, D], v [T, Hkv, D] and slots [T] (int64, a LinesPlan's) the
+    frequency (contiguous). With k_cache and v_cache [pages, page, Hkv, D], v [T, Hkv, D] and slots [T] (int64, a LinesPlan's) the
     keys and the values go to their slots of the caches instead (-1: nowhere) and k_out is None. One launch; 32-bit
     arithmetic, rounded once."""
-    T, Hq, D = q.shape
+    tensors = (q, k, rotary, positions, q_weight, k_weight, axes, v, k_cache, v_cache, slots)
+    forms = tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride()) for t in tensors])
+    checked = _ROPE_FORMS.get(forms)
+    if checked is None:
+        if len(_ROPE_FORMS) >= 4096:
+            _ROPE_FORMS.clear()
+        checked = _ROPE_FORMS[forms] = _rope_arguments(*tensors)
+    device, q_strides, k_strides, v_strides, sizes, w_f32, table, axes_n, cached = checked
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if cached is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        to = (k_out.data_ptr(), None, None, None, None, 0, 0, None)
+    else:
+        k_out = None
+        kc_strides, vc_strides, pages, page = cached
+        to = (None, k_cache.data_ptr(), kc_strides, v_cache.data_ptr(), vc_strides, pages, page, slots.data_ptr())
+    _launch(device, "qk_norm_rope", lib().d3_qk_norm_rope, q.data_ptr(), q_strides, k.data_ptr(), k_strides, _ptr(v),
+            v_strides, *sizes, _ptr(q_weight), _ptr(k_weight), w_f32, 1.0 if unit_offset else 0.0, eps,
+            rotary.data_ptr(), *table, positions.data_ptr(), axes_n, _ptr(axes), 1 if pairs else 0, q_out.data_ptr(), *to)
+    return q_out, k_out
+
+
+# forms (types, devices, shapes and strides) of qk_norm_rope's tensors that were checked -> the arguments they give. A
+# step's tensors have the same ones in every layer, and the checks took as long as the launch.
+_ROPE_FORMS = {}
+
+
+def _rope_arguments(q, k, rotary, positions, q_weight, k_weight, axes, v, k_cache, v_cache, slots):
+    """Refuses tensors of a form that qk_norm_rope does not take; the arguments that follow from their forms."""
+    device = _gpu_of(q, "qk_norm_rope")
+    for t in (k, rotary, positions, q_weight, k_weight, axes, v, k_cache, v_cache, slots):
+        if t is not None and t.device != device:
+            raise ValueError(f"qk_norm_rope: every tensor must be on {device}")
     if q.dtype not in ROW_TYPES or k.dtype != q.dtype:
         raise TypeError(f"qk_norm_rope takes bfloat16, float16 or float32 rows of one type, not {q.dtype} and {k.dtype}")
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("qk_norm_rope takes q [T, Hq, D] and k [T, Hkv, D]")
+    T, Hq, D = q.shape
     Hkv = k.shape[1]
-    if tuple(k.shape) != (T, Hkv, D) or q.stride(2) != 1 or k.stride(2) != 1:
+    if k.shape != (T, Hkv, D) or q.stride(2) != 1 or k.stride(2) != 1:
         raise ValueError("q [T, Hq, D] and k [T, Hkv, D] must agree in T and D, their last dimension contiguous")
-    device = q.device
     weights = [w for w in (q_weight, k_weight) if w is not None]
     for w in weights:
-        if tuple(w.shape) != (D,) or not w.is_contiguous() or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype:
+        if w.shape != (D,) or not w.is_contiguous() or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype:
             raise ValueError("q_weight and k_weight must be contiguous [D] tensors of the rows' type or float32, alike")
     if rotary.dtype != torch.float32 or rotary.dim() != 3 or rotary.shape[2] != 2 or not rotary.is_contiguous():
         raise ValueError("rotary must be a contiguous float32 [length, n, 2] tensor")
     length, n = rotary.shape[:2]
     if 2 * n > D:
         raise ValueError(f"rotary turns {2 * n} columns of {D}")
-    if positions.dtype != torch.int64 or positions.shape[-1] != T or positions.dim() != (1 if axes is None else 2):
-        raise ValueError("positions must be int64 [T], or [A, T] with axes")
-    positions = positions.contiguous()
-    if axes is not None and (axes.dtype != torch.uint8 or tuple(axes.shape) != (n,) or not axes.is_contiguous()):
+    if (positions.dtype != torch.int64 or positions.dim() != (1 if axes is None else 2) or positions.shape[-1] != T
+            or not positions.is_contiguous()):
+        raise ValueError("positions must be contiguous int64 [T], or [A, T] with axes")
+    if axes is not None and (axes.dtype != torch.uint8 or axes.shape != (n,) or not axes.is_contiguous()):
         raise ValueError("axes must be a contiguous uint8 tensor with the axis of each of the n frequencies")
-    cached = k_cache is not None
-    if any((x is not None) != cached for x in (v, v_cache, slots)):
+    if any((x is not None) != (k_cache is not None) for x in (v, v_cache, slots)):
         raise ValueError("v, k_cache, v_cache and slots go together")
-    if cached:
-        if tuple(v.shape) != (T, Hkv, D) or v.dtype != q.dtype or v.stride(2) != 1:
+    cached = v_strides = None
+    if k_cache is not None:
+        if v.shape != k.shape or v.dtype != q.dtype or v.stride(2) != 1:
             raise ValueError("v must be [T, Hkv, D] of the rows' type, its last dimension contiguous")
         for c in (k_cache, v_cache):
-            if c.dim() != 4 or c.shape != k_cache.shape or tuple(c.shape[2:]) != (Hkv, D) or c.dtype != q.dtype or c.stride(3) != 1:
+            if c.dim() != 4 or c.shape != k_cache.shape or c.shape[2:] != (Hkv, D) or c.dtype != q.dtype or c.stride(3) != 1:
                 raise ValueError("the caches must be [pages, page, Hkv, D] of the rows' type, alike, the last dimension contiguous")
-        if slots.dtype != torch.int64 or tuple(slots.shape) != (T,) or not slots.is_contiguous():
+        if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous int64 [T] tensor")
-    for t in (k, rotary, positions, axes, v, k_cache, v_cache, slots, *weights):
-        if t is not None and t.device != device:
-            raise ValueError(f"qk_norm_rope: every tensor must be on {device}")
-    with _on(device):
-        q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-        k_out = None if cached else torch.empty((T, Hkv, D), dtype=q.dtype, device=device)
-        pages, page = k_cache.shape[:2] if cached else (0, 0)
-        check(lib().d3_qk_norm_rope(_ptr(q), _strides(q, 2), _ptr(k), _strides(k, 2), _ptr(v),
-                                    _strides(v, 2) if cached else None, ROW_TYPES[q.dtype], T, Hq, Hkv, D, _ptr(q_weight),
-                                    _ptr(k_weight), int(bool(weights) and weights[0].dtype == torch.float32),
-                                    float(bool(unit_offset)), float(eps), _ptr(rotary), 2 * n, length, _ptr(positions),
-                                    1 if axes is None else positions.shape[0], _ptr(axes), int(bool(pairs)), _ptr(q_out),
-                                    _ptr(k_out), _ptr(k_cache), _strides(k_cache, 3) if cached else None, _ptr(v_cache),
-                                    _strides(v_cache, 3) if cached else None, pages, page, _ptr(slots), _stream(device)),
-              "qk_norm_rope")
-    return q_out, k_out
+        cached = (_int64s(k_cache.stride()), _int64s(v_cache.stride()), k_cache.shape[0], k_cache.shape[1])
+        v_strides = _int64s(v.stride())
+    return (device, _int64s(q.stride()), _int64s(k.stride()), v_strides, (ROW_TYPES[q.dtype], T, Hq, Hkv, D),
+            int(bool(weights) and weights[0].dtype == torch.float32), (2 * n, length),
+            1 if axes is None else positions.shape[0], cached)
 
 
 def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, lse=False):
@@ -620,34 +672,60 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     64. Where the lines bring few tokens, the prefix's keys are read once for all of them. Places of the plan without a
     token get zeros (lse -inf); what the cache holds past a line's length is never used."""
     T, Hq, D = q.shape
-    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    kind = ROW_TYPES.get(q.dtype)
+    if (kind != 0 and kind != 1) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise TypeError("lines_attention takes bfloat16 or float16 queries and caches of one type")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
-        raise ValueError("the caches must be [pages, page, Hkv, D], alike")
+    device = _gpu_of(q, "lines_attention")
     pages, page, Hkv = k_cache.shape[:3]
-    if q.stride(2) != 1 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+    if k_cache.shape != (pages, page, Hkv, D) or v_cache.shape != k_cache.shape:
+        raise ValueError("the caches must be [pages, page, Hkv, D], alike")
+    q_strides, kc_strides, vc_strides = q.stride(), k_cache.stride(), v_cache.stride()
+    if q_strides[2] != 1 or kc_strides[3] != 1 or vc_strides[3] != 1:
         raise ValueError("the last dimension of the queries and the caches must be contiguous")
+    table, work = plan.table, plan.work
+    B, W = table.shape
     if plan.page != page or plan.slots.shape[0] != T or plan.group * Hkv != Hq:
         raise ValueError(f"the plan is for {plan.slots.shape[0]} tokens, pages of {plan.page} and {plan.group} query heads "
                          f"per KV head, not for {T}, {page} and {Hq} / {Hkv}")
-    device = q.device
-    B = plan.cu.shape[0] - 1
+    if k_cache.device != device or v_cache.device != device or work.device != device:
+        raise ValueError(f"lines_attention: every tensor must be on {device}")
+    _ints("the plan's table", table, device, B * W)
+    prefix_pages = 0
     if prefix_table is not None:
-        _ints("prefix_table", prefix_table, device, None)
-    for t in (k_cache, v_cache, plan.work):
-        if t.device != device:
-            raise ValueError(f"lines_attention: every tensor must be on {device}")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    with _on(device):
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-        sums = torch.empty((T, Hq), dtype=torch.float32, device=device) if lse else None
-        size = lib().d3_lines_attention_workspace(T, Hq, Hkv, D)
-        if size == 0:
-            raise ValueError(f"no attention kernel for {Hq} / {Hkv} heads of {D}")
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        check(lib().d3_lines_attention(_ptr(q), _strides(q, 2), ROW_TYPES[q.dtype], T, Hq, Hkv, D, _ptr(k_cache),
-                                       _strides(k_cache, 3), _ptr(v_cache), _strides(v_cache, 3), pages, page,
-                                       _ptr(plan.table), plan.table.shape[1], _ptr(prefix_table),
-                                       0 if prefix_table is None else prefix_table.shape[0], _ptr(plan.work), B, scale, _ptr(out), _ptr(sums), _ptr(ws), size, _stream(device)),
-              "lines_attention")
+        prefix_pages = prefix_table.numel()
+        _ints("prefix_table", prefix_table, device, prefix_pages)
+    size = _attention_workspace(device.index, T, Hq, Hkv, D)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    sums = torch.empty((T, Hq), dtype=torch.float32, device=device) if lse else None
+    ws = _scratch(device, size)
+    _launch(device, "lines_attention", lib().d3_lines_attention, q.data_ptr(), _int64s(q_strides), kind, T, Hq, Hkv, D,
+            k_cache.data_ptr(), _int64s(kc_strides), v_cache.data_ptr(), _int64s(vc_strides), pages, page,
+            table.data_ptr(), W, _ptr(prefix_table), prefix_pages, work.data_ptr(), B,
+            1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(), _ptr(sums), ws.data_ptr(), size)
     return (out, sums) if lse else out
+
+
+_SCRATCH = {}
+
+
+def _scratch(device, size):
+    """`size` bytes that a call on the current stream may use until it ends: one buffer per stream, kept and grown
+    (calls on one stream never overlap); during a CUDA-graph capture a fresh one, which the graph owns."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
+    held = _SCRATCH.get(key)
+    if held is None or held.numel() < size:
+        held = _SCRATCH[key] = torch.empty(size, dtype=torch.uint8, device=device)
+    return held
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(index, T, Hq, Hkv, D):
+    """Bytes of workspace of an attention of these sizes on cuda:index; raises where there is no kernel for them."""
+    _device_ok(index)
+    with torch.cuda.device(index):
+        size = lib().d3_lines_attention_workspace(T, Hq, Hkv, D)
+    if size == 0:
+        raise ValueError(f"no attention kernel for {Hq} / {Hkv} heads of {D}")
+    return size
