@@ -135,10 +135,10 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
   if (work_ints < d3_lines_plan_ints(B, T, group)) return D3_ERR_WORKSPACE;
   DeviceInfo d;
   if (int st = device_info(&d)) return st;
-  const int smem = 5 * (B + 1) * 4;
+  const int smem = 4 * (B + 1) * 4;
   static std::atomic<uint64_t> done{0};
   if (smem > 48 * 1024)
-    if (int st = allow_smem_once(d3::lines_plan_kernel, 5 * (d3::LP_MAX_LINES + 1) * 4, done)) return st;
+    if (int st = allow_smem_once(d3::lines_plan_kernel, 4 * (d3::LP_MAX_LINES + 1) * 4, done)) return st;
   const d3::LinesPlanArgs a = {kept, counts, B, table, W, free_pages, F, used, prefix, page, T, group, slots, positions,
                                line, cu, lengths, used_out, work};
   return launch(d3::lines_plan_kernel, dim3(1 + (T + d3::LP_TOKENS - 1) / d3::LP_TOKENS), dim3(d3::LP_THREADS), smem,

@@ -7,10 +7,11 @@
 // Token t of the pass belongs to the line with cu_b <= t < cu_b+1 (cu the exclusive sum of c), is the line's own
 // token s = kept_b + t - cu_b, and goes to slot table[b, s / p] * p + s % p, at position prefix + s.
 //
-// Bound by latency: the bytes are a few per token. Block 0 scans the lines and writes the work list; every other
-// block repeats the scan (B lines, a few hundred nanoseconds) and places PLAN_TOKENS tokens, so nothing waits for
-// another block. A page is written into its table by the token that opens it, and read only from entries that
-// were there before, so no two threads race. The state that a pass advances (lengths, used) goes to fresh outputs:
+// Bound by latency: the bytes are a few per token. Every block scans the lines' counts, pages and units for itself (B
+// lines, about a microsecond), so that nothing waits for another block; then the first writes the state after the pass,
+// each other one places LP_TOKENS tokens, and all write units of the work list, a thread each: a unit's place follows from
+// its number by a closed sum. A page is written into its table by the token that opens it, and read only from entries
+// that were there before, so no two threads race. The state that a pass advances (lengths, used) goes to fresh outputs:
 // planning the same pass twice gives the same plan.
 #pragma once
 
@@ -21,7 +22,7 @@ namespace d3 {
 constexpr int LP_THREADS = 512;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOKENS = 2048;     // tokens placed by a block
-constexpr int LP_MAX_LINES = 8192;  // five int arrays of it fill 160 KB of shared memory
+constexpr int LP_MAX_LINES = 8192;  // four int arrays of it fill 128 KB of shared memory
 constexpr int LP_MAX_KEPT = 1 << 30;  // lengths are clamped to it, so no index below overflows
 
 // The attention's work list. A unit is a tile of rows, a row being a token and one of the `group` query heads of a KV
@@ -87,70 +88,108 @@ struct LinesPlanArgs {
   int* work;
 };
 
-// Inclusive sum over the block; `total` the block's. `warp_sums`: LP_WARPS + 1 values of shared memory.
-D3_DEV long long lp_block_scan(long long v, long long* warp_sums, long long& total) {
+// Exclusive sums over the B lines of N numbers each, f(b, v) filling v[N], into out[0 .. N - 1][0 .. B] (shared memory),
+// clipped to `most`. warp_sums: LP_WARPS x N values of shared memory.
+template <int N, class F>
+D3_DEV void lp_scan_lines(int B, int* const (&out)[N], long long most, long long (*warp_sums)[N], F&& f) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
-  }
-  if (lane == 31) warp_sums[warp] = incl;
-  __syncthreads();
-  long long before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < LP_WARPS; ++w) {
-    const long long s = warp_sums[w];
-    before += w < warp ? s : 0;
-    total += s;
-  }
-  __syncthreads();
-  return before + incl;
-}
-
-// Exclusive sums of f(b) over the B lines into out[0..B] (shared memory), each clipped to `most`; lines in runs of
-// one per thread.
-template <class F>
-D3_DEV void lp_scan_lines(int B, int* out, long long most, long long* warp_sums, F&& f) {
-  long long base = 0;
+  long long base[N] = {};
   for (int b0 = 0; b0 < B; b0 += LP_THREADS) {
     const int b = b0 + threadIdx.x;
-    const long long v = b < B ? (long long)f(b) : 0;
-    long long total;
-    const long long incl = lp_block_scan(v, warp_sums, total);
-    if (b < B) out[b] = (int)min(most, base + incl - v);
-    base += total;
+    long long v[N] = {}, incl[N];
+    if (b < B) f(b, v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) incl[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const long long u = __shfl_up_sync(0xffffffffu, incl[k], o);
+        if (lane >= o) incl[k] += u;
+      }
+    if (lane == 31)
+#pragma unroll
+      for (int k = 0; k < N; ++k) warp_sums[warp][k] = incl[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      long long total = 0, before = base[k];
+#pragma unroll
+      for (int w = 0; w < LP_WARPS; ++w) {
+        const long long s = warp_sums[w][k];
+        before += w < warp ? s : 0;
+        total += s;
+      }
+      if (b < B) out[k][b] = (int)min(most, before + incl[k] - v[k]);
+      base[k] += total;
+    }
+    __syncthreads();
   }
-  if (threadIdx.x == 0) out[B] = (int)min(most, base);
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k][B] = (int)min(most, base[k]);
   __syncthreads();
+}
+
+// Sum over i < n of floor((a i + b) / m), by the steps of Euclid's algorithm: whole parts of a / m and b / m are summed
+// up directly, and what is left counts the lattice points under a line, which turned about its diagonal is a sum of the
+// same kind with a and m exchanged.
+D3_DEV long long lp_floor_sum(long long n, long long m, long long a, long long b) {
+  long long sum = 0;
+  while (true) {
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const long long y = a * n + b;
+    if (y < m) return sum;
+    n = y / m;
+    b = y % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+}
+
+// What the first i units of a line cost: its tokens in tiles of `tile` (the last one shorter), each tile's key tiles up to
+// its last token behind `lead` of the prefix.
+D3_DEV long long lp_cost(int i, int n, int kept, int count, int tile, int lead) {
+  if (i == 0) return 0;
+  const int whole = i == n ? n - 1 : i;
+  long long tiles = lp_floor_sum(whole, LA_KEYS, tile, (long long)kept + tile + LA_KEYS - 1);
+  if (i == n) tiles += (kept + count + LA_KEYS - 1) / LA_KEYS;
+  return tiles + (long long)i * (lead + LA_UNIT_COST);
 }
 
 D3_DEV int lp_clamped(const int* p, int b) { return min(max(0, p[b]), LP_MAX_KEPT); }
 
 __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a) {
   extern __shared__ int lp_smem[];
-  __shared__ long long warp_sums[LP_WARPS];
-  int* cu = lp_smem;               // [B + 1] first token of each line, clipped to T
-  int* first = cu + a.B + 1;       // [B + 1] pages taken by the lines before
-  int* unit0 = first + a.B + 1;    // [B + 1] own units of the lines before
-  int* kept_of = unit0 + a.B + 1;  // [B] tokens that the line has
-  int* cost_of = kept_of + a.B;    // [B + 1] block 0: cost of the line's units, then of the lines before
-  const int tid = threadIdx.x, B = a.B;
+  __shared__ long long sums1[LP_WARPS][1], sums2[LP_WARPS][2];
+  int* cu = lp_smem;                // [B + 1] first token of each line, clipped to T
+  int* first = cu + a.B + 1;        // [B + 1] pages taken by the lines before; then what their own units cost
+  int* unit0 = first + a.B + 1;     // [B + 1] own units of the lines before
+  int* kept_of = unit0 + a.B + 1;   // [B] tokens that the line has
+  const int tid = threadIdx.x, B = a.B, G = a.group, tile = la_tile_tokens(G);
   grid_dependency_wait();
   allow_dependents();
-  lp_scan_lines(B, cu, a.T, warp_sums, [&](int b) { return lp_clamped(a.counts, b); });
   const int used = max(0, *a.used);
   const int prefix = a.prefix ? max(0, *a.prefix) : 0;
-  lp_scan_lines(B, first, 0x7fffffffLL, warp_sums, [&](int b) {
-    const int kept = lp_clamped(a.kept, b), p = a.page;
-    kept_of[b] = kept;
-    return (kept + cu[b + 1] - cu[b] + p - 1) / p - (kept + p - 1) / p;
-  });
-  const int G = a.group, tile = la_tile_tokens(G), tokens = cu[B];
-  lp_scan_lines(B, unit0, 0x7fffffffLL, warp_sums, [&](int b) { return (cu[b + 1] - cu[b] + tile - 1) / tile; });
-  const int own_units = unit0[B];
+  {
+    int* const out[1] = {cu};
+    lp_scan_lines<1>(B, out, a.T, sums1, [&](int b, long long (&v)[1]) {
+      v[0] = lp_clamped(a.counts, b);
+      kept_of[b] = lp_clamped(a.kept, b);
+    });
+  }
+  {
+    int* const out[2] = {first, unit0};
+    lp_scan_lines<2>(B, out, 0x7fffffffLL, sums2, [&](int b, long long (&v)[2]) {
+      const int kept = kept_of[b], n = cu[b + 1] - cu[b], p = a.page;
+      v[0] = (kept + n + p - 1) / p - (kept + p - 1) / p;
+      v[1] = (n + tile - 1) / tile;
+    });
+  }
+  const int tokens = cu[B], own_units = unit0[B];
   const int prefix_tiles = (prefix + LA_KEYS - 1) / LA_KEYS;
   const int prefix_units = prefix > 0 ? (tokens + tile - 1) / tile : 0;
   // The prefix is read once for the rows of all lines together, or by each line's units on the way to its own keys.
@@ -196,69 +235,54 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
       a.line[t] = b;
       a.work[LW_HEADER + t] = unit;
     }
-    return;
-  }
-  // ---- block 0: the state after the pass, and the attention's work list
-  int over = 0;
-  for (int b = tid; b < B; b += LP_THREADS) {
-    const int kept = kept_of[b], n = cu[b + 1] - cu[b];
-    over |= n < a.counts[b];
-    a.cu[b] = cu[b];
-    a.lengths[b] = kept + n;
-  }
-  if (over) record_fault(FAULT_TOKENS);
-  if (tid == 0) {
-    a.cu[B] = tokens;
-    *a.used_out = (int)min((long long)a.F, (long long)used + first[B]);
-  }
-  const int warp = tid >> 5, lane = tid & 31;
-  // The own units, a warp per line: first what each line costs, then, with the lines' costs summed up, the units
-  // themselves. (Written at once and moved to their places afterwards, each unit of a line waited for memory twice.)
-  LaUnit* units = (LaUnit*)(a.work + la_unit_offset(a.T));
-  auto cost_at = [&](int b, int i, int n, int count, int& from, int& to) {  // of unit i of line b, its tokens
-    from = i * tile;
-    to = min(from + tile, count);
-    return i < n ? lead + (kept_of[b] + to + LA_KEYS - 1) / LA_KEYS + LA_UNIT_COST : 0;
-  };
-  for (int b = warp; b < B; b += LP_WARPS) {
-    const int count = cu[b + 1] - cu[b], n = unit0[b + 1] - unit0[b];
-    int sum = 0, from, to;
-    for (int i = lane; i < n; i += 32) sum += cost_at(b, i, n, count, from, to);
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) cost_of[b] = sum;
-  }
-  __syncthreads();
-  // in place: a thread's value is read into the scan before its own place is written
-  lp_scan_lines(B, cost_of, 0x7fffffffLL, warp_sums, [&](int b) { return cost_of[b]; });
-  const int shared_cost = together ? 0 : prefix_units * (prefix_tiles + LA_UNIT_COST);
-  for (int b = warp; b < B; b += LP_WARPS) {
-    const int count = cu[b + 1] - cu[b], n = unit0[b + 1] - unit0[b];
-    int base = shared_cost + cost_of[b];
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      int from, to;
-      const int cost = cost_at(b, i, n, count, from, to);
-      int incl = cost;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const int tiles = cost - LA_UNIT_COST;
-      if (i < n)
-        units[u0 + unit0[b] + i] = LaUnit{b, cu[b] + from, (to - from) * G, base + incl - tiles, tiles,
-                                          kept_of[b] + from + 1, kept_of[b] + to, lead};
-      base += __shfl_sync(0xffffffffu, incl, 31);
+  } else {
+    // ---- the first block: the state after the pass
+    int over = 0;
+    for (int b = tid; b < B; b += LP_THREADS) {
+      const int n = cu[b + 1] - cu[b];
+      over |= n < a.counts[b];
+      a.cu[b] = cu[b];
+      a.lengths[b] = kept_of[b] + n;
+    }
+    if (over) record_fault(FAULT_TOKENS);
+    if (tid == 0) {
+      a.cu[B] = tokens;
+      *a.used_out = (int)min((long long)a.F, (long long)used + first[B]);
     }
   }
-  for (int u = tid; u < u0; u += LP_THREADS)
-    units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G, u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST,
-                      prefix_tiles, 0, 0, prefix_tiles};
-  if (tid == 0) {
+  // ---- all blocks: the attention's work list, a unit per thread
+  __syncthreads();  // first is read no more: it becomes what the lines before cost
+  {
+    int* const out[1] = {first};
+    lp_scan_lines<1>(B, out, 0x7fffffffLL, sums1, [&](int b, long long (&v)[1]) {
+      const int n = unit0[b + 1] - unit0[b];
+      v[0] = lp_cost(n, n, kept_of[b], cu[b + 1] - cu[b], tile, lead);
+    });
+  }
+  LaUnit* units = (LaUnit*)(a.work + la_unit_offset(a.T));
+  const long long shared_cost = (long long)u0 * (prefix_tiles + LA_UNIT_COST);
+  for (int u = blockIdx.x * LP_THREADS + tid; u < u0 + own_units; u += gridDim.x * LP_THREADS) {
+    if (u < u0) {
+      units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G, u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST,
+                        prefix_tiles, 0, 0, prefix_tiles};
+      continue;
+    }
+    int b = 0, hi = B;  // the last line whose units begin at or before this one: it has it
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (unit0[mid] <= u - u0) b = mid; else hi = mid;
+    }
+    const int i = u - u0 - unit0[b], n = unit0[b + 1] - unit0[b], count = cu[b + 1] - cu[b], kept = kept_of[b];
+    const int from = i * tile, to = min(from + tile, count);
+    const int at = (int)(shared_cost + first[b] + lp_cost(i, n, kept, count, tile, lead) + LA_UNIT_COST);
+    units[u] = LaUnit{b, cu[b] + from, (to - from) * G, at, lead + (kept + to + LA_KEYS - 1) / LA_KEYS, kept + from + 1,
+                      kept + to, lead};
+  }
+  if (blockIdx.x == 0 && tid == 0) {
     int* w = a.work;
     w[LW_TOGETHER] = together;
     w[LW_UNITS] = u0 + own_units;
-    w[LW_COST] = shared_cost + cost_of[B];
+    w[LW_COST] = (int)min(0x7fffffffLL, shared_cost + first[B]);  // the attention refuses 2^30 and more
     w[LW_PREFIX] = prefix;
     w[LW_PREFIX_TILES] = prefix_tiles;
     w[LW_TOKENS] = tokens;

@@ -535,7 +535,7 @@ def lines_plan(lengths, counts, table, free, used, page, tokens, prefix=None, gr
     _ints("used", used, device, 1)
     if prefix is not None:
         _ints("prefix", prefix, device, 1)
-    size = _plan_ints(B, T, group)
+    size = plan_ints(B, T, group)
     # one allocation for everything, cut up: slots and positions (int64), then the work list (16-byte aligned) and the rest
     ints = (size + T + 2 * B + 3) // 2
     slots, positions, rest = torch.empty(2 * T + ints, dtype=torch.int64, device=device).split_with_sizes((T, T, ints))
@@ -549,7 +549,7 @@ def lines_plan(lengths, counts, table, free, used, page, tokens, prefix=None, gr
 
 
 @functools.lru_cache(maxsize=4096)
-def _plan_ints(B, T, group):
+def plan_ints(B, T, group):
     """Ints of a plan's work list, an even number; raises where there is no plan for these sizes."""
     size = lib().d3_lines_plan_ints(B, T, group)
     if size == 0:

@@ -1,8 +1,9 @@
 """The library's kernels as torch.library custom ops, torch.ops.drama3_b200.<name>, for callers that build graphs
 (torch.compile, CUDA graph capture, exported programs): every op takes and returns plain tensors, ints, bools and
-strings, writes fresh outputs (shared_expert updates `out` in place and declares it), and has a fake implementation
-that gives the output shapes and dtypes without running anything. Each op calls the matching function of
-drama3_b200.kernels; there is no CPU or torch fallback, so a call on tensors that are not on a B200 fails loudly.
+strings, writes fresh outputs (shared_expert updates `out` in place and declares it, as lines_plan does its table and
+qk_norm_rope_cached its caches), and has a fake implementation that gives the output shapes and dtypes without running
+anything. Each op calls the matching function of drama3_b200.kernels; there is no CPU or torch fallback, so a call on
+tensors that are not on a B200 fails loudly.
 
 Import this module once to register the ops. The expert banks of moe_decode and grouped_mma are passed field by
 field: `w` is the bank's weight rows ("weight" for fp8 / fp8c, "_qdata" for the integer layouts), `scale` its scales
@@ -16,7 +17,7 @@ from . import _lib, kernels
 
 NAMESPACE = "drama3_b200"
 OPS = ("route", "weighted_sum", "rotate", "router", "shared_expert", "moe_decode", "grouped_mma", "prefill_plan",
-       "prefill_combine")
+       "prefill_combine", "lines_plan", "qk_norm_rope", "qk_norm_rope_cached", "lines_attention")
 
 
 def _fields(kind, w, scale, s_channel):
@@ -145,3 +146,65 @@ def prefill_combine(sorted_out: Tensor, pos: Tensor, weights: Tensor, out_f32: b
 def _(sorted_out, pos, weights, out_f32=False):
     return sorted_out.new_empty((pos.shape[0], sorted_out.shape[1]),
                                 dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+# ---- the attention half of a decoder layer, for lines decoded together
+
+@torch.library.custom_op(f"{NAMESPACE}::lines_plan", mutates_args=("table",))
+def lines_plan(lengths: Tensor, counts: Tensor, table: Tensor, free: Tensor, used: Tensor, page: int, tokens: int,
+               prefix: Optional[Tensor] = None,
+               group: int = 1) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(slots, positions, line, cu, lengths, used, work) of kernels.lines_plan; the block table is updated in place."""
+    p = kernels.lines_plan(lengths, counts, table, free, used, page, tokens, prefix=prefix, group=group)
+    # outputs of an op share no storage: the plan's are cut from one allocation
+    return tuple(t.clone() for t in (p.slots, p.positions, p.line, p.cu, p.lengths, p.used, p.work))
+
+
+@lines_plan.register_fake
+def _(lengths, counts, table, free, used, page, tokens, prefix=None, group=1):
+    B = lengths.shape[0]
+    i32 = [lengths.new_empty((n,), dtype=torch.int32) for n in (tokens, B + 1, B, 1, kernels.plan_ints(B, tokens, group))]
+    return (lengths.new_empty((tokens,), dtype=torch.int64), lengths.new_empty((tokens,), dtype=torch.int64), *i32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: Tensor, k: Tensor, rotary: Tensor, positions: Tensor, q_weight: Optional[Tensor] = None,
+                 k_weight: Optional[Tensor] = None, eps: float = 1e-6, unit_offset: bool = False,
+                 axes: Optional[Tensor] = None, pairs: bool = False) -> tuple[Tensor, Tensor]:
+    """(q, k) through the norm of each head and the rotation: kernels.qk_norm_rope without a cache."""
+    return kernels.qk_norm_rope(q, k, rotary, positions, q_weight, k_weight, eps, unit_offset, axes, pairs)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, rotary, positions, q_weight=None, k_weight=None, eps=1e-6, unit_offset=False, axes=None, pairs=False):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::qk_norm_rope_cached", mutates_args=("k_cache", "v_cache"))
+def qk_norm_rope_cached(q: Tensor, k: Tensor, v: Tensor, rotary: Tensor, positions: Tensor, k_cache: Tensor,
+                        v_cache: Tensor, slots: Tensor, q_weight: Optional[Tensor] = None,
+                        k_weight: Optional[Tensor] = None, eps: float = 1e-6, unit_offset: bool = False,
+                        axes: Optional[Tensor] = None, pairs: bool = False) -> Tensor:
+    """q through the norm of each head and the rotation; k (likewise) and v go to their slots of the paged caches."""
+    return kernels.qk_norm_rope(q, k, rotary, positions, q_weight, k_weight, eps, unit_offset, axes, pairs, v=v,
+                                k_cache=k_cache, v_cache=v_cache, slots=slots)[0]
+
+
+@qk_norm_rope_cached.register_fake
+def _(q, k, v, rotary, positions, k_cache, v_cache, slots, q_weight=None, k_weight=None, eps=1e-6, unit_offset=False,
+      axes=None, pairs=False):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::lines_attention", mutates_args=())
+def lines_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, work: Tensor, group: int,
+                    prefix_table: Optional[Tensor] = None, scale: Optional[float] = None) -> tuple[Tensor, Tensor]:
+    """(out, lse) of kernels.lines_attention with a plan's block table and work list (made for `group` query heads per
+    KV head and q's token places)."""
+    plan = kernels.LinesPlan(table, q, None, None, None, None, None, work, k_cache.shape[1], group)
+    return kernels.lines_attention(q, k_cache, v_cache, plan, prefix_table=prefix_table, scale=scale, lse=True)
+
+
+@lines_attention.register_fake
+def _(q, k_cache, v_cache, table, work, group, prefix_table=None, scale=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)

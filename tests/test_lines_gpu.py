@@ -485,3 +485,144 @@ def test_step_on_a_side_stream_and_in_a_graph(cuda):
             assert torch.equal(out, want[i]), i
     assert torch.equal(kc, kc2) and torch.equal(held[0], st[0]) and fault() == 0
     del graph
+
+
+# ---- refusals that need tensors on a GPU, the ops, the module and the example
+
+def test_wrapper_refusals(cuda):
+    from drama3_b200 import kernels
+    n = i32([1, 1], cuda)
+    t, f, u = i32([[-1], [-1]], cuda), i32([0, 1], cuda), i32([0], cuda)
+    for bad in (dict(counts=n[:1]), dict(counts=n.long()), dict(table=i32([[-1]], cuda)), dict(used=n), dict(free=f.float()),
+                dict(prefix=n), dict(group=200), dict(table=t.t()), dict(counts=n.cpu())):
+        args = dict(lengths=n, counts=n, table=t, free=f, used=u, page=16, tokens=2)
+        with pytest.raises(ValueError):
+            kernels.lines_plan(**{**args, **bad})
+    q, k, v, qw, kw, rotary, pos, amap = rope_inputs(cuda, 4, 4, 2, 64, 64, 3, torch.bfloat16, 1)
+    cache = torch.zeros((2, 16, 2, 64), dtype=torch.bfloat16, device=cuda)
+    slots = torch.arange(4, device=cuda)
+    args = dict(q=q, k=k, rotary=rotary, positions=pos, axes=amap)
+    whole = dict(v=v, k_cache=cache, v_cache=cache.clone(), slots=slots)
+    for error, bad in ((TypeError, dict(q=q.double())), (TypeError, dict(k=k.half())), (ValueError, dict(k=k[:2])),
+                       (ValueError, dict(k=k[..., :32])), (ValueError, dict(q=q.transpose(1, 2))),
+                       (ValueError, dict(q_weight=qw[:32])), (ValueError, dict(q_weight=qw, k_weight=kw.float())),
+                       (ValueError, dict(rotary=rotary.half())), (ValueError, dict(rotary=rotary.repeat(1, 2, 1))),
+                       (ValueError, dict(positions=pos[0])), (ValueError, dict(positions=pos.int())),
+                       (ValueError, dict(axes=None)), (ValueError, dict(axes=amap[:8])), (ValueError, dict(axes=amap.long())),
+                       (ValueError, dict(v=v)), (ValueError, {**whole, "slots": None}), (ValueError, {**whole, "v": v[:2]}),
+                       (ValueError, {**whole, "k_cache": cache.half()}), (ValueError, {**whole, "v_cache": cache[:1]}),
+                       (ValueError, {**whole, "slots": slots.int()}), (ValueError, dict(positions=pos.cpu())),
+                       (ValueError, {**whole, "k_cache": cache.cpu()})):
+        with pytest.raises(error):
+            kernels.qk_norm_rope(**{**args, **bad})
+    plan = kernels.lines_plan(i32([0] * 4, cuda), i32([1] * 4, cuda), i32([[-1]] * 4, cuda), i32(list(range(4)), cuda), u, 16, 4,
+                              group=2)
+    kc = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16, device=cuda)
+    for error, bad in ((TypeError, dict(q=q.float())), (TypeError, dict(k_cache=kc.half())), (ValueError, dict(v_cache=kc[:3])),
+                       (ValueError, dict(k_cache=kc[..., :32], v_cache=kc[..., :32])), (ValueError, dict(q=q[:3])),
+                       (ValueError, dict(plan=plan._replace(page=32))), (ValueError, dict(plan=plan._replace(group=4))),
+                       (ValueError, dict(prefix_table=i32([0], cuda).long())), (ValueError, dict(v_cache=kc.cpu()))):
+        with pytest.raises(error):
+            kernels.lines_attention(**{**dict(q=q, k_cache=kc, v_cache=kc, plan=plan), **bad})
+    with pytest.raises(ValueError):  # heads of 96: no kernel
+        kernels.lines_attention(torch.zeros((4, 4, 96), dtype=torch.bfloat16, device=cuda), *[torch.zeros(
+            (4, 16, 2, 96), dtype=torch.bfloat16, device=cuda)] * 2, plan)
+    with pytest.raises(_lib_error()):  # a page that no tile is made of
+        odd = kernels.lines_plan(i32([0] * 4, cuda), i32([1] * 4, cuda), i32([[-1]] * 4, cuda), i32(list(range(4)), cuda), u, 24,
+                                 4, group=2)
+        kernels.lines_attention(q, *[torch.zeros((4, 24, 2, 64), dtype=torch.bfloat16, device=cuda)] * 2, odd)
+    assert fault() == 0
+
+
+def _lib_error():
+    from drama3_b200._lib import D3Error
+    return D3Error
+
+
+def test_ops_equal_the_kernels(cuda):
+    import drama3_b200.ops  # noqa: F401
+    from drama3_b200 import kernels
+    o = torch.ops.drama3_b200
+    kept, counts, prefix = [40, 3], [5, 70], 100
+    q, kc, vc, plan, pt = attn_case(cuda, 16, 4, 128, torch.bfloat16, 32, kept, counts, prefix)
+    out, lse = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt, lse=True)
+    got = o.lines_attention(q, kc, vc, plan.table, plan.work, 4, pt)
+    assert torch.equal(out, got[0]) and torch.equal(lse, got[1])
+    table, free, used, tokens = lines_case(kept, counts, 32, 3)
+    args = lambda: (i32(kept, cuda), i32(counts, cuda), i32(table, cuda), i32(free, cuda), i32([used], cuda), 32, tokens)  # noqa: E731
+    a, b = args(), args()
+    p = kernels.lines_plan(*a, prefix=i32([9], cuda), group=4)
+    r = o.lines_plan(*b, i32([9], cuda), 4)
+    assert torch.equal(a[2], b[2])
+    for x, y in zip((p.slots, p.positions, p.line, p.cu, p.lengths, p.used), r):
+        assert torch.equal(x, y)
+    rq, rk, rv, qw, kw, rotary, pos, _ = rope_inputs(cuda, 9, 6, 2, 64, 64, 1, torch.bfloat16, 5)
+    for x, y in zip(kernels.qk_norm_rope(rq, rk, rotary, pos, qw, kw), o.qk_norm_rope(rq, rk, rotary, pos, qw, kw)):
+        assert torch.equal(x, y)
+    caches = [torch.zeros((2, 16, 2, 64), dtype=torch.bfloat16, device=cuda) for _ in range(4)]
+    slots = torch.randperm(32, device=cuda)[:9]
+    want, _ = kernels.qk_norm_rope(rq, rk, rotary, pos, v=rv, k_cache=caches[0], v_cache=caches[1], slots=slots)
+    assert torch.equal(want, o.qk_norm_rope_cached(rq, rk, rv, rotary, pos, caches[2], caches[3], slots))
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+def test_module_reads_a_prefix_and_texts_as_one_sequence(cuda):
+    """LinesAttention over a LinesCache: a shared prefix, ragged texts and two steps give each line what torch's layers
+    give the whole sequence (bf16 rounds at the same places but inside the attention: 2^-8 of sum p |V| there, and the
+    output projection sums 512 such columns; 1.5 % of the output's norm covers both)."""
+    from drama3_b200 import kernels
+    from drama3_b200.attention import LinesAttention, LinesCache
+    torch.manual_seed(3)
+    hidden, hq, hkv, D, page = 256, 8, 2, 64, 16
+    att = LinesAttention(hidden, hq, hkv, D, device=cuda, dtype=torch.bfloat16)
+    with torch.no_grad():
+        att.q_norm.mul_(1.3)
+        att.k_norm.add_(0.1 * torch.randn(D, device=cuda))
+    prefix, texts, steps = 37, [3, 20, 0, 9], 2
+    cache = LinesCache(1, 40, page, hkv, D, 4, 64, hq // hkv, cuda)
+    rotary = kernels.rotary_table(10000.0 ** (-torch.arange(16, dtype=torch.float64) / 16), 128, cuda)
+    x0 = torch.randn((prefix, hidden), device=cuda).bfloat16()
+    xs = [torch.randn((n + steps, hidden), device=cuda).bfloat16() for n in texts]
+
+    def layers(x):  # one whole sequence through torch
+        q, k, v = (t.unflatten(1, (-1, D)) for t in att.qkv_proj(x).split([hq * D, hkv * D, hkv * D], 1))
+        pos = torch.arange(x.shape[0], device=cuda)
+        q, k = (ref.norm_rope(t, w, 0, att.eps, rotary, pos, None, False).bfloat16().float() for t, w in
+                ((q, att.q_norm), (k, att.k_norm)))
+        o = torch.nn.functional.scaled_dot_product_attention(
+            q.transpose(0, 1), k.transpose(0, 1).repeat_interleave(hq // hkv, 0),
+            v.float().transpose(0, 1).repeat_interleave(hq // hkv, 0), is_causal=True)
+        return att.o_proj(o.transpose(0, 1).flatten(1).bfloat16())
+
+    def close(got, want):
+        assert float((got.float() - want.float()).norm()) <= 0.015 * float(want.float().norm())
+
+    with torch.no_grad():
+        for again in range(2):  # the second time, new lines behind the same prefix
+            if again:
+                cache.restart()
+            else:
+                close(att(x0, cache.plan_prefix(prefix), cache.k[0], cache.v[0], rotary), layers(x0))
+            want = [layers(torch.cat((x0, x)))[prefix:] for x in xs]
+            got = att(torch.cat([x[:n] for x, n in zip(xs, texts)]), cache.plan(i32(texts, cuda), sum(texts)), cache.k[0],
+                      cache.v[0], rotary, cache.prefix_table).split(texts)
+            for g, w, n in zip(got, want, texts):
+                if n:
+                    close(g, w[:n])
+            for s in range(steps):
+                g = att(torch.stack([x[n + s] for x, n in zip(xs, texts)]), cache.plan(i32([1] * 4, cuda), 4), cache.k[0],
+                        cache.v[0], rotary, cache.prefix_table)
+                close(g, torch.stack([w[n + s] for w, n in zip(want, texts)]))
+    assert fault() == 0 and cache.lengths.tolist() == [n + steps for n in texts]
+
+
+def test_example_runs(cuda):
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("lines_decode", Path(__file__).resolve().parents[1] / "examples" / "lines_decode.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    rows, ms = example.decode(lines=3, prompt=70, steps=4, n_layers=2)
+    again, _ = example.decode(lines=3, prompt=70, steps=4, n_layers=2)
+    assert rows.shape == (3, example.HIDDEN) and rows.isfinite().all() and ms > 0 and fault() == 0
+    assert torch.equal(rows, again)
