@@ -48,15 +48,6 @@ bool query_map(CUtensorMap* map, bool f16, const void* base, int D, int heads, i
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
-int attn_runs(const DeviceInfo& d) {
-  return d.sms * d3::LaShape<D>::PER_SM;
-}
-
-int attn_runs_of(const DeviceInfo& d, int D) {
-  return D == 64 ? attn_runs<64>(d) : D == 128 ? attn_runs<128>(d) : attn_runs<256>(d);
-}
-
 bool attn_shape(int T, int Hq, int Hkv, int D) {
   return T >= 0 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= d3::LA_ROWS &&
          (D == 64 || D == 128 || D == 256) && (long long)T * Hq <= 0x7fffffffLL - 1024;
@@ -200,8 +191,8 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
 size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D) {
   DeviceInfo d;
   if (!attn_shape(T, Hq, Hkv, D) || device_info(&d)) return 0;
-  const long long rows = d3::la_part_rows(attn_runs_of(d, D), T, Hq / Hkv, Hkv);
-  return (size_t)rows * (D + 2) * 4 + (size_t)attn_runs_of(d, D) * 16;
+  const long long rows = d3::la_part_rows(d.sms, T, Hq / Hkv, Hkv);
+  return (size_t)rows * (D + 2) * 4 + (size_t)d.sms * 16;
 }
 
 int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
@@ -240,7 +231,7 @@ int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T,
   a.work = work, a.B = B;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out, a.lse = lse;
-  a.runs = attn_runs_of(d, D);
+  a.runs = d.sms;
   const long long rows = d3::la_part_rows(a.runs, T, a.G, Hkv);
   a.part_o = (float4*)workspace;
   a.part_ml = (float2*)((float*)workspace + rows * D);

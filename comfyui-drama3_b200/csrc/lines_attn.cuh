@@ -11,13 +11,13 @@
 // lines_join_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
 // key is read once for all lines.
 //
-// Per CTA (320 threads; two CTAs per SM for heads of 64 and 128, so that one's products run under the other's
-// exponentials; one for 256, with two buffers for S instead):
+// Per CTA (320 threads, one per SM):
 //   warp 0     loads by TMA (128-byte swizzle) into a ring of 16 KB stages, a stage being 64 columns of a tile's 128
 //              keys of K or V: a box per page, a lane each. A page outside the cache reads as zeros (the map's fill).
 //              A unit's queries likewise, into a buffer of their own.
-//   warp 1     issues the MMAs and owns the tensor memory: S = Q K^T (128 x 128), O += P V (128 x D, A = P from tensor
-//              memory, B = V as it lies in the cache: keys are its rows, so it is the MN-major operand)
+//   warp 1     issues the MMAs and owns the tensor memory: S = Q K^T (128 x 128, two buffers, a tile ahead of the rows), O
+//              += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so it is the
+//              MN-major operand)
 //   warps 2-9  two threads own a row, 64 of a tile's keys each: S from tensor memory, mask, maximum, exponentials, P
 //              back over S, the row's sum. O is rescaled only when the maximum has grown by more than 2^8 since the
 //              last time (p <= 256 in between, the same value after the division). They also write the results.
@@ -40,26 +40,23 @@ constexpr int LA_THREADS = 320;
 constexpr int LA_ROW_WARP = 2;        // first of the eight row warps
 constexpr int LA_ROW_WARPS = 8;
 constexpr int LA_STAGE = LA_KEYS * 128;  // 64 columns of a K or V tile
-constexpr int LA_MIN_RUN = 2;         // shortest run (in costs) worth a CTA
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
 
 template <int D>
 struct LaShape {
   static constexpr int SLICES = D / 64;  // stages of a tile
   static constexpr int Q_BYTES = LA_ROWS * D * 2;
-  static constexpr int PER_SM = D == 256 ? 1 : 2;
-  static constexpr int STAGES = D == 256 ? 10 : D == 128 ? 5 : 6;
-  static constexpr int S_BUFS = D == 256 ? 2 : 1;
-  static constexpr int TMEM_COLS = D == 256 ? 512 : 256;  // O: D columns, then S_BUFS x 128
+  static constexpr int STAGES = D == 256 ? 10 : 12;
+  static constexpr int TMEM_COLS = 512;  // O: D columns, then two S buffers of 128
   // Shared memory besides the operands: barriers and the tensor-memory address, the row threads' exchange, and the row
-  // warps' copies of plan and walk (which they need only between pieces: kept in registers they were spilled
-  // inside the loop over tiles). 1 KB in all for heads of 128, two of whose CTAs fill an SM's shared memory to the byte.
+  // warps' copies of plan and walk (which they need only between pieces: kept in registers they were spilled inside the
+  // loop over tiles).
   static constexpr int BARRIERS = 2 * STAGES + 10;
   static constexpr int EXCHANGE_AT = (BARRIERS * 8 + 4 + 63) / 64 * 64, PLAN_AT = EXCHANGE_AT + LA_ROWS * 4;
   static constexpr int WALK_AT = PLAN_AT + 64, WALK_BYTES = 32;
   static constexpr int SMALL = WALK_AT + LA_ROW_WARPS * WALK_BYTES;
   static constexpr int SMEM = Q_BYTES + STAGES * LA_STAGE + SMALL;
-  static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024 && SMEM <= 227 * 1024, "the CTAs of an SM fit it");
+  static_assert(SMEM <= 227 * 1024, "a CTA fits an SM");
 };
 
 struct LaArgs {
@@ -123,7 +120,7 @@ struct LaPlan {
     const long long all = (long long)cost * a.Hkv;
     fits = y.z == a.G && y.w == a.B && T == a.T && all < 0x40000000;
     total = fits ? (int)all : 0;
-    per = max((int)((unsigned)(total + a.runs - 1) / (unsigned)a.runs), LA_MIN_RUN);
+    per = max((int)((unsigned)(total + a.runs - 1) / (unsigned)a.runs), 1);
     runs = (unsigned)(total + per - 1) / (unsigned)per;
   }
   D3_DEV LaUnit unit(int u) const {
@@ -253,7 +250,7 @@ D3_DEV void la_commit(uint32_t elected, uint64_t* bar) {
 #define LA_V8(r, o) \
   "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
 
-// 32 columns of this warp's 32 lanes. The wait is part of the statement, so that nothing reads the registers
+// 32 or 64 columns of this warp's 32 lanes. The wait is part of the statement, so that nothing reads the registers
 // ahead of it.
 D3_DEV void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -261,6 +258,16 @@ D3_DEV void tmem_ld32(uint32_t taddr, uint32_t* r) {
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : LA_R8(r, 0), LA_R8(r, 8), LA_R8(r, 16), LA_R8(r, 24)
+      : "r"(taddr)
+      : "memory");
+}
+D3_DEV void tmem_ld64(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
+      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : LA_R8(r, 0), LA_R8(r, 8), LA_R8(r, 16), LA_R8(r, 24), LA_R8(r, 32), LA_R8(r, 40), LA_R8(r, 48), LA_R8(r, 56)
       : "r"(taddr)
       : "memory");
 }
@@ -374,7 +381,7 @@ struct LaLimited { static constexpr bool value = true; };
 struct LaWhole { static constexpr bool value = false; };
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
+__global__ void __launch_bounds__(LA_THREADS, 1)
     lines_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap, LaArgs a) {
   using S = LaShape<D>;
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
   LaWalk w(plan, run, probe);
 
   if (warp == 0) {
-    // ---- loads: a piece's Q, then K0, V0, K1, V1, ... (two S buffers: K0, K1, V0, K2, V1, ...)
+    // ---- loads: a piece's Q, then K0, K1, V0, K2, V1, ...
     uint32_t seq = 0, pieces = 0;
     bool ok = true;
     int win_first = 0, win_page = -1;  // a window of 32 page ids, one per lane
@@ -483,14 +490,10 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
           t.page_id = -1;  // outside the map: zeros
         }
         fetch(&kmap, w.h, t);
-        if (S::S_BUFS == 1) {
-          if (ok) fetch(&vmap, w.h, t);
-        } else {
-          if (ok && i > 0) fetch(&vmap, w.h, before);
-          before = t;
-        }
+        if (ok && i > 0) fetch(&vmap, w.h, before);
+        before = t;
       }
-      if (S::S_BUFS == 2 && ok) fetch(&vmap, w.h, before);
+      if (ok) fetch(&vmap, w.h, before);
     }
     // nothing may land after the CTA is gone: a stage's last load has arrived once its phase is complete
     if (pieces > 0) mbar_wait(q_full, (pieces - 1) & 1);
@@ -507,7 +510,7 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
     const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(ring)),
                    v_desc = la_v_desc(smem_u32(ring));  // addresses are in 16-byte units: sums stay within 14 bits
     auto scores = [&](uint32_t tile, bool last) {
-      const uint32_t d = tmem_s + 128 * (tile % S::S_BUFS);
+      const uint32_t d = tmem_s + 128 * (tile % 2);
 #pragma unroll
       for (int sl = 0; sl < S::SLICES; ++sl) {
         const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
@@ -520,32 +523,28 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
         la_commit(elected, kv_empty + st);
       }
       if (last) la_commit(elected, q_empty);
-      la_commit(elected, s_full + tile % S::S_BUFS);
+      la_commit(elected, s_full + tile % 2);
     };
-    // S of a tile goes where P of an earlier one is (with one buffer, the last one's): the tensor core takes a CTA's
-    // products in the order in which they were issued, and O += P V of that tile was issued before
+    // S of tile t + 1 goes where P of tile t - 1 is: the tensor core takes a CTA's products in the order in which they were
+    // issued, and O += P V of tile t - 1 was issued before
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
       if (!(ok = la_warp_wait(q_full, pieces & 1))) break;
       ++pieces;
       tc_fence_after();
       scores(tiles, w.n == 1);
       for (int i = 0; ok && i < w.n; ++i, ++tiles) {
-        if (S::S_BUFS == 2 && i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
-        const uint32_t buf = tiles % S::S_BUFS;
-        // V (and the next K) before P, for which the wait is long: the products then follow one another
+        if (i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
+        const uint32_t buf = tiles % 2;
+        // V before P, for which the wait is long: the products then follow one another
         const uint32_t v0 = seq;
         seq += S::SLICES;
 #pragma unroll
         for (int sl = 0; sl < S::SLICES; ++sl)
           ok = ok && la_warp_wait(kv_full + (v0 + sl) % S::STAGES, ((v0 + sl) / S::STAGES) & 1);
-        if (S::S_BUFS == 1 && i + 1 < w.n)
-#pragma unroll
-          for (int sl = 0; sl < S::SLICES; ++sl)
-            ok = ok && la_warp_wait(kv_full + (seq + sl) % S::STAGES, ((seq + sl) / S::STAGES) & 1);
-        // the product by halves of the keys, as their weights come: keys 32 .. 63 and 96 .. 127, then the others
+        // the product by halves of the keys, as their weights come: keys 0 .. 31 and 64 .. 95, then the others
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          if (!ok || !(ok = la_warp_wait(p_full + 2 * buf + part, (tiles / S::S_BUFS) & 1))) break;
+          if (!ok || !(ok = la_warp_wait(p_full + 2 * buf + part, (tiles / 2) & 1))) break;
           tc_fence_after();
 #pragma unroll
           for (int sl = 0; sl < S::SLICES; ++sl) {
@@ -553,7 +552,7 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
             const uint64_t vb = v_desc + st * (LA_STAGE >> 4);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int c = (x & 1) + 4 * (x >> 1) + 2 * (1 - part);  // 16 keys
+              const int c = (x & 1) + 4 * (x >> 1) + 2 * part;  // 16 keys
               la_mma_ts(elected, tmem_o + 64 * sl, tmem_s + 128 * buf + 32 * (c >> 1) + 8 * (c & 1), vb + (c * 2048 >> 4),
                         idesc_o, i > 0 || part > 0 || x > 0);
             }
@@ -562,7 +561,6 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
         }
         if (!ok) break;
         la_commit(elected, o_full + (tiles & 1));
-        if (S::S_BUFS == 1 && i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
       }
     }
   } else {
@@ -605,13 +603,13 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
       }
       float m = -INFINITY, l = 0.0f;  // of the row; of this thread's keys
       for (int i = 0; i < n; ++i, ++tiles) {
-        const uint32_t buf = tiles % S::S_BUFS;
-        if (!(ok = la_warp_wait(s_full + buf, (tiles / S::S_BUFS) & 1))) break;
+        const uint32_t buf = tiles % 2;
+        if (!(ok = la_warp_wait(s_full + buf, (tiles / 2) & 1))) break;
         tc_fence_after();
         const int valid = (i < n_shared ? shared_end : own_end) - i * LA_KEYS;  // keys of this tile, if not all
         if (valid < LA_KEYS) {
           // V's rows past the end, in the stages of this tile's V
-          const uint32_t vs = seq + S::SLICES * (S::S_BUFS == 1 ? 2 * i + 1 : i + 1 < n ? 2 * i + 2 : 2 * n - 1);
+          const uint32_t vs = seq + S::SLICES * (i + 1 < n ? 2 * i + 2 : 2 * n - 1);
           for (int sl = 0; ok && sl < S::SLICES; ++sl) {
             const uint32_t st = (vs + sl) % S::STAGES;
             if (!(ok = la_warp_wait(kv_full + st, ((vs + sl) / S::STAGES) & 1))) break;
@@ -629,32 +627,23 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
           // Two forms of the same steps, with and without a limit inside the tile, chosen by the whole warp: with the
           // comparisons in the one form every tile paid for them.
           const bool cut_tile = __any_sync(0xffffffffu, lim < 64);
-          uint32_t s[32];
-          // 32 keys' scores (-inf past the limit)
-          auto load = [&](int c, auto limited) {
-            tmem_ld32(s_at + c, s);
-            if constexpr (decltype(limited)::value) {
+          uint32_t s[64];
+          auto maximum = [&](auto limited) {
+            tmem_ld64(s_at, s);
+            if constexpr (decltype(limited)::value) {  // -inf past the limit
 #pragma unroll
-              for (int x = 0; x < 32; ++x)
-                if (c + x >= lim) s[x] = 0xff800000u;
+              for (int x = 0; x < 64; ++x)
+                if (x >= lim) s[x] = 0xff800000u;
             }
-          };
-          auto top = [&]() {
             float t[4];  // four chains
 #pragma unroll
             for (int x = 0; x < 4; ++x) t[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 4]));
 #pragma unroll
-            for (int x = 8; x < 32; x += 8)
+            for (int x = 8; x < 64; x += 8)
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 t[y] = la_max3(t[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
-            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-          };
-          auto maximum = [&](auto limited) {
-            load(0, limited);
-            const float first = top();
-            load(32, limited);
-            return fmaxf(first, top()) * a.scale_log2;
+            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * a.scale_log2;
           };
           const float mx = cut_tile ? maximum(LaLimited{}) : maximum(LaWhole{});
           if (la_any(1 + quarter, 64, i == 0 || mx > m + LA_RESCALE || (m == -INFINITY && mx > m))) {
@@ -687,7 +676,8 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
             uint32_t p[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
-              const uint64_t y = f2_fma(f2_make(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, base2);
+              const uint64_t y =
+                  f2_fma(f2_make(__uint_as_float(s[c + x]), __uint_as_float(s[c + x + 1])), scale2, base2);
               float p0, p1;
               if (!decltype(limited)::value && x / 2 % 4 == 1) {  // a pair in four
                 la_exp2_poly(y, p0, p1);
@@ -705,10 +695,9 @@ __global__ void __launch_bounds__(LA_THREADS, LaShape<D>::PER_SM)
             __syncwarp();
           };
           auto weights = [&](auto limited) {
-            weigh(32, limited);  // still in registers
-            if (lane == 0) mbar_arrive(p_full + 2 * buf);
-            load(0, limited);
             weigh(0, limited);
+            if (lane == 0) mbar_arrive(p_full + 2 * buf);
+            weigh(32, limited);
             if (lane == 0) mbar_arrive(p_full + 2 * buf + 1);
           };
           if (cut_tile)

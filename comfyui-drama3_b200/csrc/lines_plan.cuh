@@ -31,7 +31,7 @@ constexpr int LP_MAX_KEPT = 1 << 30;  // lengths are clamped to it, so no index 
 // what a unit costs besides (its queries, its results) LA_UNIT_COST; the attention cuts that line into equal runs.
 constexpr int LA_ROWS = 128;
 constexpr int LA_KEYS = 128;
-constexpr int LA_UNIT_COST = 1;
+constexpr int LA_UNIT_COST = 3;
 // Most rows of a KV head (T * group) whose prefix and own units may be apart: each row then keeps two fp32 partial
 // rows per KV head in the attention's workspace (136 MB at 4 KV heads of 128).
 constexpr int LA_APART_ROWS = 32768;

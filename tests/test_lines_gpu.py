@@ -125,7 +125,7 @@ def test_work_list_covers_every_row_and_key(cuda, group, lengths, counts, prefix
     total, tile = sum(counts), 128 // group
     together = work[0] == 1
     assert work[3] == prefix and work[5] == total and work[6] == group
-    keys, unit_cost = 128, 1  # of a key tile; what a unit costs besides its tiles
+    keys, unit_cost = 128, 3  # of a key tile; what a unit costs besides its tiles
     place, own, shared = 0, [], []
     for line, token0, rows, at, tiles, sees, own_end, lead in units:
         assert at == place + unit_cost and tiles >= 1
