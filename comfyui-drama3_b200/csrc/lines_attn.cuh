@@ -11,16 +11,19 @@
 // lines_join_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
 // key is read once for all lines.
 //
-// Per CTA (320 threads, one per SM):
-//   warp 0     loads by TMA (128-byte swizzle) into a ring of 16 KB stages, a stage being 64 columns of a tile's 128
-//              keys of K or V: a box per page, a lane each. A page outside the cache reads as zeros (the map's fill).
-//              A unit's queries likewise, into a buffer of their own.
-//   warp 1     issues the MMAs and owns the tensor memory: S = Q K^T (128 x 128, two buffers, a tile ahead of the rows), O
-//              += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so it is the
-//              MN-major operand)
-//   warps 2-9  two threads own a row, 64 of a tile's keys each: S from tensor memory, mask, maximum, exponentials, P
-//              back over S, the row's sum. O is rescaled only when the maximum has grown by more than 2^8 since the
-//              last time (p <= 256 in between, the same value after the division). They also write the results.
+// Per CTA (352 threads, one per SM):
+//   warp 0     loads by TMA (128-byte swizzle) into a ring of stages, a stage being 128 columns (64 for heads of 64) of a
+//              tile's 128 keys of K or V: a box per page and 64 columns, a lane each. A page outside the cache reads as
+//              zeros (the map's fill). A unit's queries likewise, into a buffer of their own.
+//   warp 1     owns the tensor memory and issues S = Q K^T (128 x 128) into three buffers by turns (two for heads of 256,
+//              whose O takes half of the tensor memory)
+//   warps 2-9  two groups, each with a thread for every row, take the tiles by turns, so that one group's exponentials run
+//              under the other's waits: S from tensor memory, mask, maximum, exponentials, P back over S, the row's
+//              sum. A row's running maximum goes from group to group through shared memory; O is rescaled only when it has
+//              grown by more than 2^8 since the last time (p <= 256 in between, the same value after the division). They
+//              also write the results, half of the columns each.
+//   warp 10    issues O += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so it
+//              is the MN-major operand)
 // Loads and first products of a run's next unit go on while the row warps write this one's results.
 // Keys of a tile past the end of the prefix or of the line are masked in S, and their V rows are cleared in shared
 // memory before the product, since the cache may hold anything there (0 x NaN is NaN).
@@ -36,26 +39,32 @@
 
 namespace d3 {
 
-constexpr int LA_THREADS = 320;
+constexpr int LA_THREADS = 352;
 constexpr int LA_ROW_WARP = 2;        // first of the eight row warps
 constexpr int LA_ROW_WARPS = 8;
-constexpr int LA_STAGE = LA_KEYS * 128;  // 64 columns of a K or V tile
+constexpr int LA_PV_WARP = LA_ROW_WARP + LA_ROW_WARPS;
+constexpr int LA_SLICE = LA_KEYS * 128;  // 64 columns of a K or V tile
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
 
 template <int D>
 struct LaShape {
-  static constexpr int SLICES = D / 64;  // stages of a tile
+  // Columns of a stage, and of a product with V: 64 of them take as long as 128, and every stage costs the warp that
+  // issues the products a wait and a commit.
+  static constexpr int COLUMNS = D == 64 ? 64 : 128, PER_STAGE = COLUMNS / 64;
+  static constexpr int STAGE = PER_STAGE * LA_SLICE;
+  static constexpr int SLICES = D / COLUMNS;  // stages of a tile
   static constexpr int Q_BYTES = LA_ROWS * D * 2;
-  static constexpr int STAGES = D == 256 ? 10 : 12;
-  static constexpr int TMEM_COLS = 512;  // O: D columns, then two S buffers of 128
+  static constexpr int STAGES = D == 256 ? 5 : D == 128 ? 6 : 12;
+  static constexpr int S_BUFS = D == 256 ? 2 : 3;
+  static constexpr int TMEM_COLS = 512;  // O: D columns, then the S buffers of 128
   // Shared memory besides the operands: barriers and the tensor-memory address, the row threads' exchange, and the row
   // warps' copies of plan and walk (which they need only between pieces: kept in registers they were spilled inside the
   // loop over tiles).
-  static constexpr int BARRIERS = 2 * STAGES + 10;
-  static constexpr int EXCHANGE_AT = (BARRIERS * 8 + 4 + 63) / 64 * 64, PLAN_AT = EXCHANGE_AT + LA_ROWS * 4;
+  static constexpr int BARRIERS = 2 * STAGES + 3 * S_BUFS + 19;
+  static constexpr int EXCHANGE_AT = (BARRIERS * 8 + 4 + 63) / 64 * 64, PLAN_AT = EXCHANGE_AT + LA_ROWS * 16;
   static constexpr int WALK_AT = PLAN_AT + 64, WALK_BYTES = 32;
   static constexpr int SMALL = WALK_AT + LA_ROW_WARPS * WALK_BYTES;
-  static constexpr int SMEM = Q_BYTES + STAGES * LA_STAGE + SMALL;
+  static constexpr int SMEM = Q_BYTES + STAGES * STAGE + SMALL;
   static_assert(SMEM <= 227 * 1024, "a CTA fits an SM");
 };
 
@@ -195,10 +204,10 @@ D3_DEV int la_tile(const LaPlan& p, const LaUnit& u, int j, bool& own, int& vali
   return key0;
 }
 
-// Shared-memory descriptor of a V stage as the MMA's B: MN-major (columns contiguous), 128-byte swizzle, atoms of 8
-// keys x 64 columns 1024 bytes apart (SBO); N is one atom wide, so that LBO is not used.
+// Shared-memory descriptor of V stages as the MMA's B: MN-major (columns contiguous), 128-byte swizzle, atoms of 8
+// keys x 64 columns 1024 bytes apart along the keys (SBO) and LA_SLICE apart along the columns (LBO).
 D3_DEV uint64_t la_v_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(LA_STAGE >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(LA_SLICE >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
@@ -323,20 +332,6 @@ D3_DEV float la_exp2(float x) {
   return y;
 }
 
-// Whether any of the `threads` threads that meet at named barrier `id` says yes; the barrier's threads all get the answer.
-D3_DEV bool la_any(int id, int threads, bool yes) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-      "selp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)yes), "r"(id), "r"(threads)
-      : "memory");
-  return r != 0;
-}
-
 D3_DEV float la_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -388,7 +383,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t la_smem[];
   uint8_t* q_s = la_smem;
   uint8_t* ring = la_smem + S::Q_BYTES;
-  uint64_t* bars = (uint64_t*)(la_smem + S::Q_BYTES + S::STAGES * LA_STAGE);
+  uint64_t* bars = (uint64_t*)(la_smem + S::Q_BYTES + S::STAGES * S::STAGE);
   uint8_t* small = (uint8_t*)bars;
   LaPlan* plan_s = (LaPlan*)(small + S::PLAN_AT);
   LaWalk* walk_s = (LaWalk*)(small + S::WALK_AT) + (threadIdx.x >> 5) - LA_ROW_WARP;
@@ -397,10 +392,13 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
   uint64_t* kv_empty = kv_full + S::STAGES;    // [STAGES]
   uint64_t* q_full = kv_empty + S::STAGES;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;              // [2]
-  uint64_t* p_full = s_full + 2;               // [2][2], by halves of the keys
-  uint64_t* o_full = p_full + 4;               // [2], by tile parity: a waiter may be up to two products behind
-  uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+  uint64_t* s_full = q_empty + 1;              // [S_BUFS]
+  uint64_t* p_full = s_full + S::S_BUFS;       // [S_BUFS][2], by halves of the keys
+  uint64_t* o_full = p_full + 2 * S::S_BUFS;   // [4], of tiles by turns: a waiter may be up to three products behind
+  uint64_t* o_empty = o_full + 4;
+  uint64_t* m_full = o_empty + 1;              // [2][4], by group and quarter
+  uint64_t* l_full = m_full + 8;               // [4]
+  uint32_t* tmem_slot = (uint32_t*)(l_full + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = blockIdx.x;
   const bool aligned = (smem_u32(la_smem) & 1023u) == 0;  // the swizzle's atoms
   if (tid == 0) {
@@ -410,12 +408,15 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::S_BUFS; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + 2 * i, LA_ROW_WARPS);
-      mbar_init(p_full + 2 * i + 1, LA_ROW_WARPS);
-      mbar_init(o_full + i, 1);
+      mbar_init(p_full + 2 * i, LA_ROW_WARPS / 2);
+      mbar_init(p_full + 2 * i + 1, LA_ROW_WARPS / 2);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(o_full + i, 1);
+    mbar_init(o_empty, LA_ROW_WARPS);
+    for (int i = 0; i < 8; ++i) mbar_init(m_full + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(l_full + i, 2);
     fence_mbar_init();
   }
   // tensor memory only once the grids before this one are done: a CTA that held some while it waited for them could
@@ -436,9 +437,10 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
     if (tid == 0) record_fault(FAULT_PLAN);
   }
   LaWalk w(plan, run, probe);
+  const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);  // of the products' operands
 
   if (warp == 0) {
-    // ---- loads: a piece's Q, then K0, K1, V0, K2, V1, ...
+    // ---- loads: a piece's Q, then K0, K1, K2, V0, K3, V1, ... (with two S buffers K0, K1, V0, K2, V1, ...)
     uint32_t seq = 0, pieces = 0;
     bool ok = true;
     int win_first = 0, win_page = -1;  // a window of 32 page ids, one per lane
@@ -453,21 +455,23 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
         ++seq;
         if (!(ok = la_warp_wait(kv_empty + st, ph ^ 1))) return;
-        if (lane == 0) mbar_arrive_expect_tx(kv_full + st, t.n * a.page_box * 128);
+        if (lane == 0) mbar_arrive_expect_tx(kv_full + st, t.n * a.page_box * 128 * S::PER_STAGE);
         __syncwarp();
         if (lane < t.n)
-          tma_load_4d(smem_u32(ring) + st * LA_STAGE + lane * a.page_box * 128, map, sl * 64, t.in_page, h, t.page_id,
-                      kv_full + st);
+#pragma unroll
+          for (int y = 0; y < S::PER_STAGE; ++y)
+            tma_load_4d(smem_u32(ring) + st * S::STAGE + y * LA_SLICE + lane * a.page_box * 128, map,
+                        sl * S::COLUMNS + y * 64, t.in_page, h, t.page_id, kv_full + st);
       }
     };
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
       if (!(ok = la_warp_wait(q_empty, (pieces & 1) ^ 1))) break;
       ++pieces;
-      if (lane == 0) mbar_arrive_expect_tx(q_full, q_bytes * S::SLICES);
+      if (lane == 0) mbar_arrive_expect_tx(q_full, q_bytes * (D / 64));
       __syncwarp();
-      if (lane < S::SLICES)
+      if (lane < D / 64)
         tma_load_3d(smem_u32(q_s) + lane * (LA_ROWS * 128), &qmap, lane * 64, w.h * a.G, unit.token0, q_full);
-      Boxes before = {};
+      Boxes before[S::S_BUFS - 1] = {};  // tiles whose V is to come, the last one first
       for (int i = 0; ok && i < w.n; ++i) {
         bool own;
         int valid;
@@ -490,82 +494,94 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           t.page_id = -1;  // outside the map: zeros
         }
         fetch(&kmap, w.h, t);
-        if (ok && i > 0) fetch(&vmap, w.h, before);
-        before = t;
+        if (ok && i >= S::S_BUFS - 1) fetch(&vmap, w.h, before[S::S_BUFS - 2]);
+#pragma unroll
+        for (int x = S::S_BUFS - 2; x > 0; --x) before[x] = before[x - 1];
+        before[0] = t;
       }
-      if (ok) fetch(&vmap, w.h, before);
+#pragma unroll
+      for (int x = S::S_BUFS - 2; x >= 0; --x)
+        if (ok && x < w.n) fetch(&vmap, w.h, before[x]);
     }
     // nothing may land after the CTA is gone: a stage's last load has arrived once its phase is complete
     if (pieces > 0) mbar_wait(q_full, (pieces - 1) & 1);
     for (uint32_t i = seq < (uint32_t)S::STAGES ? 0 : seq - S::STAGES; i < seq; ++i)
       mbar_wait(kv_full + i % S::STAGES, (i / S::STAGES) & 1);
   } else if (warp == 1) {
-    // ---- MMAs
-    const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
-    const uint32_t idesc_s = (1u << 4) | type | ((LA_KEYS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
-    const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((64 >> 3) << 17) | ((LA_ROWS >> 4) << 24);
+    // ---- S = Q K^T, up to S_BUFS - 1 tiles ahead of O
+    const uint32_t idesc = (1u << 4) | type | ((LA_KEYS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
     const uint32_t elected = la_elect();
-    uint32_t seq = 0, tiles = 0, pieces = 0;
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(ring));
+    uint32_t seq = 0, tile = 0, pieces = 0;
     bool ok = true;
-    const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(ring)),
-                   v_desc = la_v_desc(smem_u32(ring));  // addresses are in 16-byte units: sums stay within 14 bits
-    auto scores = [&](uint32_t tile, bool last) {
-      const uint32_t d = tmem_s + 128 * (tile % 2);
-#pragma unroll
-      for (int sl = 0; sl < S::SLICES; ++sl) {
-        const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
-        ++seq;
-        if (!(ok = la_warp_wait(kv_full + st, ph))) return;
-        tc_fence_after();
-        const uint64_t kb = k_desc + st * (LA_STAGE >> 4), qb = q_desc + sl * (LA_ROWS * 128 >> 4);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) la_mma_ss(elected, d, qb + 2 * c, kb + 2 * c, idesc_s, sl > 0 || c > 0);
-        la_commit(elected, kv_empty + st);
-      }
-      if (last) la_commit(elected, q_empty);
-      la_commit(elected, s_full + tile % 2);
-    };
-    // S of tile t + 1 goes where P of tile t - 1 is: the tensor core takes a CTA's products in the order in which they were
-    // issued, and O += P V of tile t - 1 was issued before
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
       if (!(ok = la_warp_wait(q_full, pieces & 1))) break;
       ++pieces;
-      tc_fence_after();
-      scores(tiles, w.n == 1);
-      for (int i = 0; ok && i < w.n; ++i, ++tiles) {
-        if (i + 1 < w.n) scores(tiles + 1, i + 2 == w.n);
-        const uint32_t buf = tiles % 2;
-        // V before P, for which the wait is long: the products then follow one another
-        const uint32_t v0 = seq;
-        seq += S::SLICES;
+      for (int i = 0; ok && i < w.n; ++i, ++tile) {
+        const uint32_t d = tmem_s + 128 * (tile % S::S_BUFS), done = tile - S::S_BUFS;
+        // where P of the tile S_BUFS before was
+        if (tile >= (uint32_t)S::S_BUFS && !(ok = la_warp_wait(o_full + done % 4, (done / 4) & 1))) break;
+        const uint32_t k0 = seq + S::SLICES * (i + max(0, i - (S::S_BUFS - 1)));
+#pragma unroll
+        for (int sl = 0; sl < S::SLICES; ++sl) {
+          const uint32_t st = (k0 + sl) % S::STAGES;
+          if (!ok || !(ok = la_warp_wait(kv_full + st, ((k0 + sl) / S::STAGES) & 1))) break;
+          tc_fence_after();
+          const uint64_t kb = k_desc + st * (S::STAGE >> 4), qb = q_desc + sl * S::PER_STAGE * (LA_ROWS * 128 >> 4);
+#pragma unroll
+          for (int y = 0; y < S::PER_STAGE; ++y)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              la_mma_ss(elected, d, qb + y * (LA_ROWS * 128 >> 4) + 2 * c, kb + y * (LA_SLICE >> 4) + 2 * c, idesc,
+                        sl > 0 || y > 0 || c > 0);
+          la_commit(elected, kv_empty + st);
+        }
+        if (!ok) break;
+        if (i + 1 == w.n) la_commit(elected, q_empty);
+        la_commit(elected, s_full + tile % S::S_BUFS);
+      }
+      seq += 2 * S::SLICES * w.n;
+    }
+  } else if (warp == LA_PV_WARP) {
+    // ---- O += P V
+    const uint32_t idesc = (1u << 4) | type | (1u << 16) | ((S::COLUMNS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
+    const uint32_t elected = la_elect();
+    const uint64_t v_desc = la_v_desc(smem_u32(ring));  // in 16-byte units: sums stay within 14 bits
+    uint32_t seq = 0, tile = 0, pieces = 0;
+    bool ok = true;
+    for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
+      ++pieces;
+      for (int i = 0; ok && i < w.n; ++i, ++tile) {
+        const uint32_t buf = tile % S::S_BUFS, v0 = seq + S::SLICES * (min(w.n, i + S::S_BUFS) + i);
 #pragma unroll
         for (int sl = 0; sl < S::SLICES; ++sl)
           ok = ok && la_warp_wait(kv_full + (v0 + sl) % S::STAGES, ((v0 + sl) / S::STAGES) & 1);
-        // the product by halves of the keys, as their weights come: keys 0 .. 31 and 64 .. 95, then the others
+        if (i == 0) ok = ok && la_warp_wait(o_empty, pieces & 1);  // the rows have read the O before it
+        // the product by halves of the keys, as their weights come: keys 64 .. 127, then the others
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          if (!ok || !(ok = la_warp_wait(p_full + 2 * buf + part, (tiles / 2) & 1))) break;
+          if (!ok || !(ok = la_warp_wait(p_full + 2 * buf + part, (tile / S::S_BUFS) & 1))) break;
           tc_fence_after();
 #pragma unroll
           for (int sl = 0; sl < S::SLICES; ++sl) {
             const uint32_t st = (v0 + sl) % S::STAGES;
-            const uint64_t vb = v_desc + st * (LA_STAGE >> 4);
+            const uint64_t vb = v_desc + st * (S::STAGE >> 4);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int c = (x & 1) + 4 * (x >> 1) + 2 * part;  // 16 keys
-              la_mma_ts(elected, tmem_o + 64 * sl, tmem_s + 128 * buf + 32 * (c >> 1) + 8 * (c & 1), vb + (c * 2048 >> 4),
-                        idesc_o, i > 0 || part > 0 || x > 0);
+              const int c = x + 4 * (1 - part);  // 16 keys
+              la_mma_ts(elected, tmem_o + S::COLUMNS * sl, tmem_s + 128 * buf + 32 * (c >> 1) + 8 * (c & 1),
+                        vb + (c * 2048 >> 4), idesc, i > 0 || part > 0 || x > 0);
             }
             if (part == 1) la_commit(elected, kv_empty + st);
           }
         }
-        if (!ok) break;
-        la_commit(elected, o_full + (tiles & 1));
+        if (ok) la_commit(elected, o_full + tile % 4);
       }
+      seq += 2 * S::SLICES * w.n;
     }
   } else {
     // ---- rows
-    const int quarter = warp & 3, half = (warp - LA_ROW_WARP) >> 2;  // tensor-memory lanes; keys 64 half .. + 63
+    const int quarter = warp & 3, group = (warp - LA_ROW_WARP) >> 2;  // tensor-memory lanes; tiles of its parity
     const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
     const int row = 32 * quarter + lane, tok = row / a.G, g = row - tok * a.G;
     if (lane == 0) {
@@ -576,11 +592,10 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
       *walk_s = w;
     }
     named_sync(9, 32 * LA_ROW_WARPS);
-    // between a row's two threads: their maxima (as bfloat16, rounded to nearest: any number near the maximum serves,
-    // if both take the same), or a sum
-    uint16_t* maxima = (uint16_t*)(small + S::EXCHANGE_AT) + 2 * row;
-    float* total = (float*)(small + S::EXCHANGE_AT) + row;
-    uint32_t seq = 0, tiles = 0;
+    // between a row's two threads: the running maximum, of pieces by turns, and their sums
+    float* m_s = (float*)(small + S::EXCHANGE_AT) + row;
+    float* l_s = m_s + 2 * LA_ROWS;
+    uint32_t seq = 0, tiles = 0, pieces = 0;
     bool ok = true;
     while (ok) {
       int n, n_shared;  // tiles of the piece, and those of them that are the prefix's
@@ -601,41 +616,54 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         own_sees = unit.sees + tok - (w.j0 - unit.lead) * LA_KEYS;
         any = 32 * quarter < unit.rows;
       }
-      float m = -INFINITY, l = 0.0f;  // of the row; of this thread's keys
-      for (int i = 0; i < n; ++i, ++tiles) {
-        const uint32_t buf = tiles % 2;
-        if (!(ok = la_warp_wait(s_full + buf, (tiles / 2) & 1))) break;
+      float* m_row = m_s + (pieces & 1) * LA_ROWS;
+      // this thread's sum, and the maximum that it refers to
+      float m = -INFINITY, l = 0.0f;
+      auto refer = [&](float to) {
+        if (to != m) {
+          l *= m == -INFINITY ? 0.0f : la_exp2(m - to);
+          m = to;
+        }
+      };
+      for (int i = (tiles ^ group) & 1; i < n; i += 2) {
+        const uint32_t tile = tiles + i, buf = tile % S::S_BUFS;
+        if (!(ok = la_warp_wait(s_full + buf, (tile / S::S_BUFS) & 1))) break;
         tc_fence_after();
         const int valid = (i < n_shared ? shared_end : own_end) - i * LA_KEYS;  // keys of this tile, if not all
         if (valid < LA_KEYS) {
           // V's rows past the end, in the stages of this tile's V
-          const uint32_t vs = seq + S::SLICES * (i + 1 < n ? 2 * i + 2 : 2 * n - 1);
+          const uint32_t vs = seq + S::SLICES * (min(n, i + S::S_BUFS) + i);
           for (int sl = 0; ok && sl < S::SLICES; ++sl) {
             const uint32_t st = (vs + sl) % S::STAGES;
             if (!(ok = la_warp_wait(kv_full + st, ((vs + sl) / S::STAGES) & 1))) break;
-            for (int r = valid + 4 * (warp - LA_ROW_WARP) + (lane >> 3); r < LA_KEYS; r += 4 * LA_ROW_WARPS)
-              *(uint4*)(ring + st * LA_STAGE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            for (int r = valid + 4 * quarter + (lane >> 3); r < LA_KEYS; r += 2 * LA_ROW_WARPS)
+#pragma unroll
+              for (int y = 0; y < S::PER_STAGE; ++y)
+                *(uint4*)(ring + st * S::STAGE + y * LA_SLICE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           if (!ok) break;
           fence_async_smem();
           __syncwarp();
         }
         if (any) {
-          const uint32_t s_at = tmem_s + lanes + 128 * buf + 64 * half;
-          // of this thread's 64 keys, those that there are and that its row sees
-          const int lim = (i < n_shared ? valid : own_sees - i * LA_KEYS) - 64 * half;
+          const uint32_t s_at = tmem_s + lanes + 128 * buf;
+          // of the tile's keys, those that there are and that this row sees
+          const int lim = i < n_shared ? valid : own_sees - i * LA_KEYS;
           // Two forms of the same steps, with and without a limit inside the tile, chosen by the whole warp: with the
           // comparisons in the one form every tile paid for them.
-          const bool cut_tile = __any_sync(0xffffffffu, lim < 64);
+          const bool cut_tile = __any_sync(0xffffffffu, lim < LA_KEYS);
           uint32_t s[64];
-          auto maximum = [&](auto limited) {
-            tmem_ld64(s_at, s);
+          auto load = [&](int key, auto limited) {
+            tmem_ld64(s_at + key, s);
             if constexpr (decltype(limited)::value) {  // -inf past the limit
 #pragma unroll
               for (int x = 0; x < 64; ++x)
-                if (x >= lim) s[x] = 0xff800000u;
+                if (key + x >= lim) s[x] = 0xff800000u;
             }
+          };
+          auto maximum = [&](auto limited) {
             float t[4];  // four chains
+            load(0, limited);
 #pragma unroll
             for (int x = 0; x < 4; ++x) t[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 4]));
 #pragma unroll
@@ -643,36 +671,44 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 t[y] = la_max3(t[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
+            load(64, limited);
+#pragma unroll
+            for (int x = 0; x < 64; x += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                t[y] = la_max3(t[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
             return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * a.scale_log2;
           };
-          const float mx = cut_tile ? maximum(LaLimited{}) : maximum(LaWhole{});
-          if (la_any(1 + quarter, 64, i == 0 || mx > m + LA_RESCALE || (m == -INFINITY && mx > m))) {
-            maxima[half] = __bfloat16_as_ushort(__float2bfloat16_rn(mx));
-            named_sync(1 + quarter, 64);
-            const uint32_t both = *(const uint32_t*)maxima;
-            const float t = fmaxf(m, fmaxf(bf16_to_f32(both & 0xffffu), bf16_to_f32(both >> 16)));
-            const float f = m == -INFINITY ? 0.0f : la_exp2(m - t);
-            m = t;
-            l *= f;
-            if (i > 0) {
-              if (!(ok = la_warp_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
-              tc_fence_after();
+          float top = cut_tile ? maximum(LaLimited{}) : maximum(LaWhole{});
+          float before = -INFINITY;
+          if (i > 0) {
+            if (!(ok = la_warp_wait(m_full + 4 * (1 - group) + quarter, ((tile - 1) >> 1) & 1))) break;
+            before = *m_row;
+            if (!(top > before + LA_RESCALE || (before == -INFINITY && top > before))) top = before;
+          }
+          *m_row = top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(m_full + 4 * group + quarter);
+          refer(top);
+          if (i > 0 && __any_sync(0xffffffffu, top != before)) {
+            const float f = top == before ? 1.0f : before == -INFINITY ? 0.0f : la_exp2(before - top);
+            if (!(ok = la_warp_wait(o_full + (tile - 1) % 4, ((tile - 1) / 4) & 1))) break;
+            tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 2; c += 32) {  // each of the two warps half of the columns
-                uint32_t o[32];
-                const uint32_t at = tmem_o + lanes + half * (D / 2) + c;
-                tmem_ld32(at, o);
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              const uint32_t at = tmem_o + lanes + c;
+              tmem_ld32(at, o);
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                tmem_st32(at, o);
-              }
-              tmem_wait_st();
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(at, o);
             }
+            tmem_wait_st();
           }
           const float base = m == -INFINITY ? 0.0f : m;
           const uint64_t scale2 = f2_make(a.scale_log2, a.scale_log2), base2 = f2_make(-base, -base);
           uint64_t sums[2] = {0, 0};
-          auto weigh = [&](int c, auto limited) {
+          auto weigh = [&](int key, int c, auto limited) {  // s[c] is key `key`
             uint32_t p[16];
 #pragma unroll
             for (int x = 0; x < 32; x += 2) {
@@ -689,16 +725,19 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
               sums[x / 2 & 1] = f2_add(sums[x / 2 & 1], f2_make(p0, p1));
               p[x / 2] = la_pack<F16>(p0, p1);
             }
-            tmem_st16(s_at + c, p);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
+            tmem_st16(s_at + key, p);
           };
           auto weights = [&](auto limited) {
-            weigh(0, limited);
-            if (lane == 0) mbar_arrive(p_full + 2 * buf);
-            weigh(32, limited);
-            if (lane == 0) mbar_arrive(p_full + 2 * buf + 1);
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {  // keys 64 .. 127, still in registers, then the others
+              if (part == 1) load(0, limited);
+              weigh(64 * (1 - part), 0, limited);
+              weigh(64 * (1 - part) + 32, 32, limited);
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_full + 2 * buf + part);
+            }
           };
           if (cut_tile)
             weights(LaLimited{});
@@ -708,21 +747,26 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           f2_split(f2_add(sums[0], sums[1]), s0, s1);
           l += s0 + s1;
         } else if (lane == 0) {
+          mbar_arrive(m_full + 4 * group + quarter);
           mbar_arrive(p_full + 2 * buf);
           mbar_arrive(p_full + 2 * buf + 1);
         }
       }
       if (!ok) break;
       seq += 2 * S::SLICES * n;
-      if (!(ok = la_warp_wait(o_full + ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1))) break;
+      tiles += n;
+      const uint32_t end = tiles - 1;
+      if (!(ok = la_warp_wait(o_full + end % 4, (end / 4) & 1))) break;
       tc_fence_after();
-      if (any) {  // the row's sum: both threads', the same order in both
-        if (half == 1) *total = l;
-        named_sync(1 + quarter, 64);
-        if (half == 0) *total = l += *total;
-        named_sync(1 + quarter, 64);
-        l = *total;
-      }
+      if (!(ok = la_warp_wait(m_full + 4 * (end & 1) + quarter, (end >> 1) & 1))) break;
+      // the row's sum: both threads', the same order in both
+      if (any) refer(*m_row);
+      l_s[group * LA_ROWS] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(l_full + quarter);
+      if (!(ok = la_warp_wait(l_full + quarter, pieces & 1))) break;
+      l = l_s[0] + l_s[LA_ROWS];
+      ++pieces;
       // results: a whole unit's rows are done; a part's go to the workspace
       const LaPlan plan = *plan_s;
       LaWalk w = *walk_s;
@@ -744,7 +788,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           a.joints[run] = make_int4(unit.token0, unit.rows, w.h, (from + unit.tiles - 1) / plan.per);
       }
       if (any) {
-        const int t = unit.token0 + tok, head = w.h * a.G + g;
+        const int t = unit.token0 + tok, head = w.h * a.G + g, half = group;  // a thread takes half of the columns
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
 #pragma unroll 1
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
@@ -767,7 +811,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
               dst[32 * x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           }
         }
-        if (live && half == 0) {
+        if (live && group == 0) {
           if (!whole)
             a.part_ml[part] = make_float2(m, l);
           else if (a.lse)
@@ -777,7 +821,10 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
       tc_fence_before();
       w.step(plan);
       __syncwarp();
-      if (lane == 0) *walk_s = w;
+      if (lane == 0) {
+        mbar_arrive(o_empty);
+        *walk_s = w;
+      }
       __syncwarp();
     }
     // tokens of no line: nothing to see
