@@ -12,7 +12,8 @@
 // each other one places LP_TOKENS tokens, and all write units of the work list, a thread each: a unit's place follows from
 // its number by a closed sum. A page is written into its table by the token that opens it, and read only from entries
 // that were there before, so no two threads race. The state that a pass advances (lengths, used) goes to fresh outputs:
-// planning the same pass twice gives the same plan.
+// planning the same pass twice gives the same plan. Measured (B200): a token each for 16 lines 4.7 us; 1024 lines of up to
+// 512 tokens in pages of 16 (5.4 MB written) 15 us.
 #pragma once
 
 #include "common.cuh"
@@ -28,7 +29,9 @@ constexpr int LP_MAX_KEPT = 1 << 30;  // lengths are clamped to it, so no index 
 // The attention's work list. A unit is a tile of rows, a row being a token and one of the `group` query heads of a KV
 // head: la_tile_tokens(group) whole tokens, LA_ROWS rows at most; and the key tiles of LA_KEYS that these rows attend
 // to. The list is the same for every KV head. Units lie end to end on a line of costs on which a key tile takes 1 and
-// what a unit costs besides (its queries, its results) LA_UNIT_COST; the attention cuts that line into equal runs.
+// what a unit costs besides (its queries, its results) LA_UNIT_COST; the attention cuts that line into equal runs. (8192
+// tokens of a prompt: 680 us with a cost of 1, whose first runs of a head, of many short units, were late; 601 with 2,
+// 565 with 3, 556 with 4, which makes 64 lines of a token each behind 32768 2 % slower than 3.)
 constexpr int LA_ROWS = 128;
 constexpr int LA_KEYS = 128;
 constexpr int LA_UNIT_COST = 3;
