@@ -616,7 +616,9 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         tc_fence_after();
         const int valid = (i < n_shared ? shared_end : own_end) - i * LA_KEYS;  // keys of this tile, if not all
         if (valid < LA_KEYS) {
-          // V's rows past the end, in the stages of this tile's V
+          // V's rows past the end, in the stages of this tile's V. A wait for a phase passes, too, while the phase before
+          // it is not complete: where the last tile's V may still be coming into one of these stages, its product first.
+          if (S::SLICES > 1 && !(ok = la_warp_wait(o_full + (tile - 1) % 4, ((tile - 1) / 4) & 1))) break;
           const uint32_t vs = seq + S::SLICES * (min(n, i + S::S_BUFS) + i);
           for (int sl = 0; ok && sl < S::SLICES; ++sl) {
             const uint32_t st = (vs + sl) % S::STAGES;
