@@ -11,32 +11,33 @@
 // lines_join_kernel joins. With few tokens a line the rows of all lines share the prefix's tiles, so that a prefix
 // key is read once for all lines.
 //
-// Per CTA (352 threads, one per SM):
-//   warp 0     loads by TMA (128-byte swizzle) into a ring of stages, a stage being 128 columns (64 for heads of 64) of a
-//              tile's 128 keys of K or V: a box per page and 64 columns, a lane each. A page outside the cache reads as
-//              zeros (the map's fill). A unit's queries likewise, into a buffer of their own.
-//   warp 1     owns the tensor memory and issues S = Q K^T (128 x 128) into three buffers by turns (two for heads of 256,
-//              whose O takes half of the tensor memory)
-//   warps 2-9  two groups, each with a thread for every row, take the tiles by turns, so that one group's exponentials run
-//              under the other's waits: S from tensor memory, mask, maximum, exponentials, P back over S, the row's
-//              sum. A row's running maximum goes from group to group through shared memory; O is rescaled only when it has
-//              grown by more than 2^8 since the last time (p <= 256 in between, the same value after the division). They
-//              also write the results, half of the columns each.
-//   warp 10    issues O += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so it
-//              is the MN-major operand)
+// Per CTA (384 threads, one per SM):
+//   warps 0, 11  load by TMA (128-byte swizzle), K and V, each into a ring of stages of its own, a stage being 128
+//              columns (64 for heads of 64) of a tile's 128 keys: a box per page and 64 columns, a lane each. A page outside
+//              the cache reads as zeros (the map's fill). Warp 0 loads a unit's queries too, into a buffer of their own.
+//   warp 1     owns the tensor memory and issues S = Q K^T (128 x 128) into three buffers by turns (two for heads of
+//              256, whose O takes half of the tensor memory)
+//   warps 2-9  two groups, each with a thread for every row, take the tiles by turns, so that one group's exponentials
+//              run under the other's waits: S from tensor memory, mask, maximum, exponentials, P back over S, the row's
+//              sum. A row's running maximum goes from group to group through shared memory; O is rescaled only when it
+//              has grown by more than 2^8 since the last time (p <= 256 in between, the same value after the division).
+//              They also write the results, half of the columns each.
+//   warp 10    issues O += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so
+//              it is the MN-major operand)
 // Loads and first products of a run's next unit go on while the row warps write this one's results.
 // Keys of a tile past the end of the prefix or of the line are masked in S, and their V rows are cleared in shared
 // memory before the product, since the cache may hold anything there (0 x NaN is NaN).
 // Every wait is bounded (2 s) and records FAULT_WAIT_TIMEOUT instead of hanging.
 //
-// Measured (B200, bf16, 32 query heads over 4 KV heads of 128; device time): 8192 tokens of a prompt 557 us, 987 TFLOP/s;
-// 16 texts of up to 192 tokens behind 4096 138 us, 844 TFLOP/s; 64 lines, a token each, behind 32768 65 us, 3.0 TB/s;
-// 16 lines behind 4096 14.4 us; one line of 1000 10.4 us. With full runs a tile takes about 1650 clocks, 1024 of them
-// of the tensor cores: a group's steps (2800 a tile, two groups) and the issue of a tile's loads (1750) are both near
-// that, and either halved alone gave 11 % and 3 %. A unit takes about 6000 clocks besides. With few keys the time is
-// latency: about 4 us until the first scores, 2 us a tile, 3 us for the results and the join.
-// Other forms of the same tiles: two threads a row, one group, 70 us for the 64 lines and 153 for the texts; two CTAs
-// per SM with one S buffer each 74 and 165; part of the exponentials as polynomials, the same times as without.
+// Measured (B200, bf16, 32 query heads over 4 KV heads of 128; device time): 8192 tokens of a prompt 544 us, 1010 TFLOP/s;
+// 16 texts of up to 192 tokens behind 4096 138 us, 840 TFLOP/s; 64 lines, a token each, behind 32768 65 us, 3.1 TB/s;
+// 16 lines behind 4096 14.4 us; one line of 1000 10.6 us. With full runs a tile takes about 1600 clocks, 1024 of them
+// of the tensor cores: a group's steps (2800 a tile, two groups) are near that. A unit takes about 6000 clocks besides.
+// With few keys the time is latency: about 4 us until the first scores, 2 us a tile, 3 us for the results and the join.
+// Other forms of the same tiles: one warp that loads both K and V, 1750 clocks a tile, 546 to 578 us for the prompt in
+// turn with 539 to 556 for two, heads of 256 (16 lines behind 3001 in pages of 16) 16.6 us against 15.7; two threads a
+// row, one group, 70 us for the 64 lines and 153 for the texts; two CTAs per SM with one S buffer each 74 and 165; part
+// of the exponentials as polynomials, the same times as without.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -48,10 +49,11 @@
 
 namespace d3 {
 
-constexpr int LA_THREADS = 352;
+constexpr int LA_THREADS = 384;
 constexpr int LA_ROW_WARP = 2;        // first of the eight row warps
 constexpr int LA_ROW_WARPS = 8;
-constexpr int LA_PV_WARP = LA_ROW_WARP + LA_ROW_WARPS;
+constexpr int LA_PV_WARP = LA_ROW_WARP + LA_ROW_WARPS;  // issues the products with V
+constexpr int LA_V_WARP = LA_PV_WARP + 1;                // loads V
 constexpr int LA_SLICE = LA_KEYS * 128;  // 64 columns of a K or V tile
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
 
@@ -63,7 +65,8 @@ struct LaShape {
   static constexpr int STAGE = PER_STAGE * LA_SLICE;
   static constexpr int SLICES = D / COLUMNS;  // stages of a tile
   static constexpr int Q_BYTES = LA_ROWS * D * 2;
-  static constexpr int STAGES = D == 256 ? 5 : D == 128 ? 6 : 12;
+  static constexpr int K_STAGES = D == 256 ? 2 : D == 128 ? 3 : 6, V_STAGES = D == 64 ? 6 : 3;
+  static constexpr int STAGES = K_STAGES + V_STAGES;  // first the ring of K, then that of V
   static constexpr int S_BUFS = D == 256 ? 2 : 3;
   static constexpr int TMEM_COLS = 512;  // O: D columns, then the S buffers of 128
   // Shared memory besides the operands: barriers and the tensor-memory address, the row threads' exchange, and the row
@@ -375,6 +378,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
   static_assert(sizeof(LaPlan) <= 64 && sizeof(LaWalk) == S::WALK_BYTES, "layout");
   uint64_t* kv_full = bars;                    // [STAGES]
   uint64_t* kv_empty = kv_full + S::STAGES;    // [STAGES]
+  uint64_t* v_full = kv_full + S::K_STAGES;
   uint64_t* q_full = kv_empty + S::STAGES;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;              // [S_BUFS]
@@ -424,45 +428,30 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
   LaWalk w(plan, run, probe);
   const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);  // of the products' operands
 
-  if (warp == 0) {
-    // ---- loads: a piece's Q, then K0, K1, K2, V0, K3, V1, ... (with two S buffers K0, K1, V0, K2, V1, ...)
-    uint32_t seq = 0, pieces = 0;
+  if (warp == 0 || warp == LA_V_WARP) {
+    // ---- loads: warp 0 a piece's Q and K of its tiles, the other V
+    const bool is_v = warp != 0;
+    const CUtensorMap* map = is_v ? &vmap : &kmap;
+    const uint32_t stages = is_v ? S::V_STAGES : S::K_STAGES, stage0 = is_v ? S::K_STAGES : 0;
+    uint32_t st = 0, ph = 0, loads = 0, pieces = 0;
     bool ok = true;
     int win_first = 0, win_page = -1;  // a window of 32 page ids, one per lane
     const int* win_table = nullptr;
     const uint32_t q_bytes = (uint32_t)(la_tile_tokens(a.G) * a.G * 128);  // of a 64-column slice
-    struct Boxes {  // a tile's: lane l issues box l
-      int n, page_id, in_page;
-    };
-    auto fetch = [&](const CUtensorMap* map, int h, const Boxes& t) {
-#pragma unroll
-      for (int sl = 0; sl < S::SLICES; ++sl) {
-        const uint32_t st = seq % S::STAGES, ph = (seq / S::STAGES) & 1;
-        ++seq;
-        if (!(ok = la_warp_wait(kv_empty + st, ph ^ 1))) return;
-        if (lane == 0) mbar_arrive_expect_tx(kv_full + st, t.n * a.page_box * 128 * S::PER_STAGE);
-        __syncwarp();
-        if (lane < t.n)
-#pragma unroll
-          for (int y = 0; y < S::PER_STAGE; ++y)
-            tma_load_4d(smem_u32(ring) + st * S::STAGE + y * LA_SLICE + lane * a.page_box * 128, map,
-                        sl * S::COLUMNS + y * 64, t.in_page, h, t.page_id, kv_full + st);
-      }
-    };
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
-      if (!(ok = la_warp_wait(q_empty, (pieces & 1) ^ 1))) break;
-      ++pieces;
-      if (lane == 0) mbar_arrive_expect_tx(q_full, q_bytes * (D / 64));
-      __syncwarp();
-      if (lane < D / 64)
-        tma_load_3d(smem_u32(q_s) + lane * (LA_ROWS * 128), &qmap, lane * 64, w.h * a.G, unit.token0, q_full);
-      Boxes before[S::S_BUFS - 1] = {};  // tiles whose V is to come, the last one first
+      if (!is_v) {
+        if (!(ok = la_warp_wait(q_empty, (pieces & 1) ^ 1))) break;
+        ++pieces;
+        if (lane == 0) mbar_arrive_expect_tx(q_full, q_bytes * (D / 64));
+        __syncwarp();
+        if (lane < D / 64)
+          tma_load_3d(smem_u32(q_s) + lane * (LA_ROWS * 128), &qmap, lane * 64, w.h * a.G, unit.token0, q_full);
+      }
       for (int i = 0; ok && i < w.n; ++i) {
         bool own;
         int valid;
         const int key0 = la_tile(plan, unit, w.j0 + i, own, valid);
-        Boxes t;
-        t.n = (valid + a.page_box - 1) / a.page_box;
+        const int boxes = (valid + a.page_box - 1) / a.page_box;  // lane l issues box l
         const int key = key0 + lane * a.page_box, first = key0 / a.page, last = (key0 + valid - 1) / a.page;
         const int* table = own ? a.table + (size_t)unit.line * a.W : a.prefix_table;
         const int width = own ? a.W : a.PW;
@@ -472,32 +461,41 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           win_page = first + lane < width ? table[first + lane] : -1;
         }
         const int index = key / a.page;
-        t.in_page = key - index * a.page;
-        t.page_id = __shfl_sync(0xffffffffu, win_page, (index - win_first) & 31);
-        if (lane < t.n && (t.page_id < 0 || t.page_id >= a.pages)) {
+        const int in_page = key - index * a.page;
+        int page_id = __shfl_sync(0xffffffffu, win_page, (index - win_first) & 31);
+        if (lane < boxes && (page_id < 0 || page_id >= a.pages)) {
           record_fault(FAULT_PAGES);
-          t.page_id = -1;  // outside the map: zeros
+          page_id = -1;  // outside the map: zeros
         }
-        fetch(&kmap, w.h, t);
-        if (ok && i >= S::S_BUFS - 1) fetch(&vmap, w.h, before[S::S_BUFS - 2]);
 #pragma unroll
-        for (int x = S::S_BUFS - 2; x > 0; --x) before[x] = before[x - 1];
-        before[0] = t;
+        for (int sl = 0; ok && sl < S::SLICES; ++sl) {
+          uint64_t* full = kv_full + stage0 + st;
+          if (!(ok = la_warp_wait(kv_empty + stage0 + st, ph ^ 1))) break;
+          if (lane == 0) mbar_arrive_expect_tx(full, boxes * a.page_box * 128 * S::PER_STAGE);
+          __syncwarp();
+          if (lane < boxes)
+#pragma unroll
+            for (int y = 0; y < S::PER_STAGE; ++y)
+              tma_load_4d(smem_u32(ring) + (stage0 + st) * S::STAGE + y * LA_SLICE + lane * a.page_box * 128, map,
+                          sl * S::COLUMNS + y * 64, in_page, w.h, page_id, full);
+          ++loads;
+          if (++st == stages) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
       }
-#pragma unroll
-      for (int x = S::S_BUFS - 2; x >= 0; --x)
-        if (ok && x < w.n) fetch(&vmap, w.h, before[x]);
     }
     // nothing may land after the CTA is gone: a stage's last load has arrived once its phase is complete
     if (pieces > 0) mbar_wait(q_full, (pieces - 1) & 1);
-    for (uint32_t i = seq < (uint32_t)S::STAGES ? 0 : seq - S::STAGES; i < seq; ++i)
-      mbar_wait(kv_full + i % S::STAGES, (i / S::STAGES) & 1);
+    for (uint32_t i = loads < stages ? 0 : loads - stages; i < loads; ++i)
+      mbar_wait(kv_full + stage0 + i % stages, (i / stages) & 1);
   } else if (warp == 1) {
     // ---- S = Q K^T, up to S_BUFS - 1 tiles ahead of O
     const uint32_t idesc = (1u << 4) | type | ((LA_KEYS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
     const uint32_t elected = la_elect();
     const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s)), k_desc = umma_desc_sw128(smem_u32(ring));
-    uint32_t seq = 0, tile = 0, pieces = 0;
+    uint32_t tile = 0, pieces = 0;
     bool ok = true;
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
       if (!(ok = la_warp_wait(q_full, pieces & 1))) break;
@@ -506,11 +504,11 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         const uint32_t d = tmem_s + 128 * (tile % S::S_BUFS), done = tile - S::S_BUFS;
         // where P of the tile S_BUFS before was
         if (tile >= (uint32_t)S::S_BUFS && !(ok = la_warp_wait(o_full + done % 4, (done / 4) & 1))) break;
-        const uint32_t k0 = seq + S::SLICES * (i + max(0, i - (S::S_BUFS - 1)));
+        const uint32_t k0 = S::SLICES * tile;
 #pragma unroll
         for (int sl = 0; sl < S::SLICES; ++sl) {
-          const uint32_t st = (k0 + sl) % S::STAGES;
-          if (!ok || !(ok = la_warp_wait(kv_full + st, ((k0 + sl) / S::STAGES) & 1))) break;
+          const uint32_t st = (k0 + sl) % S::K_STAGES;
+          if (!ok || !(ok = la_warp_wait(kv_full + st, ((k0 + sl) / S::K_STAGES) & 1))) break;
           tc_fence_after();
           const uint64_t kb = k_desc + st * (S::STAGE >> 4), qb = q_desc + sl * S::PER_STAGE * (LA_ROWS * 128 >> 4);
 #pragma unroll
@@ -525,22 +523,21 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         if (i + 1 == w.n) la_commit(elected, q_empty);
         la_commit(elected, s_full + tile % S::S_BUFS);
       }
-      seq += 2 * S::SLICES * w.n;
     }
   } else if (warp == LA_PV_WARP) {
     // ---- O += P V
     const uint32_t idesc = (1u << 4) | type | (1u << 16) | ((S::COLUMNS >> 3) << 17) | ((LA_ROWS >> 4) << 24);
     const uint32_t elected = la_elect();
-    const uint64_t v_desc = la_v_desc(smem_u32(ring));  // in 16-byte units: sums stay within 14 bits
-    uint32_t seq = 0, tile = 0, pieces = 0;
+    const uint64_t v_desc = la_v_desc(smem_u32(ring) + S::K_STAGES * S::STAGE);  // in 16-byte units: sums stay within 14 bits
+    uint32_t tile = 0, pieces = 0;
     bool ok = true;
     for (LaUnit unit; ok && w.next(plan, unit); w.step(plan)) {
       ++pieces;
       for (int i = 0; ok && i < w.n; ++i, ++tile) {
-        const uint32_t buf = tile % S::S_BUFS, v0 = seq + S::SLICES * (min(w.n, i + S::S_BUFS) + i);
+        const uint32_t buf = tile % S::S_BUFS, v0 = S::SLICES * tile;
 #pragma unroll
         for (int sl = 0; sl < S::SLICES; ++sl)
-          ok = ok && la_warp_wait(kv_full + (v0 + sl) % S::STAGES, ((v0 + sl) / S::STAGES) & 1);
+          ok = ok && la_warp_wait(v_full + (v0 + sl) % S::V_STAGES, ((v0 + sl) / S::V_STAGES) & 1);
         if (i == 0) ok = ok && la_warp_wait(o_empty, pieces & 1);  // the rows have read the O before it
         // the product by halves of the keys, as their weights come: keys 64 .. 127, then the others
 #pragma unroll
@@ -549,7 +546,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           tc_fence_after();
 #pragma unroll
           for (int sl = 0; sl < S::SLICES; ++sl) {
-            const uint32_t st = (v0 + sl) % S::STAGES;
+            const uint32_t st = (v0 + sl) % S::V_STAGES;
             const uint64_t vb = v_desc + st * (S::STAGE >> 4);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -557,12 +554,11 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
               la_mma_ts(elected, tmem_o + S::COLUMNS * sl, tmem_s + 128 * buf + 32 * (c >> 1) + 8 * (c & 1),
                         vb + (c * 2048 >> 4), idesc, i > 0 || part > 0 || x > 0);
             }
-            if (part == 1) la_commit(elected, kv_empty + st);
+            if (part == 1) la_commit(elected, kv_empty + S::K_STAGES + st);
           }
         }
         if (ok) la_commit(elected, o_full + tile % 4);
       }
-      seq += 2 * S::SLICES * w.n;
     }
   } else {
     // ---- rows
@@ -580,7 +576,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
     // between a row's two threads: the running maximum, of pieces by turns, and their sums
     float* m_s = (float*)(small + S::EXCHANGE_AT) + row;
     float* l_s = m_s + 2 * LA_ROWS;
-    uint32_t seq = 0, tiles = 0, pieces = 0;
+    uint32_t tiles = 0, pieces = 0;
     bool ok = true;
     while (ok) {
       int n, n_shared;  // tiles of the piece, and those of them that are the prefix's
@@ -619,14 +615,14 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
           // V's rows past the end, in the stages of this tile's V. A wait for a phase passes, too, while the phase before
           // it is not complete: where the last tile's V may still be coming into one of these stages, its product first.
           if (S::SLICES > 1 && !(ok = la_warp_wait(o_full + (tile - 1) % 4, ((tile - 1) / 4) & 1))) break;
-          const uint32_t vs = seq + S::SLICES * (min(n, i + S::S_BUFS) + i);
+          const uint32_t vs = S::SLICES * tile;
           for (int sl = 0; ok && sl < S::SLICES; ++sl) {
-            const uint32_t st = (vs + sl) % S::STAGES;
-            if (!(ok = la_warp_wait(kv_full + st, ((vs + sl) / S::STAGES) & 1))) break;
+            const uint32_t st = (vs + sl) % S::V_STAGES;
+            if (!(ok = la_warp_wait(v_full + st, ((vs + sl) / S::V_STAGES) & 1))) break;
             for (int r = valid + 4 * quarter + (lane >> 3); r < LA_KEYS; r += 2 * LA_ROW_WARPS)
 #pragma unroll
               for (int y = 0; y < S::PER_STAGE; ++y)
-                *(uint4*)(ring + st * S::STAGE + y * LA_SLICE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                *(uint4*)(ring + (S::K_STAGES + st) * S::STAGE + y * LA_SLICE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           if (!ok) break;
           fence_async_smem();
@@ -736,7 +732,6 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
         }
       }
       if (!ok) break;
-      seq += 2 * S::SLICES * n;
       tiles += n;
       const uint32_t end = tiles - 1;
       if (!(ok = la_warp_wait(o_full + end % 4, (end / 4) & 1))) break;
