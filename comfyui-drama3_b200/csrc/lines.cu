@@ -127,9 +127,9 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
   DeviceInfo d;
   if (int st = device_info(&d)) return st;
   const int smem = 4 * (B + 1) * 4;
+  // asked for whatever B is: 48 KB hold the kernel's own static arrays too, so the limit is below 48 KB of these
   static std::atomic<uint64_t> done{0};
-  if (smem > 48 * 1024)
-    if (int st = allow_smem_once(d3::lines_plan_kernel, 4 * (d3::LP_MAX_LINES + 1) * 4, done)) return st;
+  if (int st = allow_smem_once(d3::lines_plan_kernel, 4 * (d3::LP_MAX_LINES + 1) * 4, done)) return st;
   const d3::LinesPlanArgs a = {kept, counts, B, table, W, free_pages, F, used, prefix, page, T, group, slots, positions,
                                line, cu, lengths, used_out, work};
   return launch(d3::lines_plan_kernel, dim3(1 + (T + d3::LP_TOKENS - 1) / d3::LP_TOKENS), dim3(d3::LP_THREADS), smem,
