@@ -117,7 +117,7 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
                   const int* used, const int* prefix, int page, int T, int group, int64_t* slots, int64_t* positions,
                   int* line, int* cu, int* lengths, int* used_out, int* work, size_t work_ints, void* stream) {
   if (B < 1 || B > d3::LP_MAX_LINES || W < 1 || F < 0 || page < 1 || T < 0 || group < 1 || group > d3::LA_ROWS ||
-      (long long)T * group > (1ll << 30))
+      (long long)T * group > d3::LP_MAX_TOKENS)
     return D3_ERR_ARG;
   if (!kept || !counts || !table || (F > 0 && !free_pages) || !used || !cu || !lengths || !used_out || !work ||
       (T > 0 && (!slots || !positions || !line)))

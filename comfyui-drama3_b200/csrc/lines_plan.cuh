@@ -24,7 +24,8 @@ constexpr int LP_THREADS = 512;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOKENS = 2048;     // tokens placed by a block
 constexpr int LP_MAX_LINES = 8192;  // four int arrays of it fill 128 KB of shared memory
-constexpr int LP_MAX_KEPT = 1 << 30;  // lengths are clamped to it, so no index below overflows
+constexpr int LP_MAX_TOKENS = 1 << 30;          // of a pass
+constexpr int LP_MAX_KEPT = LP_MAX_TOKENS - 1;  // lengths are clamped to it: with a pass's tokens they fit 32 bits
 
 // The attention's work list. A unit is a tile of rows, a row being a token and one of the `group` query heads of a KV
 // head: la_tile_tokens(group) whole tokens, LA_ROWS rows at most; and the key tiles of LA_KEYS that these rows attend
@@ -153,17 +154,18 @@ D3_DEV long long lp_floor_sum(long long n, long long m, long long a, long long b
   }
 }
 
+// ceil(n / of): unsigned, since n + of - 1 may pass 2^31 where n and of do not.
+D3_DEV int lp_parts(int n, int of) { return (int)(((unsigned)n + (unsigned)of - 1u) / (unsigned)of); }
+
 // What the first i units of a line cost: its tokens in tiles of `tile` (the last one shorter), each tile's key tiles up to
 // its last token behind `lead` of the prefix.
 D3_DEV long long lp_cost(int i, int n, int kept, int count, int tile, int lead) {
   if (i == 0) return 0;
   const int whole = i == n ? n - 1 : i;
   long long tiles = lp_floor_sum(whole, LA_KEYS, tile, (long long)kept + tile + LA_KEYS - 1);
-  if (i == n) tiles += (kept + count + LA_KEYS - 1) / LA_KEYS;
+  if (i == n) tiles += lp_parts(kept + count, LA_KEYS);
   return tiles + (long long)i * (lead + LA_UNIT_COST);
 }
-
-D3_DEV int lp_clamped(const int* p, int b) { return min(max(0, p[b]), LP_MAX_KEPT); }
 
 __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a) {
   extern __shared__ int lp_smem[];
@@ -180,21 +182,21 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
   {
     int* const out[1] = {cu};
     lp_scan_lines<1>(B, out, a.T, sums1, [&](int b, long long (&v)[1]) {
-      v[0] = lp_clamped(a.counts, b);
-      kept_of[b] = lp_clamped(a.kept, b);
+      v[0] = max(0, a.counts[b]);
+      kept_of[b] = min(max(0, a.kept[b]), LP_MAX_KEPT);
     });
   }
   {
     int* const out[2] = {first, unit0};
     lp_scan_lines<2>(B, out, 0x7fffffffLL, sums2, [&](int b, long long (&v)[2]) {
       const int kept = kept_of[b], n = cu[b + 1] - cu[b], p = a.page;
-      v[0] = (kept + n + p - 1) / p - (kept + p - 1) / p;
-      v[1] = (n + tile - 1) / tile;
+      v[0] = lp_parts(kept + n, p) - lp_parts(kept, p);
+      v[1] = lp_parts(n, tile);
     });
   }
   const int tokens = cu[B], own_units = unit0[B];
-  const int prefix_tiles = (prefix + LA_KEYS - 1) / LA_KEYS;
-  const int prefix_units = prefix > 0 ? (tokens + tile - 1) / tile : 0;
+  const int prefix_tiles = lp_parts(prefix, LA_KEYS);
+  const int prefix_units = prefix > 0 ? lp_parts(tokens, tile) : 0;
   // The prefix is read once for the rows of all lines together, or by each line's units on the way to its own keys.
   // Apart, the rows of short lines share tiles: a decode step of 16 lines x 8 heads needs one tile instead of 16. But
   // each row's parts are then merged through memory, so lines that fill most of their own tiles go together.
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
         const int kept = kept_of[b];
         unit = u0 + unit0[b] + (t - cu[b]) / tile;
         const int s = kept + t - cu[b], j = s / a.page, off = s - j * a.page;
-        const int have = (kept + a.page - 1) / a.page;
+        const int have = lp_parts(kept, a.page);
         int page = -1;
         if (j < a.W) {
           if (j < have) {
@@ -266,8 +268,8 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
   const long long shared_cost = (long long)u0 * (prefix_tiles + LA_UNIT_COST);
   for (int u = blockIdx.x * LP_THREADS + tid; u < u0 + own_units; u += gridDim.x * LP_THREADS) {
     if (u < u0) {
-      units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G, u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST,
-                        prefix_tiles, 0, 0, prefix_tiles};
+      units[u] = LaUnit{-1, tile * u, min(tile, tokens - tile * u) * G,
+                        (int)((long long)u * (prefix_tiles + LA_UNIT_COST) + LA_UNIT_COST), prefix_tiles, 0, 0, prefix_tiles};
       continue;
     }
     int b = 0, hi = B;  // the last line whose units begin at or before this one: it has it
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
     const int i = u - u0 - unit0[b], n = unit0[b + 1] - unit0[b], count = cu[b + 1] - cu[b], kept = kept_of[b];
     const int from = i * tile, to = min(from + tile, count);
     const int at = (int)(shared_cost + first[b] + lp_cost(i, n, kept, count, tile, lead) + LA_UNIT_COST);
-    units[u] = LaUnit{b, cu[b] + from, (to - from) * G, at, lead + (kept + to + LA_KEYS - 1) / LA_KEYS, kept + from + 1,
+    units[u] = LaUnit{b, cu[b] + from, (to - from) * G, at, lead + lp_parts(kept + to, LA_KEYS), kept + from + 1,
                       kept + to, lead};
   }
   if (blockIdx.x == 0 && tid == 0) {

@@ -277,9 +277,9 @@ int d3_moe_decode_static(int fmt, const void* x, int x_bf16, int M, int k, int E
  * positions (*prefix + the token's number in its line; 0 past the last) and line (-1 past the last); cu [B + 1] the
  * first token of each line; lengths [B] and used_out [1] the state after the pass (kept and used are not changed, so
  * a plan can be made again); work the attention's work list for `group` query heads per KV head,
- * d3_lines_plan_ints() ints. Negative lengths and counts are 0; tokens past T are left out (D3_FAULT_TOKENS); a page
- * past the free list or the table's width is -1 (D3_FAULT_PAGES). prefix may be null (0). B <= 8192, group <= 128,
- * T * group <= 2^30. */
+ * d3_lines_plan_ints() ints. Negative lengths and counts are 0, lengths past 2^30 - 1 are that; tokens past T are left
+ * out (D3_FAULT_TOKENS); a page past the free list or the table's width is -1 (D3_FAULT_PAGES). prefix may be null (0).
+ * B <= 8192, group <= 128, T * group <= 2^30. */
 size_t d3_lines_plan_ints(int B, int T, int group);
 int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, const int* free_pages, int F,
                   const int* used, const int* prefix, int page, int T, int group, int64_t* slots, int64_t* positions,

@@ -6,6 +6,9 @@ from pathlib import Path
 
 import pytest
 
+import lines_ref as ref
+from test_lines_gpu import fault, lines_case, run_plan
+
 pytestmark = pytest.mark.gpu
 
 ROOT = Path(__file__).resolve().parents[1]
@@ -36,3 +39,25 @@ def test_plan_of_line_counts_around_48_kb_of_shared_memory(cuda):
     # in a process of its own: a plan of more lines raises the kernel's ceiling for all later ones
     run = subprocess.run([sys.executable, "-c", FRESH.format(root=str(ROOT))], capture_output=True, text=True, timeout=600)
     assert run.returncode == 0 and run.stdout.endswith("planned\n"), run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("lengths,counts,page,prefix", [
+    ([5, 0], [1, 2], 2 ** 31 - 1, 0), ([2 ** 30 - 1], [3], 2 ** 30, 1), ([7], [2], 16, 2 ** 31 - 1),
+    ([0, 100], [1, 0], 64, 2 ** 31 - 100)])
+def test_plan_of_sums_near_32_bits(cuda, lengths, counts, page, prefix):
+    table, free, used, tokens = lines_case(lengths, counts, page, 1)
+    _, p = run_plan(cuda, lengths, counts, table, free, used, page, tokens, prefix)
+    want = ref.plan(lengths, counts, table, free, used, page, tokens, prefix)
+    for name in ("slots", "positions", "line", "cu", "lengths", "used"):
+        assert getattr(p, name).tolist() == want[name], name
+    assert p.table.tolist() == table and fault() == 0
+    work = p.work.tolist()
+    at, place = (16 + tokens + 3) & ~3, 0
+    assert work[0] == 1 and work[3] == prefix and work[4] == -(-prefix // 128) and work[1] == sum(n > 0 for n in counts)
+    live = [b for b, n in enumerate(counts) if n]
+    for u, b in enumerate(live):  # a unit per line: few tokens, which see the prefix and their own
+        end = lengths[b] + counts[b]
+        tiles = work[4] + -(-end // 128)
+        assert work[at + 8 * u:at + 8 * u + 8] == [b, want["cu"][b], counts[b], place + 3, tiles, lengths[b] + 1, end, work[4]]
+        place += 3 + tiles
+    assert work[2] == place
