@@ -164,7 +164,7 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
   a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.D = D;
   a.qw = q_weight, a.kw = k_weight, a.w_f32 = w_f32, a.w_add = w_add, a.eps = eps;
   a.rotary = (const float2*)rotary, a.rot = rot, a.length = length, a.pos = positions, a.axes = axes;
-  a.axis = axes > 1 ? axis : nullptr;
+  a.axis = axis;
   a.q_out = q_out, a.k_out = k_out, a.share = 1;
   const int64_t vec = 16 / size;
   bool vectors = aligned(q, 16) && aligned(k, 16) && aligned(q_out, 16) && aligned(q_weight, 16) &&

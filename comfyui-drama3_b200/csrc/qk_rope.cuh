@@ -51,7 +51,7 @@ struct QrArgs {
   int rot, length;
   const int64_t* pos;   // [axes, T]
   int axes;
-  const uint8_t* axis;  // [rot / 2], null with one axis
+  const uint8_t* axis;  // [rot / 2], may be null with one axis
   void* q_out;          // [T, Hq, D]
   void* k_out;          // [T, Hkv, D], or null: into the cache
   QrCache kc, vc;

@@ -289,7 +289,7 @@ int d3_lines_plan(const int* kept, const int* counts, int B, int* table, int W, 
  * root mean square (eps added to the mean square) and multiplied by q_weight / k_weight [D] + w_add (of the rows' type,
  * or fp32 with w_f32; null: no norm for that tensor), then its first rot columns turned: pair f, columns (f, f +
  * rot/2), or (2f, 2f + 1) with `pairs`, by (cos, sin) = rotary[positions[axis[f]][t]][f], rotary [length, rot/2, 2]
- * fp32, positions [axes, T], axis [rot/2] (null with one axis; axes <= 4). 32-bit arithmetic, rounded once. q_out
+ * fp32, positions [axes, T], axis [rot/2] (may be null with one axis; axes <= 4). 32-bit arithmetic, rounded once. q_out
  * [T, Hq, D]. With k_out [T, Hkv, D] the keys go there and v and the caches are not used; with k_out null the keys
  * and the rows of v go to slots[t] of the caches (-1: nowhere; past pages * page: nowhere, D3_FAULT_SLOT). Positions
  * outside the table leave their pair unturned (D3_FAULT_POSITION). D <= 1024, rot even and <= D. */

@@ -5,9 +5,10 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 import lines_ref as ref
-from test_lines_gpu import fault, lines_case, run_plan
+from test_lines_gpu import fault, lines_case, rope_inputs, run_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,22 @@ def test_plan_of_sums_near_32_bits(cuda, lengths, counts, page, prefix):
         assert work[at + 8 * u:at + 8 * u + 8] == [b, want["cu"][b], counts[b], place + 3, tiles, lengths[b] + 1, end, work[4]]
         place += 3 + tiles
     assert work[2] == place
+
+
+# ---- qk_norm_rope
+
+@pytest.mark.parametrize("strided", [0, 1])
+def test_norm_rope_axis_past_the_one_row_of_positions(cuda, strided):
+    from drama3_b200 import kernels
+    q, k, v, qw, kw, rotary, pos, _ = rope_inputs(cuda, 6, 4, 2, 128, 64, 1, torch.float32, 3, strided)
+    axes = torch.zeros(32, dtype=torch.uint8, device=cuda)
+    same = kernels.qk_norm_rope(q, k, rotary, pos, q_weight=qw, k_weight=kw)
+    got = kernels.qk_norm_rope(q, k, rotary, pos.view(1, -1), q_weight=qw, k_weight=kw, axes=axes)
+    assert torch.equal(got[0], same[0]) and torch.equal(got[1], same[1]) and fault() == 0
+    axes[5], axes[31] = 1, 255  # rows that the positions do not have: these pairs stay as they are
+    got = kernels.qk_norm_rope(q, k, rotary, pos.view(1, -1), q_weight=qw, k_weight=kw, axes=axes)
+    assert fault() == 128
+    unturned = rotary.clone()
+    unturned[:, [5, 31]] = torch.tensor([1.0, 0.0], device=cuda)
+    want = kernels.qk_norm_rope(q, k, unturned, pos, q_weight=qw, k_weight=kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
