@@ -20,7 +20,8 @@
 //   warps 2-9  two groups, each with a thread for every row, take the tiles by turns, so that one group's exponentials
 //              run under the other's waits: S from tensor memory, mask, maximum, exponentials, P back over S, the row's
 //              sum. A row's running maximum goes from group to group through shared memory; O is rescaled only when it
-//              has grown by more than 2^8 since the last time (p <= 256 in between, the same value after the division).
+//              has grown by more than 2^8 since the last time (p <= 256 in between, the same value after the division;
+//              in float16 p is 2^7 times that, see LA_F16_SHIFT).
 //              They also write the results, half of the columns each.
 //   warp 10    issues O += P V (128 x D, A = P from tensor memory, B = V as it lies in the cache: keys are its rows, so
 //              it is the MN-major operand)
@@ -56,6 +57,10 @@ constexpr int LA_PV_WARP = LA_ROW_WARP + LA_ROW_WARPS;  // issues the products w
 constexpr int LA_V_WARP = LA_PV_WARP + 1;                // loads V
 constexpr int LA_SLICE = LA_KEYS * 128;  // 64 columns of a K or V tile
 constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
+// Where the weights are held in float16 a row's refer to its maximum less this: they are 2^7 to 2^15 times what they
+// weigh (float16 ends below 2^16), and float16's smallest steps, 2^-24, are 2^-31 of the largest weight and less. Against
+// the maximum itself they were 2^-24 of it, and keys of less weight counted as double or as nothing beside a heavy one.
+constexpr float LA_F16_SHIFT = 7.0f;
 
 template <int D>
 struct LaShape {
@@ -660,7 +665,7 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 t[y] = la_max3(t[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
-            return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * a.scale_log2;
+            return fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), a.scale_log2, F16 ? -LA_F16_SHIFT : 0.0f);
           };
           float top = cut_tile ? maximum(LaLimited{}) : maximum(LaWhole{});
           float before = -INFINITY;

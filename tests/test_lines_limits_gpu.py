@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import lines_ref as ref
-from test_lines_gpu import fault, lines_case, rope_inputs, run_plan
+from test_lines_gpu import attn_case, fault, lines_case, rope_inputs, run_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,30 @@ def test_norm_rope_axis_past_the_one_row_of_positions(cuda, strided):
     unturned[:, [5, 31]] = torch.tensor([1.0, 0.0], device=cuda)
     want = kernels.qk_norm_rope(q, k, unturned, pos, q_weight=qw, k_weight=kw)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- lines_attention
+
+@pytest.mark.parametrize("kept,prefix,lines", [(300, 0, 1), (5000, 0, 60), (40, 30000, 3)])
+def test_attention_fp16_small_weights_beside_a_large_one(cuda, kept, prefix, lines):
+    """The weights of all keys but the first are exp(-17.25), under float16's smallest step beside the first one's 1.
+    A weight is rounded by half a unit in the last place, or by half of float16's smallest step, 2^-25, where the largest
+    weight is held as 2^7 or more; so to the tolerance of tests/test_lines_gpu.py comes 2^-32 sum |V|."""
+    from drama3_b200 import kernels
+    D = 64
+    q, kc, vc, plan, pt = attn_case(cuda, 4, 1, D, torch.float16, 128, [kept] * lines, [1] * lines, prefix, poison=False)
+    q[:], kc[:] = 0.0, 0.0
+    q[..., 0] = 17.25
+    vc.abs_()
+    for b in range(lines):
+        first = (pt[0], 0) if prefix else (plan.table[b, 0], 0)
+        kc[int(first[0]), 0, :, 0] = 1.0
+        vc[int(first[0]), 0] = 0.0
+    got, lse = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt, scale=1.0, lse=True)
+    args = ([kept] * lines, [1] * lines, plan.table, prefix, pt, 1.0)
+    want, want_lse, bound = ref.attention(q, kc, vc, *args)
+    total = ref.attention(torch.zeros_like(q), kc, vc, *args)[2] * (prefix + kept + 1)  # equal weights: sum |V| / keys
+    tol = 2.2 * 2.0 ** -11 * bound + 2.0 ** -24 + 2.0 ** -32 * total
+    err = (got.double() - want).abs()
+    assert fault() == 0 and (err <= tol).all(), float((err / tol).max())
+    assert ((lse.double() - want_lse).abs() <= 2e-5 + 2.0 ** -21 * want_lse.abs()).all()
