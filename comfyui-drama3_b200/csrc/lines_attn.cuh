@@ -136,7 +136,8 @@ struct LaPlan {
     // a first probe for find, on its way with the header: where the first 32 units begin
     probe = __ldg(&units[min((int)threadIdx.x & 31, a.units_most - 1)].at) - LA_UNIT_COST;
     const int4 x = __ldg((const int4*)a.work), y = __ldg((const int4*)a.work + 1);
-    const int T = __ldg(a.work + LW_T);
+    const int2 z = __ldg((const int2*)(a.work + LW_T));
+    static_assert(LW_GROUP == 6 && LW_LINES == 7 && LW_T == 8 && LW_PAGE == 9, "as they are read");
     together = x.x != 0;
     units_n = x.y;
     cost = x.z;
@@ -144,7 +145,7 @@ struct LaPlan {
     prefix_tiles = y.x;
     tokens = y.y;
     const long long all = (long long)cost * a.Hkv;
-    fits = y.z == a.G && y.w == a.B && T == a.T && all < 0x40000000;
+    fits = y.z == a.G && y.w == a.B && z.x == a.T && z.y == a.page && all < 0x40000000;
     total = fits ? (int)all : 0;
     per = max((int)((unsigned)(total + a.runs - 1) / (unsigned)a.runs), 1);
     runs = (unsigned)(total + per - 1) / (unsigned)per;

@@ -60,6 +60,7 @@ enum {
   LW_GROUP,
   LW_LINES,
   LW_T,
+  LW_PAGE,
   LW_HEADER = 16
 };
 constexpr int LA_UNIT_INTS = sizeof(LaUnit) / 4;
@@ -294,6 +295,7 @@ __global__ void __launch_bounds__(LP_THREADS) lines_plan_kernel(LinesPlanArgs a)
     w[LW_GROUP] = G;
     w[LW_LINES] = B;
     w[LW_T] = a.T;
+    w[LW_PAGE] = a.page;
   }
 }
 

@@ -200,7 +200,8 @@ def _(q, k, v, rotary, positions, k_cache, v_cache, slots, q_weight=None, k_weig
 def lines_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, work: Tensor, group: int,
                     prefix_table: Optional[Tensor] = None, scale: Optional[float] = None) -> tuple[Tensor, Tensor]:
     """(out, lse) of kernels.lines_attention with a plan's block table and work list (made for `group` query heads per
-    KV head and q's token places)."""
+    KV head, q's token places and the cache's pages; what it was made for stands in the list, and the kernel refuses one that
+    was made for something else)."""
     plan = kernels.LinesPlan(table, q, None, None, None, None, None, work, k_cache.shape[1], group)
     return kernels.lines_attention(q, k_cache, v_cache, plan, prefix_table=prefix_table, scale=scale, lse=True)
 

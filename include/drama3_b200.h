@@ -305,9 +305,11 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
  * which d3_qk_norm_rope (or the caller) has written. Query head h reads KV head h / (Hq / Hkv). Types 0 and 1 (queries
  * and caches alike); sums and softmax in 32 bits. lse [T, Hq] (or null): the log of each row's sum of exponentials.
  * Tokens past the plan's last get zeros (lse -inf). A key past a length is never used, whatever the cache holds there;
- * a page outside the cache reads as zeros (D3_FAULT_PAGES). table, W, work, B: the plan's; the workspace
- * is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128 or 256; page 16, 32 or a multiple of
- * 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and all pointers 16-byte aligned. */
+ * a page outside the cache reads as zeros (D3_FAULT_PAGES). table, W, work, B: the plan's; work has
+ * d3_lines_plan_ints(B, T, Hq / Hkv) ints, and one that was made for another B, T, Hq / Hkv or page is refused on the
+ * device (D3_FAULT_PLAN). The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128
+ * or 256; page 16, 32 or a multiple of 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and
+ * all pointers 16-byte aligned. */
 size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D);
 int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
                        const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,

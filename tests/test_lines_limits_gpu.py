@@ -108,3 +108,13 @@ def test_attention_fp16_small_weights_beside_a_large_one(cuda, kept, prefix, lin
     err = (got.double() - want).abs()
     assert fault() == 0 and (err <= tol).all(), float((err / tol).max())
     assert ((lse.double() - want_lse).abs() <= 2e-5 + 2.0 ** -21 * want_lse.abs()).all()
+
+
+def test_attention_op_refuses_a_cache_of_other_pages(cuda):
+    """The op is given a work list without the sizes that it was made for, except in the list itself."""
+    import drama3_b200.ops  # noqa: F401
+    kept, counts, prefix = [40, 3], [5, 70], 100
+    q, kc, vc, plan, pt = attn_case(cuda, 16, 4, 128, torch.bfloat16, 32, kept, counts, prefix, poison=False)
+    kc, vc = (c.reshape(-1, 16, 4, 128) for c in (kc, vc))  # the same memory as pages of 16
+    torch.ops.drama3_b200.lines_attention(q, kc, vc, plan.table, plan.work, 4, pt)
+    assert fault() == 256
