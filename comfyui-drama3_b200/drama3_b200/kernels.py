@@ -690,6 +690,10 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     if k_cache.device != device or v_cache.device != device or work.device != device:
         raise ValueError(f"lines_attention: every tensor must be on {device}")
     _ints("the plan's table", table, device, B * W)
+    _ints("the plan's work list", work, device, work.numel())
+    if work.numel() != plan_ints(B, T, plan.group):
+        # another pass's list, which the kernel must not read past its end: one of this size that it refuses instead
+        work = torch.zeros(plan_ints(B, T, plan.group), dtype=torch.int32, device=device)
     prefix_pages = 0
     if prefix_table is not None:
         prefix_pages = prefix_table.numel()
