@@ -22,7 +22,7 @@ enum : unsigned {
   FAULT_PAGES = 32u,        // a cache page that is missing or outside the cache: skipped on writing, zeros on reading
   FAULT_TOKENS = 64u,       // the lines append more tokens than the pass holds: the rest was left out
   FAULT_POSITION = 128u,    // a position or axis outside the rotary table: the pair was left unrotated
-  FAULT_PLAN = 256u,        // a plan made for another pass (lines, tokens, heads or pages): nothing was computed
+  FAULT_PLAN = 256u,        // a plan made for another pass (lines, tokens, heads or pages), or too long: zeros
 };
 __device__ unsigned int g_fault;
 

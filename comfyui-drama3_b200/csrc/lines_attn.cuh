@@ -811,16 +811,15 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
       }
       __syncwarp();
     }
-    // tokens of no line: nothing to see
-    if (plan.fits) {
-      const long long total = (long long)(a.T - plan.tokens) * a.Hq;
-      for (long long x = (long long)run * LA_ROW_WARPS + warp - LA_ROW_WARP; x < total;
-           x += (long long)a.runs * LA_ROW_WARPS) {
-        const long long r = (long long)plan.tokens * a.Hq + x;
-        for (int c = lane; c < D / 8; c += 32)
-          *(uint4*)((uint16_t*)a.out + r * D + 8 * c) = make_uint4(0, 0, 0, 0);
-        if (a.lse && lane == 0) a.lse[r] = -INFINITY;
-      }
+    // tokens of no line, or of a plan that does not fit the call: nothing to see
+    const int tokens = plan.fits ? plan.tokens : 0;
+    const long long total = (long long)(a.T - tokens) * a.Hq;
+    for (long long x = (long long)run * LA_ROW_WARPS + warp - LA_ROW_WARP; x < total;
+         x += (long long)a.runs * LA_ROW_WARPS) {
+      const long long r = (long long)tokens * a.Hq + x;
+      for (int c = lane; c < D / 8; c += 32)
+        *(uint4*)((uint16_t*)a.out + r * D + 8 * c) = make_uint4(0, 0, 0, 0);
+      if (a.lse && lane == 0) a.lse[r] = -INFINITY;
     }
   }
   tc_fence_before();

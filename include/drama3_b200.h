@@ -57,7 +57,7 @@ int d3_device_check(void);
  * grouped GEMM given fewer row tiles than its groups need, D3_FAULT_EXCHANGE (16) an expert-parallel exchange area
  * whose geometry does not fit the call, D3_FAULT_PAGES (32) a cache page that is missing or outside the cache,
  * D3_FAULT_TOKENS (64) lines that append more tokens than the pass holds, D3_FAULT_POSITION (128) a position or axis
- * outside the rotary table, D3_FAULT_PLAN (256) an attention given the plan of another pass. No counterpart in the
+ * outside the rotary table, D3_FAULT_PLAN (256) an attention given the plan of another pass, or of one that is too long. No counterpart in the
  * reference, whose kernels do not check indices. */
 #define D3_FAULT_WAIT 1u
 #define D3_FAULT_EXPERT 2u
@@ -307,7 +307,9 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
  * Tokens past the plan's last get zeros (lse -inf). A key past a length is never used, whatever the cache holds there;
  * a page outside the cache reads as zeros (D3_FAULT_PAGES). table, W, work, B: the plan's; work has
  * d3_lines_plan_ints(B, T, Hq / Hkv) ints, and one that was made for another B, T, Hq / Hkv or page is refused on the
- * device (D3_FAULT_PLAN). The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128
+ * device (D3_FAULT_PLAN; zeros, lse -inf). So is a pass of 2^30 or more key tiles in all, counted once for each KV head
+ * and each 128 rows (tokens x Hq / Hkv) that attend to them, and 3 for each such 128 rows: a prompt of about a million
+ * tokens at 32 / 4 heads. The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128
  * or 256; page 16, 32 or a multiple of 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and
  * all pointers 16-byte aligned. */
 size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D);

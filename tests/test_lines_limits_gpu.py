@@ -1,5 +1,6 @@
 """The attention half of a decoder layer on the GPU at the limits of its arguments, where tests of ordinary sizes say
 nothing."""
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -118,3 +119,22 @@ def test_attention_op_refuses_a_cache_of_other_pages(cuda):
     kc, vc = (c.reshape(-1, 16, 4, 128) for c in (kc, vc))  # the same memory as pages of 16
     torch.ops.drama3_b200.lines_attention(q, kc, vc, plan.table, plan.work, 4, pt)
     assert fault() == 256
+
+
+def test_attention_refused_by_the_kernel_gives_rows_of_nothing(cuda, monkeypatch):
+    """A plan that only the GPU can tell to be another pass's: zeros and lse -inf beside the fault bit, not whatever the
+    outputs' memory held."""
+    from drama3_b200 import kernels
+    kept, counts = [60, 20], [1, 1]
+    q, kc, vc, plan, pt = attn_case(cuda, 8, 2, 64, torch.bfloat16, 16, kept, counts, 0, spare=3)
+    empty, empty_like = torch.empty, torch.empty_like
+
+    def filled(t):
+        return t.fill_(math.nan) if t.is_floating_point() else t
+
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: filled(empty(*a, **k)))
+    monkeypatch.setattr(torch, "empty_like", lambda *a, **k: filled(empty_like(*a, **k)))
+    for work in (torch.zeros_like(plan.work), plan.work.clone()):
+        work[2] = 1 << 30  # the cost of a pass that is too long
+        out, lse = kernels.lines_attention(q, kc, vc, plan._replace(work=work), prefix_table=pt, lse=True)
+        assert fault() == 256 and (out == 0).all() and (lse == -math.inf).all()
