@@ -38,15 +38,10 @@ bool byte_tile_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint6
                                      : box_bytes == 64  ? CU_TENSOR_MAP_SWIZZLE_64B
                                      : box_bytes == 32  ? CU_TENSOR_MAP_SWIZZLE_32B
                                                         : CU_TENSOR_MAP_SWIZZLE_NONE;
-  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
-  if (!fn) return false;
   cuuint64_t dims[2] = {row_bytes, rows};
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {box_bytes, box_rows};
-  cuuint32_t elem[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, swizzle);
 }
 
 int static_smem(const void* kernel) {

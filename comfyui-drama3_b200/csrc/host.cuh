@@ -105,4 +105,21 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
+// A tiled tensor map of `rank` dimensions (strides: of all but the first), elements next to one another, not interleaved,
+// zeros outside. Encoding wants a current context, which a thread has only once it has made a runtime call that needs
+// one; where there is none yet, the current device's is made current and the map encoded again.
+inline bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  auto encode = [&] {
+    return fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  int dev = 0;
+  return encode() || (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode());
+}
+
 }  // namespace d3host

@@ -23,29 +23,21 @@ namespace {
 // columns x `box` keys of one head.
 bool cache_map(CUtensorMap* map, bool f16, const void* base, int D, int heads, int page, int pages, const int64_t* st,
                int box) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
-  if (!fn) return false;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
   cuuint64_t strides[3] = {(cuuint64_t)st[1] * 2, (cuuint64_t)st[2] * 2, (cuuint64_t)st[0] * 2};
   cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
-  cuuint32_t elem[4] = {1, 1, 1, 1};
-  return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
-            dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
+                      boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Queries [T, heads, D] as a 3-D map (column, head, token), read in boxes of 64 columns x the heads of a KV head x the
 // tokens of a unit.
 bool query_map(CUtensorMap* map, bool f16, const void* base, int D, int heads, int T, const int64_t* st, int group) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
-  if (!fn) return false;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T};
   cuuint64_t strides[2] = {(cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
   cuuint32_t boxes[3] = {64, (cuuint32_t)group, (cuuint32_t)d3::la_tile_tokens(group)};
-  cuuint32_t elem[3] = {1, 1, 1};
-  return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
-            dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides,
+                      boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool attn_shape(int T, int Hq, int Hkv, int D) {
