@@ -37,7 +37,8 @@ constexpr int LA_ROWS = 128;
 constexpr int LA_KEYS = 128;
 constexpr int LA_UNIT_COST = 3;
 // Most rows of a KV head (T * group) whose prefix and own units may be apart: each row then keeps two fp32 partial
-// rows per KV head in the attention's workspace (136 MB at 4 KV heads of 128).
+// rows per KV head in the attention's workspace, whether or not the pass has a prefix (136 MB at 4 KV heads of 128, 1.1 GB
+// at 32). Past it every line's units read the prefix for themselves, however few of their rows are taken.
 constexpr int LA_APART_ROWS = 32768;
 struct __align__(16) LaUnit {
   int line;     // the line, or -1: rows of all lines together against the prefix

@@ -703,27 +703,13 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     size = _attention_workspace(device.index, T, Hq, Hkv, D)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     sums = torch.empty((T, Hq), dtype=torch.float32, device=device) if lse else None
-    ws = _scratch(device, size)
+    # scratch of this call alone: it makes two launches, and those of another thread on the same stream may come between
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
     _launch(device, "lines_attention", lib().d3_lines_attention, q.data_ptr(), _int64s(q_strides), kind, T, Hq, Hkv, D,
             k_cache.data_ptr(), _int64s(kc_strides), v_cache.data_ptr(), _int64s(vc_strides), pages, page,
             table.data_ptr(), W, _ptr(prefix_table), prefix_pages, work.data_ptr(), B,
             1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(), _ptr(sums), ws.data_ptr(), size)
     return (out, sums) if lse else out
-
-
-_SCRATCH = {}
-
-
-def _scratch(device, size):
-    """`size` bytes that a call on the current stream may use until it ends: one buffer per stream, kept and grown
-    (calls on one stream never overlap); during a CUDA-graph capture a fresh one, which the graph owns."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(size, dtype=torch.uint8, device=device)
-    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
-    held = _SCRATCH.get(key)
-    if held is None or held.numel() < size:
-        held = _SCRATCH[key] = torch.empty(size, dtype=torch.uint8, device=device)
-    return held
 
 
 @functools.lru_cache(maxsize=1024)

@@ -309,9 +309,10 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
  * d3_lines_plan_ints(B, T, Hq / Hkv) ints, and one that was made for another B, T, Hq / Hkv or page is refused on the
  * device (D3_FAULT_PLAN; zeros, lse -inf). So is a pass of 2^30 or more key tiles in all, counted once for each KV head
  * and each 128 rows (tokens x Hq / Hkv) that attend to them, and 3 for each such 128 rows: a prompt of about a million
- * tokens at 32 / 4 heads. The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value). D 64, 128
- * or 256; page 16, 32 or a multiple of 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and
- * all pointers 16-byte aligned. */
+ * tokens at 32 / 4 heads. The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value) of this call
+ * alone until its two launches have run: another thread's call on the same stream may come between them. D 64, 128 or
+ * 256; page 16, 32 or a multiple of 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and all
+ * pointers 16-byte aligned. */
 size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D);
 int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
                        const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,

@@ -1,6 +1,7 @@
 """What kernels.lines_attention gives the library, seen without a GPU: its launch is replaced by one that looks at the
 arguments."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -59,3 +60,24 @@ def test_a_work_list_of_another_type_is_refused(launches, spoil):
     with pytest.raises(ValueError, match="work list"):
         kernels.lines_attention(q, cache, cache, plan._replace(work=spoil(plan.work)))
     assert not launches
+
+
+def test_calls_of_two_threads_have_workspaces_of_their_own(launches, monkeypatch):
+    """A call is two launches, the attention and the joining of its parts, and both threads' may be in the stream in any
+    order: neither may write where the other's parts are."""
+    both = threading.Barrier(2, timeout=30)
+    inner = kernels._launch
+
+    def launch(*args):
+        inner(*args)
+        both.wait()  # the other thread is between its launches too
+
+    monkeypatch.setattr(kernels, "_launch", launch)
+    q, cache, plan = a_pass(3, 200)
+    threads = [threading.Thread(target=kernels.lines_attention, args=(q, cache, cache, plan)) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    (a, b), size = (x["workspace"] for x in launches), launches[0]["workspace_bytes"]
+    assert a + size <= b or b + size <= a

@@ -3,6 +3,7 @@ nothing."""
 import math
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -138,3 +139,45 @@ def test_attention_refused_by_the_kernel_gives_rows_of_nothing(cuda, monkeypatch
         work[2] = 1 << 30  # the cost of a pass that is too long
         out, lse = kernels.lines_attention(q, kc, vc, plan._replace(work=work), prefix_table=pt, lse=True)
         assert fault() == 256 and (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_attention_from_two_threads_on_one_stream(cuda):
+    from drama3_b200 import kernels
+    cases, want = [], []
+    for seed in range(2):
+        q, kc, vc, plan, pt = attn_case(cuda, 16, 2, 128, torch.bfloat16, 16, [300 + seed, 20, 77], [1, 1, 1], 500, seed=seed)
+        cases.append((q, kc, vc, plan, pt))
+        want.append(kernels.lines_attention(*cases[seed][:4], prefix_table=pt))
+    assert not torch.equal(*want)
+    got, start = [[], []], threading.Barrier(2, timeout=60)
+
+    def calls(i):
+        start.wait()
+        for _ in range(500):
+            got[i].append(kernels.lines_attention(*cases[i][:4], prefix_table=cases[i][4]))
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert fault() == 0
+    for i in range(2):
+        assert len(got[i]) == 500 and all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_attention_on_two_streams_at_once(cuda):
+    from drama3_b200 import kernels
+    cases = [attn_case(cuda, 16, 2, 128, torch.bfloat16, 64, [2000 + s] * 8, [1] * 8, 9000, seed=s) for s in range(2)]
+    want = [kernels.lines_attention(*c[:4], prefix_table=c[4]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(kernels.lines_attention(*c[:4], prefix_table=c[4]))
+    torch.cuda.synchronize()
+    assert fault() == 0
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
