@@ -15,7 +15,9 @@ from .model import OPS
 class LinesCache:
     """Keys and values of `layers` layers in pages of `page` tokens ([pages, page, kv_heads, head_dim] each), the
     block tables of `lines` lines of up to `most` tokens of their own, and the pages of the prefix that they share.
-    group: query heads per KV head."""
+    page: 16, 32 or a multiple of 64 (the attention's). group: query heads per KV head. The lengths are on the GPU, so no
+    call here can tell that a line outgrows `most` or that the pages run out: such tokens have no place, their keys read
+    as zeros, and the fault word says so (_lib.take_fault)."""
 
     def __init__(self, layers, pages, page, kv_heads, head_dim, lines, most, group, device, dtype=torch.bfloat16):
         self.page, self.group, self.lines, self.width = page, group, lines, -(-most // page)
@@ -43,12 +45,12 @@ class LinesCache:
 
     def plan(self, counts, tokens):
         """The plan of a pass that appends counts [lines] (int32, on the GPU) tokens, `tokens` token places in all; the
-        cache's lengths and its used pages are those after the pass. Attend with prefix_table=cache.prefix_table."""
+        cache's lengths and its used pages are those after the pass. It brings the prefix's pages along."""
         plan = kernels.lines_plan(self.lengths, counts, self.table, self.free, self.used, self.page, tokens,
                                   prefix=self.prefix, group=self.group)
         self.lengths.copy_(plan.lengths)
         self.used.copy_(plan.used)
-        return plan
+        return plan._replace(prefix_table=self.prefix_table)
 
     def restart(self):
         """New lines behind the same prefix: the lines' own pages are free again."""
@@ -72,7 +74,8 @@ class LinesAttention(nn.Module):
 
     def forward(self, x, plan, k_cache, v_cache, rotary, prefix_table=None, positions=None, axes=None):
         """rotary: kernels.rotary_table's. positions: of the tokens, where they are not the plan's (with several axes
-        [A, T], and `axes` from kernels.rotary_axes). prefix_table: of a cache whose lines have a prefix."""
+        [A, T], and `axes` from kernels.rotary_axes). prefix_table: the prefix's pages, where the plan does not bring them
+        (LinesCache's do)."""
         T, sizes = x.shape[0], (self.heads, self.kv_heads, self.kv_heads)
         q, k, v = (t.unflatten(1, (-1, self.head_dim)) for t in
                    self.qkv_proj(x).split_with_sizes([n * self.head_dim for n in sizes], 1))

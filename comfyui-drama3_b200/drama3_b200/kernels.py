@@ -467,7 +467,7 @@ class LinesPlan(NamedTuple):
     """What `lines_plan` returns: the block tables (the caller's, updated), the new tokens' slots [T] and positions [T]
     (int64) and lines [T] (int32, -1 past the last token), the first token of each line cu [B + 1], the lines' lengths
     [B] and the used part of the free list [1] after the pass (int32), and the attention's work list for `group` query
-    heads per KV head."""
+    heads per KV head. prefix_table: of the prefix that the plan counts, where who made the plan holds it (a LinesCache)."""
     table: torch.Tensor
     slots: torch.Tensor
     positions: torch.Tensor
@@ -478,6 +478,7 @@ class LinesPlan(NamedTuple):
     work: torch.Tensor
     page: int
     group: int
+    prefix_table: torch.Tensor = None
 
 
 def _ints(name, t, device, count):
@@ -667,7 +668,7 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     """[T, Hq, D] (and, with `lse`, [T, Hq] float32: the log of each row's sum of exponentials): the attention of the
     plan's tokens q [T, Hq, D] (bfloat16 or float16) over the paged caches [pages, page, Hkv, D] of the same type, whose
     keys of this pass are written (`qk_norm_rope`). A token sees the keys of the shared prefix, in the pages of
-    prefix_table [PW] (int32; their number was given to `lines_plan`), and its line's own keys up to its own; query
+    prefix_table [PW] (int32; their number was given to `lines_plan`; None: the plan's, if it has one), and its line's own keys up to its own; query
     head h reads KV head h / (Hq / Hkv), scale defaults to 1 / sqrt(D). D 64, 128 or 256; page 16, 32 or a multiple of
     64. Where the lines bring few tokens, the prefix's keys are read once for all of them. Places of the plan without a
     token get zeros (lse -inf), and all places do where the plan is another pass's or the pass is too long (2^30 key tiles
@@ -697,6 +698,8 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
         # another pass's list, which the kernel must not read past its end: one of this size that it refuses instead
         work = torch.zeros(plan_ints(B, T, plan.group), dtype=torch.int32, device=device)
     prefix_pages = 0
+    if prefix_table is None:
+        prefix_table = plan.prefix_table
     if prefix_table is not None:
         prefix_pages = prefix_table.numel()
         _ints("prefix_table", prefix_table, device, prefix_pages)

@@ -181,3 +181,26 @@ def test_attention_on_two_streams_at_once(cuda):
     assert fault() == 0
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+# ---- the module
+
+def test_module_reads_the_prefix_that_the_plan_counts(cuda):
+    from drama3_b200 import kernels
+    from drama3_b200.attention import LinesAttention, LinesCache
+    torch.manual_seed(5)
+    att = LinesAttention(128, 4, 2, 64, device=cuda, dtype=torch.bfloat16)
+    cache = LinesCache(1, 20, 16, 2, 64, 3, 40, 2, cuda)
+    rotary = kernels.rotary_table(torch.ones(32), 128, cuda)
+    x = torch.randn((50, 128), device=cuda).bfloat16()
+    with torch.no_grad():
+        # without a prefix, and the prefix itself: there is no table
+        plan = cache.plan(torch.ones(3, dtype=torch.int32, device=cuda), 3)
+        assert plan.prefix_table is None
+        att(x[:3], plan, cache.k[0], cache.v[0], rotary)
+        cache.restart()
+        att(x, cache.plan_prefix(50), cache.k[0], cache.v[0], rotary)
+        plan = cache.plan(torch.ones(3, dtype=torch.int32, device=cuda), 3)
+        assert fault() == 0
+        want = att(x[:3], plan, cache.k[0], cache.v[0], rotary, cache.prefix_table)
+        assert torch.equal(att(x[:3], plan, cache.k[0], cache.v[0], rotary), want) and fault() == 0
