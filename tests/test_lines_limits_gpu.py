@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import lines_ref as ref
-from test_lines_gpu import attn_case, fault, lines_case, rope_inputs, run_plan
+from test_lines_gpu import attn_case, check_attn, fault, lines_case, rope_inputs, run_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -204,3 +204,42 @@ def test_module_reads_the_prefix_that_the_plan_counts(cuda):
         assert fault() == 0
         want = att(x[:3], plan, cache.k[0], cache.v[0], rotary, cache.prefix_table)
         assert torch.equal(att(x[:3], plan, cache.k[0], cache.v[0], rotary), want) and fault() == 0
+
+
+# ---- many rows
+
+@pytest.mark.parametrize("spare,together", [(4076, 0), (4077, 1)])
+def test_attention_few_lines_in_many_places(cuda, spare, together):
+    # 32768 rows of a KV head are the most whose prefix and own units may be apart; one token place more
+    kept, counts, prefix = [9 + b for b in range(20)], [1] * 20, 300
+    case = attn_case(cuda, 8, 1, 64, torch.bfloat16, 16, kept, counts, prefix, spare=spare)
+    assert int(case[3].work[0]) == together
+    check_attn(cuda, case, kept, counts, prefix)
+
+
+@pytest.mark.parametrize("lines,together", [(4096, 0), (4097, 1)])
+def test_attention_thousands_of_lines(cuda, lines, together):
+    from drama3_b200 import kernels
+    prefix, D, hq = 200, 64, 8
+    kept = [(7 * b) % 15 for b in range(lines)]
+    q, kc, vc, plan, pt = attn_case(cuda, hq, 1, D, torch.bfloat16, 16, kept, [1] * lines, prefix, spare=0)
+    work = plan.work[:2].tolist()
+    assert work == ([1, lines] if together else [0, lines + lines // 16])  # 16 tokens of 8 heads to a tile of rows
+    got, lse = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt, lse=True)
+    k, v = (torch.cat((c[pt.long()].flatten(0, 1)[:prefix, 0].expand(lines, -1, -1), c[plan.table[:, 0].long()][:, :, 0]), 1).double()
+            for c in (kc, vc))  # the prefix, then the line's one page
+    seen = torch.arange(prefix + 16, device=cuda)[None] <= prefix + torch.tensor(kept, device=cuda)[:, None]
+    v = torch.where(seen[..., None], v, torch.zeros_like(v))
+    s = torch.where(seen[:, None], q.double() @ k.transpose(1, 2) / math.sqrt(D), torch.tensor(-math.inf, device=cuda, dtype=torch.double))
+    p = s.softmax(-1)
+    assert fault() == 0
+    assert ((got.double() - p @ v).abs() <= 2.2 * 2.0 ** -8 * (p @ v.abs())).all()
+    assert ((lse.double() - s.logsumexp(-1)).abs() <= 2e-5 + 2.0 ** -21 * s.logsumexp(-1).abs()).all()
+
+
+def test_attention_of_no_tokens(cuda):
+    from drama3_b200 import kernels
+    kept = [20, 3]
+    q, kc, vc, plan, pt = attn_case(cuda, 8, 2, 64, torch.bfloat16, 16, kept, [0, 0], 40)
+    out, lse = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt, lse=True)
+    assert out.shape == (0, 8, 64) and lse.shape == (0, 8) and fault() == 0
