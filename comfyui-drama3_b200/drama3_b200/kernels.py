@@ -693,7 +693,8 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     if k_cache.device != device or v_cache.device != device or work.device != device:
         raise ValueError(f"lines_attention: every tensor must be on {device}")
     _ints("the plan's table", table, device, B * W)
-    _ints("the plan's work list", work, device, work.numel())
+    if work.dtype is not torch.int32 or not work.is_contiguous():
+        raise ValueError("the plan's work list must be a contiguous int32 tensor")
     if work.numel() != plan_ints(B, T, plan.group):
         # another pass's list, which the kernel must not read past its end: one of this size that it refuses instead
         work = torch.zeros(plan_ints(B, T, plan.group), dtype=torch.int32, device=device)
