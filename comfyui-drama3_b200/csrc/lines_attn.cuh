@@ -30,15 +30,23 @@
 // memory before the product, since the cache may hold anything there (0 x NaN is NaN).
 // Every wait is bounded (2 s) and records FAULT_WAIT_TIMEOUT instead of hanging.
 //
-// Measured (B200, bf16, 32 query heads over 4 KV heads of 128; device time): 8192 tokens of a prompt 544 us, 1010 TFLOP/s;
-// 16 texts of up to 192 tokens behind 4096 138 us, 840 TFLOP/s; 64 lines, a token each, behind 32768 65 us, 3.1 TB/s;
-// 16 lines behind 4096 14.4 us; one line of 1000 10.6 us. With full runs a tile takes about 1600 clocks, 1024 of them
-// of the tensor cores: a group's steps (2800 a tile, two groups) are near that. A unit takes about 6000 clocks besides.
-// With few keys the time is latency: about 4 us until the first scores, 2 us a tile, 3 us for the results and the join.
-// Other forms of the same tiles: one warp that loads both K and V, 1750 clocks a tile, 546 to 578 us for the prompt in
-// turn with 539 to 556 for two, heads of 256 (16 lines behind 3001 in pages of 16) 16.6 us against 15.7; two threads a
-// row, one group, 70 us for the 64 lines and 153 for the texts; two CTAs per SM with one S buffer each 74 and 165; part
-// of the exponentials as polynomials, the same times as without.
+// A value that is not finite, at a key that only some rows of its tile see, makes the others of that line's tile NaN too:
+// their weight for it is 0, and 0 x NaN is NaN.
+//
+// Measured (B200, bf16, 32 query heads over 4 KV heads of 128; device time in a few graph replays, in brackets the time of
+// a call among many from Python, whose load lowers the clocks): 8192 tokens of a prompt 545 us, 1010 TFLOP/s (614); 16 texts
+// of up to 192 tokens behind 4096 123 to 157 us from run to run, 740 to 950 TFLOP/s (143); 64 lines, a token each, behind
+// 32768 66 us, 3.0 TB/s (74); 16 lines behind 4096 14.3 us (18, the host's time); one line of 1000 10.1 us (18). Heads of 256
+// (16 over 2): the prompt 468 us, 1170 TFLOP/s, the texts 122 us; heads of 64: the prompt 444 us, 620 TFLOP/s. By the
+// counters the prompt takes 2080 clocks a tile, units' own cost included, and the tensor cores are active for half of
+// them, 1040; the texts the same. L2 and DRAM are a third busy at most: the time is that of the row groups' steps, which the
+// products wait for and which wait for them.
+// With few keys the time is latency: launch, loads and first product, two or three tiles, the results, then the join.
+// Other forms of the same tiles: one warp that loads both K and V, 546 to 578 us for the prompt in turn with 539 to 556 for
+// two, heads of 256 (16 lines behind 3001 in pages of 16) 16.6 us against 15.7; two threads a row, one group, 70 us for the
+// 64 lines and 153 for the texts; two CTAs per SM with one S buffer each 74 and 165; part of the exponentials as
+// polynomials, the same times as without; 216 registers for the row warps and 72 for the others, the texts 139 -> 127 us
+// and the prompt 541 -> 535, but 16 lines 14.35 -> 14.7 and heads of 256 15.6 -> 15.8: not kept.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -56,7 +64,9 @@ constexpr int LA_ROW_WARPS = 8;
 constexpr int LA_PV_WARP = LA_ROW_WARP + LA_ROW_WARPS;  // issues the products with V
 constexpr int LA_V_WARP = LA_PV_WARP + 1;                // loads V
 constexpr int LA_SLICE = LA_KEYS * 128;  // 64 columns of a K or V tile
-constexpr float LA_RESCALE = 8.0f;    // growth of the maximum, in powers of two, that rescales O
+// Growth of the maximum, in powers of two, that rescales O. (That it may lag behind is a published method for attention on
+// tensor cores: the division by the row's sum takes out whatever the weights refer to.)
+constexpr float LA_RESCALE = 8.0f;
 // Where the weights are held in float16 a row's refer to its maximum less this: they are 2^7 to 2^15 times what they
 // weigh (float16 ends below 2^16), and float16's smallest steps, 2^-24, are 2^-31 of the largest weight and less. Against
 // the maximum itself they were 2^-24 of it, and keys of less weight counted as double or as nothing beside a heavy one.
@@ -832,8 +842,8 @@ __global__ void __launch_bounds__(LA_THREADS, 1)
 
 // The joining: with M the largest of a row's parts' maxima, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i, the parts
 // taken in order. A lane is a row (of 32 neighbouring ones of a KV head), a warp takes groups of four columns. Bound
-// by latency: N x AHEAD loads are in flight at a time; 2 to 3 us of a decode step's attention. A kernel of its own, since a
-// barrier of the attention's CTAs would need all of them on the GPU together.
+// by latency: N x AHEAD loads are in flight at a time; 2 to 3 us of a decode step's attention. (A counter per cut unit would
+// let the last CTA to arrive join its parts, in the same order, without this launch; not built.)
 // The parts of a row: `first`, then those that the runs r0 + 1 .. r1 left at `rest` rows into theirs.
 struct LaParts {
   long long first;

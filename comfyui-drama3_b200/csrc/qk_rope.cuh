@@ -13,8 +13,10 @@
 // too few to fill the GPU, a share of its heads. The token's cosines and sines are looked up into shared memory (axis,
 // position and table are three loads that wait for one another), then the warp takes its queries, keys and values in
 // turn, with the weights in registers. 16 warps an SM of 128 registers; 24 of 80 spilled and took a quarter longer.
-// Measured (B200, bf16): 16384 tokens of 32 + 4 heads of 128 81 us, 3.7 TB/s; 2048 tokens of 16 + 2 heads of 256 with the
-// cache write 15 us, 2.8 TB/s; 16 tokens 3.4 us, the latency of a launch and four loads that wait for one another.
+// Measured (B200, bf16, device time in graph replays): 16384 tokens of 32 + 4 heads of 128 79 us, 3.8 TB/s; 2048 tokens of
+// 16 + 2 heads of 256 with the cache write 15 us, 2.8 TB/s; 16 tokens 3.3 us, the latency of a launch and four loads that
+// wait for one another (a call from Python takes the host 15 us). Rows of the other form, 16384 tokens of 32 + 4 heads of
+// 80 with 40 columns turned, 270 us; with all 80 turned, in this form, 75.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -670,10 +670,12 @@ def lines_attention(q, k_cache, v_cache, plan, prefix_table=None, scale=None, ls
     keys of this pass are written (`qk_norm_rope`). A token sees the keys of the shared prefix, in the pages of
     prefix_table [PW] (int32; their number was given to `lines_plan`; None: the plan's, if it has one), and its line's own keys up to its own; query
     head h reads KV head h / (Hq / Hkv), scale defaults to 1 / sqrt(D). D 64, 128 or 256; page 16, 32 or a multiple of
-    64. Where the lines bring few tokens, the prefix's keys are read once for all of them. Places of the plan without a
+    64. Where the lines bring few tokens, the prefix's keys are read once for all of them (up to T * Hq / Hkv = 32768,
+    token places without a token counted too; past that each line reads them for itself). Places of the plan without a
     token get zeros (lse -inf), and all places do where the plan is another pass's or the pass is too long (2^30 key tiles
     over all heads and rows: about a million tokens of a prompt), which the fault word records. What the cache holds past a
-    line's length is never used."""
+    line's length is never used; a value that is not finite reaches the line's own tokens of its tile of 128 keys, earlier
+    ones too."""
     T, Hq, D = q.shape
     kind = ROW_TYPES.get(q.dtype)
     if (kind != 0 and kind != 1) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:

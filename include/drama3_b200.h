@@ -57,8 +57,8 @@ int d3_device_check(void);
  * grouped GEMM given fewer row tiles than its groups need, D3_FAULT_EXCHANGE (16) an expert-parallel exchange area
  * whose geometry does not fit the call, D3_FAULT_PAGES (32) a cache page that is missing or outside the cache,
  * D3_FAULT_TOKENS (64) lines that append more tokens than the pass holds, D3_FAULT_POSITION (128) a position or axis
- * outside the rotary table, D3_FAULT_PLAN (256) an attention given the plan of another pass, or of one that is too long. No counterpart in the
- * reference, whose kernels do not check indices. */
+ * outside the rotary table, D3_FAULT_PLAN (256) an attention given the plan of another pass, or of one that is too
+ * long. No counterpart in the reference, whose kernels do not check indices. */
 #define D3_FAULT_WAIT 1u
 #define D3_FAULT_EXPERT 2u
 #define D3_FAULT_SLOT 4u
@@ -310,9 +310,10 @@ int d3_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, cons
  * device (D3_FAULT_PLAN; zeros, lse -inf). So is a pass of 2^30 or more key tiles in all, counted once for each KV head
  * and each 128 rows (tokens x Hq / Hkv) that attend to them, and 3 for each such 128 rows: a prompt of about a million
  * tokens at 32 / 4 heads. The workspace is scratch (d3_lines_attention_workspace() bytes, no initial value) of this call
- * alone until its two launches have run: another thread's call on the same stream may come between them. D 64, 128 or
- * 256; page 16, 32 or a multiple of 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and all
- * pointers 16-byte aligned. */
+ * alone until its two launches have run: another thread's call on the same stream may come between them. Short lines
+ * read the prefix together where T * Hq / Hkv is 32768 at most, each for itself past that (slower, the same values); the
+ * workspace has room for the former, whether there is a prefix or not. D 64, 128 or 256; page 16, 32 or a multiple of
+ * 64; Hq / Hkv <= 128; pages * page < 2^31; strides multiples of 8 elements and all pointers 16-byte aligned. */
 size_t d3_lines_attention_workspace(int T, int Hq, int Hkv, int D);
 int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T, int Hq, int Hkv, int D,
                        const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,

@@ -226,11 +226,11 @@ def test_attention_thousands_of_lines(cuda, lines, together):
     work = plan.work[:2].tolist()
     assert work == ([1, lines] if together else [0, lines + lines // 16])  # 16 tokens of 8 heads to a tile of rows
     got, lse = kernels.lines_attention(q, kc, vc, plan, prefix_table=pt, lse=True)
-    k, v = (torch.cat((c[pt.long()].flatten(0, 1)[:prefix, 0].expand(lines, -1, -1), c[plan.table[:, 0].long()][:, :, 0]), 1).double()
-            for c in (kc, vc))  # the prefix, then the line's one page
+    k, v = (torch.cat((c[pt.long()].flatten(0, 1)[:prefix, 0].expand(lines, -1, -1), c[plan.table[:, 0].long()][:, :, 0]),
+                      1).double() for c in (kc, vc))  # the prefix, then the line's one page
     seen = torch.arange(prefix + 16, device=cuda)[None] <= prefix + torch.tensor(kept, device=cuda)[:, None]
     v = torch.where(seen[..., None], v, torch.zeros_like(v))
-    s = torch.where(seen[:, None], q.double() @ k.transpose(1, 2) / math.sqrt(D), torch.tensor(-math.inf, device=cuda, dtype=torch.double))
+    s = (q.double() @ k.transpose(1, 2) / math.sqrt(D)).where(seen[:, None], -math.inf)
     p = s.softmax(-1)
     assert fault() == 0
     assert ((got.double() - p @ v).abs() <= 2.2 * 2.0 ** -8 * (p @ v.abs())).all()
