@@ -25,7 +25,8 @@
 
 using namespace d3host;
 
-int d3_lines_take_fault(unsigned int* fault);  // lines.cu
+int d3_lines_take_fault(unsigned int* fault);   // lines.cu
+int d3_linear_take_fault(unsigned int* fault);  // linear.cu
 
 namespace {
 
@@ -92,9 +93,10 @@ int d3_take_fault(unsigned int* fault) {
   if (st) return st;
   st = cuda_status(cudaMemcpyToSymbol(d3::g_fault, &zero, sizeof(zero)));
   if (st) return st;
-  unsigned int lines = 0;
-  st = d3_lines_take_fault(&lines);
-  *fault = v | lines;
+  unsigned int lines = 0, linear = 0;
+  if ((st = d3_lines_take_fault(&lines))) return st;
+  st = d3_linear_take_fault(&linear);
+  *fault = v | lines | linear;
   return st;
 }
 

@@ -22,6 +22,7 @@ _i = ctypes.c_int
 _d = ctypes.c_double
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes); every name here is a symbol include/drama3_b200.h declares
 SIGNATURES = {
@@ -69,6 +70,12 @@ SIGNATURES = {
     "d3_lines_attention_workspace": (_sz, [_i, _i, _i, _i]),
     "d3_lines_attention": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i, _p, _i, _p, _i, _f,
                                 _p, _p, _p, _sz, _p]),
+    "d3_lines_conv": (_i, [_p, _i64, _i, _i, _i, _p, _p, _i, _i, _p, _p, _p, _i, _i, _p, _p]),
+    "d3_lines_delta": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _i, _p, _p, _f, _f, _p, _p,
+                            _p, _i, _p, _p, _sz, _p]),
+    "d3_lines_delta_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "d3_gated_norm": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _p, _i, _f, _f, _i, _p, _p]),
+    "d3_add_norm": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _p, _p, _i, _f, _p, _i64, _i, _f, _f, _p, _p, _p]),
 }
 
 

@@ -727,3 +727,216 @@ def _attention_workspace(index, T, Hq, Hkv, D):
     if size == 0:
         raise ValueError(f"no attention kernel for {Hq} / {Hkv} heads of {D}")
     return size
+
+
+def _form(t):
+    return None if t is None else (t.dtype, t.get_device(), t.shape, t.stride())
+
+
+def _checked(forms, kept, check_forms, tensors):
+    """check_forms(*tensors), kept for tensors of these forms (types, devices, shapes, strides): a step's tensors have the
+    same ones in every layer."""
+    found = kept.get(forms)
+    if found is None:
+        if len(kept) >= 4096:
+            kept.clear()
+        found = kept[forms] = check_forms(*tensors)
+    return found
+
+
+def _same_device(what, device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: every tensor must be on {device}")
+
+
+def _plan_lines(what, device, plan, T):
+    """(cu, line, B) of a plan for T tokens; refuses one of another pass."""
+    cu, line = plan.cu, plan.line
+    B = cu.shape[0] - 1
+    if line.shape[0] != T:
+        raise ValueError(f"{what}: the plan is for {line.shape[0]} tokens, not for {T}")
+    _ints("the plan's cu", cu, device, B + 1)
+    _ints("the plan's line", line, device, T)
+    return cu, line, B
+
+
+def _norm_weights(what, rows, size, *weights):
+    """1 where the weights [size] are float32, 0 where they are of the rows' type; refuses others."""
+    given = [w for w in weights if w is not None]
+    for w in given:
+        if w.shape != (size,) or not w.is_contiguous() or w.dtype not in (rows.dtype, torch.float32) or w.dtype != given[0].dtype:
+            raise ValueError(f"{what}: weights must be contiguous [{size}] tensors of the rows' type or float32, alike")
+    return int(given[0].dtype == torch.float32)
+
+
+_CONV_FORMS, _DELTA_FORMS, _GATED_FORMS, _JOIN_FORMS = {}, {}, {}, {}
+
+
+def lines_conv(x, weight, state, plan, bias=None, silu=True):
+    """[T, C]: the causal convolution of each line's tokens x [T, C] (bfloat16, float16 or float32, the last dimension
+    contiguous) of a plan's pass with a filter a channel, weight [C, W] (or a Conv1d's [C, 1, W]; 2 to 8 taps, the last one
+    the token's own; of the rows' type or float32) and bias [C], through SiLU unless silu is False. state [B, W - 1, C] of the
+    rows' type: the inputs that each line had last, updated in place (zeros: a line that begins). Places of no line get
+    zeros. 32-bit arithmetic, rounded once."""
+    tensors = (x, weight, state, bias)
+    device, sizes, W, w_f32 = _checked(tuple(map(_form, tensors)), _CONV_FORMS, _conv_arguments, tensors)
+    cu, line, B = _plan_lines("lines_conv", device, plan, sizes[1])
+    if state.shape[0] != B:
+        raise ValueError(f"lines_conv: the plan has {B} lines, the state {state.shape[0]}")
+    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    _launch(device, "lines_conv", lib().d3_lines_conv, x.data_ptr(), x.stride(0), *sizes, weight.data_ptr(), _ptr(bias), W,
+            w_f32, state.data_ptr(), cu.data_ptr(), line.data_ptr(), B, 1 if silu else 0, out.data_ptr())
+    return out
+
+
+def _conv_arguments(x, weight, state, bias):
+    device = _gpu_of(x, "lines_conv")
+    _same_device("lines_conv", device, weight, state, bias)
+    if x.dtype not in ROW_TYPES:
+        raise TypeError(f"lines_conv takes bfloat16, float16 or float32 rows, not {x.dtype}")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("lines_conv takes x [T, C], the last dimension contiguous")
+    T, C = x.shape
+    W = weight.shape[-1]
+    if weight.shape not in ((C, W), (C, 1, W)) or not weight.is_contiguous() or not 2 <= W <= 8:
+        raise ValueError(f"weight must be a contiguous [{C}, W] tensor of 2 to 8 taps, not {list(weight.shape)}")
+    if weight.dtype not in (x.dtype, torch.float32) or (bias is not None and (
+            bias.shape != (C,) or bias.dtype != weight.dtype or not bias.is_contiguous())):
+        raise ValueError("weight and bias [C] must be contiguous, of the rows' type or float32, alike")
+    if state.dim() != 3 or state.shape[1:] != (W - 1, C) or state.dtype != x.dtype or not state.is_contiguous():
+        raise ValueError(f"state must be a contiguous [B, {W - 1}, {C}] tensor of the rows' type")
+    return device, (ROW_TYPES[x.dtype], T, C), W, int(weight.dtype == torch.float32)
+
+
+def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None, eps=1e-6, scale=None):
+    """[T, Hv, Dv]: linear attention with a decay for each head over the tokens of a plan's pass. For each line and value
+    head, with S of state [B, Hv, Dv, Dk] (float32, updated in place; zeros: a line that begins), token by token:
+
+        S <- exp(g) S;  u = beta (v - S k), the delta rule, or u = v without beta;  S <- S + u k^T;  out = scale S q
+
+    q, k [T, Hk, Dk] and v [T, Hv, Dv] (bfloat16 or float16; any strides with the last dimension contiguous; views whose rows
+    are not on 16-byte boundaries are copied); value head h reads key head h / (Hv / Hk). decay and beta [T, Hv] (the last
+    dimension contiguous, of the rows' type or float32, alike). With a_log [Hv] (float32) they are the projections' raw
+    outputs: g = -exp(a_log) softplus(decay + dt_bias), beta through the sigmoid; without it g is decay itself, at most 0, and
+    beta is taken as it is. q and k are divided by sqrt(sum of squares + eps) unless eps is None; scale defaults to 1 /
+    sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get zeros."""
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = (_aligned16(t) for t in (q, k, v))
+    tensors = (q, k, v, decay, state, beta, a_log, dt_bias)
+    device, copies, strides, sizes, gates_f32 = _checked(tuple(map(_form, tensors)), _DELTA_FORMS, _delta_arguments, tensors)
+    if copies:
+        q, k, v = (t.contiguous() for t in (q, k, v))
+    _, T, Hk, Hv, Dk, Dv = sizes
+    cu, line, B = _plan_lines("lines_delta", device, plan, T)
+    if state.shape[0] != B:
+        raise ValueError(f"lines_delta: the plan has {B} lines, the state {state.shape[0]}")
+    if state.data_ptr() & 15:
+        raise ValueError("state must start on a 16-byte boundary")
+    out = torch.empty((T, Hv, Dv), dtype=q.dtype, device=device)
+    # scratch of this call alone: it may make several launches, and those of another thread on the same stream may come between
+    size = _delta_workspace(T, B, Hk, Hv, Dk)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _launch(device, "lines_delta", lib().d3_lines_delta, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(),
+            strides[2], *sizes, decay.data_ptr(), decay.stride(0), _ptr(beta), 0 if beta is None else beta.stride(0), gates_f32,
+            _ptr(a_log), _ptr(dt_bias), -1.0 if eps is None else eps, Dk ** -0.5 if scale is None else scale,
+            state.data_ptr(), cu.data_ptr(), line.data_ptr(), B, out.data_ptr(), _ptr(ws), size)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _delta_workspace(T, B, Hk, Hv, Dk):
+    return lib().d3_lines_delta_workspace(T, B, Hk, Hv, Dk)
+
+
+def _delta_arguments(q, k, v, decay, state, beta, a_log, dt_bias):
+    device = _gpu_of(q, "lines_delta")
+    _same_device("lines_delta", device, k, v, decay, state, beta, a_log, dt_bias)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"lines_delta takes bfloat16 or float16 rows of one type, not {q.dtype}, {k.dtype} and {v.dtype}")
+    if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or v.shape[0] != q.shape[0]:
+        raise ValueError("lines_delta takes q and k [T, Hk, Dk] and v [T, Hv, Dv]")
+    T, Hk, Dk = q.shape
+    Hv, Dv = v.shape[1:]
+    if Dk not in (64, 128) or Dv % 16 or not 16 <= Dv <= 256 or Hk < 1 or Hv < 1 or Hv % Hk:
+        raise ValueError(f"no kernel for {Hk} / {Hv} heads of {Dk} / {Dv}: Dk 64 or 128, Dv a multiple of 16 up to 256, value "
+                         f"heads in whole groups for each key head")
+    if any(t.stride(2) != 1 for t in (q, k, v)):
+        raise ValueError("the last dimension of q, k and v must be contiguous")
+    for name, t in (("decay", decay), ("beta", beta)):
+        if t is not None and (t.shape != (T, Hv) or (Hv > 1 and t.stride(1) != 1) or t.dtype not in (q.dtype, torch.float32)
+                              or t.dtype != decay.dtype):
+            raise ValueError(f"{name} must be [{T}, {Hv}], its last dimension contiguous, of the rows' type or float32 (decay "
+                             f"and beta alike)")
+    if dt_bias is not None and a_log is None:
+        raise ValueError("dt_bias goes with a_log")
+    for name, t in (("a_log", a_log), ("dt_bias", dt_bias)):
+        if t is not None and (t.shape != (Hv,) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 [{Hv}] tensor")
+    if state.dim() != 4 or state.shape[1:] != (Hv, Dv, Dk) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"state must be a contiguous float32 [B, {Hv}, {Dv}, {Dk}] tensor")
+    copies = any(s % 8 for t in (q, k, v) for s in t.stride()[:2])
+    strides = tuple(_int64s((t.shape[1] * t.shape[2], t.shape[2]) if copies else t.stride()[:2]) for t in (q, k, v))
+    return device, copies, strides, (ROW_TYPES[q.dtype], T, Hk, Hv, Dk, Dv), int(decay.dtype == torch.float32)
+
+
+_ACTIVATIONS = {"silu": 0, "sigmoid": 1}
+
+
+def gated_norm(x, gate, weight, eps=1e-6, unit_offset=False, activation="silu"):
+    """[T, H, D]: each head of x [T, H, D] (bfloat16, float16 or float32; any strides with the last dimension contiguous)
+    divided by its root mean square, times weight [D] (of the rows' type or float32; 1 + weight with unit_offset), times
+    the gate [T, H, D] through its activation, "silu" or "sigmoid". 32-bit arithmetic, rounded once."""
+    tensors = (x, gate, weight)
+    device, x_strides, gate_strides, sizes, w_f32 = _checked(tuple(map(_form, tensors)), _GATED_FORMS, _gated_arguments, tensors)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, not {activation}")
+    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    _launch(device, "gated_norm", lib().d3_gated_norm, x.data_ptr(), x_strides, gate.data_ptr(), gate_strides, *sizes,
+            weight.data_ptr(), w_f32, 1.0 if unit_offset else 0.0, eps, _ACTIVATIONS[activation], out.data_ptr())
+    return out
+
+
+def _gated_arguments(x, gate, weight):
+    device = _gpu_of(x, "gated_norm")
+    _same_device("gated_norm", device, gate, weight)
+    if x.dtype not in ROW_TYPES or gate.dtype != x.dtype:
+        raise TypeError(f"gated_norm takes bfloat16, float16 or float32 rows of one type, not {x.dtype} and {gate.dtype}")
+    if x.dim() != 3 or gate.shape != x.shape or 0 in x.shape[1:] or (x.shape[2] > 1 and (x.stride(2) != 1 or gate.stride(2) != 1)):
+        raise ValueError("gated_norm takes x and gate [T, H, D], their last dimension contiguous")
+    w_f32 = _norm_weights("gated_norm", x, x.shape[2], weight)
+    return device, _int64s(x.stride()[:2]), _int64s(gate.stride()[:2]), (ROW_TYPES[x.dtype], *x.shape), w_f32
+
+
+def add_norm(x, residual, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6, unit_offset=False):
+    """(sum, normed), both [T, W]: a block's output x [T, W] joined to the residual [T, W] and the norm in front of the next
+    block. sum = residual + scale * gate * x, with post_weight [W] of x's RMS norm instead of x; normed = the sum's RMS norm
+    (of the sum before it is rounded) with weight [W]. Rows bfloat16, float16 or float32, of one type, the last dimension
+    contiguous; weights of the rows' type or float32, alike, plus 1 with unit_offset; gate: a tensor of the rows' type that
+    broadcasts to [T, W]. 32-bit arithmetic, rounded once."""
+    tensors = (x, residual, weight, post_weight, gate)
+    device, sizes, w_f32, gate_token, gate_kind = _checked(tuple(map(_form, tensors)), _JOIN_FORMS, _join_arguments, tensors)
+    sums, normed = (torch.empty(x.shape, dtype=x.dtype, device=device) for _ in range(2))
+    _launch(device, "add_norm", lib().d3_add_norm, x.data_ptr(), x.stride(0), residual.data_ptr(), residual.stride(0), *sizes,
+            weight.data_ptr(), _ptr(post_weight), w_f32, 1.0 if unit_offset else 0.0, _ptr(gate), gate_token, gate_kind,
+            scale, eps, sums.data_ptr(), normed.data_ptr())
+    return sums, normed
+
+
+def _join_arguments(x, residual, weight, post_weight, gate):
+    device = _gpu_of(x, "add_norm")
+    _same_device("add_norm", device, residual, weight, post_weight, gate)
+    if x.dtype not in ROW_TYPES or residual.dtype != x.dtype or (gate is not None and gate.dtype != x.dtype):
+        raise TypeError("add_norm takes bfloat16, float16 or float32 rows and gates of one type")
+    if x.dim() != 2 or residual.shape != x.shape or x.shape[1] < 1 or (x.shape[1] > 1 and (x.stride(1) != 1 or residual.stride(1) != 1)):
+        raise ValueError("add_norm takes x and residual [T, W], their last dimension contiguous")
+    T, W = x.shape
+    w_f32 = _norm_weights("add_norm", x, W, weight, post_weight)
+    token = kind = 0
+    if gate is not None:
+        wide = gate.expand(T, W)
+        token, channel = wide.stride()
+        if W > 1 and channel not in (0, 1):
+            raise ValueError("gate's last dimension must be contiguous, or of one value")
+        kind = 1 if channel == 0 or W == 1 else 2
+    return device, (ROW_TYPES[x.dtype], T, W), w_f32, token, kind

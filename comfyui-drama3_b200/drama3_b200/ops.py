@@ -1,7 +1,7 @@
 """The library's kernels as torch.library custom ops, torch.ops.drama3_b200.<name>, for callers that build graphs
 (torch.compile, CUDA graph capture, exported programs): every op takes and returns plain tensors, ints, bools and
 strings, writes fresh outputs (shared_expert updates `out` in place and declares it, as lines_plan does its table and
-qk_norm_rope_cached its caches), and has a fake implementation that gives the output shapes and dtypes without running
+qk_norm_rope_cached its caches and lines_conv and lines_delta their state), and has a fake implementation that gives the output shapes and dtypes without running
 anything. Each op calls the matching function of drama3_b200.kernels; there is no CPU or torch fallback, so a call on
 tensors that are not on a B200 fails loudly.
 
@@ -17,7 +17,8 @@ from . import _lib, kernels
 
 NAMESPACE = "drama3_b200"
 OPS = ("route", "weighted_sum", "rotate", "router", "shared_expert", "moe_decode", "grouped_mma", "prefill_plan",
-       "prefill_combine", "lines_plan", "qk_norm_rope", "qk_norm_rope_cached", "lines_attention")
+       "prefill_combine", "lines_plan", "qk_norm_rope", "qk_norm_rope_cached", "lines_attention", "lines_conv", "lines_delta",
+       "gated_norm", "add_norm")
 
 
 def _fields(kind, w, scale, s_channel):
@@ -209,3 +210,61 @@ def lines_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, table: Tensor, 
 @lines_attention.register_fake
 def _(q, k_cache, v_cache, table, work, group, prefix_table=None, scale=None):
     return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+# ---- the linear half of a hybrid decoder, for lines decoded together
+
+def _lines(cu, line):
+    """What the operators read of a plan."""
+    return kernels.LinesPlan(None, None, None, line, cu, None, None, None, 0, 0)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::lines_conv", mutates_args=("state",))
+def lines_conv(x: Tensor, weight: Tensor, state: Tensor, cu: Tensor, line: Tensor, bias: Optional[Tensor] = None,
+               silu: bool = True) -> Tensor:
+    """The causal convolution of each line's tokens (cu and line: a plan's), the state updated in place: kernels.lines_conv."""
+    return kernels.lines_conv(x, weight, state, _lines(cu, line), bias, silu)
+
+
+@lines_conv.register_fake
+def _(x, weight, state, cu, line, bias=None, silu=True):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::lines_delta", mutates_args=("state",))
+def lines_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, state: Tensor, cu: Tensor, line: Tensor,
+                beta: Optional[Tensor] = None, a_log: Optional[Tensor] = None, dt_bias: Optional[Tensor] = None,
+                eps: Optional[float] = 1e-6, scale: Optional[float] = None) -> Tensor:
+    """Linear attention with decays over a state of each line (cu and line: a plan's), the state updated in place:
+    kernels.lines_delta."""
+    return kernels.lines_delta(q, k, v, decay, state, _lines(cu, line), beta, a_log, dt_bias, eps, scale)
+
+
+@lines_delta.register_fake
+def _(q, k, v, decay, state, cu, line, beta=None, a_log=None, dt_bias=None, eps=1e-6, scale=None):
+    return v.new_empty(v.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::gated_norm", mutates_args=())
+def gated_norm(x: Tensor, gate: Tensor, weight: Tensor, eps: float = 1e-6, unit_offset: bool = False,
+               activation: str = "silu") -> Tensor:
+    """The norm of each head with its gate: kernels.gated_norm."""
+    return kernels.gated_norm(x, gate, weight, eps, unit_offset, activation)
+
+
+@gated_norm.register_fake
+def _(x, gate, weight, eps=1e-6, unit_offset=False, activation="silu"):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::add_norm", mutates_args=())
+def add_norm(x: Tensor, residual: Tensor, weight: Tensor, post_weight: Optional[Tensor] = None,
+             gate: Optional[Tensor] = None, scale: float = 1.0, eps: float = 1e-6,
+             unit_offset: bool = False) -> tuple[Tensor, Tensor]:
+    """(sum, normed): a block joined to its residual with its norms: kernels.add_norm."""
+    return kernels.add_norm(x, residual, weight, post_weight, gate, scale, eps, unit_offset)
+
+
+@add_norm.register_fake
+def _(x, residual, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6, unit_offset=False):
+    return x.new_empty(x.shape), x.new_empty(x.shape)

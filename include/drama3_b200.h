@@ -321,6 +321,47 @@ int d3_lines_attention(const void* q, const int64_t* q_strides, int type, int T,
                        int B, float scale, void* out, float* lse, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* ---- The linear half of a hybrid decoder, for lines decoded together: three of four layers of the reference's decoder
+ * (drama3/config.py:59-60) are linear attention, which its host application computes. The pass's lines are given by cu
+ * [B + 1] (the first token of each) and line [T] (-1: no line's), a plan's (d3_lines_plan). B <= 8192. */
+
+/* out [T, C] = the causal convolution of each line's tokens x [T, C] (x_token: stride of a token, in elements) with a filter
+ * weight [C, W] a channel (2 <= W <= 8), plus bias [C] (or null), through SiLU with `silu`. weight and bias of the rows'
+ * type, or fp32 with w_f32. state [B, W - 1, C] of the rows' type: each line's last inputs, read and replaced; that of a line
+ * without tokens is left as it is. Places of no line get zeros. */
+int d3_lines_conv(const void* x, int64_t x_token, int type, int T, int C, const void* weight, const void* bias, int W,
+                  int w_f32, void* state, const int* cu, const int* line, int B, int silu, void* out, void* stream);
+
+/* Linear attention with a decay for each head, S [Dv, Dk] a line and value head: S <- e^g S; u = beta (v - S k) (the delta
+ * rule; u = v where beta is null); S <- S + u k^T; out = scale S q. q and k [T, Hk, Dk], v [T, Hv, Dv] (types 0 and 1,
+ * strides in elements for token and head, multiples of 8), out [T, Hv, Dv]; value head h reads key head h / (Hv / Hk).
+ * decay and beta [T, Hv] (stride of a token in elements; of the rows' type, or fp32 with gates_f32). With a_log [Hv] they
+ * are the projections' raw outputs, g = -exp(a_log) softplus(decay + dt_bias) (dt_bias [Hv] or null) and beta is
+ * sigmoid(beta); without it g = min(decay, 0). With eps >= 0 the rows of q and k are divided by sqrt(sum of squares + eps).
+ * state [B, Hv, Dv, Dk] fp32, read and replaced; that of a line without tokens is left as it is. Places of no line get
+ * zeros. Dk 64 or 128, Dv a multiple of 16 up to 256; q, k, v, out, state and workspace 16-byte aligned. The workspace is
+ * scratch (d3_lines_delta_workspace() bytes, which may be 0; no initial value) of this call alone until its launches have
+ * run. */
+size_t d3_lines_delta_workspace(int T, int B, int Hk, int Hv, int Dk);
+int d3_lines_delta(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, int type, int T, int Hk, int Hv, int Dk, int Dv, const void* decay,
+                   int64_t decay_token, const void* beta, int64_t beta_token, int gates_f32, const float* a_log,
+                   const float* dt_bias, float eps, float scale, float* state, const int* cu, const int* line, int B,
+                   void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out [T, H, D] = x / sqrt(mean(x^2) + eps) * (weight + w_add) * act(gate) for each head, act 0 SiLU, 1 the sigmoid; x and
+ * gate [T, H, D] (strides in elements for token and head), weight [D] of the rows' type, or fp32 with w_f32. */
+int d3_gated_norm(const void* x, const int64_t* x_strides, const void* gate, const int64_t* gate_strides, int type, int T,
+                  int H, int D, const void* weight, int w_f32, float w_add, float eps, int act, void* out, void* stream);
+
+/* sum_out [T, W] = residual + scale * gate * x', x' = x, or with `post` [W] x / sqrt(mean(x^2) + eps) * (post + w_add); and
+ * norm_out [T, W] = s / sqrt(mean(s^2) + eps) * (weight + w_add) of that sum s before it is rounded. gate_kind 0: no gate, 1:
+ * one value a row (gate[t * gate_token]), 2: one each (gate[t * gate_token + c]; gate_token 0: one a channel), of the rows'
+ * type. x_token, r_token, gate_token: strides of a row in elements. weight and post of the rows' type, or fp32 with w_f32. */
+int d3_add_norm(const void* x, int64_t x_token, const void* residual, int64_t r_token, int type, int T, int W,
+                const void* weight, const void* post, int w_f32, float w_add, const void* gate, int64_t gate_token,
+                int gate_kind, float scale, float eps, void* sum_out, void* norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
