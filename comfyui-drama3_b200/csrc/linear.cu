@@ -5,7 +5,7 @@
 #include "block_norm.cuh"
 #include "host.cuh"
 #include "lines_conv.cuh"
-#include "lines_delta.cuh"
+#include "lines_delta_chunk.cuh"
 
 using namespace d3host;
 
@@ -76,8 +76,61 @@ int conv_type(const d3::LcArgs& a, bool vectors, cudaStream_t s) {
   }
 }
 
+// Whether lines_delta goes token by token (or in chunks).
+bool delta_steps(int T, int B) { return T <= 2 * B || T <= 8; }
+
+size_t delta_block_bytes(int Hk, int Hv, int Dk) {
+  return (size_t)Hk * (Dk == 64 ? sizeof(d3::LdRows<64>) : sizeof(d3::LdRows<128>)) + (size_t)Hv * sizeof(d3::LdHead);
+}
+
+// Chunks prepared and scanned by a pair of launches: so many that what the preparation leaves stays in L2 until it is read.
+int delta_blocks(int T, int Hk, int Hv, int Dk) {
+  const size_t fit = (64u << 20) / delta_block_bytes(Hk, Hv, Dk), all = ((size_t)T + d3::LD_C - 1) / d3::LD_C;
+  return (int)(all < fit ? all : fit < 8 ? 8 : fit);
+}
+
+template <int TYPE, int DK, bool DELTA, int WARPS>
+int scan_launch(const CUtensorMap& vmap, const d3::LdChunkArgs& c, cudaStream_t s) {
+  constexpr int smem = d3::LdScanShape<DK, WARPS, DELTA>::SMEM;
+  static std::atomic<uint64_t> done{0};
+  if (int st = allow_smem_once(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS>, smem, done)) return st;
+  const dim3 blocks((c.a.Dv / 16 + WARPS - 1) / WARPS, c.a.Hv, c.a.B + 1);
+  return launch(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS>, blocks, dim3((WARPS + 1) * 32), smem, s, true, vmap, c);
+}
+
+template <int TYPE, int DK, bool DELTA>
+int chunk_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cudaStream_t s) {
+  constexpr int prep_smem = d3::LdPrepShape<DK>::SMEM;
+  static std::atomic<uint64_t> done{0};
+  if (int st = allow_smem_once(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, prep_smem, done)) return st;
+  CUtensorMap vmap;
+  cuuint64_t dims[3] = {(cuuint64_t)a.Dv, (cuuint64_t)a.Hv, (cuuint64_t)a.T};
+  cuuint64_t strides[2] = {(cuuint64_t)a.v.head * 2, (cuuint64_t)a.v.token * 2};
+  cuuint32_t box[3] = {16, 1, d3::LD_C};
+  if (!encode_tiled(&vmap, TYPE == d3::QR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.v.p,
+                    dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B))
+    return D3_ERR_ARG;
+  const int all = (int)(((long long)a.T + d3::LD_C - 1) / d3::LD_C), most = delta_blocks(a.T, a.Hk, a.Hv, DK);
+  d3::LdChunkArgs c = {a, 0, 0, workspace, nullptr};
+  for (; c.block0 < all; c.block0 += most) {
+    c.blocks = all - c.block0 < most ? all - c.block0 : most;
+    c.heads = (d3::LdHead*)((char*)workspace + (size_t)c.blocks * a.Hk * sizeof(d3::LdRows<DK>));
+    if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hk), dim3(d3::LP2_THREADS), prep_smem, s,
+                        true, c))
+      return st;
+    // a whole head of 128 a CTA shares its operands; fewer rows a CTA where that leaves SMs idle
+    const long long wide = (long long)a.B * a.Hv * ((a.Dv + 127) / 128);
+    if (int st = wide >= d.sms && a.Dv > 64 ? scan_launch<TYPE, DK, DELTA, 8>(vmap, c, s)
+                                            : scan_launch<TYPE, DK, DELTA, 4>(vmap, c, s))
+      return st;
+  }
+  return D3_OK;
+}
+
 template <int TYPE, int DK>
-int delta_launch(const d3::LdArgs& a, cudaStream_t s) {
+int delta_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cudaStream_t s) {
+  if (!delta_steps(a.T, a.B))
+    return a.beta ? chunk_launch<TYPE, DK, true>(a, workspace, d, s) : chunk_launch<TYPE, DK, false>(a, workspace, d, s);
   constexpr int rows = d3::LS_WARPS * d3::LS_ROWS * (128 / DK);
   const dim3 blocks((a.Dv + rows - 1) / rows, a.Hv, a.B + 1), threads(d3::LS_WARPS * 32);
   return a.beta ? launch(d3::lines_delta_step_kernel<TYPE, DK, true>, blocks, threads, 0, s, true, a)
@@ -170,7 +223,10 @@ int d3_lines_conv(const void* x, int64_t x_token, int type, int T, int C, const 
   }
 }
 
-size_t d3_lines_delta_workspace(int, int, int, int, int) { return 0; }
+size_t d3_lines_delta_workspace(int T, int B, int Hk, int Hv, int Dk) {
+  if (T < 1 || Hk < 1 || Hv < 1 || delta_steps(T, B)) return 0;
+  return delta_blocks(T, Hk, Hv, Dk) * delta_block_bytes(Hk, Hv, Dk);
+}
 
 int d3_lines_delta(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                    const int64_t* v_strides, int type, int T, int Hk, int Hv, int Dk, int Dv, const void* decay,
@@ -185,9 +241,14 @@ int d3_lines_delta(const void* q, const int64_t* q_strides, const void* k, const
   if (!q || !q_strides || !k || !k_strides || !v || !v_strides || !decay || !state || !cu || !line || !out) return D3_ERR_ARG;
   const int gsize = gates_f32 ? 4 : 2;
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(state, 16) ||
-      !aligned(decay, gsize) || !aligned(beta, gsize) || !aligned(a_log, 4) || !aligned(dt_bias, 4) ||
+      !aligned(workspace, 128) || !aligned(decay, gsize) || !aligned(beta, gsize) || !aligned(a_log, 4) || !aligned(dt_bias, 4) ||
       !multiple(q_strides, 2, 8) || !multiple(k_strides, 2, 8) || !multiple(v_strides, 2, 8))
     return D3_ERR_ALIGN;
+  const size_t need = d3_lines_delta_workspace(T, B, Hk, Hv, Dk);
+  if (need && !workspace) return D3_ERR_ARG;
+  if (workspace_bytes < need) return D3_ERR_WORKSPACE;
+  for (int i = 0; i < 2; ++i)
+    if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 1) return D3_ERR_ARG;
   DeviceInfo d;
   if (int st = device_info(&d)) return st;
   const d3::LdArgs a = {{q, q_strides[0], q_strides[1]}, {k, k_strides[0], k_strides[1]}, {v, v_strides[0], v_strides[1]},
@@ -195,8 +256,9 @@ int d3_lines_delta(const void* q, const int64_t* q_strides, const void* k, const
                         state, cu, line, out};
   cudaStream_t s = (cudaStream_t)stream;
   const bool f16 = type == d3::QR_F16;
-  if (Dk == 64) return f16 ? delta_launch<d3::QR_F16, 64>(a, s) : delta_launch<d3::QR_BF16, 64>(a, s);
-  return f16 ? delta_launch<d3::QR_F16, 128>(a, s) : delta_launch<d3::QR_BF16, 128>(a, s);
+  if (Dk == 64)
+    return f16 ? delta_launch<d3::QR_F16, 64>(a, workspace, d, s) : delta_launch<d3::QR_BF16, 64>(a, workspace, d, s);
+  return f16 ? delta_launch<d3::QR_F16, 128>(a, workspace, d, s) : delta_launch<d3::QR_BF16, 128>(a, workspace, d, s);
 }
 
 }  // extern "C"

@@ -73,4 +73,13 @@ D3_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_
       : "memory");
 }
 
+// Box of a 3-D map.
+D3_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+
 }  // namespace d3

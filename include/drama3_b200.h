@@ -339,7 +339,8 @@ int d3_lines_conv(const void* x, int64_t x_token, int type, int T, int C, const 
  * are the projections' raw outputs, g = -exp(a_log) softplus(decay + dt_bias) (dt_bias [Hv] or null) and beta is
  * sigmoid(beta); without it g = min(decay, 0). With eps >= 0 the rows of q and k are divided by sqrt(sum of squares + eps).
  * state [B, Hv, Dv, Dk] fp32, read and replaced; that of a line without tokens is left as it is. Places of no line get
- * zeros. Dk 64 or 128, Dv a multiple of 16 up to 256; q, k, v, out, state and workspace 16-byte aligned. The workspace is
+ * zeros. Dk 64 or 128, Dv a multiple of 16 up to 256; q, k, v, out and state 16-byte aligned, the
+ * workspace 128-byte. It is
  * scratch (d3_lines_delta_workspace() bytes, which may be 0; no initial value) of this call alone until its launches have
  * run. */
 size_t d3_lines_delta_workspace(int T, int B, int Hk, int Hv, int Dk);

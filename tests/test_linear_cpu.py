@@ -40,7 +40,7 @@ def test_conv_refusals(lib, change, status):
 def delta_args(**change):
     args = dict(q=16, qs=strides(512, 128), k=16, ks=strides(512, 128), v=16, vs=strides(1024, 128), type=0, T=4, Hk=4, Hv=8,
                 Dk=128, Dv=128, decay=16, decay_token=8, beta=16, beta_token=8, gates_f32=0, a_log=None, dt_bias=None, eps=1e-6,
-                scale=0.1, state=16, cu=16, line=16, B=2, out=16, ws=16, bytes=1 << 40, stream=None)
+                scale=0.1, state=16, cu=16, line=16, B=2, out=16, ws=128, bytes=1 << 40, stream=None)
     assert set(change) <= set(args)
     return list({**args, **change}.values())
 
@@ -53,9 +53,18 @@ def delta_args(**change):
                                                              "out")],
     *[({name: 24}, 2) for name in ("q", "k", "v", "state", "out")], (dict(decay=17), 2), (dict(beta=17), 2),
     (dict(decay=18, gates_f32=1), 2), (dict(a_log=18), 2), (dict(dt_bias=18), 2), (dict(qs=strides(516, 128)), 2),
-    (dict(ks=strides(512, 132)), 2), (dict(vs=strides(1028, 128)), 2), (dict(T=0), 0)])
+    (dict(ks=strides(512, 132)), 2), (dict(vs=strides(1028, 128)), 2), (dict(ws=64), 2), (dict(T=100, ws=None), 1),
+    (dict(T=100, bytes=1000), 5), (dict(qs=strides(-512, 128)), 1), (dict(vs=strides(0, 128)), 1), (dict(T=0), 0)])
 def test_delta_refusals(lib, change, status):
     assert lib.d3_lines_delta(*delta_args(**change)) == status
+
+
+def test_delta_workspace(lib):
+    assert lib.d3_lines_delta_workspace(16, 16, 16, 32, 128) == 0 and lib.d3_lines_delta_workspace(0, 1, 1, 1, 64) == 0
+    one = 2 * 64 * 128 * 2 + 2 * (3 * 64 * 64 * 2 + 6 * 64 * 4)  # a chunk of one key and two value heads
+    assert lib.d3_lines_delta_workspace(64, 1, 1, 2, 128) == one and lib.d3_lines_delta_workspace(65, 1, 1, 2, 128) == 2 * one
+    # a pass of any length is cut into parts of bounded scratch
+    assert lib.d3_lines_delta_workspace(1 << 24, 1, 16, 32, 128) <= 64 << 20
 
 
 def gated_args(**change):
