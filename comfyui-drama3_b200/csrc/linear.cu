@@ -80,7 +80,8 @@ int conv_type(const d3::LcArgs& a, bool vectors, cudaStream_t s) {
 bool delta_steps(int T, int B) { return T <= 2 * B || T <= 8; }
 
 size_t delta_block_bytes(int Hk, int Hv, int Dk) {
-  return (size_t)Hk * (Dk == 64 ? sizeof(d3::LdRows<64>) : sizeof(d3::LdRows<128>)) + (size_t)Hv * sizeof(d3::LdHead);
+  return Dk == 64 ? Hk * sizeof(d3::LdRows<64>) + Hv * sizeof(d3::LdHead<64>)
+                  : Hk * sizeof(d3::LdRows<128>) + Hv * sizeof(d3::LdHead<128>);
 }
 
 // Chunks prepared and scanned by a pair of launches: so many that what the preparation leaves stays in L2 until it is read.
@@ -91,7 +92,7 @@ int delta_blocks(int T, int Hk, int Hv, int Dk) {
 
 template <int TYPE, int DK, bool DELTA, int WARPS>
 int scan_launch(const CUtensorMap& vmap, const d3::LdChunkArgs& c, cudaStream_t s) {
-  constexpr int smem = d3::LdScanShape<DK, WARPS, DELTA>::SMEM;
+  constexpr int smem = d3::LdScanShape<DK, WARPS>::SMEM;
   static std::atomic<uint64_t> done{0};
   if (int st = allow_smem_once(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS>, smem, done)) return st;
   const dim3 blocks((c.a.Dv / 16 + WARPS - 1) / WARPS, c.a.Hv, c.a.B + 1);
@@ -114,8 +115,8 @@ int chunk_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cuda
   d3::LdChunkArgs c = {a, 0, 0, workspace, nullptr};
   for (; c.block0 < all; c.block0 += most) {
     c.blocks = all - c.block0 < most ? all - c.block0 : most;
-    c.heads = (d3::LdHead*)((char*)workspace + (size_t)c.blocks * a.Hk * sizeof(d3::LdRows<DK>));
-    if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hk), dim3(d3::LP2_THREADS), prep_smem, s,
+    c.heads = (char*)workspace + (size_t)c.blocks * a.Hk * sizeof(d3::LdRows<DK>);
+    if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hv), dim3(d3::LD_PREP_THREADS), prep_smem, s,
                         true, c))
       return st;
     // a whole head of 128 a CTA shares its operands; fewer rows a CTA where that leaves SMs idle

@@ -1,23 +1,26 @@
 // Linear attention (lines_delta.cuh has the formulas) over many tokens of a line: in chunks of 64 tokens, with the products on
 // the tensor cores. With G_i the sum of the log decays from the chunk's first token on, gamma_i = exp(G_i), and the rows of a
-// chunk's Q, K, V and of the corrections U:
-//   (I + A) U = diag(beta) (V - diag(gamma) K S^T),   A_ij = beta_i exp(G_i - G_j) k_i . k_j  (j < i)
-//   O = scale (diag(gamma) Q S^T + P U),              P_ij = exp(G_i - G_j) q_i . k_j  (j <= i)
-//   S <- gamma_last S + (diag(exp(G_last - G_j)) U)^T K
-// so that what depends on the tokens alone, (I + A)^-1 diag(beta) and P, is formed for all chunks at once (the preparation),
-// and the chain from chunk to chunk (the scan) has four products left. Exponents are differences that are never above 0, of
-// sums in 64 bits.
+// chunk's Q, K, V, the corrections U solve a triangular system:
+//   U = T R,  R = V - diag(gamma) K S^T,  T = (I + A)^-1 diag(beta),  A_ij = beta_i exp(G_i - G_j) k_i . k_j  (j < i)
+//   O = scale (diag(gamma) Q S^T + P U),  P_ij = exp(G_i - G_j) q_i . k_j  (j <= i)
+//   S <- gamma_last S + U^T D K,          D = diag(exp(G_last - G_j))
+// What depends on the tokens alone is formed for all chunks at once (the preparation): not T itself, but P T and K~ = T^T D K,
+// with which U is never needed: O = scale (diag(gamma) Q S^T + (P T) R), S <- gamma_last S + R^T K~. So the chain from chunk
+// to chunk (the scan) has two products, S -> R -> S. Row j of K~ is what is left at the chunk's end of what token j wrote:
+// beta_j k_j through the later tokens' decays and corrections, which only shrink it. Without the delta rule R = V, T = I.
+// Exponents are differences that are never above 0, of sums in 64 bits.
 //
 // Chunks are cut from the packed tokens, whatever lines they belong to: entries of two lines are zeros, sums and exponents
 // start again with each line. A line's scan masks the tokens of others.
 //
 // Values. k and q become fp16 rows times powers of two, exactly (values below 2^-14 of the row's largest lose what is below
-// 2^-25 of it), and their norms are numbers that the results are multiplied by. What is not exact in 16 bits, S, the right-hand
-// sides, U and the inverse, is the sum of two fp16 terms, 22 bits, each row scaled by a power of two of its own; their products
-// are summed in 32 bits and the smallest of four, low times low, left out (2^-22). S itself stays in 32 bits. For the outputs, which are
-// rounded to 16 bits anyway, one term of S, P and U is enough: 2^-12 of each.
+// 2^-25 of it), and their norms are numbers that results are multiplied by. What is not exact in 16 bits, S, R, T, P and K~, is
+// the sum of two fp16 terms, 22 bits, each row scaled by a power of two of its own; products are summed in 32 bits, and of the
+// four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. For the outputs,
+// which are rounded to 16 bits anyway, the scan takes one term of S, P T and R: 2^-12 of each.
 //
-// A value that is not finite reaches the state and the tokens of its own line, in its chunk earlier ones too.
+// A value that is not finite reaches the state and the tokens of its own line, in its chunk earlier ones too; one in q its own
+// token only.
 #pragma once
 
 #include "lines_delta.cuh"
@@ -31,14 +34,13 @@ constexpr int LD_C = 64;  // tokens of a chunk
 template <int DK> struct alignas(128) LdRows {
   uint16_t k[LD_C * DK], q[LD_C * DK];
 };
-// ... and for a value head: rows [64][64] likewise, and factors of the tokens' columns.
-struct alignas(128) LdHead {
-  uint16_t t_hi[LD_C * LD_C], t_lo[LD_C * LD_C];  // (I + A)^-1 diag(beta), row i times 1 / t_scale[i]
-  uint16_t p[LD_C * LD_C];                        // P, row i times 1 / p_scale[i]
-  float t_scale[LD_C], p_scale[LD_C];
+// ... and for a value head: rows likewise, and factors of the tokens' columns.
+template <int DK> struct alignas(128) LdHead {
+  uint16_t kt_hi[LD_C * DK], kt_lo[LD_C * DK];  // K~ [64][Dk], row j times 1 / kt_scale[j]
+  uint16_t p[LD_C * LD_C];                      // P T [64][64], row i times 1 / p_scale[i]
+  float kt_scale[LD_C], p_scale[LD_C];
   float r_in[LD_C];   // gamma_i |k| factor: of K S^T
   float q_in[LD_C];   // scale gamma_i |q| factor: of Q S^T
-  float k_out[LD_C];  // exp(G_last - G_j) |k| factor: of U in the state
   float gamma[LD_C];
 };
 
@@ -49,14 +51,12 @@ template <int PIECES> D3_DEV int ld_at(int r, int c) { return (r * PIECES + (c ^
 D3_DEV void ld_matrix4(uint32_t (&r)[4], const uint16_t* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(smem_u32(p))
-               : "memory");
+               : "r"(smem_u32(p)));
 }
 D3_DEV void ld_matrix4_trans(uint32_t (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(smem_u32(p))
-               : "memory");
+               : "r"(smem_u32(p)));
 }
 D3_DEV void st_matrix4_trans(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(smem_u32(p)), "r"(a), "r"(b), "r"(c),
@@ -64,7 +64,7 @@ D3_DEV void st_matrix4_trans(void* p, uint32_t a, uint32_t b, uint32_t c, uint32
                : "memory");
 }
 D3_DEV void ld_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm (
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -92,49 +92,95 @@ struct LdChunkArgs {
   LdArgs a;
   int block0, blocks;  // of the pass's blocks of 64 tokens, those of this launch
   void* rows;          // [blocks][Hk] LdRows
-  LdHead* heads;       // [blocks][Hv]
+  void* heads;         // [blocks][Hv] LdHead
 };
 
-// ---- The preparation. A CTA per chunk and key head; its value heads two at a time. k and q come in as 16-bit rows and go out as
-// fp16 ones; K K^T and Q K^T are mma.sync products whose results stay in registers for all value heads. The inverse of I + A is
-// found by columns, a thread each: x_i = [i = j] - sum_{m < i} A_im x_m, with x in registers and A's entries broadcast from
-// shared memory, updating all later rows as soon as x_m is known so that the additions do not wait for one another.
-constexpr int LP2_THREADS = 128;
-constexpr int LD_PITCH = 68;  // floats of a column of A (and of a row of the inverse) in shared memory
+// ---- The preparation. A CTA per chunk and value head; the first of a key head's leaves the rows. K K^T and Q K^T are mma.sync
+// products. T: the 16 x 16 blocks on the diagonal of I + A are inverted by columns, a thread each, then blocks of 32 and of 64 by
+// [T1, 0; X, T2], X = -T2 A21 T1, in 32 bits. (By columns of all 64 at once the same numbers took 2000 unrolled steps and the
+// time went into fetching instructions.) K~ = T^T D K and P T are products of two fp16 terms each.
+constexpr int LD_PREP_THREADS = 128;
+constexpr int LD_PITCH = 68;    // floats of a row of A and T in shared memory
+constexpr int LD_PITCH_Y = 36;  // ... of A21 T1
+constexpr float LD_MAX = 3.4028234e38f;
 
 template <int DK> struct LdPrepShape {
-  static constexpr int ROWS = 2 * LD_C * DK * 2, A = LD_C * LD_PITCH * 4;
-  static constexpr int SMEM = ROWS + 2 * A;
+  static constexpr int K = LD_C * DK * 2, T = 2 * LD_C * LD_C * 2;
+  static constexpr int Q = K > T ? K : T;  // the rows of q, then T^T
+  static constexpr int A = LD_C * LD_PITCH * 4, Y = 32 * LD_PITCH_Y * 4;
+  static constexpr int SMEM = K + Q + T + A + Y;
+  static_assert(A >= K && T >= K, "K~'s terms take the places of A and of T^T D");
 };
 
+// X = -T2 (A21 T1) for the blocks of N x N at rows r0 + N.., columns r0..: `threads` threads, of which this is number t.
+template <int N, int THREADS> D3_DEV void ld_join(float* A, float* Y, const int* line_s, int r0, int t) {
+  constexpr int COLS = N * N / THREADS, PER = N / COLS;  // columns a thread, threads a row
+  const int r = t / PER, c = t % PER * COLS;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    float acc[COLS] = {};
+#pragma unroll 8
+    for (int m = 0; m < N; ++m) {
+      const float x = A[(r0 + N + r) * LD_PITCH + r0 + (pass ? N : 0) + m];
+      const float* y = pass ? Y + m * LD_PITCH_Y + c : A + (r0 + m) * LD_PITCH + r0 + c;
+#pragma unroll
+      for (int e = 0; e < COLS; e += 4) {
+        const float4 v = *(const float4*)(y + e);
+        acc[e] = fmaf(x, v.x, acc[e]), acc[e + 1] = fmaf(x, v.y, acc[e + 1]);
+        acc[e + 2] = fmaf(x, v.z, acc[e + 2]), acc[e + 3] = fmaf(x, v.w, acc[e + 3]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) {
+      if (pass)  // entries of two lines are zeros whatever the sums met
+        A[(r0 + N + r) * LD_PITCH + r0 + c + e] = line_s[r0 + N + r] == line_s[r0 + c + e] ? -acc[e] : 0.0f;
+      else
+        Y[r * LD_PITCH_Y + c + e] = acc[e];
+    }
+    __syncthreads();
+  }
+}
+
 template <int TYPE, int DK, bool DELTA>
-__global__ void __launch_bounds__(LP2_THREADS, 3) lines_delta_prep_kernel(LdChunkArgs c) {
+__global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(LdChunkArgs c) {
   using TT = QrType<TYPE>;
   using E = typename TT::T;
+  using Shape = LdPrepShape<DK>;
   constexpr int PIECES = DK / 8, LANES = PIECES, AT_ONCE = 32 / LANES;
   extern __shared__ __align__(128) uint8_t ld_smem[];
   uint16_t* const ks = (uint16_t*)ld_smem;
-  uint16_t* const qs = ks + LD_C * DK;
-  float* const As = (float*)(ld_smem + LdPrepShape<DK>::ROWS);  // [2][64 columns][LD_PITCH]
+  uint16_t* const qs = (uint16_t*)(ld_smem + Shape::K);
+  uint16_t* const tt = qs;                                              // T^T, two terms, where q was
+  uint16_t* const td = (uint16_t*)(ld_smem + Shape::K + Shape::Q);      // T^T D, two terms
+  float* const A = (float*)(ld_smem + Shape::K + Shape::Q + Shape::T);  // A, then T
+  float* const Y = A + LD_C * LD_PITCH;
   __shared__ int line_s[LD_C];
-  __shared__ int last_s[LD_C];  // the last token of token i's line in the chunk
-  __shared__ float k_factor[LD_C], q_factor[LD_C];
-  __shared__ double G_s[2][LD_C];
-  __shared__ float beta_s[2][LD_C];
-  __shared__ int bad_s[2][LD_C];  // row i of the inverse has a value that is not finite
+  __shared__ uint32_t starts_s[2];
+  __shared__ float k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], d_s[LD_C], t_scale[LD_C], kt_scale[LD_C];
+  __shared__ double G_s[LD_C];
+  __shared__ int bad_s[LD_C];  // by a line's first token in the chunk: something of it is not finite
   const LdArgs& a = c.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
-  const int block = blockIdx.x, hk = blockIdx.y, many = a.Hv / a.Hk;
+  const int block = blockIdx.x, h = blockIdx.y, many = a.Hv / a.Hk, hk = h / many;
   const long long t0 = (long long)(c.block0 + block) * LD_C;
+  LdHead<DK>* const out = (LdHead<DK>*)c.heads + (size_t)block * a.Hv + h;
   grid_dependency_wait();
   allow_dependents();
+  float decay = 0.0f, beta = 0.0f;
+  int my_line = -1;
   if (tid < LD_C) {
     const int l = t0 + tid < a.T ? a.line[t0 + tid] : -1;
-    line_s[tid] = l >= 0 && l < a.B ? l : -1;
+    my_line = l >= 0 && l < a.B ? l : -1;
+    line_s[tid] = my_line;
+    bad_s[tid] = 0;
+    if (my_line >= 0) {
+      decay = ld_log_decay<TYPE>(a, t0 + tid, h);
+      if (DELTA) beta = ld_beta<TYPE>(a, t0 + tid, h);
+    }
   }
   // rows to fp16, each by the power of two that brings its largest value into [1, 2)
   const int l = lane % LANES;
-#pragma unroll 2
+#pragma unroll 4
   for (int i = 0; i < 2 * LD_C / 4; i += AT_ONCE) {  // a warp: 16 rows of k, then 16 of q
     const int at = i + lane / LANES;
     const bool is_q = at >= LD_C / 4;
@@ -149,11 +195,11 @@ __global__ void __launch_bounds__(LP2_THREADS, 3) lines_delta_prep_kernel(LdChun
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       most = fmaxf(most, fabsf(v[e]));
-      finite = finite && fabsf(v[e]) <= 3.4028234e38f;
+      finite = finite && fabsf(v[e]) <= LD_MAX;
     }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const uint32_t group = (LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u)) << (lane / LANES * LANES);
+    const uint32_t group = ((1u << LANES) - 1u) << (lane / LANES * LANES);
     finite = (__ballot_sync(0xffffffffu, finite) & group) == group;
     float up, down;
     ld_scale(most, up, down);
@@ -175,173 +221,316 @@ __global__ void __launch_bounds__(LP2_THREADS, 3) lines_delta_prep_kernel(LdChun
     if (l == 0) (is_q ? q_factor : k_factor)[row] = is_q ? f * a.scale : f;
   }
   __syncthreads();
+  // sums of the log decays that start again with each line
+  double G = decay < -104.0f ? -104.0f : decay;  // exp of it is 0 already; keeps infinities out of the sums
+  int first = 0, last = 0;
+  if (warp < 2) {
+    const uint32_t starts = __ballot_sync(0xffffffffu, tid == 0 || line_s[tid - 1] != my_line);
+    if (lane == 0) starts_s[warp] = starts;
+    const int from = 31 - __clz(starts & (0xffffffffu >> (31 - lane)));  // in this warp; -1: before it
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double before = __shfl_up_sync(0xffffffffu, G, o);
+      if (lane - o >= max(from, 0)) G += before;
+    }
+    G_s[tid] = G;
+  }
+  __syncthreads();
+  const unsigned long long starts = starts_s[0] | (unsigned long long)starts_s[1] << 32;
+  auto first_of = [&](int i) { return 63 - __clzll(starts & (~0ull >> (63 - i))); };
+  if (tid >= 32 && tid < LD_C && first_of(tid) < 32) G_s[tid] = G + G_s[31];
   if (tid < LD_C) {
-    int last = tid;
-    while (last + 1 < LD_C && line_s[last + 1] == line_s[tid]) ++last;
-    last_s[tid] = last;
+    first = first_of(tid);
+    const unsigned long long later = tid == 63 ? 0 : starts >> (tid + 1);
+    last = later ? tid + __ffsll((long long)later) - 1 : 63;
   }
+  __syncthreads();
+  if (tid < LD_C) {
+    G = G_s[tid];
+    float kf = k_factor[tid];
+    if (my_line >= 0 && !(fabsf(kf) <= LD_MAX && fabsf((float)G) <= LD_MAX && fabsf(beta) <= LD_MAX)) {
+      bad_s[first] = 1;
+      beta = 0.0f;
+    }
+    beta_s[tid] = beta;
+    d_s[tid] = my_line >= 0 ? expf((float)(G_s[last] - G)) * kf : 0.0f;
+  }
+  __syncthreads();
   // K K^T and Q K^T: rows 16 warp + g, + 8, columns 8 n + 2 cc, + 1 up to the diagonal
-  float kk[8][4] = {}, qk[8][4] = {};
-#pragma unroll
-  for (int kt = 0; kt < DK / 16; ++kt) {
-    uint32_t ak[4], aq[4];
-    const int ar = warp * 16 + (lane & 15), ap = kt * 2 + (lane >> 4);
-    if (DELTA) ld_matrix4(ak, ks + ld_at<PIECES>(ar, ap));
-    ld_matrix4(aq, qs + ld_at<PIECES>(ar, ap));
-#pragma unroll
-    for (int n = 0; n < 8; n += 2)
-      if (n <= 2 * warp) {
-        uint32_t b[4];
-        ld_matrix4(b, ks + ld_at<PIECES>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-        if (DELTA) ld_mma(kk[n], ak, b[0], b[1]), ld_mma(kk[n + 1], ak, b[2], b[3]);
-        ld_mma(qk[n], aq, b[0], b[1]), ld_mma(qk[n + 1], aq, b[2], b[3]);
-      }
-  }
-  // the rows, as every value head's scan reads them
+  float p[8][4] = {};
   {
-    LdRows<DK>* out = (LdRows<DK>*)c.rows + (size_t)block * a.Hk + hk;
-    const uint4* from = (const uint4*)ks;
-    for (int i = tid; i < (int)sizeof(LdRows<DK>) / 16; i += LP2_THREADS) ((uint4*)out)[i] = from[i];
+    float kk[8][4] = {};
+#pragma unroll
+    for (int kt = 0; kt < DK / 16; ++kt) {
+      uint32_t ak[4], aq[4];
+      const int ar = warp * 16 + (lane & 15), ap = kt * 2 + (lane >> 4);
+      if (DELTA) ld_matrix4(ak, ks + ld_at<PIECES>(ar, ap));
+      ld_matrix4(aq, qs + ld_at<PIECES>(ar, ap));
+#pragma unroll
+      for (int n = 0; n < 8; n += 2)
+        if (n <= 2 * warp) {
+          uint32_t b[4];
+          ld_matrix4(b, ks + ld_at<PIECES>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+          if (DELTA) ld_mma(kk[n], ak, b[0], b[1]), ld_mma(kk[n + 1], ak, b[2], b[3]);
+          ld_mma(p[n], aq, b[0], b[1]), ld_mma(p[n + 1], aq, b[2], b[3]);
+        }
+    }
+    float qf[2], kf[2], bt[2];
+    double Gi[2];
+    int li[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = warp * 16 + g + r * 8;
+      qf[r] = q_factor[i], kf[r] = k_factor[i] * beta_s[i], Gi[r] = G_s[i], li[r] = line_s[i];
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = n * 8 + cc * 2 + x;
+        float kfj = 0.0f;
+        double Gj = 0.0;
+        int lj = -1;
+        if (n <= 2 * warp + 1) kfj = k_factor[j], Gj = G_s[j], lj = line_s[j];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = warp * 16 + g + r * 8, e = r * 2 + x;
+          float pv = 0.0f, av = 0.0f;
+          if (n <= 2 * warp + 1 && j <= i && li[r] == lj && lj >= 0) {
+            const float ratio = expf((float)(Gi[r] - Gj)) * kfj;
+            pv = ratio * qf[r] * p[n][e];
+            if (DELTA && j < i) av = ratio * kf[r] * kk[n][e];
+          }
+          if (DELTA) {
+            if (!(fabsf(av) <= LD_MAX)) bad_s[first_of(i)] = 1, av = 0.0f;
+            A[i * LD_PITCH + j] = av;
+          }
+          p[n][e] = pv;
+        }
+      }
   }
-  for (int y0 = 0; y0 < many; y0 += 2) {
-    const int n_heads = min(2, many - y0);
-    __syncthreads();
-    {  // gates: two threads of a token's two heads; sums of the log decays that start again with each line
-      const int y = tid >> 6, i = tid & 63, h = hk * many + y0 + y;
-      double G = 0.0;
-      float beta = 0.0f;
-      if (y < n_heads && line_s[i] >= 0) {
-        const float decay = ld_log_decay<TYPE>(a, t0 + i, h);
-        G = decay < -104.0f ? -104.0f : decay;  // exp of it is 0 already; keeps infinities out of the sums, and NaN in
-        if (DELTA) beta = ld_beta<TYPE>(a, t0 + i, h);
-      }
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double before = __shfl_up_sync(0xffffffffu, G, o);
-        if (lane >= o && line_s[i - o] == line_s[i]) G += before;
-      }
-      G_s[y][i] = G;
-      beta_s[y][i] = beta;
-      bad_s[y][i] = 0;
-      __syncthreads();
-      if (i >= 32 && line_s[31] == line_s[i]) G_s[y][i] += G_s[y][31];
+  __syncthreads();  // also: q has been read
+  if (h == hk * many) {  // the rows, as every value head's scan reads them
+    LdRows<DK>* rows = (LdRows<DK>*)c.rows + (size_t)block * a.Hk + hk;
+    for (int i = tid; i < (int)sizeof(rows->k) / 16; i += LD_PREP_THREADS) {
+      ((uint4*)rows->k)[i] = ((const uint4*)ks)[i];
+      ((uint4*)rows->q)[i] = ((const uint4*)qs)[i];
     }
-    __syncthreads();
-    for (int y = 0; y < n_heads; ++y) {
-      LdHead* out = c.heads + (size_t)block * a.Hv + hk * many + y0 + y;
-      float* A = As + y * LD_C * LD_PITCH;
-      float most[2] = {0.0f, 0.0f};
-      bool good[2] = {true, true};
-      float pv[8][4];
+  }
+  float most[2] = {0.0f, 0.0f};
+  bool good[2] = {true, true};
+  float tp[8][4];  // P T
+  if constexpr (DELTA) {
+    if (tid < LD_C) {  // the blocks on the diagonal
+      const int d = tid & ~15, j = tid & 15;
+      float x[16];
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int i = 0; i < 16; ++i) {
+        x[i] = i == j ? 1.0f : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = warp * 16 + g + (e >> 1) * 8, j = n * 8 + cc * 2 + (e & 1);
-          float p = 0.0f, x = 0.0f;
-          if (n <= 2 * warp + 1 && j <= i && line_s[i] == line_s[j] && line_s[i] >= 0) {
-            const float ratio = expf((float)(G_s[y][i] - G_s[y][j])) * k_factor[j];
-            p = ratio * q_factor[i] * qk[n][e];
-            if (DELTA && j < i) x = ratio * k_factor[i] * beta_s[y][i] * kk[n][e];
+        for (int m = 0; m < 16; m += 4)
+          if (m < i) {
+            const float4 v = *(const float4*)(A + (d + i) * LD_PITCH + d + m);
+            x[i] = fmaf(-v.x, x[m], x[i]);
+            if (m + 1 < i) x[i] = fmaf(-v.y, x[m + 1], x[i]);
+            if (m + 2 < i) x[i] = fmaf(-v.z, x[m + 2], x[i]);
+            if (m + 3 < i) x[i] = fmaf(-v.w, x[m + 3], x[i]);
           }
-          if (!(fabsf(p) <= 3.4028234e38f)) good[e >> 1] = false, p = 0.0f;
-          if (DELTA && !(fabsf(x) <= 3.4028234e38f)) bad_s[y][i] = 1, x = 0.0f;
-          most[e >> 1] = fmaxf(most[e >> 1], fabsf(p));
-          pv[n][e] = p;
-          if (DELTA) A[j * LD_PITCH + i] = x;
-        }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = warp * 16 + g + r * 8;
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], o));
-        const uint32_t row = 0xfu << (lane & ~3);
-        const bool all_good = (__ballot_sync(0xffffffffu, good[r]) & row) == row;
-        float up, down;
-        ld_scale(most[r], up, down);
-        if (cc == 0) out->p_scale[i] = all_good ? down : __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-          *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(pv[n][r * 2] * up, pv[n][r * 2 + 1] * up);
       }
-      if (tid < LD_C) {
-        const int i = tid;
-        const float gamma = expf((float)G_s[y][i]);
-        const bool live = line_s[i] >= 0;
-        out->gamma[i] = gamma;
-        out->q_in[i] = live ? gamma * q_factor[i] : 0.0f;
-        out->r_in[i] = live ? gamma * k_factor[i] : 0.0f;
-        out->k_out[i] = live ? expf((float)(G_s[y][last_s[i]] - G_s[y][i])) * k_factor[i] : 0.0f;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) A[(d + i) * LD_PITCH + d + j] = line_s[d + i] == line_s[d + j] ? x[i] : 0.0f;
+    }
+    __syncthreads();
+    ld_join<16, 64>(A, Y + (tid >> 6) * 16 * LD_PITCH_Y, line_s, (tid >> 6) * 32, tid & 63);
+    ld_join<32, 128>(A, Y, line_s, 0, tid);
+    {  // columns of T become rows of T^T and T^T D: two threads each, four rows by turns
+      const int j = tid >> 1, half = tid & 1;
+      const float b = beta_s[j];
+      float v[32], d[32], m_t = 0.0f, m_d = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int i = (e >> 2) * 8 + half * 4 + (e & 3);
+        v[e] = i >= j ? A[i * LD_PITCH + j] * b : 0.0f;
+        if (!(fabsf(v[e]) <= LD_MAX)) bad_s[first_of(j)] = 1, v[e] = 0.0f;
+        d[e] = v[e] != 0.0f ? v[e] * d_s[i] : 0.0f;  // nothing of another line, where that is not finite
+        if (!(fabsf(d[e]) <= LD_MAX)) bad_s[first_of(j)] = 1, d[e] = 0.0f;
+        m_t = fmaxf(m_t, fabsf(v[e])), m_d = fmaxf(m_d, fabsf(d[e]));
+      }
+      m_t = fmaxf(m_t, __shfl_xor_sync(0xffffffffu, m_t, 1));
+      m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
+      float up, down;
+      ld_scale(m_t, up, down);
+      if (half == 0) t_scale[j] = down;
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        uint2 hi, lo;
+        ld_split(v[e] * up, v[e + 1] * up, hi.x, lo.x), ld_split(v[e + 2] * up, v[e + 3] * up, hi.y, lo.y);
+        const int at = ld_at<8>(j, e >> 2) + half * 4;
+        *(uint2*)(tt + at) = hi, *(uint2*)(tt + LD_C * LD_C + at) = lo;
+      }
+      ld_scale(m_d, up, down);
+      if (half == 0) kt_scale[j] = m_d > 0.0f ? down * 0x1p6f : 0.0f;  // a row of zeros must not set a scale
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        uint2 hi, lo;
+        ld_split(d[e] * up, d[e + 1] * up, hi.x, lo.x), ld_split(d[e + 2] * up, d[e + 3] * up, hi.y, lo.y);
+        const int at = ld_at<8>(j, e >> 2) + half * 4;
+        *(uint2*)(td + at) = hi, *(uint2*)(td + LD_C * LD_C + at) = lo;
       }
     }
-    if constexpr (DELTA) {
-      __syncthreads();
-      const int y = tid >> 6, j = tid & 63;
-      float x[LD_C];
-      float* A = As + y * LD_C * LD_PITCH;
-      if (y < n_heads) {
+    __syncthreads();
+    // K~ = T^T D K: a warp has Dk / 4 columns
+    constexpr int N = DK / 32;
+    float kt[4][N][4] = {};
 #pragma unroll
-        for (int i = 0; i < LD_C; ++i) x[i] = i == j ? 1.0f : 0.0f;
+    for (int i = 0; i < 4; ++i) {  // 16 tokens i of the sum
+      uint32_t b[N][2];
 #pragma unroll
-        for (int m = 0; m < LD_C - 1; ++m) {
-#pragma unroll
-          for (int i = (m + 1) & ~3; i < LD_C; i += 4) {
-            const float4 v = *(const float4*)(A + m * LD_PITCH + i);
-            if (i > m) x[i] = fmaf(-v.x, x[m], x[i]);
-            if (i + 1 > m) x[i + 1] = fmaf(-v.y, x[m], x[i + 1]);
-            if (i + 2 > m) x[i + 2] = fmaf(-v.z, x[m], x[i + 2]);
-            if (i + 3 > m) x[i + 3] = fmaf(-v.w, x[m], x[i + 3]);
-          }
-        }
+      for (int n = 0; n < N; n += 2) {
+        uint32_t b4[4];
+        ld_matrix4_trans(b4, ks + ld_at<PIECES>(i * 16 + (lane & 15), warp * N + n + (lane >> 4)));
+        b[n][0] = b4[0], b[n][1] = b4[1], b[n + 1][0] = b4[2], b[n + 1][1] = b4[3];
       }
-      __syncthreads();
-      if (y < n_heads) {  // rows of the inverse, entries of two lines as zeros
-        const float beta = beta_s[y][j];
 #pragma unroll
-        for (int i = 0; i < LD_C; ++i) A[i * LD_PITCH + j] = line_s[i] == line_s[j] && i >= j ? x[i] * beta : 0.0f;
-      }
-      __syncthreads();
-      // a row's 64 values by two threads, 32 each
-      for (int y2 = 0; y2 < n_heads; ++y2) {
-        LdHead* out = c.heads + (size_t)block * a.Hv + hk * many + y0 + y2;
-        const int i = tid >> 1, half = tid & 1;
-        float* row = As + y2 * LD_C * LD_PITCH + i * LD_PITCH + half * 32;
-        float most = 0.0f;
-        bool good = bad_s[y2][i] == 0;
-        for (int e = 0; e < 32; ++e) {
-          if (!(fabsf(row[e]) <= 3.4028234e38f)) good = false, row[e] = 0.0f;
-          most = fmaxf(most, fabsf(row[e]));
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        good = __shfl_xor_sync(0xffffffffu, good, 1) && good;
-        float up, down;
-        ld_scale(most, up, down);
-        if (half == 0) out->t_scale[i] = good ? down : __uint_as_float(0x7fc00000u);
+      for (int j = 0; j <= i; ++j) {
+        uint32_t hi[4], lo[4];
+        const int at = ld_at<8>(j * 16 + (lane & 15), i * 2 + (lane >> 4));
+        ld_matrix4(lo, td + LD_C * LD_C + at);
+        ld_matrix4(hi, td + at);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          uint4 hi, lo;
-          const float4 v0 = *(const float4*)(row + p * 8), v1 = *(const float4*)(row + p * 8 + 4);
-          ld_split(v0.x * up, v0.y * up, hi.x, lo.x), ld_split(v0.z * up, v0.w * up, hi.y, lo.y);
-          ld_split(v1.x * up, v1.y * up, hi.z, lo.z), ld_split(v1.z * up, v1.w * up, hi.w, lo.w);
-          *(uint4*)(out->t_hi + ld_at<8>(i, half * 4 + p)) = hi;
-          *(uint4*)(out->t_lo + ld_at<8>(i, half * 4 + p)) = lo;
-        }
+        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], lo, b[n][0], b[n][1]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], hi, b[n][0], b[n][1]);
       }
     }
+    // P T: a warp has 16 rows
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!(fabsf(p[n][e]) <= LD_MAX)) good[e >> 1] = false, p[n][e] = 0.0f;
+        most[e >> 1] = fmaxf(most[e >> 1], fabsf(p[n][e]));
+        tp[n][e] = 0.0f;
+      }
+    float up[2], down[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], o));
+      ld_scale(most[r], up[r], down[r]);
+      most[r] = 0.0f;
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (m <= warp) {
+        uint32_t hi[4], lo[4];
+        ld_split(p[2 * m][0] * up[0], p[2 * m][1] * up[0], hi[0], lo[0]);
+        ld_split(p[2 * m][2] * up[1], p[2 * m][3] * up[1], hi[1], lo[1]);
+        ld_split(p[2 * m + 1][0] * up[0], p[2 * m + 1][1] * up[0], hi[2], lo[2]);
+        ld_split(p[2 * m + 1][2] * up[1], p[2 * m + 1][3] * up[1], hi[3], lo[3]);
+#pragma unroll
+        for (int n = 0; n <= 2 * m; n += 2) {
+          uint32_t b_hi[4], b_lo[4];
+          const int at = ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, m * 2 + ((lane >> 3) & 1));
+          ld_matrix4(b_hi, tt + at);
+          ld_matrix4(b_lo, tt + LD_C * LD_C + at);
+          ld_mma(tp[n], lo, b_hi[0], b_hi[1]), ld_mma(tp[n + 1], lo, b_hi[2], b_hi[3]);
+          ld_mma(tp[n], hi, b_lo[0], b_lo[1]), ld_mma(tp[n + 1], hi, b_lo[2], b_lo[3]);
+          ld_mma(tp[n], hi, b_hi[0], b_hi[1]), ld_mma(tp[n + 1], hi, b_hi[2], b_hi[3]);
+        }
+      }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 f = *(const float2*)(t_scale + n * 8 + cc * 2);
+      tp[n][0] *= f.x * down[0], tp[n][1] *= f.y * down[0], tp[n][2] *= f.x * down[1], tp[n][3] *= f.y * down[1];
+    }
+    __syncthreads();  // T^T D has been read
+    uint16_t* const kt_hi = (uint16_t*)A;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {  // at most 64 x 2^14 x 2: 2^-6 of it is an fp16 number
+          uint32_t hi, lo;
+          ld_split(kt[j][n][2 * r] * 0x1p-6f, kt[j][n][2 * r + 1] * 0x1p-6f, hi, lo);
+          const int at = ld_at<PIECES>(j * 16 + g + r * 8, warp * N + n) + cc * 2;
+          *(uint32_t*)(kt_hi + at) = hi, *(uint32_t*)(td + at) = lo;
+        }
+    __syncthreads();
+    for (int i = tid; i < (int)sizeof(out->kt_hi) / 16; i += LD_PREP_THREADS) {
+      ((uint4*)out->kt_hi)[i] = ((const uint4*)kt_hi)[i];
+      ((uint4*)out->kt_lo)[i] = ((const uint4*)td)[i];
+    }
+  } else {
+    // K~ = D K
+    for (int i = tid; i < LD_C * PIECES; i += LD_PREP_THREADS) {
+      const int j = i / PIECES;
+      const uint4 raw = *(const uint4*)(ks + i * 8);  // the piece's place in its row does not matter: row j's are together
+      float up, down;
+      ld_scale(fabsf(d_s[j]) <= LD_MAX ? fabsf(d_s[j]) : 1.0f, up, down);
+      const float f = fabsf(d_s[j]) <= LD_MAX ? d_s[j] * up * 0x1p-7f : 0.0f;
+      uint4 hi, lo;
+      ld_split(h_lo(raw.x) * f, h_hi(raw.x) * f, hi.x, lo.x), ld_split(h_lo(raw.y) * f, h_hi(raw.y) * f, hi.y, lo.y);
+      ld_split(h_lo(raw.z) * f, h_hi(raw.z) * f, hi.z, lo.z), ld_split(h_lo(raw.w) * f, h_hi(raw.w) * f, hi.w, lo.w);
+      ((uint4*)out->kt_hi)[i] = hi, ((uint4*)out->kt_lo)[i] = lo;
+    }
+    if (tid < LD_C) {
+      float up, down;
+      ld_scale(fabsf(d_s[tid]) <= LD_MAX ? fabsf(d_s[tid]) : 1.0f, up, down);
+      kt_scale[tid] = d_s[tid] != 0.0f ? down * 0x1p7f : 0.0f;
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tp[n][e] = p[n][e];
+  }
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (!(fabsf(tp[n][e]) <= LD_MAX)) good[e >> 1] = false, tp[n][e] = 0.0f;
+      most[e >> 1] = fmaxf(most[e >> 1], fabsf(tp[n][e]));
+    }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = warp * 16 + g + r * 8;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], o));
+    const uint32_t row = 0xfu << (lane & ~3);
+    const bool all_good = (__ballot_sync(0xffffffffu, good[r]) & row) == row;
+    float up, down;
+    ld_scale(most[r], up, down);
+    if (cc == 0) out->p_scale[i] = all_good ? down : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+      *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(tp[n][r * 2] * up, tp[n][r * 2 + 1] * up);
+  }
+  if (tid < LD_C) {
+    const float nan = __uint_as_float(0x7fc00000u), gamma = expf((float)G);
+    const bool bad = bad_s[first] != 0, live = my_line >= 0;
+    out->gamma[tid] = gamma;
+    out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
+    out->r_in[tid] = live && !bad ? gamma * k_factor[tid] : 0.0f;
+    out->q_in[tid] = !live ? 0.0f : bad ? nan : gamma * q_factor[tid];
   }
 }
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks; a warp has 16 rows
-// by itself, S in its registers as the accumulator of S^T-shaped products [rows of S, tokens or columns of K]. An accumulator of
-// mma.sync is laid out as the next product's A operand is, so S -> R -> U -> S needs no exchange between warps: K, Q, the
-// inverse and P, as B operands, come from shared memory, where a producer warp keeps LdScanShape::STAGES chunks coming (bulk
-// copies; the rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory and R and U brought
-// there and back between the products: with 16 rows a warp the chain is shorter in registers.)
-template <int DK, int WARPS, bool DELTA> struct LdScanShape {
-  static constexpr int V = WARPS * LD_C * 32, STAGE = (int)(sizeof(LdRows<DK>) + sizeof(LdHead)) + V;
-  static constexpr int STAGES = (227 * 1024 - 2048) / STAGE < 4 ? (227 * 1024 - 2048) / STAGE : 4;
+// by itself, S in its registers as the accumulator of products [rows of S, tokens or columns of K]. An accumulator of mma.sync
+// is laid out as the next product's A operand is, so S -> R -> S needs no exchange between warps: K, Q, K~ and P T, as B
+// operands, come from shared memory, where a producer warp keeps chunks coming (bulk copies; the rows of v by TMA). (tcgen05
+// would want S as a 16-bit operand in shared or tensor memory, and R brought there and back between the products: with 16 rows a
+// warp the chain is shorter in registers.)
+template <int DK, int WARPS> struct LdScanShape {
+  static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
+  static constexpr int ROOM = 227 * 1024 - 2048, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + 1024;
 };
+
+// 1 / x of a power of two.
+D3_DEV float ld_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 
 // Largest of the values of a row held by the four lanes of a group.
 D3_DEV float ld_row_most(float m) {
@@ -353,8 +542,8 @@ template <int TYPE, int DK, bool DELTA, int WARPS>
 __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
     lines_delta_scan_kernel(const __grid_constant__ CUtensorMap vmap, LdChunkArgs c) {
   using TT = QrType<TYPE>;
-  using S_ = LdScanShape<DK, WARPS, DELTA>;
-  constexpr int PIECES = DK / 8, NK = DK / 8, NT = LD_C / 8, STAGES = S_::STAGES;
+  using Shape = LdScanShape<DK, WARPS>;
+  constexpr int PIECES = DK / 8, NK = DK / 8, NT = LD_C / 8, STAGES = Shape::STAGES;
   extern __shared__ uint8_t ld_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
   const LdArgs& a = c.a;
@@ -384,22 +573,22 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
     if (lane == 0) {
       bool ok = true;
       int i = 0;
+      const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
+      constexpr uint32_t skip = DELTA ? 0 : sizeof(LdRows<DK>) / 2, row_bytes = sizeof(LdRows<DK>) - skip;  // k is for K S^T
+      const uint64_t keep = policy_evict_last();
       for (; i < chunks && ok; ++i) {
         const int st = i % STAGES;
         if (i >= STAGES) ok = mbar_wait(&empty[st], (i / STAGES - 1) & 1);
         if (!ok) break;
-        uint8_t* to = ring + st * S_::STAGE;
+        uint8_t* to = ring + st * Shape::STAGE;
         const size_t block = block_a + i;
-        const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
-        const uint32_t head_bytes = DELTA ? sizeof(LdHead) : sizeof(LdHead) - offsetof(LdHead, p);
-        mbar_arrive_expect_tx(&full[st], (uint32_t)sizeof(LdRows<DK>) + head_bytes + v_boxes * LD_C * 32);
-        const uint64_t keep = policy_evict_last();
-        bulk_g2s(to, (const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk), sizeof(LdRows<DK>), &full[st], keep);
-        const uint8_t* head = (const uint8_t*)(c.heads + block * a.Hv + h);
-        bulk_g2s(to + sizeof(LdRows<DK>) + sizeof(LdHead) - head_bytes, head + sizeof(LdHead) - head_bytes, head_bytes, &full[st], keep);
+        mbar_arrive_expect_tx(&full[st], row_bytes + (uint32_t)sizeof(LdHead<DK>) + v_boxes * LD_C * 32);
+        bulk_g2s(to + skip, (const uint8_t*)((const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk)) + skip, row_bytes,
+                 &full[st], keep);
+        bulk_g2s(to + Shape::HEAD, (const LdHead<DK>*)c.heads + block * a.Hv + h, sizeof(LdHead<DK>), &full[st], keep);
         for (int w = 0; w < v_boxes; ++w)
-          tma_load_3d(smem_u32(to + sizeof(LdRows<DK>) + sizeof(LdHead) + w * LD_C * 32), &vmap,
-                      (blockIdx.x * WARPS + w) * 16, h, (int)(first_token + (long long)block * LD_C), &full[st]);
+          tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h,
+                      (int)(first_token + (long long)block * LD_C), &full[st]);
       }
       if (!ok)  // the copies in flight land before the block ends
         for (int st = 0; st < STAGES && st < i; ++st) mbar_wait(&full[st], ((i - 1 - st) / STAGES) & 1);
@@ -408,7 +597,8 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
   }
   float* const state = a.state + (((size_t)b * a.Hv + h) * a.Dv + row0) * DK;
   const bool there = row0 < a.Dv;
-  float S[NK][4] = {};
+  float S[NK][4] = {};  // times down[] it is the state
+  float down[2] = {1.0f, 1.0f};
   if (there)
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
@@ -422,25 +612,37 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
     ok = mbar_wait(&full[st], (i / STAGES) & 1);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
-    const uint8_t* stage = ring + st * S_::STAGE;
+    uint8_t* const stage = ring + st * Shape::STAGE;
     const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
-    const LdHead& head = *(const LdHead*)(stage + sizeof(LdRows<DK>));
-    uint8_t* v_s = ring + st * S_::STAGE + sizeof(LdRows<DK>) + sizeof(LdHead) + warp * LD_C * 32;  // and, later, its outputs
+    const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
+    uint8_t* const v_s = stage + Shape::V + warp * LD_C * 32;  // and, later, its outputs
     const long long t0 = first_token + (long long)(block_a + i) * LD_C;
     const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
     const bool partial = lo > 0 || hi < LD_C;
-    float up[2], down[2], m_s[2] = {0.0f, 0.0f};
-    {
-      float (&m)[2] = m_s;
+    // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already
+    float m_s[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        m[0] = fmaxf(m[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
-      }
+    for (int n = 0; n < NK; ++n) {
+      m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
+      m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
+    }
+    {
+      bool off = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        m[r] = ld_row_most(m[r]);
-        ld_scale(m[r], up[r], down[r]);
+        m_s[r] = ld_row_most(m_s[r]);
+        off = off || (m_s[r] != 0.0f && !(m_s[r] >= 0x1p9f && m_s[r] < 0x1p15f));
+      }
+      if (__any_sync(0xffffffffu, off)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float up, dn;
+          ld_scale(m_s[r] * down[r], up, dn);
+          up *= down[r];
+          m_s[r] *= up, down[r] = dn;
+#pragma unroll
+          for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
+        }
       }
     }
     // S K^T and S Q^T
@@ -448,24 +650,31 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
 #pragma unroll
     for (int kt = 0; kt < DK / 16; ++kt) {
       uint32_t hi4[4], lo4[4];
-      ld_split(S[2 * kt][0] * up[0], S[2 * kt][1] * up[0], hi4[0], lo4[0]);
-      ld_split(S[2 * kt][2] * up[1], S[2 * kt][3] * up[1], hi4[1], lo4[1]);
-      ld_split(S[2 * kt + 1][0] * up[0], S[2 * kt + 1][1] * up[0], hi4[2], lo4[2]);
-      ld_split(S[2 * kt + 1][2] * up[1], S[2 * kt + 1][3] * up[1], hi4[3], lo4[3]);
+      ld_split(S[2 * kt][0], S[2 * kt][1], hi4[0], lo4[0]);
+      ld_split(S[2 * kt][2], S[2 * kt][3], hi4[1], lo4[1]);
+      ld_split(S[2 * kt + 1][0], S[2 * kt + 1][1], hi4[2], lo4[2]);
+      ld_split(S[2 * kt + 1][2], S[2 * kt + 1][3], hi4[3], lo4[3]);
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t bk[4];
-        const int at = ld_at<PIECES>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1));
-        if (DELTA) {
-          ld_matrix4(bk, rows.k + at);
-          ld_mma(R[n], lo4, bk[0], bk[1]), ld_mma(R[n + 1], lo4, bk[2], bk[3]);
-          ld_mma(R[n], hi4, bk[0], bk[1]), ld_mma(R[n + 1], hi4, bk[2], bk[3]);
+      for (int n = 0; n < NT; n += 4) {
+        uint32_t k4[2][4], q4[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = ld_at<PIECES>((n + 2 * x) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1));
+          if (DELTA) ld_matrix4(k4[x], rows.k + at);
+          ld_matrix4(q4[x], rows.q + at);
         }
-        ld_matrix4(bk, rows.q + at);
-        ld_mma(O[n], hi4, bk[0], bk[1]), ld_mma(O[n + 1], hi4, bk[2], bk[3]);
+        if (DELTA)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ld_mma(R[n + x], lo4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) ld_mma(O[n + x], hi4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
+        if (DELTA)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ld_mma(R[n + x], hi4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
       }
     }
-    // R = V - gamma K S^T (without the delta rule V is U), zeros for the tokens of other lines
+    // R = V - gamma K S^T, zeros for the tokens of other lines
+    float m_r[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
       uint32_t v4[4];
@@ -487,74 +696,24 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
           if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = 0.0f;
         }
 #pragma unroll
-        for (int y = 0; y < 4; ++y) R[n + x][y] = v[y];
-      }
-    }
-    float U[NT][4];
-    if (DELTA) {  // U = inverse R
-      float m[2] = {0.0f, 0.0f}, ru[2], rd[2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0]), fabsf(R[n][1])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2]), fabsf(R[n][3])));
-      }
-      ld_scale(ld_row_most(m[0]), ru[0], rd[0]);
-      ld_scale(ld_row_most(m[1]), ru[1], rd[1]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) U[n][y] = 0.0f;
-#pragma unroll
-      for (int kt = 0; kt < LD_C / 16; ++kt) {
-        uint32_t hi4[4], lo4[4];
-        ld_split(R[2 * kt][0] * ru[0], R[2 * kt][1] * ru[0], hi4[0], lo4[0]);
-        ld_split(R[2 * kt][2] * ru[1], R[2 * kt][3] * ru[1], hi4[1], lo4[1]);
-        ld_split(R[2 * kt + 1][0] * ru[0], R[2 * kt + 1][1] * ru[0], hi4[2], lo4[2]);
-        ld_split(R[2 * kt + 1][2] * ru[1], R[2 * kt + 1][3] * ru[1], hi4[3], lo4[3]);
-#pragma unroll
-        for (int n = 2 * kt; n < NT; n += 2) {
-          uint32_t t4[4];
-          const int at = ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1));
-          ld_matrix4(t4, head.t_lo + at);
-          ld_mma(U[n], hi4, t4[0], t4[1]), ld_mma(U[n + 1], hi4, t4[2], t4[3]);
-          ld_matrix4(t4, head.t_hi + at);
-          ld_mma(U[n], lo4, t4[0], t4[1]), ld_mma(U[n + 1], lo4, t4[2], t4[3]);
-          ld_mma(U[n], hi4, t4[0], t4[1]), ld_mma(U[n + 1], hi4, t4[2], t4[3]);
+        for (int y = 0; y < 4; ++y) {
+          R[n + x][y] = v[y];
+          m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int j = n * 8 + cc * 2;
-        const float2 f = *(const float2*)(head.t_scale + j);
-        U[n][0] *= f.x * rd[0], U[n][1] *= f.y * rd[0], U[n][2] *= f.x * rd[1], U[n][3] *= f.y * rd[1];
-        if (partial) {
-          if (j < lo || j >= hi) U[n][0] = U[n][2] = 0.0f;
-          if (j + 1 < lo || j + 1 >= hi) U[n][1] = U[n][3] = 0.0f;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) U[n][y] = R[n][y];
     }
-    // O = gamma Q S^T + P U
+    // O = gamma Q S^T + P T R
     {
-      float m[2] = {0.0f, 0.0f}, uu[2], ud[2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        m[0] = fmaxf(m[0], fmaxf(fabsf(U[n][0]), fabsf(U[n][1])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(U[n][2]), fabsf(U[n][3])));
-      }
-      ld_scale(ld_row_most(m[0]), uu[0], ud[0]);
-      ld_scale(ld_row_most(m[1]), uu[1], ud[1]);
+      float uu[2], ud[2];
+      ld_scale(ld_row_most(m_r[0]), uu[0], ud[0]);
+      ld_scale(ld_row_most(m_r[1]), uu[1], ud[1]);
       uint32_t u4[LD_C / 16][4];
 #pragma unroll
       for (int kt = 0; kt < LD_C / 16; ++kt) {
-        u4[kt][0] = ld_half2(U[2 * kt][0] * uu[0], U[2 * kt][1] * uu[0]);
-        u4[kt][1] = ld_half2(U[2 * kt][2] * uu[1], U[2 * kt][3] * uu[1]);
-        u4[kt][2] = ld_half2(U[2 * kt + 1][0] * uu[0], U[2 * kt + 1][1] * uu[0]);
-        u4[kt][3] = ld_half2(U[2 * kt + 1][2] * uu[1], U[2 * kt + 1][3] * uu[1]);
+        u4[kt][0] = ld_half2(R[2 * kt][0] * uu[0], R[2 * kt][1] * uu[0]);
+        u4[kt][1] = ld_half2(R[2 * kt][2] * uu[1], R[2 * kt][3] * uu[1]);
+        u4[kt][2] = ld_half2(R[2 * kt + 1][0] * uu[0], R[2 * kt + 1][1] * uu[0]);
+        u4[kt][3] = ld_half2(R[2 * kt + 1][2] * uu[1], R[2 * kt + 1][3] * uu[1]);
       }
       __syncwarp();  // v has been read by all lanes
 #pragma unroll
@@ -589,48 +748,63 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
                 *(const uint4*)(v_s + token * 32 + piece * 16);
         }
     }
-    // S = gamma_last S + (k_out U)^T K, the sum in the scale of U's row
+    // S = gamma_last S + R^T K~, in S's scale or, where the terms are larger (or S has shrunk away), one that suits them
     {
-      float m[2] = {0.0f, 0.0f}, wu[2], wd[2];
+      float m[2] = {0.0f, 0.0f}, up[2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int j = n * 8 + cc * 2;
-        float2 f = *(const float2*)(head.k_out + j);
+        float2 f = *(const float2*)(head.kt_scale + j);
         if (partial) {
           if (j < lo || j >= hi) f.x = 0.0f;
           if (j + 1 < lo || j + 1 >= hi) f.y = 0.0f;
         }
-        U[n][0] *= f.x, U[n][1] *= f.y, U[n][2] *= f.x, U[n][3] *= f.y;
-        m[0] = fmaxf(m[0], fmaxf(fabsf(U[n][0]), fabsf(U[n][1])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(U[n][2]), fabsf(U[n][3])));
+        R[n][0] *= f.x, R[n][1] *= f.y, R[n][2] *= f.x, R[n][3] *= f.y;
+        m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0]), fabsf(R[n][1])));
+        m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2]), fabsf(R[n][3])));
       }
       const float gamma = head.gamma[hi - 1];
+      float g2[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // no less than 2^-40 of the state's size: what is smaller does not change it, and the state stays within 32 bits
-        ld_scale(fmaxf(ld_row_most(m[r]), m_s[r] * 0x1p-40f), wu[r], wd[r]);
+        // of a size: gamma S, and R times K~'s rows, which are below 2^15 and mostly near 2^7
+        const float most = fmaxf(gamma * m_s[r] * down[r], ld_row_most(m[r]) * 0x1p7f);
+        const float at = most * ld_inverse(down[r]);
+        float dn = down[r];
+        if (!(at >= 0x1p9f && at < 0x1p15f)) {
+          float u;
+          ld_scale(most, u, dn);
+        }
+        up[r] = ld_inverse(dn);
+        g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
+        down[r] = dn;
       }
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        S[n][0] *= gamma * wu[0], S[n][1] *= gamma * wu[0], S[n][2] *= gamma * wu[1], S[n][3] *= gamma * wu[1];
-      }
+      for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
 #pragma unroll
       for (int kt = 0; kt < LD_C / 16; ++kt) {
         uint32_t hi4[4], lo4[4];
-        ld_split(U[2 * kt][0] * wu[0], U[2 * kt][1] * wu[0], hi4[0], lo4[0]);
-        ld_split(U[2 * kt][2] * wu[1], U[2 * kt][3] * wu[1], hi4[1], lo4[1]);
-        ld_split(U[2 * kt + 1][0] * wu[0], U[2 * kt + 1][1] * wu[0], hi4[2], lo4[2]);
-        ld_split(U[2 * kt + 1][2] * wu[1], U[2 * kt + 1][3] * wu[1], hi4[3], lo4[3]);
+        ld_split(R[2 * kt][0] * up[0], R[2 * kt][1] * up[0], hi4[0], lo4[0]);
+        ld_split(R[2 * kt][2] * up[1], R[2 * kt][3] * up[1], hi4[1], lo4[1]);
+        ld_split(R[2 * kt + 1][0] * up[0], R[2 * kt + 1][1] * up[0], hi4[2], lo4[2]);
+        ld_split(R[2 * kt + 1][2] * up[1], R[2 * kt + 1][3] * up[1], hi4[3], lo4[3]);
 #pragma unroll
-        for (int n = 0; n < NK; n += 2) {
-          uint32_t b4[4];
-          ld_matrix4_trans(b4, rows.k + ld_at<PIECES>(kt * 16 + (lane & 15), n + (lane >> 4)));
-          ld_mma(S[n], lo4, b4[0], b4[1]), ld_mma(S[n + 1], lo4, b4[2], b4[3]);
-          ld_mma(S[n], hi4, b4[0], b4[1]), ld_mma(S[n + 1], hi4, b4[2], b4[3]);
+        for (int n = 0; n < NK; n += 4) {
+          uint32_t b_hi[2][4], b_lo[2][4];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int at = ld_at<PIECES>(kt * 16 + (lane & 15), n + 2 * x + (lane >> 4));
+            ld_matrix4_trans(b_lo[x], head.kt_lo + at);
+            ld_matrix4_trans(b_hi[x], head.kt_hi + at);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], hi4, b_lo[x / 2][x % 2 * 2], b_lo[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], lo4, b_hi[x / 2][x % 2 * 2], b_hi[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], hi4, b_hi[x / 2][x % 2 * 2], b_hi[x / 2][x % 2 * 2 + 1]);
         }
       }
-#pragma unroll
-      for (int n = 0; n < NK; ++n) S[n][0] *= wd[0], S[n][1] *= wd[0], S[n][2] *= wd[1], S[n][3] *= wd[1];
     }
     fence_async_smem();  // the outputs' place is the next TMA load's
     __syncwarp();
@@ -639,8 +813,8 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
   if (there && ok)
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
-      *(float2*)(state + g * DK + n * 8 + cc * 2) = make_float2(S[n][0], S[n][1]);
-      *(float2*)(state + (g + 8) * DK + n * 8 + cc * 2) = make_float2(S[n][2], S[n][3]);
+      *(float2*)(state + g * DK + n * 8 + cc * 2) = make_float2(S[n][0] * down[0], S[n][1] * down[0]);
+      *(float2*)(state + (g + 8) * DK + n * 8 + cc * 2) = make_float2(S[n][2] * down[1], S[n][3] * down[1]);
     }
 }
 
