@@ -107,13 +107,14 @@ constexpr float LD_MAX = 3.4028234e38f;
 template <int DK> struct LdPrepShape {
   static constexpr int K = LD_C * DK * 2, T = 2 * LD_C * LD_C * 2;
   static constexpr int Q = K > T ? K : T;  // the rows of q, then T^T
-  static constexpr int A = LD_C * LD_PITCH * 4, Y = 32 * LD_PITCH_Y * 4;
-  static constexpr int SMEM = K + Q + T + A + Y;
+  static constexpr int A = LD_C * LD_PITCH * 4;
+  static constexpr int SMEM = K + Q + T + A;
   static_assert(A >= K && T >= K, "K~'s terms take the places of A and of T^T D");
+  static_assert(T >= 32 * LD_PITCH_Y * 4, "A21 T1 takes that of T^T D");
 };
 
 // X = -T2 (A21 T1) for the blocks of N x N at rows r0 + N.., columns r0..: `threads` threads, of which this is number t.
-template <int N, int THREADS> D3_DEV void ld_join(float* A, float* Y, const int* line_s, int r0, int t) {
+template <int N, int THREADS> D3_DEV void ld_join(float* A, float* Y, unsigned long long starts, int r0, int t) {
   constexpr int COLS = N * N / THREADS, PER = N / COLS;  // columns a thread, threads a row
   const int r = t / PER, c = t % PER * COLS;
 #pragma unroll
@@ -132,13 +133,30 @@ template <int N, int THREADS> D3_DEV void ld_join(float* A, float* Y, const int*
     }
 #pragma unroll
     for (int e = 0; e < COLS; ++e) {
-      if (pass)  // entries of two lines are zeros whatever the sums met
-        A[(r0 + N + r) * LD_PITCH + r0 + c + e] = line_s[r0 + N + r] == line_s[r0 + c + e] ? -acc[e] : 0.0f;
+      if (pass)  // entries of two lines (one starts in between) are zeros whatever the sums met
+        A[(r0 + N + r) * LD_PITCH + r0 + c + e] = (starts & (~0ull >> (63 - (r0 + N + r)))) >> (r0 + c + e + 1) ? 0.0f : -acc[e];
       else
         Y[r * LD_PITCH_Y + c + e] = acc[e];
     }
     __syncthreads();
   }
+}
+
+// A shared-memory area into global memory by the copy engine: `bytes` a multiple of 16, both 16-byte aligned. One thread issues
+// it after every writer's fence_async_smem and a barrier, and waits for it (ld_bulk_read) before the area is used again.
+D3_DEV void ld_bulk_out(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
+D3_DEV void ld_bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The areas have been read; with ld_bulk_done what was written is there too.
+D3_DEV void ld_bulk_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+D3_DEV void ld_bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// e^x for x <= 0, off by about (2 + |x|) 2^-22 of itself: an exponent of which the argument is rounded to 32 bits is no nearer.
+D3_DEV float ld_exp(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
 }
 
 template <int TYPE, int DK, bool DELTA>
@@ -153,12 +171,13 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
   uint16_t* const tt = qs;                                              // T^T, two terms, where q was
   uint16_t* const td = (uint16_t*)(ld_smem + Shape::K + Shape::Q);      // T^T D, two terms
   float* const A = (float*)(ld_smem + Shape::K + Shape::Q + Shape::T);  // A, then T
-  float* const Y = A + LD_C * LD_PITCH;
+  float* const Y = (float*)td;
   __shared__ int line_s[LD_C];
   __shared__ uint32_t starts_s[2];
   __shared__ float k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], d_s[LD_C], t_scale[LD_C], kt_scale[LD_C];
-  __shared__ double G_s[LD_C];
-  __shared__ int bad_s[LD_C];  // by a line's first token in the chunk: something of it is not finite
+  __shared__ double sum_s;
+  __shared__ float2 G_s[LD_C];  // as the sum of two
+  __shared__ int bad_s[LD_C];   // by a line's first token in the chunk: something of it is not finite
   const LdArgs& a = c.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
   const int block = blockIdx.x, h = blockIdx.y, many = a.Hv / a.Hk, hk = h / many;
@@ -173,153 +192,150 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
     my_line = l >= 0 && l < a.B ? l : -1;
     line_s[tid] = my_line;
     bad_s[tid] = 0;
-    if (my_line >= 0) {
-      decay = ld_log_decay<TYPE>(a, t0 + tid, h);
-      if (DELTA) beta = ld_beta<TYPE>(a, t0 + tid, h);
-    }
   }
   // rows to fp16, each by the power of two that brings its largest value into [1, 2)
-  const int l = lane % LANES;
-#pragma unroll 4
-  for (int i = 0; i < 2 * LD_C / 4; i += AT_ONCE) {  // a warp: 16 rows of k, then 16 of q
-    const int at = i + lane / LANES;
-    const bool is_q = at >= LD_C / 4;
-    const int row = warp * (LD_C / 4) + (is_q ? at - LD_C / 4 : at);
-    const QrTensor& x = is_q ? a.q : a.k;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (t0 + row < a.T) raw = *(const uint4*)((const E*)x.p + (t0 + row) * x.token + hk * x.head + l * 8);
-    float v[8];
-    qr_unpack<TYPE, 8>(&raw.x, v);
-    float most = 0.0f;
-    bool finite = true;
+  {
+    const int l = lane % LANES;
+    constexpr int ROUNDS = 2 * LD_C / 4 / AT_ONCE, AHEAD = 4;  // a warp: 16 rows of k, then 16 of q
+#pragma unroll 1
+    for (int i0 = 0; i0 < ROUNDS; i0 += AHEAD) {
+      const bool is_q = i0 >= ROUNDS / 2;
+      const QrTensor& x = is_q ? a.q : a.k;
+      const int row0 = warp * (LD_C / 4) + (is_q ? i0 - ROUNDS / 2 : i0) * AT_ONCE + lane / LANES;
+      uint4 raw[AHEAD];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      most = fmaxf(most, fabsf(v[e]));
-      finite = finite && fabsf(v[e]) <= LD_MAX;
+      for (int i = 0; i < AHEAD; ++i) {
+        const int row = row0 + i * AT_ONCE;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (t0 + row < a.T) raw[i] = *(const uint4*)((const E*)x.p + (t0 + row) * x.token + hk * x.head + l * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int row = row0 + i * AT_ONCE;
+        float v[8], most = 0.0f, sum = 0.0f, up, down;
+        qr_unpack<TYPE, 8>(&raw[i].x, v);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) most = fmaxf(most, fmaxf(fabsf(v[e]), fabsf(v[e + 1])));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        ld_scale(most, up, down);
+        up *= 0x1p-13f, down *= 0x1p13f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] *= up;
+          sum = fmaf(v[e], v[e], sum);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        // x / sqrt(|x|^2 + eps) = (up x) / sqrt(|up x|^2 + up^2 eps)
+        float f = a.eps >= 0.0f ? rsqrtf(sum + a.eps * up * up) : down;
+        if (most == 0.0f) f = 0.0f;  // a row of zeros: its factor must not set the scale of what it is summed with
+        uint4 w = make_uint4(ld_half2(v[0], v[1]), ld_half2(v[2], v[3]), ld_half2(v[4], v[5]), ld_half2(v[6], v[7]));
+        if (!(sum <= LD_MAX)) f = __uint_as_float(0x7fc00000u), w = make_uint4(0, 0, 0, 0);
+        *(uint4*)((is_q ? qs : ks) + ld_at<PIECES>(row, l)) = w;
+        if (l == 0) (is_q ? q_factor : k_factor)[row] = is_q ? f * a.scale : f;
+      }
     }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const uint32_t group = ((1u << LANES) - 1u) << (lane / LANES * LANES);
-    finite = (__ballot_sync(0xffffffffu, finite) & group) == group;
-    float up, down;
-    ld_scale(most, up, down);
-    up *= 0x1p-13f, down *= 0x1p13f;
-    float sum = 0.0f;
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      w[e / 2] = finite ? ld_half2(v[e] * up, v[e + 1] * up) : 0u;
-      sum = fmaf(v[e] * up, v[e] * up, fmaf(v[e + 1] * up, v[e + 1] * up, sum));
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    *(uint4*)((is_q ? qs : ks) + ld_at<PIECES>(row, l)) = make_uint4(w[0], w[1], w[2], w[3]);
-    // x / sqrt(|x|^2 + eps) = (up x) / sqrt(|up x|^2 + up^2 eps)
-    float f = a.eps >= 0.0f ? rsqrtf(sum + a.eps * up * up) : down;
-    if (most == 0.0f) f = 0.0f;  // a row of zeros: its factor must not set the scale of what it is summed with
-    if (!finite) f = __uint_as_float(0x7fc00000u);
-    if (l == 0) (is_q ? q_factor : k_factor)[row] = is_q ? f * a.scale : f;
   }
+  if (my_line >= 0) {
+    decay = ld_log_decay<TYPE>(a, t0 + tid, h);
+    if (DELTA) beta = ld_beta<TYPE>(a, t0 + tid, h);
+  }
+  fence_async_smem();
   __syncthreads();
+  if (h == hk * many && tid == 0) {  // the rows, as every value head's scan reads them
+    LdRows<DK>* rows = (LdRows<DK>*)c.rows + (size_t)block * a.Hk + hk;
+    ld_bulk_out(rows->k, ks, sizeof(rows->k));
+    ld_bulk_out(rows->q, qs, sizeof(rows->q));
+    ld_bulk_commit();
+  }
   // sums of the log decays that start again with each line
   double G = decay < -104.0f ? -104.0f : decay;  // exp of it is 0 already; keeps infinities out of the sums
-  int first = 0, last = 0;
   if (warp < 2) {
     const uint32_t starts = __ballot_sync(0xffffffffu, tid == 0 || line_s[tid - 1] != my_line);
     if (lane == 0) starts_s[warp] = starts;
-    const int from = 31 - __clz(starts & (0xffffffffu >> (31 - lane)));  // in this warp; -1: before it
+    const int from = max(31 - __clz(starts & (0xffffffffu >> (31 - lane))), 0);  // in this warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double before = __shfl_up_sync(0xffffffffu, G, o);
-      if (lane - o >= max(from, 0)) G += before;
+      if (lane - o >= from) G += before;
     }
-    G_s[tid] = G;
+    if (tid == 31) sum_s = G;
   }
   __syncthreads();
   const unsigned long long starts = starts_s[0] | (unsigned long long)starts_s[1] << 32;
   auto first_of = [&](int i) { return 63 - __clzll(starts & (~0ull >> (63 - i))); };
-  if (tid >= 32 && tid < LD_C && first_of(tid) < 32) G_s[tid] = G + G_s[31];
+  int first = 0, last = 0;
   if (tid < LD_C) {
     first = first_of(tid);
     const unsigned long long later = tid == 63 ? 0 : starts >> (tid + 1);
     last = later ? tid + __ffsll((long long)later) - 1 : 63;
+    if (tid >= 32 && first < 32) G += sum_s;
+    const float G_hi = (float)G;
+    G_s[tid] = make_float2(G_hi, (float)(G - G_hi));
+    beta_s[tid] = beta;
+  }
+  // K K^T and Q K^T: rows 16 warp + g, + 8, columns 8 n + 2 cc, + 1 up to the diagonal
+  float p[8][4] = {}, kk[8][4] = {};
+#pragma unroll
+  for (int kt = 0; kt < DK / 16; ++kt) {
+    uint32_t ak[4], aq[4];
+    const int ar = warp * 16 + (lane & 15), ap = kt * 2 + (lane >> 4);
+    if (DELTA) ld_matrix4(ak, ks + ld_at<PIECES>(ar, ap));
+    ld_matrix4(aq, qs + ld_at<PIECES>(ar, ap));
+#pragma unroll
+    for (int n = 0; n < 8; n += 2)
+      if (n <= 2 * warp) {
+        uint32_t b[4];
+        ld_matrix4(b, ks + ld_at<PIECES>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+        if (DELTA) ld_mma(kk[n], ak, b[0], b[1]), ld_mma(kk[n + 1], ak, b[2], b[3]);
+        ld_mma(p[n], aq, b[0], b[1]), ld_mma(p[n + 1], aq, b[2], b[3]);
+      }
   }
   __syncthreads();
   if (tid < LD_C) {
-    G = G_s[tid];
-    float kf = k_factor[tid];
-    if (my_line >= 0 && !(fabsf(kf) <= LD_MAX && fabsf((float)G) <= LD_MAX && fabsf(beta) <= LD_MAX)) {
-      bad_s[first] = 1;
-      beta = 0.0f;
-    }
-    beta_s[tid] = beta;
-    d_s[tid] = my_line >= 0 ? expf((float)(G_s[last] - G)) * kf : 0.0f;
+    const float2 Gl = G_s[last], Gi = G_s[tid];
+    d_s[tid] = my_line >= 0 ? ld_exp((Gl.x - Gi.x) + (Gl.y - Gi.y)) * k_factor[tid] : 0.0f;
   }
-  __syncthreads();
-  // K K^T and Q K^T: rows 16 warp + g, + 8, columns 8 n + 2 cc, + 1 up to the diagonal
-  float p[8][4] = {};
   {
-    float kk[8][4] = {};
-#pragma unroll
-    for (int kt = 0; kt < DK / 16; ++kt) {
-      uint32_t ak[4], aq[4];
-      const int ar = warp * 16 + (lane & 15), ap = kt * 2 + (lane >> 4);
-      if (DELTA) ld_matrix4(ak, ks + ld_at<PIECES>(ar, ap));
-      ld_matrix4(aq, qs + ld_at<PIECES>(ar, ap));
-#pragma unroll
-      for (int n = 0; n < 8; n += 2)
-        if (n <= 2 * warp) {
-          uint32_t b[4];
-          ld_matrix4(b, ks + ld_at<PIECES>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-          if (DELTA) ld_mma(kk[n], ak, b[0], b[1]), ld_mma(kk[n + 1], ak, b[2], b[3]);
-          ld_mma(p[n], aq, b[0], b[1]), ld_mma(p[n + 1], aq, b[2], b[3]);
-        }
-    }
-    float qf[2], kf[2], bt[2];
-    double Gi[2];
-    int li[2];
+    float qf[2], kf[2];
+    float2 Gi[2];
+    int from[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int i = warp * 16 + g + r * 8;
-      qf[r] = q_factor[i], kf[r] = k_factor[i] * beta_s[i], Gi[r] = G_s[i], li[r] = line_s[i];
+      qf[r] = q_factor[i], kf[r] = k_factor[i] * beta_s[i], Gi[r] = G_s[i];
+      from[r] = line_s[i] >= 0 ? first_of(i) : LD_C;  // the row's first entry
     }
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int j = n * 8 + cc * 2 + x;
-        float kfj = 0.0f;
-        double Gj = 0.0;
-        int lj = -1;
-        if (n <= 2 * warp + 1) kfj = k_factor[j], Gj = G_s[j], lj = line_s[j];
+        float av[2] = {0.0f, 0.0f}, pv[2] = {0.0f, 0.0f};
+        if (n <= 2 * warp + 1) {
+          const float kfj = k_factor[j];
+          const float2 Gj = G_s[j];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int i = warp * 16 + g + r * 8, e = r * 2 + x;
+            const float ratio = ld_exp((Gi[r].x - Gj.x) + (Gi[r].y - Gj.y)) * kfj;
+            const bool in = j >= from[r] && j <= i;
+            pv[r] = in ? ratio * qf[r] * p[n][e] : 0.0f;
+            if (DELTA) av[r] = in && j < i ? ratio * kf[r] * kk[n][e] : 0.0f;
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int i = warp * 16 + g + r * 8, e = r * 2 + x;
-          float pv = 0.0f, av = 0.0f;
-          if (n <= 2 * warp + 1 && j <= i && li[r] == lj && lj >= 0) {
-            const float ratio = expf((float)(Gi[r] - Gj)) * kfj;
-            pv = ratio * qf[r] * p[n][e];
-            if (DELTA && j < i) av = ratio * kf[r] * kk[n][e];
-          }
-          if (DELTA) {
-            if (!(fabsf(av) <= LD_MAX)) bad_s[first_of(i)] = 1, av = 0.0f;
-            A[i * LD_PITCH + j] = av;
-          }
-          p[n][e] = pv;
+          p[n][r * 2 + x] = pv[r];
+          if (DELTA) A[(warp * 16 + g + r * 8) * LD_PITCH + j] = av[r];
         }
       }
   }
-  __syncthreads();  // also: q has been read
-  if (h == hk * many) {  // the rows, as every value head's scan reads them
-    LdRows<DK>* rows = (LdRows<DK>*)c.rows + (size_t)block * a.Hk + hk;
-    for (int i = tid; i < (int)sizeof(rows->k) / 16; i += LD_PREP_THREADS) {
-      ((uint4*)rows->k)[i] = ((const uint4*)ks)[i];
-      ((uint4*)rows->q)[i] = ((const uint4*)qs)[i];
-    }
-  }
+  if (tid == 0) ld_bulk_read();  // the rows of q are on their way
+  __syncthreads();
   float most[2] = {0.0f, 0.0f};
   bool good[2] = {true, true};
-  float tp[8][4];  // P T
   if constexpr (DELTA) {
     if (tid < LD_C) {  // the blocks on the diagonal
       const int d = tid & ~15, j = tid & 15;
@@ -336,29 +352,33 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
             if (m + 2 < i) x[i] = fmaf(-v.z, x[m + 2], x[i]);
             if (m + 3 < i) x[i] = fmaf(-v.w, x[m + 3], x[i]);
           }
+        if (i < j) x[i] = 0.0f;  // whatever stands in the rows of an earlier line
       }
       __syncwarp();
+      const int from = first_of(d + j);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) A[(d + i) * LD_PITCH + d + j] = line_s[d + i] == line_s[d + j] ? x[i] : 0.0f;
+      for (int i = 0; i < 16; ++i) A[(d + i) * LD_PITCH + d + j] = first_of(d + i) == from ? x[i] : 0.0f;
     }
     __syncthreads();
-    ld_join<16, 64>(A, Y + (tid >> 6) * 16 * LD_PITCH_Y, line_s, (tid >> 6) * 32, tid & 63);
-    ld_join<32, 128>(A, Y, line_s, 0, tid);
+    ld_join<16, 64>(A, Y + (tid >> 6) * 16 * LD_PITCH_Y, starts, (tid >> 6) * 32, tid & 63);
+    ld_join<32, 128>(A, Y, starts, 0, tid);
     {  // columns of T become rows of T^T and T^T D: two threads each, four rows by turns
       const int j = tid >> 1, half = tid & 1;
       const float b = beta_s[j];
-      float v[32], d[32], m_t = 0.0f, m_d = 0.0f;
+      float v[32], m_t = 0.0f, m_d = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
         const int i = (e >> 2) * 8 + half * 4 + (e & 3);
-        v[e] = i >= j ? A[i * LD_PITCH + j] * b : 0.0f;
-        if (!(fabsf(v[e]) <= LD_MAX)) bad_s[first_of(j)] = 1, v[e] = 0.0f;
-        d[e] = v[e] != 0.0f ? v[e] * d_s[i] : 0.0f;  // nothing of another line, where that is not finite
-        if (!(fabsf(d[e]) <= LD_MAX)) bad_s[first_of(j)] = 1, d[e] = 0.0f;
-        m_t = fmaxf(m_t, fabsf(v[e])), m_d = fmaxf(m_d, fabsf(d[e]));
+        v[e] = A[i * LD_PITCH + j] * b;
+        sum += fabsf(v[e]);  // finite where all are
+        m_t = fmaxf(m_t, fabsf(v[e]));
+      }
+      if (!(sum <= LD_MAX)) {
+        bad_s[first_of(j)] = 1;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
       }
       m_t = fmaxf(m_t, __shfl_xor_sync(0xffffffffu, m_t, 1));
-      m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
       float up, down;
       ld_scale(m_t, up, down);
       if (half == 0) t_scale[j] = down;
@@ -369,51 +389,40 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
         const int at = ld_at<8>(j, e >> 2) + half * 4;
         *(uint2*)(tt + at) = hi, *(uint2*)(tt + LD_C * LD_C + at) = lo;
       }
+      sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const int i = (e >> 2) * 8 + half * 4 + (e & 3);
+        v[e] = v[e] != 0.0f ? v[e] * d_s[i] : 0.0f;  // nothing of another line, where that is not finite
+        sum += fabsf(v[e]);
+        m_d = fmaxf(m_d, fabsf(v[e]));
+      }
+      if (!(sum <= LD_MAX)) {
+        bad_s[first_of(j)] = 1;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+      }
+      m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
       ld_scale(m_d, up, down);
       if (half == 0) kt_scale[j] = m_d > 0.0f ? down * 0x1p6f : 0.0f;  // a row of zeros must not set a scale
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         uint2 hi, lo;
-        ld_split(d[e] * up, d[e + 1] * up, hi.x, lo.x), ld_split(d[e + 2] * up, d[e + 3] * up, hi.y, lo.y);
+        ld_split(v[e] * up, v[e + 1] * up, hi.x, lo.x), ld_split(v[e + 2] * up, v[e + 3] * up, hi.y, lo.y);
         const int at = ld_at<8>(j, e >> 2) + half * 4;
         *(uint2*)(td + at) = hi, *(uint2*)(td + LD_C * LD_C + at) = lo;
       }
     }
     __syncthreads();
-    // K~ = T^T D K: a warp has Dk / 4 columns
-    constexpr int N = DK / 32;
-    float kt[4][N][4] = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // 16 tokens i of the sum
-      uint32_t b[N][2];
-#pragma unroll
-      for (int n = 0; n < N; n += 2) {
-        uint32_t b4[4];
-        ld_matrix4_trans(b4, ks + ld_at<PIECES>(i * 16 + (lane & 15), warp * N + n + (lane >> 4)));
-        b[n][0] = b4[0], b[n][1] = b4[1], b[n + 1][0] = b4[2], b[n + 1][1] = b4[3];
-      }
-#pragma unroll
-      for (int j = 0; j <= i; ++j) {
-        uint32_t hi[4], lo[4];
-        const int at = ld_at<8>(j * 16 + (lane & 15), i * 2 + (lane >> 4));
-        ld_matrix4(lo, td + LD_C * LD_C + at);
-        ld_matrix4(hi, td + at);
-#pragma unroll
-        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], lo, b[n][0], b[n][1]);
-#pragma unroll
-        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], hi, b[n][0], b[n][1]);
-      }
-    }
     // P T: a warp has 16 rows
+    float tp[8][4] = {}, up[2], down[2];
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (!(fabsf(p[n][e]) <= LD_MAX)) good[e >> 1] = false, p[n][e] = 0.0f;
         most[e >> 1] = fmaxf(most[e >> 1], fabsf(p[n][e]));
-        tp[n][e] = 0.0f;
       }
-    float up[2], down[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -443,55 +452,17 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const float2 f = *(const float2*)(t_scale + n * 8 + cc * 2);
-      tp[n][0] *= f.x * down[0], tp[n][1] *= f.y * down[0], tp[n][2] *= f.x * down[1], tp[n][3] *= f.y * down[1];
+      p[n][0] = tp[n][0] * (f.x * down[0]), p[n][1] = tp[n][1] * (f.y * down[0]);
+      p[n][2] = tp[n][2] * (f.x * down[1]), p[n][3] = tp[n][3] * (f.y * down[1]);
     }
-    __syncthreads();  // T^T D has been read
-    uint16_t* const kt_hi = (uint16_t*)A;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {  // at most 64 x 2^14 x 2: 2^-6 of it is an fp16 number
-          uint32_t hi, lo;
-          ld_split(kt[j][n][2 * r] * 0x1p-6f, kt[j][n][2 * r + 1] * 0x1p-6f, hi, lo);
-          const int at = ld_at<PIECES>(j * 16 + g + r * 8, warp * N + n) + cc * 2;
-          *(uint32_t*)(kt_hi + at) = hi, *(uint32_t*)(td + at) = lo;
-        }
-    __syncthreads();
-    for (int i = tid; i < (int)sizeof(out->kt_hi) / 16; i += LD_PREP_THREADS) {
-      ((uint4*)out->kt_hi)[i] = ((const uint4*)kt_hi)[i];
-      ((uint4*)out->kt_lo)[i] = ((const uint4*)td)[i];
-    }
-  } else {
-    // K~ = D K
-    for (int i = tid; i < LD_C * PIECES; i += LD_PREP_THREADS) {
-      const int j = i / PIECES;
-      const uint4 raw = *(const uint4*)(ks + i * 8);  // the piece's place in its row does not matter: row j's are together
-      float up, down;
-      ld_scale(fabsf(d_s[j]) <= LD_MAX ? fabsf(d_s[j]) : 1.0f, up, down);
-      const float f = fabsf(d_s[j]) <= LD_MAX ? d_s[j] * up * 0x1p-7f : 0.0f;
-      uint4 hi, lo;
-      ld_split(h_lo(raw.x) * f, h_hi(raw.x) * f, hi.x, lo.x), ld_split(h_lo(raw.y) * f, h_hi(raw.y) * f, hi.y, lo.y);
-      ld_split(h_lo(raw.z) * f, h_hi(raw.z) * f, hi.z, lo.z), ld_split(h_lo(raw.w) * f, h_hi(raw.w) * f, hi.w, lo.w);
-      ((uint4*)out->kt_hi)[i] = hi, ((uint4*)out->kt_lo)[i] = lo;
-    }
-    if (tid < LD_C) {
-      float up, down;
-      ld_scale(fabsf(d_s[tid]) <= LD_MAX ? fabsf(d_s[tid]) : 1.0f, up, down);
-      kt_scale[tid] = d_s[tid] != 0.0f ? down * 0x1p7f : 0.0f;
-    }
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) tp[n][e] = p[n][e];
   }
+  // the rows of P T (of P) out, one term
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (!(fabsf(tp[n][e]) <= LD_MAX)) good[e >> 1] = false, tp[n][e] = 0.0f;
-      most[e >> 1] = fmaxf(most[e >> 1], fabsf(tp[n][e]));
+      if (!(fabsf(p[n][e]) <= LD_MAX)) good[e >> 1] = false, p[n][e] = 0.0f;
+      most[e >> 1] = fmaxf(most[e >> 1], fabsf(p[n][e]));
     }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -505,16 +476,85 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
     if (cc == 0) out->p_scale[i] = all_good ? down : __uint_as_float(0x7fc00000u);
 #pragma unroll
     for (int n = 0; n < 8; ++n)
-      *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(tp[n][r * 2] * up, tp[n][r * 2 + 1] * up);
+      *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(p[n][r * 2] * up, p[n][r * 2 + 1] * up);
+  }
+  uint16_t* const kt_hi = (uint16_t*)A;
+  uint16_t* const kt_lo = td;
+  if constexpr (DELTA) {
+    // K~ = T^T D K: a warp has Dk / 4 columns
+    constexpr int N = DK / 32;
+    float kt[4][N][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // 16 tokens i of the sum
+      uint32_t b[N][2];
+#pragma unroll
+      for (int n = 0; n < N; n += 2) {
+        uint32_t b4[4];
+        ld_matrix4_trans(b4, ks + ld_at<PIECES>(i * 16 + (lane & 15), warp * N + n + (lane >> 4)));
+        b[n][0] = b4[0], b[n][1] = b4[1], b[n + 1][0] = b4[2], b[n + 1][1] = b4[3];
+      }
+#pragma unroll
+      for (int j = 0; j <= i; ++j) {
+        uint32_t hi[4], lo[4];
+        const int at = ld_at<8>(j * 16 + (lane & 15), i * 2 + (lane >> 4));
+        ld_matrix4(lo, td + LD_C * LD_C + at);
+        ld_matrix4(hi, td + at);
+#pragma unroll
+        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], lo, b[n][0], b[n][1]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) ld_mma(kt[j][n], hi, b[n][0], b[n][1]);
+      }
+    }
+    __syncthreads();  // T^T D has been read
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {  // at most 64 x 2^14 x 2: 2^-6 of it is an fp16 number
+          uint32_t hi, lo;
+          ld_split(kt[j][n][2 * r] * 0x1p-6f, kt[j][n][2 * r + 1] * 0x1p-6f, hi, lo);
+          const int at = ld_at<PIECES>(j * 16 + g + r * 8, warp * N + n) + cc * 2;
+          *(uint32_t*)(kt_hi + at) = hi, *(uint32_t*)(kt_lo + at) = lo;
+        }
+  } else {
+    // K~ = D K
+    for (int i = tid; i < LD_C * PIECES; i += LD_PREP_THREADS) {
+      const int j = i / PIECES;
+      const uint4 raw = *(const uint4*)(ks + i * 8);  // the piece's place in its row does not matter: row j's are together
+      const bool finite = fabsf(d_s[j]) <= LD_MAX;
+      float up, down;
+      ld_scale(finite ? fabsf(d_s[j]) : 1.0f, up, down);
+      const float f = finite ? d_s[j] * up * 0x1p-7f : 0.0f;
+      uint4 hi, lo;
+      ld_split(h_lo(raw.x) * f, h_hi(raw.x) * f, hi.x, lo.x), ld_split(h_lo(raw.y) * f, h_hi(raw.y) * f, hi.y, lo.y);
+      ld_split(h_lo(raw.z) * f, h_hi(raw.z) * f, hi.z, lo.z), ld_split(h_lo(raw.w) * f, h_hi(raw.w) * f, hi.w, lo.w);
+      ((uint4*)kt_hi)[i] = hi, ((uint4*)kt_lo)[i] = lo;
+    }
+    if (tid < LD_C) {
+      const bool finite = fabsf(d_s[tid]) <= LD_MAX;
+      float up, down;
+      ld_scale(finite ? fabsf(d_s[tid]) : 1.0f, up, down);
+      kt_scale[tid] = d_s[tid] != 0.0f ? down * 0x1p7f : 0.0f;
+      if (!finite) bad_s[first] = 1;
+    }
+  }
+  fence_async_smem();
+  __syncthreads();
+  if (tid == 0) {
+    ld_bulk_out(out->kt_hi, kt_hi, sizeof(out->kt_hi));
+    ld_bulk_out(out->kt_lo, kt_lo, sizeof(out->kt_lo));
+    ld_bulk_commit();
   }
   if (tid < LD_C) {
-    const float nan = __uint_as_float(0x7fc00000u), gamma = expf((float)G);
+    const float nan = __uint_as_float(0x7fc00000u), gamma = ld_exp(G_s[tid].x + G_s[tid].y);
     const bool bad = bad_s[first] != 0, live = my_line >= 0;
     out->gamma[tid] = gamma;
     out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
     out->r_in[tid] = live && !bad ? gamma * k_factor[tid] : 0.0f;
     out->q_in[tid] = !live ? 0.0f : bad ? nan : gamma * q_factor[tid];
   }
+  if (tid == 0) ld_bulk_done();
 }
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks; a warp has 16 rows
