@@ -90,13 +90,13 @@ int delta_blocks(int T, int Hk, int Hv, int Dk) {
   return (int)(all < fit ? all : fit < 8 ? 8 : fit);
 }
 
-template <int TYPE, int DK, bool DELTA, int WARPS>
+template <int TYPE, int DK, bool DELTA, int WARPS, int PARTS>
 int scan_launch(const CUtensorMap& vmap, const d3::LdChunkArgs& c, cudaStream_t s) {
-  constexpr int smem = d3::LdScanShape<DK, WARPS>::SMEM;
+  constexpr int smem = d3::LdScanShape<DK, WARPS, PARTS>::SMEM;
   static std::atomic<uint64_t> done{0};
-  if (int st = allow_smem_once(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS>, smem, done)) return st;
+  if (int st = allow_smem_once(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS, PARTS>, smem, done)) return st;
   const dim3 blocks((c.a.Dv / 16 + WARPS - 1) / WARPS, c.a.Hv, c.a.B + 1);
-  return launch(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS>, blocks, dim3((WARPS + 1) * 32), smem, s, true, vmap, c);
+  return launch(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS, PARTS>, blocks, dim3(d3::LdScanShape<DK, WARPS, PARTS>::THREADS), smem, s, true, vmap, c);
 }
 
 template <int TYPE, int DK, bool DELTA>
@@ -119,10 +119,8 @@ int chunk_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cuda
     if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hv), dim3(d3::LD_PREP_THREADS), prep_smem, s,
                         true, c))
       return st;
-    // a whole head of 128 a CTA shares its operands; fewer rows a CTA where that leaves SMs idle
-    const long long wide = (long long)a.B * a.Hv * ((a.Dv + 127) / 128);
-    if (int st = wide >= d.sms && a.Dv > 64 ? scan_launch<TYPE, DK, DELTA, 8>(vmap, c, s)
-                                            : scan_launch<TYPE, DK, DELTA, 4>(vmap, c, s))
+    const long long wide = (long long)a.B * a.Hv * ((a.Dv + 63) / 64);
+    if (int st = wide >= d.sms ? scan_launch<TYPE, DK, DELTA, 4, 1>(vmap, c, s) : scan_launch<TYPE, DK, DELTA, 2, 2>(vmap, c, s))
       return st;
   }
   return D3_OK;

@@ -557,16 +557,22 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
   if (tid == 0) ld_bulk_done();
 }
 
-// ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks; a warp has 16 rows
-// by itself, S in its registers as the accumulator of products [rows of S, tokens or columns of K]. An accumulator of mma.sync
-// is laid out as the next product's A operand is, so S -> R -> S needs no exchange between warps: K, Q, K~ and P T, as B
-// operands, come from shared memory, where a producer warp keeps chunks coming (bulk copies; the rows of v by TMA). (tcgen05
-// would want S as a 16-bit operand in shared or tensor memory, and R brought there and back between the products: with 16 rows a
-// warp the chain is shorter in registers.)
-template <int DK, int WARPS> struct LdScanShape {
+// ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks. 16 rows are a team of
+// warps: one, or PARTS = 2 that have half of the columns each and add up their shares of K S^T, carry the state, S -> R -> S; the
+// last makes the outputs from what they leave in shared memory (S's high terms, R), one step behind, so that its products fill
+// the tensor core while the others' values are being converted. S stays in registers, as the
+// accumulator of products [rows of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand
+// is, so the chain has no exchange in it: K, Q, K~ and P T, as B operands, come from shared memory, where the first output warp keeps
+// chunks coming (bulk copies; the rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought
+// there and back between the products: with 16 rows a warp the chain is shorter in registers.)
+template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
-  static constexpr int ROOM = 227 * 1024 - 2048, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
-  static constexpr int SMEM = STAGES * STAGE + 1024;
+  // a team's place: S's high terms as A fragments, R's likewise, the rows' scales (of S's parts, of R), the outputs, shares of K S^T
+  static constexpr int R = DK * 32, SCALES = R + LD_C * 32, OUT = SCALES + 256, SHARES = OUT + LD_C * 32;
+  static constexpr int TEAM = SHARES + (PARTS > 1 ? 2 * PARTS * LD_C * 64 : 0);
+  static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
+  static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024, THREADS = WARPS * (PARTS + 1) * 32;
+  static_assert(STAGES >= 2, "a chunk is loaded while the one before it is worked on");
 };
 
 // 1 / x of a power of two.
@@ -578,30 +584,47 @@ D3_DEV float ld_row_most(float m) {
   return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 
-template <int TYPE, int DK, bool DELTA, int WARPS>
-__global__ void __launch_bounds__((WARPS + 1) * 32, 1)
+// mbar_wait by a whole warp, the same answer in all lanes.
+D3_DEV bool ld_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+// What this warp has written or read is done with: one arrival.
+D3_DEV void ld_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+template <int TYPE, int DK, bool DELTA, int WARPS, int PARTS>
+__global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     lines_delta_scan_kernel(const __grid_constant__ CUtensorMap vmap, LdChunkArgs c) {
   using TT = QrType<TYPE>;
-  using Shape = LdScanShape<DK, WARPS>;
-  constexpr int PIECES = DK / 8, NK = DK / 8, NT = LD_C / 8, STAGES = Shape::STAGES;
+  using Shape = LdScanShape<DK, WARPS, PARTS>;
+  constexpr int PIECES = DK / 8, NK = DK / 8 / PARTS, KT = DK / 16 / PARTS, NT = LD_C / 8, STAGES = Shape::STAGES;
+  constexpr int G = NK < 8 ? NK : 8;  // sums of S that take turns
   extern __shared__ uint8_t ld_raw[];
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS], s_empty[WARPS], r_full[WARPS], r_empty[WARPS], shares[WARPS][PARTS];
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
+  const bool outputs = warp >= WARPS * PARTS;
+  const int team = outputs ? warp - WARPS * PARTS : warp / PARTS, part = outputs ? 0 : warp % PARTS;
   uint8_t* const ring = (uint8_t*)(((uintptr_t)ld_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* const place = ring + STAGES * Shape::STAGE + team * Shape::TEAM;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], WARPS);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + 1) * WARPS);
+    for (int i = 0; i < WARPS; ++i) {
+      mbar_init(&s_full[i], PARTS), mbar_init(&s_empty[i], 1), mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], 1);
+      for (int j = 0; j < PARTS; ++j) mbar_init(&shares[i][j], 1);
+    }
     fence_mbar_init();
   }
   __syncthreads();
   grid_dependency_wait();
   allow_dependents();
   const long long first_token = (long long)c.block0 * LD_C, end_token = min((long long)a.T, first_token + (long long)c.blocks * LD_C);
-  const int row0 = (blockIdx.x * WARPS + warp) * 16;  // this warp's rows of the state
+  const int row0 = (blockIdx.x * WARPS + team) * 16;  // this team's rows of the state
+  const bool there = row0 < a.Dv;
   if (b == a.B) {  // the places past the lines' last token
     const long long from = max((long long)min(max(a.cu[b], 0), a.T), first_token);
-    if (warp < WARPS && row0 < a.Dv)
+    if (outputs && there)
       for (long long t = from + (lane >> 1); t < end_token; t += 16)
         *(uint4*)((uint16_t*)a.out + (t * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8) = make_uint4(0, 0, 0, 0);
     return;
@@ -609,153 +632,76 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
   const long long s = max((long long)min(max(a.cu[b], 0), a.T), first_token), e = min((long long)a.cu[b + 1], end_token);
   if (e <= s) return;
   const int block_a = (int)((s - first_token) / LD_C), chunks = (int)((e - 1 - first_token) / LD_C) - block_a + 1;
-  if (warp == WARPS) {  // the producer
-    if (lane == 0) {
-      bool ok = true;
-      int i = 0;
-      const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
-      constexpr uint32_t skip = DELTA ? 0 : sizeof(LdRows<DK>) / 2, row_bytes = sizeof(LdRows<DK>) - skip;  // k is for K S^T
-      const uint64_t keep = policy_evict_last();
-      for (; i < chunks && ok; ++i) {
-        const int st = i % STAGES;
-        if (i >= STAGES) ok = mbar_wait(&empty[st], (i / STAGES - 1) & 1);
-        if (!ok) break;
-        uint8_t* to = ring + st * Shape::STAGE;
-        const size_t block = block_a + i;
-        mbar_arrive_expect_tx(&full[st], row_bytes + (uint32_t)sizeof(LdHead<DK>) + v_boxes * LD_C * 32);
-        bulk_g2s(to + skip, (const uint8_t*)((const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk)) + skip, row_bytes,
-                 &full[st], keep);
-        bulk_g2s(to + Shape::HEAD, (const LdHead<DK>*)c.heads + block * a.Hv + h, sizeof(LdHead<DK>), &full[st], keep);
-        for (int w = 0; w < v_boxes; ++w)
-          tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h,
-                      (int)(first_token + (long long)block * LD_C), &full[st]);
-      }
-      if (!ok)  // the copies in flight land before the block ends
-        for (int st = 0; st < STAGES && st < i; ++st) mbar_wait(&full[st], ((i - 1 - st) / STAGES) & 1);
-    }
-    return;
-  }
-  float* const state = a.state + (((size_t)b * a.Hv + h) * a.Dv + row0) * DK;
-  const bool there = row0 < a.Dv;
-  float S[NK][4] = {};  // times down[] it is the state
-  float down[2] = {1.0f, 1.0f};
-  if (there)
-#pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      const float2 x = *(const float2*)(state + g * DK + n * 8 + cc * 2), y = *(const float2*)(state + (g + 8) * DK + n * 8 + cc * 2);
-      S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
-    }
   bool ok = true;
+  if (outputs) {
+    constexpr uint32_t skip = DELTA ? 0 : sizeof(LdRows<DK>) / 2, row_bytes = sizeof(LdRows<DK>) - skip;  // k is for K S^T
+    const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
+    int loads = 0;
+    auto load = [&] {  // the next chunk; by one lane, whose stage is free
+      uint8_t* const to = ring + loads % STAGES * Shape::STAGE;
+      uint64_t* const bar = &full[loads % STAGES];
+      const size_t block = block_a + loads;
+      const uint64_t keep = policy_evict_last();
+      mbar_arrive_expect_tx(bar, row_bytes + (uint32_t)sizeof(LdHead<DK>) + v_boxes * LD_C * 32);
+      bulk_g2s(to + skip, (const uint8_t*)((const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk)) + skip, row_bytes, bar, keep);
+      bulk_g2s(to + Shape::HEAD, (const LdHead<DK>*)c.heads + block * a.Hv + h, sizeof(LdHead<DK>), bar, keep);
+      for (int w = 0; w < v_boxes; ++w)
+        tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h,
+                    (int)(first_token + (long long)block * LD_C), bar);
+      ++loads;
+    };
+    if (team == 0 && lane == 0)
+      for (int i = 0; i < STAGES && i < chunks; ++i) load();
 #pragma unroll 1
-  for (int i = 0; i < chunks; ++i) {
-    const int st = i % STAGES;
-    ok = mbar_wait(&full[st], (i / STAGES) & 1);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    uint8_t* const stage = ring + st * Shape::STAGE;
-    const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
-    const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
-    uint8_t* const v_s = stage + Shape::V + warp * LD_C * 32;  // and, later, its outputs
-    const long long t0 = first_token + (long long)(block_a + i) * LD_C;
-    const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
-    const bool partial = lo > 0 || hi < LD_C;
-    // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already
-    float m_s[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-      m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
-    }
-    {
-      bool off = false;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        m_s[r] = ld_row_most(m_s[r]);
-        off = off || (m_s[r] != 0.0f && !(m_s[r] >= 0x1p9f && m_s[r] < 0x1p15f));
+    for (int i = 0; i < chunks && ok; ++i) {
+      const int st = i % STAGES;
+      ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team], i & 1);
+      if (!ok) break;
+      if (team == 0 && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
+        ok = mbar_wait(&empty[(i - 1) % STAGES], ((i - 1) / STAGES) & 1);
+        if (ok) load();
       }
-      if (__any_sync(0xffffffffu, off)) {
+      const uint8_t* const stage = ring + st * Shape::STAGE;
+      const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
+      const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
+      const long long t0 = first_token + (long long)(block_a + i) * LD_C;
+      const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
+      float O[PARTS][NT][4] = {};
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float up, dn;
-          ld_scale(m_s[r] * down[r], up, dn);
-          up *= down[r];
-          m_s[r] *= up, down[r] = dn;
+      for (int kt = 0; kt < DK / 16; ++kt) {
+        const uint4 s4 = *(const uint4*)(place + (kt * 32 + lane) * 16);
+        const uint32_t a4[4] = {s4.x, s4.y, s4.z, s4.w};
+        uint32_t q4[4][4];
 #pragma unroll
-          for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
-        }
+        for (int x = 0; x < 4; ++x)
+          ld_matrix4(q4[x], rows.q + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int x = 0; x < NT; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
-    }
-    // S K^T and S Q^T
-    float R[NT][4] = {}, O[NT][4] = {};
+      const float* const scales = (const float*)(place + Shape::SCALES);
 #pragma unroll
-    for (int kt = 0; kt < DK / 16; ++kt) {
-      uint32_t hi4[4], lo4[4];
-      ld_split(S[2 * kt][0], S[2 * kt][1], hi4[0], lo4[0]);
-      ld_split(S[2 * kt][2], S[2 * kt][3], hi4[1], lo4[1]);
-      ld_split(S[2 * kt + 1][0], S[2 * kt + 1][1], hi4[2], lo4[2]);
-      ld_split(S[2 * kt + 1][2], S[2 * kt + 1][3], hi4[3], lo4[3]);
+      for (int y = 0; y < PARTS; ++y) {
+        const float s_down[2] = {scales[y * 16 + g], scales[y * 16 + g + 8]};
 #pragma unroll
-      for (int n = 0; n < NT; n += 4) {
-        uint32_t k4[2][4], q4[2][4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int at = ld_at<PIECES>((n + 2 * x) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1));
-          if (DELTA) ld_matrix4(k4[x], rows.k + at);
-          ld_matrix4(q4[x], rows.q + at);
-        }
-        if (DELTA)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) ld_mma(R[n + x], lo4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) ld_mma(O[n + x], hi4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
-        if (DELTA)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) ld_mma(R[n + x], hi4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
+          for (int x = 0; x < 4; ++x) {
+            if (y == 0) O[0][n][x] *= s_down[x >> 1];
+            if (y > 0) O[0][n][x] = fmaf(O[y][n][x], s_down[x >> 1], O[0][n][x]);
+          }
       }
-    }
-    // R = V - gamma K S^T, zeros for the tokens of other lines
-    float m_r[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < NT; n += 2) {
-      uint32_t v4[4];
-      const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
-      ld_matrix4_trans(v4, v_s + token * 32 + piece * 16);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float v[4];
-        TT::get2(v4[2 * x], v[0], v[1]);
-        TT::get2(v4[2 * x + 1], v[2], v[3]);
-        const int j = (n + x) * 8 + cc * 2;
-        if (DELTA) {
-          const float2 f = *(const float2*)(head.r_in + j);
-          v[0] = fmaf(-R[n + x][0] * down[0], f.x, v[0]), v[1] = fmaf(-R[n + x][1] * down[0], f.y, v[1]);
-          v[2] = fmaf(-R[n + x][2] * down[1], f.x, v[2]), v[3] = fmaf(-R[n + x][3] * down[1], f.y, v[3]);
-        }
-        if (partial) {
-          if (j < lo || j >= hi) v[0] = v[2] = 0.0f;
-          if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = 0.0f;
-        }
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          R[n + x][y] = v[y];
-          m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
-        }
-      }
-    }
-    // O = gamma Q S^T + P T R
-    {
-      float uu[2], ud[2];
-      ld_scale(ld_row_most(m_r[0]), uu[0], ud[0]);
-      ld_scale(ld_row_most(m_r[1]), uu[1], ud[1]);
+      ld_arrive(&s_empty[team], lane);
+      ok = ld_wait(&r_full[team], i & 1);
+      if (!ok) break;
       uint32_t u4[LD_C / 16][4];
 #pragma unroll
       for (int kt = 0; kt < LD_C / 16; ++kt) {
-        u4[kt][0] = ld_half2(R[2 * kt][0] * uu[0], R[2 * kt][1] * uu[0]);
-        u4[kt][1] = ld_half2(R[2 * kt][2] * uu[1], R[2 * kt][3] * uu[1]);
-        u4[kt][2] = ld_half2(R[2 * kt + 1][0] * uu[0], R[2 * kt + 1][1] * uu[0]);
-        u4[kt][3] = ld_half2(R[2 * kt + 1][2] * uu[1], R[2 * kt + 1][3] * uu[1]);
+        const uint4 r4 = *(const uint4*)(place + Shape::R + (kt * 32 + lane) * 16);
+        u4[kt][0] = r4.x, u4[kt][1] = r4.y, u4[kt][2] = r4.z, u4[kt][3] = r4.w;
       }
-      __syncwarp();  // v has been read by all lanes
+      const float r_down[2] = {scales[32 + g], scales[32 + g + 8]};
+      ld_arrive(&r_empty[team], lane);
+      uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
         float pu[2][4] = {};
@@ -771,84 +717,228 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1)
           const int j = (n + x) * 8 + cc * 2;
           const float2 fq = *(const float2*)(head.q_in + j), fp = *(const float2*)(head.p_scale + j);
           float o[4];
-          o[0] = fmaf(O[n + x][0] * down[0], fq.x, pu[x][0] * ud[0] * fp.x), o[1] = fmaf(O[n + x][1] * down[0], fq.y, pu[x][1] * ud[0] * fp.y);
-          o[2] = fmaf(O[n + x][2] * down[1], fq.x, pu[x][2] * ud[1] * fp.x), o[3] = fmaf(O[n + x][3] * down[1], fq.y, pu[x][3] * ud[1] * fp.y);
+          o[0] = fmaf(O[0][n + x][0], fq.x, pu[x][0] * r_down[0] * fp.x), o[1] = fmaf(O[0][n + x][1], fq.y, pu[x][1] * r_down[0] * fp.y);
+          o[2] = fmaf(O[0][n + x][2], fq.x, pu[x][2] * r_down[1] * fp.x), o[3] = fmaf(O[0][n + x][3], fq.y, pu[x][3] * r_down[1] * fp.y);
           o4[2 * x] = TT::put2(o[0], o[1]), o4[2 * x + 1] = TT::put2(o[2], o[3]);
         }
         const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
-        st_matrix4_trans(v_s + token * 32 + piece * 16, o4[0], o4[1], o4[2], o4[3]);
+        st_matrix4_trans(out_s + token * 32 + piece * 16, o4[0], o4[1], o4[2], o4[3]);
       }
-      __syncwarp();
+      ld_arrive(&empty[st], lane);
       if (there)
 #pragma unroll
         for (int x = 0; x < LD_C / 16; ++x) {
           const int token = x * 16 + (lane >> 1), piece = (lane & 1) ^ ((token >> 2) & 1);
           if (token >= lo && token < hi)
             *(uint4*)((uint16_t*)a.out + ((t0 + token) * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8) =
-                *(const uint4*)(v_s + token * 32 + piece * 16);
+                *(const uint4*)(out_s + token * 32 + piece * 16);
         }
+      __syncwarp();  // the outputs have been read
     }
-    // S = gamma_last S + R^T K~, in S's scale or, where the terms are larger (or S has shrunk away), one that suits them
-    {
-      float m[2] = {0.0f, 0.0f}, up[2];
+    // copies in flight land before the block ends (where a wait ran out: those of the other chunks have been waited for)
+    if (team == 0 && lane == 0 && !ok)
+      for (int i = loads - 1; i >= 0 && i >= loads - STAGES; --i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
+    return;
+  }
+  // ---- the state
+  float* const state = a.state + (((size_t)b * a.Hv + h) * a.Dv + row0) * DK + part * (DK / PARTS);
+  float S[NK][4] = {};  // times down[] it is the state
+  float down[2] = {1.0f, 1.0f};
+  if (there)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int j = n * 8 + cc * 2;
-        float2 f = *(const float2*)(head.kt_scale + j);
-        if (partial) {
-          if (j < lo || j >= hi) f.x = 0.0f;
-          if (j + 1 < lo || j + 1 >= hi) f.y = 0.0f;
-        }
-        R[n][0] *= f.x, R[n][1] *= f.y, R[n][2] *= f.x, R[n][3] *= f.y;
-        m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0]), fabsf(R[n][1])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2]), fabsf(R[n][3])));
-      }
-      const float gamma = head.gamma[hi - 1];
-      float g2[2];
+    for (int n = 0; n < NK; ++n) {
+      const float2 x = *(const float2*)(state + g * DK + n * 8 + cc * 2), y = *(const float2*)(state + (g + 8) * DK + n * 8 + cc * 2);
+      S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
+    }
+  float* const scales = (float*)(place + Shape::SCALES);
+#pragma unroll 1
+  for (int i = 0; i < chunks; ++i) {
+    const int st = i % STAGES;
+    const uint8_t* const stage = ring + st * Shape::STAGE;
+    const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
+    const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
+    const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
+    const long long t0 = first_token + (long long)(block_a + i) * LD_C;
+    const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
+    const bool partial = lo > 0 || hi < LD_C;
+    ok = mbar_wait(&full[st], (i / STAGES) & 1) && (i == 0 || mbar_wait(&s_empty[team], (i - 1) & 1));
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    // operands are asked for before what they are multiplied by is known
+    uint32_t k4[4][4];
+    auto get_k = [&](int kt) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        ld_matrix4(k4[x], rows.k + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, (part * KT + kt) * 2 + ((lane >> 3) & 1)));
+    };
+    if (DELTA) get_k(0);
+    // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already
+    float m_s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
+      m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
+    }
+    bool off = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      m_s[r] = ld_row_most(m_s[r]);
+      off = off || (m_s[r] != 0.0f && !(m_s[r] >= 0x1p9f && m_s[r] < 0x1p15f));
+    }
+    if (__any_sync(0xffffffffu, off)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        // of a size: gamma S, and R times K~'s rows, which are below 2^15 and mostly near 2^7
-        const float most = fmaxf(gamma * m_s[r] * down[r], ld_row_most(m[r]) * 0x1p7f);
-        const float at = most * ld_inverse(down[r]);
-        float dn = down[r];
-        if (!(at >= 0x1p9f && at < 0x1p15f)) {
-          float u;
-          ld_scale(most, u, dn);
-        }
-        up[r] = ld_inverse(dn);
-        g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
-        down[r] = dn;
-      }
+        float up, dn;
+        ld_scale(m_s[r] * down[r], up, dn);
+        up *= down[r];
+        m_s[r] *= up, down[r] = dn;
 #pragma unroll
-      for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
-#pragma unroll
-      for (int kt = 0; kt < LD_C / 16; ++kt) {
-        uint32_t hi4[4], lo4[4];
-        ld_split(R[2 * kt][0] * up[0], R[2 * kt][1] * up[0], hi4[0], lo4[0]);
-        ld_split(R[2 * kt][2] * up[1], R[2 * kt][3] * up[1], hi4[1], lo4[1]);
-        ld_split(R[2 * kt + 1][0] * up[0], R[2 * kt + 1][1] * up[0], hi4[2], lo4[2]);
-        ld_split(R[2 * kt + 1][2] * up[1], R[2 * kt + 1][3] * up[1], hi4[3], lo4[3]);
-#pragma unroll
-        for (int n = 0; n < NK; n += 4) {
-          uint32_t b_hi[2][4], b_lo[2][4];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int at = ld_at<PIECES>(kt * 16 + (lane & 15), n + 2 * x + (lane >> 4));
-            ld_matrix4_trans(b_lo[x], head.kt_lo + at);
-            ld_matrix4_trans(b_hi[x], head.kt_hi + at);
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], hi4, b_lo[x / 2][x % 2 * 2], b_lo[x / 2][x % 2 * 2 + 1]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], lo4, b_hi[x / 2][x % 2 * 2], b_hi[x / 2][x % 2 * 2 + 1]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) ld_mma(S[n + x], hi4, b_hi[x / 2][x % 2 * 2], b_hi[x / 2][x % 2 * 2 + 1]);
-        }
+        for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
       }
     }
-    fence_async_smem();  // the outputs' place is the next TMA load's
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
+    // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs
+    float R[NT][4] = {}, low[NT][4] = {};
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      uint32_t hi4[4], lo4[4];
+      ld_split(S[2 * kt][0], S[2 * kt][1], hi4[0], lo4[0]);
+      ld_split(S[2 * kt][2], S[2 * kt][3], hi4[1], lo4[1]);
+      ld_split(S[2 * kt + 1][0], S[2 * kt + 1][1], hi4[2], lo4[2]);
+      ld_split(S[2 * kt + 1][2], S[2 * kt + 1][3], hi4[3], lo4[3]);
+      *(uint4*)(place + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+      if (DELTA) {
+        if (kt > 0) get_k(kt);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) ld_mma(R[x], hi4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) ld_mma(low[x], lo4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
+      }
+    }
+    if (cc == 0) scales[part * 16 + g] = down[0], scales[part * 16 + g + 8] = down[1];
+    ld_arrive(&s_full[team], lane);
+    uint32_t v4[NT / 2][4];
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
+      ld_matrix4_trans(v4[n / 2], v_s + token * 32 + piece * 16);
+    }
+    if (DELTA) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) R[n][x] = (R[n][x] + low[n][x]) * down[x >> 1];
+    }
+    if constexpr (DELTA && PARTS > 1) {  // the parts' shares, each the sum of both in the same order
+      float4* const mine = (float4*)(place + Shape::SHARES + ((i & 1) * PARTS + part) * LD_C * 64) + lane;
+      const float4* const theirs = (const float4*)(place + Shape::SHARES + ((i & 1) * PARTS + 1 - part) * LD_C * 64) + lane;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mine[n * 32] = make_float4(R[n][0], R[n][1], R[n][2], R[n][3]);
+      ld_arrive(&shares[team][part], lane);
+      ok = mbar_wait(&shares[team][1 - part], i & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float4 y = theirs[n * 32];
+        R[n][0] += y.x, R[n][1] += y.y, R[n][2] += y.z, R[n][3] += y.w;
+      }
+    } else {
+      if (i > 0) ok = ld_wait(&r_empty[team], (i - 1) & 1);
+      if (!ok) break;
+    }
+    uint32_t b_hi[2][G / 2][4], b_lo[2][G / 2][4];
+    auto get_b = [&](int at) {  // the G columns and 16 tokens of step `at`
+      const int kt = at / (NK / G), n = at % (NK / G) * G;
+#pragma unroll
+      for (int x = 0; x < G / 2; ++x) {
+        const int where = ld_at<PIECES>(kt * 16 + (lane & 15), part * NK + n + 2 * x + (lane >> 4));
+        ld_matrix4_trans(b_lo[at & 1][x], head.kt_lo + where);
+        ld_matrix4_trans(b_hi[at & 1][x], head.kt_hi + where);
+      }
+    };
+    get_b(0);
+    // R = V - gamma K S^T, zeros for the tokens of other lines; how large its rows are, alone and with K~'s factors
+    float m_r[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+    float2 f[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float v[4];
+      TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
+      TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
+      const int j = n * 8 + cc * 2;
+      f[n] = *(const float2*)(head.kt_scale + j);
+      if (DELTA) {
+        const float2 in = *(const float2*)(head.r_in + j);
+        v[0] = fmaf(-R[n][0], in.x, v[0]), v[1] = fmaf(-R[n][1], in.y, v[1]);
+        v[2] = fmaf(-R[n][2], in.x, v[2]), v[3] = fmaf(-R[n][3], in.y, v[3]);
+      }
+      if (partial) {
+        if (j < lo || j >= hi) v[0] = v[2] = f[n].x = 0.0f;
+        if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f[n].y = 0.0f;
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        R[n][y] = v[y];
+        m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
+        m[y >> 1] = fmaxf(m[y >> 1], fabsf(v[y] * (y & 1 ? f[n].y : f[n].x)));
+      }
+    }
+    // S = gamma_last S + R^T K~, in S's scale or, where the terms are larger (or S has shrunk away), one that suits them
+    const float gamma = head.gamma[hi - 1];
+    float up[2], g2[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      // of a size: gamma S, and R times K~'s rows, which are below 2^15 and mostly near 2^7
+      const float most = fmaxf(gamma * m_s[r] * down[r], ld_row_most(m[r]) * 0x1p7f);
+      const float at = most * ld_inverse(down[r]);
+      float dn = down[r];
+      if (!(at >= 0x1p9f && at < 0x1p15f)) {
+        float u;
+        ld_scale(most, u, dn);
+      }
+      up[r] = ld_inverse(dn);
+      g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
+      down[r] = dn;
+    }
+#pragma unroll
+    for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
+#pragma unroll
+    for (int kt = 0; kt < LD_C / 16; ++kt) {
+      uint32_t hi4[4], lo4[4];
+      const float2 f0 = f[2 * kt], f1 = f[2 * kt + 1];
+      ld_split(R[2 * kt][0] * f0.x * up[0], R[2 * kt][1] * f0.y * up[0], hi4[0], lo4[0]);
+      ld_split(R[2 * kt][2] * f0.x * up[1], R[2 * kt][3] * f0.y * up[1], hi4[1], lo4[1]);
+      ld_split(R[2 * kt + 1][0] * f1.x * up[0], R[2 * kt + 1][1] * f1.y * up[0], hi4[2], lo4[2]);
+      ld_split(R[2 * kt + 1][2] * f1.x * up[1], R[2 * kt + 1][3] * f1.y * up[1], hi4[3], lo4[3]);
+#pragma unroll
+      for (int n = 0; n < NK; n += G) {
+        const int at = kt * (NK / G) + n / G;
+        if (at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1);
+        const auto& bh = b_hi[at & 1];
+        const auto& bl = b_lo[at & 1];
+#pragma unroll
+        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4, bl[x / 2][x % 2 * 2], bl[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+        for (int x = 0; x < G; ++x) ld_mma(S[n + x], lo4, bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4, bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
+      }
+      if (kt == 0) {  // R for the outputs, one term, beside the products
+        float uu[2], ud[2];
+        ld_scale(ld_row_most(m_r[0]), uu[0], ud[0]);
+        ld_scale(ld_row_most(m_r[1]), uu[1], ud[1]);
+#pragma unroll
+        for (int y = 0; y < LD_C / 16; ++y)
+          if (y % PARTS == part)
+            *(uint4*)(place + Shape::R + (y * 32 + lane) * 16) =
+                make_uint4(ld_half2(R[2 * y][0] * uu[0], R[2 * y][1] * uu[0]), ld_half2(R[2 * y][2] * uu[1], R[2 * y][3] * uu[1]),
+                           ld_half2(R[2 * y + 1][0] * uu[0], R[2 * y + 1][1] * uu[0]),
+                           ld_half2(R[2 * y + 1][2] * uu[1], R[2 * y + 1][3] * uu[1]));
+        if (cc == 0 && part == 0) scales[32 + g] = ud[0], scales[32 + g + 8] = ud[1];
+        ld_arrive(&r_full[team], lane);
+      }
+    }
+    ld_arrive(&empty[st], lane);
   }
   if (there && ok)
 #pragma unroll
