@@ -42,6 +42,7 @@ template <int DK> struct alignas(128) LdHead {
   float r_in[LD_C];   // gamma_i |k| factor: of K S^T
   float q_in[LD_C];   // scale gamma_i |q| factor: of Q S^T
   float gamma[LD_C];
+  float kt_most, unused[63];  // the largest of kt_scale; to whole 256 bytes
 };
 
 // Element offset of 16-byte piece c of row r in rows of `pieces` of them (a multiple of 8): eight rows' pieces of one column lie
@@ -550,11 +551,19 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
     const float nan = __uint_as_float(0x7fc00000u), gamma = ld_exp(G_s[tid].x + G_s[tid].y);
     const bool bad = bad_s[first] != 0, live = my_line >= 0;
     out->gamma[tid] = gamma;
+    float kt_most = live ? kt_scale[tid] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) kt_most = fmaxf(kt_most, __shfl_xor_sync(0xffffffffu, kt_most, o));
+    if (lane == 0) ((float*)&sum_s)[warp] = kt_most;
     out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
     out->r_in[tid] = live && !bad ? gamma * k_factor[tid] : 0.0f;
     out->q_in[tid] = !live ? 0.0f : bad ? nan : gamma * q_factor[tid];
   }
-  if (tid == 0) ld_bulk_done();
+  __syncthreads();
+  if (tid == 0) {
+    out->kt_most = fmaxf(((float*)&sum_s)[0], ((float*)&sum_s)[1]);
+    ld_bulk_done();
+  }
 }
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks. 16 rows are a team of
@@ -567,8 +576,9 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
 // there and back between the products: with 16 rows a warp the chain is shorter in registers.)
 template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
-  // a team's place: S's high terms as A fragments, R's likewise, the rows' scales (of S's parts, of R), the outputs, shares of K S^T
-  static constexpr int R = DK * 32, SCALES = R + LD_C * 32, OUT = SCALES + 256, SHARES = OUT + LD_C * 32;
+  // a team's place: S's high terms as A fragments and its rows' scales (two chunks' by turns), R's terms and scales, the outputs,
+  // shares of K S^T (two chunks')
+  static constexpr int S = DK * 32 + 128, R = 2 * S, SCALES = R + LD_C * 32, OUT = SCALES + 128, SHARES = OUT + LD_C * 32;
   static constexpr int TEAM = SHARES + (PARTS > 1 ? 2 * PARTS * LD_C * 64 : 0);
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024, THREADS = WARPS * (PARTS + 1) * 32;
@@ -600,7 +610,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   constexpr int PIECES = DK / 8, NK = DK / 8 / PARTS, KT = DK / 16 / PARTS, NT = LD_C / 8, STAGES = Shape::STAGES;
   constexpr int G = NK < 8 ? NK : 8;  // sums of S that take turns
   extern __shared__ uint8_t ld_raw[];
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS], s_empty[WARPS], r_full[WARPS], r_empty[WARPS], shares[WARPS][PARTS];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], r_full[WARPS],
+      r_empty[WARPS], shares[WARPS][PARTS][2];  // [2]: odd and even chunks', as their places
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -611,8 +622,11 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + 1) * WARPS);
     for (int i = 0; i < WARPS; ++i) {
-      mbar_init(&s_full[i], PARTS), mbar_init(&s_empty[i], 1), mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], 1);
-      for (int j = 0; j < PARTS; ++j) mbar_init(&shares[i][j], 1);
+      mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], 1);
+      for (int y = 0; y < 2; ++y) {
+        mbar_init(&s_full[i][y], PARTS);
+        for (int j = 0; j < PARTS; ++j) mbar_init(&shares[i][j][y], 1);
+      }
     }
     fence_mbar_init();
   }
@@ -655,7 +669,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll 1
     for (int i = 0; i < chunks && ok; ++i) {
       const int st = i % STAGES;
-      ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team], i & 1);
+      ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team][i & 1], (i >> 1) & 1);
       if (!ok) break;
       if (team == 0 && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
         ok = mbar_wait(&empty[(i - 1) % STAGES], ((i - 1) / STAGES) & 1);
@@ -669,7 +683,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       float O[PARTS][NT][4] = {};
 #pragma unroll
       for (int kt = 0; kt < DK / 16; ++kt) {
-        const uint4 s4 = *(const uint4*)(place + (kt * 32 + lane) * 16);
+        const uint4 s4 = *(const uint4*)(place + (i & 1) * Shape::S + (kt * 32 + lane) * 16);
         const uint32_t a4[4] = {s4.x, s4.y, s4.z, s4.w};
         uint32_t q4[4][4];
 #pragma unroll
@@ -678,10 +692,10 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
         for (int x = 0; x < NT; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
-      const float* const scales = (const float*)(place + Shape::SCALES);
+      const float* const s_scales = (const float*)(place + (i & 1) * Shape::S + DK * 32);
 #pragma unroll
       for (int y = 0; y < PARTS; ++y) {
-        const float s_down[2] = {scales[y * 16 + g], scales[y * 16 + g + 8]};
+        const float s_down[2] = {s_scales[y * 16 + g], s_scales[y * 16 + g + 8]};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -690,7 +704,6 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
             if (y > 0) O[0][n][x] = fmaf(O[y][n][x], s_down[x >> 1], O[0][n][x]);
           }
       }
-      ld_arrive(&s_empty[team], lane);
       ok = ld_wait(&r_full[team], i & 1);
       if (!ok) break;
       uint32_t u4[LD_C / 16][4];
@@ -699,7 +712,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         const uint4 r4 = *(const uint4*)(place + Shape::R + (kt * 32 + lane) * 16);
         u4[kt][0] = r4.x, u4[kt][1] = r4.y, u4[kt][2] = r4.z, u4[kt][3] = r4.w;
       }
-      const float r_down[2] = {scales[32 + g], scales[32 + g + 8]};
+      const float* const r_scales = (const float*)(place + Shape::SCALES);
+      const float r_down[2] = {r_scales[g], r_scales[g + 8]};
       ld_arrive(&r_empty[team], lane);
       uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
@@ -742,7 +756,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   }
   // ---- the state
   float* const state = a.state + (((size_t)b * a.Hv + h) * a.Dv + row0) * DK + part * (DK / PARTS);
-  float S[NK][4] = {};  // times down[] it is the state
+  const uint32_t quad = 0xfu << (lane & ~3);  // the lanes of this one's rows
+  float S[NK][4] = {};                        // times down[] it is the state
   float down[2] = {1.0f, 1.0f};
   if (there)
 #pragma unroll
@@ -750,7 +765,6 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const float2 x = *(const float2*)(state + g * DK + n * 8 + cc * 2), y = *(const float2*)(state + (g + 8) * DK + n * 8 + cc * 2);
       S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
     }
-  float* const scales = (float*)(place + Shape::SCALES);
 #pragma unroll 1
   for (int i = 0; i < chunks; ++i) {
     const int st = i % STAGES;
@@ -761,8 +775,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     const long long t0 = first_token + (long long)(block_a + i) * LD_C;
     const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
     const bool partial = lo > 0 || hi < LD_C;
-    ok = mbar_wait(&full[st], (i / STAGES) & 1) && (i == 0 || mbar_wait(&s_empty[team], (i - 1) & 1));
-    ok = __all_sync(0xffffffffu, ok);
+    ok = ld_wait(&full[st], (i / STAGES) & 1);
     if (!ok) break;
     // operands are asked for before what they are multiplied by is known
     uint32_t k4[4][4];
@@ -772,28 +785,30 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         ld_matrix4(k4[x], rows.k + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, (part * KT + kt) * 2 + ((lane >> 3) & 1)));
     };
     if (DELTA) get_k(0);
-    // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already
-    float m_s[2] = {0.0f, 0.0f};
+    // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already: votes tell, without the largest itself
+    bool fresh = false;  // a row of zeros, which has no size
+    {
+      float m[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-      m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
-    }
-    bool off = false;
+      for (int n = 0; n < NK; ++n) {
+        m[0] = fmaxf(m[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
+        m[1] = fmaxf(m[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
+      }
+      const uint32_t some[2] = {__ballot_sync(0xffffffffu, m[0] >= 0x1p9f), __ballot_sync(0xffffffffu, m[1] >= 0x1p9f)};
+      const bool off = fmaxf(m[0], m[1]) >= 0x1p15f || !(some[0] & quad) || !(some[1] & quad);
+      if (__any_sync(0xffffffffu, off)) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      m_s[r] = ld_row_most(m_s[r]);
-      off = off || (m_s[r] != 0.0f && !(m_s[r] >= 0x1p9f && m_s[r] < 0x1p15f));
-    }
-    if (__any_sync(0xffffffffu, off)) {
+        for (int r = 0; r < 2; ++r) {
+          const float most = ld_row_most(m[r]);  // by all lanes
+          float up, dn;
+          ld_scale(most * down[r], up, dn);
+          up *= down[r];
+          fresh |= most == 0.0f;
+          down[r] = dn;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float up, dn;
-        ld_scale(m_s[r] * down[r], up, dn);
-        up *= down[r];
-        m_s[r] *= up, down[r] = dn;
-#pragma unroll
-        for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
+          for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
+        }
+        fresh = __any_sync(0xffffffffu, fresh);
       }
     }
     // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs
@@ -805,7 +820,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       ld_split(S[2 * kt][2], S[2 * kt][3], hi4[1], lo4[1]);
       ld_split(S[2 * kt + 1][0], S[2 * kt + 1][1], hi4[2], lo4[2]);
       ld_split(S[2 * kt + 1][2], S[2 * kt + 1][3], hi4[3], lo4[3]);
-      *(uint4*)(place + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+      *(uint4*)(place + (i & 1) * Shape::S + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
       if (DELTA) {
         if (kt > 0) get_k(kt);
 #pragma unroll
@@ -814,8 +829,11 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         for (int x = 0; x < NT; ++x) ld_mma(low[x], lo4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
       }
     }
-    if (cc == 0) scales[part * 16 + g] = down[0], scales[part * 16 + g + 8] = down[1];
-    ld_arrive(&s_full[team], lane);
+    if (cc == 0) {
+      float* const s_scales = (float*)(place + (i & 1) * Shape::S + DK * 32) + part * 16;
+      s_scales[g] = down[0], s_scales[g + 8] = down[1];
+    }
+    ld_arrive(&s_full[team][i & 1], lane);
     uint32_t v4[NT / 2][4];
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
@@ -833,8 +851,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const float4* const theirs = (const float4*)(place + Shape::SHARES + ((i & 1) * PARTS + 1 - part) * LD_C * 64) + lane;
 #pragma unroll
       for (int n = 0; n < NT; ++n) mine[n * 32] = make_float4(R[n][0], R[n][1], R[n][2], R[n][3]);
-      ld_arrive(&shares[team][part], lane);
-      ok = mbar_wait(&shares[team][1 - part], i & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
+      ld_arrive(&shares[team][part][i & 1], lane);
+      ok = mbar_wait(&shares[team][1 - part][i & 1], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
 #pragma unroll
@@ -857,8 +875,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       }
     };
     get_b(0);
-    // R = V - gamma K S^T, zeros for the tokens of other lines; how large its rows are, alone and with K~'s factors
-    float m_r[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+    // R = V - gamma K S^T, zeros for the tokens of other lines
+    float m_r[2] = {0.0f, 0.0f};
     float2 f[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -880,48 +898,62 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       for (int y = 0; y < 4; ++y) {
         R[n][y] = v[y];
         m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
-        m[y >> 1] = fmaxf(m[y >> 1], fabsf(v[y] * (y & 1 ? f[n].y : f[n].x)));
       }
     }
-    // S = gamma_last S + R^T K~, in S's scale or, where the terms are larger (or S has shrunk away), one that suits them
+    // S = gamma_last S + R^T K~, in S's scale: R times K~'s rows, which are below 2^15 and mostly near 2^7, must not pass it. Where
+    // that is not certain, or S nearly vanishes, in one that suits the larger of the two.
     const float gamma = head.gamma[hi - 1];
-    float up[2], g2[2];
+    float up[2] = {ld_inverse(down[0]), ld_inverse(down[1])}, g2[2] = {gamma, gamma};
+    if (__any_sync(0xffffffffu, fresh || !(gamma >= 0x1p-5f) ||
+                                    !(fmaxf(m_r[0] * up[0], m_r[1] * up[1]) * head.kt_most < 0x1p8f))) {
+      float m[2] = {0.0f, 0.0f}, m_s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      // of a size: gamma S, and R times K~'s rows, which are below 2^15 and mostly near 2^7
-      const float most = fmaxf(gamma * m_s[r] * down[r], ld_row_most(m[r]) * 0x1p7f);
-      const float at = most * ld_inverse(down[r]);
-      float dn = down[r];
-      if (!(at >= 0x1p9f && at < 0x1p15f)) {
-        float u;
-        ld_scale(most, u, dn);
+      for (int n = 0; n < NT; ++n) {
+        m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0] * f[n].x), fabsf(R[n][1] * f[n].y)));
+        m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2] * f[n].x), fabsf(R[n][3] * f[n].y)));
       }
-      up[r] = ld_inverse(dn);
-      g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
-      down[r] = dn;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
+        m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float dn;
+        ld_scale(fmaxf(gamma * (ld_row_most(m_s[r]) * down[r]), ld_row_most(m[r]) * 0x1p7f), up[r], dn);
+        g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
+        down[r] = dn;
+      }
     }
 #pragma unroll
     for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
+    float small[G][4] = {};  // the products of one low term, in sums of their own for the first G columns: more take turns
+    uint32_t hi4[2][4], lo4[2][4];
+    auto terms = [&](int kt) {
+      const float2 f0 = f[2 * kt], f1 = f[2 * kt + 1];
+      uint32_t (&hi)[4] = hi4[kt & 1], (&lo)[4] = lo4[kt & 1];
+      ld_split(R[2 * kt][0] * f0.x * up[0], R[2 * kt][1] * f0.y * up[0], hi[0], lo[0]);
+      ld_split(R[2 * kt][2] * f0.x * up[1], R[2 * kt][3] * f0.y * up[1], hi[1], lo[1]);
+      ld_split(R[2 * kt + 1][0] * f1.x * up[0], R[2 * kt + 1][1] * f1.y * up[0], hi[2], lo[2]);
+      ld_split(R[2 * kt + 1][2] * f1.x * up[1], R[2 * kt + 1][3] * f1.y * up[1], hi[3], lo[3]);
+    };
+    terms(0);
 #pragma unroll
     for (int kt = 0; kt < LD_C / 16; ++kt) {
-      uint32_t hi4[4], lo4[4];
-      const float2 f0 = f[2 * kt], f1 = f[2 * kt + 1];
-      ld_split(R[2 * kt][0] * f0.x * up[0], R[2 * kt][1] * f0.y * up[0], hi4[0], lo4[0]);
-      ld_split(R[2 * kt][2] * f0.x * up[1], R[2 * kt][3] * f0.y * up[1], hi4[1], lo4[1]);
-      ld_split(R[2 * kt + 1][0] * f1.x * up[0], R[2 * kt + 1][1] * f1.y * up[0], hi4[2], lo4[2]);
-      ld_split(R[2 * kt + 1][2] * f1.x * up[1], R[2 * kt + 1][3] * f1.y * up[1], hi4[3], lo4[3]);
 #pragma unroll
       for (int n = 0; n < NK; n += G) {
         const int at = kt * (NK / G) + n / G;
-        if (at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1);
         const auto& bh = b_hi[at & 1];
         const auto& bl = b_lo[at & 1];
+        float (*const low)[4] = n == 0 ? small : S + n;
 #pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4, bl[x / 2][x % 2 * 2], bl[x / 2][x % 2 * 2 + 1]);
+        for (int x = 0; x < G; ++x) ld_mma(low[x], hi4[kt & 1], bl[x / 2][x % 2 * 2], bl[x / 2][x % 2 * 2 + 1]);
+        if (at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1);
 #pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(S[n + x], lo4, bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
+        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4[kt & 1], bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
+        if (n == 0 && kt + 1 < LD_C / 16) terms(kt + 1);
 #pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4, bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
+        for (int x = 0; x < G; ++x) ld_mma(low[x], lo4[kt & 1], bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
       }
       if (kt == 0) {  // R for the outputs, one term, beside the products
         float uu[2], ud[2];
@@ -934,10 +966,17 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
                 make_uint4(ld_half2(R[2 * y][0] * uu[0], R[2 * y][1] * uu[0]), ld_half2(R[2 * y][2] * uu[1], R[2 * y][3] * uu[1]),
                            ld_half2(R[2 * y + 1][0] * uu[0], R[2 * y + 1][1] * uu[0]),
                            ld_half2(R[2 * y + 1][2] * uu[1], R[2 * y + 1][3] * uu[1]));
-        if (cc == 0 && part == 0) scales[32 + g] = ud[0], scales[32 + g + 8] = ud[1];
+        if (cc == 0 && part == 0) {
+          float* const r_scales = (float*)(place + Shape::SCALES);
+          r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
+        }
         ld_arrive(&r_full[team], lane);
       }
     }
+#pragma unroll
+    for (int x = 0; x < G; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) S[x][y] += small[x][y];
     ld_arrive(&empty[st], lane);
   }
   if (there && ok)
