@@ -102,45 +102,77 @@ struct LdChunkArgs {
 // time went into fetching instructions.) K~ = T^T D K and P T are products of two fp16 terms each.
 constexpr int LD_PREP_THREADS = 128;
 constexpr int LD_PITCH = 68;    // floats of a row of A and T in shared memory
-constexpr int LD_PITCH_Y = 36;  // ... of A21 T1
+constexpr int LD_PITCH_Y = 40;  // ... of A21 T1
 constexpr float LD_MAX = 3.4028234e38f;
 
 template <int DK> struct LdPrepShape {
   static constexpr int K = LD_C * DK * 2, T = 2 * LD_C * LD_C * 2;
-  static constexpr int Q = K > T ? K : T;  // the rows of q, then T^T
-  static constexpr int A = LD_C * LD_PITCH * 4;
-  static constexpr int SMEM = K + Q + T + A;
-  static_assert(A >= K && T >= K, "K~'s terms take the places of A and of T^T D");
-  static_assert(T >= 32 * LD_PITCH_Y * 4, "A21 T1 takes that of T^T D");
+  static constexpr int Q = K > T ? K : T;  // the rows of q; A21 T1; T^T; K~'s low terms
+  static constexpr int A = LD_C * LD_PITCH * 4 > K ? LD_C * LD_PITCH * 4 : K;  // A and T; T^T D; K~'s high terms
+  static constexpr int SMEM = K + Q + A;
+  static_assert(A >= T && Q >= 32 * LD_PITCH_Y * 4, "");
 };
 
-// X = -T2 (A21 T1) for the blocks of N x N at rows r0 + N.., columns r0..: `threads` threads, of which this is number t.
-template <int N, int THREADS> D3_DEV void ld_join(float* A, float* Y, unsigned long long starts, int r0, int t) {
-  constexpr int COLS = N * N / THREADS, PER = N / COLS;  // columns a thread, threads a row
-  const int r = t / PER, c = t % PER * COLS;
+D3_DEV void ld_mma_tf32(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// x as two tf32 terms, 22 bits and the whole range of exponents.
+D3_DEV void ld_split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+
+// acc += X Y by a warp: X [16][8 STEPS] at x, Y [8 STEPS][8 TILES] at y, 32-bit rows of pitch px and py.
+template <int STEPS, int TILES>
+D3_DEV void ld_product(float (&acc)[TILES][4], const float* x, int px, const float* y, int py, int lane) {
+  const int g = lane >> 2, cc = lane & 3;
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    float acc[COLS] = {};
-#pragma unroll 8
-    for (int m = 0; m < N; ++m) {
-      const float x = A[(r0 + N + r) * LD_PITCH + r0 + (pass ? N : 0) + m];
-      const float* y = pass ? Y + m * LD_PITCH_Y + c : A + (r0 + m) * LD_PITCH + r0 + c;
+  for (int k = 0; k < STEPS; ++k) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < COLS; e += 4) {
-        const float4 v = *(const float4*)(y + e);
-        acc[e] = fmaf(x, v.x, acc[e]), acc[e + 1] = fmaf(x, v.y, acc[e + 1]);
-        acc[e + 2] = fmaf(x, v.z, acc[e + 2]), acc[e + 3] = fmaf(x, v.w, acc[e + 3]);
-      }
+    for (int e = 0; e < 4; ++e) ld_split_tf32(x[(g + (e & 1) * 8) * px + k * 8 + cc + (e >> 1) * 4], hi[e], lo[e]);
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+      uint32_t b_hi[2], b_lo[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) ld_split_tf32(y[(k * 8 + cc + e * 4) * py + n * 8 + g], b_hi[e], b_lo[e]);
+      ld_mma_tf32(acc[n], lo, b_hi);
+      ld_mma_tf32(acc[n], hi, b_lo);
+      ld_mma_tf32(acc[n], hi, b_hi);
     }
-#pragma unroll
-    for (int e = 0; e < COLS; ++e) {
-      if (pass)  // entries of two lines (one starts in between) are zeros whatever the sums met
-        A[(r0 + N + r) * LD_PITCH + r0 + c + e] = (starts & (~0ull >> (63 - (r0 + N + r)))) >> (r0 + c + e + 1) ? 0.0f : -acc[e];
-      else
-        Y[r * LD_PITCH_Y + c + e] = acc[e];
-    }
-    __syncthreads();
   }
+}
+
+// X = -T2 (A21 T1) for the blocks of N x N at rows r0 + N.., columns r0.. of A, of which a warp has 16 rows from `row` on and 8
+// TILES columns from `col` on; all four warps go through it together.
+template <int N, int TILES> D3_DEV void ld_join(float* A, float* Y, unsigned long long starts, int r0, int row, int col, int lane) {
+  const int g = lane >> 2, cc = lane & 3;
+  {
+    float acc[TILES][4] = {};
+    ld_product<N / 8, TILES>(acc, A + (r0 + N + row) * LD_PITCH + r0, LD_PITCH, A + r0 * LD_PITCH + r0 + col, LD_PITCH, lane);
+#pragma unroll
+    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        *(float2*)(Y + (row + g + r * 8) * LD_PITCH_Y + col + n * 8 + cc * 2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+  }
+  __syncthreads();
+  float acc[TILES][4] = {};
+  ld_product<N / 8, TILES>(acc, A + (r0 + N + row) * LD_PITCH + r0 + N, LD_PITCH, Y + col, LD_PITCH_Y, lane);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = r0 + N + row + g + r * 8;
+    const unsigned long long until = starts & (~0ull >> (63 - i));
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+      const int j = r0 + col + n * 8 + cc * 2;  // entries of two lines (one starts in between) are zeros whatever the sums met
+      *(float2*)(A + i * LD_PITCH + j) =
+          make_float2(until >> (j + 1) ? 0.0f : -acc[n][2 * r], until >> (j + 2) ? 0.0f : -acc[n][2 * r + 1]);
+    }
+  }
+  __syncthreads();
 }
 
 // A shared-memory area into global memory by the copy engine: `bytes` a multiple of 16, both 16-byte aligned. One thread issues
@@ -161,21 +193,22 @@ D3_DEV float ld_exp(float x) {
 }
 
 template <int TYPE, int DK, bool DELTA>
-__global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(LdChunkArgs c) {
+__global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(LdChunkArgs c) {
   using TT = QrType<TYPE>;
   using E = typename TT::T;
   using Shape = LdPrepShape<DK>;
-  constexpr int PIECES = DK / 8, LANES = PIECES, AT_ONCE = 32 / LANES;
+  constexpr int PIECES = DK / 8;
   extern __shared__ __align__(128) uint8_t ld_smem[];
   uint16_t* const ks = (uint16_t*)ld_smem;
   uint16_t* const qs = (uint16_t*)(ld_smem + Shape::K);
-  uint16_t* const tt = qs;                                              // T^T, two terms, where q was
-  uint16_t* const td = (uint16_t*)(ld_smem + Shape::K + Shape::Q);      // T^T D, two terms
-  float* const A = (float*)(ld_smem + Shape::K + Shape::Q + Shape::T);  // A, then T
-  float* const Y = (float*)td;
+  float* const A = (float*)(ld_smem + Shape::K + Shape::Q);  // A, then T
+  float* const Y = (float*)qs;                               // A21 T1, when q has been read
+  uint16_t* const tt = qs;                                   // T^T, two terms, after that
+  uint16_t* const td = (uint16_t*)A;                         // T^T D, two terms, when T has been read
+  __shared__ __align__(8) uint64_t arrived;
   __shared__ int line_s[LD_C];
   __shared__ uint32_t starts_s[2];
-  __shared__ float k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], d_s[LD_C], t_scale[LD_C], kt_scale[LD_C];
+  __shared__ __align__(16) float d_s[LD_C], t_scale[LD_C], k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], kt_scale[LD_C];
   __shared__ double sum_s;
   __shared__ float2 G_s[LD_C];  // as the sum of two
   __shared__ int bad_s[LD_C];   // by a line's first token in the chunk: something of it is not finite
@@ -184,8 +217,26 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
   const int block = blockIdx.x, h = blockIdx.y, many = a.Hv / a.Hk, hk = h / many;
   const long long t0 = (long long)(c.block0 + block) * LD_C;
   LdHead<DK>* const out = (LdHead<DK>*)c.heads + (size_t)block * a.Hv + h;
+  if (tid == 0) {
+    mbar_init(&arrived, 1);
+    fence_mbar_init();
+  }
   grid_dependency_wait();
   allow_dependents();
+  __syncthreads();
+  // the rows of k and q come together, a copy each; where the pass has ended, zeros
+  {
+    const bool is_q = tid >= LD_C;
+    const int row = tid & (LD_C - 1), live = (int)min((long long)LD_C, a.T - t0);
+    uint16_t* const to = (is_q ? qs : ks) + row * DK;
+    if (tid == 0) mbar_arrive_expect_tx(&arrived, 2 * live * DK * 2);
+    if (row < live) {
+      const QrTensor& x = is_q ? a.q : a.k;
+      bulk_g2s(to, (const E*)x.p + (t0 + row) * x.token + hk * x.head, DK * 2, &arrived, policy_evict_last());
+    } else {
+      for (int i = 0; i < PIECES; ++i) ((uint4*)to)[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
   float decay = 0.0f, beta = 0.0f;
   int my_line = -1;
   if (tid < LD_C) {
@@ -193,54 +244,57 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
     my_line = l >= 0 && l < a.B ? l : -1;
     line_s[tid] = my_line;
     bad_s[tid] = 0;
-  }
-  // rows to fp16, each by the power of two that brings its largest value into [1, 2)
-  {
-    const int l = lane % LANES;
-    constexpr int ROUNDS = 2 * LD_C / 4 / AT_ONCE, AHEAD = 4;  // a warp: 16 rows of k, then 16 of q
-#pragma unroll 1
-    for (int i0 = 0; i0 < ROUNDS; i0 += AHEAD) {
-      const bool is_q = i0 >= ROUNDS / 2;
-      const QrTensor& x = is_q ? a.q : a.k;
-      const int row0 = warp * (LD_C / 4) + (is_q ? i0 - ROUNDS / 2 : i0) * AT_ONCE + lane / LANES;
-      uint4 raw[AHEAD];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int row = row0 + i * AT_ONCE;
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (t0 + row < a.T) raw[i] = *(const uint4*)((const E*)x.p + (t0 + row) * x.token + hk * x.head + l * 8);
-      }
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int row = row0 + i * AT_ONCE;
-        float v[8], most = 0.0f, sum = 0.0f, up, down;
-        qr_unpack<TYPE, 8>(&raw[i].x, v);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) most = fmaxf(most, fmaxf(fabsf(v[e]), fabsf(v[e + 1])));
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        ld_scale(most, up, down);
-        up *= 0x1p-13f, down *= 0x1p13f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] *= up;
-          sum = fmaf(v[e], v[e], sum);
-        }
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        // x / sqrt(|x|^2 + eps) = (up x) / sqrt(|up x|^2 + up^2 eps)
-        float f = a.eps >= 0.0f ? rsqrtf(sum + a.eps * up * up) : down;
-        if (most == 0.0f) f = 0.0f;  // a row of zeros: its factor must not set the scale of what it is summed with
-        uint4 w = make_uint4(ld_half2(v[0], v[1]), ld_half2(v[2], v[3]), ld_half2(v[4], v[5]), ld_half2(v[6], v[7]));
-        if (!(sum <= LD_MAX)) f = __uint_as_float(0x7fc00000u), w = make_uint4(0, 0, 0, 0);
-        *(uint4*)((is_q ? qs : ks) + ld_at<PIECES>(row, l)) = w;
-        if (l == 0) (is_q ? q_factor : k_factor)[row] = is_q ? f * a.scale : f;
-      }
+    if (my_line >= 0) {
+      decay = ld_log_decay<TYPE>(a, t0 + tid, h);
+      if (DELTA) beta = ld_beta<TYPE>(a, t0 + tid, h);
     }
   }
-  if (my_line >= 0) {
-    decay = ld_log_decay<TYPE>(a, t0 + tid, h);
-    if (DELTA) beta = ld_beta<TYPE>(a, t0 + tid, h);
+  __syncthreads();  // the zeros
+  if (!__syncthreads_and(mbar_wait(&arrived, 0))) return;
+  // rows to fp16, each by the power of two that brings its largest value into [1, 2): four lanes a row, in place
+#pragma unroll 1
+  for (int i0 = 0; i0 < 4; ++i0) {
+    const bool is_q = i0 >= 2;
+    const int row = warp * 16 + (i0 & 1) * 8 + g;
+    uint16_t* const at = (is_q ? qs : ks) + row * DK;
+    constexpr int MINE = PIECES / 4;
+    uint4 raw[MINE];
+    float most = 0.0f, sum = 0.0f, up, down;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) raw[i] = *(const uint4*)(at + ((cc + 4 * i + 4 * (row & 1)) & (PIECES - 1)) * 8);
+    float v[MINE][8];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      qr_unpack<TYPE, 8>(&raw[i].x, v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) most = fmaxf(most, fmaxf(fabsf(v[i][e]), fabsf(v[i][e + 1])));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    ld_scale(most, up, down);
+    up *= 0x1p-13f, down *= 0x1p13f;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] *= up;
+        sum = fmaf(v[i][e], v[i][e], sum);
+      }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    // x / sqrt(|x|^2 + eps) = (up x) / sqrt(|up x|^2 + up^2 eps)
+    float f = a.eps >= 0.0f ? rsqrtf(sum + a.eps * up * up) : down;
+    if (most == 0.0f) f = 0.0f;  // a row of zeros: its factor must not set the scale of what it is summed with
+    const bool finite = sum <= LD_MAX;
+    if (!finite) f = __uint_as_float(0x7fc00000u);
+    __syncwarp();  // the row has been read
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      uint4 w = make_uint4(ld_half2(v[i][0], v[i][1]), ld_half2(v[i][2], v[i][3]), ld_half2(v[i][4], v[i][5]), ld_half2(v[i][6], v[i][7]));
+      if (!finite) w = make_uint4(0, 0, 0, 0);
+      *(uint4*)((is_q ? qs : ks) + ld_at<PIECES>(row, (cc + 4 * i + 4 * (row & 1)) & (PIECES - 1))) = w;
+    }
+    if (cc == 0) (is_q ? q_factor : k_factor)[row] = is_q ? f * a.scale : f;
   }
   fence_async_smem();
   __syncthreads();
@@ -361,56 +415,48 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
       for (int i = 0; i < 16; ++i) A[(d + i) * LD_PITCH + d + j] = first_of(d + i) == from ? x[i] : 0.0f;
     }
     __syncthreads();
-    ld_join<16, 64>(A, Y + (tid >> 6) * 16 * LD_PITCH_Y, starts, (tid >> 6) * 32, tid & 63);
-    ld_join<32, 128>(A, Y, starts, 0, tid);
+    ld_join<16, 1>(A, Y + (warp >> 1) * 16 * LD_PITCH_Y, starts, (warp >> 1) * 32, 0, (warp & 1) * 8, lane);
+    ld_join<32, 2>(A, Y, starts, 0, (warp >> 1) * 16, (warp & 1) * 16, lane);
     {  // columns of T become rows of T^T and T^T D: two threads each, four rows by turns
       const int j = tid >> 1, half = tid & 1;
       const float b = beta_s[j];
-      float v[32], m_t = 0.0f, m_d = 0.0f, sum = 0.0f;
+      float v[32], d[32], m_t = 0.0f, m_d = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int i = (e >> 2) * 8 + half * 4 + (e & 3);
-        v[e] = A[i * LD_PITCH + j] * b;
-        sum += fabsf(v[e]);  // finite where all are
-        m_t = fmaxf(m_t, fabsf(v[e]));
-      }
-      if (!(sum <= LD_MAX)) {
-        bad_s[first_of(j)] = 1;
+      for (int e = 0; e < 32; e += 4) {
+        const int i = e * 2 + half * 4;
+        const float4 d4 = *(const float4*)(d_s + i);
+        const float ds[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+        for (int x = 0; x < 4; ++x) {
+          v[e + x] = A[(i + x) * LD_PITCH + j] * b;
+          d[e + x] = v[e + x] != 0.0f ? v[e + x] * ds[x] : 0.0f;  // nothing of another line, where that is not finite
+          sum += fabsf(d[e + x]);                               // finite where all are
+        }
+        m_t = fmaxf(m_t, fmaxf(fmaxf(fabsf(v[e]), fabsf(v[e + 1])), fmaxf(fabsf(v[e + 2]), fabsf(v[e + 3]))));
+        m_d = fmaxf(m_d, fmaxf(fmaxf(fabsf(d[e]), fabsf(d[e + 1])), fmaxf(fabsf(d[e + 2]), fabsf(d[e + 3]))));
       }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       m_t = fmaxf(m_t, __shfl_xor_sync(0xffffffffu, m_t, 1));
-      float up, down;
-      ld_scale(m_t, up, down);
-      if (half == 0) t_scale[j] = down;
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        uint2 hi, lo;
-        ld_split(v[e] * up, v[e + 1] * up, hi.x, lo.x), ld_split(v[e + 2] * up, v[e + 3] * up, hi.y, lo.y);
-        const int at = ld_at<8>(j, e >> 2) + half * 4;
-        *(uint2*)(tt + at) = hi, *(uint2*)(tt + LD_C * LD_C + at) = lo;
-      }
-      sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const int i = (e >> 2) * 8 + half * 4 + (e & 3);
-        v[e] = v[e] != 0.0f ? v[e] * d_s[i] : 0.0f;  // nothing of another line, where that is not finite
-        sum += fabsf(v[e]);
-        m_d = fmaxf(m_d, fabsf(v[e]));
-      }
-      if (!(sum <= LD_MAX)) {
-        bad_s[first_of(j)] = 1;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
-      }
       m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
-      ld_scale(m_d, up, down);
+      if (!(sum <= LD_MAX && m_t <= LD_MAX)) {
+        bad_s[first_of(j)] = 1;
+        m_t = m_d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = d[e] = 0.0f;
+      }
+      float up_t, up_d, down;
+      ld_scale(m_t, up_t, down);
+      if (half == 0) t_scale[j] = down;
+      ld_scale(m_d, up_d, down);
       if (half == 0) kt_scale[j] = m_d > 0.0f ? down * 0x1p6f : 0.0f;  // a row of zeros must not set a scale
+      __syncthreads();                                                  // T has been read
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         uint2 hi, lo;
-        ld_split(v[e] * up, v[e + 1] * up, hi.x, lo.x), ld_split(v[e + 2] * up, v[e + 3] * up, hi.y, lo.y);
         const int at = ld_at<8>(j, e >> 2) + half * 4;
+        ld_split(v[e] * up_t, v[e + 1] * up_t, hi.x, lo.x), ld_split(v[e + 2] * up_t, v[e + 3] * up_t, hi.y, lo.y);
+        *(uint2*)(tt + at) = hi, *(uint2*)(tt + LD_C * LD_C + at) = lo;
+        ld_split(d[e] * up_d, d[e + 1] * up_d, hi.x, lo.x), ld_split(d[e + 2] * up_d, d[e + 3] * up_d, hi.y, lo.y);
         *(uint2*)(td + at) = hi, *(uint2*)(td + LD_C * LD_C + at) = lo;
       }
     }
@@ -480,7 +526,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
       *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(p[n][r * 2] * up, p[n][r * 2 + 1] * up);
   }
   uint16_t* const kt_hi = (uint16_t*)A;
-  uint16_t* const kt_lo = td;
+  uint16_t* const kt_lo = qs;
   if constexpr (DELTA) {
     // K~ = T^T D K: a warp has Dk / 4 columns
     constexpr int N = DK / 32;
@@ -506,7 +552,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 3) lines_delta_prep_kernel(Ld
         for (int n = 0; n < N; ++n) ld_mma(kt[j][n], hi, b[n][0], b[n][1]);
       }
     }
-    __syncthreads();  // T^T D has been read
+    __syncthreads();  // T^T D and T^T have been read
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
