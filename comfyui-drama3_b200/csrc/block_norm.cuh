@@ -17,8 +17,6 @@ namespace d3 {
 constexpr int BN_WARPS = 4;        // a block of the gated rows
 constexpr int BN_MAX_THREADS = 1024;
 
-D3_DEV float bn_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
-
 struct GnArgs {
   QrTensor x, gate;  // rows [T, H, D]
   int T, H, D;
@@ -35,17 +33,16 @@ __global__ void __launch_bounds__(BN_WARPS * 32) gated_norm_kernel(GnArgs a) {
   using E = typename QrType<TYPE>::T;
   constexpr int VEC = 16 / (int)sizeof(E), GROUPS = 32 / LANES;
   const int lane = threadIdx.x & 31, l = lane % LANES, vectors = a.D / VEC;
-  const long long rows = (long long)a.T * a.H;
-  const long long row0 = ((long long)blockIdx.x * BN_WARPS + (threadIdx.x >> 5)) * (GROUPS * AHEAD) + lane / LANES;
+  const unsigned rows = (unsigned)a.T * (unsigned)a.H;  // at most 2^31
+  const unsigned row0 = (blockIdx.x * BN_WARPS + (threadIdx.x >> 5)) * (GROUPS * AHEAD) + lane / LANES;
   grid_dependency_wait();
   allow_dependents();
   uint4 x[AHEAD][NV] = {}, z[AHEAD][NV] = {};
 #pragma unroll
   for (int r = 0; r < AHEAD; ++r) {
-    const long long row = row0 + r * GROUPS;
+    const unsigned row = row0 + r * GROUPS;
     if (row < rows) {
-      const long long t = row / a.H;
-      const int h = (int)(row - t * a.H);
+      const unsigned t = row / (unsigned)a.H, h = row - t * (unsigned)a.H;
       const E* xr = (const E*)a.x.p + t * a.x.token + h * a.x.head;
       const E* zr = (const E*)a.gate.p + t * a.gate.token + h * a.gate.head;
 #pragma unroll
@@ -62,7 +59,7 @@ __global__ void __launch_bounds__(BN_WARPS * 32) gated_norm_kernel(GnArgs a) {
     if (l + i * LANES < vectors) qr_weights<TYPE, VEC>(a.w, a.w_f32, a.w_add, (l + i * LANES) * VEC, w[i]);
 #pragma unroll
   for (int r = 0; r < AHEAD; ++r) {
-    const long long row = row0 + r * GROUPS;
+    const unsigned row = row0 + r * GROUPS;
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -83,12 +80,12 @@ __global__ void __launch_bounds__(BN_WARPS * 32) gated_norm_kernel(GnArgs a) {
         qr_unpack<TYPE, VEC>(&z[r][i].x, g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float s = bn_sigmoid(g[e]);
+          const float s = row_sigmoid<TYPE>(g[e]);
           v[e] = v[e] * scale * w[i][e] * (a.act ? s : g[e] * s);
         }
         uint4 out;
         qr_pack<TYPE, VEC>(v, &out.x);
-        *(uint4*)((E*)a.out + row * a.D + (l + i * LANES) * VEC) = out;
+        *(uint4*)((E*)a.out + (size_t)row * a.D + (l + i * LANES) * VEC) = out;
       }
   }
 }
@@ -114,7 +111,7 @@ __global__ void __launch_bounds__(BN_WARPS * 32) gated_norm_any_kernel(GnArgs a)
   }
   const float scale = rsqrtf(warp_sum(sum) / a.D + a.eps);
   for (int d = lane; d < a.D; d += 32) {
-    const float g = TT::get(zr[d]), s = bn_sigmoid(g);
+    const float g = TT::get(zr[d]), s = row_sigmoid<TYPE>(g);
     ((E*)a.out)[row * a.D + d] =
         TT::put(TT::get(xr[d]) * scale * qr_weight<TYPE>(a.w, a.w_f32, a.w_add, d) * (a.act ? s : g * s));
   }
@@ -149,86 +146,99 @@ D3_DEV float bn_block_sum(float v, float* part) {
   return warp_sum(v);
 }
 
-template <int TYPE, int NV>
-__global__ void __launch_bounds__(BN_MAX_THREADS) add_norm_kernel(AnArgs a) {
+// What a thread does with its vectors of one row: NV of them, `step` apart from the first one on. SUM(v) adds v up over the row's threads.
+template <int TYPE, int NV, class SUM>
+D3_DEV void an_row(const AnArgs& a, long long t, int first, int step, SUM&& row_sum) {
   using TT = QrType<TYPE>;
   using E = typename TT::T;
   constexpr int VEC = 16 / (int)sizeof(E);
-  __shared__ float part[4][32];
   const int vectors = a.W / VEC;
+  uint4 x[NV] = {}, r[NV] = {};
+  float row_gate = 1.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = first + i * step;
+    if (v < vectors) {
+      x[i] = *(const uint4*)((const E*)a.x + t * a.x_token + v * VEC);
+      r[i] = *(const uint4*)((const E*)a.residual + t * a.r_token + v * VEC);
+    }
+  }
+  if (a.gate_kind == AN_ROW) row_gate = TT::get(((const E*)a.gate)[t * a.gate_token]);
+  float factor = a.scale * row_gate;
+  if (a.post) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float v[VEC];
+      qr_unpack<TYPE, VEC>(&x[i].x, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum = fmaf(v[e], v[e], sum);
+    }
+    factor *= rsqrtf(row_sum(sum) / a.W + a.eps);
+  }
+  float sum = 0.0f;
+  float total[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = first + i * step;
+    if (v < vectors) {
+      float b[VEC], m[VEC];
+      qr_unpack<TYPE, VEC>(&x[i].x, b);
+      qr_unpack<TYPE, VEC>(&r[i].x, total[i]);
+      if (a.post) {
+        qr_weights<TYPE, VEC>(a.post, a.w_f32, a.w_add, v * VEC, m);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) b[e] *= m[e];
+      }
+      if (a.gate_kind == AN_EACH) {
+        const uint4 g = *(const uint4*)((const E*)a.gate + t * a.gate_token + v * VEC);
+        qr_unpack<TYPE, VEC>(&g.x, m);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) b[e] *= m[e];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        total[i][e] = fmaf(factor, b[e], total[i][e]);
+        sum = fmaf(total[i][e], total[i][e], sum);
+      }
+      uint4 out;
+      qr_pack<TYPE, VEC>(total[i], &out.x);
+      *(uint4*)((E*)a.sum_out + t * a.W + v * VEC) = out;
+    }
+  }
+  const float scale = rsqrtf(row_sum(sum) / a.W + a.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = first + i * step;
+    if (v < vectors) {
+      float w[VEC];
+      qr_weights<TYPE, VEC>(a.w, a.w_f32, a.w_add, v * VEC, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] *= total[i][e] * scale;
+      uint4 out;
+      qr_pack<TYPE, VEC>(w, &out.x);
+      *(uint4*)((E*)a.norm_out + t * a.W + v * VEC) = out;
+    }
+  }
+}
+
+// A block a row.
+template <int TYPE, int NV>
+__global__ void __launch_bounds__(BN_MAX_THREADS) add_norm_kernel(AnArgs a) {
+  __shared__ float part[2][32];
   int which = 0;
   grid_dependency_wait();
   allow_dependents();
-  for (long long t = blockIdx.x; t < a.T; t += gridDim.x) {
-    uint4 x[NV] = {}, r[NV] = {}, g[NV] = {};
-    float row_gate = 1.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < vectors) {
-        x[i] = *(const uint4*)((const E*)a.x + t * a.x_token + v * VEC);
-        r[i] = *(const uint4*)((const E*)a.residual + t * a.r_token + v * VEC);
-        if (a.gate_kind == AN_EACH) g[i] = *(const uint4*)((const E*)a.gate + t * a.gate_token + v * VEC);
-      }
-    }
-    if (a.gate_kind == AN_ROW) row_gate = TT::get(((const E*)a.gate)[t * a.gate_token]);
-    float factor = a.scale * row_gate;
-    if (a.post) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float v[VEC];
-        qr_unpack<TYPE, VEC>(&x[i].x, v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum = fmaf(v[e], v[e], sum);
-      }
-      factor *= rsqrtf(bn_block_sum(sum, part[which]) / a.W + a.eps);
-      which = (which + 1) & 3;
-    }
-    float total[NV][VEC], sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < vectors) {
-        float b[VEC], m[VEC];
-        qr_unpack<TYPE, VEC>(&x[i].x, b);
-        qr_unpack<TYPE, VEC>(&r[i].x, total[i]);
-        if (a.post) {
-          qr_weights<TYPE, VEC>(a.post, a.w_f32, a.w_add, v * VEC, m);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) b[e] *= m[e];
-        }
-        if (a.gate_kind == AN_EACH) {
-          qr_unpack<TYPE, VEC>(&g[i].x, m);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) b[e] *= m[e];
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          total[i][e] = fmaf(factor, b[e], total[i][e]);
-          sum = fmaf(total[i][e], total[i][e], sum);
-        }
-        uint4 out;
-        qr_pack<TYPE, VEC>(total[i], &out.x);
-        *(uint4*)((E*)a.sum_out + t * a.W + v * VEC) = out;
-      }
-    }
-    const float scale = rsqrtf(bn_block_sum(sum, part[which]) / a.W + a.eps);
-    which = (which + 1) & 3;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
-      if (v < vectors) {
-        float w[VEC];
-        qr_weights<TYPE, VEC>(a.w, a.w_f32, a.w_add, v * VEC, w);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) w[e] *= total[i][e] * scale;
-        uint4 out;
-        qr_pack<TYPE, VEC>(w, &out.x);
-        *(uint4*)((E*)a.norm_out + t * a.W + v * VEC) = out;
-      }
-    }
-  }
+  an_row<TYPE, NV>(a, blockIdx.x, threadIdx.x, blockDim.x, [&](float v) { return bn_block_sum(v, part[which++]); });
+}
+
+// A warp a row: no step of the block, and a row's loads are all in flight together.
+template <int TYPE, int NV>
+__global__ void __launch_bounds__(BN_WARPS * 32) add_norm_warp_kernel(AnArgs a) {
+  const long long t = (long long)blockIdx.x * BN_WARPS + (threadIdx.x >> 5);
+  grid_dependency_wait();
+  allow_dependents();
+  if (t < a.T) an_row<TYPE, NV>(a, t, threadIdx.x & 31, 32, [](float v) { return warp_sum(v); });
 }
 
 // Rows of any size and alignment: a block each; x and the residual are read again for each sum, from the caches.

@@ -55,6 +55,13 @@ int join_type(const d3::AnArgs& a, bool vectors, const DeviceInfo& d, cudaStream
   const int n = a.W / VEC;
   if (!vectors || a.W % VEC || n > 2 * d3::BN_MAX_THREADS)
     return launch(d3::add_norm_any_kernel<TYPE>, dim3(a.T), dim3(256), 0, s, true, a);
+  // a warp a row where that leaves every SM 16 warps
+  if (n <= 256 && a.T >= 16 * d.sms) {
+    const dim3 blocks((a.T + d3::BN_WARPS - 1) / d3::BN_WARPS), threads(d3::BN_WARPS * 32);
+    if (n <= 64) return launch(d3::add_norm_warp_kernel<TYPE, 2>, blocks, threads, 0, s, true, a);
+    if (n <= 128) return launch(d3::add_norm_warp_kernel<TYPE, 4>, blocks, threads, 0, s, true, a);
+    return launch(d3::add_norm_warp_kernel<TYPE, 8>, blocks, threads, 0, s, true, a);
+  }
   const int nv = n <= d3::BN_MAX_THREADS ? 1 : 2;
   const int threads = ((n + nv - 1) / nv + 31) / 32 * 32;
   const dim3 blocks(a.T);

@@ -16,7 +16,7 @@ namespace d3 {
 
 constexpr int LC_THREADS = 128;
 constexpr int LC_TILE = 32;  // tokens
-constexpr int LC_AHEAD = 4;  // of them loaded together
+constexpr int LC_AHEAD = 8;  // of them loaded together
 constexpr int LC_MAX_TAPS = 8;
 
 struct LcArgs {
@@ -33,13 +33,6 @@ struct LcArgs {
   void* out;  // [T, C]
   int tiles;  // blocks of tokens; the lines' blocks come behind them
 };
-
-// y * sigmoid(y). Rows of 16 bits take the fast exponential and reciprocal: off by about (2 + |y|) 2^-23 of the result, and
-// half a step of bf16 and fp16 is 2^-9 and 2^-12.
-template <int TYPE> D3_DEV float lc_silu(float y) {
-  if constexpr (TYPE == QR_F32) return y / (1.0f + expf(-y));
-  return __fdividef(y, 1.0f + __expf(-y));
-}
 
 // What a tile does with token t: compute it (2), zeros (1, no line's token), or nothing (0, one of a line's first W - 1).
 D3_DEV int lc_role(const LcArgs& a, long long t) {
@@ -77,7 +70,7 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_kernel(LcArgs a) {
   auto finish = [&](const float (&y)[VEC], long long t) {
     float v[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = a.silu ? lc_silu<TYPE>(y[e]) : y[e];
+    for (int e = 0; e < VEC; ++e) v[e] = a.silu ? y[e] * row_sigmoid<TYPE>(y[e]) : y[e];
     uint4 q;
     qr_pack<TYPE, VEC>(v, &q.x);
     *(uint4*)(out + t * a.C) = q;
@@ -128,6 +121,7 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_kernel(LcArgs a) {
   }
   const long long t0 = (long long)blockIdx.x * LC_TILE;
   if (threadIdx.x < LC_TILE) roles[threadIdx.x] = lc_role(a, t0 + threadIdx.x);
+  const bool plain = __syncthreads_and(threadIdx.x >= LC_TILE || roles[threadIdx.x] == 2);  // nearly always, of a long text
   if (!__syncthreads_or(threadIdx.x < LC_TILE && roles[threadIdx.x]) || !there) return;
   weights();
   float in[W][VEC];  // in[(i + j) % W]: the input j of token i
@@ -156,7 +150,7 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_kernel(LcArgs a) {
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) in[j][e] = in[j + 1][e];
       }
-      const int role = roles[i0 + i];
+      const int role = plain ? 2 : roles[i0 + i];
       if (role == 2) finish(y, t0 + i0 + i);
       if (role == 1) *(uint4*)(out + (t0 + i0 + i) * a.C) = make_uint4(0, 0, 0, 0);
     }
@@ -197,7 +191,7 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_any_kernel(LcArgs a) {
         if (k == W - 1 - j) tap = w[k];
       if (j < W) y = fmaf(tap, in[j], y);
     }
-    out[t * a.C] = TT::put(a.silu ? lc_silu<TYPE>(y) : y);
+    out[t * a.C] = TT::put(a.silu ? y * row_sigmoid<TYPE>(y) : y);
   };
   if ((int)blockIdx.x >= a.tiles) {
     long long s, n;

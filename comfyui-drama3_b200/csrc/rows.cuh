@@ -101,4 +101,14 @@ D3_DEV void qr_weights(const void* w, bool f32, float add, int d, float* out) {
   for (int e = 0; e < VEC; ++e) out[e] += add;
 }
 
+// 1 / (1 + e^-z). Rows of 16 bits take the fast exponential and reciprocal: off by about (2 + |z|) 2^-22 of the value, and half a step of
+// bf16 and fp16 is 2^-8 and 2^-11.
+template <int TYPE> D3_DEV float row_sigmoid(float z) {
+  if constexpr (TYPE == QR_F32) return 1.0f / (1.0f + expf(-z));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+
 }  // namespace d3
