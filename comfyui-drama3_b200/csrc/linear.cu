@@ -220,7 +220,8 @@ int d3_lines_conv(const void* x, int64_t x_token, int type, int T, int C, const 
   d3::LcArgs a = {x, x_token, T, C, W, B, weight, bias, w_f32, state, cu, line, silu, out, 0};
   a.tiles = (T + d3::LC_TILE - 1) / d3::LC_TILE;
   const int vec = 16 / size;
-  const bool vectors = C % vec == 0 && x_token % vec == 0 && aligned(x, 16) && aligned(state, 16) && aligned(out, 16);
+  const bool vectors = C % vec == 0 && x_token % vec == 0 && aligned(x, 16) && aligned(state, 16) && aligned(out, 16) &&
+                       aligned(weight, 16);
   cudaStream_t s = (cudaStream_t)stream;
   switch (type) {
     case d3::QR_BF16: return conv_type<d3::QR_BF16>(a, vectors, s);

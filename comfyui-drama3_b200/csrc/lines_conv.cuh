@@ -10,13 +10,14 @@
 // another block writes: a decode step has only such blocks' work.
 #pragma once
 
+#include "f32x2.cuh"
 #include "rows.cuh"
 
 namespace d3 {
 
 constexpr int LC_THREADS = 128;
-constexpr int LC_TILE = 32;  // tokens
-constexpr int LC_AHEAD = 8;  // of them loaded together
+constexpr int LC_TILE = 64;  // tokens
+constexpr int LC_AHEAD = 4;  // of them loaded together, while as many before them are summed
 constexpr int LC_MAX_TAPS = 8;
 
 struct LcArgs {
@@ -59,11 +60,14 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_kernel(LcArgs a) {
   const E* x = (const E*)a.x + c;
   E* out = (E*)a.out + c;
   float w[W][VEC], bias[VEC];
-  auto weights = [&] {
+  auto weights = [&] {  // the filters of neighbouring channels lie next to one another
+    float all[W * VEC];
+#pragma unroll
+    for (int i = 0; i < W; ++i) qr_weights<TYPE, VEC>(a.w, a.w_f32, 0.0f, c * W + i * VEC, all + i * VEC);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[j][e] = qr_weight<TYPE>(a.w, a.w_f32, 0.0f, (c + e) * W + j);
+      for (int j = 0; j < W; ++j) w[j][e] = all[e * W + j];
       bias[e] = a.bias ? qr_weight<TYPE>(a.bias, a.w_f32, 0.0f, c + e) : 0.0f;
     }
   };
@@ -132,23 +136,33 @@ __global__ void __launch_bounds__(LC_THREADS) lines_conv_kernel(LcArgs a) {
     if (t >= 0) q = row(t);
     qr_unpack<TYPE, VEC>(&q.x, in[j]);
   }
+  uint4 next[LC_AHEAD];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < LC_AHEAD; ++i) {
+      next[i] = make_uint4(0, 0, 0, 0);
+      if (i0 + i < LC_TILE && t0 + i0 + i < a.T) next[i] = row(t0 + i0 + i);
+    }
+  };
+  fetch(0);
 #pragma unroll 1
   for (int i0 = 0; i0 < LC_TILE; i0 += LC_AHEAD) {
-    uint4 q[LC_AHEAD] = {};
+    uint4 q[LC_AHEAD];
 #pragma unroll
-    for (int i = 0; i < LC_AHEAD; ++i)
-      if (t0 + i0 + i < a.T) q[i] = row(t0 + i0 + i);
+    for (int i = 0; i < LC_AHEAD; ++i) q[i] = next[i];
+    fetch(i0 + LC_AHEAD);
 #pragma unroll
     for (int i = 0; i < LC_AHEAD; ++i) {
       float y[VEC];
       qr_unpack<TYPE, VEC>(&q[i].x, in[W - 1]);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        y[e] = bias[e];
+      for (int e = 0; e < VEC; e += 2) {
+        uint64_t two = f2_make(bias[e], bias[e + 1]);
 #pragma unroll
-        for (int j = 0; j < W; ++j) y[e] = fmaf(w[j][e], in[j][e], y[e]);
+        for (int j = 0; j < W; ++j) two = f2_fma(f2_make(w[j][e], w[j][e + 1]), f2_make(in[j][e], in[j][e + 1]), two);
+        f2_split(two, y[e], y[e + 1]);
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) in[j][e] = in[j + 1][e];
+        for (int j = 0; j < W - 1; ++j) in[j][e] = in[j + 1][e], in[j][e + 1] = in[j + 1][e + 1];
       }
       const int role = plain ? 2 : roles[i0 + i];
       if (role == 2) finish(y, t0 + i0 + i);
