@@ -627,7 +627,9 @@ template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int S = DK * 32 + 128, R = 2 * S, SCALES = R + LD_C * 32, OUT = SCALES + 128, SHARES = OUT + LD_C * 32;
   static constexpr int TEAM = SHARES + (PARTS > 1 ? 2 * PARTS * LD_C * 64 : 0);
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
-  static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024, THREADS = WARPS * (PARTS + 1) * 32;
+  static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024;
+  static constexpr int OUTS = PARTS;  // warps for the outputs, each of a share of the tokens: as many on every quarter of an SM
+  static constexpr int THREADS = WARPS * (PARTS + OUTS) * 32;
   static_assert(STAGES >= 2, "a chunk is loaded while the one before it is worked on");
 };
 
@@ -655,6 +657,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   using Shape = LdScanShape<DK, WARPS, PARTS>;
   constexpr int PIECES = DK / 8, NK = DK / 8 / PARTS, KT = DK / 16 / PARTS, NT = LD_C / 8, STAGES = Shape::STAGES;
   constexpr int G = NK < 8 ? NK : 8;  // sums of S that take turns
+  constexpr int OUTS = Shape::OUTS, NO = NT / OUTS;
   extern __shared__ uint8_t ld_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], r_full[WARPS],
       r_empty[WARPS], shares[WARPS][PARTS][2];  // [2]: odd and even chunks', as their places
@@ -662,13 +665,13 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
   const bool outputs = warp >= WARPS * PARTS;
-  const int team = outputs ? warp - WARPS * PARTS : warp / PARTS, part = outputs ? 0 : warp % PARTS;
+  const int team = (outputs ? warp - WARPS * PARTS : warp) / PARTS, part = warp % PARTS;  // OUTS is PARTS
   uint8_t* const ring = (uint8_t*)(((uintptr_t)ld_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* const place = ring + STAGES * Shape::STAGE + team * Shape::TEAM;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + 1) * WARPS);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + OUTS) * WARPS);
     for (int i = 0; i < WARPS; ++i) {
-      mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], 1);
+      mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], OUTS);
       for (int y = 0; y < 2; ++y) {
         mbar_init(&s_full[i][y], PARTS);
         for (int j = 0; j < PARTS; ++j) mbar_init(&shares[i][j][y], 1);
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   const bool there = row0 < a.Dv;
   if (b == a.B) {  // the places past the lines' last token
     const long long from = max((long long)min(max(a.cu[b], 0), a.T), first_token);
-    if (outputs && there)
+    if (outputs && part == 0 && there)
       for (long long t = from + (lane >> 1); t < end_token; t += 16)
         *(uint4*)((uint16_t*)a.out + (t * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8) = make_uint4(0, 0, 0, 0);
     return;
@@ -710,14 +713,14 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
                     (int)(first_token + (long long)block * LD_C), bar);
       ++loads;
     };
-    if (team == 0 && lane == 0)
+    if (warp == WARPS * PARTS && lane == 0)
       for (int i = 0; i < STAGES && i < chunks; ++i) load();
 #pragma unroll 1
     for (int i = 0; i < chunks && ok; ++i) {
       const int st = i % STAGES;
       ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team][i & 1], (i >> 1) & 1);
       if (!ok) break;
-      if (team == 0 && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
+      if (warp == WARPS * PARTS && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
         ok = mbar_wait(&empty[(i - 1) % STAGES], ((i - 1) / STAGES) & 1);
         if (ok) load();
       }
@@ -726,24 +729,24 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
       const long long t0 = first_token + (long long)(block_a + i) * LD_C;
       const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
-      float O[PARTS][NT][4] = {};
+      float O[PARTS][NO][4] = {};
 #pragma unroll
       for (int kt = 0; kt < DK / 16; ++kt) {
         const uint4 s4 = *(const uint4*)(place + (i & 1) * Shape::S + (kt * 32 + lane) * 16);
         const uint32_t a4[4] = {s4.x, s4.y, s4.z, s4.w};
-        uint32_t q4[4][4];
+        uint32_t q4[NO / 2][4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          ld_matrix4(q4[x], rows.q + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+        for (int x = 0; x < NO / 2; ++x)
+          ld_matrix4(q4[x], rows.q + ld_at<PIECES>((part * NO + x * 2) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-        for (int x = 0; x < NT; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
+        for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
       const float* const s_scales = (const float*)(place + (i & 1) * Shape::S + DK * 32);
 #pragma unroll
       for (int y = 0; y < PARTS; ++y) {
         const float s_down[2] = {s_scales[y * 16 + g], s_scales[y * 16 + g + 8]};
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NO; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             if (y == 0) O[0][n][x] *= s_down[x >> 1];
@@ -763,22 +766,24 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       ld_arrive(&r_empty[team], lane);
       uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
+      for (int m = 0; m < NO; m += 2) {
+        const int n = part * NO + m;
         float pu[2][4] = {};
 #pragma unroll
-        for (int kt = 0; kt <= n / 2; ++kt) {
-          uint32_t p4[4];
-          ld_matrix4(p4, head.p + ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-          ld_mma(pu[0], u4[kt], p4[0], p4[1]), ld_mma(pu[1], u4[kt], p4[2], p4[3]);
-        }
+        for (int kt = 0; kt < LD_C / 16; ++kt)
+          if (kt <= n / 2) {
+            uint32_t p4[4];
+            ld_matrix4(p4, head.p + ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+            ld_mma(pu[0], u4[kt], p4[0], p4[1]), ld_mma(pu[1], u4[kt], p4[2], p4[3]);
+          }
         uint32_t o4[4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int j = (n + x) * 8 + cc * 2;
           const float2 fq = *(const float2*)(head.q_in + j), fp = *(const float2*)(head.p_scale + j);
           float o[4];
-          o[0] = fmaf(O[0][n + x][0], fq.x, pu[x][0] * r_down[0] * fp.x), o[1] = fmaf(O[0][n + x][1], fq.y, pu[x][1] * r_down[0] * fp.y);
-          o[2] = fmaf(O[0][n + x][2], fq.x, pu[x][2] * r_down[1] * fp.x), o[3] = fmaf(O[0][n + x][3], fq.y, pu[x][3] * r_down[1] * fp.y);
+          o[0] = fmaf(O[0][m + x][0], fq.x, pu[x][0] * r_down[0] * fp.x), o[1] = fmaf(O[0][m + x][1], fq.y, pu[x][1] * r_down[0] * fp.y);
+          o[2] = fmaf(O[0][m + x][2], fq.x, pu[x][2] * r_down[1] * fp.x), o[3] = fmaf(O[0][m + x][3], fq.y, pu[x][3] * r_down[1] * fp.y);
           o4[2 * x] = TT::put2(o[0], o[1]), o4[2 * x + 1] = TT::put2(o[2], o[3]);
         }
         const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
@@ -787,16 +792,16 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       ld_arrive(&empty[st], lane);
       if (there)
 #pragma unroll
-        for (int x = 0; x < LD_C / 16; ++x) {
-          const int token = x * 16 + (lane >> 1), piece = (lane & 1) ^ ((token >> 2) & 1);
+        for (int x = 0; x < LD_C / 16 / OUTS; ++x) {
+          const int token = part * NO * 8 + x * 16 + (lane >> 1), piece = (lane & 1) ^ ((token >> 2) & 1);
           if (token >= lo && token < hi)
             *(uint4*)((uint16_t*)a.out + ((t0 + token) * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8) =
                 *(const uint4*)(out_s + token * 32 + piece * 16);
         }
-      __syncwarp();  // the outputs have been read
+      __syncwarp();  // its outputs have been read
     }
     // copies in flight land before the block ends (where a wait ran out: those of the other chunks have been waited for)
-    if (team == 0 && lane == 0 && !ok)
+    if (warp == WARPS * PARTS && lane == 0 && !ok)
       for (int i = loads - 1; i >= 0 && i >= loads - STAGES; --i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1);
     return;
   }
@@ -811,26 +816,26 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const float2 x = *(const float2*)(state + g * DK + n * 8 + cc * 2), y = *(const float2*)(state + (g + 8) * DK + n * 8 + cc * 2);
       S[n][0] = x.x, S[n][1] = x.y, S[n][2] = y.x, S[n][3] = y.y;
     }
+  ok = ld_wait(&full[0], 0);
 #pragma unroll 1
-  for (int i = 0; i < chunks; ++i) {
-    const int st = i % STAGES;
+  for (int i = 0; i < chunks && ok; ++i) {
+    const int st = i % STAGES, odd = i & 1;
     const uint8_t* const stage = ring + st * Shape::STAGE;
     const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
     const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
     const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
+    uint8_t* const s_place = place + odd * Shape::S;
     const long long t0 = first_token + (long long)(block_a + i) * LD_C;
     const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
     const bool partial = lo > 0 || hi < LD_C;
-    ok = ld_wait(&full[st], (i / STAGES) & 1);
-    if (!ok) break;
     // operands are asked for before what they are multiplied by is known
-    uint32_t k4[4][4];
-    auto get_k = [&](int kt) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        ld_matrix4(k4[x], rows.k + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, (part * KT + kt) * 2 + ((lane >> 3) & 1)));
+    uint32_t k4[2][4][4];
+    auto get_k = [&](int kt, int x) {
+      ld_matrix4(k4[kt & 1][x], rows.k + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, (part * KT + kt) * 2 + ((lane >> 3) & 1)));
     };
-    if (DELTA) get_k(0);
+    if (DELTA)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) get_k(0, x);
     // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already: votes tell, without the largest itself
     bool fresh = false;  // a row of zeros, which has no size
     {
@@ -857,48 +862,89 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         fresh = __any_sync(0xffffffffu, fresh);
       }
     }
-    // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs
+    // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs. Conversions and loads of the
+    // next step stand between the products of this one: a warp's instructions issue in order, and a product holds its pipe for 8 clocks.
     float R[NT][4] = {}, low[NT][4] = {};
+    uint32_t hi4[2][4], lo4[2][4];
+    auto s_terms = [&](int kt, int x) {
+      ld_split(S[2 * kt + (x >> 1)][(x & 1) * 2], S[2 * kt + (x >> 1)][(x & 1) * 2 + 1], hi4[kt & 1][x], lo4[kt & 1][x]);
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) s_terms(0, x);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      uint32_t hi4[4], lo4[4];
-      ld_split(S[2 * kt][0], S[2 * kt][1], hi4[0], lo4[0]);
-      ld_split(S[2 * kt][2], S[2 * kt][3], hi4[1], lo4[1]);
-      ld_split(S[2 * kt + 1][0], S[2 * kt + 1][1], hi4[2], lo4[2]);
-      ld_split(S[2 * kt + 1][2], S[2 * kt + 1][3], hi4[3], lo4[3]);
-      *(uint4*)(place + (i & 1) * Shape::S + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-      if (DELTA) {
-        if (kt > 0) get_k(kt);
+      const auto& k = k4[kt & 1];
+      *(uint4*)(s_place + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[kt & 1][0], hi4[kt & 1][1], hi4[kt & 1][2], hi4[kt & 1][3]);
 #pragma unroll
-        for (int x = 0; x < NT; ++x) ld_mma(R[x], hi4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
-#pragma unroll
-        for (int x = 0; x < NT; ++x) ld_mma(low[x], lo4, k4[x / 2][x % 2 * 2], k4[x / 2][x % 2 * 2 + 1]);
+      for (int x = 0; x < 2 * NT; ++x) {
+        const int n = x % NT;
+        if (DELTA) {
+          if (x < NT)
+            ld_mma(R[n], hi4[kt & 1], k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
+          else
+            ld_mma(low[n], lo4[kt & 1], k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
+        }
+        if (kt + 1 < KT) {
+          if (x % 4 == 1) s_terms(kt + 1, x / 4);
+          if (DELTA && x % 4 == 3) get_k(kt + 1, x / 4);
+        }
       }
     }
     if (cc == 0) {
-      float* const s_scales = (float*)(place + (i & 1) * Shape::S + DK * 32) + part * 16;
+      float* const s_scales = (float*)(s_place + DK * 32) + part * 16;
       s_scales[g] = down[0], s_scales[g + 8] = down[1];
     }
-    ld_arrive(&s_full[team][i & 1], lane);
-    uint32_t v4[NT / 2][4];
+    ld_arrive(&s_full[team][odd], lane);
+    // R = V - gamma K S^T, zeros for the tokens of other lines
+    float2 f[NT];
+    {
+      uint32_t v4[NT / 2][4];
 #pragma unroll
-    for (int n = 0; n < NT; n += 2) {
-      const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
-      ld_matrix4_trans(v4[n / 2], v_s + token * 32 + piece * 16);
+      for (int n = 0; n < NT; n += 2) {
+        const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
+        ld_matrix4_trans(v4[n / 2], v_s + token * 32 + piece * 16);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int j = n * 8 + cc * 2;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        f[n] = *(const float2*)(head.kt_scale + j);
+        if (part == 0) {  // v is the first part's to add
+          TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
+          TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
+        }
+        if (DELTA) {
+          const float2 in = *(const float2*)(head.r_in + j);
+          const float i0 = -in.x * down[0], i1 = -in.y * down[0], i2 = -in.x * down[1], i3 = -in.y * down[1];
+          v[0] = fmaf(R[n][0] + low[n][0], i0, v[0]), v[1] = fmaf(R[n][1] + low[n][1], i1, v[1]);
+          v[2] = fmaf(R[n][2] + low[n][2], i2, v[2]), v[3] = fmaf(R[n][3] + low[n][3], i3, v[3]);
+        } else if (part > 0) {
+          TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
+          TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
+        }
+        if (partial) {
+          if (j < lo || j >= hi) v[0] = v[2] = f[n].x = 0.0f;
+          if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f[n].y = 0.0f;
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) R[n][y] = v[y];
+      }
     }
-    if (DELTA) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) R[n][x] = (R[n][x] + low[n][x]) * down[x >> 1];
-    }
-    if constexpr (DELTA && PARTS > 1) {  // the parts' shares, each the sum of both in the same order
-      float4* const mine = (float4*)(place + Shape::SHARES + ((i & 1) * PARTS + part) * LD_C * 64) + lane;
-      const float4* const theirs = (const float4*)(place + Shape::SHARES + ((i & 1) * PARTS + 1 - part) * LD_C * 64) + lane;
+    uint32_t b_hi[2][G / 2][4], b_lo[2][G / 2][4];
+    auto get_b = [&](int at, int x) {  // of the G columns and 16 tokens of step `at`
+      const int where = ld_at<PIECES>(at / (NK / G) * 16 + (lane & 15), part * NK + at % (NK / G) * G + x / 2 * 2 + (lane >> 4));
+      if (x % 2) ld_matrix4_trans(b_hi[at & 1][x / 2], head.kt_hi + where);
+      else ld_matrix4_trans(b_lo[at & 1][x / 2], head.kt_lo + where);
+    };
+    if constexpr (DELTA && PARTS > 1) {  // the parts' shares: each has the sum of both
+      float4* const mine = (float4*)(place + Shape::SHARES + (odd * PARTS + part) * LD_C * 64) + lane;
+      const float4* const theirs = (const float4*)(place + Shape::SHARES + (odd * PARTS + 1 - part) * LD_C * 64) + lane;
 #pragma unroll
       for (int n = 0; n < NT; ++n) mine[n * 32] = make_float4(R[n][0], R[n][1], R[n][2], R[n][3]);
-      ld_arrive(&shares[team][part][i & 1], lane);
-      ok = mbar_wait(&shares[team][1 - part][i & 1], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
+      ld_arrive(&shares[team][part][odd], lane);
+#pragma unroll
+      for (int x = 0; x < G; ++x) get_b(0, x);
+      ok = mbar_wait(&shares[team][1 - part][odd], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
 #pragma unroll
@@ -907,44 +953,16 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         R[n][0] += y.x, R[n][1] += y.y, R[n][2] += y.z, R[n][3] += y.w;
       }
     } else {
+#pragma unroll
+      for (int x = 0; x < G; ++x) get_b(0, x);
       if (i > 0) ok = ld_wait(&r_empty[team], (i - 1) & 1);
       if (!ok) break;
     }
-    uint32_t b_hi[2][G / 2][4], b_lo[2][G / 2][4];
-    auto get_b = [&](int at) {  // the G columns and 16 tokens of step `at`
-      const int kt = at / (NK / G), n = at % (NK / G) * G;
-#pragma unroll
-      for (int x = 0; x < G / 2; ++x) {
-        const int where = ld_at<PIECES>(kt * 16 + (lane & 15), part * NK + n + 2 * x + (lane >> 4));
-        ld_matrix4_trans(b_lo[at & 1][x], head.kt_lo + where);
-        ld_matrix4_trans(b_hi[at & 1][x], head.kt_hi + where);
-      }
-    };
-    get_b(0);
-    // R = V - gamma K S^T, zeros for the tokens of other lines
     float m_r[2] = {0.0f, 0.0f};
-    float2 f[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float v[4];
-      TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
-      TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
-      const int j = n * 8 + cc * 2;
-      f[n] = *(const float2*)(head.kt_scale + j);
-      if (DELTA) {
-        const float2 in = *(const float2*)(head.r_in + j);
-        v[0] = fmaf(-R[n][0], in.x, v[0]), v[1] = fmaf(-R[n][1], in.y, v[1]);
-        v[2] = fmaf(-R[n][2], in.x, v[2]), v[3] = fmaf(-R[n][3], in.y, v[3]);
-      }
-      if (partial) {
-        if (j < lo || j >= hi) v[0] = v[2] = f[n].x = 0.0f;
-        if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f[n].y = 0.0f;
-      }
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        R[n][y] = v[y];
-        m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
-      }
+      m_r[0] = fmaxf(m_r[0], fmaxf(fabsf(R[n][0]), fabsf(R[n][1])));
+      m_r[1] = fmaxf(m_r[1], fmaxf(fabsf(R[n][2]), fabsf(R[n][3])));
     }
     // S = gamma_last S + R^T K~, in S's scale: R times K~'s rows, which are below 2^15 and mostly near 2^7, must not pass it. Where
     // that is not certain, or S nearly vanishes, in one that suits the larger of the two.
@@ -952,21 +970,22 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     float up[2] = {ld_inverse(down[0]), ld_inverse(down[1])}, g2[2] = {gamma, gamma};
     if (__any_sync(0xffffffffu, fresh || !(gamma >= 0x1p-5f) ||
                                     !(fmaxf(m_r[0] * up[0], m_r[1] * up[1]) * head.kt_most < 0x1p8f))) {
-      float m[2] = {0.0f, 0.0f}, m_s[2] = {0.0f, 0.0f};
+      float m[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0] * f[n].x), fabsf(R[n][1] * f[n].y)));
         m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2] * f[n].x), fabsf(R[n][3] * f[n].y)));
       }
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        m_s[0] = fmaxf(m_s[0], fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-        m_s[1] = fmaxf(m_s[1], fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
-      }
-#pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float dn;
-        ld_scale(fmaxf(gamma * (ld_row_most(m_s[r]) * down[r]), ld_row_most(m[r]) * 0x1p7f), up[r], dn);
+        float dn, m_s = 0x1p15f;  // S's rows are below that; not by more than 2^6
+        if (fresh) {
+          m_s = 0.0f;
+#pragma unroll
+          for (int n = 0; n < NK; ++n) m_s = fmaxf(m_s, fmaxf(fabsf(S[n][2 * r]), fabsf(S[n][2 * r + 1])));
+          m_s = ld_row_most(m_s);
+        }
+        ld_scale(fmaxf(gamma * (m_s * down[r]), ld_row_most(m[r]) * 0x1p7f), up[r], dn);
         g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
         down[r] = dn;
       }
@@ -974,16 +993,14 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
     for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
     float small[G][4] = {};  // the products of one low term, in sums of their own for the first G columns: more take turns
-    uint32_t hi4[2][4], lo4[2][4];
-    auto terms = [&](int kt) {
-      const float2 f0 = f[2 * kt], f1 = f[2 * kt + 1];
-      uint32_t (&hi)[4] = hi4[kt & 1], (&lo)[4] = lo4[kt & 1];
-      ld_split(R[2 * kt][0] * f0.x * up[0], R[2 * kt][1] * f0.y * up[0], hi[0], lo[0]);
-      ld_split(R[2 * kt][2] * f0.x * up[1], R[2 * kt][3] * f0.y * up[1], hi[1], lo[1]);
-      ld_split(R[2 * kt + 1][0] * f1.x * up[0], R[2 * kt + 1][1] * f1.y * up[0], hi[2], lo[2]);
-      ld_split(R[2 * kt + 1][2] * f1.x * up[1], R[2 * kt + 1][3] * f1.y * up[1], hi[3], lo[3]);
+    auto r_terms = [&](int kt, int x) {
+      const int n = 2 * kt + (x >> 1), y = x & 1;
+      ld_split(R[n][2 * y] * (f[n].x * up[y]), R[n][2 * y + 1] * (f[n].y * up[y]), hi4[kt & 1][x], lo4[kt & 1][x]);
     };
-    terms(0);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) r_terms(0, x);
+    float uu[2], ud[2];
+    bool next = true;
 #pragma unroll
     for (int kt = 0; kt < LD_C / 16; ++kt) {
 #pragma unroll
@@ -991,32 +1008,36 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         const int at = kt * (NK / G) + n / G;
         const auto& bh = b_hi[at & 1];
         const auto& bl = b_lo[at & 1];
-        float (*const low)[4] = n == 0 ? small : S + n;
+        float (*const less)[4] = n == 0 ? small : S + n;
 #pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(low[x], hi4[kt & 1], bl[x / 2][x % 2 * 2], bl[x / 2][x % 2 * 2 + 1]);
-        if (at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1);
-#pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(S[n + x], hi4[kt & 1], bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
-        if (n == 0 && kt + 1 < LD_C / 16) terms(kt + 1);
-#pragma unroll
-        for (int x = 0; x < G; ++x) ld_mma(low[x], lo4[kt & 1], bh[x / 2][x % 2 * 2], bh[x / 2][x % 2 * 2 + 1]);
-      }
-      if (kt == 0) {  // R for the outputs, one term, beside the products
-        float uu[2], ud[2];
-        ld_scale(ld_row_most(m_r[0]), uu[0], ud[0]);
-        ld_scale(ld_row_most(m_r[1]), uu[1], ud[1]);
-#pragma unroll
-        for (int y = 0; y < LD_C / 16; ++y)
-          if (y % PARTS == part)
-            *(uint4*)(place + Shape::R + (y * 32 + lane) * 16) =
-                make_uint4(ld_half2(R[2 * y][0] * uu[0], R[2 * y][1] * uu[0]), ld_half2(R[2 * y][2] * uu[1], R[2 * y][3] * uu[1]),
-                           ld_half2(R[2 * y + 1][0] * uu[0], R[2 * y + 1][1] * uu[0]),
-                           ld_half2(R[2 * y + 1][2] * uu[1], R[2 * y + 1][3] * uu[1]));
-        if (cc == 0 && part == 0) {
-          float* const r_scales = (float*)(place + Shape::SCALES);
-          r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
+        for (int x = 0; x < 3 * G; ++x) {
+          const int y = x % G;
+          if (x < G) ld_mma(less[y], hi4[kt & 1], bl[y / 2][y % 2 * 2], bl[y / 2][y % 2 * 2 + 1]);
+          else if (x < 2 * G) ld_mma(S[n + y], hi4[kt & 1], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
+          else ld_mma(less[y], lo4[kt & 1], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
+          if (x % 3 == 0 && at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1, x / 3);
+          if (n == 0 && x % (3 * G / 4) == 2 && kt + 1 < LD_C / 16) r_terms(kt + 1, x / (3 * G / 4));
+          // R for the outputs, one term
+          if (kt == 0 && n == 0 && x % 6 == 4) {
+            if (x / 6 < 2) ld_scale(ld_row_most(m_r[x / 6]), uu[x / 6], ud[x / 6]);
+          }
+          if (kt == 1 && n == 0 && x % 3 == 1) {
+            const int z = x / 3;
+            if (z < LD_C / 16 && z % PARTS == part)
+              *(uint4*)(place + Shape::R + (z * 32 + lane) * 16) =
+                  make_uint4(ld_half2(R[2 * z][0] * uu[0], R[2 * z][1] * uu[0]), ld_half2(R[2 * z][2] * uu[1], R[2 * z][3] * uu[1]),
+                             ld_half2(R[2 * z + 1][0] * uu[0], R[2 * z + 1][1] * uu[0]),
+                             ld_half2(R[2 * z + 1][2] * uu[1], R[2 * z + 1][3] * uu[1]));
+          }
+          if (kt == 2 && n == 0 && x == 1) {
+            if (cc == 0 && part == 0) {
+              float* const r_scales = (float*)(place + Shape::SCALES);
+              r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
+            }
+            ld_arrive(&r_full[team], lane);
+          }
+          if (kt == 2 && n == 0 && x == 3 * G / 2 && i + 1 < chunks) next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1);
         }
-        ld_arrive(&r_full[team], lane);
       }
     }
 #pragma unroll
@@ -1024,6 +1045,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
       for (int y = 0; y < 4; ++y) S[x][y] += small[x][y];
     ld_arrive(&empty[st], lane);
+    ok = __all_sync(0xffffffffu, next);
   }
   if (there && ok)
 #pragma unroll
