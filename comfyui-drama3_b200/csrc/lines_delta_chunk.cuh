@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
       for (int x = 0; x < 4; ++x) get_k(0, x);
     // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already: votes tell, without the largest itself
-    bool fresh = false;  // a row of zeros, which has no size
+    float m_s[2] = {0x1p15f, 0x1p15f};  // S's rows are below that, by no more than 2^6, or zeros
     {
       float m[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -854,12 +854,11 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           float up, dn;
           ld_scale(most * down[r], up, dn);
           up *= down[r];
-          fresh |= most == 0.0f;
+          if (most == 0.0f) m_s[r] = 0.0f;
           down[r] = dn;
 #pragma unroll
           for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
         }
-        fresh = __any_sync(0xffffffffu, fresh);
       }
     }
     // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs. Conversions and loads of the
@@ -967,28 +966,16 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     // S = gamma_last S + R^T K~, in S's scale: R times K~'s rows, which are below 2^15 and mostly near 2^7, must not pass it. Where
     // that is not certain, or S nearly vanishes, in one that suits the larger of the two.
     const float gamma = head.gamma[hi - 1];
-    float up[2] = {ld_inverse(down[0]), ld_inverse(down[1])}, g2[2] = {gamma, gamma};
-    if (__any_sync(0xffffffffu, fresh || !(gamma >= 0x1p-5f) ||
-                                    !(fmaxf(m_r[0] * up[0], m_r[1] * up[1]) * head.kt_most < 0x1p8f))) {
-      float m[2] = {0.0f, 0.0f};
+    float up[2], g2[2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        m[0] = fmaxf(m[0], fmaxf(fabsf(R[n][0] * f[n].x), fabsf(R[n][1] * f[n].y)));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(R[n][2] * f[n].x), fabsf(R[n][3] * f[n].y)));
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float dn, m_s = 0x1p15f;  // S's rows are below that; not by more than 2^6
-        if (fresh) {
-          m_s = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NK; ++n) m_s = fmaxf(m_s, fmaxf(fabsf(S[n][2 * r]), fabsf(S[n][2 * r + 1])));
-          m_s = ld_row_most(m_s);
-        }
-        ld_scale(fmaxf(gamma * (m_s * down[r]), ld_row_most(m[r]) * 0x1p7f), up[r], dn);
-        g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
-        down[r] = dn;
-      }
+    for (int r = 0; r < 2; ++r) {
+      m_r[r] = ld_row_most(m_r[r]);
+      const float added = m_r[r] * head.kt_most * 0x1p7f, kept = gamma * m_s[r] * down[r];
+      float dn = down[r];
+      up[r] = ld_inverse(dn);
+      if (!(kept * up[r] >= 0x1p10f && added * up[r] < 0x1p15f)) ld_scale(fmaxf(kept, added), up[r], dn);
+      g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
+      down[r] = dn;
     }
 #pragma unroll
     for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
@@ -1019,7 +1006,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           if (n == 0 && x % (3 * G / 4) == 2 && kt + 1 < LD_C / 16) r_terms(kt + 1, x / (3 * G / 4));
           // R for the outputs, one term
           if (kt == 0 && n == 0 && x % 6 == 4) {
-            if (x / 6 < 2) ld_scale(ld_row_most(m_r[x / 6]), uu[x / 6], ud[x / 6]);
+            if (x / 6 < 2) ld_scale(m_r[x / 6], uu[x / 6], ud[x / 6]);
           }
           if (kt == 1 && n == 0 && x % 3 == 1) {
             const int z = x / 3;
