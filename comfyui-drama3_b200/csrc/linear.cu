@@ -83,8 +83,10 @@ int conv_type(const d3::LcArgs& a, bool vectors, cudaStream_t s) {
   }
 }
 
-// Whether lines_delta goes token by token (or in chunks).
-bool delta_steps(int T, int B) { return T <= 2 * B || T <= 8; }
+// Whether lines_delta goes token by token (or in chunks). Measured (B200, 16 / 32 heads of 128, us by tokens / in chunks): lines of 4
+// tokens each, 1 line 4.8 / 23, 16 lines 20 / 62, 256 lines 274 / 701; of 16 each 13 / 23, 62 / 65, 918 / 847; all but one line with a token,
+// the last with the rest of 4 a line, 16 lines 46 / 62, 256 lines 866 / 714; one line of 32 23 / 22.
+bool delta_steps(int T, int B) { return T <= 4LL * B || T <= 16; }
 
 size_t delta_block_bytes(int Hk, int Hv, int Dk) {
   return Dk == 64 ? Hk * sizeof(d3::LdRows<64>) + Hv * sizeof(d3::LdHead<64>)
