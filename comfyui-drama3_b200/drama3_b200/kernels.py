@@ -729,13 +729,10 @@ def _attention_workspace(index, T, Hq, Hkv, D):
     return size
 
 
-def _form(t):
-    return None if t is None else (t.dtype, t.get_device(), t.shape, t.stride())
-
-
-def _checked(forms, kept, check_forms, tensors):
+def _checked(kept, check_forms, *tensors):
     """check_forms(*tensors), kept for tensors of these forms (types, devices, shapes, strides): a step's tensors have the
     same ones in every layer."""
+    forms = tuple([None if t is None else (t.dtype, t.get_device(), t.shape, t.stride()) for t in tensors])
     found = kept.get(forms)
     if found is None:
         if len(kept) >= 4096:
@@ -750,15 +747,14 @@ def _same_device(what, device, *tensors):
             raise ValueError(f"{what}: every tensor must be on {device}")
 
 
-def _plan_lines(what, device, plan, T):
-    """(cu, line, B) of a plan for T tokens; refuses one of another pass."""
-    cu, line = plan.cu, plan.line
-    B = cu.shape[0] - 1
+def _plan_lines(what, device, cu, line, T, lines):
+    """Refuses what a plan says of its lines where it is another pass's, of T tokens and `lines` lines."""
     if line.shape[0] != T:
         raise ValueError(f"{what}: the plan is for {line.shape[0]} tokens, not for {T}")
-    _ints("the plan's cu", cu, device, B + 1)
+    if cu.shape[0] != lines + 1:
+        raise ValueError(f"{what}: the plan has {cu.shape[0] - 1} lines, the state {lines}")
+    _ints("the plan's cu", cu, device, lines + 1)
     _ints("the plan's line", line, device, T)
-    return cu, line, B
 
 
 def _norm_weights(what, rows, size, *weights):
@@ -779,18 +775,15 @@ def lines_conv(x, weight, state, plan, bias=None, silu=True):
     the token's own; of the rows' type or float32) and bias [C], through SiLU unless silu is False. state [B, W - 1, C] of the
     rows' type: the inputs that each line had last, updated in place (zeros: a line that begins). Places of no line get
     zeros. 32-bit arithmetic, rounded once."""
-    tensors = (x, weight, state, bias)
-    device, sizes, W, w_f32 = _checked(tuple(map(_form, tensors)), _CONV_FORMS, _conv_arguments, tensors)
-    cu, line, B = _plan_lines("lines_conv", device, plan, sizes[1])
-    if state.shape[0] != B:
-        raise ValueError(f"lines_conv: the plan has {B} lines, the state {state.shape[0]}")
-    out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    _launch(device, "lines_conv", lib().d3_lines_conv, x.data_ptr(), x.stride(0), *sizes, weight.data_ptr(), _ptr(bias), W,
-            w_f32, state.data_ptr(), cu.data_ptr(), line.data_ptr(), B, 1 if silu else 0, out.data_ptr())
+    cu, line = plan.cu, plan.line
+    device, sizes, W, w_f32, B = _checked(_CONV_FORMS, _conv_arguments, x, weight, state, bias, cu, line)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _launch(device, "lines_conv", lib().d3_lines_conv, x.data_ptr(), *sizes, weight.data_ptr(), _ptr(bias), W, w_f32,
+            state.data_ptr(), cu.data_ptr(), line.data_ptr(), B, 1 if silu else 0, out.data_ptr())
     return out
 
 
-def _conv_arguments(x, weight, state, bias):
+def _conv_arguments(x, weight, state, bias, cu, line):
     device = _gpu_of(x, "lines_conv")
     _same_device("lines_conv", device, weight, state, bias)
     if x.dtype not in ROW_TYPES:
@@ -806,7 +799,9 @@ def _conv_arguments(x, weight, state, bias):
         raise ValueError("weight and bias [C] must be contiguous, of the rows' type or float32, alike")
     if state.dim() != 3 or state.shape[1:] != (W - 1, C) or state.dtype != x.dtype or not state.is_contiguous():
         raise ValueError(f"state must be a contiguous [B, {W - 1}, {C}] tensor of the rows' type")
-    return device, (ROW_TYPES[x.dtype], T, C), W, int(weight.dtype == torch.float32)
+    B = state.shape[0]
+    _plan_lines("lines_conv", device, cu, line, T, B)
+    return device, (x.stride(0), ROW_TYPES[x.dtype], T, C), W, int(weight.dtype == torch.float32), B
 
 
 def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None, eps=1e-6, scale=None):
@@ -823,33 +818,24 @@ def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None
     sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get zeros."""
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         q, k, v = (_aligned16(t) for t in (q, k, v))
-    tensors = (q, k, v, decay, state, beta, a_log, dt_bias)
-    device, copies, strides, sizes, gates_f32 = _checked(tuple(map(_form, tensors)), _DELTA_FORMS, _delta_arguments, tensors)
+    cu, line = plan.cu, plan.line
+    device, copies, strides, sizes, (decay_token, beta_token, gates_f32), usual_scale, B, size = _checked(
+        _DELTA_FORMS, _delta_arguments, q, k, v, decay, state, beta, a_log, dt_bias, cu, line)
     if copies:
         q, k, v = (t.contiguous() for t in (q, k, v))
-    _, T, Hk, Hv, Dk, Dv = sizes
-    cu, line, B = _plan_lines("lines_delta", device, plan, T)
-    if state.shape[0] != B:
-        raise ValueError(f"lines_delta: the plan has {B} lines, the state {state.shape[0]}")
     if state.data_ptr() & 15:
         raise ValueError("state must start on a 16-byte boundary")
-    out = torch.empty((T, Hv, Dv), dtype=q.dtype, device=device)
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
     # scratch of this call alone: it may make several launches, and those of another thread on the same stream may come between
-    size = _delta_workspace(T, B, Hk, Hv, Dk)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _launch(device, "lines_delta", lib().d3_lines_delta, q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(),
-            strides[2], *sizes, decay.data_ptr(), decay.stride(0), _ptr(beta), 0 if beta is None else beta.stride(0), gates_f32,
-            _ptr(a_log), _ptr(dt_bias), -1.0 if eps is None else eps, Dk ** -0.5 if scale is None else scale,
-            state.data_ptr(), cu.data_ptr(), line.data_ptr(), B, out.data_ptr(), _ptr(ws), size)
+            strides[2], *sizes, decay.data_ptr(), decay_token, _ptr(beta), beta_token, gates_f32, _ptr(a_log), _ptr(dt_bias),
+            -1.0 if eps is None else eps, usual_scale if scale is None else scale, state.data_ptr(), cu.data_ptr(),
+            line.data_ptr(), B, out.data_ptr(), _ptr(ws), size)
     return out
 
 
-@functools.lru_cache(maxsize=4096)
-def _delta_workspace(T, B, Hk, Hv, Dk):
-    return lib().d3_lines_delta_workspace(T, B, Hk, Hv, Dk)
-
-
-def _delta_arguments(q, k, v, decay, state, beta, a_log, dt_bias):
+def _delta_arguments(q, k, v, decay, state, beta, a_log, dt_bias, cu, line):
     device = _gpu_of(q, "lines_delta")
     _same_device("lines_delta", device, k, v, decay, state, beta, a_log, dt_bias)
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -877,7 +863,11 @@ def _delta_arguments(q, k, v, decay, state, beta, a_log, dt_bias):
         raise ValueError(f"state must be a contiguous float32 [B, {Hv}, {Dv}, {Dk}] tensor")
     copies = any(s % 8 for t in (q, k, v) for s in t.stride()[:2])
     strides = tuple(_int64s((t.shape[1] * t.shape[2], t.shape[2]) if copies else t.stride()[:2]) for t in (q, k, v))
-    return device, copies, strides, (ROW_TYPES[q.dtype], T, Hk, Hv, Dk, Dv), int(decay.dtype == torch.float32)
+    B = state.shape[0]
+    _plan_lines("lines_delta", device, cu, line, T, B)
+    return (device, copies, strides, (ROW_TYPES[q.dtype], T, Hk, Hv, Dk, Dv),
+            (decay.stride(0), 0 if beta is None else beta.stride(0), int(decay.dtype == torch.float32)), Dk ** -0.5, B,
+            lib().d3_lines_delta_workspace(T, B, Hk, Hv, Dk))
 
 
 _ACTIVATIONS = {"silu": 0, "sigmoid": 1}
@@ -887,11 +877,10 @@ def gated_norm(x, gate, weight, eps=1e-6, unit_offset=False, activation="silu"):
     """[T, H, D]: each head of x [T, H, D] (bfloat16, float16 or float32; any strides with the last dimension contiguous)
     divided by its root mean square, times weight [D] (of the rows' type or float32; 1 + weight with unit_offset), times
     the gate [T, H, D] through its activation, "silu" or "sigmoid". 32-bit arithmetic, rounded once."""
-    tensors = (x, gate, weight)
-    device, x_strides, gate_strides, sizes, w_f32 = _checked(tuple(map(_form, tensors)), _GATED_FORMS, _gated_arguments, tensors)
+    device, x_strides, gate_strides, sizes, w_f32 = _checked(_GATED_FORMS, _gated_arguments, x, gate, weight)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, not {activation}")
-    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     _launch(device, "gated_norm", lib().d3_gated_norm, x.data_ptr(), x_strides, gate.data_ptr(), gate_strides, *sizes,
             weight.data_ptr(), w_f32, 1.0 if unit_offset else 0.0, eps, _ACTIVATIONS[activation], out.data_ptr())
     return out
@@ -914,11 +903,11 @@ def add_norm(x, residual, weight, post_weight=None, gate=None, scale=1.0, eps=1e
     (of the sum before it is rounded) with weight [W]. Rows bfloat16, float16 or float32, of one type, the last dimension
     contiguous; weights of the rows' type or float32, alike, plus 1 with unit_offset; gate: a tensor of the rows' type that
     broadcasts to [T, W]. 32-bit arithmetic, rounded once."""
-    tensors = (x, residual, weight, post_weight, gate)
-    device, sizes, w_f32, gate_token, gate_kind = _checked(tuple(map(_form, tensors)), _JOIN_FORMS, _join_arguments, tensors)
-    sums, normed = (torch.empty(x.shape, dtype=x.dtype, device=device) for _ in range(2))
-    _launch(device, "add_norm", lib().d3_add_norm, x.data_ptr(), x.stride(0), residual.data_ptr(), residual.stride(0), *sizes,
-            weight.data_ptr(), _ptr(post_weight), w_f32, 1.0 if unit_offset else 0.0, _ptr(gate), gate_token, gate_kind,
+    device, (x_token, r_token), sizes, w_f32, gate_token, gate_kind = _checked(_JOIN_FORMS, _join_arguments, x, residual, weight,
+                                                                              post_weight, gate)
+    sums = torch.empty_like(x, memory_format=torch.contiguous_format)
+    normed = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _launch(device, "add_norm", lib().d3_add_norm, x.data_ptr(), x_token, residual.data_ptr(), r_token, *sizes, weight.data_ptr(), _ptr(post_weight), w_f32, 1.0 if unit_offset else 0.0, _ptr(gate), gate_token, gate_kind,
             scale, eps, sums.data_ptr(), normed.data_ptr())
     return sums, normed
 
@@ -939,4 +928,4 @@ def _join_arguments(x, residual, weight, post_weight, gate):
         if W > 1 and channel not in (0, 1):
             raise ValueError("gate's last dimension must be contiguous, or of one value")
         kind = 1 if channel == 0 or W == 1 else 2
-    return device, (ROW_TYPES[x.dtype], T, W), w_f32, token, kind
+    return device, (x.stride(0), residual.stride(0)), (ROW_TYPES[x.dtype], T, W), w_f32, token, kind

@@ -133,34 +133,37 @@ def half(*shape):
 
 
 def test_conv_forms(anywhere):
-    x, w, s = half(5, 16), half(16, 4), half(2, 3, 16)
-    device, sizes, taps, w_f32 = kernels._conv_arguments(x, w, s, None)
-    assert sizes == (0, 5, 16) and taps == 4 and w_f32 == 0
-    assert kernels._conv_arguments(half(5, 32)[:, 16:], w.view(16, 1, 4).float(), s, torch.zeros(16))[3] == 1
+    x, w, s, plan = half(5, 16), half(16, 4), half(2, 3, 16), plan_of([2, 3])
+    plan = (plan.cu, plan.line)
+    device, sizes, taps, w_f32, B = kernels._conv_arguments(x, w, s, None, *plan)
+    assert sizes == (16, 0, 5, 16) and taps == 4 and w_f32 == 0 and B == 2
+    assert kernels._conv_arguments(half(5, 32)[:, 16:], w.view(16, 1, 4).float(), s, torch.zeros(16), *plan)[3] == 1
     for bad in [(x.int(), w, s, None), (half(16, 5).T, w, s, None), (x, half(16, 9), s, None), (x, half(16, 1), s, None),
                 (x, half(15, 4), s, None), (x, w.half(), s, None), (x, w, s, torch.zeros(16)), (x, w, s, half(15)),
                 (x, w, half(2, 4, 16), None), (x, w, s.float(), None), (x, w, half(2, 3, 32)[..., ::2], None),
-                (x, half(4, 16).T, s, None)]:
+                (x, half(4, 16).T, s, None), (x, w, half(3, 3, 16), None), (half(6, 16), w, s, None)]:
         with pytest.raises((TypeError, ValueError)):
-            kernels._conv_arguments(*bad)
+            kernels._conv_arguments(*bad, *plan)
 
 
 def test_delta_forms(anywhere):
     q, k, v, g, s = half(5, 2, 64), half(5, 2, 64), half(5, 4, 48), half(5, 4), torch.zeros((3, 4, 48, 64))
-    a = torch.zeros(4)
-    device, copies, st, sizes, f32 = kernels._delta_arguments(q, k, v, g, s, g, a, a)
-    assert not copies and sizes == (0, 5, 2, 4, 64, 48) and f32 == 0 and list(st[2]) == [192, 48]
+    a, plan = torch.zeros(4), plan_of([2, 0, 3])
+    plan = (plan.cu, plan.line)
+    device, copies, st, sizes, gates, scale, B, size = kernels._delta_arguments(q, k, v, g, s, g, a, a, *plan)
+    assert not copies and sizes == (0, 5, 2, 4, 64, 48) and gates == (4, 4, 0) and list(st[2]) == [192, 48] and B == 3 and size == 0
     wide = half(5, 2 * 64 + 3)
-    assert kernels._delta_arguments(wide[:, 3:].view(5, 2, 64), k, v, g.float(), s, None, None, None)[1]
+    assert kernels._delta_arguments(wide[:, 3:].view(5, 2, 64), k, v, g.float(), s, None, None, None, *plan)[1]
     for bad in [(q.float(), k.float(), v.float(), g, s), (q, k.half(), v, g, s), (q, half(5, 4, 64), v, g, s),
                 (half(5, 3, 64), half(5, 3, 64), v, g, s), (half(5, 2, 96), half(5, 2, 96), v, g, s),
                 (q, k, half(5, 4, 40), g, s), (q, k, half(4, 4, 48), g, s), (half(5, 64, 2).transpose(1, 2), k, v, g, s),
                 (q, k, v, half(5, 3), s), (q, k, v, half(4, 5).T, s), (q, k, v, g.half(), s), (q, k, v, g, s.to(torch.bfloat16)),
                 (q, k, v, g, torch.zeros((3, 4, 64, 48))), (q, k, v, g, torch.zeros((3, 4, 64, 48)).transpose(2, 3)),
                 (q, k, v, g, s, g.float()), (q, k, v, g, s, g, None, a), (q, k, v, g, s, g, a.double()),
-                (q, k, v, g, s, g, torch.zeros(3)), (q, k, v, g, s, g, a, torch.zeros(8)[::2])]:
+                (q, k, v, g, s, g, torch.zeros(3)), (q, k, v, g, s, g, a, torch.zeros(8)[::2]),
+                (q, k, v, g, torch.zeros((2, 4, 48, 64)))]:
         with pytest.raises((TypeError, ValueError)):
-            kernels._delta_arguments(*bad, *[None] * (8 - len(bad)))
+            kernels._delta_arguments(*bad, *[None] * (8 - len(bad)), *plan)
 
 
 def test_norm_forms(anywhere):
@@ -173,7 +176,7 @@ def test_norm_forms(anywhere):
     x = half(5, 64)
     for gate, token, kind in [(None, 0, 0), (half(5, 1), 1, 1), (half(1, 64), 0, 2), (half(64), 0, 2), (half(5, 64), 64, 2),
                               (half(1, 1), 0, 1), (half(5, 128)[:, :64], 128, 2), (half(5, 3)[:, :1], 3, 1)]:
-        assert kernels._join_arguments(x, x, w, None, gate)[3:] == (token, kind)
+        assert kernels._join_arguments(x, x, w, None, gate)[4:] == (token, kind)
     for bad in [(x.int(), x.int(), w, None, None), (x, x.half(), w, None, None), (x, half(4, 64), w, None, None),
                 (half(64, 5).T, x, w, None, None), (x, x, half(32), None, None), (x, x, w, w.float(), None),
                 (x, x, w, None, half(4, 1)), (x, x, w, None, half(5, 32)), (x, x, w, None, half(64, 5).T),
@@ -183,12 +186,27 @@ def test_norm_forms(anywhere):
 
 
 def test_plan_of_another_pass_is_refused():
-    device = torch.device("cpu")
-    assert kernels._plan_lines("lines_delta", device, plan_of([2, 3]), 5)[2] == 2
+    device, plan = torch.device("cpu"), plan_of([2, 3])
+    kernels._plan_lines("lines_delta", device, plan.cu, plan.line, 5, 2)
     with pytest.raises(ValueError, match="5 tokens"):
-        kernels._plan_lines("lines_delta", device, plan_of([2, 3]), 6)
+        kernels._plan_lines("lines_delta", device, plan.cu, plan.line, 6, 2)
+    with pytest.raises(ValueError, match="2 lines"):
+        kernels._plan_lines("lines_delta", device, plan.cu, plan.line, 5, 3)
     with pytest.raises(ValueError, match="int32"):
-        kernels._plan_lines("lines_delta", device, plan_of([2, 3])._replace(cu=torch.zeros(3, dtype=torch.int64)), 5)
+        kernels._plan_lines("lines_delta", device, torch.zeros(3, dtype=torch.int64), plan.line, 5, 2)
+
+
+def test_state_shapes():
+    from drama3_b200.hybrid import LinesDelta, LinesState
+    state = LinesState(2, 3, 2, 4, 64, 80, 4, "cpu")
+    assert len(state.conv) == 2 and state.conv[0].shape == (3, 3, 2 * 2 * 64 + 4 * 80) and state.delta[1].shape == (3, 4, 80, 64)
+    state.prefix_delta[1].fill_(2)
+    state.begin()
+    assert (state.delta[1] == 2).all() and not state.delta[0].any()
+    state.clear()
+    assert not state.delta[1].any() and not state.prefix_delta[1].any()
+    m = LinesDelta(32, 2, 4, 64, 80)
+    assert m.in_proj.weight.shape == (sum(m.sizes), 32) and m.out_proj.weight.shape == (32, 320) and m.a_log.dtype == torch.float32
 
 
 # ---- restatements
