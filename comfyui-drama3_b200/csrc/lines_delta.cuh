@@ -55,6 +55,8 @@ template <int TYPE> D3_DEV float ld_beta(const LdArgs& a, long long t, int h) {
 // u (k . q)). Bound by memory where the tokens are few: a state is read once and written once, 8 Dk Dv bytes a head against 7
 // Dk Dv operations a token, so that all of a warp's rows are asked for at once. Sums over a row's lanes halve the values as
 // they halve the lanes: nine exchanges for eight rows where a butterfly for each would take forty.
+// Measured (B200, bf16, 16 / 32 heads of 128): 256 lines of a token 126 us device time, 6.5 TB/s; 16 lines 13.4 us in a stream of calls, 9.3
+// where the states stay in L2; one line 2.8 to 3.1 us, the latency of a launch and three loads that wait for one another.
 constexpr int LS_WARPS = 4;
 constexpr int LS_ROWS = 8;
 
@@ -129,7 +131,9 @@ __global__ void __launch_bounds__(LS_WARPS * 32) lines_delta_step_kernel(LdArgs 
       qq += __shfl_xor_sync(0xffffffffu, qq, o);
       kq += __shfl_xor_sync(0xffffffffu, kq, o);
     }
-    const float rk = a.eps >= 0.0f ? rsqrtf(kk + a.eps) : 1.0f, rq = (a.eps >= 0.0f ? rsqrtf(qq + a.eps) : 1.0f) * a.scale;
+    // a row of zeros stays one, with eps 0 too
+    const float rk = a.eps < 0.0f ? 1.0f : kk == 0.0f ? 0.0f : rsqrtf(kk + a.eps);
+    const float rq = (a.eps < 0.0f ? 1.0f : qq == 0.0f ? 0.0f : rsqrtf(qq + a.eps)) * a.scale;
     float sk[LS_ROWS], sq[LS_ROWS];
 #pragma unroll
     for (int r = 0; r < LS_ROWS; ++r) {

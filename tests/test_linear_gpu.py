@@ -221,6 +221,18 @@ def test_delta_extremes(cuda, counts):
     check_delta(cuda, (q, k, v, decay, state), dict(beta=beta), cu, plan)
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [40, 50]])
+def test_delta_rows_of_zeros_without_eps(cuda, counts):
+    """eps 0: rows of zeros stay zeros, whatever form the call takes."""
+    from drama3_b200 import kernels
+    cu, plan = plan_of(counts, 0, cuda)
+    (q, k, v, decay, state), more = delta_case(cuda, (2, 2, 64, 64), counts, 0, torch.bfloat16, "raw", 26)
+    q, k = q.clone(), k.clone()
+    q[::3], k[::2] = 0, 0
+    out = kernels.lines_delta(q, k, v, decay, state, plan, eps=0.0, **more)
+    assert out.isfinite().all() and state.isfinite().all() and not out[::3].any()
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e-12, 1e12, 1e25])
 @pytest.mark.parametrize("counts", [[1, 1], [100, 130]])
 def test_delta_states_of_any_size(cuda, size, counts):
@@ -321,6 +333,43 @@ def test_delta_many_lines(cuda):
     cu, plan = plan_of(counts, 2, cuda)
     args, more = delta_case(cuda, (1, 1, 64, 16), counts, 2, torch.float16, "raw", 17)
     check_delta(cuda, args, more, cu, plan)
+
+
+def test_delta_first_call_of_a_thread(cuda):
+    """A thread that has made no CUDA call yet, whose first one encodes a tensor map."""
+    from drama3_b200 import kernels
+    cu, plan = plan_of([100, 30], 0, cuda)
+    args, more = delta_case(cuda, (1, 2, 64, 64), [100, 30], 0, torch.bfloat16, "raw", 27)
+    want, got = kernels.lines_delta(*args[:4], args[4].clone(), plan, **more), []
+    state = args[4].clone()
+    thread = threading.Thread(target=lambda: got.append(kernels.lines_delta(*args[:4], state, plan, **more)))
+    thread.start()
+    thread.join()
+    assert got and torch.equal(got[0], want)
+
+
+def test_delta_parts_of_a_long_pass_follow_one_another(cuda):
+    """A pass of more chunks than the scratch of one part holds: two parts, each from the states that the one before leaves."""
+    from drama3_b200 import _lib, kernels
+    heads = (16, 64, 64, 16)
+    chunk = _lib.lib().d3_lines_delta_workspace(64, 1, 16, 64, 64)
+    n = (256 << 20) // chunk * 64 + 100
+    assert _lib.lib().d3_lines_delta_workspace(n, 1, 16, 64, 64) <= 256 << 20
+    counts = [n - 130, 70]
+    cu, plan = plan_of(counts, 60, cuda)
+    (q, k, v, decay, state), more = delta_case(cuda, heads, counts, 60, torch.bfloat16, "raw", 28)
+    out = kernels.lines_delta(q, k, v, decay, state, plan, **more)
+    want = []
+    again = delta_case(cuda, heads, counts, 60, torch.bfloat16, "raw", 28)[0][4]
+    s0, s1 = again[:1].clone(), again[1:].clone()
+    for a, b, s in ((0, 1000, s0), (1000, cu[1], s0), (cu[1], cu[2], s1)):  # the same texts, in other pieces
+        cut = {name: t[a:b] if t.dim() == 2 else t for name, t in more.items()}
+        want.append(kernels.lines_delta(q[a:b], k[a:b], v[a:b], decay[a:b], s, plan_of([b - a], 0, cuda)[1], **cut))
+    want = torch.cat(want)
+    # both within the tolerance of the definition: twice its share of the rows' size, which the norms stand for
+    size = want.double().norm()
+    assert (out[:cu[2]].double() - want.double()).norm() <= 2 * (HALF[torch.bfloat16] + 2.0 ** -10) * size and not out[cu[2]:].any()
+    assert (state.double() - torch.cat((s0, s1)).double()).norm() <= 2 * 2.0 ** -15 * state.double().norm() and fault() == 0
 
 
 def test_delta_from_two_threads_on_one_stream(cuda):
