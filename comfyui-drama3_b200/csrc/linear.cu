@@ -106,7 +106,8 @@ int scan_launch(const CUtensorMap& vmap, const d3::LdChunkArgs& c, cudaStream_t 
   static std::atomic<uint64_t> done{0};
   if (int st = allow_smem_once(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS, PARTS>, smem, done)) return st;
   const dim3 blocks((c.a.Dv / 16 + WARPS - 1) / WARPS, c.a.Hv, c.a.B + 1);
-  return launch(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS, PARTS>, blocks, dim3(d3::LdScanShape<DK, WARPS, PARTS>::THREADS), smem, s, true, vmap, c);
+  return launch(d3::lines_delta_scan_kernel<TYPE, DK, DELTA, WARPS, PARTS>, blocks,
+                dim3(d3::LdScanShape<DK, WARPS, PARTS>::THREADS), smem, s, true, vmap, c);
 }
 
 template <int TYPE, int DK, bool DELTA>
@@ -129,6 +130,8 @@ int chunk_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cuda
     if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hv), dim3(d3::LD_PREP_THREADS), prep_smem, s,
                         true, c))
       return st;
+    // four teams of one warp a CTA where that gives every SM one, else two of two (us, the former / the latter: 8192 tokens of one line 561 /
+    // 438, 16 texts of up to 192 tokens 114 / 139)
     const long long wide = (long long)a.B * a.Hv * ((a.Dv + 63) / 64);
     if (int st = wide >= d.sms ? scan_launch<TYPE, DK, DELTA, 4, 1>(vmap, c, s) : scan_launch<TYPE, DK, DELTA, 2, 2>(vmap, c, s))
       return st;

@@ -42,7 +42,6 @@ template <int DK> struct alignas(128) LdHead {
   float r_in[LD_C];   // gamma_i |k| factor: of K S^T
   float q_in[LD_C];   // scale gamma_i |q| factor: of Q S^T
   float gamma[LD_C];
-  float kt_most, unused[63];  // the largest of kt_scale; to whole 256 bytes
 };
 
 // Element offset of 16-byte piece c of row r in rows of `pieces` of them (a multiple of 8): eight rows' pieces of one column lie
@@ -597,35 +596,34 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     const float nan = __uint_as_float(0x7fc00000u), gamma = ld_exp(G_s[tid].x + G_s[tid].y);
     const bool bad = bad_s[first] != 0, live = my_line >= 0;
     out->gamma[tid] = gamma;
-    float kt_most = live ? kt_scale[tid] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) kt_most = fmaxf(kt_most, __shfl_xor_sync(0xffffffffu, kt_most, o));
-    if (lane == 0) ((float*)&sum_s)[warp] = kt_most;
     out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
     out->r_in[tid] = live && !bad ? gamma * k_factor[tid] : 0.0f;
     out->q_in[tid] = !live ? 0.0f : bad ? nan : gamma * q_factor[tid];
   }
-  __syncthreads();
-  if (tid == 0) {
-    out->kt_most = fmaxf(((float*)&sum_s)[0], ((float*)&sum_s)[1]);
-    ld_bulk_done();
-  }
+  if (tid == 0) ld_bulk_done();
 }
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks. 16 rows are a team of
-// warps: one, or PARTS = 2 that have half of the columns each and add up their shares of K S^T, carry the state, S -> R -> S; the
-// last makes the outputs from what they leave in shared memory (S's high terms, R), one step behind, so that its products fill
-// the tensor core while the others' values are being converted. S stays in registers, as the
-// accumulator of products [rows of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand
-// is, so the chain has no exchange in it: K, Q, K~ and P T, as B operands, come from shared memory, where the first output warp keeps
-// chunks coming (bulk copies; the rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought
-// there and back between the products: with 16 rows a warp the chain is shorter in registers.)
+// warps: one, or PARTS = 2 that have half of the state's columns and half of the chunk's tokens each, carry the state, S -> R -> S;
+// as many others make the outputs from what those leave in shared memory (S's high terms, R), a step behind, so that their products
+// fill the tensor core while the first ones' values are being converted. S stays in registers, as the accumulator of products [rows
+// of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand is, so that a single warp's
+// chain has no exchange in it. Two warps give one another their terms of S and of R, and each begins with its own while the other's
+// come. K, Q, K~ and P T, as B operands, come from shared memory, where the first output warp keeps chunks coming (bulk copies; the
+// rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought there and back between the
+// products: with 16 rows a warp the chain is shorter in registers.)
+//
+// Bound by the chain's latency: 8192 tokens are 128 chunks one after another, and a head's rows are all that can be spread. Measured
+// (B200, 16 / 32 heads of 128, one line): 2.3 us a chunk, 3900 clocks, of which the 160 products of a warp that carries the state take
+// 1330 of its tensor core's time, those of the output warp beside it 350; the rest are conversions (370 for R, 480 for the
+// terms), barriers and the latency of what they wait for. One warp a team with four teams a CTA (which share the operands'
+// loads) takes 3.4 us a chunk and half the SMs: the better where lines and heads fill the GPU.
 template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
-  // a team's place: S's high terms as A fragments and its rows' scales (two chunks' by turns), R's terms and scales, the outputs,
-  // shares of K S^T (two chunks')
-  static constexpr int S = DK * 32 + 128, R = 2 * S, SCALES = R + LD_C * 32, OUT = SCALES + 128, SHARES = OUT + LD_C * 32;
-  static constexpr int TEAM = SHARES + (PARTS > 1 ? 2 * PARTS * LD_C * 64 : 0);
+  // a team's place: S's terms as A fragments (high ones, and low ones for the other part) with its rows' scales, two chunks' by turns;
+  // R's high terms with theirs; R times K~'s factors, both terms, with theirs, for the other part; the outputs
+  static constexpr int TERMS = DK * 32 * PARTS, S = TERMS + 128, R = 2 * S, R_SCALES = R + LD_C * 32, RK = R_SCALES + 128;
+  static constexpr int RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0), OUT = RK_SCALES + 128, TEAM = OUT + LD_C * 32;
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024;
   static constexpr int OUTS = PARTS;  // warps for the outputs, each of a share of the tokens: as many on every quarter of an SM
@@ -660,7 +658,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   constexpr int OUTS = Shape::OUTS, NO = NT / OUTS;
   extern __shared__ uint8_t ld_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], r_full[WARPS],
-      r_empty[WARPS], shares[WARPS][PARTS][2];  // [2]: odd and even chunks', as their places
+      r_empty[WARPS];  // [2]: odd and even chunks', as their places
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -672,10 +670,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + OUTS) * WARPS);
     for (int i = 0; i < WARPS; ++i) {
       mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], OUTS);
-      for (int y = 0; y < 2; ++y) {
-        mbar_init(&s_full[i][y], PARTS);
-        for (int j = 0; j < PARTS; ++j) mbar_init(&shares[i][j][y], 1);
-      }
+      mbar_init(&s_full[i][0], PARTS), mbar_init(&s_full[i][1], PARTS);
     }
     fence_mbar_init();
   }
@@ -741,7 +736,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
         for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
-      const float* const s_scales = (const float*)(place + (i & 1) * Shape::S + DK * 32);
+      const float* const s_scales = (const float*)(place + (i & 1) * Shape::S + Shape::TERMS);
 #pragma unroll
       for (int y = 0; y < PARTS; ++y) {
         const float s_down[2] = {s_scales[y * 16 + g], s_scales[y * 16 + g + 8]};
@@ -761,20 +756,25 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         const uint4 r4 = *(const uint4*)(place + Shape::R + (kt * 32 + lane) * 16);
         u4[kt][0] = r4.x, u4[kt][1] = r4.y, u4[kt][2] = r4.z, u4[kt][3] = r4.w;
       }
-      const float* const r_scales = (const float*)(place + Shape::SCALES);
-      const float r_down[2] = {r_scales[g], r_scales[g + 8]};
+      float r_down[PARTS][2];
+#pragma unroll
+      for (int y = 0; y < PARTS; ++y) {
+        const float* const r_scales = (const float*)(place + Shape::R_SCALES) + y * 16;
+        r_down[y][0] = r_scales[g], r_down[y][1] = r_scales[g + 8];
+      }
       ld_arrive(&r_empty[team], lane);
       uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
       for (int m = 0; m < NO; m += 2) {
         const int n = part * NO + m;
-        float pu[2][4] = {};
+        float pu[PARTS][2][4] = {};
 #pragma unroll
         for (int kt = 0; kt < LD_C / 16; ++kt)
           if (kt <= n / 2) {
             uint32_t p4[4];
             ld_matrix4(p4, head.p + ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-            ld_mma(pu[0], u4[kt], p4[0], p4[1]), ld_mma(pu[1], u4[kt], p4[2], p4[3]);
+            float (&sum)[2][4] = pu[kt / (LD_C / 16 / PARTS)];
+            ld_mma(sum[0], u4[kt], p4[0], p4[1]), ld_mma(sum[1], u4[kt], p4[2], p4[3]);
           }
         uint32_t o4[4];
 #pragma unroll
@@ -782,8 +782,12 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           const int j = (n + x) * 8 + cc * 2;
           const float2 fq = *(const float2*)(head.q_in + j), fp = *(const float2*)(head.p_scale + j);
           float o[4];
-          o[0] = fmaf(O[0][m + x][0], fq.x, pu[x][0] * r_down[0] * fp.x), o[1] = fmaf(O[0][m + x][1], fq.y, pu[x][1] * r_down[0] * fp.y);
-          o[2] = fmaf(O[0][m + x][2], fq.x, pu[x][2] * r_down[1] * fp.x), o[3] = fmaf(O[0][m + x][3], fq.y, pu[x][3] * r_down[1] * fp.y);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            float from_r = pu[0][x][y] * r_down[0][y >> 1];
+            if (PARTS > 1) from_r = fmaf(pu[PARTS - 1][x][y], r_down[PARTS - 1][y >> 1], from_r);
+            o[y] = fmaf(O[0][m + x][y], y & 1 ? fq.y : fq.x, from_r * (y & 1 ? fp.y : fp.x));
+          }
           o4[2 * x] = TT::put2(o[0], o[1]), o4[2 * x + 1] = TT::put2(o[2], o[3]);
         }
         const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
@@ -829,15 +833,14 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
     const bool partial = lo > 0 || hi < LD_C;
     // operands are asked for before what they are multiplied by is known
-    uint32_t k4[2][4][4];
-    auto get_k = [&](int kt, int x) {
-      ld_matrix4(k4[kt & 1][x], rows.k + ld_at<PIECES>(x * 16 + (lane & 7) + (lane >> 4) * 8, (part * KT + kt) * 2 + ((lane >> 3) & 1)));
+    uint32_t k4[2][NO / 2][4];
+    auto get_k = [&](int step, int at, int x) {  // 16 columns `at` of 16 of this part's tokens
+      ld_matrix4(k4[step & 1][x], rows.k + ld_at<PIECES>((part * NO + x * 2) * 8 + (lane & 7) + (lane >> 4) * 8, at * 2 + ((lane >> 3) & 1)));
     };
     if (DELTA)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) get_k(0, x);
+      for (int x = 0; x < NO / 2; ++x) get_k(0, part * KT, x);
     // S's rows between 2^9 and 2^15 at their largest, which is nearly always so already: votes tell, without the largest itself
-    float m_s[2] = {0x1p15f, 0x1p15f};  // S's rows are below that, by no more than 2^6, or zeros
     {
       float m[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -850,188 +853,246 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       if (__any_sync(0xffffffffu, off)) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float most = ld_row_most(m[r]);  // by all lanes
           float up, dn;
-          ld_scale(most * down[r], up, dn);
+          ld_scale(ld_row_most(m[r]) * down[r], up, dn);
           up *= down[r];
-          if (most == 0.0f) m_s[r] = 0.0f;
           down[r] = dn;
 #pragma unroll
           for (int n = 0; n < NK; ++n) S[n][2 * r] *= up, S[n][2 * r + 1] *= up;
         }
       }
     }
-    // S K^T, high and low terms of S apart so that sixteen sums take turns; S's high terms for the outputs. Conversions and loads of the
-    // next step stand between the products of this one: a warp's instructions issue in order, and a product holds its pipe for 8 clocks.
-    float R[NT][4] = {}, low[NT][4] = {};
-    uint32_t hi4[2][4], lo4[2][4];
-    auto s_terms = [&](int kt, int x) {
-      ld_split(S[2 * kt + (x >> 1)][(x & 1) * 2], S[2 * kt + (x >> 1)][(x & 1) * 2 + 1], hi4[kt & 1][x], lo4[kt & 1][x]);
+    // S K^T for this part's tokens, high and low terms of S apart so that the sums take turns. S's terms go to the outputs and to the
+    // other part, whose columns' products come second, when its terms are there. Conversions and loads of the next step stand between the
+    // products of this one: a warp's instructions issue in order, and a product holds its pipe for 8 clocks.
+    float high[PARTS][NO][4] = {}, low[PARTS][NO][4] = {};
+    auto s_term = [&](int kt, int x, uint32_t& h, uint32_t& l) {
+      ld_split(S[2 * kt + (x >> 1)][(x & 1) * 2], S[2 * kt + (x >> 1)][(x & 1) * 2 + 1], h, l);
     };
+    auto products = [&](int who, int step, const uint32_t (&h)[4], const uint32_t (&l)[4], auto&& between) {
+      const auto& k = k4[step & 1];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) s_terms(0, x);
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      const auto& k = k4[kt & 1];
-      *(uint4*)(s_place + ((part * KT + kt) * 32 + lane) * 16) = make_uint4(hi4[kt & 1][0], hi4[kt & 1][1], hi4[kt & 1][2], hi4[kt & 1][3]);
-#pragma unroll
-      for (int x = 0; x < 2 * NT; ++x) {
-        const int n = x % NT;
+      for (int x = 0; x < 2 * NO; ++x) {
+        const int n = x % NO;
         if (DELTA) {
-          if (x < NT)
-            ld_mma(R[n], hi4[kt & 1], k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
+          if (x < NO)
+            ld_mma(high[who][n], h, k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
           else
-            ld_mma(low[n], lo4[kt & 1], k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
+            ld_mma(low[who][n], l, k[n / 2][n % 2 * 2], k[n / 2][n % 2 * 2 + 1]);
         }
-        if (kt + 1 < KT) {
-          if (x % 4 == 1) s_terms(kt + 1, x / 4);
-          if (DELTA && x % 4 == 3) get_k(kt + 1, x / 4);
+        between(x);
+      }
+    };
+    float other_down[2] = {0.0f, 0.0f};
+    auto publish_scales = [&] {
+      if (cc == 0) {
+        float* const s_scales = (float*)(s_place + Shape::TERMS) + part * 16;
+        s_scales[g] = down[0], s_scales[g + 8] = down[1];
+      }
+      ld_arrive(&s_full[team][odd], lane);
+    };
+    if constexpr (PARTS == 1) {
+      uint32_t h4[2][4], l4[2][4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s_term(0, x, h4[0][x], l4[0][x]);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        *(uint4*)(s_place + (kt * 32 + lane) * 16) = make_uint4(h4[kt & 1][0], h4[kt & 1][1], h4[kt & 1][2], h4[kt & 1][3]);
+        products(0, kt, h4[kt & 1], l4[kt & 1], [&](int x) {
+          if (kt + 1 < KT) {
+            if (x % 4 == 1) s_term(kt + 1, x / 4, h4[(kt + 1) & 1][x / 4], l4[(kt + 1) & 1][x / 4]);
+            if (DELTA && x % 4 == 3) get_k(kt + 1, kt + 1, x / 4);
+          }
+        });
+      }
+      publish_scales();
+      if (i > 0) ok = ld_wait(&r_empty[team], (i - 1) & 1);
+      if (!ok) break;
+    } else {
+      uint32_t h4[KT][4], l4[KT][4];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s_term(kt, x, h4[kt][x], l4[kt][x]);
+        uint4* const to = (uint4*)s_place + (part * KT + kt) * 32 + lane;
+        to[0] = make_uint4(h4[kt][0], h4[kt][1], h4[kt][2], h4[kt][3]);
+        to[DK * 2] = make_uint4(l4[kt][0], l4[kt][1], l4[kt][2], l4[kt][3]);
+      }
+      publish_scales();
+      const int other = (1 - part) * KT;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        products(0, kt, h4[kt], l4[kt], [&](int x) {
+          if (DELTA && x % 4 == 3) get_k(kt + 1, kt + 1 < KT ? part * KT + kt + 1 : other, x / 4);
+        });
+      ok = mbar_wait(&s_full[team][odd], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (DELTA) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const uint4* const from = (const uint4*)s_place + (other + kt) * 32 + lane;
+          const uint4 h = from[0], l = from[DK * 2];
+          h4[kt][0] = h.x, h4[kt][1] = h.y, h4[kt][2] = h.z, h4[kt][3] = h.w;
+          l4[kt][0] = l.x, l4[kt][1] = l.y, l4[kt][2] = l.z, l4[kt][3] = l.w;
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+          products(PARTS - 1, KT + kt, h4[kt], l4[kt], [&](int x) {
+            if (kt + 1 < KT && x % 4 == 3) get_k(KT + kt + 1, other + kt + 1, x / 4);
+          });
+        const float* const s_scales = (const float*)(s_place + Shape::TERMS) + (1 - part) * 16;
+        other_down[0] = s_scales[g], other_down[1] = s_scales[g + 8];
       }
     }
-    if (cc == 0) {
-      float* const s_scales = (float*)(s_place + DK * 32) + part * 16;
-      s_scales[g] = down[0], s_scales[g + 8] = down[1];
-    }
-    ld_arrive(&s_full[team][odd], lane);
-    // R = V - gamma K S^T, zeros for the tokens of other lines
-    float2 f[NT];
-    {
-      uint32_t v4[NT / 2][4];
-#pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
-        ld_matrix4_trans(v4[n / 2], v_s + token * 32 + piece * 16);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int j = n * 8 + cc * 2;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        f[n] = *(const float2*)(head.kt_scale + j);
-        if (part == 0) {  // v is the first part's to add
-          TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
-          TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
-        }
-        if (DELTA) {
-          const float2 in = *(const float2*)(head.r_in + j);
-          const float i0 = -in.x * down[0], i1 = -in.y * down[0], i2 = -in.x * down[1], i3 = -in.y * down[1];
-          v[0] = fmaf(R[n][0] + low[n][0], i0, v[0]), v[1] = fmaf(R[n][1] + low[n][1], i1, v[1]);
-          v[2] = fmaf(R[n][2] + low[n][2], i2, v[2]), v[3] = fmaf(R[n][3] + low[n][3], i3, v[3]);
-        } else if (part > 0) {
-          TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
-          TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
-        }
-        if (partial) {
-          if (j < lo || j >= hi) v[0] = v[2] = f[n].x = 0.0f;
-          if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f[n].y = 0.0f;
-        }
-#pragma unroll
-        for (int y = 0; y < 4; ++y) R[n][y] = v[y];
-      }
-    }
+    // K~'s first columns; R = V - gamma K S^T of this part's tokens, zeros for those of other lines; R times K~'s factors
     uint32_t b_hi[2][G / 2][4], b_lo[2][G / 2][4];
-    auto get_b = [&](int at, int x) {  // of the G columns and 16 tokens of step `at`
-      const int where = ld_at<PIECES>(at / (NK / G) * 16 + (lane & 15), part * NK + at % (NK / G) * G + x / 2 * 2 + (lane >> 4));
+    constexpr int KR = LD_C / 16 / PARTS, STEPS = LD_C / 16 * (NK / G);
+    auto get_b = [&](int at, int x) {  // step `at`: G columns of this part, 16 tokens, its own first
+      const int group = at / (LD_C / 16), kt = (at % (LD_C / 16) + part * KR) % (LD_C / 16);
+      const int where = ld_at<PIECES>(kt * 16 + (lane & 15), part * NK + group * G + x / 2 * 2 + (lane >> 4));
       if (x % 2) ld_matrix4_trans(b_hi[at & 1][x / 2], head.kt_hi + where);
       else ld_matrix4_trans(b_lo[at & 1][x / 2], head.kt_lo + where);
     };
-    if constexpr (DELTA && PARTS > 1) {  // the parts' shares: each has the sum of both
-      float4* const mine = (float4*)(place + Shape::SHARES + (odd * PARTS + part) * LD_C * 64) + lane;
-      const float4* const theirs = (const float4*)(place + Shape::SHARES + (odd * PARTS + 1 - part) * LD_C * 64) + lane;
+    float R[NO][4], RK[NO][4], m_r[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+    {
+      uint32_t v4[NO / 2][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mine[n * 32] = make_float4(R[n][0], R[n][1], R[n][2], R[n][3]);
-      ld_arrive(&shares[team][part][odd], lane);
-#pragma unroll
-      for (int x = 0; x < G; ++x) get_b(0, x);
-      ok = mbar_wait(&shares[team][1 - part][odd], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float4 y = theirs[n * 32];
-        R[n][0] += y.x, R[n][1] += y.y, R[n][2] += y.z, R[n][3] += y.w;
+      for (int n = 0; n < NO; n += 2) {
+        const int token = (part * NO + n) * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
+        ld_matrix4_trans(v4[n / 2], v_s + token * 32 + piece * 16);
       }
-    } else {
 #pragma unroll
-      for (int x = 0; x < G; ++x) get_b(0, x);
-      if (i > 0) ok = ld_wait(&r_empty[team], (i - 1) & 1);
-      if (!ok) break;
-    }
-    float m_r[2] = {0.0f, 0.0f};
+      for (int n = 0; n < NO; ++n) {
+        const int j = (part * NO + n) * 8 + cc * 2;
+        float v[4];
+        float2 f = *(const float2*)(head.kt_scale + j);
+        TT::get2(v4[n / 2][n % 2 * 2], v[0], v[1]);
+        TT::get2(v4[n / 2][n % 2 * 2 + 1], v[2], v[3]);
+        if (DELTA) {
+          const float2 in = *(const float2*)(head.r_in + j);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m_r[0] = fmaxf(m_r[0], fmaxf(fabsf(R[n][0]), fabsf(R[n][1])));
-      m_r[1] = fmaxf(m_r[1], fmaxf(fabsf(R[n][2]), fabsf(R[n][3])));
+          for (int y = 0; y < 4; ++y) {
+            float ks = (high[0][n][y] + low[0][n][y]) * down[y >> 1];
+            if (PARTS > 1) ks = fmaf(high[PARTS - 1][n][y] + low[PARTS - 1][n][y], other_down[y >> 1], ks);
+            v[y] = fmaf(-ks, y & 1 ? in.y : in.x, v[y]);
+          }
+        }
+        if (partial) {
+          if (j < lo || j >= hi) v[0] = v[2] = f.x = 0.0f;
+          if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f.y = 0.0f;
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          R[n][y] = v[y], RK[n][y] = v[y] * (y & 1 ? f.y : f.x);
+          m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
+          m[y >> 1] = fmaxf(m[y >> 1], fabsf(RK[n][y]));
+        }
+        if (n < G) get_b(0, n);
+      }
+      if (NO < G)
+#pragma unroll
+        for (int n = NO; n < G; ++n) get_b(0, n);
     }
-    // S = gamma_last S + R^T K~, in S's scale: R times K~'s rows, which are below 2^15 and mostly near 2^7, must not pass it. Where
-    // that is not certain, or S nearly vanishes, in one that suits the larger of the two.
+    // R's terms: one, for the outputs; two, with K~'s factors, for this part's columns and the other's. Each part's tokens have a scale.
+    uint32_t h4[LD_C / 16][4], l4[LD_C / 16][4];
+    float rk_down[PARTS][2];
+    {
+      float uu[2], ud[2], up[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        ld_scale(ld_row_most(m[r]), up[r], rk_down[0][r]);
+        ld_scale(ld_row_most(m_r[r]), uu[r], ud[r]);
+      }
+#pragma unroll
+      for (int kt = 0; kt < KR; ++kt) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int n = 2 * kt + (x >> 1), y = x & 1;
+          ld_split(RK[n][2 * y] * up[y], RK[n][2 * y + 1] * up[y], h4[kt][x], l4[kt][x]);
+        }
+        if (PARTS > 1) {
+          uint4* const to = (uint4*)(place + Shape::RK) + (part * KR + kt) * 64 + lane;
+          to[0] = make_uint4(h4[kt][0], h4[kt][1], h4[kt][2], h4[kt][3]);
+          to[32] = make_uint4(l4[kt][0], l4[kt][1], l4[kt][2], l4[kt][3]);
+        }
+        *(uint4*)(place + Shape::R + ((part * KR + kt) * 32 + lane) * 16) =
+            make_uint4(ld_half2(R[2 * kt][0] * uu[0], R[2 * kt][1] * uu[0]), ld_half2(R[2 * kt][2] * uu[1], R[2 * kt][3] * uu[1]),
+                       ld_half2(R[2 * kt + 1][0] * uu[0], R[2 * kt + 1][1] * uu[0]),
+                       ld_half2(R[2 * kt + 1][2] * uu[1], R[2 * kt + 1][3] * uu[1]));
+      }
+      if (cc == 0) {
+        float* const r_scales = (float*)(place + Shape::R_SCALES) + part * 16;
+        float* const rk_scales = (float*)(place + Shape::RK_SCALES) + part * 16;
+        r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
+        rk_scales[g] = rk_down[0][0], rk_scales[g + 8] = rk_down[0][1];
+      }
+      ld_arrive(&r_full[team], lane);
+    }
+    // S = gamma_last S + R^T K~, G columns at a time, each part's tokens in a sum of their own
     const float gamma = head.gamma[hi - 1];
-    float up[2], g2[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      m_r[r] = ld_row_most(m_r[r]);
-      const float added = m_r[r] * head.kt_most * 0x1p7f, kept = gamma * m_s[r] * down[r];
-      float dn = down[r];
-      up[r] = ld_inverse(dn);
-      if (!(kept * up[r] >= 0x1p10f && added * up[r] < 0x1p15f)) ld_scale(fmaxf(kept, added), up[r], dn);
-      g2[r] = gamma * fminf(down[r] * up[r], LD_MAX);
-      down[r] = dn;
-    }
-#pragma unroll
-    for (int n = 0; n < NK; ++n) S[n][0] *= g2[0], S[n][1] *= g2[0], S[n][2] *= g2[1], S[n][3] *= g2[1];
-    float small[G][4] = {};  // the products of one low term, in sums of their own for the first G columns: more take turns
-    auto r_terms = [&](int kt, int x) {
-      const int n = 2 * kt + (x >> 1), y = x & 1;
-      ld_split(R[n][2 * y] * (f[n].x * up[y]), R[n][2 * y + 1] * (f[n].y * up[y]), hi4[kt & 1][x], lo4[kt & 1][x]);
-    };
-#pragma unroll
-    for (int x = 0; x < 4; ++x) r_terms(0, x);
-    float uu[2], ud[2];
     bool next = true;
 #pragma unroll
-    for (int kt = 0; kt < LD_C / 16; ++kt) {
+    for (int group = 0; group < NK / G; ++group) {
+      float sum[PARTS][G][4] = {};
 #pragma unroll
-      for (int n = 0; n < NK; n += G) {
-        const int at = kt * (NK / G) + n / G;
+      for (int kt = 0; kt < LD_C / 16; ++kt) {
+        const int at = group * (LD_C / 16) + kt, who = kt / KR;
+        if (PARTS > 1 && kt == KR) {  // the other part's
+          ok = ld_wait(&r_full[team], i & 1);
+#pragma unroll
+          for (int y = 0; y < KR; ++y) {
+            const uint4* const from = (const uint4*)(place + Shape::RK) + ((1 - part) * KR + y) * 64 + lane;
+            const uint4 h = from[0], l = from[32];
+            h4[(KR + y) % (LD_C / 16)][0] = h.x, h4[(KR + y) % (LD_C / 16)][1] = h.y;
+            h4[(KR + y) % (LD_C / 16)][2] = h.z, h4[(KR + y) % (LD_C / 16)][3] = h.w;
+            l4[(KR + y) % (LD_C / 16)][0] = l.x, l4[(KR + y) % (LD_C / 16)][1] = l.y;
+            l4[(KR + y) % (LD_C / 16)][2] = l.z, l4[(KR + y) % (LD_C / 16)][3] = l.w;
+          }
+          const float* const rk_scales = (const float*)(place + Shape::RK_SCALES) + (1 - part) * 16;
+          rk_down[PARTS - 1][0] = rk_scales[g], rk_down[PARTS - 1][1] = rk_scales[g + 8];
+        }
         const auto& bh = b_hi[at & 1];
         const auto& bl = b_lo[at & 1];
-        float (*const less)[4] = n == 0 ? small : S + n;
 #pragma unroll
         for (int x = 0; x < 3 * G; ++x) {
           const int y = x % G;
-          if (x < G) ld_mma(less[y], hi4[kt & 1], bl[y / 2][y % 2 * 2], bl[y / 2][y % 2 * 2 + 1]);
-          else if (x < 2 * G) ld_mma(S[n + y], hi4[kt & 1], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
-          else ld_mma(less[y], lo4[kt & 1], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
-          if (x % 3 == 0 && at + 1 < LD_C / 16 * (NK / G)) get_b(at + 1, x / 3);
-          if (n == 0 && x % (3 * G / 4) == 2 && kt + 1 < LD_C / 16) r_terms(kt + 1, x / (3 * G / 4));
-          // R for the outputs, one term
-          if (kt == 0 && n == 0 && x % 6 == 4) {
-            if (x / 6 < 2) ld_scale(m_r[x / 6], uu[x / 6], ud[x / 6]);
-          }
-          if (kt == 1 && n == 0 && x % 3 == 1) {
-            const int z = x / 3;
-            if (z < LD_C / 16 && z % PARTS == part)
-              *(uint4*)(place + Shape::R + (z * 32 + lane) * 16) =
-                  make_uint4(ld_half2(R[2 * z][0] * uu[0], R[2 * z][1] * uu[0]), ld_half2(R[2 * z][2] * uu[1], R[2 * z][3] * uu[1]),
-                             ld_half2(R[2 * z + 1][0] * uu[0], R[2 * z + 1][1] * uu[0]),
-                             ld_half2(R[2 * z + 1][2] * uu[1], R[2 * z + 1][3] * uu[1]));
-          }
-          if (kt == 2 && n == 0 && x == 1) {
-            if (cc == 0 && part == 0) {
-              float* const r_scales = (float*)(place + Shape::SCALES);
-              r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
-            }
-            ld_arrive(&r_full[team], lane);
-          }
-          if (kt == 2 && n == 0 && x == 3 * G / 2 && i + 1 < chunks) next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1);
+          if (x < G) ld_mma(sum[who][y], h4[kt], bl[y / 2][y % 2 * 2], bl[y / 2][y % 2 * 2 + 1]);
+          else if (x < 2 * G) ld_mma(sum[who][y], l4[kt], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
+          else ld_mma(sum[who][y], h4[kt], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
+          if (x % 3 == 0 && at + 1 < STEPS) get_b(at + 1, x / 3);
+          if (at == STEPS - 1 && x == 3 * G / 2 && i + 1 < chunks)
+            next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1);
         }
       }
+      if (group == 0) {  // where S vanishes beside what is added, in the scale of that: all stays within 32 bits
+        const float most[2] = {fmaxf(rk_down[0][0], rk_down[PARTS - 1][0]), fmaxf(rk_down[0][1], rk_down[PARTS - 1][1])};
+        if (__any_sync(0xffffffffu, most[0] > down[0] * 0x1p50f || most[1] > down[1] * 0x1p50f))
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (most[r] > down[r] * 0x1p50f) {
+              const float f = down[r] * ld_inverse(most[r]);
+              down[r] = most[r];
+#pragma unroll
+              for (int n = 0; n < NK; ++n) S[n][2 * r] *= f, S[n][2 * r + 1] *= f;
+            }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float up = ld_inverse(down[r]);
+        const float c0 = rk_down[0][r] * up, c1 = PARTS > 1 ? rk_down[PARTS - 1][r] * up : 0.0f;
+#pragma unroll
+        for (int n = 0; n < G; ++n)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float& to = S[group * G + n][2 * r + y];
+            to = fmaf(sum[0][n][2 * r + y], c0, to * gamma);
+            if (PARTS > 1) to = fmaf(sum[PARTS - 1][n][2 * r + y], c1, to);
+          }
+      }
     }
-#pragma unroll
-    for (int x = 0; x < G; ++x)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) S[x][y] += small[x][y];
     ld_arrive(&empty[st], lane);
+    next = next && ok;
     ok = __all_sync(0xffffffffu, next);
   }
   if (there && ok)
