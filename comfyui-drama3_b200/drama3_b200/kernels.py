@@ -9,7 +9,10 @@ and every launch goes on the device's current stream, so calls can be captured i
   - `moe_decode` is new: the whole resident decode (gate_up, SwiGLU, down, combine) for 1..16 rows in one pass;
   - `grouped_mma` is new: the grouped kernels on the tensor cores for banks held whole on the GPU;
   - `lines_plan`, `qk_norm_rope` and `lines_attention` are new: the attention half of a decoder layer for lines decoded
-    together, over a paged key/value cache with a prefix that the lines share.
+    together, over a paged key/value cache with a prefix that the lines share;
+  - `lines_conv`, `lines_delta`, `gated_norm` and `add_norm` are new: linear attention with the delta rule over a state of
+    each line, the short convolution in front of it, the norm of its heads with their gate, and the join of a block to its
+    residual with the norms before and after it.
 """
 import ctypes
 import functools
