@@ -6,8 +6,11 @@
 // All in 32 bits, rounded once when stored.
 //
 // Bound by memory: each row is read once and written once, in 16-byte vectors that stay in registers between the sum of
-// squares and the product. Gated rows are short (a head): a group of lanes each, BN_AHEAD rows of a group at a time so that
-// enough loads are in flight, and no block-wide step. Joined rows are long: a block each, whose threads hold one or two vectors.
+// squares and the product. Gated rows are short (a head): a group of lanes each, four rows of a group at a time so that enough
+// loads are in flight (two 35.6, eight 43.9 us in the case below), and no block-wide step. Joined rows are long: a warp each where
+// they are many (a row's loads are in flight together), a block each, whose threads hold one or two vectors, where they are few.
+// Measured (B200, bf16): gated, 8192 tokens of 32 heads of 128 34 us, 5.9 TB/s; joined, 16384 rows of 2048 with a norm after the block
+// and a gate a row 52 us, 5.2 TB/s (a block a row: 73); 16 tokens 1.6 and 1.9 us, latency.
 #pragma once
 
 #include "rows.cuh"
