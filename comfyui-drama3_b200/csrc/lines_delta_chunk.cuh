@@ -4,10 +4,13 @@
 //   U = T R,  R = V - diag(gamma) K S^T,  T = (I + A)^-1 diag(beta),  A_ij = beta_i exp(G_i - G_j) k_i . k_j  (j < i)
 //   O = scale (diag(gamma) Q S^T + P U),  P_ij = exp(G_i - G_j) q_i . k_j  (j <= i)
 //   S <- gamma_last S + U^T D K,          D = diag(exp(G_last - G_j))
-// What depends on the tokens alone is formed for all chunks at once (the preparation): not T itself, but P T and K~ = T^T D K,
-// with which U is never needed: O = scale (diag(gamma) Q S^T + (P T) R), S <- gamma_last S + R^T K~. So the chain from chunk
-// to chunk (the scan) has two products, S -> R -> S. Row j of K~ is what is left at the chunk's end of what token j wrote:
-// beta_j k_j through the later tokens' decays and corrections, which only shrink it. Without the delta rule R = V, T = I.
+// What depends on the tokens alone is formed for all chunks at once (the preparation): not T itself, but P T, K~ = T^T D K and
+// Q~ = diag(gamma) Q - P T diag(gamma) K, with which U is never needed:
+//   O = scale (Q~ S^T + P T V),  S <- gamma_last S + R^T K~
+// So the chain from chunk to chunk (the scan) has two products, S -> R -> S, and an output is what is left of the state and of each v
+// by then: row j of K~ is beta_j k_j through the later tokens' decays and corrections, row i of Q~ gamma_i q_i through the earlier ones',
+// and those only shrink them. (As Q S^T + P T R the outputs are differences of large terms where the chunk overwrites the state.)
+// Without the delta rule R = V, T = I, Q~ = diag(gamma) Q.
 // Exponents are differences that are never above 0, of sums in 64 bits.
 //
 // Chunks are cut from the packed tokens, whatever lines they belong to: entries of two lines are zeros, sums and exponents
@@ -15,9 +18,9 @@
 //
 // Values. k and q become fp16 rows times powers of two, exactly (values below 2^-14 of the row's largest lose what is below
 // 2^-25 of it), and their norms are numbers that results are multiplied by. What is not exact in 16 bits, S, R, T, P and K~, is
-// the sum of two fp16 terms, 22 bits, each row scaled by a power of two of its own; products are summed in 32 bits, and of the
-// four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. For the outputs,
-// which are rounded to 16 bits anyway, the scan takes one term of S, P T and R: 2^-12 of each.
+// the sum of two fp16 or tf32 terms, 22 bits, rows of fp16 scaled by a power of two of their own; products are summed in 32 bits, and
+// of the four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. For the outputs,
+// which are rounded to 16 bits anyway, the scan takes one term of S, Q~ and P T: 2^-12 of each.
 //
 // A value that is not finite reaches the state and the tokens of its own line, in its chunk earlier ones too; one in q its own
 // token only.
@@ -32,15 +35,15 @@ constexpr int LD_C = 64;  // tokens of a chunk
 
 // What the preparation leaves of a chunk for a key head: fp16 rows [64][Dk], 16-byte pieces in the order of ld_at.
 template <int DK> struct alignas(128) LdRows {
-  uint16_t k[LD_C * DK], q[LD_C * DK];
+  uint16_t k[LD_C * DK];
 };
 // ... and for a value head: rows likewise, and factors of the tokens' columns.
 template <int DK> struct alignas(128) LdHead {
   uint16_t kt_hi[LD_C * DK], kt_lo[LD_C * DK];  // K~ [64][Dk], row j times 1 / kt_scale[j]
+  uint16_t q[LD_C * DK];                        // Q~ [64][Dk], row i times 1 / q_scale[i]
   uint16_t p[LD_C * LD_C];                      // P T [64][64], row i times 1 / p_scale[i]
-  float kt_scale[LD_C], p_scale[LD_C];
-  float r_in[LD_C];   // gamma_i |k| factor: of K S^T
-  float q_in[LD_C];   // scale gamma_i |q| factor: of Q S^T
+  float kt_scale[LD_C], q_scale[LD_C], p_scale[LD_C];
+  float r_in[LD_C];  // gamma_i |k| factor: of K S^T
   float gamma[LD_C];
 };
 
@@ -97,19 +100,19 @@ struct LdChunkArgs {
 
 // ---- The preparation. A CTA per chunk and value head; the first of a key head's leaves the rows. K K^T and Q K^T are mma.sync
 // products. T: the 16 x 16 blocks on the diagonal of I + A are inverted by columns, a thread each, then blocks of 32 and of 64 by
-// [T1, 0; X, T2], X = -T2 A21 T1, in 32 bits. (By columns of all 64 at once the same numbers took 2000 unrolled steps and the
-// time went into fetching instructions.) K~ = T^T D K and P T are products of two fp16 terms each.
+// [T1, 0; X, T2], X = -T2 A21 T1, in tf32 terms. (By columns of all 64 at once the same numbers took 2000 unrolled steps and the time
+// went into fetching instructions.) P T in tf32 terms too, whose range of exponents needs no scales; Q~ and K~ in fp16 terms.
+// Bound by instructions and their latency, 0.41 of the issue slots with four CTAs an SM: 32 chunks of 32 value heads 70 us (B200), of
+// which P T and Q~, whose longest rows are one warp's, take 20.
 constexpr int LD_PREP_THREADS = 128;
-constexpr int LD_PITCH = 68;    // floats of a row of A and T in shared memory
-constexpr int LD_PITCH_Y = 40;  // ... of A21 T1
+constexpr int LD_PITCH = 68;  // floats of a row of A and T in shared memory
 constexpr float LD_MAX = 3.4028234e38f;
 
 template <int DK> struct LdPrepShape {
-  static constexpr int K = LD_C * DK * 2, T = 2 * LD_C * LD_C * 2;
-  static constexpr int Q = K > T ? K : T;  // the rows of q; A21 T1; T^T; K~'s low terms
-  static constexpr int A = LD_C * LD_PITCH * 4 > K ? LD_C * LD_PITCH * 4 : K;  // A and T; T^T D; K~'s high terms
-  static constexpr int SMEM = K + Q + A;
-  static_assert(A >= T && Q >= 32 * LD_PITCH_Y * 4, "");
+  static constexpr int K = LD_C * DK * 2;          // the rows of k, K~'s low terms; the rows of q, Q~
+  static constexpr int A = LD_C * LD_PITCH * 4;  // A and T, A21 T1 above them; T^T D, two terms; K~'s high terms
+  static constexpr int SMEM = 2 * K + A;
+  static_assert(A >= K && A >= 2 * LD_C * LD_C * 2, "");
 };
 
 D3_DEV void ld_mma_tf32(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
@@ -155,11 +158,11 @@ template <int N, int TILES> D3_DEV void ld_join(float* A, float* Y, unsigned lon
     for (int n = 0; n < TILES; ++n)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        *(float2*)(Y + (row + g + r * 8) * LD_PITCH_Y + col + n * 8 + cc * 2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
+        *(float2*)(Y + (row + g + r * 8) * LD_PITCH + col + n * 8 + cc * 2) = make_float2(acc[n][2 * r], acc[n][2 * r + 1]);
   }
   __syncthreads();
   float acc[TILES][4] = {};
-  ld_product<N / 8, TILES>(acc, A + (r0 + N + row) * LD_PITCH + r0 + N, LD_PITCH, Y + col, LD_PITCH_Y, lane);
+  ld_product<N / 8, TILES>(acc, A + (r0 + N + row) * LD_PITCH + r0 + N, LD_PITCH, Y + col, LD_PITCH, lane);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = r0 + N + row + g + r * 8;
@@ -200,14 +203,13 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   extern __shared__ __align__(128) uint8_t ld_smem[];
   uint16_t* const ks = (uint16_t*)ld_smem;
   uint16_t* const qs = (uint16_t*)(ld_smem + Shape::K);
-  float* const A = (float*)(ld_smem + Shape::K + Shape::Q);  // A, then T
-  float* const Y = (float*)qs;                               // A21 T1, when q has been read
-  uint16_t* const tt = qs;                                   // T^T, two terms, after that
-  uint16_t* const td = (uint16_t*)A;                         // T^T D, two terms, when T has been read
+  float* const A = (float*)(ld_smem + 2 * Shape::K);  // A, then T
+  float* const Y = A + LD_C / 2;                      // A21 T1, in the upper right quarter, of which T has nothing
+  uint16_t* const td = (uint16_t*)A;                  // T^T D, two terms, when T has been read
   __shared__ __align__(8) uint64_t arrived;
   __shared__ int line_s[LD_C];
   __shared__ uint32_t starts_s[2];
-  __shared__ __align__(16) float d_s[LD_C], t_scale[LD_C], k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], kt_scale[LD_C];
+  __shared__ __align__(16) float d_s[LD_C], r_in_s[LD_C], k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], kt_scale[LD_C], q_scale_s[LD_C];
   __shared__ double sum_s;
   __shared__ float2 G_s[LD_C];  // as the sum of two
   __shared__ int bad_s[LD_C];   // by a line's first token in the chunk: something of it is not finite
@@ -300,7 +302,6 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   if (h == hk * many && tid == 0) {  // the rows, as every value head's scan reads them
     LdRows<DK>* rows = (LdRows<DK>*)c.rows + (size_t)block * a.Hk + hk;
     ld_bulk_out(rows->k, ks, sizeof(rows->k));
-    ld_bulk_out(rows->q, qs, sizeof(rows->q));
     ld_bulk_commit();
   }
   // sums of the log decays that start again with each line
@@ -350,11 +351,12 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   if (tid < LD_C) {
     const float2 Gl = G_s[last], Gi = G_s[tid];
     d_s[tid] = my_line >= 0 ? ld_exp((Gl.x - Gi.x) + (Gl.y - Gi.y)) * k_factor[tid] : 0.0f;
+    r_in_s[tid] = my_line >= 0 ? ld_exp(Gi.x + Gi.y) * k_factor[tid] : 0.0f;
   }
+  int from[2];  // the first token of the row's line
   {
     float qf[2], kf[2];
     float2 Gi[2];
-    int from[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int i = warp * 16 + g + r * 8;
@@ -386,7 +388,6 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
         }
       }
   }
-  if (tid == 0) ld_bulk_read();  // the rows of q are on their way
   __syncthreads();
   float most[2] = {0.0f, 0.0f};
   bool good[2] = {true, true};
@@ -414,93 +415,34 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
       for (int i = 0; i < 16; ++i) A[(d + i) * LD_PITCH + d + j] = first_of(d + i) == from ? x[i] : 0.0f;
     }
     __syncthreads();
-    ld_join<16, 1>(A, Y + (warp >> 1) * 16 * LD_PITCH_Y, starts, (warp >> 1) * 32, 0, (warp & 1) * 8, lane);
+    ld_join<16, 1>(A, Y + (warp >> 1) * 16 * LD_PITCH, starts, (warp >> 1) * 32, 0, (warp & 1) * 8, lane);
     ld_join<32, 2>(A, Y, starts, 0, (warp >> 1) * 16, (warp & 1) * 16, lane);
-    {  // columns of T become rows of T^T and T^T D: two threads each, four rows by turns
-      const int j = tid >> 1, half = tid & 1;
-      const float b = beta_s[j];
-      float v[32], d[32], m_t = 0.0f, m_d = 0.0f, sum = 0.0f;
+    // P T: a warp has 16 rows, in steps of 8 columns of P; two neighbouring columns of an accumulator are columns cc and cc + 4 of a
+    // tf32 operand, with T's rows taken in that order
+    float tp[8][4] = {};
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const int i = e * 2 + half * 4;
-        const float4 d4 = *(const float4*)(d_s + i);
-        const float ds[4] = {d4.x, d4.y, d4.z, d4.w};
+    for (int m = 0; m < 8; ++m)
+      if (m <= 2 * warp + 1) {
+        uint32_t hi[4], lo[4];
+        ld_split_tf32(p[m][0], hi[0], lo[0]), ld_split_tf32(p[m][2], hi[1], lo[1]);
+        ld_split_tf32(p[m][1], hi[2], lo[2]), ld_split_tf32(p[m][3], hi[3], lo[3]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          v[e + x] = A[(i + x) * LD_PITCH + j] * b;
-          d[e + x] = v[e + x] != 0.0f ? v[e + x] * ds[x] : 0.0f;  // nothing of another line, where that is not finite
-          sum += fabsf(d[e + x]);                               // finite where all are
+        for (int n = 0; n <= m; ++n) {
+          uint32_t b_hi[2], b_lo[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) ld_split_tf32(A[(m * 8 + cc * 2 + e) * LD_PITCH + n * 8 + g], b_hi[e], b_lo[e]);
+          ld_mma_tf32(tp[n], lo, b_hi);
+          ld_mma_tf32(tp[n], hi, b_lo);
+          ld_mma_tf32(tp[n], hi, b_hi);
         }
-        m_t = fmaxf(m_t, fmaxf(fmaxf(fabsf(v[e]), fabsf(v[e + 1])), fmaxf(fabsf(v[e + 2]), fabsf(v[e + 3]))));
-        m_d = fmaxf(m_d, fmaxf(fmaxf(fabsf(d[e]), fabsf(d[e + 1])), fmaxf(fabsf(d[e + 2]), fabsf(d[e + 3]))));
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      m_t = fmaxf(m_t, __shfl_xor_sync(0xffffffffu, m_t, 1));
-      m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
-      if (!(sum <= LD_MAX && m_t <= LD_MAX)) {
-        bad_s[first_of(j)] = 1;
-        m_t = m_d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = d[e] = 0.0f;
-      }
-      float up_t, up_d, down;
-      ld_scale(m_t, up_t, down);
-      if (half == 0) t_scale[j] = down;
-      ld_scale(m_d, up_d, down);
-      if (half == 0) kt_scale[j] = m_d > 0.0f ? down * 0x1p6f : 0.0f;  // a row of zeros must not set a scale
-      __syncthreads();                                                  // T has been read
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        uint2 hi, lo;
-        const int at = ld_at<8>(j, e >> 2) + half * 4;
-        ld_split(v[e] * up_t, v[e + 1] * up_t, hi.x, lo.x), ld_split(v[e + 2] * up_t, v[e + 3] * up_t, hi.y, lo.y);
-        *(uint2*)(tt + at) = hi, *(uint2*)(tt + LD_C * LD_C + at) = lo;
-        ld_split(d[e] * up_d, d[e + 1] * up_d, hi.x, lo.x), ld_split(d[e + 2] * up_d, d[e + 3] * up_d, hi.y, lo.y);
-        *(uint2*)(td + at) = hi, *(uint2*)(td + LD_C * LD_C + at) = lo;
-      }
-    }
-    __syncthreads();
-    // P T: a warp has 16 rows
-    float tp[8][4] = {}, up[2], down[2];
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (!(fabsf(p[n][e]) <= LD_MAX)) good[e >> 1] = false, p[n][e] = 0.0f;
-        most[e >> 1] = fmaxf(most[e >> 1], fabsf(p[n][e]));
+        const int j = n * 8 + cc * 2 + (e & 1), i = warp * 16 + g + (e >> 1) * 8;  // zeros for other lines whatever the sums met
+        p[n][e] = j >= from[e >> 1] && j <= i ? tp[n][e] * beta_s[j] : 0.0f;
       }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], o));
-      ld_scale(most[r], up[r], down[r]);
-      most[r] = 0.0f;
-    }
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-      if (m <= warp) {
-        uint32_t hi[4], lo[4];
-        ld_split(p[2 * m][0] * up[0], p[2 * m][1] * up[0], hi[0], lo[0]);
-        ld_split(p[2 * m][2] * up[1], p[2 * m][3] * up[1], hi[1], lo[1]);
-        ld_split(p[2 * m + 1][0] * up[0], p[2 * m + 1][1] * up[0], hi[2], lo[2]);
-        ld_split(p[2 * m + 1][2] * up[1], p[2 * m + 1][3] * up[1], hi[3], lo[3]);
-#pragma unroll
-        for (int n = 0; n <= 2 * m; n += 2) {
-          uint32_t b_hi[4], b_lo[4];
-          const int at = ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, m * 2 + ((lane >> 3) & 1));
-          ld_matrix4(b_hi, tt + at);
-          ld_matrix4(b_lo, tt + LD_C * LD_C + at);
-          ld_mma(tp[n], lo, b_hi[0], b_hi[1]), ld_mma(tp[n + 1], lo, b_hi[2], b_hi[3]);
-          ld_mma(tp[n], hi, b_lo[0], b_lo[1]), ld_mma(tp[n + 1], hi, b_lo[2], b_lo[3]);
-          ld_mma(tp[n], hi, b_hi[0], b_hi[1]), ld_mma(tp[n + 1], hi, b_hi[2], b_hi[3]);
-        }
-      }
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 f = *(const float2*)(t_scale + n * 8 + cc * 2);
-      p[n][0] = tp[n][0] * (f.x * down[0]), p[n][1] = tp[n][1] * (f.y * down[0]);
-      p[n][2] = tp[n][2] * (f.x * down[1]), p[n][3] = tp[n][3] * (f.y * down[1]);
-    }
   }
   // the rows of P T (of P) out, one term
 #pragma unroll
@@ -524,8 +466,108 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     for (int n = 0; n < 8; ++n)
       *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(p[n][r * 2] * up, p[n][r * 2 + 1] * up);
   }
+  float q_base[2];  // of Q's rows
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = warp * 16 + g + r * 8;
+    q_base[r] = ld_exp(G_s[i].x + G_s[i].y) * q_factor[i];
+  }
+  if constexpr (DELTA) {
+    // Q~ = gamma Q - (P T) gamma K in Q's place, its rows below 2^15: what is taken off only shrinks them, and single values of them
+    // grow by sqrt(Dk) at most
+    float m[2] = {0.0f, 0.0f}, up[2], down[2], q_up[2], q_down[2];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 f = *(const float2*)(r_in_s + n * 8 + cc * 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[n][e] = p[n][e] != 0.0f ? p[n][e] * (e & 1 ? f.y : f.x) : 0.0f;  // nothing of another line, where that is not finite
+        m[e >> 1] = fmaxf(m[e >> 1], fabsf(p[n][e]));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], o));
+      ld_scale(m[r], up[r], down[r]);
+      ld_scale(q_base[r], q_up[r], q_down[r]);
+      if (cc == 0) q_scale_s[warp * 16 + g + r * 8] = q_base[r] == 0.0f ? 0.0f : q_down[r] * 0x1p5f;
+    }
+    uint32_t hi[4][4], lo[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ld_split(p[2 * j][0] * up[0], p[2 * j][1] * up[0], hi[j][0], lo[j][0]);
+      ld_split(p[2 * j][2] * up[1], p[2 * j][3] * up[1], hi[j][1], lo[j][1]);
+      ld_split(p[2 * j + 1][0] * up[0], p[2 * j + 1][1] * up[0], hi[j][2], lo[j][2]);
+      ld_split(p[2 * j + 1][2] * up[1], p[2 * j + 1][3] * up[1], hi[j][3], lo[j][3]);
+    }
+#pragma unroll
+    for (int n0 = 0; n0 < PIECES; n0 += 4) {
+      float acc[4][4] = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= warp)
+#pragma unroll
+          for (int n = 0; n < 4; n += 2) {
+            uint32_t b[4];
+            ld_matrix4_trans(b, ks + ld_at<PIECES>(j * 16 + (lane & 15), n0 + n + (lane >> 4)));
+            ld_mma(acc[n], lo[j], b[0], b[1]), ld_mma(acc[n + 1], lo[j], b[2], b[3]);
+            ld_mma(acc[n], hi[j], b[0], b[1]), ld_mma(acc[n + 1], hi[j], b[2], b[3]);
+          }
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t* const at = (uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2);
+          const uint32_t w = *at;
+          const float f = q_up[r] * 0x1p-5f;
+          *at = ld_half2((q_base[r] * h_lo(w) - acc[n][2 * r] * down[r]) * f, (q_base[r] * h_hi(w) - acc[n][2 * r + 1] * down[r]) * f);
+        }
+    }
+    {  // columns of T become rows of T^T D: two threads each, four rows by turns
+      const int j = tid >> 1, half = tid & 1;
+      const float b = beta_s[j];
+      float d[32], m_d = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const int i = e * 2 + half * 4;
+        const float4 d4 = *(const float4*)(d_s + i);
+        const float ds[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float v = i + x >= j ? A[(i + x) * LD_PITCH + j] * b : 0.0f;
+          d[e + x] = v != 0.0f ? v * ds[x] : 0.0f;  // nothing of another line, where that is not finite
+          sum += fabsf(d[e + x]);                   // finite where all are
+        }
+        m_d = fmaxf(m_d, fmaxf(fmaxf(fabsf(d[e]), fabsf(d[e + 1])), fmaxf(fabsf(d[e + 2]), fabsf(d[e + 3]))));
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      m_d = fmaxf(m_d, __shfl_xor_sync(0xffffffffu, m_d, 1));
+      if (!(sum <= LD_MAX)) {
+        bad_s[first_of(j)] = 1;
+        m_d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) d[e] = 0.0f;
+      }
+      float up_d, down_d;
+      ld_scale(m_d, up_d, down_d);
+      if (half == 0) kt_scale[j] = m_d > 0.0f ? down_d * 0x1p6f : 0.0f;  // a row of zeros must not set a scale
+      __syncthreads();                                                    // T has been read
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        uint2 h2, l2;
+        const int at = ld_at<8>(j, e >> 2) + half * 4;
+        ld_split(d[e] * up_d, d[e + 1] * up_d, h2.x, l2.x), ld_split(d[e + 2] * up_d, d[e + 3] * up_d, h2.y, l2.y);
+        *(uint2*)(td + at) = h2, *(uint2*)(td + LD_C * LD_C + at) = l2;
+      }
+    }
+  } else if (cc == 0) {
+    q_scale_s[warp * 16 + g] = q_base[0], q_scale_s[warp * 16 + g + 8] = q_base[1];
+  }
+  if (tid == 0) ld_bulk_read();  // the rows of k are on their way
+  __syncthreads();
   uint16_t* const kt_hi = (uint16_t*)A;
-  uint16_t* const kt_lo = qs;
+  uint16_t* const kt_lo = ks;
   if constexpr (DELTA) {
     // K~ = T^T D K: a warp has Dk / 4 columns
     constexpr int N = DK / 32;
@@ -551,7 +593,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
         for (int n = 0; n < N; ++n) ld_mma(kt[j][n], hi, b[n][0], b[n][1]);
       }
     }
-    __syncthreads();  // T^T D and T^T have been read
+    __syncthreads();  // T^T D and the rows of k have been read
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -572,7 +614,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
       float up, down;
       ld_scale(finite ? fabsf(d_s[j]) : 1.0f, up, down);
       const float f = finite ? d_s[j] * up * 0x1p-7f : 0.0f;
-      uint4 hi, lo;
+      uint4 hi, lo;  // the low ones in the piece's own place
       ld_split(h_lo(raw.x) * f, h_hi(raw.x) * f, hi.x, lo.x), ld_split(h_lo(raw.y) * f, h_hi(raw.y) * f, hi.y, lo.y);
       ld_split(h_lo(raw.z) * f, h_hi(raw.z) * f, hi.z, lo.z), ld_split(h_lo(raw.w) * f, h_hi(raw.w) * f, hi.w, lo.w);
       ((uint4*)kt_hi)[i] = hi, ((uint4*)kt_lo)[i] = lo;
@@ -590,40 +632,41 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   if (tid == 0) {
     ld_bulk_out(out->kt_hi, kt_hi, sizeof(out->kt_hi));
     ld_bulk_out(out->kt_lo, kt_lo, sizeof(out->kt_lo));
+    ld_bulk_out(out->q, qs, sizeof(out->q));
     ld_bulk_commit();
   }
   if (tid < LD_C) {
-    const float nan = __uint_as_float(0x7fc00000u), gamma = ld_exp(G_s[tid].x + G_s[tid].y);
+    const float nan = __uint_as_float(0x7fc00000u);
     const bool bad = bad_s[first] != 0, live = my_line >= 0;
-    out->gamma[tid] = gamma;
+    out->gamma[tid] = ld_exp(G_s[tid].x + G_s[tid].y);
     out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
-    out->r_in[tid] = live && !bad ? gamma * k_factor[tid] : 0.0f;
-    out->q_in[tid] = !live ? 0.0f : bad ? nan : gamma * q_factor[tid];
+    out->r_in[tid] = bad ? 0.0f : r_in_s[tid];
+    out->q_scale[tid] = !live ? 0.0f : bad ? nan : q_scale_s[tid];
   }
   if (tid == 0) ld_bulk_done();
 }
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks. 16 rows are a team of
 // warps: one, or PARTS = 2 that have half of the state's columns and half of the chunk's tokens each, carry the state, S -> R -> S;
-// as many others make the outputs from what those leave in shared memory (S's high terms, R), a step behind, so that their products
+// as many others make the outputs from what those leave in shared memory (S's high terms) and V, a step behind, so that their products
 // fill the tensor core while the first ones' values are being converted. S stays in registers, as the accumulator of products [rows
 // of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand is, so that a single warp's
 // chain has no exchange in it. Two warps give one another their terms of S and of R, and each begins with its own while the other's
-// come. K, Q, K~ and P T, as B operands, come from shared memory, where the first output warp keeps chunks coming (bulk copies; the
+// come. K, Q~, K~ and P T, as B operands, come from shared memory, where the first output warp keeps chunks coming (bulk copies; the
 // rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought there and back between the
 // products: with 16 rows a warp the chain is shorter in registers.)
 //
 // Bound by the chain's latency: 8192 tokens are 128 chunks one after another, and a head's rows are all that can be spread. Measured
-// (B200, 16 / 32 heads of 128, one line): 2.3 us a chunk, 3900 clocks, of which the 160 products of a warp that carries the state take
-// 1330 of its tensor core's time, those of the output warp beside it 350; the rest are conversions (370 for R, 480 for the
+// (B200, 16 / 32 heads of 128, one line): 2.4 us a chunk, 3900 clocks, of which the 160 products of a warp that carries the state take
+// 1330 of its tensor core's time, those of the output warp beside it 350; the rest are conversions (370 for R, 400 for its
 // terms), barriers and the latency of what they wait for. One warp a team with four teams a CTA (which share the operands'
 // loads) takes 3.4 us a chunk and half the SMs: the better where lines and heads fill the GPU.
 template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
   // a team's place: S's terms as A fragments (high ones, and low ones for the other part) with its rows' scales, two chunks' by turns;
-  // R's high terms with theirs; R times K~'s factors, both terms, with theirs, for the other part; the outputs
-  static constexpr int TERMS = DK * 32 * PARTS, S = TERMS + 128, R = 2 * S, R_SCALES = R + LD_C * 32, RK = R_SCALES + 128;
-  static constexpr int RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0), OUT = RK_SCALES + 128, TEAM = OUT + LD_C * 32;
+  // R times K~'s factors, both terms, with their scales, for the other part; the outputs
+  static constexpr int TERMS = DK * 32 * PARTS, S = TERMS + 128, RK = 2 * S, RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0);
+  static constexpr int OUT = RK_SCALES + 128, TEAM = OUT + LD_C * 32;
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024;
   static constexpr int OUTS = PARTS;  // warps for the outputs, each of a share of the tokens: as many on every quarter of an SM
@@ -657,8 +700,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   constexpr int G = NK < 8 ? NK : 8;  // sums of S that take turns
   constexpr int OUTS = Shape::OUTS, NO = NT / OUTS;
   extern __shared__ uint8_t ld_raw[];
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], r_full[WARPS],
-      r_empty[WARPS];  // [2]: odd and even chunks', as their places
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], s_empty[WARPS][2],
+      r_full[WARPS];  // [2]: odd and even chunks', as their places
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -669,8 +712,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + OUTS) * WARPS);
     for (int i = 0; i < WARPS; ++i) {
-      mbar_init(&r_full[i], PARTS), mbar_init(&r_empty[i], OUTS);
-      mbar_init(&s_full[i][0], PARTS), mbar_init(&s_full[i][1], PARTS);
+      mbar_init(&r_full[i], PARTS);
+      for (int y = 0; y < 2; ++y) mbar_init(&s_full[i][y], PARTS), mbar_init(&s_empty[i][y], OUTS);
     }
     fence_mbar_init();
   }
@@ -692,7 +735,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   const int block_a = (int)((s - first_token) / LD_C), chunks = (int)((e - 1 - first_token) / LD_C) - block_a + 1;
   bool ok = true;
   if (outputs) {
-    constexpr uint32_t skip = DELTA ? 0 : sizeof(LdRows<DK>) / 2, row_bytes = sizeof(LdRows<DK>) - skip;  // k is for K S^T
+    constexpr uint32_t row_bytes = DELTA ? sizeof(LdRows<DK>) : 0;  // for K S^T
     const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
     int loads = 0;
     auto load = [&] {  // the next chunk; by one lane, whose stage is free
@@ -701,7 +744,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const size_t block = block_a + loads;
       const uint64_t keep = policy_evict_last();
       mbar_arrive_expect_tx(bar, row_bytes + (uint32_t)sizeof(LdHead<DK>) + v_boxes * LD_C * 32);
-      bulk_g2s(to + skip, (const uint8_t*)((const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk)) + skip, row_bytes, bar, keep);
+      if (DELTA) bulk_g2s(to, (const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk), row_bytes, bar, keep);
       bulk_g2s(to + Shape::HEAD, (const LdHead<DK>*)c.heads + block * a.Hv + h, sizeof(LdHead<DK>), bar, keep);
       for (int w = 0; w < v_boxes; ++w)
         tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h,
@@ -720,8 +763,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         if (ok) load();
       }
       const uint8_t* const stage = ring + st * Shape::STAGE;
-      const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
       const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
+      const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
       const long long t0 = first_token + (long long)(block_a + i) * LD_C;
       const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
       float O[PARTS][NO][4] = {};
@@ -732,7 +775,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         uint32_t q4[NO / 2][4];
 #pragma unroll
         for (int x = 0; x < NO / 2; ++x)
-          ld_matrix4(q4[x], rows.q + ld_at<PIECES>((part * NO + x * 2) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+          ld_matrix4(q4[x], head.q + ld_at<PIECES>((part * NO + x * 2) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
         for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
@@ -748,46 +791,65 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
             if (y > 0) O[0][n][x] = fmaf(O[y][n][x], s_down[x >> 1], O[0][n][x]);
           }
       }
-      ok = ld_wait(&r_full[team], i & 1);
-      if (!ok) break;
-      uint32_t u4[LD_C / 16][4];
+      ld_arrive(&s_empty[team][i & 1], lane);
+      // V as A fragments, fp16 (exactly, but for values of bf16 below 2^-14 of the row's largest, which lose what is below 2^-25 of
+      // that), zeros for the tokens of other lines
+      uint32_t v4[LD_C / 16][4];
+      float v_down[2] = {1.0f, 1.0f};
 #pragma unroll
       for (int kt = 0; kt < LD_C / 16; ++kt) {
-        const uint4 r4 = *(const uint4*)(place + Shape::R + (kt * 32 + lane) * 16);
-        u4[kt][0] = r4.x, u4[kt][1] = r4.y, u4[kt][2] = r4.z, u4[kt][3] = r4.w;
-      }
-      float r_down[PARTS][2];
+        const int token = kt * 16 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
+        ld_matrix4_trans(v4[kt], v_s + token * 32 + piece * 16);
+        if (lo > 0 || hi < LD_C)
 #pragma unroll
-      for (int y = 0; y < PARTS; ++y) {
-        const float* const r_scales = (const float*)(place + Shape::R_SCALES) + y * 16;
-        r_down[y][0] = r_scales[g], r_down[y][1] = r_scales[g + 8];
+          for (int x = 0; x < 4; ++x) {
+            const int j = kt * 16 + (x >> 1) * 8 + cc * 2;
+            if (j < lo || j >= hi) v4[kt][x] &= 0xffff0000u;
+            if (j + 1 < lo || j + 1 >= hi) v4[kt][x] &= 0x0000ffffu;
+          }
       }
-      ld_arrive(&r_empty[team], lane);
+      if constexpr (TYPE == QR_BF16) {
+        float most[2] = {0.0f, 0.0f}, up[2];
+#pragma unroll
+        for (int kt = 0; kt < LD_C / 16; ++kt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float y0, y1;
+            TT::get2(v4[kt][x], y0, y1);
+            most[x & 1] = fmaxf(most[x & 1], fmaxf(fabsf(y0), fabsf(y1)));
+          }
+        ld_scale(ld_row_most(most[0]), up[0], v_down[0]);
+        ld_scale(ld_row_most(most[1]), up[1], v_down[1]);
+#pragma unroll
+        for (int kt = 0; kt < LD_C / 16; ++kt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float y0, y1;
+            TT::get2(v4[kt][x], y0, y1);
+            v4[kt][x] = ld_half2(y0 * up[x & 1], y1 * up[x & 1]);
+          }
+      }
       uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
       for (int m = 0; m < NO; m += 2) {
         const int n = part * NO + m;
-        float pu[PARTS][2][4] = {};
+        float pv[2][4] = {};
 #pragma unroll
         for (int kt = 0; kt < LD_C / 16; ++kt)
           if (kt <= n / 2) {
             uint32_t p4[4];
             ld_matrix4(p4, head.p + ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-            float (&sum)[2][4] = pu[kt / (LD_C / 16 / PARTS)];
-            ld_mma(sum[0], u4[kt], p4[0], p4[1]), ld_mma(sum[1], u4[kt], p4[2], p4[3]);
+            ld_mma(pv[0], v4[kt], p4[0], p4[1]), ld_mma(pv[1], v4[kt], p4[2], p4[3]);
           }
         uint32_t o4[4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int j = (n + x) * 8 + cc * 2;
-          const float2 fq = *(const float2*)(head.q_in + j), fp = *(const float2*)(head.p_scale + j);
+          const float2 fq = *(const float2*)(head.q_scale + j), fp = *(const float2*)(head.p_scale + j);
           float o[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            float from_r = pu[0][x][y] * r_down[0][y >> 1];
-            if (PARTS > 1) from_r = fmaf(pu[PARTS - 1][x][y], r_down[PARTS - 1][y >> 1], from_r);
-            o[y] = fmaf(O[0][m + x][y], y & 1 ? fq.y : fq.x, from_r * (y & 1 ? fp.y : fp.x));
-          }
+          for (int y = 0; y < 4; ++y)
+            o[y] = fmaf(O[0][m + x][y], y & 1 ? fq.y : fq.x, pv[x][y] * v_down[y >> 1] * (y & 1 ? fp.y : fp.x));
           o4[2 * x] = TT::put2(o[0], o[1]), o4[2 * x + 1] = TT::put2(o[2], o[3]);
         }
         const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
@@ -906,8 +968,6 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         });
       }
       publish_scales();
-      if (i > 0) ok = ld_wait(&r_empty[team], (i - 1) & 1);
-      if (!ok) break;
     } else {
       uint32_t h4[KT][4], l4[KT][4];
 #pragma unroll
@@ -925,8 +985,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         products(0, kt, h4[kt], l4[kt], [&](int x) {
           if (DELTA && x % 4 == 3) get_k(kt + 1, kt + 1 < KT ? part * KT + kt + 1 : other, x / 4);
         });
-      ok = mbar_wait(&s_full[team][odd], (i >> 1) & 1) && (i == 0 || mbar_wait(&r_empty[team], (i - 1) & 1));
-      ok = __all_sync(0xffffffffu, ok);
+      ok = ld_wait(&s_full[team][odd], (i >> 1) & 1);
       if (!ok) break;
       if (DELTA) {
 #pragma unroll
@@ -954,7 +1013,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       if (x % 2) ld_matrix4_trans(b_hi[at & 1][x / 2], head.kt_hi + where);
       else ld_matrix4_trans(b_lo[at & 1][x / 2], head.kt_lo + where);
     };
-    float R[NO][4], RK[NO][4], m_r[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+    float RK[NO][4], m[2] = {0.0f, 0.0f};
     {
       uint32_t v4[NO / 2][4];
 #pragma unroll
@@ -984,8 +1043,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         }
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          R[n][y] = v[y], RK[n][y] = v[y] * (y & 1 ? f.y : f.x);
-          m_r[y >> 1] = fmaxf(m_r[y >> 1], fabsf(v[y]));
+          RK[n][y] = v[y] * (y & 1 ? f.y : f.x);
           m[y >> 1] = fmaxf(m[y >> 1], fabsf(RK[n][y]));
         }
         if (n < G) get_b(0, n);
@@ -994,16 +1052,13 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
         for (int n = NO; n < G; ++n) get_b(0, n);
     }
-    // R's terms: one, for the outputs; two, with K~'s factors, for this part's columns and the other's. Each part's tokens have a scale.
+    // its two terms, for this part's columns and the other's. Each part's tokens have a scale.
     uint32_t h4[LD_C / 16][4], l4[LD_C / 16][4];
     float rk_down[PARTS][2];
     {
-      float uu[2], ud[2], up[2];
+      float up[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        ld_scale(ld_row_most(m[r]), up[r], rk_down[0][r]);
-        ld_scale(ld_row_most(m_r[r]), uu[r], ud[r]);
-      }
+      for (int r = 0; r < 2; ++r) ld_scale(ld_row_most(m[r]), up[r], rk_down[0][r]);
 #pragma unroll
       for (int kt = 0; kt < KR; ++kt) {
 #pragma unroll
@@ -1016,18 +1071,14 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           to[0] = make_uint4(h4[kt][0], h4[kt][1], h4[kt][2], h4[kt][3]);
           to[32] = make_uint4(l4[kt][0], l4[kt][1], l4[kt][2], l4[kt][3]);
         }
-        *(uint4*)(place + Shape::R + ((part * KR + kt) * 32 + lane) * 16) =
-            make_uint4(ld_half2(R[2 * kt][0] * uu[0], R[2 * kt][1] * uu[0]), ld_half2(R[2 * kt][2] * uu[1], R[2 * kt][3] * uu[1]),
-                       ld_half2(R[2 * kt + 1][0] * uu[0], R[2 * kt + 1][1] * uu[0]),
-                       ld_half2(R[2 * kt + 1][2] * uu[1], R[2 * kt + 1][3] * uu[1]));
       }
-      if (cc == 0) {
-        float* const r_scales = (float*)(place + Shape::R_SCALES) + part * 16;
-        float* const rk_scales = (float*)(place + Shape::RK_SCALES) + part * 16;
-        r_scales[g] = ud[0], r_scales[g + 8] = ud[1];
-        rk_scales[g] = rk_down[0][0], rk_scales[g + 8] = rk_down[0][1];
+      if (PARTS > 1) {
+        if (cc == 0) {
+          float* const rk_scales = (float*)(place + Shape::RK_SCALES) + part * 16;
+          rk_scales[g] = rk_down[0][0], rk_scales[g + 8] = rk_down[0][1];
+        }
+        ld_arrive(&r_full[team], lane);
       }
-      ld_arrive(&r_full[team], lane);
     }
     // S = gamma_last S + R^T K~, G columns at a time, each part's tokens in a sum of their own
     const float gamma = head.gamma[hi - 1];
@@ -1062,7 +1113,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           else ld_mma(sum[who][y], h4[kt], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
           if (x % 3 == 0 && at + 1 < STEPS) get_b(at + 1, x / 3);
           if (at == STEPS - 1 && x == 3 * G / 2 && i + 1 < chunks)
-            next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1);
+            next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1) &&
+                   (i == 0 || mbar_wait(&s_empty[team][(i + 1) & 1], (((i + 1) >> 1) - 1) & 1));
         }
       }
       if (group == 0) {  // where S vanishes beside what is added, in the scale of that: all stays within 32 bits

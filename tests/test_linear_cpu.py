@@ -61,7 +61,7 @@ def test_delta_refusals(lib, change, status):
 
 def test_delta_workspace(lib):
     assert lib.d3_lines_delta_workspace(16, 16, 16, 32, 128) == 0 and lib.d3_lines_delta_workspace(0, 1, 1, 1, 64) == 0
-    one = 2 * 64 * 128 * 2 + 2 * (2 * 64 * 128 * 2 + 64 * 64 * 2 + 5 * 64 * 4)  # a chunk of one key and two value heads
+    one = 64 * 128 * 2 + 2 * (3 * 64 * 128 * 2 + 64 * 64 * 2 + 5 * 64 * 4)  # a chunk of one key and two value heads
     assert lib.d3_lines_delta_workspace(64, 1, 1, 2, 128) == one and lib.d3_lines_delta_workspace(65, 1, 1, 2, 128) == 2 * one
     # a pass of any length is cut into parts of bounded scratch
     assert lib.d3_lines_delta_workspace(1 << 24, 1, 16, 32, 128) <= 256 << 20

@@ -7,8 +7,9 @@ the value. Every output is rounded once: half a step of it. On top of that:
   of 16 bits) is off by (2 + |y|) 2^-22 of the value, which |y| <= 16 (past that a value is zero or y itself) makes 2^-17.
 - delta: with W_t the size of a row of the state, a chunk's products each sum at most 128 terms in 32 bits (128 x 2^-24 =
   2^-17 of the size) of factors held as two fp16 terms (2^-22 each, 2^-21 both); three such products follow one another, so
-  3 (2^-17 + 2^-21) < 2^-15 for the state and for what an output takes from it. An output's own two products take the state,
-  the corrections and the weights rounded to fp16: 2^-11 of each factor, at most two of them in a product, 2^-10 of the size.
+  3 (2^-17 + 2^-21) < 2^-15 for the state and for what an output takes from it. An output's own two products take the state, what
+  is left of the query and the weights of the values rounded to fp16: 2^-11 of each factor, at most two of them in a product,
+  2^-10 of the size.
 - norms: a mean of D squares in 32 bits is off by (D + 4) 2^-24 of it, its root by half of that, and a dozen operations by
   2^-20: (D / 2 + 16) 2^-24 of the value. The joined sum: 2^-21 of its terms' size plus the norm's share of x's term, and the
   normed row that much of the terms' size over the row's root mean square."""
