@@ -93,11 +93,13 @@ size_t delta_block_bytes(int Hk, int Hv, int Dk) {
                   : Hk * sizeof(d3::LdRows<128>) + Hv * sizeof(d3::LdHead<128>);
 }
 
-// Chunks prepared and scanned by a pair of launches: as many as 256 MB hold. (B200, 8192 tokens of 16 / 32 heads of 128: 438 us in one
-// pair, 469 in parts of 37 chunks, whose 70 MB stay in L2, 714 in parts of 9: the scan starts anew in each.)
+// Chunks prepared and scanned by a pair of launches: as many as 384 MB hold, or equal parts below that. (B200, 8192 tokens of 16 / 32
+// heads of 128, an earlier form of the scan: 438 us in one pair, 469 in parts of 37 chunks, whose 70 MB stay in L2, 714 in parts of 9:
+// the scan starts anew in each.)
 int delta_blocks(int T, int Hk, int Hv, int Dk) {
-  const size_t fit = (256u << 20) / delta_block_bytes(Hk, Hv, Dk), all = ((size_t)T + d3::LD_C - 1) / d3::LD_C;
-  return (int)(all < fit ? all : fit < 8 ? 8 : fit);
+  const size_t all = ((size_t)T + d3::LD_C - 1) / d3::LD_C, most = (384u << 20) / delta_block_bytes(Hk, Hv, Dk);
+  const size_t fit = most < 8 ? 8 : most, parts = (all + fit - 1) / fit;
+  return (int)((all + parts - 1) / parts);
 }
 
 template <int TYPE, int DK, bool DELTA, int WARPS, int PARTS>

@@ -130,7 +130,7 @@ D3_DEV void ld_split_tf32(float x, uint32_t& hi, uint32_t& lo) {
 template <int STEPS, int TILES>
 D3_DEV void ld_product(float (&acc)[TILES][4], const float* x, int px, const float* y, int py, int lane) {
   const int g = lane >> 2, cc = lane & 3;
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < STEPS; ++k) {
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   }
   // K K^T and Q K^T: rows 16 warp + g, + 8, columns 8 n + 2 cc, + 1 up to the diagonal
   float p[8][4] = {}, kk[8][4] = {};
-#pragma unroll
+#pragma unroll 2
   for (int kt = 0; kt < DK / 16; ++kt) {
     uint32_t ak[4], aq[4];
     const int ar = warp * 16 + (lane & 15), ap = kt * 2 + (lane >> 4);
@@ -501,28 +501,33 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
       ld_split(p[2 * j + 1][0] * up[0], p[2 * j + 1][1] * up[0], hi[j][2], lo[j][2]);
       ld_split(p[2 * j + 1][2] * up[1], p[2 * j + 1][3] * up[1], hi[j][3], lo[j][3]);
     }
-#pragma unroll
+    const float q_f[2] = {q_base[0] * q_up[0] * 0x1p-5f, q_base[1] * q_up[1] * 0x1p-5f};
+    const float k_f[2] = {-down[0] * q_up[0] * 0x1p-5f, -down[1] * q_up[1] * 0x1p-5f};
+#pragma unroll 1
     for (int n0 = 0; n0 < PIECES; n0 += 4) {
       float acc[4][4] = {};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= warp)
-#pragma unroll
-          for (int n = 0; n < 4; n += 2) {
-            uint32_t b[4];
-            ld_matrix4_trans(b, ks + ld_at<PIECES>(j * 16 + (lane & 15), n0 + n + (lane >> 4)));
-            ld_mma(acc[n], lo[j], b[0], b[1]), ld_mma(acc[n + 1], lo[j], b[2], b[3]);
-            ld_mma(acc[n], hi[j], b[0], b[1]), ld_mma(acc[n + 1], hi[j], b[2], b[3]);
-          }
+      uint32_t w[4][2];
 #pragma unroll
       for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          uint32_t* const at = (uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2);
-          const uint32_t w = *at;
-          const float f = q_up[r] * 0x1p-5f;
-          *at = ld_half2((q_base[r] * h_lo(w) - acc[n][2 * r] * down[r]) * f, (q_base[r] * h_hi(w) - acc[n][2 * r + 1] * down[r]) * f);
+        for (int r = 0; r < 2; ++r) w[n][r] = *(const uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= warp) {
+          uint32_t b[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) ld_matrix4_trans(b[n], ks + ld_at<PIECES>(j * 16 + (lane & 15), n0 + 2 * n + (lane >> 4)));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) ld_mma(acc[n], lo[j], b[n / 2][n % 2 * 2], b[n / 2][n % 2 * 2 + 1]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) ld_mma(acc[n], hi[j], b[n / 2][n % 2 * 2], b[n / 2][n % 2 * 2 + 1]);
         }
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *(uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2) =
+              ld_half2(fmaf(acc[n][2 * r], k_f[r], q_f[r] * h_lo(w[n][r])), fmaf(acc[n][2 * r + 1], k_f[r], q_f[r] * h_hi(w[n][r])));
     }
     {  // columns of T become rows of T^T D: two threads each, four rows by turns
       const int j = tid >> 1, half = tid & 1;

@@ -354,8 +354,8 @@ def test_delta_parts_of_a_long_pass_follow_one_another(cuda):
     from drama3_b200 import _lib, kernels
     heads = (16, 64, 64, 16)
     chunk = _lib.lib().d3_lines_delta_workspace(64, 1, 16, 64, 64)
-    n = (256 << 20) // chunk * 64 + 100
-    assert _lib.lib().d3_lines_delta_workspace(n, 1, 16, 64, 64) <= 256 << 20
+    n = (384 << 20) // chunk * 64 + 100
+    assert _lib.lib().d3_lines_delta_workspace(n, 1, 16, 64, 64) <= 384 << 20
     counts = [n - 130, 70]
     cu, plan = plan_of(counts, 60, cuda)
     (q, k, v, decay, state), more = delta_case(cuda, heads, counts, 60, torch.bfloat16, "raw", 28)
