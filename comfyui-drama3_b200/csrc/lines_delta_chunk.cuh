@@ -102,8 +102,8 @@ struct LdChunkArgs {
 // products. T: the 16 x 16 blocks on the diagonal of I + A are inverted by columns, a thread each, then blocks of 32 and of 64 by
 // [T1, 0; X, T2], X = -T2 A21 T1, in tf32 terms. (By columns of all 64 at once the same numbers took 2000 unrolled steps and the time
 // went into fetching instructions.) P T in tf32 terms too, whose range of exponents needs no scales; Q~ and K~ in fp16 terms.
-// Bound by instructions and their latency, 0.41 of the issue slots with four CTAs an SM: 32 chunks of 32 value heads 70 us (B200), of
-// which P T and Q~, whose longest rows are one warp's, take 20.
+// Bound by instructions, their latency and their fetch, 0.48 of the issue slots with four CTAs an SM: 32 chunks of 32 value heads 57 us
+// (B200). Loops that need not be unrolled are not: with those of Q K^T, of the joins and of Q~ unrolled it took 70.
 constexpr int LD_PREP_THREADS = 128;
 constexpr int LD_PITCH = 68;  // floats of a row of A and T in shared memory
 constexpr float LD_MAX = 3.4028234e38f;
