@@ -814,11 +814,12 @@ def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None
         S <- exp(g) S;  u = beta (v - S k), the delta rule, or u = v without beta;  S <- S + u k^T;  out = scale S q
 
     q, k [T, Hk, Dk] and v [T, Hv, Dv] (bfloat16 or float16; any strides with the last dimension contiguous; views whose rows
-    are not on 16-byte boundaries are copied); value head h reads key head h / (Hv / Hk). decay and beta [T, Hv] (the last
-    dimension contiguous, of the rows' type or float32, alike). With a_log [Hv] (float32) they are the projections' raw
-    outputs: g = -exp(a_log) softplus(decay + dt_bias), beta through the sigmoid; without it g is decay itself, at most 0, and
-    beta is taken as it is. q and k are divided by sqrt(sum of squares + eps) unless eps is None; scale defaults to 1 /
-    sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get zeros."""
+    are not on 16-byte boundaries are copied, and values that heads or tokens share); value head h reads key head h / (Hv /
+    Hk). decay and beta [T, Hv] (the last dimension contiguous, of the rows' type or float32, alike). With a_log [Hv]
+    (float32) they are the projections' raw outputs: g = -exp(a_log) softplus(decay + dt_bias), beta through the sigmoid;
+    without it g is decay itself, at most 0, and beta is taken as it is. q and k are divided by sqrt(sum of squares + eps)
+    unless eps is None; scale defaults to 1 / sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get
+    zeros."""
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         q, k, v = (_aligned16(t) for t in (q, k, v))
     cu, line = plan.cu, plan.line
@@ -864,7 +865,7 @@ def _delta_arguments(q, k, v, decay, state, beta, a_log, dt_bias, cu, line):
             raise ValueError(f"{name} must be a contiguous float32 [{Hv}] tensor")
     if state.dim() != 4 or state.shape[1:] != (Hv, Dv, Dk) or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"state must be a contiguous float32 [B, {Hv}, {Dv}, {Dk}] tensor")
-    copies = any(s % 8 for t in (q, k, v) for s in t.stride()[:2])
+    copies = any(s % 8 for t in (q, k, v) for s in t.stride()[:2]) or 0 in v.stride()[:2]  # a tensor map has no stride of 0
     strides = tuple(_int64s((t.shape[1] * t.shape[2], t.shape[2]) if copies else t.stride()[:2]) for t in (q, k, v))
     B = state.shape[0]
     _plan_lines("lines_delta", device, cu, line, T, B)
@@ -910,8 +911,9 @@ def add_norm(x, residual, weight, post_weight=None, gate=None, scale=1.0, eps=1e
                                                                               post_weight, gate)
     sums = torch.empty_like(x, memory_format=torch.contiguous_format)
     normed = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _launch(device, "add_norm", lib().d3_add_norm, x.data_ptr(), x_token, residual.data_ptr(), r_token, *sizes, weight.data_ptr(), _ptr(post_weight), w_f32, 1.0 if unit_offset else 0.0, _ptr(gate), gate_token, gate_kind,
-            scale, eps, sums.data_ptr(), normed.data_ptr())
+    _launch(device, "add_norm", lib().d3_add_norm, x.data_ptr(), x_token, residual.data_ptr(), r_token, *sizes,
+            weight.data_ptr(), _ptr(post_weight), w_f32, 1.0 if unit_offset else 0.0, _ptr(gate), gate_token, gate_kind, scale, eps,
+            sums.data_ptr(), normed.data_ptr())
     return sums, normed
 
 

@@ -334,9 +334,9 @@ int d3_lines_conv(const void* x, int64_t x_token, int type, int T, int C, const 
 
 /* Linear attention with a decay for each head, S [Dv, Dk] a line and value head: S <- e^g S; u = beta (v - S k) (the delta
  * rule; u = v where beta is null); S <- S + u k^T; out = scale S q. q and k [T, Hk, Dk], v [T, Hv, Dv] (types 0 and 1,
- * strides in elements for token and head, multiples of 8), out [T, Hv, Dv]; value head h reads key head h / (Hv / Hk).
- * decay and beta [T, Hv] (stride of a token in elements; of the rows' type, or fp32 with gates_f32). With a_log [Hv] they
- * are the projections' raw outputs, g = -exp(a_log) softplus(decay + dt_bias) (dt_bias [Hv] or null) and beta is
+ * strides in elements for token and head, multiples of 8, v's above 0), out [T, Hv, Dv]; value head h reads key head
+ * h / (Hv / Hk). decay and beta [T, Hv] (stride of a token in elements; of the rows' type, or fp32 with gates_f32). With
+ * a_log [Hv] they are the projections' raw outputs, g = -exp(a_log) softplus(decay + dt_bias) (dt_bias [Hv] or null) and beta is
  * sigmoid(beta); without it g = min(decay, 0). With eps >= 0 the rows of q and k are divided by sqrt(sum of squares + eps).
  * state [B, Hv, Dv, Dk] fp32, read and replaced; that of a line without tokens is left as it is. Places of no line get
  * zeros. Dk 64 or 128, Dv a multiple of 16 up to 256; q, k, v, out and state 16-byte aligned, the

@@ -205,6 +205,16 @@ def test_delta_rows_off_16_byte_boundaries(cuda, counts):
                        kernels.lines_delta(*long, decay, second, plan, **more)) and torch.equal(first, second)
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [150, 20]])
+@pytest.mark.parametrize("over", ["heads", "tokens"])
+def test_delta_rows_that_heads_or_tokens_share(cuda, over, counts):
+    cu, plan = plan_of(counts, 0, cuda)
+    args, more = delta_case(cuda, (2, 4, 64, 64), counts, 0, torch.bfloat16, "raw", 13)
+    shared = [(t[:, :1] if over == "heads" else t[:1]).expand_as(t) for t in args[:3]]
+    assert all(0 in t.stride() for t in shared)
+    check_delta(cuda, (*shared, *args[3:]), more, cu, plan)
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [150, 200]])
 def test_delta_extremes(cuda, counts):
     """Decays of nothing and of everything, above 0 (which count as 0), rows of zeros, strengths of 0 and 1, the same key over
