@@ -763,10 +763,12 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       const int st = i % STAGES;
       ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team][i & 1], (i >> 1) & 1);
       if (!ok) break;
+      bool released = true;
       if (warp == WARPS * PARTS && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
-        ok = mbar_wait(&empty[(i - 1) % STAGES], ((i - 1) / STAGES) & 1);
-        if (ok) load();
+        released = mbar_wait(&empty[(i - 1) % STAGES], ((i - 1) / STAGES) & 1);
+        if (released) load();
       }
+      ok = __all_sync(0xffffffffu, released);  // where it ran out, the warp goes through this chunk and leaves the loop together
       const uint8_t* const stage = ring + st * Shape::STAGE;
       const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
       const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
