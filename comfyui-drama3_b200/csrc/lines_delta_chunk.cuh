@@ -251,7 +251,10 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     }
   }
   __syncthreads();  // the zeros
-  if (!__syncthreads_and(mbar_wait(&arrived, 0))) return;
+  if (!__syncthreads_and(mbar_wait(&arrived, 0))) {  // copies in flight land before the block ends
+    mbar_wait(&arrived, 0);
+    return;
+  }
   // rows to fp16, each by the power of two that brings its largest value into [1, 2): four lanes a row, in place
 #pragma unroll 1
   for (int i0 = 0; i0 < 4; ++i0) {

@@ -29,3 +29,15 @@ def test_the_scans_loops_end_for_whole_warps():
     for value in given:
         terms = [t.strip() for t in value.split("&&")]
         assert all(re.match(r"(true$|ld_wait\(|__all_sync\(0xffffffffu, )", t) for t in terms), value
+
+
+def test_no_block_ends_with_copies_in_flight():
+    """Where the preparation's wait for its rows ran out, it waits for them once more before it returns; the scan's loading lane
+    waits for every stage that it has asked for."""
+    body = kernel("lines_delta_prep_kernel")
+    bulk = body.index("bulk_g2s(")
+    returns = [m.start() for m in re.finditer(r"\breturn;", body)]
+    assert len(returns) == 1 and returns[0] > bulk  # no way out before the copies are asked for
+    assert body[bulk:returns[0]].count("mbar_wait(&arrived, 0)") == 2
+    body = kernel("lines_delta_scan_kernel")
+    assert re.search(r"lane == 0 && !ok\)\s*for \(int i = loads - 1; i >= 0 && i >= loads - STAGES; --i\) mbar_wait\(&full", body)
