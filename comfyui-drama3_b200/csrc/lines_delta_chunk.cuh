@@ -9,7 +9,9 @@
 //   O = scale (Q~ S^T + P T V),  S <- gamma_last S + R^T K~
 // So the chain from chunk to chunk (the scan) has two products, S -> R -> S, and an output is what is left of the state and of each v
 // by then: row j of K~ is beta_j k_j through the later tokens' decays and corrections, row i of Q~ gamma_i q_i through the earlier ones',
-// and those only shrink them. (As Q S^T + P T R the outputs are differences of large terms where the chunk overwrites the state.)
+// and those only shrink them while beta |k|^2 is at most 2. (As Q S^T + P T R the outputs are differences of large terms where the
+// chunk overwrites the state.) Past 2 a correction overshoots, and rows grow as the definition's do; every scale below is taken from what
+// it scales.
 // Without the delta rule R = V, T = I, Q~ = diag(gamma) Q.
 // Exponents are differences that are never above 0, of sums in 64 bits.
 //
@@ -476,8 +478,9 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     q_base[r] = ld_exp(G_s[i].x + G_s[i].y) * q_factor[i];
   }
   if constexpr (DELTA) {
-    // Q~ = gamma Q - (P T) gamma K in Q's place, its rows below 2^15: what is taken off only shrinks them, and single values of them
-    // grow by sqrt(Dk) at most
+    // Q~ = gamma Q - (P T) gamma K in Q's place. Values of k and q are below 2, so that a row is below 2 q_base + 64 x 2 m, m the largest
+    // of the row of P T gamma: below 130 x 2^14 / 64 < 2^15.1 in the scale of the larger of the two. (Where corrections shrink what they
+    // correct, beta |k|^2 at most 2, the first term alone would do; past that a row grows by as much a token.)
     float m[2] = {0.0f, 0.0f}, up[2], down[2], q_up[2], q_down[2];
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
@@ -493,8 +496,9 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], o));
       ld_scale(m[r], up[r], down[r]);
-      ld_scale(q_base[r], q_up[r], q_down[r]);
-      if (cc == 0) q_scale_s[warp * 16 + g + r * 8] = q_base[r] == 0.0f ? 0.0f : q_down[r] * 0x1p5f;
+      const float most_q = fmaxf(q_base[r], m[r]);
+      ld_scale(most_q, q_up[r], q_down[r]);
+      if (cc == 0) q_scale_s[warp * 16 + g + r * 8] = most_q == 0.0f ? 0.0f : q_down[r] * 0x1p6f;
     }
     uint32_t hi[4][4], lo[4][4];
 #pragma unroll
@@ -504,8 +508,8 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
       ld_split(p[2 * j + 1][0] * up[0], p[2 * j + 1][1] * up[0], hi[j][2], lo[j][2]);
       ld_split(p[2 * j + 1][2] * up[1], p[2 * j + 1][3] * up[1], hi[j][3], lo[j][3]);
     }
-    const float q_f[2] = {q_base[0] * q_up[0] * 0x1p-5f, q_base[1] * q_up[1] * 0x1p-5f};
-    const float k_f[2] = {-down[0] * q_up[0] * 0x1p-5f, -down[1] * q_up[1] * 0x1p-5f};
+    const float q_f[2] = {q_base[0] * q_up[0] * 0x1p-6f, q_base[1] * q_up[1] * 0x1p-6f};
+    const float k_f[2] = {-down[0] * q_up[0] * 0x1p-6f, -down[1] * q_up[1] * 0x1p-6f};
 #pragma unroll 1
     for (int n0 = 0; n0 < PIECES; n0 += 4) {
       float acc[4][4] = {};

@@ -1,0 +1,97 @@
+"""lines_delta over the whole range of its arguments, against the 64-bit restatements of tests/linear_ref.py: corrections that
+grow what they correct, token by token and in chunks.
+
+Tolerances. Half a step of a type is 2^-8 (bf16), 2^-11 (fp16) of the value; the multiples of a row's size are those of
+tests/test_linear_gpu.py: 2^-15 for the state and what an output takes from it, 2^-10 for factors of an output in 16 bits.
+Where a correction grows what it corrects (the token's map of a row of the state, M_t = exp(g) (I - beta k k^T), has a norm
+above 1 for beta |k|^2 above 2), it grows what was rounded before as well, and the row of the state may be smaller than what it is
+summed from. With M_jt the maps from token j to t, errors are then multiples of
+    a row of the state:  N = W_t + |S_0| |M_0t|_F / sqrt(Dk) + sum_j |beta_j v_j| |k_j M_jt|
+    an output:           scale (W_t |q_t| + |S_0| |M_0t q_t| + sum_j |beta_j v_j| |k_j M_jt q_t|)
+W as in linear_ref.delta, what the row's own sums are; the second terms an error in the first state, of any direction, by the time of
+t; the third ones the values' shares. Without growth they are W and W |q| scale but for a factor of about 2."""
+import pytest
+import torch
+
+import linear_ref as ref
+from test_linear_gpu import HALF, TINY, fault, generator, near, plan_of
+
+pytestmark = pytest.mark.gpu
+
+
+def sizes(q, k, v, decay, state, cu, beta, eps=1e-6, scale=None):
+    """(size of the outputs, of the state's rows) as in the head of this file; the gates given, not raw."""
+    Hk, Dk, Hv = q.shape[1], q.shape[2], v.shape[1]
+    _, after, out, W = ref.delta(q, k, v, decay, state, cu, beta, eps=eps, scale=scale)
+    scale = Dk ** -0.5 if scale is None else scale
+    q, k = q.double(), k.double()
+    if eps is not None:
+        q, k = (x / torch.sqrt(x.square().sum(-1, keepdim=True) + eps) for x in (q, k))
+    q, k = (x.repeat_interleave(Hv // Hk, 1) for x in (q, k))
+    g, beta = ref.gates(decay, beta)
+    out, N, start = out.clone(), W.clone(), state.double().norm(dim=-1)
+    for b in range(len(cu) - 1):
+        X = torch.eye(Dk, dtype=torch.float64, device=q.device).expand(Hv, Dk, Dk)  # M_0t, and below it the rows k_j M_jt
+        values = torch.zeros((Hv, v.shape[2], 0), dtype=torch.float64, device=q.device)
+        for t in range(cu[b], cu[b + 1]):
+            X = torch.exp(g[t])[:, None, None] * (X - beta[t][:, None, None] * (X @ k[t][..., None]) * k[t][:, None])
+            X = torch.cat((X, k[t][:, None]), 1)
+            values = torch.cat((values, (beta[t][:, None] * v[t].double()).abs()[..., None]), 2)
+            left = (X @ q[t][..., None])[..., 0]
+            shares = left[:, :Dk].norm(dim=-1)[:, None] * start[b] + (values @ left[:, Dk:, None].abs())[..., 0]
+            out[t] += scale * shares
+        if cu[b + 1] > cu[b]:
+            N[b] += start[b] * X[:, :Dk].norm(dim=(1, 2))[:, None] / Dk ** 0.5 + (values @ X[:, Dk:].norm(dim=-1)[..., None])[..., 0]
+    return out, N
+
+
+def check(args, cu, plan, **more):
+    from drama3_b200 import kernels
+    q, k, v, decay, state = args
+    dtype = q.dtype
+    want, after, _, _ = ref.delta(*args, cu, **more)
+    size, state_size = sizes(*args, cu, **more)
+    assert after.abs().max() < 1e30 and want.abs().max() < (6e4 if dtype == torch.float16 else 1e30)  # the definition's own range
+    out = kernels.lines_delta(*args, plan, **more)
+    near(out, want, (1 + HALF[dtype]) * (2.0 ** -15 + 2.0 ** -10) * size + HALF[dtype] * want.abs() + TINY[dtype], "out")
+    near(state, after, 2.0 ** -15 * state_size[..., None].expand_as(after), "state")
+    # in the 2-norm: a result's own rounding, uniform within half a step (a root of 1/3 of it, a tenth more for the finite sample), and
+    # that of two factors to 16 bits, as many errors to either side: sqrt(2 / 3) 2^-12
+    assert (out.double() - want).norm() <= HALF[dtype] * 3 ** -0.5 * 1.1 * want.norm() + 2.0 ** -12 * size.norm()
+    assert fault() == 0
+
+
+GROWING = [  # keys, |k|^2, tokens of each line, rows; a line of 16 tokens alone and four a line go token by token, the others in chunks
+    ("random", 5.0, [16], torch.bfloat16), ("random", 5.0, [64], torch.bfloat16), ("random", 5.0, [90, 0, 130, 1], torch.bfloat16),
+    ("random", 10.0, [4, 1, 3], torch.bfloat16), ("random", 10.0, [64], torch.bfloat16), ("random", 10.0, [30, 33, 2], torch.bfloat16),
+    ("repeated", 5.0, [3, 4, 4], torch.bfloat16), ("repeated", 5.0, [17], torch.bfloat16), ("repeated", 5.0, [20, 1, 24], torch.bfloat16),
+    ("repeated", 10.0, [16], torch.bfloat16), ("repeated", 10.0, [17], torch.bfloat16), ("repeated", 10.0, [20, 3, 20], torch.bfloat16),
+    ("random", 3.0, [8], torch.float16), ("random", 3.0, [40], torch.float16), ("repeated", 2.5, [18], torch.float16)]
+
+
+@pytest.mark.parametrize("heads", [(2, 4, 128, 128), (1, 2, 64, 48)])
+@pytest.mark.parametrize("keys,length2,counts,dtype", GROWING)
+def test_delta_corrections_that_grow(cuda, heads, keys, length2, counts, dtype):
+    """Keys as they are with beta 1: a correction overshoots by |k|^2 - 1."""
+    Hk, Hv, Dk, Dv = heads
+    spare = int(len(counts) > 1)
+    cu, plan = plan_of(counts, spare, cuda)
+    g, T = generator(cuda, 31), sum(counts) + spare
+    normal = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    k = normal(1 if keys == "repeated" else T, Hk, Dk).expand(T, Hk, Dk)
+    k = (k * (length2 ** 0.5 / k.norm(dim=-1, keepdim=True))).to(dtype)
+    q = normal(T, Hk, Dk)
+    q = (0.5 * q / q.norm(dim=-1, keepdim=True)).to(dtype) if keys == "random" else (k.float() + 0.05 * q).to(dtype)
+    args = (q, k, normal(T, Hv, Dv).to(dtype), -0.01 * torch.rand((T, Hv), generator=g, device=cuda), normal(len(counts), Hv, Dv, Dk))
+    check(args, cu, plan, beta=torch.ones((T, Hv), device=cuda), eps=None, scale=0.1 if dtype == torch.bfloat16 else 2.0 ** -6)
+
+
+@pytest.mark.parametrize("counts", [[12], [20], [40, 0, 50]])
+def test_delta_strengths_past_two(cuda, counts):
+    """Keys of length 1 and strengths given up to 4."""
+    cu, plan = plan_of(counts, 0, cuda)
+    g, T = generator(cuda, 32), sum(counts)
+    normal = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    q, k, v = (normal(T, 2, 128).bfloat16() for _ in range(3))
+    args = (q, k, v, -0.1 * torch.rand((T, 2), generator=g, device=cuda), normal(len(counts), 2, 128, 128))
+    check(args, cu, plan, beta=4 * torch.rand((T, 2), generator=g, device=cuda))
