@@ -50,6 +50,22 @@ template <int TYPE> D3_DEV float ld_beta(const LdArgs& a, long long t, int h) {
   return a.a_log ? 1.0f / (1.0f + expf(-b)) : b;
 }
 
+// The power of two that takes values of at most `most` below 2^14, and its inverse (exact, normal numbers both; 1 for a row
+// of zeros).
+D3_DEV void ld_scale(float most, float& up, float& down) {
+  const int e = most > 0.0f ? max((int)(__float_as_uint(most) >> 23) - 127, -113) : 13;
+  up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+  down = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+}
+
+// What takes a row up x, with squares that add up to `sum`, to x / sqrt(|x|^2 + eps), or with eps < 0 to x: up a power of two, down its
+// inverse. (Where eps is past 32 bits in the row's scale, nothing of the row counts beside it.)
+D3_DEV float ld_unit(float sum, float eps, float up, float down) {
+  if (eps < 0.0f) return down;
+  const float e = eps * up * up;
+  return e <= 3.4028234e38f ? rsqrtf(sum + e) : rsqrtf(eps) * down;
+}
+
 // ---- Token by token. A warp holds LS_ROWS x (32 / lanes) rows of a head's state in registers, 16 bytes of a row a lane,
 // and takes the line's tokens in turn. S k and S q are summed in one go, on the state before the token: o = scale (e^g S q +
 // u (k . q)). Bound by memory where the tokens are few: a state is read once and written once, 8 Dk Dv bytes a head against 7
@@ -122,18 +138,37 @@ __global__ void __launch_bounds__(LS_WARPS * 32) lines_delta_step_kernel(LdArgs 
     const float v = mine < a.Dv ? TT::get(((const E*)a.v.p)[t * a.v.token + h * a.v.head + mine]) : 0.0f;
     const float alpha = expf(ld_log_decay<TYPE>(a, t, h));
     const float beta = DELTA ? ld_beta<TYPE>(a, t, h) : 1.0f;
-    float kk = 0.0f, qq = 0.0f, kq = 0.0f;
+    float kk, qq, kq, k_up = 1.0f, k_down = 1.0f, q_up = 1.0f, q_down = 1.0f;
+    auto sums = [&] {
+      kk = qq = kq = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kk = fmaf(k[i], k[i], kk), qq = fmaf(q[i], q[i], qq), kq = fmaf(k[i], q[i], kq);
+      for (int i = 0; i < 4; ++i) kk = fmaf(k[i], k[i], kk), qq = fmaf(q[i], q[i], qq), kq = fmaf(k[i], q[i], kq);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-      kk += __shfl_xor_sync(0xffffffffu, kk, o);
-      qq += __shfl_xor_sync(0xffffffffu, qq, o);
-      kq += __shfl_xor_sync(0xffffffffu, kq, o);
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        kk += __shfl_xor_sync(0xffffffffu, kk, o);
+        qq += __shfl_xor_sync(0xffffffffu, qq, o);
+        kq += __shfl_xor_sync(0xffffffffu, kq, o);
+      }
+    };
+    sums();
+    // rows whose squares leave 32 bits, or come near to (or are zeros): by a power of two that brings the largest value into [1, 2)
+    if (__any_sync(0xffffffffu, !(fminf(kk, qq) >= 0x1p-60f && fmaxf(kk, qq) <= 0x1p100f))) {
+      float most[2] = {fmaxf(fmaxf(fabsf(k[0]), fabsf(k[1])), fmaxf(fabsf(k[2]), fabsf(k[3]))),
+                       fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3])))};
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], o));
+      ld_scale(most[0], k_up, k_down);
+      ld_scale(most[1], q_up, q_down);
+      k_up *= 0x1p-13f, k_down *= 0x1p13f, q_up *= 0x1p-13f, q_down *= 0x1p13f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] *= k_up, q[i] *= q_up;
+      sums();
     }
     // a row of zeros stays one, with eps 0 too
-    const float rk = a.eps < 0.0f ? 1.0f : kk == 0.0f ? 0.0f : rsqrtf(kk + a.eps);
-    const float rq = (a.eps < 0.0f ? 1.0f : qq == 0.0f ? 0.0f : rsqrtf(qq + a.eps)) * a.scale;
+    const float rk = kk == 0.0f ? 0.0f : ld_unit(kk, a.eps, k_up, k_down);
+    const float rq = (qq == 0.0f ? 0.0f : ld_unit(qq, a.eps, q_up, q_down)) * a.scale;
     float sk[LS_ROWS], sq[LS_ROWS];
 #pragma unroll
     for (int r = 0; r < LS_ROWS; ++r) {

@@ -85,14 +85,6 @@ D3_DEV void ld_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = ld_half2(x - h_lo(hi), y - h_hi(hi));
 }
 
-// The power of two that takes values of at most `most` below 2^14, and its inverse (exact, normal numbers both; 1 for a row
-// of zeros).
-D3_DEV void ld_scale(float most, float& up, float& down) {
-  const int e = most > 0.0f ? max((int)(__float_as_uint(most) >> 23) - 127, -113) : 13;
-  up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-  down = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-}
-
 struct LdChunkArgs {
   LdArgs a;
   int block0, blocks;  // of the pass's blocks of 64 tokens, those of this launch

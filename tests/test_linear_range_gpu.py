@@ -9,7 +9,8 @@ summed from. With M_jt the maps from token j to t, errors are then multiples of
     a row of the state:  N = W_t + |S_0| |M_0t|_F / sqrt(Dk) + sum_j |beta_j v_j| |k_j M_jt|
     an output:           scale (W_t |q_t| + |S_0| |M_0t q_t| + sum_j |beta_j v_j| |k_j M_jt q_t|)
 W as in linear_ref.delta, what the row's own sums are; the second terms an error in the first state, of any direction, by the time of
-t; the third ones the values' shares. Without growth they are W and W |q| scale but for a factor of about 2."""
+t; the third ones the values' shares. Without growth they are W and W |q| scale but for a factor of about 2. What is below the
+smallest normal number of 32 bits, 2^-126, may vanish."""
 import pytest
 import torch
 
@@ -49,12 +50,13 @@ def check(args, cu, plan, **more):
     from drama3_b200 import kernels
     q, k, v, decay, state = args
     dtype = q.dtype
-    want, after, _, _ = ref.delta(*args, cu, **more)
-    size, state_size = sizes(*args, cu, **more)
+    exact = {**more, "eps": 1e-200} if more.get("eps") == 0 else more  # rows of zeros are zeros
+    want, after, _, _ = ref.delta(*args, cu, **exact)
+    size, state_size = sizes(*args, cu, **exact)
     assert after.abs().max() < 1e30 and want.abs().max() < (6e4 if dtype == torch.float16 else 1e30)  # the definition's own range
     out = kernels.lines_delta(*args, plan, **more)
-    near(out, want, (1 + HALF[dtype]) * (2.0 ** -15 + 2.0 ** -10) * size + HALF[dtype] * want.abs() + TINY[dtype], "out")
-    near(state, after, 2.0 ** -15 * state_size[..., None].expand_as(after), "state")
+    near(out, want, (1 + HALF[dtype]) * (2.0 ** -15 + 2.0 ** -10) * size + HALF[dtype] * want.abs() + TINY[dtype] + 2.0 ** -126, "out")
+    near(state, after, 2.0 ** -15 * state_size[..., None].expand_as(after) + 2.0 ** -126, "state")
     # in the 2-norm: a result's own rounding, uniform within half a step (a root of 1/3 of it, a tenth more for the finite sample), and
     # that of two factors to 16 bits, as many errors to either side: sqrt(2 / 3) 2^-12
     assert (out.double() - want).norm() <= HALF[dtype] * 3 ** -0.5 * 1.1 * want.norm() + 2.0 ** -12 * size.norm()
@@ -95,3 +97,21 @@ def test_delta_strengths_past_two(cuda, counts):
     q, k, v = (normal(T, 2, 128).bfloat16() for _ in range(3))
     args = (q, k, v, -0.1 * torch.rand((T, 2), generator=g, device=cuda), normal(len(counts), 2, 128, 128))
     check(args, cu, plan, beta=4 * torch.rand((T, 2), generator=g, device=cuda))
+
+
+@pytest.mark.parametrize("heads", [(2, 4, 64, 48), (2, 2, 128, 64)])
+@pytest.mark.parametrize("counts,eps", [([1, 1, 1], 0.0), ([1, 1, 1], 1e-6), ([5, 0, 4, 3], 0.0), ([5, 0, 4, 3], 1e-6), ([100, 130], 0.0)])
+def test_delta_rows_of_any_size(cuda, heads, counts, eps):
+    """Queries and keys whose squares leave 32 bits to either side, next to ordinary ones; rows of zeros."""
+    Hk, Hv, Dk, Dv = heads
+    cu, plan = plan_of(counts, 0, cuda)
+    g, T = generator(cuda, 33), sum(counts)
+    normal = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    powers = torch.tensor([20.0, -33.0, 36.0, 0.0, -24.0, 25.0, -12.0, 1.0, -20.0], device=cuda)
+    turn = torch.arange(T * Hk, device=cuda).view(T, Hk, 1)
+    q, k = ((normal(T, Hk, Dk) * 10.0 ** powers[(turn * step + 1) % 9]).bfloat16() for step in (2, 1))
+    k[3::7, 0], q[4::5, 1] = 0, 0
+    assert k.float().square().sum(-1).isinf().any() and q.isfinite().all() and k.isfinite().all()
+    args = (q, k, normal(T, Hv, Dv).bfloat16(), -torch.exp(normal(T, Hv) - 2), normal(len(counts), Hv, Dv, Dk))
+    beta = torch.rand((T, Hv), generator=g, device=cuda)
+    check(args, cu, plan, beta=beta, eps=eps)
