@@ -280,8 +280,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
       }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    // x / sqrt(|x|^2 + eps) = (up x) / sqrt(|up x|^2 + up^2 eps)
-    float f = a.eps >= 0.0f ? rsqrtf(sum + a.eps * up * up) : down;
+    float f = ld_unit(sum, a.eps, up, down);
     if (most == 0.0f) f = 0.0f;  // a row of zeros: its factor must not set the scale of what it is summed with
     const bool finite = sum <= LD_MAX;
     if (!finite) f = __uint_as_float(0x7fc00000u);

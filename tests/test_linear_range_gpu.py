@@ -100,7 +100,8 @@ def test_delta_strengths_past_two(cuda, counts):
 
 
 @pytest.mark.parametrize("heads", [(2, 4, 64, 48), (2, 2, 128, 64)])
-@pytest.mark.parametrize("counts,eps", [([1, 1, 1], 0.0), ([1, 1, 1], 1e-6), ([5, 0, 4, 3], 0.0), ([5, 0, 4, 3], 1e-6), ([100, 130], 0.0)])
+@pytest.mark.parametrize("counts,eps", [([1, 1, 1], 0.0), ([1, 1, 1], 1e-6), ([5, 0, 4, 3], 0.0), ([5, 0, 4, 3], 1e-6), ([100, 130], 0.0),
+                                        ([100, 130], 1e-6)])
 def test_delta_rows_of_any_size(cuda, heads, counts, eps):
     """Queries and keys whose squares leave 32 bits to either side, next to ordinary ones; rows of zeros."""
     Hk, Hv, Dk, Dv = heads
