@@ -132,8 +132,9 @@ int chunk_launch(const d3::LdArgs& a, void* workspace, const DeviceInfo& d, cuda
     if (int st = launch(d3::lines_delta_prep_kernel<TYPE, DK, DELTA>, dim3(c.blocks, a.Hv), dim3(d3::LD_PREP_THREADS), prep_smem, s,
                         true, c))
       return st;
-    // four teams of one warp a CTA where that gives every SM one, else two of two (us, the former / the latter: 8192 tokens of one line 561 /
-    // 438, 16 texts of up to 192 tokens 114 / 139)
+    // four teams of one warp a CTA where that gives every SM one, else two of two (B200, 16 / 32 heads of 128, us in a graph, the former / the
+    // latter: 8192 tokens of one line 670 / 473, 16 texts of up to 192 tokens 132 / 151). Lines without tokens count: how many have some is
+    // known on the GPU alone.
     const long long wide = (long long)a.B * a.Hv * ((a.Dv + 63) / 64);
     if (int st = wide >= d.sms ? scan_launch<TYPE, DK, DELTA, 4, 1>(vmap, c, s) : scan_launch<TYPE, DK, DELTA, 2, 2>(vmap, c, s))
       return st;

@@ -4,25 +4,21 @@
 //   U = T R,  R = V - diag(gamma) K S^T,  T = (I + A)^-1 diag(beta),  A_ij = beta_i exp(G_i - G_j) k_i . k_j  (j < i)
 //   O = scale (diag(gamma) Q S^T + P U),  P_ij = exp(G_i - G_j) q_i . k_j  (j <= i)
 //   S <- gamma_last S + U^T D K,          D = diag(exp(G_last - G_j))
-// What depends on the tokens alone is formed for all chunks at once (the preparation): not T itself, but P T, K~ = T^T D K and
-// Q~ = diag(gamma) Q - P T diag(gamma) K, with which U is never needed:
-//   O = scale (Q~ S^T + P T V),  S <- gamma_last S + R^T K~
-// So the chain from chunk to chunk (the scan) has two products, S -> R -> S, and an output is what is left of the state and of each v
-// by then: row j of K~ is beta_j k_j through the later tokens' decays and corrections, row i of Q~ gamma_i q_i through the earlier ones',
-// and those only shrink them while beta |k|^2 is at most 2. (As Q S^T + P T R the outputs are differences of large terms where the
-// chunk overwrites the state.) Past 2 a correction overshoots, and rows grow as the definition's do; every scale below is taken from what
-// it scales.
-// Without the delta rule R = V, T = I, Q~ = diag(gamma) Q.
+// What depends on the tokens alone is formed for all chunks at once (the preparation): not T itself, but P T and K~ = T^T D K, with
+// which U is never needed:
+//   O = scale (diag(gamma) Q S^T + P T R),  S <- gamma_last S + R^T K~
+// So the chain from chunk to chunk (the scan) has two products, S -> R -> S. Without the delta rule R = V, T = I.
 // Exponents are differences that are never above 0, of sums in 64 bits.
 //
 // Chunks are cut from the packed tokens, whatever lines they belong to: entries of two lines are zeros, sums and exponents
 // start again with each line. A line's scan masks the tokens of others.
 //
 // Values. k and q become fp16 rows times powers of two, exactly (values below 2^-14 of the row's largest lose what is below
-// 2^-25 of it), and their norms are numbers that results are multiplied by. What is not exact in 16 bits, S, R, T, P and K~, is
+// 2^-25 of it), and their norms are numbers that results are multiplied by. What is not exact in 16 bits, S, R, T, P T and K~, is
 // the sum of two fp16 or tf32 terms, 22 bits, rows of fp16 scaled by a power of two of their own; products are summed in 32 bits, and
-// of the four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. For the outputs,
-// which are rounded to 16 bits anyway, the scan takes one term of S, Q~ and P T: 2^-12 of each.
+// of the four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. Where the chunk
+// overwrites the state an output is the difference of two terms as large as the state, so that all of its factors have two terms too; the
+// second one of P T has eight bits (2^-15 of it): an output's own rounding is 2^-11 of it at least.
 //
 // A value that is not finite reaches the state and the tokens of its own line, in its chunk earlier ones too; one in q its own
 // token only.
@@ -42,8 +38,9 @@ template <int DK> struct alignas(128) LdRows {
 // ... and for a value head: rows likewise, and factors of the tokens' columns.
 template <int DK> struct alignas(128) LdHead {
   uint16_t kt_hi[LD_C * DK], kt_lo[LD_C * DK];  // K~ [64][Dk], row j times 1 / kt_scale[j]
-  uint16_t q[LD_C * DK];                        // Q~ [64][Dk], row i times 1 / q_scale[i]
-  uint16_t p[LD_C * LD_C];                      // P T [64][64], row i times 1 / p_scale[i]
+  uint16_t q[LD_C * DK];                        // Q [64][Dk], row i times 1 / q_scale[i] (gamma_i among it)
+  uint16_t p[LD_C * LD_C];                      // P T [64][64], row i times 1 / p_scale[i]: blocks of 16 x 16 up to the diagonal, second
+                                                // terms where the others would be (ld_rest)
   float kt_scale[LD_C], q_scale[LD_C], p_scale[LD_C];
   float r_in[LD_C];  // gamma_i |k| factor: of K S^T
   float gamma[LD_C];
@@ -52,6 +49,13 @@ template <int DK> struct alignas(128) LdHead {
 // Element offset of 16-byte piece c of row r in rows of `pieces` of them (a multiple of 8): eight rows' pieces of one column lie
 // in different banks.
 template <int PIECES> D3_DEV int ld_at(int r, int c) { return (r * PIECES + (c ^ (r & 7))) * 8; }
+
+// Element offset of a lane's eight second terms of block (i, j) of P T, j <= i, each 2^11 times the term and rounded to e5m2, in the order
+// of ld_matrix4's registers: in the 16-byte pieces of the blocks above the diagonal.
+D3_DEV int ld_rest(int i, int j, int lane) {  // rows 0 to 15 hold those of i 0 to 2, the next ones those of i 3
+  const int row = (i == 3 ? 16 : 0) + (lane >> 1), piece = i == 3 ? 4 + j : i * (i + 1) / 2 + 2 + j;
+  return ld_at<8>(row, piece) + (lane & 1) * 4;
+}
 
 D3_DEV void ld_matrix4(uint32_t (&r)[4], const uint16_t* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -79,6 +83,12 @@ D3_DEV uint32_t ld_half2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// x, y as e5m2 bytes.
+D3_DEV uint32_t ld_bytes(float x, float y) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y), "f"(x));
+  return r;
+}
 // x, y as two fp16 terms each.
 D3_DEV void ld_split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = ld_half2(x, y);
@@ -95,15 +105,15 @@ struct LdChunkArgs {
 // ---- The preparation. A CTA per chunk and value head; the first of a key head's leaves the rows. K K^T and Q K^T are mma.sync
 // products. T: the 16 x 16 blocks on the diagonal of I + A are inverted by columns, a thread each, then blocks of 32 and of 64 by
 // [T1, 0; X, T2], X = -T2 A21 T1, in tf32 terms. (By columns of all 64 at once the same numbers took 2000 unrolled steps and the time
-// went into fetching instructions.) P T in tf32 terms too, whose range of exponents needs no scales; Q~ and K~ in fp16 terms.
+// went into fetching instructions.) P T in tf32 terms too, whose range of exponents needs no scales; K~ in fp16 terms.
 // Bound by instructions, their latency and their fetch, 0.48 of the issue slots with four CTAs an SM: 32 chunks of 32 value heads 57 us
-// (B200). Loops that need not be unrolled are not: with those of Q K^T, of the joins and of Q~ unrolled it took 70.
+// (B200). Loops that need not be unrolled are not: an earlier form took a fifth longer with them unrolled.
 constexpr int LD_PREP_THREADS = 128;
 constexpr int LD_PITCH = 68;  // floats of a row of A and T in shared memory
 constexpr float LD_MAX = 3.4028234e38f;
 
 template <int DK> struct LdPrepShape {
-  static constexpr int K = LD_C * DK * 2;          // the rows of k, K~'s low terms; the rows of q, Q~
+  static constexpr int K = LD_C * DK * 2;          // the rows of k, K~'s low terms; the rows of q
   static constexpr int A = LD_C * LD_PITCH * 4;  // A and T, A21 T1 above them; T^T D, two terms; K~'s high terms
   static constexpr int SMEM = 2 * K + A;
   static_assert(A >= K && A >= 2 * LD_C * LD_C * 2, "");
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
         p[n][e] = j >= from[e >> 1] && j <= i ? tp[n][e] * beta_s[j] : 0.0f;
       }
   }
-  // the rows of P T (of P) out, one term
+  // the rows of P T (of P) out, both terms
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -457,76 +467,28 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     const bool all_good = (__ballot_sync(0xffffffffu, good[r]) & row) == row;
     float up, down;
     ld_scale(most[r], up, down);
-    if (cc == 0) out->p_scale[i] = all_good ? down : __uint_as_float(0x7fc00000u);
+    if (cc == 0) {
+      out->p_scale[i] = all_good ? down : __uint_as_float(0x7fc00000u);
+      q_scale_s[i] = ld_exp(G_s[i].x + G_s[i].y) * q_factor[i];
+    }
 #pragma unroll
     for (int n = 0; n < 8; ++n)
-      *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = ld_half2(p[n][r * 2] * up, p[n][r * 2 + 1] * up);
-  }
-  float q_base[2];  // of Q's rows
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int i = warp * 16 + g + r * 8;
-    q_base[r] = ld_exp(G_s[i].x + G_s[i].y) * q_factor[i];
-  }
-  if constexpr (DELTA) {
-    // Q~ = gamma Q - (P T) gamma K in Q's place. Values of k and q are below 2, so that a row is below 2 q_base + 64 x 2 m, m the largest
-    // of the row of P T gamma: below 130 x 2^14 / 64 < 2^15.1 in the scale of the larger of the two. (Where corrections shrink what they
-    // correct, beta |k|^2 at most 2, the first term alone would do; past that a row grows by as much a token.)
-    float m[2] = {0.0f, 0.0f}, up[2], down[2], q_up[2], q_down[2];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 f = *(const float2*)(r_in_s + n * 8 + cc * 2);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[n][e] = p[n][e] != 0.0f ? p[n][e] * (e & 1 ? f.y : f.x) : 0.0f;  // nothing of another line, where that is not finite
-        m[e >> 1] = fmaxf(m[e >> 1], fabsf(p[n][e]));
+      if (n <= 2 * warp + 1) {
+        float& x = p[n][r * 2];
+        float& y = p[n][r * 2 + 1];
+        x *= up, y *= up;
+        const uint32_t hi = ld_half2(x, y);
+        *(uint32_t*)(out->p + ld_at<8>(i, n) + cc * 2) = hi;
+        x = (x - h_lo(hi)) * 0x1p11f, y = (y - h_hi(hi)) * 0x1p11f;
       }
-    }
+  }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], o));
-      ld_scale(m[r], up[r], down[r]);
-      const float most_q = fmaxf(q_base[r], m[r]);
-      ld_scale(most_q, q_up[r], q_down[r]);
-      if (cc == 0) q_scale_s[warp * 16 + g + r * 8] = most_q == 0.0f ? 0.0f : q_down[r] * 0x1p6f;
-    }
-    uint32_t hi[4][4], lo[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ld_split(p[2 * j][0] * up[0], p[2 * j][1] * up[0], hi[j][0], lo[j][0]);
-      ld_split(p[2 * j][2] * up[1], p[2 * j][3] * up[1], hi[j][1], lo[j][1]);
-      ld_split(p[2 * j + 1][0] * up[0], p[2 * j + 1][1] * up[0], hi[j][2], lo[j][2]);
-      ld_split(p[2 * j + 1][2] * up[1], p[2 * j + 1][3] * up[1], hi[j][3], lo[j][3]);
-    }
-    const float q_f[2] = {q_base[0] * q_up[0] * 0x1p-6f, q_base[1] * q_up[1] * 0x1p-6f};
-    const float k_f[2] = {-down[0] * q_up[0] * 0x1p-6f, -down[1] * q_up[1] * 0x1p-6f};
-#pragma unroll 1
-    for (int n0 = 0; n0 < PIECES; n0 += 4) {
-      float acc[4][4] = {};
-      uint32_t w[4][2];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) w[n][r] = *(const uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j <= warp) {
-          uint32_t b[2][4];
-#pragma unroll
-          for (int n = 0; n < 2; ++n) ld_matrix4_trans(b[n], ks + ld_at<PIECES>(j * 16 + (lane & 15), n0 + 2 * n + (lane >> 4)));
-#pragma unroll
-          for (int n = 0; n < 4; ++n) ld_mma(acc[n], lo[j], b[n / 2][n % 2 * 2], b[n / 2][n % 2 * 2 + 1]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) ld_mma(acc[n], hi[j], b[n / 2][n % 2 * 2], b[n / 2][n % 2 * 2 + 1]);
-        }
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          *(uint32_t*)(qs + ld_at<PIECES>(warp * 16 + g + r * 8, n0 + n) + cc * 2) =
-              ld_half2(fmaf(acc[n][2 * r], k_f[r], q_f[r] * h_lo(w[n][r])), fmaf(acc[n][2 * r + 1], k_f[r], q_f[r] * h_hi(w[n][r])));
-    }
+  for (int j = 0; j < 4; ++j)
+    if (j <= warp)
+      *(uint2*)(out->p + ld_rest(warp, j, lane)) =
+          make_uint2(ld_bytes(p[2 * j][0], p[2 * j][1]) | ld_bytes(p[2 * j + 1][0], p[2 * j + 1][1]) << 16,
+                     ld_bytes(p[2 * j][2], p[2 * j][3]) | ld_bytes(p[2 * j + 1][2], p[2 * j + 1][3]) << 16);
+  if constexpr (DELTA) {
     {  // columns of T become rows of T^T D: two threads each, four rows by turns
       const int j = tid >> 1, half = tid & 1;
       const float b = beta_s[j];
@@ -564,8 +526,6 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
         *(uint2*)(td + at) = h2, *(uint2*)(td + LD_C * LD_C + at) = l2;
       }
     }
-  } else if (cc == 0) {
-    q_scale_s[warp * 16 + g] = q_base[0], q_scale_s[warp * 16 + g + 8] = q_base[1];
   }
   if (tid == 0) ld_bulk_read();  // the rows of k are on their way
   __syncthreads();
@@ -651,25 +611,26 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
 
 // ---- The scan. A CTA has 16 x WARPS rows of a head's state of one line and goes along the line's chunks. 16 rows are a team of
 // warps: one, or PARTS = 2 that have half of the state's columns and half of the chunk's tokens each, carry the state, S -> R -> S;
-// as many others make the outputs from what those leave in shared memory (S's high terms) and V, a step behind, so that their products
-// fill the tensor core while the first ones' values are being converted. S stays in registers, as the accumulator of products [rows
-// of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand is, so that a single warp's
-// chain has no exchange in it. Two warps give one another their terms of S and of R, and each begins with its own while the other's
-// come. K, Q~, K~ and P T, as B operands, come from shared memory, where the first output warp keeps chunks coming (bulk copies; the
-// rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought there and back between the
-// products: with 16 rows a warp the chain is shorter in registers.)
+// as many others make the outputs from what those leave in shared memory (S's terms, and R as it is), a step behind, so that their
+// products and conversions fill what the first ones leave of the tensor core and of the issue slots. They take P T into registers and
+// let the chunk's stage go before R comes: the next chunk but one is asked for by then. S stays in registers, as the accumulator of
+// products [rows of S, tokens or columns of K]; an accumulator of mma.sync is laid out as the next product's A operand is, so that a
+// single warp's chain has no exchange in it. Two warps give one another their terms of S and of R, and each begins with its own while
+// the other's come. K, Q, K~ and P T, as B operands, come from shared memory, where the first output warp keeps chunks coming (bulk
+// copies; the rows of v by TMA). (tcgen05 would want S as a 16-bit operand in shared or tensor memory, and R brought there and back
+// between the products: with 16 rows a warp the chain is shorter in registers.)
 //
 // Bound by the chain's latency: 8192 tokens are 128 chunks one after another, and a head's rows are all that can be spread. Measured
-// (B200, 16 / 32 heads of 128, one line): 2.4 us a chunk, 3900 clocks, of which the 160 products of a warp that carries the state take
-// 1330 of its tensor core's time, those of the output warp beside it 350; the rest are conversions (370 for R, 400 for its
-// terms), barriers and the latency of what they wait for. One warp a team with four teams a CTA (which share the operands'
-// loads) takes 3.4 us a chunk and half the SMs: the better where lines and heads fill the GPU.
+// (B200, 16 / 32 heads of 128, one line): 2.4 us a chunk, of which the 160 products of a warp that carries the state take 1330 of its
+// tensor core's clocks and the 94 of the output warp beside it 780; the rest are conversions (500 for R, 320 for its terms), barriers
+// and the latency of what they wait for. One warp a team with four teams a CTA (which share the operands' loads) takes 3.9 us a chunk
+// and half the SMs: the better where lines and heads fill the GPU.
 template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
-  // a team's place: S's terms as A fragments (high ones, and low ones for the other part) with its rows' scales, two chunks' by turns;
-  // R times K~'s factors, both terms, with their scales, for the other part; the outputs
-  static constexpr int TERMS = DK * 32 * PARTS, S = TERMS + 128, RK = 2 * S, RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0);
-  static constexpr int OUT = RK_SCALES + 128, TEAM = OUT + LD_C * 32;
+  // a team's place: S's terms as A fragments, with its rows' scales of each part; R times K~'s factors likewise, for the other part; R
+  // itself, for the outputs; and those
+  static constexpr int S_SCALES = DK * 64, RK = S_SCALES + 128, RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0);
+  static constexpr int R = RK_SCALES + 128, OUT = R + LD_C * 64, TEAM = OUT + LD_C * 32;
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024;
   static constexpr int OUTS = PARTS;  // warps for the outputs, each of a share of the tokens: as many on every quarter of an SM
@@ -703,8 +664,10 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   constexpr int G = NK < 8 ? NK : 8;  // sums of S that take turns
   constexpr int OUTS = Shape::OUTS, NO = NT / OUTS;
   extern __shared__ uint8_t ld_raw[];
-  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[WARPS][2], s_empty[WARPS][2],
-      r_full[WARPS];  // [2]: odd and even chunks', as their places
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];  // the chunks' stages
+  // a team's S and R: written (R times K~'s factors too), and both read by the outputs. A part writes the next S when the outputs have
+  // read this one, and has the other part's when that has written it, so that none is ever two phases ahead.
+  __shared__ __align__(8) uint64_t s_full[WARPS], rk_full[WARPS], r_full[WARPS], read[WARPS];
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
@@ -715,8 +678,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], (PARTS + OUTS) * WARPS);
     for (int i = 0; i < WARPS; ++i) {
-      mbar_init(&r_full[i], PARTS);
-      for (int y = 0; y < 2; ++y) mbar_init(&s_full[i][y], PARTS), mbar_init(&s_empty[i][y], OUTS);
+      mbar_init(&s_full[i], PARTS), mbar_init(&rk_full[i], PARTS), mbar_init(&r_full[i], PARTS);
+      mbar_init(&read[i], OUTS);
     }
     fence_mbar_init();
   }
@@ -739,27 +702,33 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   bool ok = true;
   if (outputs) {
     constexpr uint32_t row_bytes = DELTA ? sizeof(LdRows<DK>) : 0;  // for K S^T
+    // 16 tokens at a time, of two warps' two times those that have as many blocks of P T before them
+    auto tokens = [&](int x) { return (PARTS == 1 ? x : x == 0 ? part : 3 - part) * 16; };
+    auto blocks_of = [](int x) constexpr { return PARTS == 1 ? x + 1 : x == 0 ? 2 : 4; };  // at most
     const int v_boxes = min(WARPS, (a.Dv - (int)blockIdx.x * WARPS * 16) / 16);
-    int loads = 0;
+    const uint64_t keep = policy_evict_last();
+    const LdRows<DK>* rows_at = (const LdRows<DK>*)c.rows + (size_t)block_a * a.Hk + h / (a.Hv / a.Hk);
+    const LdHead<DK>* head_at = (const LdHead<DK>*)c.heads + (size_t)block_a * a.Hv + h;
+    int token_at = (int)(first_token + (long long)block_a * LD_C), loads = 0;
     auto load = [&] {  // the next chunk; by one lane, whose stage is free
       uint8_t* const to = ring + loads % STAGES * Shape::STAGE;
       uint64_t* const bar = &full[loads % STAGES];
-      const size_t block = block_a + loads;
-      const uint64_t keep = policy_evict_last();
       mbar_arrive_expect_tx(bar, row_bytes + (uint32_t)sizeof(LdHead<DK>) + v_boxes * LD_C * 32);
-      if (DELTA) bulk_g2s(to, (const LdRows<DK>*)c.rows + block * a.Hk + h / (a.Hv / a.Hk), row_bytes, bar, keep);
-      bulk_g2s(to + Shape::HEAD, (const LdHead<DK>*)c.heads + block * a.Hv + h, sizeof(LdHead<DK>), bar, keep);
+      if (DELTA) bulk_g2s(to, rows_at, row_bytes, bar, keep);
+      bulk_g2s(to + Shape::HEAD, head_at, sizeof(LdHead<DK>), bar, keep);
       for (int w = 0; w < v_boxes; ++w)
-        tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h,
-                    (int)(first_token + (long long)block * LD_C), bar);
+        tma_load_3d(smem_u32(to + Shape::V + w * LD_C * 32), &vmap, (blockIdx.x * WARPS + w) * 16, h, token_at, bar);
+      rows_at += a.Hk, head_at += a.Hv, token_at += LD_C;
       ++loads;
     };
     if (warp == WARPS * PARTS && lane == 0)
       for (int i = 0; i < STAGES && i < chunks; ++i) load();
+    const uint32_t out_token = (uint32_t)a.Hv * a.Dv;  // at most 2^24
+    uint16_t* out_at = (uint16_t*)a.out + ((first_token + (long long)block_a * LD_C) * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8;
 #pragma unroll 1
     for (int i = 0; i < chunks && ok; ++i) {
       const int st = i % STAGES;
-      ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team][i & 1], (i >> 1) & 1);
+      ok = ld_wait(&full[st], (i / STAGES) & 1) && ld_wait(&s_full[team], i & 1);
       if (!ok) break;
       bool released = true;
       if (warp == WARPS * PARTS && lane == 0 && i > 0 && loads < chunks) {  // the stage of the chunk before this one
@@ -769,106 +738,115 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       ok = __all_sync(0xffffffffu, released);  // where it ran out, the warp goes through this chunk and leaves the loop together
       const uint8_t* const stage = ring + st * Shape::STAGE;
       const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
-      const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
       const long long t0 = first_token + (long long)(block_a + i) * LD_C;
       const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
       float O[PARTS][NO][4] = {};
 #pragma unroll
       for (int kt = 0; kt < DK / 16; ++kt) {
-        const uint4 s4 = *(const uint4*)(place + (i & 1) * Shape::S + (kt * 32 + lane) * 16);
-        const uint32_t a4[4] = {s4.x, s4.y, s4.z, s4.w};
+        const uint4* const from = (const uint4*)place + kt * 32 + lane;
+        const uint4 h = from[0], l = from[DK * 2];
+        const uint32_t h4[4] = {h.x, h.y, h.z, h.w}, l4[4] = {l.x, l.y, l.z, l.w};
         uint32_t q4[NO / 2][4];
 #pragma unroll
         for (int x = 0; x < NO / 2; ++x)
-          ld_matrix4(q4[x], head.q + ld_at<PIECES>((part * NO + x * 2) * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+          ld_matrix4(q4[x], head.q + ld_at<PIECES>(tokens(x) + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-        for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], a4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
+        for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], l4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
+#pragma unroll
+        for (int x = 0; x < NO; ++x) ld_mma(O[kt / KT][x], h4, q4[x / 2][x % 2 * 2], q4[x / 2][x % 2 * 2 + 1]);
       }
-      const float* const s_scales = (const float*)(place + (i & 1) * Shape::S + Shape::TERMS);
+      // P T and the factors of the columns, so that the stage is free before R comes
+      uint32_t p_hi[NO / 2][LD_C / 16][4];
+      uint2 p_rest[NO / 2][LD_C / 16];
+      float2 fp[NO];
 #pragma unroll
-      for (int y = 0; y < PARTS; ++y) {
-        const float s_down[2] = {s_scales[y * 16 + g], s_scales[y * 16 + g + 8]};
+      for (int x = 0; x < NO / 2; ++x)
 #pragma unroll
-        for (int n = 0; n < NO; ++n)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (y == 0) O[0][n][x] *= s_down[x >> 1];
-            if (y > 0) O[0][n][x] = fmaf(O[y][n][x], s_down[x >> 1], O[0][n][x]);
+        for (int kt = 0; kt < blocks_of(x); ++kt)
+          if (kt * 16 <= tokens(x)) {
+            ld_matrix4(p_hi[x][kt], head.p + ld_at<8>(tokens(x) + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
+            p_rest[x][kt] = *(const uint2*)(head.p + ld_rest(tokens(x) / 16, kt, lane));
           }
-      }
-      ld_arrive(&s_empty[team][i & 1], lane);
-      // V as A fragments, fp16 (exactly, but for values of bf16 below 2^-14 of the row's largest, which lose what is below 2^-25 of
-      // that), zeros for the tokens of other lines
-      uint32_t v4[LD_C / 16][4];
-      float v_down[2] = {1.0f, 1.0f};
+      const float* const s_scales = (const float*)(place + Shape::S_SCALES);
 #pragma unroll
-      for (int kt = 0; kt < LD_C / 16; ++kt) {
-        const int token = kt * 16 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
-        ld_matrix4_trans(v4[kt], v_s + token * 32 + piece * 16);
-        if (lo > 0 || hi < LD_C)
+      for (int n = 0; n < NO; ++n) {
+        const int j = tokens(n / 2) + n % 2 * 8 + cc * 2;
+        const float2 fq = *(const float2*)(head.q_scale + j);
+        fp[n] = *(const float2*)(head.p_scale + j);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = kt * 16 + (x >> 1) * 8 + cc * 2;
-            if (j < lo || j >= hi) v4[kt][x] &= 0xffff0000u;
-            if (j + 1 < lo || j + 1 >= hi) v4[kt][x] &= 0x0000ffffu;
-          }
+        for (int x = 0; x < 4; ++x) {
+          float o = O[0][n][x] * s_scales[g + (x >> 1) * 8];
+#pragma unroll
+          for (int y = 1; y < PARTS; ++y) o = fmaf(O[y][n][x], s_scales[y * 16 + g + (x >> 1) * 8], o);
+          O[0][n][x] = o * (x & 1 ? fq.y : fq.x);
+        }
       }
-      if constexpr (TYPE == QR_BF16) {
+      ld_arrive(&empty[st], lane);
+      ok = ld_wait(&r_full[team], i & 1);
+      if (!ok) break;
+      // R as A fragments of two terms, rows by a power of two; low ones times 2^11, as P T's: what is small beside the row's largest
+      // keeps its bits
+      uint32_t r_hi[LD_C / 16][4], r_lo[LD_C / 16][4];
+      float r_down[2];
+      {
+        float4 v[NT];
         float most[2] = {0.0f, 0.0f}, up[2];
 #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          v[n] = ((const float4*)(place + Shape::R))[n * 32 + lane];
+          most[0] = fmaxf(most[0], fmaxf(fabsf(v[n].x), fabsf(v[n].y)));
+          most[1] = fmaxf(most[1], fmaxf(fabsf(v[n].z), fabsf(v[n].w)));
+        }
+        ld_arrive(&read[team], lane);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) ld_scale(ld_row_most(most[r]), up[r], r_down[r]);
+#pragma unroll
         for (int kt = 0; kt < LD_C / 16; ++kt)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            float y0, y1;
-            TT::get2(v4[kt][x], y0, y1);
-            most[x & 1] = fmaxf(most[x & 1], fmaxf(fabsf(y0), fabsf(y1)));
-          }
-        ld_scale(ld_row_most(most[0]), up[0], v_down[0]);
-        ld_scale(ld_row_most(most[1]), up[1], v_down[1]);
-#pragma unroll
-        for (int kt = 0; kt < LD_C / 16; ++kt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float y0, y1;
-            TT::get2(v4[kt][x], y0, y1);
-            v4[kt][x] = ld_half2(y0 * up[x & 1], y1 * up[x & 1]);
+            const float4& from = v[2 * kt + (x >> 1)];
+            const float v0 = (x & 1 ? from.z : from.x) * up[x & 1], v1 = (x & 1 ? from.w : from.y) * up[x & 1];
+            r_hi[kt][x] = ld_half2(v0, v1);
+            r_lo[kt][x] = ld_half2((v0 - h_lo(r_hi[kt][x])) * 0x1p11f, (v1 - h_hi(r_hi[kt][x])) * 0x1p11f);
           }
       }
       uint8_t* const out_s = place + Shape::OUT;
 #pragma unroll
       for (int m = 0; m < NO; m += 2) {
-        const int n = part * NO + m;
-        float pv[2][4] = {};
+        float high[2][4] = {}, low[2][4] = {};  // the latter times 2^11
 #pragma unroll
-        for (int kt = 0; kt < LD_C / 16; ++kt)
-          if (kt <= n / 2) {
-            uint32_t p4[4];
-            ld_matrix4(p4, head.p + ld_at<8>(n * 8 + (lane & 7) + (lane >> 4) * 8, kt * 2 + ((lane >> 3) & 1)));
-            ld_mma(pv[0], v4[kt], p4[0], p4[1]), ld_mma(pv[1], v4[kt], p4[2], p4[3]);
+        for (int kt = 0; kt < blocks_of(m / 2); ++kt)
+          if (kt * 16 <= tokens(m / 2)) {
+            const auto& p = p_hi[m / 2][kt];
+            const uint2 rest = p_rest[m / 2][kt];
+            // a byte of e5m2 is the upper one of an fp16 number
+            const uint32_t p_lo[4] = {__byte_perm(rest.x, 0, 0x1404), __byte_perm(rest.x, 0, 0x3424), __byte_perm(rest.y, 0, 0x1404),
+                                      __byte_perm(rest.y, 0, 0x3424)};
+            ld_mma(low[0], r_lo[kt], p[0], p[1]), ld_mma(low[1], r_lo[kt], p[2], p[3]);
+            ld_mma(high[0], r_hi[kt], p[0], p[1]), ld_mma(high[1], r_hi[kt], p[2], p[3]);
+            ld_mma(low[0], r_hi[kt], p_lo[0], p_lo[1]), ld_mma(low[1], r_hi[kt], p_lo[2], p_lo[3]);
           }
         uint32_t o4[4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int j = (n + x) * 8 + cc * 2;
-          const float2 fq = *(const float2*)(head.q_scale + j), fp = *(const float2*)(head.p_scale + j);
           float o[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y)
-            o[y] = fmaf(O[0][m + x][y], y & 1 ? fq.y : fq.x, pv[x][y] * v_down[y >> 1] * (y & 1 ? fp.y : fp.x));
+            o[y] = fmaf(fmaf(low[x][y], 0x1p-11f, high[x][y]) * (y & 1 ? fp[m + x].y : fp[m + x].x), r_down[y >> 1], O[0][m + x][y]);
           o4[2 * x] = TT::put2(o[0], o[1]), o4[2 * x + 1] = TT::put2(o[2], o[3]);
         }
-        const int token = n * 8 + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
+        const int token = tokens(m / 2) + (lane & 7) + (lane >> 4) * 8, piece = ((lane >> 3) & 1) ^ ((token >> 2) & 1);
         st_matrix4_trans(out_s + token * 32 + piece * 16, o4[0], o4[1], o4[2], o4[3]);
       }
-      ld_arrive(&empty[st], lane);
+      __syncwarp();
       if (there)
 #pragma unroll
         for (int x = 0; x < LD_C / 16 / OUTS; ++x) {
-          const int token = part * NO * 8 + x * 16 + (lane >> 1), piece = (lane & 1) ^ ((token >> 2) & 1);
+          const int token = tokens(x) + (lane >> 1), piece = (lane & 1) ^ ((token >> 2) & 1);
           if (token >= lo && token < hi)
-            *(uint4*)((uint16_t*)a.out + ((t0 + token) * a.Hv + h) * a.Dv + row0 + (lane & 1) * 8) =
-                *(const uint4*)(out_s + token * 32 + piece * 16);
+            *(uint4*)(out_at + (size_t)token * out_token) = *(const uint4*)(out_s + token * 32 + piece * 16);
         }
+      out_at += (size_t)LD_C * out_token;
       __syncwarp();  // its outputs have been read
     }
     // copies in flight land before the block ends (where a wait ran out: those of the other chunks have been waited for)
@@ -890,12 +868,11 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   ok = ld_wait(&full[0], 0);
 #pragma unroll 1
   for (int i = 0; i < chunks && ok; ++i) {
-    const int st = i % STAGES, odd = i & 1;
+    const int st = i % STAGES;
     const uint8_t* const stage = ring + st * Shape::STAGE;
     const LdRows<DK>& rows = *(const LdRows<DK>*)stage;
     const LdHead<DK>& head = *(const LdHead<DK>*)(stage + Shape::HEAD);
     const uint8_t* const v_s = stage + Shape::V + team * LD_C * 32;
-    uint8_t* const s_place = place + odd * Shape::S;
     const long long t0 = first_token + (long long)(block_a + i) * LD_C;
     const int lo = (int)max(0ll, s - t0), hi = (int)min((long long)LD_C, e - t0);
     const bool partial = lo > 0 || hi < LD_C;
@@ -953,10 +930,10 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     float other_down[2] = {0.0f, 0.0f};
     auto publish_scales = [&] {
       if (cc == 0) {
-        float* const s_scales = (float*)(s_place + Shape::TERMS) + part * 16;
+        float* const s_scales = (float*)(place + Shape::S_SCALES) + part * 16;
         s_scales[g] = down[0], s_scales[g + 8] = down[1];
       }
-      ld_arrive(&s_full[team][odd], lane);
+      ld_arrive(&s_full[team], lane);
     };
     if constexpr (PARTS == 1) {
       uint32_t h4[2][4], l4[2][4];
@@ -964,7 +941,9 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       for (int x = 0; x < 4; ++x) s_term(0, x, h4[0][x], l4[0][x]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        *(uint4*)(s_place + (kt * 32 + lane) * 16) = make_uint4(h4[kt & 1][0], h4[kt & 1][1], h4[kt & 1][2], h4[kt & 1][3]);
+        uint4* const to = (uint4*)place + kt * 32 + lane;
+        to[0] = make_uint4(h4[kt & 1][0], h4[kt & 1][1], h4[kt & 1][2], h4[kt & 1][3]);
+        to[DK * 2] = make_uint4(l4[kt & 1][0], l4[kt & 1][1], l4[kt & 1][2], l4[kt & 1][3]);
         products(0, kt, h4[kt & 1], l4[kt & 1], [&](int x) {
           if (kt + 1 < KT) {
             if (x % 4 == 1) s_term(kt + 1, x / 4, h4[(kt + 1) & 1][x / 4], l4[(kt + 1) & 1][x / 4]);
@@ -979,7 +958,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) s_term(kt, x, h4[kt][x], l4[kt][x]);
-        uint4* const to = (uint4*)s_place + (part * KT + kt) * 32 + lane;
+        uint4* const to = (uint4*)place + (part * KT + kt) * 32 + lane;
         to[0] = make_uint4(h4[kt][0], h4[kt][1], h4[kt][2], h4[kt][3]);
         to[DK * 2] = make_uint4(l4[kt][0], l4[kt][1], l4[kt][2], l4[kt][3]);
       }
@@ -990,12 +969,12 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         products(0, kt, h4[kt], l4[kt], [&](int x) {
           if (DELTA && x % 4 == 3) get_k(kt + 1, kt + 1 < KT ? part * KT + kt + 1 : other, x / 4);
         });
-      ok = ld_wait(&s_full[team][odd], (i >> 1) & 1);
+      ok = ld_wait(&s_full[team], i & 1);
       if (!ok) break;
       if (DELTA) {
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-          const uint4* const from = (const uint4*)s_place + (other + kt) * 32 + lane;
+          const uint4* const from = (const uint4*)place + (other + kt) * 32 + lane;
           const uint4 h = from[0], l = from[DK * 2];
           h4[kt][0] = h.x, h4[kt][1] = h.y, h4[kt][2] = h.z, h4[kt][3] = h.w;
           l4[kt][0] = l.x, l4[kt][1] = l.y, l4[kt][2] = l.z, l4[kt][3] = l.w;
@@ -1005,7 +984,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           products(PARTS - 1, KT + kt, h4[kt], l4[kt], [&](int x) {
             if (kt + 1 < KT && x % 4 == 3) get_k(KT + kt + 1, other + kt + 1, x / 4);
           });
-        const float* const s_scales = (const float*)(s_place + Shape::TERMS) + (1 - part) * 16;
+        const float* const s_scales = (const float*)(place + Shape::S_SCALES) + (1 - part) * 16;
         other_down[0] = s_scales[g], other_down[1] = s_scales[g + 8];
       }
     }
@@ -1046,6 +1025,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           if (j < lo || j >= hi) v[0] = v[2] = f.x = 0.0f;
           if (j + 1 < lo || j + 1 >= hi) v[1] = v[3] = f.y = 0.0f;
         }
+        ((float4*)(place + Shape::R))[(part * NO + n) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           RK[n][y] = v[y] * (y & 1 ? f.y : f.x);
@@ -1057,6 +1037,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
         for (int n = NO; n < G; ++n) get_b(0, n);
     }
+    ld_arrive(&r_full[team], lane);
     // its two terms, for this part's columns and the other's. Each part's tokens have a scale.
     uint32_t h4[LD_C / 16][4], l4[LD_C / 16][4];
     float rk_down[PARTS][2];
@@ -1082,7 +1063,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           float* const rk_scales = (float*)(place + Shape::RK_SCALES) + part * 16;
           rk_scales[g] = rk_down[0][0], rk_scales[g + 8] = rk_down[0][1];
         }
-        ld_arrive(&r_full[team], lane);
+        ld_arrive(&rk_full[team], lane);
       }
     }
     // S = gamma_last S + R^T K~, G columns at a time, each part's tokens in a sum of their own
@@ -1095,7 +1076,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       for (int kt = 0; kt < LD_C / 16; ++kt) {
         const int at = group * (LD_C / 16) + kt, who = kt / KR;
         if (PARTS > 1 && kt == KR) {  // the other part's
-          ok = ld_wait(&r_full[team], i & 1);
+          ok = ld_wait(&rk_full[team], i & 1);
 #pragma unroll
           for (int y = 0; y < KR; ++y) {
             const uint4* const from = (const uint4*)(place + Shape::RK) + ((1 - part) * KR + y) * 64 + lane;
@@ -1118,8 +1099,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           else ld_mma(sum[who][y], h4[kt], bh[y / 2][y % 2 * 2], bh[y / 2][y % 2 * 2 + 1]);
           if (x % 3 == 0 && at + 1 < STEPS) get_b(at + 1, x / 3);
           if (at == STEPS - 1 && x == 3 * G / 2 && i + 1 < chunks)
-            next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1) &&
-                   (i == 0 || mbar_wait(&s_empty[team][(i + 1) & 1], (((i + 1) >> 1) - 1) & 1));
+            next = mbar_wait(&full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1) && mbar_wait(&read[team], i & 1);
         }
       }
       if (group == 0) {  // where S vanishes beside what is added, in the scale of that: all stays within 32 bits

@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import linear_ref as ref
-from test_linear_gpu import HALF, TINY, fault, generator, near, plan_of
+from test_linear_gpu import HALF, TINY, delta_case, fault, generator, near, plan_of
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,55 @@ def test_delta_rows_of_any_size(cuda, heads, counts, eps):
     args = (q, k, normal(T, Hv, Dv).bfloat16(), -torch.exp(normal(T, Hv) - 2), normal(len(counts), Hv, Dv, Dk))
     beta = torch.rand((T, Hv), generator=g, device=cuda)
     check(args, cu, plan, beta=beta, eps=eps)
+
+
+@pytest.mark.parametrize("heads", [(2, 4, 128, 128), (1, 2, 64, 48)])
+@pytest.mark.parametrize("with_beta", [True, False])
+@pytest.mark.parametrize("counts", [[3, 2, 4], [14], [100, 130]])
+def test_delta_values_far_larger_than_others(cuda, heads, with_beta, counts):
+    """Values of 1e9 among ordinary ones: tokens before them keep their bits, tokens after them forget them as the decays say.
+
+    Besides the usual terms, for tokens from a large value on: an entry of P T, which decays may make that small, ends at the second
+    term's smallest step, 2^-16 of e5m2, rounded to half of it and held 2^11 times, where the row's largest entry is held as 2^13 at
+    least: off by 2^-17 / 2^11 / 2^13 = 2^-41 of that, which is at most scale |q| here (beta and |k| at most 1: corrections
+    shrink). It is multiplied by R_j = v_j - S k_j, at most |v_j| + W_j."""
+    from drama3_b200 import kernels
+    Hk, Hv, Dk, Dv = heads
+    cu, plan = plan_of(counts, 0, cuda)
+    g, T = generator(cuda, 34), sum(counts)
+    normal = lambda *s: torch.randn(s, generator=g, device=cuda)  # noqa: E731
+    q, k, v = normal(T, Hk, Dk).bfloat16(), normal(T, Hk, Dk).bfloat16(), normal(T, Hv, Dv)
+    large = torch.rand((T, Hv, Dv), generator=g, device=cuda) < 0.02
+    args = (q, k, torch.where(large, 1e9 * v, v).bfloat16(), -torch.exp(2 * normal(T, Hv)), normal(len(counts), Hv, Dv, Dk))
+    more = dict(beta=torch.rand((T, Hv), generator=g, device=cuda)) if with_beta else {}
+    want, after, size, state_size = ref.delta(*args, cu, **more)
+    out = kernels.lines_delta(*args, plan, **more)
+    half, length = HALF[torch.bfloat16], (q.double() / torch.sqrt(q.double().square().sum(-1, keepdim=True) + 1e-6)).norm(dim=-1)
+    length = Dk ** -0.5 * length.repeat_interleave(Hv // Hk, 1)[..., None]  # scale |q|
+    left = args[2].double().abs() + size / length
+    left = torch.cat([left[a:b].cumsum(0) for a, b in zip(cu, cu[1:])])
+    near(out, want, (1 + half) * ((2.0 ** -15 + 2.0 ** -10) * size + 2.0 ** -41 * length * left) + half * want.abs(), "out")
+    near(args[4], after, 2.0 ** -15 * state_size[..., None].expand_as(after), "state")
+    assert fault() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads", [(2, 4, 128, 128), (1, 2, 64, 64), (8, 16, 128, 256)])
+@pytest.mark.parametrize("form", ["raw", "given", "decay only", "raw without beta", "raw without dt_bias"])
+@pytest.mark.parametrize("counts", [[1] * 7, [90, 0, 200, 33]])
+def test_delta_outputs_are_as_near_as_their_rounding(cuda, dtype, heads, form, counts):
+    """Outputs in the 2-norm, over tokens, heads and channels: what rounding the exact ones leaves, and apart from that at most the
+    last bit of P T's second terms, 2^-15 of them, of which the root mean square is below 2^-16. A term is a query and a key of
+    random directions times a value, so the size over sqrt(Dk), a product's largest being about sqrt(10) of that."""
+    from drama3_b200 import kernels
+    cu, plan = plan_of(counts, 1, cuda)
+    args, more = delta_case(cuda, heads, counts, 1, dtype, form.split(" without")[0], 35)
+    if "without" in form:
+        del more[form.split()[-1]]
+    want, after, size, state_size = ref.delta(*args, cu, **more)
+    out = kernels.lines_delta(*args, plan, **more)
+    rounding = (want.to(dtype).double() - want).norm()
+    other = 2.0 ** -16 * (10 / heads[2]) ** 0.5 * size.norm()
+    assert (out.double() - want).norm() <= (rounding ** 2 + other ** 2) ** 0.5
+    assert (args[4].double() - after).norm() <= 2.0 ** -18 * state_size.norm() * max(1, heads[2] ** 0.5 / 8)
+    assert not out[cu[-1]:].any() and fault() == 0
