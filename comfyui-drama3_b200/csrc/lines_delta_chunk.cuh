@@ -20,7 +20,7 @@
 // overwrites the state an output is the difference of two terms as large as the state, so that all of its factors have two terms too; the
 // second one of P T has eight bits (2^-15 of it): an output's own rounding is 2^-11 of it at least.
 //
-// A value that is not finite reaches the state and the tokens of its own line, in its chunk earlier ones too; one in q its own
+// A value that is not finite reaches its line's state and tokens from its own token on, one in v those of its column, one in q its own
 // token only.
 #pragma once
 
@@ -212,11 +212,11 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
   uint16_t* const td = (uint16_t*)A;                  // T^T D, two terms, when T has been read
   __shared__ __align__(8) uint64_t arrived;
   __shared__ int line_s[LD_C];
-  __shared__ uint32_t starts_s[2];
+  __shared__ uint32_t starts_s[2], odd_s[2];  // a bit a token: a line's first one; something of it is not finite
   __shared__ __align__(16) float d_s[LD_C], r_in_s[LD_C], k_factor[LD_C], q_factor[LD_C], beta_s[LD_C], kt_scale[LD_C], q_scale_s[LD_C];
   __shared__ double sum_s;
   __shared__ float2 G_s[LD_C];  // as the sum of two
-  __shared__ int bad_s[LD_C];   // by a line's first token in the chunk: something of it is not finite
+  __shared__ int bad_s[LD_C];   // by a line's first token in the chunk: its state will not be finite
   const LdArgs& a = c.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
   const int block = blockIdx.x, h = blockIdx.y, many = a.Hv / a.Hk, hk = h / many;
@@ -310,12 +310,30 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     ld_bulk_out(rows->k, ks, sizeof(rows->k));
     ld_bulk_commit();
   }
+  if (warp < 2) {
+    const uint32_t starts = __ballot_sync(0xffffffffu, tid == 0 || line_s[tid - 1] != my_line);
+    const bool finite = k_factor[tid] == k_factor[tid] && decay == decay && fabsf(beta) <= LD_MAX;
+    const uint32_t odd = __ballot_sync(0xffffffffu, my_line >= 0 && !finite);
+    if (lane == 0) starts_s[warp] = starts, odd_s[warp] = odd;
+  }
+  __syncthreads();
+  const unsigned long long starts = starts_s[0] | (unsigned long long)starts_s[1] << 32;
+  auto first_of = [&](int i) { return 63 - __clzll(starts & (~0ull >> (63 - i))); };
+  // From a line's first token on whose key, decay or strength is not finite, its tokens count as not there, and get NaN in the end: what
+  // comes before stays clear of it.
+  int first = 0, last = 0;
+  bool lost = false;
+  if (tid < LD_C) {
+    first = first_of(tid);
+    const unsigned long long later = tid == 63 ? 0 : starts >> (tid + 1), odd = odd_s[0] | (unsigned long long)odd_s[1] << 32;
+    last = later ? tid + __ffsll((long long)later) - 1 : 63;
+    lost = (odd & (~0ull >> (63 - tid))) >> first;
+    if (lost) decay = beta = k_factor[tid] = 0.0f, bad_s[first] = 1;
+  }
   // sums of the log decays that start again with each line
   double G = decay < -104.0f ? -104.0f : decay;  // exp of it is 0 already; keeps infinities out of the sums
   if (warp < 2) {
-    const uint32_t starts = __ballot_sync(0xffffffffu, tid == 0 || line_s[tid - 1] != my_line);
-    if (lane == 0) starts_s[warp] = starts;
-    const int from = max(31 - __clz(starts & (0xffffffffu >> (31 - lane))), 0);  // in this warp
+    const int from = max(first - warp * 32, 0);  // in this warp
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double before = __shfl_up_sync(0xffffffffu, G, o);
@@ -324,13 +342,7 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     if (tid == 31) sum_s = G;
   }
   __syncthreads();
-  const unsigned long long starts = starts_s[0] | (unsigned long long)starts_s[1] << 32;
-  auto first_of = [&](int i) { return 63 - __clzll(starts & (~0ull >> (63 - i))); };
-  int first = 0, last = 0;
   if (tid < LD_C) {
-    first = first_of(tid);
-    const unsigned long long later = tid == 63 ? 0 : starts >> (tid + 1);
-    last = later ? tid + __ffsll((long long)later) - 1 : 63;
     if (tid >= 32 && first < 32) G += sum_s;
     const float G_hi = (float)G;
     G_s[tid] = make_float2(G_hi, (float)(G - G_hi));
@@ -603,8 +615,8 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
     const bool bad = bad_s[first] != 0, live = my_line >= 0;
     out->gamma[tid] = ld_exp(G_s[tid].x + G_s[tid].y);
     out->kt_scale[tid] = !live ? 0.0f : bad ? nan : kt_scale[tid];
-    out->r_in[tid] = bad ? 0.0f : r_in_s[tid];
-    out->q_scale[tid] = !live ? 0.0f : bad ? nan : q_scale_s[tid];
+    out->r_in[tid] = r_in_s[tid];
+    out->q_scale[tid] = !live ? 0.0f : lost ? nan : q_scale_s[tid];
   }
   if (tid == 0) ld_bulk_done();
 }
@@ -628,9 +640,9 @@ __global__ void __launch_bounds__(LD_PREP_THREADS, 4) lines_delta_prep_kernel(Ld
 template <int DK, int WARPS, int PARTS> struct LdScanShape {
   static constexpr int HEAD = sizeof(LdRows<DK>), V = HEAD + sizeof(LdHead<DK>), STAGE = V + WARPS * LD_C * 32;
   // a team's place: S's terms as A fragments, with its rows' scales of each part; R times K~'s factors likewise, for the other part; R
-  // itself, for the outputs; and those
+  // itself, for the outputs; those; and each part's first tokens that are not finite, where there are such
   static constexpr int S_SCALES = DK * 64, RK = S_SCALES + 128, RK_SCALES = RK + (PARTS > 1 ? LD_C * 64 : 0);
-  static constexpr int R = RK_SCALES + 128, OUT = R + LD_C * 64, TEAM = OUT + LD_C * 32;
+  static constexpr int R = RK_SCALES + 128, OUT = R + LD_C * 64, CLEAN = OUT + LD_C * 32, TEAM = CLEAN + 128;
   static constexpr int ROOM = 227 * 1024 - 2048 - WARPS * TEAM, STAGES = ROOM / STAGE < 4 ? ROOM / STAGE : 4;
   static constexpr int SMEM = STAGES * STAGE + WARPS * TEAM + 1024;
   static constexpr int OUTS = PARTS;  // warps for the outputs, each of a share of the tokens: as many on every quarter of an SM
@@ -645,6 +657,13 @@ D3_DEV float ld_inverse(float x) { return __uint_as_float(0x7f000000u - __float_
 D3_DEV float ld_row_most(float m) {
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
   return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+
+// The larger one; NaN where one is.
+D3_DEV float ld_most(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // mbar_wait by a whole warp, the same answer in all lanes.
@@ -667,6 +686,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];  // the chunks' stages
   // a team's S and R: written (R times K~'s factors too), and both read by the outputs. A part writes the next S when the outputs have
   // read this one, and has the other part's when that has written it, so that none is ever two phases ahead.
+  __shared__ int odd_s[WARPS][PARTS];  // 1 + the last chunk with values that are not finite
   __shared__ __align__(8) uint64_t s_full[WARPS], rk_full[WARPS], r_full[WARPS], read[WARPS];
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
@@ -680,6 +700,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
     for (int i = 0; i < WARPS; ++i) {
       mbar_init(&s_full[i], PARTS), mbar_init(&rk_full[i], PARTS), mbar_init(&r_full[i], PARTS);
       mbar_init(&read[i], OUTS);
+      for (int y = 0; y < PARTS; ++y) odd_s[i][y] = 0;
     }
     fence_mbar_init();
   }
@@ -788,6 +809,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       // keeps its bits
       uint32_t r_hi[LD_C / 16][4], r_lo[LD_C / 16][4];
       float r_down[2];
+      int until = LD_C;  // of column lane % 16
       {
         float4 v[NT];
         float most[2] = {0.0f, 0.0f}, up[2];
@@ -797,6 +819,9 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           most[0] = fmaxf(most[0], fmaxf(fabsf(v[n].x), fabsf(v[n].y)));
           most[1] = fmaxf(most[1], fmaxf(fabsf(v[n].z), fabsf(v[n].w)));
         }
+#pragma unroll
+        for (int y = 0; y < PARTS; ++y)  // a value that is not finite: its column's outputs from there on
+          if (odd_s[team][y] == i + 1) until = min(until, ((const int*)(place + Shape::CLEAN))[y * 16 + lane % 16]);
         ld_arrive(&read[team], lane);
 #pragma unroll
         for (int r = 0; r < 2; ++r) ld_scale(ld_row_most(most[r]), up[r], r_down[r]);
@@ -839,6 +864,14 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
         st_matrix4_trans(out_s + token * 32 + piece * 16, o4[0], o4[1], o4[2], o4[3]);
       }
       __syncwarp();
+      if (__any_sync(0xffffffffu, until < LD_C)) {
+#pragma unroll 1
+        for (int x = 0; x < NO / 2; ++x)
+#pragma unroll 1
+          for (int token = max(tokens(x) + lane / 16 * 8, until); token < tokens(x) + lane / 16 * 8 + 8; ++token)
+            *(uint16_t*)(out_s + token * 32 + ((lane / 8 & 1) ^ ((token >> 2) & 1)) * 16 + lane % 8 * 2) = 0x7fff;  // NaN in both types
+        __syncwarp();
+      }
       if (there)
 #pragma unroll
         for (int x = 0; x < LD_C / 16 / OUTS; ++x) {
@@ -1029,13 +1062,30 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           RK[n][y] = v[y] * (y & 1 ? f.y : f.x);
-          m[y >> 1] = fmaxf(m[y >> 1], fabsf(RK[n][y]));
+          m[y >> 1] = ld_most(m[y >> 1], fabsf(RK[n][y]));
         }
         if (n < G) get_b(0, n);
       }
       if (NO < G)
 #pragma unroll
         for (int n = NO; n < G; ++n) get_b(0, n);
+    }
+    if (__any_sync(0xffffffffu, !(ld_most(m[0], m[1]) <= LD_MAX))) {  // outputs before a value that is not finite stay clear of it
+      int clean[2] = {LD_C, LD_C};
+#pragma unroll 1
+      for (int n = NO - 1; n >= 0; --n) {
+        float* const v = (float*)(place + Shape::R) + ((part * NO + n) * 32 + lane) * 4;
+#pragma unroll
+        for (int y = 3; y >= 0; --y)
+          if (!(fabsf(v[y]) <= LD_MAX)) v[y] = 0.0f, clean[y >> 1] = (part * NO + n) * 8 + cc * 2 + (y & 1);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) clean[r] = min(clean[r], __shfl_xor_sync(0xffffffffu, clean[r], o));
+        if (cc == 0) ((int*)(place + Shape::CLEAN))[part * 16 + g + r * 8] = clean[r];
+      }
+      odd_s[team][part] = i + 1;
     }
     ld_arrive(&r_full[team], lane);
     // its two terms, for this part's columns and the other's. Each part's tokens have a scale.

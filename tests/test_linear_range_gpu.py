@@ -168,3 +168,36 @@ def test_delta_outputs_are_as_near_as_their_rounding(cuda, dtype, heads, form, c
     assert (out.double() - want).norm() <= (rounding ** 2 + other ** 2) ** 0.5
     assert (args[4].double() - after).norm() <= 2.0 ** -18 * state_size.norm() * max(1, heads[2] ** 0.5 / 8)
     assert not out[cu[-1]:].any() and fault() == 0
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("what", ["v", "k", "q", "decay", "beta"])
+@pytest.mark.parametrize("counts,line,at", [([2, 9, 3], 1, 4), ([3, 60, 5, 100], 1, 20), ([3, 60, 5, 100], 3, 0), ([150, 20], 0, 63),
+                                            ([150, 20], 0, 80), ([150, 20], 0, 149)])
+def test_delta_a_value_that_is_not_finite_reaches_nothing_before_it(cuda, value, what, counts, line, at):
+    """One value of one token: its line's later tokens and its state, of v those of its column alone, of q nothing but its own token."""
+    from drama3_b200 import kernels
+    if what == "decay" and value == -float("inf"):
+        pytest.skip("a decay of everything is one")
+    cu, plan = plan_of(counts, 2, cuda)
+    (q, k, v, decay, state), more = delta_case(cuda, (2, 4, 64, 64), counts, 2, torch.bfloat16, "given", 36)
+    if what == "decay" and value > 0:
+        value = float("nan")  # above 0 counts as 0
+    good = {"q": q, "k": k, "v": v, "decay": decay, "beta": more["beta"]}
+    bad = {name: t.clone() for name, t in good.items()}
+    t = cu[line] + at
+    bad[what][(t, 1, 7) if bad[what].dim() == 3 else (t, 1)] = value
+    runs = []
+    for d in (good, bad):
+        s = state.clone()
+        runs.append((kernels.lines_delta(d["q"], d["k"], d["v"], d["decay"], s, plan, beta=d["beta"]), s))
+    (want, want_state), (got, got_state) = runs
+    heads = [2, 3] if what in ("q", "k") else [1]  # of 4, of which two share a key head
+    reached = torch.zeros(want.shape, dtype=torch.bool, device=cuda)
+    reached_state = torch.zeros(want_state.shape, dtype=torch.bool, device=cuda)
+    for h in heads:
+        reached[t:t + 1 if what == "q" else cu[line + 1], h, 7 if what == "v" else slice(None)] = True
+        if what != "q":
+            reached_state[line, h, 7 if what == "v" else slice(None)] = True
+    assert not got[reached].isfinite().any() and torch.equal(got[~reached], want[~reached]) and want.isfinite().all()
+    assert not got_state[reached_state].isfinite().any() and torch.equal(got_state[~reached_state], want_state[~reached_state])
