@@ -820,6 +820,8 @@ def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None
     without it g is decay itself, at most 0, and beta is taken as it is. q and k are divided by sqrt(sum of squares + eps)
     unless eps is None; scale defaults to 1 / sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get
     zeros."""
+    if eps is not None and not eps >= 0:
+        raise ValueError(f"eps must be at least 0, or None for rows as they are, not {eps}")
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         q, k, v = (_aligned16(t) for t in (q, k, v))
     cu, line = plan.cu, plan.line
