@@ -10,7 +10,8 @@
 // loads are in flight (two 35.6, eight 43.9 us in the case below), and no block-wide step. Joined rows are long: a warp each where
 // they are many (a row's loads are in flight together), a block each, whose threads hold one or two vectors, where they are few.
 // Measured (B200, bf16): gated, 8192 tokens of 32 heads of 128 34 us, 5.9 TB/s; joined, 16384 rows of 2048 with a norm after the block
-// and a gate a row 52 us, 5.2 TB/s (a block a row: 73); 16 tokens 1.6 and 1.9 us, latency.
+// and a gate a row 52 us, 5.2 TB/s (a block a row: 73), without them 43 where the calls follow one another; 16 tokens 1.6 and 1.9 us, latency.
+// fp32 63 and 92 us. Rows that are no whole vectors are read in single values, twice and three times: heads of 129 107 us, 1001 columns 69 to 104.
 #pragma once
 
 #include "rows.cuh"

@@ -84,8 +84,10 @@ int conv_type(const d3::LcArgs& a, bool vectors, cudaStream_t s) {
 }
 
 // Whether lines_delta goes token by token (or in chunks). Measured (B200, 16 / 32 heads of 128, us by tokens / in chunks): lines of 4
-// tokens each, 1 line 4.8 / 23, 16 lines 20 / 62, 256 lines 274 / 701; of 16 each 13 / 23, 62 / 65, 918 / 847; all but one line with a token,
-// the last with the rest of 4 a line, 16 lines 46 / 62, 256 lines 866 / 714; one line of 32 23 / 22.
+// tokens each, 1 line 5.7 / 27, 16 lines 21 / 68, 256 lines 303 / 753; of 8, 16 lines 37 / 69, 256 lines 537 / 778; of 16, 1 line 17 / 26,
+// 16 lines 69 / 75, 256 lines 1017 / 835; one line of 32 31 / 26. So lines of equal length meet near 12 tokens, but how tokens are spread is
+// known on the GPU alone, and the longest line sets the time by tokens: all but one line with a token, the last with the rest of 4 a
+// line, 16 lines 58 / 68, 256 lines 1082 / 796; 1024 tokens of one line, the other 255 idle, 985 / 115.
 bool delta_steps(int T, int B) { return T <= 4LL * B || T <= 16; }
 
 size_t delta_block_bytes(int Hk, int Hv, int Dk) {
@@ -93,7 +95,7 @@ size_t delta_block_bytes(int Hk, int Hv, int Dk) {
                   : Hk * sizeof(d3::LdRows<128>) + Hv * sizeof(d3::LdHead<128>);
 }
 
-// Chunks prepared and scanned by a pair of launches: as many as 384 MB hold, or equal parts below that. (B200, 8192 tokens of 16 / 32
+// Chunks prepared and scanned by a pair of launches: as many as 384 MB hold (eight at least), or equal parts below that. (B200, 8192 tokens of 16 / 32
 // heads of 128, an earlier form of the scan: 438 us in one pair, 469 in parts of 37 chunks, whose 70 MB stay in L2, 714 in parts of 9:
 // the scan starts anew in each.)
 int delta_blocks(int T, int Hk, int Hv, int Dk) {

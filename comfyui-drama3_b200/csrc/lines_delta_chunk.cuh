@@ -19,6 +19,8 @@
 // of the four of two such factors the smallest, low times low, is left out (2^-22). S and T are formed in 32 bits. Where the chunk
 // overwrites the state an output is the difference of two terms as large as the state, so that all of its factors have two terms too; the
 // second one of P T has eight bits (2^-15 of it): an output's own rounding is 2^-11 of it at least.
+// Where a row's values lie far apart fp16 ends: S and R towards the state keep 2^-38 of the row's largest, R towards the outputs, whose
+// second terms are held 2^11 times, 2^-49, P T 2^-41.
 //
 // A value that is not finite reaches its line's state and tokens from its own token on, one in v those of its column, one in q its own
 // token only.

@@ -74,7 +74,7 @@ class LinesDelta(nn.Module):
 class LinesStack(nn.Module):
     """Decoder layers: mixers (LinesDelta or LinesAttention) and feed-forward blocks by turns, x + mixer(norm(x)), then x +
     block(norm(x)), and the norm behind the last one. A block takes [T, 1, hidden], as model.SparseMoeBlock does. Each sum and
-    the norm that follows it are one launch."""
+    the norm that follows it are one launch (kernels.add_norm); the first norm, which follows no sum, is torch's."""
 
     def __init__(self, hidden, mixers, blocks, eps=1e-6, device=None, dtype=None):
         super().__init__()

@@ -819,7 +819,8 @@ def lines_delta(q, k, v, decay, state, plan, beta=None, a_log=None, dt_bias=None
     (float32) they are the projections' raw outputs: g = -exp(a_log) softplus(decay + dt_bias), beta through the sigmoid;
     without it g is decay itself, at most 0, and beta is taken as it is. q and k are divided by sqrt(sum of squares + eps)
     unless eps is None; scale defaults to 1 / sqrt(Dk). Dk 64 or 128, Dv a multiple of 16 up to 256. Places of no line get
-    zeros."""
+    zeros. Token by token where T is at most 16 or four times the state's lines, else in chunks of 64: a long text is best planned
+    without lines that idle, which would have it go token by token, about 1 us each."""
     if eps is not None and not eps >= 0:
         raise ValueError(f"eps must be at least 0, or None for rows as they are, not {eps}")
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
