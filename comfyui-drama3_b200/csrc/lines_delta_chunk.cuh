@@ -21,6 +21,8 @@
 // second one of P T has eight bits (2^-15 of it): an output's own rounding is 2^-11 of it at least.
 // Where a row's values lie far apart fp16 ends: S and R towards the state keep 2^-38 of the row's largest, R towards the outputs, whose
 // second terms are held 2^11 times, 2^-49, P T 2^-41.
+// Corrections with beta |k|^2 above 2 overshoot, and T grows with them; where that leaves 32 bits, the line's other tokens of the chunk may
+// be lost with it.
 //
 // A value that is not finite reaches its line's state and tokens from its own token on, one in v those of its column, one in q its own
 // token only.
@@ -688,8 +690,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];  // the chunks' stages
   // a team's S and R: written (R times K~'s factors too), and both read by the outputs. A part writes the next S when the outputs have
   // read this one, and has the other part's when that has written it, so that none is ever two phases ahead.
-  __shared__ int odd_s[WARPS][PARTS];  // 1 + the last chunk with values that are not finite
   __shared__ __align__(8) uint64_t s_full[WARPS], rk_full[WARPS], r_full[WARPS], read[WARPS];
+  __shared__ int odd_s[WARPS][PARTS];  // 1 + the last chunk with values that are not finite
   const LdArgs& a = c.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
   const int h = blockIdx.y, b = blockIdx.z;
