@@ -810,7 +810,8 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
       ok = ld_wait(&r_full[team], i & 1);
       if (!ok) break;
       // R as A fragments of two terms, rows by a power of two; low ones times 2^11, as P T's: what is small beside the row's largest
-      // keeps its bits
+      // keeps its bits. (Without the delta rule R is V, and values of fp16 are one term as they are.)
+      constexpr bool ONE_TERM = !DELTA && TYPE == QR_F16;
       uint32_t r_hi[LD_C / 16][4], r_lo[LD_C / 16][4];
       float r_down[2];
       int until = LD_C;  // of column lane % 16
@@ -828,7 +829,10 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
           if (odd_s[team][y] == i + 1) until = min(until, ((const int*)(place + Shape::CLEAN))[y * 16 + lane % 16]);
         ld_arrive(&read[team], lane);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) ld_scale(ld_row_most(most[r]), up[r], r_down[r]);
+        for (int r = 0; r < 2; ++r) {
+          up[r] = r_down[r] = 1.0f;
+          if (!ONE_TERM) ld_scale(ld_row_most(most[r]), up[r], r_down[r]);
+        }
 #pragma unroll
         for (int kt = 0; kt < LD_C / 16; ++kt)
 #pragma unroll
@@ -836,7 +840,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
             const float4& from = v[2 * kt + (x >> 1)];
             const float v0 = (x & 1 ? from.z : from.x) * up[x & 1], v1 = (x & 1 ? from.w : from.y) * up[x & 1];
             r_hi[kt][x] = ld_half2(v0, v1);
-            r_lo[kt][x] = ld_half2((v0 - h_lo(r_hi[kt][x])) * 0x1p11f, (v1 - h_hi(r_hi[kt][x])) * 0x1p11f);
+            if (!ONE_TERM) r_lo[kt][x] = ld_half2((v0 - h_lo(r_hi[kt][x])) * 0x1p11f, (v1 - h_hi(r_hi[kt][x])) * 0x1p11f);
           }
       }
       uint8_t* const out_s = place + Shape::OUT;
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(LdScanShape<DK, WARPS, PARTS>::THREADS, 1)
             // a byte of e5m2 is the upper one of an fp16 number
             const uint32_t p_lo[4] = {__byte_perm(rest.x, 0, 0x1404), __byte_perm(rest.x, 0, 0x3424), __byte_perm(rest.y, 0, 0x1404),
                                       __byte_perm(rest.y, 0, 0x3424)};
-            ld_mma(low[0], r_lo[kt], p[0], p[1]), ld_mma(low[1], r_lo[kt], p[2], p[3]);
+            if (!ONE_TERM) ld_mma(low[0], r_lo[kt], p[0], p[1]), ld_mma(low[1], r_lo[kt], p[2], p[3]);
             ld_mma(high[0], r_hi[kt], p[0], p[1]), ld_mma(high[1], r_hi[kt], p[2], p[3]);
             ld_mma(low[0], r_hi[kt], p_lo[0], p_lo[1]), ld_mma(low[1], r_hi[kt], p_lo[2], p_lo[3]);
           }
